@@ -94,6 +94,15 @@ int ziggy_hip_create_empty_buffer(ZiggyHipContext *ctx, size_t length, ZiggyHipB
                                   char *error_message, size_t error_message_len);
 void ziggy_hip_destroy_buffer(ZiggyHipBuffer *buffer);
 size_t ziggy_hip_buffer_length(const ZiggyHipBuffer *buffer);
+/* A buffer over device memory that the caller owns (no counterpart in the
+ * reference): nothing is copied, and destroy_buffer leaves the memory alone.
+ * `length` bytes from `device_memory`, 16-byte aligned, have to lie within one
+ * allocation on the context's device and outlive the buffer.  The context's
+ * stream is ordered with no other: work of other streams on the memory has to
+ * be over before a call that takes the buffer, and the sequence committed (or
+ * the call returned, without one) before they use it again. */
+int ziggy_hip_wrap_buffer(ZiggyHipContext *ctx, void *device_memory, size_t length, ZiggyHipBuffer **out_buffer,
+                          char *error_message, size_t error_message_len);
 int ziggy_hip_write_buffer(ZiggyHipBuffer *buffer, const void *bytes, size_t length, size_t offset,
                            char *error_message, size_t error_message_len);
 int ziggy_hip_read_buffer(const ZiggyHipBuffer *buffer, void *out_bytes, size_t length, size_t offset,
@@ -295,6 +304,93 @@ int ziggy_hip_weighted_sum_topk_f32(ZiggyHipContext *ctx, ZiggyHipBuffer *dst, c
 int ziggy_hip_sigmoid_scale_add_f32(ZiggyHipContext *ctx, ZiggyHipBuffer *dst, const ZiggyHipBuffer *src,
                                     const ZiggyHipBuffer *scalar, uint32_t count, char *error_message,
                                     size_t error_message_len);
+
+/* ---- operators of a step over a long context (no counterpart in the reference) ----
+ * Like the calls above they run in an open sequence or wait for the stream,
+ * and they take buffers of the context's own device only.  Row strides count
+ * floats; a stride of 0 stands for rows without a gap. */
+
+enum {
+    ZIGGY_HIP_ROPE_NONE = 0,   /* f */
+    ZIGGY_HIP_ROPE_LINEAR = 1, /* f / factor */
+    ZIGGY_HIP_ROPE_YARN = 2,   /* blended by pair: see below */
+    ZIGGY_HIP_ROPE_BANDS = 3,  /* blended by turns: see below */
+};
+/* Rotary frequencies f_i = freq_base^(-2 i / rope_dim), i < rope_dim / 2, and
+ * how they are scaled for contexts longer than the model was trained on
+ * (original_context, L).  Blended: f_i (g_i + (1 - g_i) / factor) with
+ *   YARN   g_i = 1 - clamp((i - a) / max(0.001, b - a), 0, 1),
+ *          a = max(0, floor(c(high))), b = min(rope_dim - 1, ceil(c(low))),
+ *          c(t) = rope_dim ln(L / (2 pi t)) / (2 ln freq_base): the pair that
+ *          makes t turns over L (GGUF's rope.scaling.type "yarn": low 1, high 32);
+ *   BANDS  g_i = clamp((L f_i / 2 pi - low) / (high - low), 0, 1)
+ *          (low_freq_factor and high_freq_factor of Llama-3.1's scaling).
+ * magnitude multiplies the rotated values (1: none; YaRN's own is
+ * 0.1 ln(factor) + 1). */
+typedef struct {
+    uint32_t head_dim;   /* even, at most 512 */
+    uint32_t rope_dim;   /* rotated values at the head's start: even, 2 .. head_dim */
+    uint32_t rope_style; /* 0 = interleaved pairs (2i, 2i + 1), 1 = halves (i, i + rope_dim / 2) */
+    uint32_t scaling;    /* ZIGGY_HIP_ROPE_* */
+    uint32_t original_context;
+    float freq_base, factor, low, high, magnitude;
+} ZiggyHipRopeDesc;
+/* Rotates head_count heads of `rows` rows: row r at positions[r] (u32), or at
+ * first_position + r where positions is NULL.  The values past rope_dim are
+ * copied.  src and dst may be the same rows (same offset and stride); other
+ * overlaps are refused.  freq_factors (or NULL): rope_dim / 2 floats that
+ * divide the frequencies (GGUF's rope_freqs.weight).  The angles are 64-bit. */
+int ziggy_hip_rope_rows_f32(ZiggyHipContext *ctx, const ZiggyHipRopeDesc *desc, const ZiggyHipBuffer *src,
+                            size_t src_offset_bytes, size_t src_row_stride, ZiggyHipBuffer *dst,
+                            size_t dst_offset_bytes, size_t dst_row_stride, const ZiggyHipBuffer *positions,
+                            uint32_t first_position, const ZiggyHipBuffer *freq_factors, uint32_t rows,
+                            uint32_t head_count, char *error_message, size_t error_message_len);
+
+/* K/V cache in 8 bits.  Of each layer and kv head, 32 consecutive positions (a
+ * block) share a scale; a value is code * scale with the code in [-127, 127].
+ *   k_codes int8 [layer][kv head][position][dim]
+ *   v_codes int8 [layer][kv head][block][dim][position within the block]
+ *   k_scales, v_scales f32 [layer][kv head][block]
+ * with the positions of a layer rounded up to whole blocks.  A cache starts as
+ * any bytes at all: what was never stored is never read. */
+#define ZIGGY_HIP_KV8_BLOCK 32
+typedef struct {
+    ZiggyHipBuffer *k_codes, *k_scales, *v_codes, *v_scales;
+    uint32_t layers, head_count_kv, head_dim, context_length; /* head_dim 64, 96, 128 or 256 */
+} ZiggyHipKv8Cache;
+/* Bytes of each codes and of each scales buffer of such a cache (0: a shape that is not served). */
+size_t ziggy_hip_kv8_codes_length(uint32_t layers, uint32_t head_count_kv, uint32_t head_dim, uint32_t context_length);
+size_t ziggy_hip_kv8_scales_length(uint32_t layers, uint32_t head_count_kv, uint32_t head_dim,
+                                   uint32_t context_length);
+/* Stores the rows k, v ([rows][head_count_kv * head_dim] f32, row_stride apart,
+ * from k_offset_bytes and v_offset_bytes on) at positions position ..
+ * position + rows - 1.  A block whose first position is among them starts
+ * anew: its scale is max|x| / 127 over its new rows, a code the nearest
+ * integer to x / scale (ties to even).  In a block that begins before
+ * `position` the earlier rows stay: its scale grows to that of the new rows
+ * where that is larger (the earlier codes are then rounded to the new scale),
+ * and never shrinks.  Rows behind the last one keep their codes.  A row with an
+ * infinity or NaN makes its block's scale NaN, and every row of the block read
+ * as NaN until the block starts anew. */
+int ziggy_hip_kv8_store(ZiggyHipContext *ctx, const ZiggyHipKv8Cache *cache, const ZiggyHipBuffer *k,
+                        size_t k_offset_bytes, const ZiggyHipBuffer *v, size_t v_offset_bytes, size_t row_stride,
+                        uint32_t layer, uint32_t position, uint32_t rows, char *error_message,
+                        size_t error_message_len);
+/* Reads rows position .. position + rows - 1 back as f32 ([rows][head_count_kv * head_dim]). */
+int ziggy_hip_kv8_load_f32(ZiggyHipContext *ctx, const ZiggyHipKv8Cache *cache, ZiggyHipBuffer *k_out,
+                           ZiggyHipBuffer *v_out, uint32_t layer, uint32_t position, uint32_t rows,
+                           char *error_message, size_t error_message_len);
+/* Attention of `queries` queries (rows of head_count * head_dim, q_row_stride
+ * apart, already rotated) at positions position .. position + queries - 1, their
+ * K/V rows stored.  The query at position p attends to the positions up to p,
+ * or, with window > 0, to the last `window` of them; what lies at other
+ * positions is not read into the result, whatever it is.  output:
+ * [queries][head_count * head_dim].  head_count is a multiple of the cache's
+ * head_count_kv (at most 64 times as many). */
+int ziggy_hip_kv8_attention_f32(ZiggyHipContext *ctx, const ZiggyHipKv8Cache *cache, const ZiggyHipBuffer *q,
+                                size_t q_row_stride, ZiggyHipBuffer *output, uint32_t head_count, uint32_t layer,
+                                uint32_t position, uint32_t queries, uint32_t window, float scale,
+                                char *error_message, size_t error_message_len);
 
 /* ---- decode session (replaces the Zig gpu.Session, runtime/gpu/session.zig:27-651,
  * which drives the entry points above one dispatch at a time).  The session
@@ -550,6 +646,25 @@ int ziggy_hip_sample_shortlist(const ZiggyHipShortlistEntry *entries, uint32_t c
                                uint32_t *out_token);
 int ziggy_hip_sample_logits(const float *logits, uint32_t count, const uint32_t *recent, uint32_t recent_count,
                             const ZiggyHipSamplingOptions *options, double uniform, uint32_t *out_token);
+
+/* The same draw on the device, a row at a time in one call: token[r] of
+ * logits row r ([rows][vocab], row_stride floats apart) as
+ * ziggy_hip_sample_logits draws it with uniforms[r] (f64; taken into [0, 1)),
+ * without the limit of 64 candidates.  recent (or NULL): u32
+ * [rows][recent_count], the tokens so far of each row; ids of vocab and above
+ * are passed over, so shorter lists are padded with 0xFFFFFFFF.  top_k is 0 or
+ * at least vocab (no limit), or at most 1024; vocab at most 262144; top_p and min_p in [0, 1].
+ * temperature <= 0 gives the row's argmax.  Weights are 64-bit; their sums are
+ * exact integers of 2^-s (s = 62 less the bits of the candidates' count: at
+ * least 44), so a row's token depends on nothing but its inputs; a weight below
+ * 2^-(s+1) of the largest counts as 0, and a token of weight 0 is not drawn.
+ * Logits of NaN count as -infinity.  A row without a finite largest logit
+ * gives its first candidate of the largest value, as the host sampler. */
+int ziggy_hip_sample_rows_f32(ZiggyHipContext *ctx, const ZiggyHipBuffer *logits, size_t row_stride,
+                              const ZiggyHipBuffer *recent, uint32_t recent_count,
+                              const ZiggyHipSamplingOptions *options, const ZiggyHipBuffer *uniforms,
+                              ZiggyHipBuffer *out_tokens, uint32_t rows, uint32_t vocab, char *error_message,
+                              size_t error_message_len);
 
 /* Times one kernel of the decode step (no counterpart in the reference; its
  * Metal profiler times host-side encode, runtime/metal_profile.zig:80-315):

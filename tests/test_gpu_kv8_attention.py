@@ -1,0 +1,134 @@
+"""Attention over the 8-bit cache against a 64-bit form, element by element within the bound that its 32-bit sums
+allow (longctx_oracle.kv8_attention derives it).  Blocks that no query sees hold NaN scales."""
+import numpy as np
+import pytest
+
+from tests import longctx_oracle as oracle
+from tests.test_gpu_kv8 import upload
+from zhip import hip
+
+pytestmark = pytest.mark.gpu
+
+
+def attend(ctx, heads, kvh, hd, position, queries=1, window=0, layer=0, layers=1, context=None, scale=None, sharp=1.0,
+           stride=0, spoil=True, seed=0):
+    print("kv8 attention", heads, kvh, hd, position, queries, window, layer, flush=True)
+    rng = np.random.default_rng(seed + heads * 1000 + hd + position + queries)
+    n = position + queries
+    context = context or n + 40
+    ls = [oracle.Kv8(kvh, context, hd, rng) for _ in range(layers)]
+    c = ls[layer]
+    if spoil:
+        first = max(0, position + 1 - window) if window else 0
+        for w in range(2):
+            c.scales[w][:, :first // 32] = np.nan
+            c.scales[w][:, (n - 1) // 32 + 1:] = np.inf
+            # rows behind the last query's, in its own block
+            c.codes[w][:, n:] = 127
+    cache = upload(ctx, ls, context)
+    width = heads * hd
+    stride = stride or width
+    qf = rng.normal(0, sharp, queries * stride).astype(np.float32)
+    q = qf[np.arange(queries)[:, None] * stride + np.arange(width)].reshape(queries, heads, hd)
+    out = ctx.buffer(np.full(queries * width + 64, 3, np.float32))
+    scale = hd ** -0.5 if scale is None else scale
+    ctx.kv8_attention(cache, ctx.buffer(qf), out, heads, layer, position, queries, window=window, scale=scale, q_stride=stride)
+    got = out.read()
+    assert np.all(got[queries * width:] == 3)
+    want, bound = oracle.kv8_attention(c, q, position, scale, window)
+    err = np.abs(got[:queries * width].reshape(want.shape) - want)
+    assert np.all(err <= bound), (err / bound).max()
+    return cache, q, got[:queries * width]
+
+
+@pytest.mark.parametrize("heads,kvh,hd", [(32, 8, 128), (32, 4, 64), (6, 6, 96), (8, 1, 256), (1, 1, 64), (5, 1, 128), (24, 2, 96), (16, 1, 128),
+                                          (64, 1, 64), (34, 2, 256)])
+@pytest.mark.parametrize("position", [0, 1, 30, 31, 32, 33, 63, 64, 150, 511, 1000])
+def test_one_query(hip_ctx, heads, kvh, hd, position):
+    attend(hip_ctx, heads, kvh, hd, position)
+
+
+@pytest.mark.parametrize("heads,kvh,hd", [(32, 8, 128), (4, 4, 64), (8, 2, 256), (12, 4, 96)])
+@pytest.mark.parametrize("position", [4111, 8191, 20000])
+def test_one_query_far_out(hip_ctx, heads, kvh, hd, position):
+    attend(hip_ctx, heads, kvh, hd, position, layer=1, layers=2)
+
+
+@pytest.mark.parametrize("position,window", [(0, 1), (100, 1), (100, 32), (100, 33), (100, 101), (100, 102), (4000, 64), (4000, 65),
+                                             (4000, 1023), (5000, 4096), (37, 4294967295)])
+@pytest.mark.parametrize("queries", [1, 5])
+def test_windows(hip_ctx, position, window, queries):
+    attend(hip_ctx, 8, 2, 128, position, queries, window)
+
+
+@pytest.mark.parametrize("heads,kvh,hd", [(32, 8, 128), (8, 8, 64), (7, 1, 96), (4, 2, 256)])
+@pytest.mark.parametrize("position,queries", [(0, 2), (0, 9), (31, 2), (50, 16), (1500, 9), (0, 17), (20, 40), (3, 100)])
+def test_several_queries(hip_ctx, heads, kvh, hd, position, queries):
+    attend(hip_ctx, heads, kvh, hd, position, queries)
+
+
+@pytest.mark.parametrize("heads,kvh,hd", [(8, 2, 128), (4, 1, 64), (3, 3, 96), (2, 1, 256)])
+@pytest.mark.parametrize("position,queries,window", [(0, 300, 0), (77, 257, 0), (900, 130, 0), (64, 200, 50), (2000, 70, 333), (10, 128, 129)])
+def test_prompts(hip_ctx, heads, kvh, hd, position, queries, window):
+    attend(hip_ctx, heads, kvh, hd, position, queries, window)
+
+
+@pytest.mark.parametrize("queries", [1, 9, 90])
+def test_strided_queries_and_scales(hip_ctx, queries):
+    attend(hip_ctx, 4, 2, 64, 200, queries, stride=4 * 64 + 3, scale=0.3, sharp=3.0)
+    attend(hip_ctx, 4, 2, 128, 200, queries, stride=1000, scale=-0.1)
+    attend(hip_ctx, 4, 2, 128, 200, queries, scale=0.0)
+
+
+@pytest.mark.parametrize("queries", [1, 70])
+@pytest.mark.parametrize("position", [400, 6000])
+def test_small_weights_beside_a_dominant_key_keep_their_value(hip_ctx, queries, position):
+    """One key whose score is 13 above thousands of others (weights of 2e-6 beside 1), with a value of 0 in the
+    output's dims: what is left is the sum of the small ones.  Bound: a weight is held to 2^-21 of itself, its
+    score's error (longctx_oracle) added, or to 2^-38 of the largest."""
+    heads, kvh, hd = 2, 1, 64
+    n = position + queries
+    rng = np.random.default_rng(position)
+    c = oracle.Kv8(kvh, n, hd, rng)
+    c.scales[0][:] = np.float32(1 / 64)
+    c.scales[1][:] = np.float32(1 / 64)
+    c.codes[0][:] = rng.integers(-2, 3, c.codes[0].shape)
+    c.codes[1][:] = rng.integers(30, 100, c.codes[1].shape)
+    c.codes[0][:, 3] = 13
+    c.codes[1][:, 3] = 0
+    q = np.full((queries, heads, hd), 1.0, np.float32)
+    cache = upload(hip_ctx, [c], n)
+    out = hip_ctx.empty(q.nbytes)
+    hip_ctx.kv8_attention(cache, hip_ctx.buffer(q), out, heads, 0, position, queries, scale=1.0)
+    want, _ = oracle.kv8_attention(c, q, position, 1.0)
+    got = out.read().reshape(want.shape)
+    e = 2 * (hd + 8) * 2.0 ** -23 * 13 * hd / 64
+    bound = (e + 2.0 ** -19 + n * 2.0 ** -22) * np.abs(want) + n * 2.0 ** -38 * 100 / 64
+    assert np.all(np.abs(got - want) <= bound), (np.abs(got - want) / bound).max()
+
+
+def test_a_marked_block_in_sight_reads_as_nan(hip_ctx):
+    for queries in (1, 80):
+        rng = np.random.default_rng(2)
+        c = oracle.Kv8(2, 200, 64, rng)
+        c.scales[1][1, 3] = np.nan
+        cache = upload(hip_ctx, [c], 200)
+        q = rng.normal(0, 1, (queries, 4, 64)).astype(np.float32)
+        out = hip_ctx.empty(q.nbytes)
+        hip_ctx.kv8_attention(cache, hip_ctx.buffer(q), out, 4, 0, 60, queries)
+        got = out.read().reshape(queries, 4, 64)
+        seen = np.arange(60, 60 + queries) >= 96
+        assert np.array_equal(np.isnan(got), np.broadcast_to((seen[:, None] & (np.arange(4) >= 2))[..., None], got.shape))
+
+
+@pytest.mark.parametrize("queries", [1, 9, 200])
+def test_same_bits_each_time(hip_ctx, queries):
+    cache, q, first = attend(hip_ctx, 32, 8, 128, 3000, queries)
+    qb, out = hip_ctx.buffer(q), hip_ctx.empty(q.nbytes)
+    other = hip_ctx.empty(q.nbytes)
+    hip_ctx.begin()
+    for _ in range(5):
+        hip_ctx.kv8_attention(cache, qb, other, 32, 0, 1000, queries)
+        hip_ctx.kv8_attention(cache, qb, out, 32, 0, 3000, queries)
+    hip_ctx.commit()
+    assert np.array_equal(out.read().view(np.uint32), first.view(np.uint32))

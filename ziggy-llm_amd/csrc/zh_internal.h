@@ -50,6 +50,7 @@ struct ZiggyHipBuffer {
     int device = 0;  // destroy needs only this, so a buffer may outlive its context
     void *ptr = nullptr;
     size_t len = 0;
+    bool owned = true;  // false: the caller's memory (ziggy_hip_wrap_buffer)
 };
 
 namespace zh {

@@ -1,0 +1,70 @@
+// zh_rope.hip -- rotary positions of many rows, with frequencies scaled for long contexts.
+//
+// (x0, x1) -> m (x0 cos t - x1 sin t, x0 sin t + x1 cos t), t = position * f_i.  The angle is taken in
+// turns and in 64 bits, f_i / 2 pi = 2^(i exponent) / 2 pi, and reduced to half a turn either way
+// before it is rounded to 32 bits: at position 10^6 a 32-bit angle would be off by 0.06 rad.
+#include "zh_longctx.h"
+
+namespace zh {
+
+namespace {
+
+constexpr int kPairs = 4;  // pairs of a thread: two float4 of every head it takes
+
+__device__ __forceinline__ double turns_per_position(const RopeRows &p, int i) {
+    double f = exp2((double)i * p.freq.exponent) * 0.15915494309189533577;
+    const double g = fmin(fmax(p.freq.a + p.freq.b * (p.freq.by_turns ? f : (double)i), 0.0), 1.0);
+    f *= g + (1.0 - g) * p.freq.inv_factor;
+    return p.factors ? f / (double)p.factors[i] : f;
+}
+
+// A thread takes four pairs (or eight values behind the rotated ones) of every hp-th head of its rows.
+template <bool ALIGNED> __global__ void __launch_bounds__(256) rope_rows_kernel(RopeRows p, int units, int hp) {
+    const int u = threadIdx.x % units, h0 = threadIdx.x / units, half = p.rd / 2, turning = (half + kPairs - 1) / kPairs;
+    if (h0 >= hp) return;
+    const bool rotates = u < turning;
+    const int i0 = rotates ? kPairs * u : p.rd + 8 * (u - turning);
+    const int n = rotates ? min(kPairs, half - i0) : min(8, p.hd - i0);
+    double f[kPairs];
+    if (rotates)
+        for (int j = 0; j < kPairs; j++) f[j] = turns_per_position(p, min(i0 + j, half - 1));
+    for (uint32_t r = blockIdx.x; r < p.rows; r += gridDim.x) {
+        const float *src = p.src + (size_t)r * p.src_stride;
+        float *dst = p.dst + (size_t)r * p.dst_stride;
+        float c[kPairs], s[kPairs];
+        if (rotates) {
+            const double at = (double)(p.positions ? p.positions[r] : p.first + r);
+            for (int j = 0; j < kPairs; j++) {
+                const double t = at * f[j];
+                sincospif((float)(2.0 * (t - rint(t))), &s[j], &c[j]);
+                c[j] *= p.magnitude, s[j] *= p.magnitude;
+            }
+        }
+        for (int h = blockIdx.y * hp + h0; h < p.heads; h += gridDim.y * hp) {
+            const float *x = src + (size_t)h * p.hd;
+            float *y = dst + (size_t)h * p.hd;
+            if (!rotates) {
+                for (int j = 0; j < n; j++) y[i0 + j] = x[i0 + j];
+                continue;
+            }
+            for (int j = 0; j < n; j++) {
+                const int a = p.style ? i0 + j : 2 * (i0 + j), b = p.style ? a + half : a + 1;
+                const float xa = x[a], xb = x[b];
+                y[a] = xa * c[j] - xb * s[j];
+                y[b] = xa * s[j] + xb * c[j];
+            }
+        }
+    }
+}
+
+}  // namespace
+
+hipError_t launch_rope_rows(const RopeRows &p, int cus, hipStream_t s) {
+    const int units = (p.rd / 2 + kPairs - 1) / kPairs + (p.hd - p.rd + 7) / 8, hp = 256 / units;
+    const int passes = (p.heads + hp - 1) / hp;
+    const dim3 grid(p.rows < 65536u ? p.rows : 65536u, passes);
+    hipLaunchKernelGGL(rope_rows_kernel<false>, grid, dim3(256), 0, s, p, units, hp);
+    return hipGetLastError();
+}
+
+}  // namespace zh

@@ -288,7 +288,7 @@ int ziggy_hip_create_buffer(ZiggyHipContext *ctx, const void *bytes, size_t leng
 
 void ziggy_hip_destroy_buffer(ZiggyHipBuffer *b) {
     if (!b) return;
-    if (b->ptr) {
+    if (b->ptr && b->owned) {
         // hipFree waits for the device; the context may already be gone
         hipSetDevice(b->device);
         hipFree(b->ptr);

@@ -100,6 +100,43 @@ class SamplingOptions(ctypes.Structure):
         super().__init__(temperature, repeat_penalty, top_k, top_p, min_p)
 
 
+ROPE_NONE, ROPE_LINEAR, ROPE_YARN, ROPE_BANDS = 0, 1, 2, 3
+
+
+class RopeDesc(ctypes.Structure):
+    """Rotary frequencies and their scaling (ZiggyHipRopeDesc)."""
+    _fields_ = [(n, ctypes.c_uint32) for n in ("head_dim", "rope_dim", "rope_style", "scaling", "original_context")] + [
+        (n, ctypes.c_float) for n in ("freq_base", "factor", "low", "high", "magnitude")]
+
+    def __init__(self, head_dim, rope_dim=None, style=0, base=10000.0, scaling=ROPE_NONE, factor=1.0,
+                 original_context=0, low=1.0, high=32.0, magnitude=1.0):
+        super().__init__(head_dim, head_dim if rope_dim is None else rope_dim, style, scaling, original_context, base,
+                         factor, low, high, magnitude)
+
+
+KV8_BLOCK = 32  # ZIGGY_HIP_KV8_BLOCK
+
+
+class Kv8CacheDesc(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_void_p) for n in ("k_codes", "k_scales", "v_codes", "v_scales")] + [
+        (n, ctypes.c_uint32) for n in ("layers", "head_count_kv", "head_dim", "context_length")]
+
+
+class Kv8Cache:
+    """A K/V cache in 8 bits over four buffers (ZiggyHipKv8Cache has their layout); Context.kv8_cache makes one."""
+
+    def __init__(self, k_codes: "Buffer", k_scales: "Buffer", v_codes: "Buffer", v_scales: "Buffer", layers: int,
+                 heads_kv: int, head_dim: int, context: int):
+        self.buffers = (k_codes, k_scales, v_codes, v_scales)
+        self._desc = Kv8CacheDesc(*(b.h for b in self.buffers), layers, heads_kv, head_dim, context)
+
+    @property
+    def desc(self) -> Kv8CacheDesc:
+        if not all(b.h for b in self.buffers):
+            raise HipError(6, "a buffer of the cache was freed")
+        return self._desc
+
+
 class MoeLayerDesc(ctypes.Structure):
     _fields_ = [(n, TensorDesc) for n in MOE_LAYER_FIELDS]
 
@@ -141,6 +178,7 @@ def lib() -> ctypes.CDLL:
         "ziggy_hip_create_buffer": [vp, vp, sz, ctypes.POINTER(vp)] + E,
         "ziggy_hip_create_empty_buffer": [vp, sz, ctypes.POINTER(vp)] + E,
         "ziggy_hip_destroy_buffer": [vp],
+        "ziggy_hip_wrap_buffer": [vp, vp, sz, ctypes.POINTER(vp)] + E,
         "ziggy_hip_buffer_length": [vp],
         "ziggy_hip_write_buffer": [vp, vp, sz, sz] + E,
         "ziggy_hip_read_buffer": [vp, vp, sz, sz] + E,
@@ -175,6 +213,13 @@ def lib() -> ctypes.CDLL:
         "ziggy_hip_normalize_topk_f32": [vp, vp, u32, ctypes.c_bool, ctypes.c_bool, f] + E,
         "ziggy_hip_weighted_sum_topk_f32": [vp, vp, vp, vp, u32, u32] + E,
         "ziggy_hip_sigmoid_scale_add_f32": [vp, vp, vp, vp, u32] + E,
+        "ziggy_hip_rope_rows_f32": [vp, ctypes.POINTER(RopeDesc), vp, sz, sz, vp, sz, sz, vp, u32, vp, u32, u32] + E,
+        "ziggy_hip_kv8_codes_length": [u32, u32, u32, u32],
+        "ziggy_hip_kv8_scales_length": [u32, u32, u32, u32],
+        "ziggy_hip_kv8_store": [vp, ctypes.POINTER(Kv8CacheDesc), vp, sz, vp, sz, sz, u32, u32, u32] + E,
+        "ziggy_hip_kv8_load_f32": [vp, ctypes.POINTER(Kv8CacheDesc), vp, vp, u32, u32, u32] + E,
+        "ziggy_hip_kv8_attention_f32": [vp, ctypes.POINTER(Kv8CacheDesc), vp, sz, vp, u32, u32, u32, u32, u32, f] + E,
+        "ziggy_hip_sample_rows_f32": [vp, vp, sz, vp, u32, ctypes.POINTER(SamplingOptions), vp, vp, u32, u32] + E,
         "ziggy_hip_session_create": [vp, ctypes.POINTER(ModelDesc), ctypes.POINTER(TensorDesc),
                                      ctypes.POINTER(TensorDesc), ctypes.POINTER(TensorDesc),
                                      ctypes.POINTER(LayerDesc), ctypes.POINTER(vp)] + E,
@@ -222,6 +267,7 @@ def lib() -> ctypes.CDLL:
                 "ziggy_hip_session_destroy": None, "ziggy_hip_moe_stack_destroy": None, "ziggy_hip_buffer_length": sz,
                 "ziggy_hip_session_position": u32, "ziggy_hip_version": ctypes.c_char_p,
                 "ziggy_hip_session_kv_pages": u32,
+                "ziggy_hip_kv8_codes_length": sz, "ziggy_hip_kv8_scales_length": sz,
                 "ziggy_hip_shortlist_len": u32}
     for name, args in sigs.items():
         fn = getattr(L, name)
@@ -298,6 +344,22 @@ class Context:
         b = Buffer(self, h, nbytes)
         self._owned.add(b)
         return b
+
+    def wrap(self, address: int, nbytes: int) -> Buffer:
+        """A buffer over the caller's device memory (ziggy_hip_wrap_buffer), a torch tensor's data_ptr() for
+        instance; the caller keeps it alive and orders other streams' work on it."""
+        h = ctypes.c_void_p()
+        _call("ziggy_hip_wrap_buffer", self.h, address, nbytes, ctypes.byref(h))
+        b = Buffer(self, h, nbytes)
+        self._owned.add(b)
+        return b
+
+    def kv8_cache(self, layers: int, heads_kv: int, head_dim: int, context: int) -> Kv8Cache:
+        """An empty 8-bit K/V cache."""
+        codes = lib().ziggy_hip_kv8_codes_length(layers, heads_kv, head_dim, context)
+        scales = lib().ziggy_hip_kv8_scales_length(layers, heads_kv, head_dim, context)
+        return Kv8Cache(self.empty(codes), self.empty(scales), self.empty(codes), self.empty(scales), layers, heads_kv,
+                        head_dim, context)
 
     # ---- primitive ops ----
     def matvec(self, ttype, m: Buffer, x: Buffer, y: Buffer, rows, cols, add=False, m_off=0, y_off=0):
@@ -401,6 +463,33 @@ class Context:
 
     def sigmoid_scale_add(self, d, s, scalar, n):
         _call("ziggy_hip_sigmoid_scale_add_f32", self.h, d.h, s.h, scalar.h, n)
+
+    # ---- operators of a step over a long context ----
+    def rope_rows(self, desc: RopeDesc, src: Buffer, dst: Buffer, rows: int, heads: int, positions: Buffer | None = None,
+                  first_position: int = 0, src_stride: int = 0, dst_stride: int = 0, src_off: int = 0, dst_off: int = 0,
+                  freq_factors: Buffer | None = None):
+        _call("ziggy_hip_rope_rows_f32", self.h, ctypes.byref(desc), src.h, src_off, src_stride, dst.h, dst_off,
+              dst_stride, positions.h if positions else None, first_position,
+              freq_factors.h if freq_factors else None, rows, heads)
+
+    def kv8_store(self, cache: Kv8Cache, k: Buffer, v: Buffer, layer: int, position: int, rows: int,
+                  row_stride: int = 0, k_off: int = 0, v_off: int = 0):
+        _call("ziggy_hip_kv8_store", self.h, ctypes.byref(cache.desc), k.h, k_off, v.h, v_off, row_stride, layer,
+              position, rows)
+
+    def kv8_load(self, cache: Kv8Cache, k_out: Buffer, v_out: Buffer, layer: int, position: int, rows: int):
+        _call("ziggy_hip_kv8_load_f32", self.h, ctypes.byref(cache.desc), k_out.h, v_out.h, layer, position, rows)
+
+    def kv8_attention(self, cache: Kv8Cache, q: Buffer, out: Buffer, heads: int, layer: int, position: int,
+                      queries: int = 1, window: int = 0, scale: float | None = None, q_stride: int = 0):
+        scale = 1.0 / np.sqrt(cache.desc.head_dim) if scale is None else scale
+        _call("ziggy_hip_kv8_attention_f32", self.h, ctypes.byref(cache.desc), q.h, q_stride, out.h, heads, layer,
+              position, queries, window, float(scale))
+
+    def sample_rows(self, logits: Buffer, out: Buffer, uniforms: Buffer, options: SamplingOptions, rows: int, vocab: int,
+                    recent: Buffer | None = None, recent_count: int = 0, row_stride: int = 0):
+        _call("ziggy_hip_sample_rows_f32", self.h, logits.h, row_stride, recent.h if recent else None, recent_count,
+              ctypes.byref(options), uniforms.h, out.h, rows, vocab)
 
     def begin(self):
         _call("ziggy_hip_begin_sequence", self.h)

@@ -1,71 +1,562 @@
 // zh_kv8_attn.hip -- attention over the cache held in 8 bits.
 //
-// o = sum_t w_t v_t / sum_t w_t, w_t = 2^(qscale q.k_t - max), in one pass with the running maximum and
-// sum; a block's scale multiplies its scores and its weights, so the codes enter as they are.
+// o = sum_t w_t v_t / sum_t w_t, w_t = 2^(s_t - max), s_t = qscale q.k_t, in one pass with the running
+// maximum and sum.  The codes are integers of at most 127, exact in binary16, and enter the matrix
+// cores as they are; a block's scales multiply its scores and its weights.  A query enters as two
+// binary16 pieces of q 2^e (the power of two that brings the row's largest value to [2^14, 2^15)), a
+// weight as two of 2^14 w, each rounded to nearest: q to 2^-22, w to 2^-22 of itself or 2^-39 of the
+// largest.  Products accumulate in binary32, maximum and sum are binary32.
+//
+// Two kernels.  Few (query, head) rows of a kv head (decoding): a wavefront streams blocks of 32
+// positions, K and V straight from memory into operands.  Many (prompts): a workgroup's 128 rows share
+// tiles of 64 positions in LDS.  Both split the positions over workgroups where rows alone leave CUs
+// idle; a second launch joins the splits in their order, so results don't change from run to run.
 #include "zh_longctx.h"
 
 namespace zh {
 
 namespace {
 
+typedef _Float16 kh2 __attribute__((ext_vector_type(2)));
+typedef _Float16 kh8 __attribute__((ext_vector_type(8)));
+typedef float kf4 __attribute__((ext_vector_type(4)));
+typedef float kf16 __attribute__((ext_vector_type(16)));
+
+constexpr float kWeight = 16384.f;  // of the largest weight: its pieces below binary16's 65504
+
 __device__ __forceinline__ uint32_t first_seen(uint32_t pos, uint32_t window) {
     return window && pos >= window ? pos + 1 - window : 0u;
 }
 
-// A workgroup takes one head of one query, 256 positions at a time.
-template <int HD> __global__ void __launch_bounds__(256) kv8_attn_simple_kernel(Kv8Attn p) {
-    __shared__ float q[HD], w[256], red[4];
-    const int tid = threadIdx.x, head = blockIdx.x, kvh = head / (p.heads / p.c.nkv);
-    const size_t base = (size_t)kvh * p.c.blocks;
-    for (uint32_t qi = blockIdx.y; qi < p.queries; qi += gridDim.y) {
-        const uint32_t pos = p.position + qi, lo = first_seen(pos, p.window);
-        __syncthreads();
-        for (int d = tid; d < HD; d += 256) q[d] = p.q[qi * p.q_stride + (size_t)head * HD + d] * p.qscale;
-        __syncthreads();
-        float m = -INFINITY, l = 0.f, o = 0.f;
-        for (uint32_t at = lo & ~31u; at <= pos; at += 256) {
-            const uint32_t t = at + tid;
-            const bool seen = t >= lo && t <= pos;
-            float s = -INFINITY;
-            if (seen) {
-                const int8_t *k = p.c.kc + (base * kKv8Block + t) * HD;
-                float a = 0.f;
-                for (int d = 0; d < HD; d++) a += q[d] * (float)k[d];
-                s = a * p.c.ks[base + t / kKv8Block];
+// four codes -> binary16: 0x64XX is 1024 + XX, XX = code + 128
+__device__ __forceinline__ void widen4(uint32_t w, uint32_t &a, uint32_t &b) {
+    const uint32_t u = w ^ 0x80808080u;
+    const kh2 off = {(_Float16)-1152.f, (_Float16)-1152.f};
+    a = __builtin_bit_cast(uint32_t, __builtin_bit_cast(kh2, __builtin_amdgcn_perm(0x64646464u, u, 0x04010400u)) + off);
+    b = __builtin_bit_cast(uint32_t, __builtin_bit_cast(kh2, __builtin_amdgcn_perm(0x64646464u, u, 0x04030402u)) + off);
+}
+__device__ __forceinline__ kh8 widen8(uint32_t x, uint32_t y) {
+    uint4 r;
+    widen4(x, r.x, r.y);
+    widen4(y, r.z, r.w);
+    return __builtin_bit_cast(kh8, r);
+}
+
+// The power of two that brings a row's largest value to [2^14, 2^15), and its inverse.
+__device__ __forceinline__ void row_power(float largest, float &up, float &down) {
+    const uint32_t e = max(__float_as_uint(largest) >> 23 & 255u, 15u);
+    const bool fine = e < 255u;  // (an infinity or NaN: as it is)
+    up = fine ? __uint_as_float((268u - e) << 23) : 1.f;
+    down = fine ? __uint_as_float((e - 14u) << 23) : 1.f;
+}
+
+__device__ __forceinline__ float finite(float v) { return v == -INFINITY ? 0.f : v; }
+
+struct Kv8Params {
+    Kv8Layer c;
+    const float *q;
+    size_t q_stride;
+    float *out, *part, *part_ml;  // splits > 1: row r of split z at part + (z rows + r) hd, {max, sum} at part_ml + ...2
+    uint32_t position, queries, window;
+    int heads, group, splits;
+    uint32_t row_groups;
+    float qscale;
+};
+
+// ---- few rows ----
+//
+// A wavefront takes blocks of 32 positions (4 wavefronts of a workgroup in turn).  Scores on
+// 16x16x32 products, S[position][column] = K Q^T; lane (i, g) holds K row 8 (i / 4) + 4 pt + i % 4 of
+// its half pt, so that the 8 scores it gets back are of positions 8 g .. 8 g + 7, in order: what the
+// value products O[column][dim] = P V take as their left operand, and what its 8 bytes of a V dim
+// hold.  NR 8: 16 columns are the two pieces of 8 rows; NR 16: of 16 rows, each piece a product.
+template <int HD, int NR> struct Few {
+    static constexpr int KS = HD / 32, DT = HD / 16;   // k-steps, dim tiles
+    static constexpr int KB = HD % 64 ? 8 : 16;        // bytes of a lane's K load
+    static constexpr int KL = HD / 4 / KB;             // K loads of a row
+    static constexpr int KW = KB / 4;
+};
+template <int HD> struct Block8 {
+    uint32_t k[2][HD / 16], v[HD / 16][2];
+};
+
+template <int HD, int NR, int PER_CU>
+__global__ void __launch_bounds__(256, PER_CU) kv8_few_kernel(Kv8Params p) {
+    using F = Few<HD, NR>;
+    constexpr int P = NR == 16 ? 2 : 1;  // products of a step: one for each piece, or both in one
+    __shared__ float os[4][NR][HD + 4], ms[4][NR], ls[4][NR];
+    const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, i16 = lane & 15, g = lane >> 4;
+    const int kvh = blockIdx.x % p.c.nkv, z = blockIdx.y;
+    const uint32_t rows = p.queries * (uint32_t)p.group, r0 = blockIdx.x / p.c.nkv * NR;
+    const uint32_t rlast = min(r0 + NR, rows) - 1;
+    // the blocks that any of the rows sees, and this split's share of them
+    const uint32_t pos_min = p.position + r0 / p.group, pos_max = p.position + rlast / p.group;
+    const uint32_t lo_min = first_seen(pos_min, p.window), lo_max = first_seen(pos_max, p.window);
+    const uint32_t b_first = lo_min / kKv8Block, nb_all = pos_max / kKv8Block - b_first + 1;
+    const uint32_t b0 = b_first + (uint32_t)((uint64_t)nb_all * z / p.splits);
+    const uint32_t b1 = b_first + (uint32_t)((uint64_t)nb_all * (z + 1) / p.splits);
+    const int nb = (int)(b1 - b0) > wave ? (int)((b1 - b0 - wave + 3) / 4) : 0;  // of this wavefront: b0 + wave + 4 t
+
+    // this lane's column: a row, and for NR 8 a piece of it
+    const uint32_t row = min(r0 + (uint32_t)(NR == 8 ? i16 >> 1 : i16), rlast);
+    const uint32_t qi = row / p.group, pos = p.position + qi, lo = first_seen(pos, p.window);
+    const int head = kvh * p.group + (int)(row % p.group);
+    const float *q = p.q + (size_t)qi * p.q_stride + (size_t)head * HD;
+    // dim of value e of step s: byte 8 s + e of a lane's row
+    auto dim_of = [&](int s, int e) { return 4 * F::KB * (8 * s / F::KB) + F::KB * g + 8 * s % F::KB + e; };
+    kh8 qb[P][F::KS];
+    float down;
+    {
+        float x[F::KS][8], top = 0.f, up;
+#pragma unroll
+        for (int s = 0; s < F::KS; s++)
+#pragma unroll
+            for (int e = 0; e < 8; e++) x[s][e] = q[dim_of(s, e)] * p.qscale, top = fmaxf(top, fabsf(x[s][e]));
+        top = xmax<32>(xmax<16>(top));
+        row_power(top, up, down);
+#pragma unroll
+        for (int s = 0; s < F::KS; s++)
+#pragma unroll
+            for (int e = 0; e < 8; e++) {
+                const float v = x[s][e] * up;
+                const _Float16 h = (_Float16)v, l = (_Float16)(v - (float)h);
+                if constexpr (NR == 8) qb[0][s][e] = i16 & 1 ? l : h;
+                else qb[0][s][e] = h, qb[1][s][e] = l;
             }
-            float mx = wave_max_f32(s);
-            if ((tid & 63) == 0) red[tid >> 6] = mx;
-            __syncthreads();
-            mx = fmaxf(m, fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3])));
-            const float al = exp2f(m - mx), e = seen ? exp2f(s - mx) : 0.f;
-            m = mx;
-            w[tid] = e;
-            __syncthreads();
-            l *= al, o *= al;
-            if (tid < HD) {
-                const int n = (int)min(256u, pos - at + 1);
-                for (int i = 0; i < n; i++) {
-                    if (at + i < lo) continue;
-                    const size_t b = base + (at + i) / kKv8Block;
-                    l += w[i];
-                    o += w[i] * p.c.vs[b] * (float)p.c.vc[b * (kKv8Block * HD) + tid * kKv8Block + ((at + i) & 31)];
+    }
+    const size_t head0 = (size_t)kvh * p.c.blocks;
+    const int8_t *kl = p.c.kc + head0 * (kKv8Block * HD) + (size_t)(8 * (i16 >> 2) + (i16 & 3)) * HD + F::KB * g;
+    const int8_t *vl = p.c.vc + head0 * (kKv8Block * HD) + (size_t)i16 * kKv8Block + 8 * g;
+    auto block_of = [&](int t) { return b0 + wave + 4 * (uint32_t)min(t, nb - 1); };
+    auto load = [&](Block8<HD> &r, int t) {
+        const size_t at = (size_t)block_of(t) * (kKv8Block * HD);
+#pragma unroll
+        for (int pt = 0; pt < 2; pt++)
+#pragma unroll
+            for (int j = 0; j < F::KL; j++)
+                __builtin_memcpy(&r.k[pt][F::KW * j], kl + at + 4 * pt * HD + 4 * F::KB * j, F::KB);
+#pragma unroll
+        for (int d = 0; d < F::DT; d++) __builtin_memcpy(r.v[d], vl + at + d * (16 * kKv8Block), 8);
+    };
+    float ksl = 0.f, vsl = 0.f;  // scales of the wavefront's next 64 blocks, one a lane
+    auto load_scales = [&](int t) {
+        const uint32_t b = block_of(t + lane);
+        ksl = p.c.ks[head0 + b], vsl = p.c.vs[head0 + b];
+    };
+    kf4 o[F::DT];
+#pragma unroll
+    for (int d = 0; d < F::DT; d++) o[d] = kf4{0.f, 0.f, 0.f, 0.f};
+    float m = -INFINITY, l = 0.f;
+
+    auto compute = [&](const Block8<HD> &r, int t) {
+        const uint32_t b = block_of(t), first = b * kKv8Block;
+        const float ks = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(ksl), t & 63)) * down;
+        const float vs = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(vsl), t & 63));
+        kf4 s[2];
+#pragma unroll
+        for (int pt = 0; pt < 2; pt++) {
+            s[pt] = kf4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int k = 0; k < F::KS; k++) {
+                const kh8 a = widen8(r.k[pt][2 * k], r.k[pt][2 * k + 1]);
+#pragma unroll
+                for (int j = 0; j < P; j++) s[pt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, qb[j][k], s[pt], 0, 0, 0);
+            }
+        }
+        const bool edge = first < lo_max || first + kKv8Block - 1 > pos_min;
+        float w[8], mx = -INFINITY;
+#pragma unroll
+        for (int e = 0; e < 8; e++) {
+            float v = s[e >> 2][e & 3];
+            if constexpr (NR == 8)  // the other piece's column
+                v += __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), 0xB1, 0xF, 0xF, false));
+            w[e] = v * ks;
+        }
+        if (edge)
+#pragma unroll
+            for (int e = 0; e < 8; e++) {
+                const uint32_t at = first + 8 * g + e;
+                if (at < lo || at > pos) w[e] = -INFINITY;
+            }
+#pragma unroll
+        for (int e = 0; e < 8; e++) mx = fmaxf(mx, w[e]);
+        mx = xmax<32>(xmax<16>(mx));
+        if (__any(mx > m)) {
+            const float mn = fmaxf(m, mx), al = __builtin_amdgcn_exp2f(m - finite(mn));
+            m = mn;
+            l *= al;
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                const float a = __shfl(al, 4 * g + j);
+#pragma unroll
+                for (int d = 0; d < F::DT; d++) o[d][j] *= a;
+            }
+        }
+        const float mf = finite(m);
+        kh8 ph[P];
+#pragma unroll
+        for (int e = 0; e < 8; e++) {
+            const float x = __builtin_amdgcn_exp2f(w[e] - mf);
+            l += x;
+            const _Float16 h = (_Float16)(x * kWeight), lw = (_Float16)fmaf(x, kWeight, -(float)h);
+            if constexpr (NR == 8) ph[0][e] = i16 & 1 ? lw : h;
+            else ph[0][e] = h, ph[1][e] = lw;
+        }
+        const float unit = vs * (1.f / kWeight);
+        float f[4] = {unit, unit, unit, unit};
+        if (edge)  // a block out of a row's sight adds nothing to it, whatever its scale
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                const uint32_t other = min(r0 + (uint32_t)(NR == 8 ? (4 * g + j) >> 1 : 4 * g + j), rlast), at = p.position + other / p.group;
+                if (first + kKv8Block - 1 < first_seen(at, p.window) || first > at) f[j] = 0.f;
+            }
+#pragma unroll
+        for (int d = 0; d < F::DT; d++) {
+            const kh8 v = widen8(r.v[d][0], r.v[d][1]);
+            kf4 a = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int j = 0; j < P; j++) a = __builtin_amdgcn_mfma_f32_16x16x32_f16(ph[j], v, a, 0, 0, 0);
+#pragma unroll
+            for (int j = 0; j < 4; j++) o[d][j] = fmaf(f[j], a[j], o[d][j]);
+        }
+    };
+
+    if (nb > 0) {
+        Block8<HD> x, y;
+        load_scales(0);
+        load(x, 0);
+        load(y, 1);
+        for (int t = 0; t < nb; t += 2) {
+            if (t && (t & 63) == 0) load_scales(t);
+            compute(x, t);
+            load(x, t + 2);
+            if (t + 1 < nb) compute(y, t + 1);
+            load(y, t + 3);
+        }
+    }
+    // the wavefront's rows: both pieces' outputs, the sum over its lanes
+    l = xsum<32>(xsum<16>(l));
+#pragma unroll
+    for (int d = 0; d < F::DT; d++)
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            if constexpr (NR == 8) {
+                if (j % 2 == 0) os[wave][2 * g + j / 2][16 * d + i16] = o[d][j] + o[d][j + 1];
+            } else
+                os[wave][4 * g + j][16 * d + i16] = o[d][j];
+        }
+    if (lane < 16 && (NR == 16 || lane % 2 == 0)) ms[wave][NR == 8 ? lane / 2 : lane] = m, ls[wave][NR == 8 ? lane / 2 : lane] = l;
+    __syncthreads();
+    const uint32_t live = rlast - r0 + 1;
+    for (int u = tid; u < (int)live * HD; u += 256) {
+        const int r = u / HD, d = u % HD;
+        const float mx = fmaxf(fmaxf(ms[0][r], ms[1][r]), fmaxf(ms[2][r], ms[3][r])), mf = finite(mx);
+        float sum = 0.f, a = 0.f;
+#pragma unroll
+        for (int w = 0; w < 4; w++) {
+            const float al = __builtin_amdgcn_exp2f(ms[w][r] - mf);
+            sum = fmaf(al, ls[w][r], sum), a = fmaf(al, os[w][r][d], a);
+        }
+        const uint32_t gr = r0 + r;
+        const size_t to = (size_t)(gr / p.group) * p.heads + kvh * p.group + gr % p.group;
+        if (p.splits == 1) {
+            p.out[to * HD + d] = a / sum;
+        } else {  // a split's outputs are those of its own positions (0 where it has none in sight)
+            const size_t at = (size_t)z * p.queries * p.heads + to;
+            p.part[at * HD + d] = mx == -INFINITY && sum == 0.f ? 0.f : a / sum;
+            if (d == 0) p.part_ml[2 * at] = mx, p.part_ml[2 * at + 1] = sum;
+        }
+    }
+}
+
+// ---- many rows ----
+//
+// A workgroup takes 128 (query, head) rows of one kv head, 32 a wavefront, over tiles of 64 positions
+// (two blocks), widened to binary16 on their way into LDS, two tiles deep.  S[position][row] = K Q^T
+// and O[dim][row] = V^T P^T on 32x32x16 products.  K rows are read with bits 2 and 3 of their index
+// exchanged, so that a lane's weights are of positions 16 k + 8 h .. + 7: 16 bytes of a V dim in LDS.
+// The V scale of a block goes into the exponent, w = 2^(s + log2 v - max), v its share of the largest
+// scale in the workgroup's range; the block's weights over v add to the sum.  (Shares below 2^-60, an
+// all-zero block's among them, count as 2^-60: their values are below what the largest one's rounding
+// leaves, and the sum keeps their weight.)  A multiplication of the outputs per block instead would be
+// 128 more vector instructions a tile.
+template <int HD> constexpr int kManyPerCu = HD <= 128 ? 2 : 1;
+
+template <int HD> __global__ void __launch_bounds__(256, kManyPerCu<HD>) kv8_many_kernel(Kv8Params p) {
+    constexpr int KT = HD / 16, DT = HD / 32;
+    constexpr int KST = 2 * HD + 16, VST = 2 * 64 + 16;      // bytes of a K row and of a V dim: 16 rows in distinct banks
+    constexpr int BUF = 64 * KST + HD * VST;
+    constexpr int UN = 4 * HD, NU = (UN + 255) / 256;         // 16-byte pieces of a K or V tile, of a thread
+    __shared__ __align__(16) char lds[2 * BUF];
+    __shared__ float top_scale[4];
+    const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, l32 = lane & 31, lh = lane >> 5;
+    const int kvh = blockIdx.x % p.c.nkv, z = blockIdx.y;
+    const int qn = 128 / p.group, nqb = ((int)p.queries + qn - 1) / qn, qb = nqb - 1 - (int)blockIdx.x / p.c.nkv;
+    const int q0 = qb * qn, qlast = min(q0 + qn, (int)p.queries) - 1;
+    const uint32_t kv_last = p.position + qlast, kv_first = first_seen(p.position + q0, p.window);
+    const int t_first = (int)(kv_first >> 6), nt_all = (int)(kv_last >> 6) + 1 - t_first;
+    const int t0 = t_first + (int)((int64_t)nt_all * z / p.splits), t1 = t_first + (int)((int64_t)nt_all * (z + 1) / p.splits);
+    const int v = wave * 32 + l32, qi = q0 + v / p.group, head = kvh * p.group + v % p.group;
+    const bool valid = v < qn * p.group && qi <= qlast;
+    const int qc = min(qi, qlast);
+    const uint32_t qpos = p.position + qc, qlo = first_seen(qpos, p.window);
+    // the wavefront's earliest query, and the latest one's first position: tiles between need no mask
+    const uint32_t wave_first = p.position + min(q0 + wave * 32 / p.group, qlast);
+    const uint32_t wave_lo = first_seen(p.position + min(q0 + (wave * 32 + 31) / p.group, qlast), p.window);
+    const size_t head0 = (size_t)kvh * p.c.blocks;
+    const uint32_t last_block = kv_last / kKv8Block;
+
+    uint4 kr[NU], vr[NU];
+    auto load = [&](int t) {
+        const uint32_t ba = 2 * (uint32_t)t, bb = min(ba + 1, last_block);
+        const int8_t *ka = p.c.kc + (head0 + ba) * (kKv8Block * HD), *kb = p.c.kc + (head0 + bb) * (kKv8Block * HD);
+        const int8_t *va = p.c.vc + (head0 + ba) * (kKv8Block * HD), *vb = p.c.vc + (head0 + bb) * (kKv8Block * HD);
+#pragma unroll
+        for (int i = 0; i < NU; i++) {
+            const int u = min(tid + 256 * i, UN - 1);
+            const bool second = u >= UN / 2;
+            const int at = 16 * (second ? u - UN / 2 : u);
+            kr[i] = *reinterpret_cast<const uint4 *>((second ? kb : ka) + at);
+            vr[i] = *reinterpret_cast<const uint4 *>((second ? vb : va) + at);
+        }
+    };
+    auto put = [&](int t) {
+        char *ks = lds + (t & 1) * BUF, *vs = ks + 64 * KST;
+#pragma unroll
+        for (int i = 0; i < NU; i++) {
+            const int u = tid + 256 * i;
+            if (UN % 256 && u >= UN) break;
+            constexpr int R = HD / 16;  // 16-code pieces of a K row
+            uint4 a, b;
+            auto widen = [&](const uint4 &x) {
+                widen4(x.x, a.x, a.y), widen4(x.y, a.z, a.w), widen4(x.z, b.x, b.y), widen4(x.w, b.z, b.w);
+            };
+            widen(kr[i]);
+            uint4 *kd = reinterpret_cast<uint4 *>(ks + u / R * KST + u % R * 32);
+            kd[0] = a, kd[1] = b;
+            widen(vr[i]);
+            const int w = u % (2 * HD), half = u / (2 * HD);  // a block's dims hold two pieces each
+            uint4 *vd = reinterpret_cast<uint4 *>(vs + w / 2 * VST + half * 64 + w % 2 * 32);
+            vd[0] = a, vd[1] = b;
+        }
+    };
+
+    // the largest V scale in this workgroup's range
+    float big = 0.f;
+    for (int b = 2 * t0 + tid; b < 2 * t1; b += 256)
+        if ((uint32_t)b <= last_block) big = fmaxf(big, p.c.vs[head0 + b]);
+    big = wave_max_f32(big);
+    if (lane == 0) top_scale[wave] = big;
+    if (t0 < t1) load(t0);
+
+    kh8 qh[KT], ql[KT];
+    float down;
+    {
+        const float *q = p.q + (size_t)qc * p.q_stride + (size_t)(kvh * p.group + (valid ? v % p.group : 0)) * HD + 8 * lh;
+        float top = 0.f, up;
+        for (int t = 0; t < KT; t++)
+            for (int e = 0; e < 8; e++) top = fmaxf(top, fabsf(q[16 * t + e] * p.qscale));
+        top = xmax<32>(top);
+        row_power(top, up, down);
+#pragma unroll
+        for (int t = 0; t < KT; t++)
+#pragma unroll
+            for (int e = 0; e < 8; e++) {
+                const float x = q[16 * t + e] * p.qscale * up;
+                qh[t][e] = (_Float16)x;
+                ql[t][e] = (_Float16)(x - (float)qh[t][e]);
+            }
+    }
+    kf16 o[DT];
+#pragma unroll
+    for (int d = 0; d < DT; d++)
+#pragma unroll
+        for (int r = 0; r < 16; r++) o[d][r] = 0.f;
+    float m = -INFINITY, l = 0.f;
+    if (t0 < t1) put(t0);
+    __syncthreads();
+    big = fmaxf(fmaxf(top_scale[0], top_scale[1]), fmaxf(top_scale[2], top_scale[3]));
+    const int krow = (l32 & 0x13) | (l32 & 4) << 1 | (l32 & 8) >> 1;
+
+    for (int t = t0; t < t1; t++) {
+        const uint32_t ba = 2 * (uint32_t)t, bb = min(ba + 1, last_block);
+        const float kscale[2] = {p.c.ks[head0 + ba], p.c.ks[head0 + bb]}, vscale[2] = {p.c.vs[head0 + ba], p.c.vs[head0 + bb]};
+        if (t + 1 < t1) load(t + 1);
+        __builtin_amdgcn_sched_barrier(0);
+        const char *ks = lds + (t & 1) * BUF + krow * KST + 16 * lh, *vs = lds + (t & 1) * BUF + 64 * KST + l32 * VST + 16 * lh;
+        kf16 s[2];
+#pragma unroll
+        for (int pt = 0; pt < 2; pt++) {
+#pragma unroll
+            for (int r = 0; r < 16; r++) s[pt][r] = 0.f;
+#pragma unroll
+            for (int k = 0; k < KT; k++) {
+                const kh8 a = *reinterpret_cast<const kh8 *>(ks + pt * 32 * KST + 32 * k);
+                s[pt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, qh[k], s[pt], 0, 0, 0);
+                s[pt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, ql[k], s[pt], 0, 0, 0);
+            }
+        }
+        const bool edge = 64 * (uint32_t)t + 63 > wave_first || 64 * (uint32_t)t < wave_lo;
+        uint32_t keep = 0xFFFFFFFFu;
+        if (edge) {
+            keep = 0;
+#pragma unroll
+            for (int pt = 0; pt < 2; pt++)
+#pragma unroll
+                for (int r = 0; r < 16; r++) {
+                    const uint32_t at = 64 * (uint32_t)t + 32 * pt + 16 * (r >> 3) + 8 * lh + (r & 7);
+                    const bool in = at >= qlo && at <= qpos;
+                    keep |= (uint32_t)in << (16 * pt + r);
+                    if (!in) s[pt][r] = -INFINITY;
+                }
+        }
+        float f[2], lv[2], mx = -INFINITY;
+#pragma unroll
+        for (int pt = 0; pt < 2; pt++) {
+            f[pt] = kscale[pt] * down;
+            const float share = vscale[pt] / big;
+            lv[pt] = big > 0.f ? __builtin_amdgcn_logf(share < 0x1p-60f ? 0x1p-60f : share) : 0.f * vscale[pt];
+            float a = s[pt][0];
+#pragma unroll
+            for (int r = 1; r < 16; r++) a = fmaxf(a, s[pt][r]);
+            mx = fmaxf(mx, fmaf(a, f[pt], lv[pt]));
+        }
+        mx = xmax<32>(mx);
+        if (__any(mx > m)) {
+            const float mn = fmaxf(m, mx), al = __builtin_amdgcn_exp2f(m - finite(mn));
+            m = mn;
+            l *= al;
+#pragma unroll
+            for (int d = 0; d < DT; d++)
+#pragma unroll
+                for (int r = 0; r < 16; r++) o[d][r] *= al;
+        }
+        const float mf = finite(m);
+#pragma unroll
+        for (int pt = 0; pt < 2; pt++) {
+            const float c = lv[pt] - mf;
+            float sum = 0.f;
+#pragma unroll
+            for (int r = 0; r < 16; r++) s[pt][r] = __builtin_amdgcn_exp2f(fmaf(s[pt][r], f[pt], c));
+            if (edge)
+#pragma unroll
+                for (int r = 0; r < 16; r++)
+                    if (!(keep >> (16 * pt + r) & 1u)) s[pt][r] = 0.f;
+            uint32_t hi[8], lo[8];
+#pragma unroll
+            for (int i = 0; i < 8; i++) {
+                const float a = s[pt][2 * i], b = s[pt][2 * i + 1];
+                sum += a + b;
+                const kh2 h = kh2{(_Float16)a, (_Float16)b} * (_Float16)kWeight;  // (exact)
+                const kh2 w = {(_Float16)fmaf(a, kWeight, -(float)h[0]), (_Float16)fmaf(b, kWeight, -(float)h[1])};
+                hi[i] = __builtin_bit_cast(uint32_t, h);
+                lo[i] = __builtin_bit_cast(uint32_t, w);
+            }
+            // (a row with none of the block in sight takes nothing from it, whatever its scale)
+            l += sum == 0.f ? 0.f : sum * __builtin_amdgcn_exp2f(-lv[pt]);
+#pragma unroll
+            for (int k = 0; k < 2; k++) {
+                const kh8 ph = __builtin_bit_cast(kh8, uint4{hi[4 * k], hi[4 * k + 1], hi[4 * k + 2], hi[4 * k + 3]}),
+                          pl = __builtin_bit_cast(kh8, uint4{lo[4 * k], lo[4 * k + 1], lo[4 * k + 2], lo[4 * k + 3]});
+#pragma unroll
+                for (int d = 0; d < DT; d++) {
+                    const kh8 a = *reinterpret_cast<const kh8 *>(vs + d * 32 * VST + pt * 64 + 32 * k);
+                    o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, ph, o[d], 0, 0, 0);
+                    o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, pl, o[d], 0, 0, 0);
                 }
             }
-            __syncthreads();
+            __builtin_amdgcn_sched_barrier(0);
         }
-        if (tid < HD) p.out[((size_t)qi * p.heads + head) * HD + tid] = o / l;
+        if (t + 1 < t1) put(t + 1);
+        __syncthreads();
     }
+    l = xsum<32>(l);
+    if (!valid) return;
+    // a split's outputs are those of its own positions (0 where it has none in sight)
+    const float inv = p.splits > 1 && m == -INFINITY && l == 0.f ? 0.f : big / (l * kWeight);
+    const size_t row = (size_t)qi * p.heads + head, at = (size_t)z * p.queries * p.heads + row;
+    float *dst = (p.splits > 1 ? p.part + at * HD : p.out + row * HD) + 4 * lh;
+#pragma unroll
+    for (int d = 0; d < DT; d++)
+#pragma unroll
+        for (int g = 0; g < 4; g++)
+            *reinterpret_cast<float4 *>(dst + 32 * d + 8 * g) =
+                make_float4(o[d][4 * g] * inv, o[d][4 * g + 1] * inv, o[d][4 * g + 2] * inv, o[d][4 * g + 3] * inv);
+    if (p.splits > 1 && lh == 0) *reinterpret_cast<float2 *>(p.part_ml + 2 * at) = make_float2(m, l);
+}
+
+// The splits' partial results of a row joined in their order, a workgroup per row.
+template <int HD> __global__ void __launch_bounds__(256) kv8_join_kernel(const float *__restrict__ part, const float *__restrict__ ml,
+                                                                       float *__restrict__ out, size_t rows, int splits) {
+    constexpr int C = HD / 4, N = 256 / C;  // float4s of a row, splits read at a time
+    __shared__ float4 acc[N][C];
+    __shared__ float sums[N];
+    const size_t row = blockIdx.x;
+    const int c = threadIdx.x % C, n = threadIdx.x / C;
+    float m = -INFINITY;
+    for (int z = 0; z < splits; z++) m = fmaxf(m, ml[2 * (z * rows + row)]);
+    const float mf = finite(m);
+    if (n < N) {
+        float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
+        float l = 0.f;
+        for (int z = n; z < splits; z += N) {
+            const size_t at = z * rows + row;
+            const float w = __builtin_amdgcn_exp2f(ml[2 * at] - mf) * ml[2 * at + 1];
+            const float4 v = *reinterpret_cast<const float4 *>(part + at * HD + 4 * c);
+            a.x = fmaf(w, v.x, a.x), a.y = fmaf(w, v.y, a.y), a.z = fmaf(w, v.z, a.z), a.w = fmaf(w, v.w, a.w);
+            l += w;
+        }
+        acc[n][c] = a;
+        if (c == 0) sums[n] = l;
+    }
+    __syncthreads();
+    if (n) return;
+    float4 a = acc[0][c];
+    float l = sums[0];
+    for (int k = 1; k < N; k++) {
+        const float4 v = acc[k][c];
+        a.x += v.x, a.y += v.y, a.z += v.z, a.w += v.w, l += sums[k];
+    }
+    *reinterpret_cast<float4 *>(out + row * HD + 4 * c) = make_float4(a.x / l, a.y / l, a.z / l, a.w / l);
 }
 
 }  // namespace
 
-hipError_t launch_kv8_attention(const Kv8Attn &p, int cus, hipStream_t s) {
-    const dim3 grid(p.heads, p.queries < 32768u ? p.queries : 32768u);
-    switch (p.c.hd) {
-    case 64: hipLaunchKernelGGL(kv8_attn_simple_kernel<64>, grid, dim3(256), 0, s, p); break;
-    case 96: hipLaunchKernelGGL(kv8_attn_simple_kernel<96>, grid, dim3(256), 0, s, p); break;
-    case 128: hipLaunchKernelGGL(kv8_attn_simple_kernel<128>, grid, dim3(256), 0, s, p); break;
-    case 256: hipLaunchKernelGGL(kv8_attn_simple_kernel<256>, grid, dim3(256), 0, s, p); break;
+hipError_t launch_kv8_attention(const Kv8Attn &a, int cus, hipStream_t s) {
+    Kv8Params p{};
+    p.c = a.c, p.q = a.q, p.q_stride = a.q_stride, p.out = a.out;
+    p.position = a.position, p.queries = a.queries, p.window = a.window;
+    p.heads = a.heads, p.group = a.heads / a.c.nkv, p.qscale = a.qscale;
+    const uint64_t rows = (uint64_t)a.queries * p.group;  // of a kv head
+    const bool many = rows > 32;
+    const int nr = rows > 8 ? 16 : 8, qn = 128 / p.group;
+    const uint64_t wgs = p.c.nkv * (many ? (a.queries + (uint64_t)qn - 1) / qn : (rows + nr - 1) / nr);
+    if (wgs > 0x7FFFFFFFu) return hipErrorInvalidValue;
+    // positions: of the query that sees the fewest
+    const uint32_t seen = a.window && a.window <= a.position ? a.window : a.position + 1;
+    const uint64_t least = many ? 4 * 64 : 4 * kKv8Block, most = many ? 16 : 64;
+    const uint64_t total = (uint64_t)a.queries * a.heads;
+    uint64_t splits = 2 * (uint64_t)cus / wgs;
+    splits = splits < seen / least ? splits : seen / least;
+    splits = splits < most ? splits : most;
+    while (splits > 1 && splits * total * (a.c.hd + 2) > a.part_floats) splits--;
+    p.splits = splits > 1 ? (int)splits : 1;
+    p.part = a.part, p.part_ml = a.part + (size_t)p.splits * total * a.c.hd;
+    const dim3 grid((unsigned)wgs, (unsigned)p.splits);
+    auto go = [&](auto h) {
+        constexpr int HD = decltype(h)::value, PER_CU = HD == 256 ? 1 : 2;
+        if (many) hipLaunchKernelGGL(kv8_many_kernel<HD>, grid, dim3(256), 0, s, p);
+        else if (nr == 8) hipLaunchKernelGGL((kv8_few_kernel<HD, 8, PER_CU>), grid, dim3(256), 0, s, p);
+        else hipLaunchKernelGGL((kv8_few_kernel<HD, 16, PER_CU>), grid, dim3(256), 0, s, p);
+        if (p.splits > 1)
+            hipLaunchKernelGGL(kv8_join_kernel<HD>, dim3((unsigned)total), dim3(256), 0, s, p.part, p.part_ml, p.out,
+                               (size_t)total, p.splits);
+    };
+    switch (a.c.hd) {
+    case 64: go(std::integral_constant<int, 64>{}); break;
+    case 96: go(std::integral_constant<int, 96>{}); break;
+    case 128: go(std::integral_constant<int, 128>{}); break;
+    case 256: go(std::integral_constant<int, 256>{}); break;
     default: return hipErrorInvalidValue;
     }
     return hipGetLastError();

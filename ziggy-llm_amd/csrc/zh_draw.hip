@@ -2,23 +2,199 @@
 // penalty, with given random numbers.
 //
 // Every limit keeps a beginning of the candidates in some order, and the draw is the first candidate
-// whose running sum reaches a target.  So all of it is one search: the first element, in descending
-// order of a key, whose running sum of weights (or count) reaches a target, found digit by digit of
-// the key from histograms of the sums.  Weights are exp((a - max) / T) in 64 bits, rounded to integers
-// of 2^-s, so that sums are exact whatever their order.
+// whose running sum reaches a target.  Weights are exp((a - max) / T) in 64 bits, rounded to integers
+// of 2^-s, so that sums are exact whatever their order and a row's token depends on its inputs alone.
+//
+// Three launches, none of which sorts the row:
+//   stats   slices of 2048 logits: maximum, minimum and mean, from which a linear scale of 256 bins
+//           is laid over the values, the largest in bin 0;
+//   bins    each logit's bin, and per slice the bins' sums of weights (top-k: counts);
+//   finish  a workgroup per row: the bin in which a target lies, then 1024 finer bins of that bin's
+//           logits, then the few logits of the finer bin in order.  With top-k the bins above the k-th
+//           logit are sorted in LDS instead, and everything else is prefix sums of at most 1024.
+// A row whose fine bin (or whose bins above the k-th) hold more than LDS does -- thousands of equal
+// logits -- goes digit by digit of the key through the whole row instead.
 #include "zh_longctx.h"
 
 namespace zh {
 
 namespace {
 
-constexpr int kThreads = 1024;
+constexpr int kSliceLogits = 2048, kBins = 256, kFine = 1024, kThreads = 1024, kMaxSlices = 262144 / kSliceLogits;
+constexpr int kTopKMax = 1024, kList = 4096;  // candidates of a limited row, logits sorted in LDS
+
+typedef unsigned long long u64;
+
+// a row's part of the workspace
+struct RowHead {
+    float max, per_bin;  // of the binned logits; bins per unit
+    u64 pad;
+};
+struct SliceStats {
+    float max, min, sum, count;  // of what is finite and no mask (above -1e30)
+};
+__host__ __device__ constexpr size_t up256(size_t n) { return (n + 255) / 256 * 256; }
+__host__ __device__ constexpr uint32_t slices_of(uint32_t vocab) { return (vocab + kSliceLogits - 1) / kSliceLogits; }
+__host__ __device__ constexpr size_t row_bytes(uint32_t vocab) {
+    return 256 + up256(slices_of(vocab) * sizeof(SliceStats)) + slices_of(vocab) * (kBins + 1) * sizeof(u64) + up256(vocab) + 256;
+}
+struct RowWork {
+    RowHead *head;
+    SliceStats *stats;
+    u64 *sums;     // [slice][kBins]
+    u64 *whole;    // [slice]
+    uint8_t *bin;  // [vocab]
+};
+__device__ __forceinline__ RowWork row_work(const SampleRows &p, uint32_t row) {
+    char *at = (char *)p.work + row * up256(row_bytes(p.vocab));
+    RowWork w;
+    const uint32_t n = slices_of(p.vocab);
+    w.head = (RowHead *)at, at += 256;
+    w.stats = (SliceStats *)at, at += up256(n * sizeof(SliceStats));
+    w.bin = (uint8_t *)at, at += up256(p.vocab);
+    w.sums = (u64 *)at, at += (size_t)n * kBins * sizeof(u64);
+    w.whole = (u64 *)at;
+    return w;
+}
 
 // float -> an integer that orders as it does; NaN as -infinity, the zeros equal
 __device__ __forceinline__ uint32_t ordered(float v) {
     const uint32_t b = __float_as_uint(v != v ? -INFINITY : v + 0.f);
     return (b & 0x80000000u) ? ~b : (b | 0x80000000u);
 }
+__device__ __forceinline__ float unordered(uint32_t o) { return __uint_as_float((o & 0x80000000u) ? (o & 0x7FFFFFFFu) : ~o); }
+
+__device__ __forceinline__ float penalised(float v, float r) { return v < 0.f ? v * r : v / r; }
+
+// What a row's limits come to.
+struct Policy {
+    bool limited, sorted;
+    uint32_t top_k;
+    double per_t, least, unit;  // unit 2^s
+    __device__ explicit Policy(const SampleRows &p) {
+        top_k = p.o.top_k == 0 ? p.vocab : min(p.o.top_k, p.vocab);
+        limited = top_k < p.vocab, sorted = p.o.top_p < 1.f;
+        per_t = 1.0 / (double)p.o.temperature, least = (double)p.o.min_p;
+        const int bits = top_k > 1 ? 32 - __clz((int)top_k - 1) : 0;
+        unit = __longlong_as_double((long long)(1023 + 62 - bits) << 52);
+    }
+    // (the same operations wherever it is called: the sums of the bins and of their logits agree)
+    __device__ __forceinline__ u64 weight(float a, float mx) const {
+#pragma clang fp contract(off)
+        if (!(a > -INFINITY)) return 0;
+        const double e = exp(((double)a - (double)mx) * per_t);
+        return e >= least ? (u64)rint(e * unit) : 0;
+    }
+};
+
+__device__ __forceinline__ int bin_of(float a, float mx, float per_bin, float &t) {
+    t = fmaxf((mx - a) * per_bin, 0.f);  // (0 times infinity: 0)
+    return (int)fminf(t, (float)(kBins - 1));
+}
+__device__ __forceinline__ int fine_of(float t, int bin) {
+    return (int)fminf(fmaxf((t - (float)bin) * (float)kFine, 0.f), (float)(kFine - 1));
+}
+
+// The bits of the row's recent tokens with ids first .. first + 32 words - 1, into LDS.
+__device__ __forceinline__ void mark_recent(const SampleRows &p, uint32_t row, uint32_t *bits, uint32_t words, uint32_t first) {
+    for (uint32_t i = threadIdx.x; i < words; i += blockDim.x) bits[i] = 0;
+    __syncthreads();
+    for (uint32_t i = threadIdx.x; i < p.recent_count; i += blockDim.x) {
+        const uint32_t id = p.recent[(size_t)row * p.recent_count + i];
+        if (id < p.vocab && id >= first && id - first < 32 * words) atomicOr(&bits[(id - first) / 32], 1u << (id % 32));
+    }
+    __syncthreads();
+}
+
+// The logits that the bins order: penalised, or, with top-k (which comes first), as they are.
+struct Slice {
+    uint32_t first, n;
+    float a[kSliceLogits / 256];
+    __device__ Slice(const SampleRows &p, uint32_t row, bool penalise, uint32_t *bits) {
+        first = blockIdx.x * kSliceLogits, n = min(p.vocab - first, (uint32_t)kSliceLogits);
+        const float *x = p.x + row * p.stride + first;
+#pragma unroll
+        for (int i = 0; i < kSliceLogits / 256; i++) {
+            const uint32_t j = threadIdx.x + 256 * i;
+            const float v = x[min(j, n - 1)];
+            a[i] = j < n && v == v ? v : -INFINITY;
+        }
+        if (!penalise) return;
+        mark_recent(p, row, bits, kSliceLogits / 32, first);
+#pragma unroll
+        for (int i = 0; i < kSliceLogits / 256; i++) {
+            const uint32_t j = threadIdx.x + 256 * i;
+            if (bits[j / 32] >> (j % 32) & 1u) a[i] = penalised(a[i], p.o.repeat_penalty);
+        }
+    }
+};
+
+__global__ void __launch_bounds__(256) draw_stats_kernel(SampleRows p) {
+    __shared__ uint32_t bits[kSliceLogits / 32];
+    __shared__ float4 red[4];
+    const uint32_t row = blockIdx.y;
+    const Slice s(p, row, p.recent && !Policy(p).limited, bits);
+    float mx = -INFINITY, mn = INFINITY, sum = 0.f, count = 0.f;
+#pragma unroll
+    for (int i = 0; i < kSliceLogits / 256; i++) {
+        mx = fmaxf(mx, s.a[i]);
+        if (s.a[i] > -1e30f && s.a[i] < INFINITY) mn = fminf(mn, s.a[i]), sum += s.a[i], count += 1.f;
+    }
+    for (int d = 32; d; d >>= 1) {
+        mx = fmaxf(mx, __shfl_xor(mx, d)), mn = fminf(mn, __shfl_xor(mn, d));
+        sum += __shfl_xor(sum, d), count += __shfl_xor(count, d);
+    }
+    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = make_float4(mx, mn, sum, count);
+    __syncthreads();
+    if (threadIdx.x) return;
+    for (int w = 1; w < 4; w++) mx = fmaxf(mx, red[w].x), mn = fminf(mn, red[w].y), sum += red[w].z, count += red[w].w;
+    row_work(p, row).stats[blockIdx.x] = SliceStats{mx, mn, sum, count};
+}
+
+__global__ void __launch_bounds__(256) draw_bins_kernel(SampleRows p) {
+    __shared__ uint32_t bits[kSliceLogits / 32];
+    __shared__ float4 all[kMaxSlices];
+    __shared__ u64 sums[kBins], red[4];
+    const uint32_t row = blockIdx.y, slices = slices_of(p.vocab);
+    const RowWork w = row_work(p, row);
+    const Policy policy(p);
+    if (threadIdx.x < slices) all[threadIdx.x] = *reinterpret_cast<const float4 *>(w.stats + threadIdx.x);
+    sums[threadIdx.x] = 0;
+    const Slice s(p, row, p.recent && !policy.limited, bits);
+    __syncthreads();
+    float mx = -INFINITY, mn = INFINITY, sum = 0.f, count = 0.f;
+    for (uint32_t i = threadIdx.x & 63; i < slices; i += 64)
+        mx = fmaxf(mx, all[i].x), mn = fminf(mn, all[i].y), sum += all[i].z, count += all[i].w;
+    for (int d = 32; d; d >>= 1) {
+        mx = fmaxf(mx, __shfl_xor(mx, d)), mn = fminf(mn, __shfl_xor(mn, d));
+        sum += __shfl_xor(sum, d), count += __shfl_xor(count, d);
+    }
+    // the scale: with top-k down to the mean; else to the lowest, or to where weights are 0, or, where
+    // few lie far below the others, as far below the mean as half again the largest is above it
+    const float above = mx - sum / count;
+    float range = policy.limited ? above : fminf(fminf(43.7f * p.o.temperature, mx - mn), 2.5f * above);
+    const float per_bin = range > 0.f && fabsf(mx) < INFINITY ? (float)kBins / range : 0.f;
+    if (blockIdx.x == 0 && threadIdx.x == 0) w.head->max = mx, w.head->per_bin = per_bin;
+    u64 whole = 0;
+#pragma unroll
+    for (int i = 0; i < kSliceLogits / 256; i++) {
+        const uint32_t j = threadIdx.x + 256 * i;
+        if (j >= s.n) continue;
+        float t;
+        const int b = bin_of(s.a[i], mx, per_bin, t);
+        w.bin[s.first + j] = (uint8_t)b;
+        const u64 v = !(fabsf(mx) < INFINITY) ? 0ull : policy.limited ? (s.a[i] > -INFINITY ? 1ull : 0ull) : policy.weight(s.a[i], mx);
+        if (v) atomicAdd(&sums[b], v);
+        whole += v;
+    }
+    for (int d = 32; d; d >>= 1) whole += (u64)__shfl_xor((long long)whole, d);
+    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = whole;
+    __syncthreads();
+    w.sums[blockIdx.x * kBins + threadIdx.x] = sums[threadIdx.x];
+    if (threadIdx.x == 0) w.whole[blockIdx.x] = red[0] + red[1] + red[2] + red[3];
+}
+
+// ---- finish: a workgroup of 1024 per row ----
 
 struct Key {
     uint32_t w[3];
@@ -27,59 +203,103 @@ __device__ __forceinline__ bool at_least(const Key &a, const Key &b) {
     return a.w[0] != b.w[0] ? a.w[0] > b.w[0] : a.w[1] != b.w[1] ? a.w[1] > b.w[1] : a.w[2] >= b.w[2];
 }
 
-struct Shared {
-    unsigned long long hist[256], sum;
-    uint32_t digit;
-    uint32_t seen[262144 / 32];
-    Key best;
-    unsigned long long red[kThreads / 64];
-    Key redk[kThreads / 64];
+struct Finish {
+    u64 list[kList];              // keys being sorted
+    u64 sums[kFine];              // bins' sums; fine bins'
+    u64 wave[kThreads / 64];
+    uint32_t seen[262144 / 32];   // recent tokens
+    u64 value;
+    uint32_t found, count;
+    Key key[kThreads / 64];
 };
 
+// Inclusive prefix sum over the workgroup; *total: the whole.
+__device__ u64 prefix(Finish &f, u64 v, u64 *total) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    for (int d = 1; d < 64; d <<= 1) {
+        const u64 o = (u64)__shfl_up((long long)v, d);
+        if (lane >= d) v += o;
+    }
+    __syncthreads();
+    if (lane == 63) f.wave[wave] = v;
+    __syncthreads();
+    u64 before = 0, all = 0;
+    for (int i = 0; i < kThreads / 64; i++) {
+        if (i == wave) before = all;
+        all += f.wave[i];
+    }
+    *total = all;
+    return v + before;
+}
+// The lowest thread whose running sum `run` (of its own v) reaches target; *before: the sum ahead of it.
+// (None, which the callers' targets exclude: the last one with a weight.)
+__device__ uint32_t first_reaching(Finish &f, u64 run, u64 v, u64 target, u64 *before) {
+    __syncthreads();
+    if (threadIdx.x == 0) f.found = 0, f.value = 0;
+    __syncthreads();
+    const bool mine = v && run >= target && run - v < target;
+    if (mine) f.found = threadIdx.x, f.value = run - v;
+    __syncthreads();
+    *before = f.value;
+    return f.found;
+}
+
+__device__ u64 target_of(double share, u64 total) {
+    const double t = ceil(share * (double)total);
+    const u64 c = t >= 1.0 ? (u64)t : 1ull;
+    return c < total ? c : total;
+}
+
+// f.list[0 .. n) in descending order (n at most kList; the places up to a power of two are filled).
+__device__ void sort_list(Finish &f, uint32_t n) {
+    uint32_t size = 2;
+    while (size < n) size <<= 1;
+    for (uint32_t i = n + threadIdx.x; i < size; i += kThreads) f.list[i] = 0;
+    __syncthreads();
+    for (uint32_t run = 2; run <= size; run <<= 1)
+        for (uint32_t d = run >> 1; d; d >>= 1) {
+            for (uint32_t i = threadIdx.x; i < size / 2; i += kThreads) {
+                const uint32_t a = 2 * d * (i / d) + i % d, b = a + d;
+                const u64 x = f.list[a], y = f.list[b];
+                if ((x < y) == ((a & run) == 0)) f.list[a] = y, f.list[b] = x;
+            }
+            __syncthreads();
+        }
+}
+
 // The first element, in descending order of key(i), at which the sum of weight(i) reaches target (1 ..
-// the whole sum); *before: the sum of those ahead of it.
+// the whole sum); *before: the sum of those ahead of it.  Digit by digit, whatever the row.
 template <class K, class W>
-__device__ Key reach(Shared &sh, uint32_t n, unsigned long long target, unsigned long long *before, K key, W weight) {
+__device__ Key reach(Finish &f, uint32_t n, u64 target, u64 *before, K key, W weight) {
     Key b{};
-    unsigned long long done = 0;
+    u64 done = 0;
     for (int d = 0; d < 12; d++) {
         const int word = d / 4, shift = 24 - 8 * (d % 4);
         __syncthreads();
-        if (threadIdx.x < 256) sh.hist[threadIdx.x] = 0;
+        if (threadIdx.x < 256) f.sums[threadIdx.x] = 0;
         __syncthreads();
         for (uint32_t i = threadIdx.x; i < n; i += kThreads) {
-            const unsigned long long w = weight(i);
-            if (w == 0) continue;
             const Key k = key(i);
             bool in = true;
             for (int j = 0; j < 3; j++) {
                 const uint32_t mask = j < word ? 0xFFFFFFFFu : j > word || shift == 24 ? 0u : 0xFFFFFFFFu << (shift + 8);
                 in = in && ((k.w[j] ^ b.w[j]) & mask) == 0;
             }
-            if (in) atomicAdd(&sh.hist[k.w[word] >> shift & 255u], w);
+            const u64 w = in ? weight(i) : 0;
+            if (w) atomicAdd(&f.sums[k.w[word] >> shift & 255u], w);
         }
         __syncthreads();
-        if (threadIdx.x == 0) {
-            unsigned long long sum = done;
-            uint32_t last = 0, at = 256;
-            for (int g = 255; g >= 0 && at == 256; g--) {
-                if (!sh.hist[g]) continue;
-                last = g;
-                if (sum + sh.hist[g] >= target) at = g;
-                else sum += sh.hist[g];
-            }
-            sh.digit = at < 256 ? at : last;
-            sh.sum = sum;
-        }
-        __syncthreads();
-        b.w[word] |= sh.digit << shift;
-        done = sh.sum;
+        const u64 v = threadIdx.x < 256 ? f.sums[255 - threadIdx.x] : 0;
+        u64 total, ahead;
+        const u64 run = prefix(f, v, &total);
+        b.w[word] |= (255 - first_reaching(f, run, v, target - done, &ahead)) << shift;
+        done += ahead;
     }
     *before = done;
     return b;
 }
 
-template <class K> __device__ Key largest(Shared &sh, uint32_t n, K key) {
+template <class K> __device__ Key largest(Finish &f, uint32_t n, K key) {
     Key k{};
     for (uint32_t i = threadIdx.x; i < n; i += kThreads) {
         const Key c = key(i);
@@ -91,116 +311,199 @@ template <class K> __device__ Key largest(Shared &sh, uint32_t n, K key) {
         if (at_least(o, k)) k = o;
     }
     __syncthreads();
-    if ((threadIdx.x & 63) == 0) sh.redk[threadIdx.x >> 6] = k;
+    if ((threadIdx.x & 63) == 0) f.key[threadIdx.x >> 6] = k;
     __syncthreads();
-    if (threadIdx.x == 0) {
-        for (int j = 1; j < kThreads / 64; j++)
-            if (at_least(sh.redk[j], k)) k = sh.redk[j];
-        sh.best = k;
-    }
-    __syncthreads();
-    return sh.best;
+    for (int j = 0; j < kThreads / 64; j++)
+        if (at_least(f.key[j], k)) k = f.key[j];
+    return k;
 }
 
-__device__ unsigned long long block_sum(Shared &sh, unsigned long long v) {
-    for (int d = 32; d; d >>= 1) {
-        const uint32_t lo = (uint32_t)__shfl_xor((int)(uint32_t)v, d), hi = (uint32_t)__shfl_xor((int)(uint32_t)(v >> 32), d);
-        v += (unsigned long long)hi << 32 | lo;
+// Calls take(i) for the logits of the bins that `wanted` names.
+template <class B, class T> __device__ __forceinline__ void of_bins(const uint8_t *bin, uint32_t n, B wanted, T take) {
+    for (uint32_t at = 16 * threadIdx.x; at < n; at += 16 * kThreads) {
+        const uint4 v = *reinterpret_cast<const uint4 *>(bin + at);
+        const uint32_t word[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+        for (int j = 0; j < 16; j++)
+            if (wanted(word[j / 4] >> (8 * (j % 4)) & 255u) && at + j < n) take(at + j);
     }
-    __syncthreads();
-    if ((threadIdx.x & 63) == 0) sh.red[threadIdx.x >> 6] = v;
-    __syncthreads();
-    v = 0;
-    for (int j = 0; j < kThreads / 64; j++) v += sh.red[j];
-    return v;
 }
 
-__device__ unsigned long long target_of(double share, unsigned long long total) {
-    const double t = ceil(share * (double)total);
-    const unsigned long long c = t >= 1.0 ? (unsigned long long)t : 1ull;
-    return c < total ? c : total;
-}
-
-// A workgroup takes one row.
-__global__ void __launch_bounds__(kThreads) draw_simple_kernel(SampleRows p, unsigned long long *weights, size_t ld) {
-    __shared__ Shared sh;
-    const uint32_t n = p.vocab;
-    const float *x = p.x + blockIdx.x * p.stride;
-    unsigned long long *w = weights + blockIdx.x * ld;
-    auto raw = [&](uint32_t i) { return x[i]; };
-    if (p.o.temperature <= 0.f) {
-        const Key k = largest(sh, n, [&](uint32_t i) { return Key{{ordered(raw(i)), ~i, 0}}; });
-        if (threadIdx.x == 0) p.out[blockIdx.x] = ~k.w[1];
-        return;
-    }
-    if (p.recent) {
-        for (uint32_t i = threadIdx.x; i < (n + 31) / 32; i += kThreads) sh.seen[i] = 0;
-        __syncthreads();
-        for (uint32_t i = threadIdx.x; i < p.recent_count; i += kThreads) {
-            const uint32_t id = p.recent[(size_t)blockIdx.x * p.recent_count + i];
-            if (id < n) atomicOr(&sh.seen[id / 32], 1u << (id % 32));
-        }
-        __syncthreads();
-    }
-    auto logit = [&](uint32_t i) {
-        const float v = x[i], r = p.o.repeat_penalty;
-        if (!p.recent || !(sh.seen[i / 32] >> (i % 32) & 1u)) return v;
-        return v < 0.f ? v * r : v / r;
+__global__ void __launch_bounds__(kThreads) draw_finish_kernel(SampleRows p) {
+    __shared__ Finish f;
+    const uint32_t row = blockIdx.x, n = p.vocab, tid = threadIdx.x;
+    const float *x = p.x + row * p.stride;
+    auto answer = [&](uint32_t id) {
+        if (tid == 0) p.out[row] = id;
     };
-    const uint32_t top_k = p.o.top_k == 0 ? n : min(p.o.top_k, n);
-    const bool limited = top_k < n, sorted = p.o.top_p < 1.f;
-    unsigned long long before;
-    auto by_raw = [&](uint32_t i) { return Key{{ordered(raw(i)), ~i, 0}}; };
-    Key last{};
-    if (limited) last = reach(sh, n, top_k, &before, by_raw, [&](uint32_t) { return 1ull; });
-    auto in = [&](uint32_t i) { return !limited || at_least(by_raw(i), last); };
-    auto by_logit = [&](uint32_t i) { return Key{{ordered(logit(i)), limited ? ordered(raw(i)) : 0u, ~i}}; };
-    const Key best = largest(sh, n, [&](uint32_t i) { return in(i) ? by_logit(i) : Key{}; });
-    const float mx = logit(~best.w[2]);
-    if (!(fabsf(mx) < INFINITY)) {
-        if (threadIdx.x == 0) p.out[blockIdx.x] = ~best.w[2];
+    if (p.o.temperature <= 0.f) return answer(~largest(f, n, [&](uint32_t i) { return Key{{ordered(x[i]), ~i, 0}}; }).w[1]);
+    const Policy policy(p);
+    const RowWork w = row_work(p, row);
+    if (p.recent) mark_recent(p, row, f.seen, (n + 31) / 32, 0);
+    auto logit_of = [&](uint32_t i, float v) {
+        return p.recent && (f.seen[i / 32] >> (i % 32) & 1u) ? penalised(v, p.o.repeat_penalty) : v;
+    };
+    auto logit = [&](uint32_t i) { return logit_of(i, x[i]); };
+    const double given = p.uniforms[row], u = given >= 0.0 ? fmin(given, 1.0) : 0.0;
+    const float top = w.head->max, per_bin = w.head->per_bin;
+    if (!(fabsf(top) < INFINITY))  // no largest number: the first of the largest logits
+        return answer(~largest(f, n, [&](uint32_t i) { return Key{{ordered(x[i]), ~i, 0}}; }).w[1]);
+
+    // the bins' sums over the slices, the largest logits' first
+    const uint32_t slices = slices_of(n);
+    u64 total, before;
+    auto sum_bins = [&]() {
+        u64 v = 0;
+        for (uint32_t s = tid / kBins; s < slices; s += kThreads / kBins) v += w.sums[s * kBins + tid % kBins];
+        __syncthreads();
+        f.sums[tid] = v;
+        __syncthreads();
+        return tid < kBins ? f.sums[tid] + f.sums[tid + kBins] + f.sums[tid + 2 * kBins] + f.sums[tid + 3 * kBins] : 0ull;
+    };
+
+    if (policy.limited) {
+        auto by_raw = [&](uint32_t i) { return Key{{ordered(x[i]), ~i, 0}}; };
+        const u64 c = sum_bins(), run = prefix(f, c, &total);
+        const uint32_t k = (uint32_t)(total < policy.top_k ? total : policy.top_k);  // candidates above -infinity
+        const uint32_t last = first_reaching(f, run, c, k, &before);
+        __syncthreads();
+        if (tid == 0) f.count = 0;
+        __syncthreads();
+        of_bins(w.bin, n, [&](uint32_t b) { return b <= last; }, [&](uint32_t i) {
+            const float v = x[i];
+            if (!(v > -INFINITY)) return;
+            const uint32_t at = atomicAdd(&f.count, 1u);
+            if (at < kList) f.list[at] = (u64)ordered(v) << 32 | (uint32_t)~i;
+        });
+        __syncthreads();
+        uint32_t m = f.count;
+        __syncthreads();
+        if (m > kList) {  // thousands of logits about the k-th: the k-th by its digits, then those down to it
+            const Key end = reach(f, n, k, &before, by_raw, [&](uint32_t i) { return x[i] > -INFINITY ? 1ull : 0ull; });
+            __syncthreads();
+            if (tid == 0) f.count = 0;
+            __syncthreads();
+            for (uint32_t i = tid; i < n; i += kThreads)
+                if (x[i] > -INFINITY && at_least(by_raw(i), end)) f.list[atomicAdd(&f.count, 1u)] = (u64)ordered(x[i]) << 32 | (uint32_t)~i;
+            __syncthreads();
+            m = k;
+        }
+        sort_list(f, m);
+        // this thread's candidate: rank tid in the order of the logits
+        u64 mine = tid < k ? f.list[tid] : 0;
+        const uint32_t id = ~(uint32_t)mine;
+        const float a = tid < k ? logit_of(id, unordered((uint32_t)(mine >> 32))) : -INFINITY;
+        const Key best = largest(f, kThreads, [&](uint32_t) { return tid < k ? Key{{ordered(a), (uint32_t)(mine >> 32), ~id}} : Key{}; });
+        const float mx = unordered(best.w[0]);
+        if (!(fabsf(mx) < INFINITY)) return answer(~best.w[2]);
+        float b = a;
+        uint32_t token = id;
+        if (policy.sorted && p.recent) {  // by weight: the penalised logits, ties as they stand
+            __syncthreads();
+            uint32_t *ids = reinterpret_cast<uint32_t *>(f.sums);
+            ids[tid] = id;
+            f.list[tid] = tid < k ? (u64)ordered(a) << 32 | (uint32_t)~tid : 0;
+            sort_list(f, k);
+            mine = tid < k ? f.list[tid] : 0;
+            b = tid < k ? unordered((uint32_t)(mine >> 32)) : -INFINITY;
+            token = tid < k ? ids[~(uint32_t)mine] : 0;
+        }
+        const u64 v = policy.weight(b, mx), sum = prefix(f, v, &total);
+        if (policy.sorted) {
+            const uint32_t end = first_reaching(f, sum, v, target_of((double)p.o.top_p, total), &before);
+            __syncthreads();
+            if (tid == end) f.value = sum;
+            __syncthreads();
+            total = f.value;
+        }
+        const uint32_t at = first_reaching(f, sum, v, target_of(u, total), &before);
+        if (tid == at) p.out[row] = token;
         return;
     }
-    int bits = 0;
-    while ((1u << bits) < top_k) bits++;
-    const double unit = ldexp(1.0, 62 - bits), t = (double)p.o.temperature, least = (double)p.o.min_p;
-    unsigned long long total = 0;
-    for (uint32_t i = threadIdx.x; i < n; i += kThreads) {
-        const float a = logit(i);
-        unsigned long long v = 0;
-        if (a > -INFINITY && in(i)) {
-            const double e = exp(((double)a - (double)mx) / t);
-            if (e >= least) v = (unsigned long long)rint(e * unit);
+
+    if (!policy.sorted) {  // in the order of the ids: the slice, then the logit
+        const u64 s = tid < slices ? w.whole[tid] : 0, run = prefix(f, s, &total), target = target_of(u, total);
+        const uint32_t slice = first_reaching(f, run, s, target, &before);
+        u64 v[2];
+#pragma unroll
+        for (int j = 0; j < 2; j++) {
+            const uint32_t i = slice * kSliceLogits + 2 * tid + j;
+            v[j] = i < n ? policy.weight(logit(i), top) : 0;
         }
-        w[i] = v;
-        total += v;
+        const u64 pair = prefix(f, v[0] + v[1], &total);
+        u64 ahead;
+        const uint32_t at = first_reaching(f, pair, v[0] + v[1], target - before, &ahead);
+        if (tid == at) p.out[row] = slice * kSliceLogits + 2 * tid + (v[0] && ahead + v[0] >= target - before ? 0u : 1u);
+        return;
     }
-    total = block_sum(sh, total);
-    auto weight = [&](uint32_t i) { return w[i]; };
-    if (sorted) {
-        const Key end = reach(sh, n, target_of((double)p.o.top_p, total), &before, by_logit, weight);
-        total = before + w[~end.w[2]];
+
+    const u64 c = sum_bins(), run = prefix(f, c, &total);
+    auto by_logit = [&](uint32_t i) { return Key{{ordered(logit(i)), ~i, 0}}; };
+    // The logit at which the sum reaches target, as its key (value, then lowest id); *upto: the sum with it.
+    auto find = [&](u64 target, u64 *upto) {
+        u64 ahead, fine_ahead, all;
+        const int bin = (int)first_reaching(f, run, c, target, &ahead);
         __syncthreads();
-        for (uint32_t i = threadIdx.x; i < n; i += kThreads)
-            if (!at_least(by_logit(i), end)) w[i] = 0;
+        f.sums[tid] = 0;
         __syncthreads();
-    }
-    const double given = p.uniforms[blockIdx.x], u = given >= 0.0 ? fmin(given, 1.0) : 0.0;
-    const unsigned long long target = target_of(u, total);
-    uint32_t id;
-    if (sorted) id = ~reach(sh, n, target, &before, by_logit, weight).w[2];
-    else if (limited) id = ~reach(sh, n, target, &before, by_raw, weight).w[1];
-    else id = ~reach(sh, n, target, &before, [&](uint32_t i) { return Key{{~i, 0, 0}}; }, weight).w[0];
-    if (threadIdx.x == 0) p.out[blockIdx.x] = id;
+        of_bins(w.bin, n, [&](uint32_t b) { return b == (uint32_t)bin; }, [&](uint32_t i) {
+            const float a = logit(i);
+            float t;
+            bin_of(a, top, per_bin, t);
+            const u64 v = policy.weight(a, top);
+            if (v) atomicAdd(&f.sums[fine_of(t, bin)], v);
+        });
+        __syncthreads();
+        const u64 v = f.sums[tid], r = prefix(f, v, &all);
+        const int fine = (int)first_reaching(f, r, v, target - ahead, &fine_ahead);
+        __syncthreads();
+        if (tid == 0) f.count = 0;
+        __syncthreads();
+        of_bins(w.bin, n, [&](uint32_t b) { return b == (uint32_t)bin; }, [&](uint32_t i) {
+            const float a = logit(i);
+            float t;
+            bin_of(a, top, per_bin, t);
+            if (fine_of(t, bin) != fine || !policy.weight(a, top)) return;
+            const uint32_t at = atomicAdd(&f.count, 1u);
+            if (at < kThreads) f.list[at] = (u64)ordered(a) << 32 | (uint32_t)~i;
+        });
+        __syncthreads();
+        const uint32_t m = f.count;
+        __syncthreads();
+        if (m > kThreads) {
+            u64 b;
+            const Key k = reach(f, n, target, &b, by_logit, [&](uint32_t i) { return policy.weight(logit(i), top); });
+            *upto = b + policy.weight(unordered(k.w[0]), top);
+            return (u64)k.w[0] << 32 | k.w[1];
+        }
+        sort_list(f, m);
+        const u64 mine = tid < m ? f.list[tid] : 0;
+        const u64 wt = tid < m ? policy.weight(unordered((uint32_t)(mine >> 32)), top) : 0;
+        const u64 rr = prefix(f, wt, &all);
+        u64 last;
+        const uint32_t at = first_reaching(f, rr, wt, target - ahead - fine_ahead, &last);
+        const u64 key = f.list[at];
+        *upto = ahead + fine_ahead + last + policy.weight(unordered((uint32_t)(key >> 32)), top);
+        __syncthreads();
+        return key;
+    };
+    u64 upto;
+    find(target_of((double)p.o.top_p, total), &upto);
+    const u64 key = find(target_of(u, upto), &upto);
+    answer(~(uint32_t)key);
 }
 
 }  // namespace
 
-size_t sample_rows_bytes(uint32_t vocab) { return ((size_t)vocab * 8 + 255) / 256 * 256; }
+size_t sample_rows_bytes(uint32_t vocab) { return up256(row_bytes(vocab)); }
 
 hipError_t launch_sample_rows(const SampleRows &p, hipStream_t s) {
-    hipLaunchKernelGGL(draw_simple_kernel, dim3(p.rows), dim3(kThreads), 0, s, p, (unsigned long long *)p.work,
-                       sample_rows_bytes(p.vocab) / 8);
+    if (p.o.temperature > 0.f) {
+        const dim3 grid(slices_of(p.vocab), p.rows);
+        hipLaunchKernelGGL(draw_stats_kernel, grid, dim3(256), 0, s, p);
+        hipLaunchKernelGGL(draw_bins_kernel, grid, dim3(256), 0, s, p);
+    }
+    hipLaunchKernelGGL(draw_finish_kernel, dim3(p.rows), dim3(kThreads), 0, s, p);
     return hipGetLastError();
 }
 

@@ -10,6 +10,7 @@ namespace zh {
 namespace {
 
 constexpr int kPairs = 4;  // pairs of a thread: two float4 of every head it takes
+constexpr int kBatch = 3;  // heads whose loads go out together
 
 __device__ __forceinline__ double turns_per_position(const RopeRows &p, int i) {
     double f = exp2((double)i * p.freq.exponent) * 0.15915494309189533577;
@@ -40,6 +41,41 @@ template <bool ALIGNED> __global__ void __launch_bounds__(256) rope_rows_kernel(
                 c[j] *= p.magnitude, s[j] *= p.magnitude;
             }
         }
+        if constexpr (ALIGNED) {
+            // this thread's two float4: the pairs' (interleaved: side by side), or what is copied
+            const int a0 = rotates && !p.style ? 2 * i0 : i0, a1 = rotates && p.style ? i0 + half : a0 + 4;
+            const bool two = rotates || n > 4;
+            for (int h = blockIdx.y * hp + h0; h < p.heads; h += kBatch * gridDim.y * hp) {
+                float4 x[kBatch], y[kBatch];
+#pragma unroll
+                for (int j = 0; j < kBatch; j++) {
+                    const float *at = src + (size_t)min(h + j * (int)gridDim.y * hp, p.heads - 1) * p.hd;
+                    x[j] = *reinterpret_cast<const float4 *>(at + a0);
+                    y[j] = *reinterpret_cast<const float4 *>(at + (two ? a1 : a0));
+                }
+#pragma unroll
+                for (int j = 0; j < kBatch; j++) {
+                    const int g = h + j * (int)gridDim.y * hp;
+                    if (g >= p.heads) break;
+                    float *at = dst + (size_t)g * p.hd;
+                    float4 u = x[j], v = y[j];
+                    if (rotates && p.style) {
+                        u = make_float4(x[j].x * c[0] - y[j].x * s[0], x[j].y * c[1] - y[j].y * s[1],
+                                        x[j].z * c[2] - y[j].z * s[2], x[j].w * c[3] - y[j].w * s[3]);
+                        v = make_float4(x[j].x * s[0] + y[j].x * c[0], x[j].y * s[1] + y[j].y * c[1],
+                                        x[j].z * s[2] + y[j].z * c[2], x[j].w * s[3] + y[j].w * c[3]);
+                    } else if (rotates) {
+                        u = make_float4(x[j].x * c[0] - x[j].y * s[0], x[j].x * s[0] + x[j].y * c[0],
+                                        x[j].z * c[1] - x[j].w * s[1], x[j].z * s[1] + x[j].w * c[1]);
+                        v = make_float4(y[j].x * c[2] - y[j].y * s[2], y[j].x * s[2] + y[j].y * c[2],
+                                        y[j].z * c[3] - y[j].w * s[3], y[j].z * s[3] + y[j].w * c[3]);
+                    }
+                    *reinterpret_cast<float4 *>(at + a0) = u;
+                    if (two) *reinterpret_cast<float4 *>(at + a1) = v;
+                }
+            }
+            continue;
+        }
         for (int h = blockIdx.y * hp + h0; h < p.heads; h += gridDim.y * hp) {
             const float *x = src + (size_t)h * p.hd;
             float *y = dst + (size_t)h * p.hd;
@@ -61,9 +97,15 @@ template <bool ALIGNED> __global__ void __launch_bounds__(256) rope_rows_kernel(
 
 hipError_t launch_rope_rows(const RopeRows &p, int cus, hipStream_t s) {
     const int units = (p.rd / 2 + kPairs - 1) / kPairs + (p.hd - p.rd + 7) / 8, hp = 256 / units;
-    const int passes = (p.heads + hp - 1) / hp;
-    const dim3 grid(p.rows < 65536u ? p.rows : 65536u, passes);
-    hipLaunchKernelGGL(rope_rows_kernel<false>, grid, dim3(256), 0, s, p, units, hp);
+    // few rows: their heads over workgroups; many: a workgroup takes every head of several rows, whose
+    // frequencies it computes once
+    const uint32_t passes = (uint32_t)(p.heads + hp - 1) / hp, want = 8u * (uint32_t)cus;
+    const uint32_t spread = want / p.rows < 1 ? 1 : want / p.rows, gy = passes < spread ? passes : spread;
+    const dim3 grid(p.rows < want / gy ? p.rows : want / gy, gy);
+    if (p.aligned && p.hd % 4 == 0 && p.rd % 8 == 0)
+        hipLaunchKernelGGL(rope_rows_kernel<true>, grid, dim3(256), 0, s, p, units, hp);
+    else
+        hipLaunchKernelGGL(rope_rows_kernel<false>, grid, dim3(256), 0, s, p, units, hp);
     return hipGetLastError();
 }
 

@@ -22,6 +22,7 @@ typedef _Float16 kh8 __attribute__((ext_vector_type(8)));
 typedef float kf4 __attribute__((ext_vector_type(4)));
 typedef float kf16 __attribute__((ext_vector_type(16)));
 
+constexpr int kMaxSplits = 64;  // one a lane when they are joined
 constexpr float kWeight = 16384.f;  // of the largest weight: its pieces below binary16's 65504
 
 __device__ __forceinline__ uint32_t first_seen(uint32_t pos, uint32_t window) {
@@ -97,33 +98,6 @@ __global__ void __launch_bounds__(256, PER_CU) kv8_few_kernel(Kv8Params p) {
     const uint32_t b1 = b_first + (uint32_t)((uint64_t)nb_all * (z + 1) / p.splits);
     const int nb = (int)(b1 - b0) > wave ? (int)((b1 - b0 - wave + 3) / 4) : 0;  // of this wavefront: b0 + wave + 4 t
 
-    // this lane's column: a row, and for NR 8 a piece of it
-    const uint32_t row = min(r0 + (uint32_t)(NR == 8 ? i16 >> 1 : i16), rlast);
-    const uint32_t qi = row / p.group, pos = p.position + qi, lo = first_seen(pos, p.window);
-    const int head = kvh * p.group + (int)(row % p.group);
-    const float *q = p.q + (size_t)qi * p.q_stride + (size_t)head * HD;
-    // dim of value e of step s: byte 8 s + e of a lane's row
-    auto dim_of = [&](int s, int e) { return 4 * F::KB * (8 * s / F::KB) + F::KB * g + 8 * s % F::KB + e; };
-    kh8 qb[P][F::KS];
-    float down;
-    {
-        float x[F::KS][8], top = 0.f, up;
-#pragma unroll
-        for (int s = 0; s < F::KS; s++)
-#pragma unroll
-            for (int e = 0; e < 8; e++) x[s][e] = q[dim_of(s, e)] * p.qscale, top = fmaxf(top, fabsf(x[s][e]));
-        top = xmax<32>(xmax<16>(top));
-        row_power(top, up, down);
-#pragma unroll
-        for (int s = 0; s < F::KS; s++)
-#pragma unroll
-            for (int e = 0; e < 8; e++) {
-                const float v = x[s][e] * up;
-                const _Float16 h = (_Float16)v, l = (_Float16)(v - (float)h);
-                if constexpr (NR == 8) qb[0][s][e] = i16 & 1 ? l : h;
-                else qb[0][s][e] = h, qb[1][s][e] = l;
-            }
-    }
     const size_t head0 = (size_t)kvh * p.c.blocks;
     const int8_t *kl = p.c.kc + head0 * (kKv8Block * HD) + (size_t)(8 * (i16 >> 2) + (i16 & 3)) * HD + F::KB * g;
     const int8_t *vl = p.c.vc + head0 * (kKv8Block * HD) + (size_t)i16 * kKv8Block + 8 * g;
@@ -143,6 +117,46 @@ __global__ void __launch_bounds__(256, PER_CU) kv8_few_kernel(Kv8Params p) {
         const uint32_t b = block_of(t + lane);
         ksl = p.c.ks[head0 + b], vsl = p.c.vs[head0 + b];
     };
+    // the queries' loads go first, K and V right behind them: all are under way while the queries are cut
+    Block8<HD> x, y;
+
+    // this lane's column: a row, and for NR 8 a piece of it
+    const uint32_t row = min(r0 + (uint32_t)(NR == 8 ? i16 >> 1 : i16), rlast);
+    const uint32_t qi = row / p.group, pos = p.position + qi, lo = first_seen(pos, p.window);
+    const int head = kvh * p.group + (int)(row % p.group);
+    const float *q = p.q + (size_t)qi * p.q_stride + (size_t)head * HD;
+    // dim of value e of step s: byte 8 s + e of a lane's row
+    auto dim_of = [&](int s, int e) { return 4 * F::KB * (8 * s / F::KB) + F::KB * g + 8 * s % F::KB + e; };
+    kh8 qb[P][F::KS];
+    float down;
+    {
+        float qv[F::KS][8], top = 0.f, up;
+#pragma unroll
+        for (int s = 0; s < F::KS; s++)
+#pragma unroll
+            for (int e = 0; e < 8; e++) qv[s][e] = q[dim_of(s, e)];
+        if (nb > 0) {
+            load_scales(0);
+            load(x, 0);
+            load(y, 1);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int s = 0; s < F::KS; s++)
+#pragma unroll
+            for (int e = 0; e < 8; e++) qv[s][e] *= p.qscale, top = fmaxf(top, fabsf(qv[s][e]));
+        top = xmax<32>(xmax<16>(top));
+        row_power(top, up, down);
+#pragma unroll
+        for (int s = 0; s < F::KS; s++)
+#pragma unroll
+            for (int e = 0; e < 8; e++) {
+                const float v = qv[s][e] * up;
+                const _Float16 h = (_Float16)v, l = (_Float16)(v - (float)h);
+                if constexpr (NR == 8) qb[0][s][e] = i16 & 1 ? l : h;
+                else qb[0][s][e] = h, qb[1][s][e] = l;
+            }
+    }
     kf4 o[F::DT];
 #pragma unroll
     for (int d = 0; d < F::DT; d++) o[d] = kf4{0.f, 0.f, 0.f, 0.f};
@@ -222,10 +236,6 @@ __global__ void __launch_bounds__(256, PER_CU) kv8_few_kernel(Kv8Params p) {
     };
 
     if (nb > 0) {
-        Block8<HD> x, y;
-        load_scales(0);
-        load(x, 0);
-        load(y, 1);
         for (int t = 0; t < nb; t += 2) {
             if (t && (t & 63) == 0) load_scales(t);
             compute(x, t);
@@ -375,6 +385,7 @@ template <int HD> __global__ void __launch_bounds__(256, kManyPerCu<HD>) kv8_man
     float m = -INFINITY, l = 0.f;
     if (t0 < t1) put(t0);
     __syncthreads();
+    const bool rows_here = wave * 32 < (qlast - q0 + 1) * p.group;  // else the wavefront only fills LDS
     big = fmaxf(fmaxf(top_scale[0], top_scale[1]), fmaxf(top_scale[2], top_scale[3]));
     const int krow = (l32 & 0x13) | (l32 & 4) << 1 | (l32 & 8) >> 1;
 
@@ -383,89 +394,91 @@ template <int HD> __global__ void __launch_bounds__(256, kManyPerCu<HD>) kv8_man
         const float kscale[2] = {p.c.ks[head0 + ba], p.c.ks[head0 + bb]}, vscale[2] = {p.c.vs[head0 + ba], p.c.vs[head0 + bb]};
         if (t + 1 < t1) load(t + 1);
         __builtin_amdgcn_sched_barrier(0);
-        const char *ks = lds + (t & 1) * BUF + krow * KST + 16 * lh, *vs = lds + (t & 1) * BUF + 64 * KST + l32 * VST + 16 * lh;
-        kf16 s[2];
+        if (rows_here) {
+            const char *ks = lds + (t & 1) * BUF + krow * KST + 16 * lh, *vs = lds + (t & 1) * BUF + 64 * KST + l32 * VST + 16 * lh;
+            kf16 s[2];
 #pragma unroll
-        for (int pt = 0; pt < 2; pt++) {
+            for (int pt = 0; pt < 2; pt++) {
 #pragma unroll
-            for (int r = 0; r < 16; r++) s[pt][r] = 0.f;
+                for (int r = 0; r < 16; r++) s[pt][r] = 0.f;
 #pragma unroll
-            for (int k = 0; k < KT; k++) {
-                const kh8 a = *reinterpret_cast<const kh8 *>(ks + pt * 32 * KST + 32 * k);
-                s[pt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, qh[k], s[pt], 0, 0, 0);
-                s[pt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, ql[k], s[pt], 0, 0, 0);
-            }
-        }
-        const bool edge = 64 * (uint32_t)t + 63 > wave_first || 64 * (uint32_t)t < wave_lo;
-        uint32_t keep = 0xFFFFFFFFu;
-        if (edge) {
-            keep = 0;
-#pragma unroll
-            for (int pt = 0; pt < 2; pt++)
-#pragma unroll
-                for (int r = 0; r < 16; r++) {
-                    const uint32_t at = 64 * (uint32_t)t + 32 * pt + 16 * (r >> 3) + 8 * lh + (r & 7);
-                    const bool in = at >= qlo && at <= qpos;
-                    keep |= (uint32_t)in << (16 * pt + r);
-                    if (!in) s[pt][r] = -INFINITY;
-                }
-        }
-        float f[2], lv[2], mx = -INFINITY;
-#pragma unroll
-        for (int pt = 0; pt < 2; pt++) {
-            f[pt] = kscale[pt] * down;
-            const float share = vscale[pt] / big;
-            lv[pt] = big > 0.f ? __builtin_amdgcn_logf(share < 0x1p-60f ? 0x1p-60f : share) : 0.f * vscale[pt];
-            float a = s[pt][0];
-#pragma unroll
-            for (int r = 1; r < 16; r++) a = fmaxf(a, s[pt][r]);
-            mx = fmaxf(mx, fmaf(a, f[pt], lv[pt]));
-        }
-        mx = xmax<32>(mx);
-        if (__any(mx > m)) {
-            const float mn = fmaxf(m, mx), al = __builtin_amdgcn_exp2f(m - finite(mn));
-            m = mn;
-            l *= al;
-#pragma unroll
-            for (int d = 0; d < DT; d++)
-#pragma unroll
-                for (int r = 0; r < 16; r++) o[d][r] *= al;
-        }
-        const float mf = finite(m);
-#pragma unroll
-        for (int pt = 0; pt < 2; pt++) {
-            const float c = lv[pt] - mf;
-            float sum = 0.f;
-#pragma unroll
-            for (int r = 0; r < 16; r++) s[pt][r] = __builtin_amdgcn_exp2f(fmaf(s[pt][r], f[pt], c));
-            if (edge)
-#pragma unroll
-                for (int r = 0; r < 16; r++)
-                    if (!(keep >> (16 * pt + r) & 1u)) s[pt][r] = 0.f;
-            uint32_t hi[8], lo[8];
-#pragma unroll
-            for (int i = 0; i < 8; i++) {
-                const float a = s[pt][2 * i], b = s[pt][2 * i + 1];
-                sum += a + b;
-                const kh2 h = kh2{(_Float16)a, (_Float16)b} * (_Float16)kWeight;  // (exact)
-                const kh2 w = {(_Float16)fmaf(a, kWeight, -(float)h[0]), (_Float16)fmaf(b, kWeight, -(float)h[1])};
-                hi[i] = __builtin_bit_cast(uint32_t, h);
-                lo[i] = __builtin_bit_cast(uint32_t, w);
-            }
-            // (a row with none of the block in sight takes nothing from it, whatever its scale)
-            l += sum == 0.f ? 0.f : sum * __builtin_amdgcn_exp2f(-lv[pt]);
-#pragma unroll
-            for (int k = 0; k < 2; k++) {
-                const kh8 ph = __builtin_bit_cast(kh8, uint4{hi[4 * k], hi[4 * k + 1], hi[4 * k + 2], hi[4 * k + 3]}),
-                          pl = __builtin_bit_cast(kh8, uint4{lo[4 * k], lo[4 * k + 1], lo[4 * k + 2], lo[4 * k + 3]});
-#pragma unroll
-                for (int d = 0; d < DT; d++) {
-                    const kh8 a = *reinterpret_cast<const kh8 *>(vs + d * 32 * VST + pt * 64 + 32 * k);
-                    o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, ph, o[d], 0, 0, 0);
-                    o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, pl, o[d], 0, 0, 0);
+                for (int k = 0; k < KT; k++) {
+                    const kh8 a = *reinterpret_cast<const kh8 *>(ks + pt * 32 * KST + 32 * k);
+                    s[pt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, qh[k], s[pt], 0, 0, 0);
+                    s[pt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, ql[k], s[pt], 0, 0, 0);
                 }
             }
-            __builtin_amdgcn_sched_barrier(0);
+            const bool edge = 64 * (uint32_t)t + 63 > wave_first || 64 * (uint32_t)t < wave_lo;
+            uint32_t keep = 0xFFFFFFFFu;
+            if (edge) {
+                keep = 0;
+#pragma unroll
+                for (int pt = 0; pt < 2; pt++)
+#pragma unroll
+                    for (int r = 0; r < 16; r++) {
+                        const uint32_t at = 64 * (uint32_t)t + 32 * pt + 16 * (r >> 3) + 8 * lh + (r & 7);
+                        const bool in = at >= qlo && at <= qpos;
+                        keep |= (uint32_t)in << (16 * pt + r);
+                        if (!in) s[pt][r] = -INFINITY;
+                    }
+            }
+            float f[2], lv[2], mx = -INFINITY;
+#pragma unroll
+            for (int pt = 0; pt < 2; pt++) {
+                f[pt] = kscale[pt] * down;
+                const float share = vscale[pt] / big;
+                lv[pt] = big > 0.f ? __builtin_amdgcn_logf(share < 0x1p-60f ? 0x1p-60f : share) : 0.f * vscale[pt];
+                float a = s[pt][0];
+#pragma unroll
+                for (int r = 1; r < 16; r++) a = fmaxf(a, s[pt][r]);
+                mx = fmaxf(mx, fmaf(a, f[pt], lv[pt]));
+            }
+            mx = xmax<32>(mx);
+            if (__any(mx > m)) {
+                const float mn = fmaxf(m, mx), al = __builtin_amdgcn_exp2f(m - finite(mn));
+                m = mn;
+                l *= al;
+#pragma unroll
+                for (int d = 0; d < DT; d++)
+#pragma unroll
+                    for (int r = 0; r < 16; r++) o[d][r] *= al;
+            }
+            const float mf = finite(m);
+#pragma unroll
+            for (int pt = 0; pt < 2; pt++) {
+                const float c = lv[pt] - mf;
+                float sum = 0.f;
+#pragma unroll
+                for (int r = 0; r < 16; r++) s[pt][r] = __builtin_amdgcn_exp2f(fmaf(s[pt][r], f[pt], c));
+                if (edge)
+#pragma unroll
+                    for (int r = 0; r < 16; r++)
+                        if (!(keep >> (16 * pt + r) & 1u)) s[pt][r] = 0.f;
+                uint32_t hi[8], lo[8];
+#pragma unroll
+                for (int i = 0; i < 8; i++) {
+                    const float a = s[pt][2 * i], b = s[pt][2 * i + 1];
+                    sum += a + b;
+                    const kh2 h = kh2{(_Float16)a, (_Float16)b} * (_Float16)kWeight;  // (exact)
+                    const kh2 w = {(_Float16)fmaf(a, kWeight, -(float)h[0]), (_Float16)fmaf(b, kWeight, -(float)h[1])};
+                    hi[i] = __builtin_bit_cast(uint32_t, h);
+                    lo[i] = __builtin_bit_cast(uint32_t, w);
+                }
+                // (a row with none of the block in sight takes nothing from it, whatever its scale)
+                l += sum == 0.f ? 0.f : sum * __builtin_amdgcn_exp2f(-lv[pt]);
+#pragma unroll
+                for (int k = 0; k < 2; k++) {
+                    const kh8 ph = __builtin_bit_cast(kh8, uint4{hi[4 * k], hi[4 * k + 1], hi[4 * k + 2], hi[4 * k + 3]}),
+                              pl = __builtin_bit_cast(kh8, uint4{lo[4 * k], lo[4 * k + 1], lo[4 * k + 2], lo[4 * k + 3]});
+#pragma unroll
+                    for (int d = 0; d < DT; d++) {
+                        const kh8 a = *reinterpret_cast<const kh8 *>(vs + d * 32 * VST + pt * 64 + 32 * k);
+                        o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, ph, o[d], 0, 0, 0);
+                        o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, pl, o[d], 0, 0, 0);
+                    }
+                }
+                __builtin_amdgcn_sched_barrier(0);
+            }
         }
         if (t + 1 < t1) put(t + 1);
         __syncthreads();
@@ -485,39 +498,40 @@ template <int HD> __global__ void __launch_bounds__(256, kManyPerCu<HD>) kv8_man
     if (p.splits > 1 && lh == 0) *reinterpret_cast<float2 *>(p.part_ml + 2 * at) = make_float2(m, l);
 }
 
-// The splits' partial results of a row joined in their order, a workgroup per row.
-template <int HD> __global__ void __launch_bounds__(256) kv8_join_kernel(const float *__restrict__ part, const float *__restrict__ ml,
+// The splits' partial results of a row joined in their order, a workgroup per row.  What a thread reads
+// goes out at once: the splits' maxima and sums a lane each, and its float4 of every N-th split.
+template <int HD> __global__ void __launch_bounds__(256) kv8_join_kernel(const float *__restrict__ part, const float2 *__restrict__ ml,
                                                                        float *__restrict__ out, size_t rows, int splits) {
-    constexpr int C = HD / 4, N = 256 / C;  // float4s of a row, splits read at a time
+    constexpr int C = HD / 4, N = 256 / C, Z = (kMaxSplits + N - 1) / N;  // float4s of a row; splits side by side; of a thread
     __shared__ float4 acc[N][C];
-    __shared__ float sums[N];
+    __shared__ float weight[kMaxSplits];
     const size_t row = blockIdx.x;
-    const int c = threadIdx.x % C, n = threadIdx.x / C;
-    float m = -INFINITY;
-    for (int z = 0; z < splits; z++) m = fmaxf(m, ml[2 * (z * rows + row)]);
-    const float mf = finite(m);
-    if (n < N) {
-        float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
-        float l = 0.f;
-        for (int z = n; z < splits; z += N) {
-            const size_t at = z * rows + row;
-            const float w = __builtin_amdgcn_exp2f(ml[2 * at] - mf) * ml[2 * at + 1];
-            const float4 v = *reinterpret_cast<const float4 *>(part + at * HD + 4 * c);
-            a.x = fmaf(w, v.x, a.x), a.y = fmaf(w, v.y, a.y), a.z = fmaf(w, v.z, a.z), a.w = fmaf(w, v.w, a.w);
-            l += w;
+    const int c = threadIdx.x % C, n = threadIdx.x / C, lane = threadIdx.x & 63;
+    const float2 own = ml[(size_t)min(lane, splits - 1) * rows + row];
+    float4 v[Z];
+#pragma unroll
+    for (int i = 0; i < Z; i++)
+        v[i] = *reinterpret_cast<const float4 *>(part + ((size_t)min(n + N * i, splits - 1) * rows + row) * HD + 4 * c);
+    const float m = finite(wave_max_f32(own.x));
+    float w = lane < splits ? __builtin_amdgcn_exp2f(own.x - m) * own.y : 0.f;
+    if (threadIdx.x < 64) weight[lane] = w;
+    for (int d = 1; d < 64; d <<= 1) w += __shfl_xor(w, d);
+    __syncthreads();
+    float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+    for (int i = 0; i < Z; i++)
+        if (n + N * i < splits) {
+            const float f = weight[n + N * i];
+            a.x = fmaf(f, v[i].x, a.x), a.y = fmaf(f, v[i].y, a.y), a.z = fmaf(f, v[i].z, a.z), a.w = fmaf(f, v[i].w, a.w);
         }
-        acc[n][c] = a;
-        if (c == 0) sums[n] = l;
-    }
+    if (n < N) acc[n][c] = a;
     __syncthreads();
     if (n) return;
-    float4 a = acc[0][c];
-    float l = sums[0];
     for (int k = 1; k < N; k++) {
-        const float4 v = acc[k][c];
-        a.x += v.x, a.y += v.y, a.z += v.z, a.w += v.w, l += sums[k];
+        const float4 o = acc[k][c];
+        a.x += o.x, a.y += o.y, a.z += o.z, a.w += o.w;
     }
-    *reinterpret_cast<float4 *>(out + row * HD + 4 * c) = make_float4(a.x / l, a.y / l, a.z / l, a.w / l);
+    *reinterpret_cast<float4 *>(out + row * HD + 4 * c) = make_float4(a.x / w, a.y / w, a.z / w, a.w / w);
 }
 
 }  // namespace
@@ -534,11 +548,11 @@ hipError_t launch_kv8_attention(const Kv8Attn &a, int cus, hipStream_t s) {
     if (wgs > 0x7FFFFFFFu) return hipErrorInvalidValue;
     // positions: of the query that sees the fewest
     const uint32_t seen = a.window && a.window <= a.position ? a.window : a.position + 1;
-    const uint64_t least = many ? 4 * 64 : 4 * kKv8Block, most = many ? 16 : 64;
+    const uint64_t least = many ? 4 * 64 : 4 * kKv8Block;
     const uint64_t total = (uint64_t)a.queries * a.heads;
     uint64_t splits = 2 * (uint64_t)cus / wgs;
     splits = splits < seen / least ? splits : seen / least;
-    splits = splits < most ? splits : most;
+    splits = splits < kMaxSplits ? splits : kMaxSplits;
     while (splits > 1 && splits * total * (a.c.hd + 2) > a.part_floats) splits--;
     p.splits = splits > 1 ? (int)splits : 1;
     p.part = a.part, p.part_ml = a.part + (size_t)p.splits * total * a.c.hd;
@@ -549,7 +563,7 @@ hipError_t launch_kv8_attention(const Kv8Attn &a, int cus, hipStream_t s) {
         else if (nr == 8) hipLaunchKernelGGL((kv8_few_kernel<HD, 8, PER_CU>), grid, dim3(256), 0, s, p);
         else hipLaunchKernelGGL((kv8_few_kernel<HD, 16, PER_CU>), grid, dim3(256), 0, s, p);
         if (p.splits > 1)
-            hipLaunchKernelGGL(kv8_join_kernel<HD>, dim3((unsigned)total), dim3(256), 0, s, p.part, p.part_ml, p.out,
+            hipLaunchKernelGGL(kv8_join_kernel<HD>, dim3((unsigned)total), dim3(256), 0, s, p.part, (const float2 *)p.part_ml, p.out,
                                (size_t)total, p.splits);
     };
     switch (a.c.hd) {

@@ -8,7 +8,7 @@
 // Three launches, none of which sorts the row:
 //   stats   slices of 2048 logits: maximum, minimum and mean, from which a linear scale of 256 bins
 //           is laid over the values, the largest in bin 0;
-//   bins    each logit's bin, and per slice the bins' sums of weights (top-k: counts);
+//   bins    per slice the bins' sums of weights (top-k: counts), and its logits in the order of their bins;
 //   finish  a workgroup per row: the bin in which a target lies, then 1024 finer bins of that bin's
 //           logits, then the few logits of the finer bin in order.  With top-k the bins above the k-th
 //           logit are sorted in LDS instead, and everything else is prefix sums of at most 1024.
@@ -36,14 +36,17 @@ struct SliceStats {
 __host__ __device__ constexpr size_t up256(size_t n) { return (n + 255) / 256 * 256; }
 __host__ __device__ constexpr uint32_t slices_of(uint32_t vocab) { return (vocab + kSliceLogits - 1) / kSliceLogits; }
 __host__ __device__ constexpr size_t row_bytes(uint32_t vocab) {
-    return 256 + up256(slices_of(vocab) * sizeof(SliceStats)) + slices_of(vocab) * (kBins + 1) * sizeof(u64) + up256(vocab) + 256;
+    return 256 + up256(slices_of(vocab) * sizeof(SliceStats)) +
+           slices_of(vocab) * (kBins * (sizeof(u64) + 4) + sizeof(u64) + kSliceLogits * (sizeof(float) + 2)) + 256;
 }
 struct RowWork {
     RowHead *head;
     SliceStats *stats;
-    u64 *sums;     // [slice][kBins]
-    u64 *whole;    // [slice]
-    uint8_t *bin;  // [vocab]
+    u64 *sums;       // [slice][kBins]
+    uint32_t *run;   // [slice][kBins]: where the bin's logits begin in the slice's order, and (high half) end
+    float *value;    // [slice][kSliceLogits], in the order of their bins
+    uint16_t *from;  // [slice][kSliceLogits]: of which logit of the slice
+    u64 *whole;      // [slice]
 };
 __device__ __forceinline__ RowWork row_work(const SampleRows &p, uint32_t row) {
     char *at = (char *)p.work + row * up256(row_bytes(p.vocab));
@@ -51,8 +54,10 @@ __device__ __forceinline__ RowWork row_work(const SampleRows &p, uint32_t row) {
     const uint32_t n = slices_of(p.vocab);
     w.head = (RowHead *)at, at += 256;
     w.stats = (SliceStats *)at, at += up256(n * sizeof(SliceStats));
-    w.bin = (uint8_t *)at, at += up256(p.vocab);
     w.sums = (u64 *)at, at += (size_t)n * kBins * sizeof(u64);
+    w.value = (float *)at, at += (size_t)n * kSliceLogits * sizeof(float);
+    w.run = (uint32_t *)at, at += (size_t)n * kBins * 4;
+    w.from = (uint16_t *)at, at += (size_t)n * kSliceLogits * 2;
     w.whole = (u64 *)at;
     return w;
 }
@@ -155,43 +160,71 @@ __global__ void __launch_bounds__(256) draw_bins_kernel(SampleRows p) {
     __shared__ uint32_t bits[kSliceLogits / 32];
     __shared__ float4 all[kMaxSlices];
     __shared__ u64 sums[kBins], red[4];
+    __shared__ uint32_t count[kBins], begin[kBins], wave_count[4];
+    __shared__ float value[kSliceLogits];
+    __shared__ uint16_t from[kSliceLogits];
     const uint32_t row = blockIdx.y, slices = slices_of(p.vocab);
     const RowWork w = row_work(p, row);
     const Policy policy(p);
     if (threadIdx.x < slices) all[threadIdx.x] = *reinterpret_cast<const float4 *>(w.stats + threadIdx.x);
-    sums[threadIdx.x] = 0;
+    sums[threadIdx.x] = 0, count[threadIdx.x] = 0;
     const Slice s(p, row, p.recent && !policy.limited, bits);
     __syncthreads();
-    float mx = -INFINITY, mn = INFINITY, sum = 0.f, count = 0.f;
+    float mx = -INFINITY, mn = INFINITY, sum = 0.f, known = 0.f;
     for (uint32_t i = threadIdx.x & 63; i < slices; i += 64)
-        mx = fmaxf(mx, all[i].x), mn = fminf(mn, all[i].y), sum += all[i].z, count += all[i].w;
+        mx = fmaxf(mx, all[i].x), mn = fminf(mn, all[i].y), sum += all[i].z, known += all[i].w;
     for (int d = 32; d; d >>= 1) {
         mx = fmaxf(mx, __shfl_xor(mx, d)), mn = fminf(mn, __shfl_xor(mn, d));
-        sum += __shfl_xor(sum, d), count += __shfl_xor(count, d);
+        sum += __shfl_xor(sum, d), known += __shfl_xor(known, d);
     }
     // the scale: with top-k down to the mean; else to the lowest, or to where weights are 0, or, where
     // few lie far below the others, as far below the mean as half again the largest is above it
-    const float above = mx - sum / count;
+    const float above = mx - sum / known;
     float range = policy.limited ? above : fminf(fminf(43.7f * p.o.temperature, mx - mn), 2.5f * above);
     const float per_bin = range > 0.f && fabsf(mx) < INFINITY ? (float)kBins / range : 0.f;
     if (blockIdx.x == 0 && threadIdx.x == 0) w.head->max = mx, w.head->per_bin = per_bin;
     u64 whole = 0;
+    uint32_t at[kSliceLogits / 256];  // bin, and the logit's place in it (in no order: their sums are exact)
 #pragma unroll
     for (int i = 0; i < kSliceLogits / 256; i++) {
-        const uint32_t j = threadIdx.x + 256 * i;
-        if (j >= s.n) continue;
         float t;
         const int b = bin_of(s.a[i], mx, per_bin, t);
-        w.bin[s.first + j] = (uint8_t)b;
         const u64 v = !(fabsf(mx) < INFINITY) ? 0ull : policy.limited ? (s.a[i] > -INFINITY ? 1ull : 0ull) : policy.weight(s.a[i], mx);
-        if (v) atomicAdd(&sums[b], v);
+        at[i] = 0xFFFFFFFFu;  // no candidate: in no bin
+        if (v) {
+            atomicAdd(&sums[b], v);
+            at[i] = (uint32_t)b << 16 | atomicAdd(&count[b], 1u);
+        }
         whole += v;
     }
     for (int d = 32; d; d >>= 1) whole += (u64)__shfl_xor((long long)whole, d);
     if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = whole;
     __syncthreads();
-    w.sums[blockIdx.x * kBins + threadIdx.x] = sums[threadIdx.x];
-    if (threadIdx.x == 0) w.whole[blockIdx.x] = red[0] + red[1] + red[2] + red[3];
+    const uint32_t mine = count[threadIdx.x];
+    uint32_t upto = mine;
+    for (int d = 1; d < 64; d <<= 1) {
+        const uint32_t o = (uint32_t)__shfl_up((int)upto, d);
+        if ((int)(threadIdx.x & 63) >= d) upto += o;
+    }
+    if ((threadIdx.x & 63) == 63) wave_count[threadIdx.x >> 6] = upto;
+    __syncthreads();
+    for (uint32_t k = 0; k < threadIdx.x >> 6; k++) upto += wave_count[k];
+    begin[threadIdx.x] = upto - mine;
+    const size_t slice = blockIdx.x;
+    w.run[slice * kBins + threadIdx.x] = (upto - mine) | upto << 16;
+    w.sums[slice * kBins + threadIdx.x] = sums[threadIdx.x];
+    if (threadIdx.x == 0) w.whole[slice] = red[0] + red[1] + red[2] + red[3];
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < kSliceLogits / 256; i++)
+        if (at[i] != 0xFFFFFFFFu) {
+            const uint32_t to = begin[at[i] >> 16] + (at[i] & 0xFFFFu);
+            value[to] = s.a[i], from[to] = (uint16_t)(threadIdx.x + 256 * i);
+        }
+    __syncthreads();
+    const uint32_t held = wave_count[0] + wave_count[1] + wave_count[2] + wave_count[3];
+    for (uint32_t i = threadIdx.x; i < held; i += 256)
+        w.value[slice * kSliceLogits + i] = value[i], w.from[slice * kSliceLogits + i] = from[i];
 }
 
 // ---- finish: a workgroup of 1024 per row ----
@@ -252,7 +285,17 @@ __device__ u64 target_of(double share, u64 total) {
 
 // f.list[0 .. n) in descending order (n at most kList; the places up to a power of two are filled).
 __device__ void sort_list(Finish &f, uint32_t n) {
-    uint32_t size = 2;
+    if (n <= 64) {  // a wavefront: each key's place is the count of larger ones (keys differ)
+        if (threadIdx.x < 64) {
+            const u64 k = threadIdx.x < n ? f.list[threadIdx.x] : 0;
+            uint32_t place = 0;
+            for (uint32_t i = 0; i < n; i++) place += f.list[i] > k;
+            if (threadIdx.x < n) f.list[place] = k;
+        }
+        __syncthreads();
+        return;
+    }
+    uint32_t size = 128;
     while (size < n) size <<= 1;
     for (uint32_t i = n + threadIdx.x; i < size; i += kThreads) f.list[i] = 0;
     __syncthreads();
@@ -318,16 +361,15 @@ template <class K> __device__ Key largest(Finish &f, uint32_t n, K key) {
     return k;
 }
 
-// Calls take(i) for the logits of the bins that `wanted` names.
-template <class B, class T> __device__ __forceinline__ void of_bins(const uint8_t *bin, uint32_t n, B wanted, T take) {
-    for (uint32_t at = 16 * threadIdx.x; at < n; at += 16 * kThreads) {
-        const uint4 v = *reinterpret_cast<const uint4 *>(bin + at);
-        const uint32_t word[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-        for (int j = 0; j < 16; j++)
-            if (wanted(word[j / 4] >> (8 * (j % 4)) & 255u) && at + j < n) take(at + j);
-    }
+// Calls take(logit, its id) for the row's logits of bins first .. last, 8 lanes a slice.
+template <class T> __device__ __forceinline__ void of_bins(const RowWork &w, uint32_t slices, uint32_t first, uint32_t last, T take) {
+    const size_t slice = threadIdx.x / 8;
+    if (slice >= slices) return;
+    const uint32_t begin = w.run[slice * kBins + first] & 0xFFFFu, end = w.run[slice * kBins + last] >> 16;
+    for (uint32_t e = begin + threadIdx.x % 8; e < end; e += 8)
+        take(w.value[slice * kSliceLogits + e], (uint32_t)slice * kSliceLogits + w.from[slice * kSliceLogits + e]);
 }
+static_assert(kThreads / 8 >= kMaxSlices, "8 lanes for every slice");
 
 __global__ void __launch_bounds__(kThreads) draw_finish_kernel(SampleRows p) {
     __shared__ Finish f;
@@ -339,6 +381,7 @@ __global__ void __launch_bounds__(kThreads) draw_finish_kernel(SampleRows p) {
     if (p.o.temperature <= 0.f) return answer(~largest(f, n, [&](uint32_t i) { return Key{{ordered(x[i]), ~i, 0}}; }).w[1]);
     const Policy policy(p);
     const RowWork w = row_work(p, row);
+    // (the bins hold penalised logits, but for top-k's)
     if (p.recent) mark_recent(p, row, f.seen, (n + 31) / 32, 0);
     auto logit_of = [&](uint32_t i, float v) {
         return p.recent && (f.seen[i / 32] >> (i % 32) & 1u) ? penalised(v, p.o.repeat_penalty) : v;
@@ -354,6 +397,7 @@ __global__ void __launch_bounds__(kThreads) draw_finish_kernel(SampleRows p) {
     u64 total, before;
     auto sum_bins = [&]() {
         u64 v = 0;
+#pragma unroll 8
         for (uint32_t s = tid / kBins; s < slices; s += kThreads / kBins) v += w.sums[s * kBins + tid % kBins];
         __syncthreads();
         f.sums[tid] = v;
@@ -369,9 +413,7 @@ __global__ void __launch_bounds__(kThreads) draw_finish_kernel(SampleRows p) {
         __syncthreads();
         if (tid == 0) f.count = 0;
         __syncthreads();
-        of_bins(w.bin, n, [&](uint32_t b) { return b <= last; }, [&](uint32_t i) {
-            const float v = x[i];
-            if (!(v > -INFINITY)) return;
+        of_bins(w, slices, 0, last, [&](float v, uint32_t i) {
             const uint32_t at = atomicAdd(&f.count, 1u);
             if (at < kList) f.list[at] = (u64)ordered(v) << 32 | (uint32_t)~i;
         });
@@ -446,12 +488,10 @@ __global__ void __launch_bounds__(kThreads) draw_finish_kernel(SampleRows p) {
         __syncthreads();
         f.sums[tid] = 0;
         __syncthreads();
-        of_bins(w.bin, n, [&](uint32_t b) { return b == (uint32_t)bin; }, [&](uint32_t i) {
-            const float a = logit(i);
+        of_bins(w, slices, bin, bin, [&](float a, uint32_t) {
             float t;
             bin_of(a, top, per_bin, t);
-            const u64 v = policy.weight(a, top);
-            if (v) atomicAdd(&f.sums[fine_of(t, bin)], v);
+            atomicAdd(&f.sums[fine_of(t, bin)], policy.weight(a, top));
         });
         __syncthreads();
         const u64 v = f.sums[tid], r = prefix(f, v, &all);
@@ -459,11 +499,10 @@ __global__ void __launch_bounds__(kThreads) draw_finish_kernel(SampleRows p) {
         __syncthreads();
         if (tid == 0) f.count = 0;
         __syncthreads();
-        of_bins(w.bin, n, [&](uint32_t b) { return b == (uint32_t)bin; }, [&](uint32_t i) {
-            const float a = logit(i);
+        of_bins(w, slices, bin, bin, [&](float a, uint32_t i) {
             float t;
             bin_of(a, top, per_bin, t);
-            if (fine_of(t, bin) != fine || !policy.weight(a, top)) return;
+            if (fine_of(t, bin) != fine) return;
             const uint32_t at = atomicAdd(&f.count, 1u);
             if (at < kThreads) f.list[at] = (u64)ordered(a) << 32 | (uint32_t)~i;
         });

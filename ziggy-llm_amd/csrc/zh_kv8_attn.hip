@@ -51,6 +51,16 @@ __device__ __forceinline__ void row_power(float largest, float &up, float &down)
     down = fine ? __uint_as_float((e - 14u) << 23) : 1.f;
 }
 
+// eight values of a query row, the row's start on 16 bytes or not
+__device__ __forceinline__ void load8(const float *q, int aligned, float (&v)[8]) {
+    if (aligned) {
+        const float4 a = *reinterpret_cast<const float4 *>(q), b = *reinterpret_cast<const float4 *>(q + 4);
+        v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
+    } else {
+        for (int e = 0; e < 8; e++) v[e] = q[e];
+    }
+}
+
 __device__ __forceinline__ float finite(float v) { return v == -INFINITY ? 0.f : v; }
 
 struct Kv8Params {
@@ -59,8 +69,7 @@ struct Kv8Params {
     size_t q_stride;
     float *out, *part, *part_ml;  // splits > 1: row r of split z at part + (z rows + r) hd, {max, sum} at part_ml + ...2
     uint32_t position, queries, window;
-    int heads, group, splits;
-    uint32_t row_groups;
+    int heads, group, splits, q_aligned;
     float qscale;
 };
 
@@ -125,16 +134,14 @@ __global__ void __launch_bounds__(256, PER_CU) kv8_few_kernel(Kv8Params p) {
     const uint32_t qi = row / p.group, pos = p.position + qi, lo = first_seen(pos, p.window);
     const int head = kvh * p.group + (int)(row % p.group);
     const float *q = p.q + (size_t)qi * p.q_stride + (size_t)head * HD;
-    // dim of value e of step s: byte 8 s + e of a lane's row
-    auto dim_of = [&](int s, int e) { return 4 * F::KB * (8 * s / F::KB) + F::KB * g + 8 * s % F::KB + e; };
+    // first dim of step s: byte 8 s of a lane's row
+    auto dim_of = [&](int s) { return 4 * F::KB * (8 * s / F::KB) + F::KB * g + 8 * s % F::KB; };
     kh8 qb[P][F::KS];
     float down;
     {
         float qv[F::KS][8], top = 0.f, up;
 #pragma unroll
-        for (int s = 0; s < F::KS; s++)
-#pragma unroll
-            for (int e = 0; e < 8; e++) qv[s][e] = q[dim_of(s, e)];
+        for (int s = 0; s < F::KS; s++) load8(q + dim_of(s), p.q_aligned, qv[s]);
         if (nb > 0) {
             load_scales(0);
             load(x, 0);
@@ -363,16 +370,20 @@ template <int HD> __global__ void __launch_bounds__(256, kManyPerCu<HD>) kv8_man
     float down;
     {
         const float *q = p.q + (size_t)qc * p.q_stride + (size_t)(kvh * p.group + (valid ? v % p.group : 0)) * HD + 8 * lh;
-        float top = 0.f, up;
+        float qv[KT][8], top = 0.f, up;
+#pragma unroll
+        for (int t = 0; t < KT; t++) load8(q + 16 * t, p.q_aligned, qv[t]);
+#pragma unroll
         for (int t = 0; t < KT; t++)
-            for (int e = 0; e < 8; e++) top = fmaxf(top, fabsf(q[16 * t + e] * p.qscale));
+#pragma unroll
+            for (int e = 0; e < 8; e++) qv[t][e] *= p.qscale, top = fmaxf(top, fabsf(qv[t][e]));
         top = xmax<32>(top);
         row_power(top, up, down);
 #pragma unroll
         for (int t = 0; t < KT; t++)
 #pragma unroll
             for (int e = 0; e < 8; e++) {
-                const float x = q[16 * t + e] * p.qscale * up;
+                const float x = qv[t][e] * up;
                 qh[t][e] = (_Float16)x;
                 ql[t][e] = (_Float16)(x - (float)qh[t][e]);
             }
@@ -541,6 +552,7 @@ hipError_t launch_kv8_attention(const Kv8Attn &a, int cus, hipStream_t s) {
     p.c = a.c, p.q = a.q, p.q_stride = a.q_stride, p.out = a.out;
     p.position = a.position, p.queries = a.queries, p.window = a.window;
     p.heads = a.heads, p.group = a.heads / a.c.nkv, p.qscale = a.qscale;
+    p.q_aligned = (uintptr_t)a.q % 16 == 0 && a.q_stride % 4 == 0;
     const uint64_t rows = (uint64_t)a.queries * p.group;  // of a kv head
     const bool many = rows > 32;
     const int nr = rows > 8 ? 16 : 8, qn = 128 / p.group;

@@ -10,6 +10,7 @@ from __future__ import annotations
 
 import ctypes
 import os
+import threading
 
 import numpy as np
 
@@ -277,11 +278,22 @@ def lib() -> ctypes.CDLL:
     return L
 
 
+_fns: dict = {}
+_thread = threading.local()  # a thread's error buffer
+
+
 def _call(fn_name: str, *args):
-    err = ctypes.create_string_buffer(ERR_LEN)
-    st = getattr(lib(), fn_name)(*args, err, ERR_LEN)
+    fn = _fns.get(fn_name)
+    if fn is None:
+        fn = _fns[fn_name] = getattr(lib(), fn_name)
+    err = getattr(_thread, "err", None)
+    if err is None:
+        err = _thread.err = ctypes.create_string_buffer(ERR_LEN)
+    st = fn(*args, err, ERR_LEN)
     if st:
-        raise HipError(st, err.value.decode(errors="replace"))
+        msg = err.value.decode(errors="replace")
+        err[0] = b"\0"
+        raise HipError(st, msg)
 
 
 class Buffer:

@@ -63,6 +63,24 @@ __device__ __forceinline__ void load8(const float *q, int aligned, float (&v)[8]
 
 __device__ __forceinline__ float finite(float v) { return v == -INFINITY ? 0.f : v; }
 
+// two weights' pieces
+__device__ __forceinline__ void pieces(float a, float b, uint32_t &hi, uint32_t &lo) {
+    const kh2 h = kh2{(_Float16)a, (_Float16)b} * (_Float16)kWeight;  // (exact)
+    const kh2 l = {(_Float16)fmaf(a, kWeight, -(float)h[0]), (_Float16)fmaf(b, kWeight, -(float)h[1])};
+    hi = __builtin_bit_cast(uint32_t, h), lo = __builtin_bit_cast(uint32_t, l);
+}
+
+// A block's V scale as a share of the largest: its log2 goes into the weights' exponent, w = 2^(s +
+// log2 share - max), and the weights over the share add to the sum.  Shares below 2^-60, an all-zero
+// block's among them, count as 2^-60: their values are below what the largest one's rounding leaves,
+// and the sum keeps their weight.  (A multiplication of a block's outputs instead would be an FMA per
+// output and block.)
+__device__ __forceinline__ void share_of(float scale, float big, float &log_share, float &inverse) {
+    const float share = scale / big;
+    log_share = big > 0.f ? __builtin_amdgcn_logf(share < 0x1p-60f ? 0x1p-60f : share) : 0.f * scale;
+    inverse = __builtin_amdgcn_exp2f(-log_share);
+}
+
 struct Kv8Params {
     Kv8Layer c;
     const float *q;
@@ -70,6 +88,8 @@ struct Kv8Params {
     float *out, *part, *part_ml;  // splits > 1: row r of split z at part + (z rows + r) hd, {max, sum} at part_ml + ...2
     uint32_t position, queries, window;
     int heads, group, splits, q_aligned;
+    uint32_t per_group;  // ceil(2^16 / group): rows / group of the few and of a workgroup (both below 128) by a product
+    __device__ __forceinline__ uint32_t query_of(uint32_t row) const { return row * per_group >> 16; }
     float qscale;
 };
 
@@ -79,28 +99,34 @@ struct Kv8Params {
 // 16x16x32 products, S[position][column] = K Q^T; lane (i, g) holds K row 8 (i / 4) + 4 pt + i % 4 of
 // its half pt, so that the 8 scores it gets back are of positions 8 g .. 8 g + 7, in order: what the
 // value products O[column][dim] = P V take as their left operand, and what its 8 bytes of a V dim
-// hold.  NR 8: 16 columns are the two pieces of 8 rows; NR 16: of 16 rows, each piece a product.
+// hold.  Up to 8 rows (NR 8): 16 columns are their two pieces.  More: CT tiles of 16 rows, each piece
+// a product, which share the blocks' loads and widening.
 template <int HD, int NR> struct Few {
+    static constexpr bool PAIRED = NR == 8;
+    static constexpr int CT = PAIRED ? 1 : NR / 16;    // column tiles
+    static constexpr int P = PAIRED ? 1 : 2;           // products of a step: both pieces in one, or one for each
     static constexpr int KS = HD / 32, DT = HD / 16;   // k-steps, dim tiles
     static constexpr int KB = HD % 64 ? 8 : 16;        // bytes of a lane's K load
     static constexpr int KL = HD / 4 / KB;             // K loads of a row
     static constexpr int KW = KB / 4;
+    static constexpr int PER_CU = NR <= 16 && HD <= 128 ? 2 : 1;  // workgroups whose registers a CU holds
 };
 template <int HD> struct Block8 {
     uint32_t k[2][HD / 16], v[HD / 16][2];
 };
 
-template <int HD, int NR, int PER_CU>
-__global__ void __launch_bounds__(256, PER_CU) kv8_few_kernel(Kv8Params p) {
+template <int HD, int NR>
+__global__ void __launch_bounds__(256, (Few<HD, NR>::PER_CU)) kv8_few_kernel(Kv8Params p) {
     using F = Few<HD, NR>;
-    constexpr int P = NR == 16 ? 2 : 1;  // products of a step: one for each piece, or both in one
-    __shared__ float os[4][NR][HD + 4], ms[4][NR], ls[4][NR];
+    constexpr int CT = F::CT, P = F::P;
+    __shared__ __align__(16) float os[4][NR][HD + 4];
+    __shared__ float ms[4][NR], ls[4][NR];
     const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, i16 = lane & 15, g = lane >> 4;
     const int kvh = blockIdx.x % p.c.nkv, z = blockIdx.y;
     const uint32_t rows = p.queries * (uint32_t)p.group, r0 = blockIdx.x / p.c.nkv * NR;
     const uint32_t rlast = min(r0 + NR, rows) - 1;
     // the blocks that any of the rows sees, and this split's share of them
-    const uint32_t pos_min = p.position + r0 / p.group, pos_max = p.position + rlast / p.group;
+    const uint32_t pos_min = p.position + p.query_of(r0), pos_max = p.position + p.query_of(rlast);
     const uint32_t lo_min = first_seen(pos_min, p.window), lo_max = first_seen(pos_max, p.window);
     const uint32_t b_first = lo_min / kKv8Block, nb_all = pos_max / kKv8Block - b_first + 1;
     const uint32_t b0 = b_first + (uint32_t)((uint64_t)nb_all * z / p.splits);
@@ -121,27 +147,31 @@ __global__ void __launch_bounds__(256, PER_CU) kv8_few_kernel(Kv8Params p) {
 #pragma unroll
         for (int d = 0; d < F::DT; d++) __builtin_memcpy(r.v[d], vl + at + d * (16 * kKv8Block), 8);
     };
-    float ksl = 0.f, vsl = 0.f;  // scales of the wavefront's next 64 blocks, one a lane
+    // of the wavefront's next 64 blocks, one a lane: the K scale, log2 of the V scale's share of `big` (the
+    // largest V scale so far), and the share's inverse
+    float ksl = 0.f, vsl = 0.f, lvl = 0.f, inl = 0.f, big = 0.f;
     auto load_scales = [&](int t) {
         const uint32_t b = block_of(t + lane);
         ksl = p.c.ks[head0 + b], vsl = p.c.vs[head0 + b];
     };
-    // the queries' loads go first, K and V right behind them: all are under way while the queries are cut
     Block8<HD> x, y;
 
-    // this lane's column: a row, and for NR 8 a piece of it
-    const uint32_t row = min(r0 + (uint32_t)(NR == 8 ? i16 >> 1 : i16), rlast);
-    const uint32_t qi = row / p.group, pos = p.position + qi, lo = first_seen(pos, p.window);
-    const int head = kvh * p.group + (int)(row % p.group);
-    const float *q = p.q + (size_t)qi * p.q_stride + (size_t)head * HD;
+    // this lane's column of tile c: a row, and of paired ones a piece of it
+    auto row_of = [&](int c, int column) { return min(r0 + (uint32_t)(F::PAIRED ? column >> 1 : 16 * c + column), rlast); };
     // first dim of step s: byte 8 s of a lane's row
     auto dim_of = [&](int s) { return 4 * F::KB * (8 * s / F::KB) + F::KB * g + 8 * s % F::KB; };
-    kh8 qb[P][F::KS];
-    float down;
+    kh8 qb[CT][P][F::KS];
+    float down[CT];
     {
-        float qv[F::KS][8], top = 0.f, up;
+        float qv[CT][F::KS][8];
 #pragma unroll
-        for (int s = 0; s < F::KS; s++) load8(q + dim_of(s), p.q_aligned, qv[s]);
+        for (int c = 0; c < CT; c++) {
+            const uint32_t row = row_of(c, i16), qi = p.query_of(row);
+            const float *q = p.q + (size_t)qi * p.q_stride + (size_t)(kvh * p.group + (int)(row - qi * p.group)) * HD;
+#pragma unroll
+            for (int s = 0; s < F::KS; s++) load8(q + dim_of(s), p.q_aligned, qv[c][s]);
+        }
+        // the queries' loads go first, K and V right behind them: all are under way while the queries are cut
         if (nb > 0) {
             load_scales(0);
             load(x, 0);
@@ -149,102 +179,140 @@ __global__ void __launch_bounds__(256, PER_CU) kv8_few_kernel(Kv8Params p) {
         }
         __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-        for (int s = 0; s < F::KS; s++)
+        for (int c = 0; c < CT; c++) {
+            float top = 0.f, up;
 #pragma unroll
-            for (int e = 0; e < 8; e++) qv[s][e] *= p.qscale, top = fmaxf(top, fabsf(qv[s][e]));
-        top = xmax<32>(xmax<16>(top));
-        row_power(top, up, down);
+            for (int s = 0; s < F::KS; s++)
 #pragma unroll
-        for (int s = 0; s < F::KS; s++)
+                for (int e = 0; e < 8; e++) qv[c][s][e] *= p.qscale, top = fmaxf(top, fabsf(qv[c][s][e]));
+            top = xmax<32>(xmax<16>(top));
+            row_power(top, up, down[c]);
 #pragma unroll
-            for (int e = 0; e < 8; e++) {
-                const float v = qv[s][e] * up;
-                const _Float16 h = (_Float16)v, l = (_Float16)(v - (float)h);
-                if constexpr (NR == 8) qb[0][s][e] = i16 & 1 ? l : h;
-                else qb[0][s][e] = h, qb[1][s][e] = l;
-            }
+            for (int s = 0; s < F::KS; s++)
+#pragma unroll
+                for (int e = 0; e < 8; e++) {
+                    const float v = qv[c][s][e] * up;
+                    const _Float16 h = (_Float16)v, l = (_Float16)(v - (float)h);
+                    if constexpr (F::PAIRED) qb[c][0][s][e] = i16 & 1 ? l : h;
+                    else qb[c][0][s][e] = h, qb[c][1][s][e] = l;
+                }
+        }
     }
-    kf4 o[F::DT];
+    kf4 o[CT][F::DT];
+    float m[CT], l[CT];
 #pragma unroll
-    for (int d = 0; d < F::DT; d++) o[d] = kf4{0.f, 0.f, 0.f, 0.f};
-    float m = -INFINITY, l = 0.f;
+    for (int c = 0; c < CT; c++) {
+        m[c] = -INFINITY, l[c] = 0.f;
+#pragma unroll
+        for (int d = 0; d < F::DT; d++) o[c][d] = kf4{0.f, 0.f, 0.f, 0.f};
+    }
+    // the next 64 blocks' scales against the largest so far: outputs are in its unit, maxima hold its log2
+    auto take_scales = [&]() {
+        const float next = fmaxf(big, wave_max_f32(vsl));
+        if (next > big) {
+            const float r = big > 0.f ? next / big : 1.f, lg = __builtin_amdgcn_logf(r);
+#pragma unroll
+            for (int c = 0; c < CT; c++) {
+                l[c] *= r, m[c] -= lg;
+#pragma unroll
+                for (int d = 0; d < F::DT; d++)
+                    if (big == 0.f) o[c][d] = kf4{0.f, 0.f, 0.f, 0.f};  // (of zeros alone)
+            }
+            big = next;
+        }
+        share_of(vsl, big, lvl, inl);
+    };
 
     auto compute = [&](const Block8<HD> &r, int t) {
-        const uint32_t b = block_of(t), first = b * kKv8Block;
-        const float ks = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(ksl), t & 63)) * down;
-        const float vs = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(vsl), t & 63));
-        kf4 s[2];
+        const uint32_t first = block_of(t) * kKv8Block;
+        auto of_block = [&](float v) { return __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(v), t & 63)); };
+        const float ks = of_block(ksl), lv = of_block(lvl), inv = of_block(inl);
+        const bool edge = first < lo_max || first + kKv8Block - 1 > pos_min;
+        kf4 s[CT][2];
 #pragma unroll
         for (int pt = 0; pt < 2; pt++) {
-            s[pt] = kf4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int c = 0; c < CT; c++) s[c][pt] = kf4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
             for (int k = 0; k < F::KS; k++) {
                 const kh8 a = widen8(r.k[pt][2 * k], r.k[pt][2 * k + 1]);
 #pragma unroll
-                for (int j = 0; j < P; j++) s[pt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, qb[j][k], s[pt], 0, 0, 0);
+                for (int c = 0; c < CT; c++)
+#pragma unroll
+                    for (int j = 0; j < P; j++) s[c][pt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, qb[c][j][k], s[c][pt], 0, 0, 0);
             }
         }
-        const bool edge = first < lo_max || first + kKv8Block - 1 > pos_min;
-        float w[8], mx = -INFINITY;
+        kh8 ph[CT][P];
 #pragma unroll
-        for (int e = 0; e < 8; e++) {
-            float v = s[e >> 2][e & 3];
-            if constexpr (NR == 8)  // the other piece's column
-                v += __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), 0xB1, 0xF, 0xF, false));
-            w[e] = v * ks;
-        }
-        if (edge)
+        for (int c = 0; c < CT; c++) {
+            float w[8], mx = -INFINITY;
+            const float f = ks * down[c];
 #pragma unroll
             for (int e = 0; e < 8; e++) {
-                const uint32_t at = first + 8 * g + e;
-                if (at < lo || at > pos) w[e] = -INFINITY;
+                w[e] = s[c][e >> 2][e & 3];
+                if constexpr (F::PAIRED)  // the other piece's column
+                    w[e] += __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(w[e]), 0xB1, 0xF, 0xF, false));
+            }
+            uint32_t keep = 255;
+            if (edge) {
+                const uint32_t pos = p.position + p.query_of(row_of(c, i16)), lo = first_seen(pos, p.window);
+                keep = 0;
+#pragma unroll
+                for (int e = 0; e < 8; e++) {
+                    const uint32_t at = first + 8 * g + e;
+                    const bool in = at >= lo && at <= pos;
+                    keep |= (uint32_t)in << e;
+                    if (!in) w[e] = -INFINITY;
+                }
             }
 #pragma unroll
-        for (int e = 0; e < 8; e++) mx = fmaxf(mx, w[e]);
-        mx = xmax<32>(xmax<16>(mx));
-        if (__any(mx > m)) {
-            const float mn = fmaxf(m, mx), al = __builtin_amdgcn_exp2f(m - finite(mn));
-            m = mn;
-            l *= al;
+            for (int e = 0; e < 8; e++) mx = fmaxf(mx, w[e]);
+            mx = fmaf(xmax<32>(xmax<16>(mx)), f, lv);
+            if (__any(mx > m[c])) {
+                const float mn = fmaxf(m[c], mx), al = __builtin_amdgcn_exp2f(m[c] - finite(mn));
+                m[c] = mn;
+                l[c] *= al;
 #pragma unroll
-            for (int j = 0; j < 4; j++) {
-                const float a = __shfl(al, 4 * g + j);
+                for (int j = 0; j < 4; j++) {
+                    const float a = __shfl(al, 4 * g + j);
 #pragma unroll
-                for (int d = 0; d < F::DT; d++) o[d][j] *= a;
+                    for (int d = 0; d < F::DT; d++) o[c][d][j] *= a;
+                }
             }
+            const float to = lv - finite(m[c]);
+            float sum = 0.f;
+#pragma unroll
+            for (int e = 0; e < 8; e++) w[e] = __builtin_amdgcn_exp2f(fmaf(w[e], f, to));
+            if (edge)
+#pragma unroll
+                for (int e = 0; e < 8; e++)
+                    if (!(keep >> e & 1u)) w[e] = 0.f;
+            uint32_t hi[4], lo[4];
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                sum += w[2 * e] + w[2 * e + 1];
+                pieces(w[2 * e], w[2 * e + 1], hi[e], lo[e]);
+                if constexpr (F::PAIRED) hi[e] = i16 & 1 ? lo[e] : hi[e];
+            }
+            ph[c][0] = __builtin_bit_cast(kh8, uint4{hi[0], hi[1], hi[2], hi[3]});
+            if constexpr (!F::PAIRED) ph[c][1] = __builtin_bit_cast(kh8, uint4{lo[0], lo[1], lo[2], lo[3]});
+            // (a row with none of the block in sight takes nothing from it, whatever its scale)
+            l[c] += sum == 0.f ? 0.f : sum * inv;
         }
-        const float mf = finite(m);
-        kh8 ph[P];
-#pragma unroll
-        for (int e = 0; e < 8; e++) {
-            const float x = __builtin_amdgcn_exp2f(w[e] - mf);
-            l += x;
-            const _Float16 h = (_Float16)(x * kWeight), lw = (_Float16)fmaf(x, kWeight, -(float)h);
-            if constexpr (NR == 8) ph[0][e] = i16 & 1 ? lw : h;
-            else ph[0][e] = h, ph[1][e] = lw;
-        }
-        const float unit = vs * (1.f / kWeight);
-        float f[4] = {unit, unit, unit, unit};
-        if (edge)  // a block out of a row's sight adds nothing to it, whatever its scale
-#pragma unroll
-            for (int j = 0; j < 4; j++) {
-                const uint32_t other = min(r0 + (uint32_t)(NR == 8 ? (4 * g + j) >> 1 : 4 * g + j), rlast), at = p.position + other / p.group;
-                if (first + kKv8Block - 1 < first_seen(at, p.window) || first > at) f[j] = 0.f;
-            }
 #pragma unroll
         for (int d = 0; d < F::DT; d++) {
             const kh8 v = widen8(r.v[d][0], r.v[d][1]);
-            kf4 a = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-            for (int j = 0; j < P; j++) a = __builtin_amdgcn_mfma_f32_16x16x32_f16(ph[j], v, a, 0, 0, 0);
+            for (int c = 0; c < CT; c++)
 #pragma unroll
-            for (int j = 0; j < 4; j++) o[d][j] = fmaf(f[j], a[j], o[d][j]);
+                for (int j = 0; j < P; j++) o[c][d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ph[c][j], v, o[c][d], 0, 0, 0);
         }
     };
 
     if (nb > 0) {
+        take_scales();
         for (int t = 0; t < nb; t += 2) {
-            if (t && (t & 63) == 0) load_scales(t);
+            if (t && (t & 63) == 0) load_scales(t), take_scales();
             compute(x, t);
             load(x, t + 2);
             if (t + 1 < nb) compute(y, t + 1);
@@ -252,37 +320,44 @@ __global__ void __launch_bounds__(256, PER_CU) kv8_few_kernel(Kv8Params p) {
         }
     }
     // the wavefront's rows: both pieces' outputs, the sum over its lanes
-    l = xsum<32>(xsum<16>(l));
+    const float unit = big * (1.f / kWeight);
 #pragma unroll
-    for (int d = 0; d < F::DT; d++)
+    for (int c = 0; c < CT; c++) {
+        const float sum = xsum<32>(xsum<16>(l[c]));
 #pragma unroll
-        for (int j = 0; j < 4; j++) {
-            if constexpr (NR == 8) {
-                if (j % 2 == 0) os[wave][2 * g + j / 2][16 * d + i16] = o[d][j] + o[d][j + 1];
-            } else
-                os[wave][4 * g + j][16 * d + i16] = o[d][j];
+        for (int d = 0; d < F::DT; d++)
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                if constexpr (F::PAIRED) {
+                    if (j % 2 == 0) os[wave][2 * g + j / 2][16 * d + i16] = (o[c][d][j] + o[c][d][j + 1]) * unit;
+                } else
+                    os[wave][16 * c + 4 * g + j][16 * d + i16] = o[c][d][j] * unit;
+            }
+        if (lane < 16 && (!F::PAIRED || lane % 2 == 0)) {
+            const int r = F::PAIRED ? lane / 2 : 16 * c + lane;
+            ms[wave][r] = m[c], ls[wave][r] = sum;
         }
-    if (lane < 16 && (NR == 16 || lane % 2 == 0)) ms[wave][NR == 8 ? lane / 2 : lane] = m, ls[wave][NR == 8 ? lane / 2 : lane] = l;
+    }
     __syncthreads();
     const uint32_t live = rlast - r0 + 1;
-    for (int u = tid; u < (int)live * HD; u += 256) {
-        const int r = u / HD, d = u % HD;
+    for (int u = tid; u < (int)live * (HD / 4); u += 256) {
+        const int r = u / (HD / 4), d = 4 * (u % (HD / 4));
         const float mx = fmaxf(fmaxf(ms[0][r], ms[1][r]), fmaxf(ms[2][r], ms[3][r])), mf = finite(mx);
-        float sum = 0.f, a = 0.f;
+        float sum = 0.f;
+        float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
         for (int w = 0; w < 4; w++) {
             const float al = __builtin_amdgcn_exp2f(ms[w][r] - mf);
-            sum = fmaf(al, ls[w][r], sum), a = fmaf(al, os[w][r][d], a);
+            const float4 v = *reinterpret_cast<const float4 *>(&os[w][r][d]);
+            sum = fmaf(al, ls[w][r], sum);
+            a.x = fmaf(al, v.x, a.x), a.y = fmaf(al, v.y, a.y), a.z = fmaf(al, v.z, a.z), a.w = fmaf(al, v.w, a.w);
         }
-        const uint32_t gr = r0 + r;
-        const size_t to = (size_t)(gr / p.group) * p.heads + kvh * p.group + gr % p.group;
-        if (p.splits == 1) {
-            p.out[to * HD + d] = a / sum;
-        } else {  // a split's outputs are those of its own positions (0 where it has none in sight)
-            const size_t at = (size_t)z * p.queries * p.heads + to;
-            p.part[at * HD + d] = mx == -INFINITY && sum == 0.f ? 0.f : a / sum;
-            if (d == 0) p.part_ml[2 * at] = mx, p.part_ml[2 * at + 1] = sum;
-        }
+        const uint32_t gr = r0 + r, qi = p.query_of(gr);
+        const size_t to = (size_t)qi * p.heads + kvh * p.group + (gr - qi * p.group), at = (size_t)z * p.queries * p.heads + to;
+        // a split's outputs are those of its own positions (0 where it has none in sight)
+        const float n = p.splits > 1 && mx == -INFINITY && sum == 0.f ? 0.f : 1.f / sum;
+        *reinterpret_cast<float4 *>(p.splits > 1 ? p.part + at * HD + d : p.out + to * HD + d) = make_float4(a.x * n, a.y * n, a.z * n, a.w * n);
+        if (p.splits > 1 && d == 0) *reinterpret_cast<float2 *>(p.part_ml + 2 * at) = make_float2(mx, sum);
     }
 }
 
@@ -292,11 +367,6 @@ __global__ void __launch_bounds__(256, PER_CU) kv8_few_kernel(Kv8Params p) {
 // (two blocks), widened to binary16 on their way into LDS, two tiles deep.  S[position][row] = K Q^T
 // and O[dim][row] = V^T P^T on 32x32x16 products.  K rows are read with bits 2 and 3 of their index
 // exchanged, so that a lane's weights are of positions 16 k + 8 h .. + 7: 16 bytes of a V dim in LDS.
-// The V scale of a block goes into the exponent, w = 2^(s + log2 v - max), v its share of the largest
-// scale in the workgroup's range; the block's weights over v add to the sum.  (Shares below 2^-60, an
-// all-zero block's among them, count as 2^-60: their values are below what the largest one's rounding
-// leaves, and the sum keeps their weight.)  A multiplication of the outputs per block instead would be
-// 128 more vector instructions a tile.
 template <int HD> constexpr int kManyPerCu = HD <= 128 ? 2 : 1;
 
 template <int HD> __global__ void __launch_bounds__(256, kManyPerCu<HD>) kv8_many_kernel(Kv8Params p) {
@@ -313,7 +383,7 @@ template <int HD> __global__ void __launch_bounds__(256, kManyPerCu<HD>) kv8_man
     const uint32_t kv_last = p.position + qlast, kv_first = first_seen(p.position + q0, p.window);
     const int t_first = (int)(kv_first >> 6), nt_all = (int)(kv_last >> 6) + 1 - t_first;
     const int t0 = t_first + (int)((int64_t)nt_all * z / p.splits), t1 = t_first + (int)((int64_t)nt_all * (z + 1) / p.splits);
-    const int v = wave * 32 + l32, qi = q0 + v / p.group, head = kvh * p.group + v % p.group;
+    const int v = wave * 32 + l32, vq = (int)p.query_of(v), qi = q0 + vq, vh = v - vq * p.group, head = kvh * p.group + vh;
     const bool valid = v < qn * p.group && qi <= qlast;
     const int qc = min(qi, qlast);
     const uint32_t qpos = p.position + qc, qlo = first_seen(qpos, p.window);
@@ -369,7 +439,7 @@ template <int HD> __global__ void __launch_bounds__(256, kManyPerCu<HD>) kv8_man
     kh8 qh[KT], ql[KT];
     float down;
     {
-        const float *q = p.q + (size_t)qc * p.q_stride + (size_t)(kvh * p.group + (valid ? v % p.group : 0)) * HD + 8 * lh;
+        const float *q = p.q + (size_t)qc * p.q_stride + (size_t)(kvh * p.group + (valid ? vh : 0)) * HD + 8 * lh;
         float qv[KT][8], top = 0.f, up;
 #pragma unroll
         for (int t = 0; t < KT; t++) load8(q + 16 * t, p.q_aligned, qv[t]);
@@ -433,12 +503,11 @@ template <int HD> __global__ void __launch_bounds__(256, kManyPerCu<HD>) kv8_man
                         if (!in) s[pt][r] = -INFINITY;
                     }
             }
-            float f[2], lv[2], mx = -INFINITY;
+            float f[2], lv[2], inv[2], mx = -INFINITY;
 #pragma unroll
             for (int pt = 0; pt < 2; pt++) {
                 f[pt] = kscale[pt] * down;
-                const float share = vscale[pt] / big;
-                lv[pt] = big > 0.f ? __builtin_amdgcn_logf(share < 0x1p-60f ? 0x1p-60f : share) : 0.f * vscale[pt];
+                share_of(vscale[pt], big, lv[pt], inv[pt]);
                 float a = s[pt][0];
 #pragma unroll
                 for (int r = 1; r < 16; r++) a = fmaxf(a, s[pt][r]);
@@ -470,13 +539,10 @@ template <int HD> __global__ void __launch_bounds__(256, kManyPerCu<HD>) kv8_man
                 for (int i = 0; i < 8; i++) {
                     const float a = s[pt][2 * i], b = s[pt][2 * i + 1];
                     sum += a + b;
-                    const kh2 h = kh2{(_Float16)a, (_Float16)b} * (_Float16)kWeight;  // (exact)
-                    const kh2 w = {(_Float16)fmaf(a, kWeight, -(float)h[0]), (_Float16)fmaf(b, kWeight, -(float)h[1])};
-                    hi[i] = __builtin_bit_cast(uint32_t, h);
-                    lo[i] = __builtin_bit_cast(uint32_t, w);
+                    pieces(a, b, hi[i], lo[i]);
                 }
                 // (a row with none of the block in sight takes nothing from it, whatever its scale)
-                l += sum == 0.f ? 0.f : sum * __builtin_amdgcn_exp2f(-lv[pt]);
+                l += sum == 0.f ? 0.f : sum * inv[pt];
 #pragma unroll
                 for (int k = 0; k < 2; k++) {
                     const kh8 ph = __builtin_bit_cast(kh8, uint4{hi[4 * k], hi[4 * k + 1], hi[4 * k + 2], hi[4 * k + 3]}),
@@ -552,17 +618,22 @@ hipError_t launch_kv8_attention(const Kv8Attn &a, int cus, hipStream_t s) {
     p.c = a.c, p.q = a.q, p.q_stride = a.q_stride, p.out = a.out;
     p.position = a.position, p.queries = a.queries, p.window = a.window;
     p.heads = a.heads, p.group = a.heads / a.c.nkv, p.qscale = a.qscale;
+    p.per_group = (65536u + p.group - 1) / p.group;
     p.q_aligned = (uintptr_t)a.q % 16 == 0 && a.q_stride % 4 == 0;
     const uint64_t rows = (uint64_t)a.queries * p.group;  // of a kv head
-    const bool many = rows > 32;
-    const int nr = rows > 8 ? 16 : 8, qn = 128 / p.group;
-    const uint64_t wgs = p.c.nkv * (many ? (a.queries + (uint64_t)qn - 1) / qn : (rows + nr - 1) / nr);
+    // (9 queries x 4 heads over 16k positions: 25.8 us here, 27.3 by the other kernel; 16 x 4: 33.1 and 30.3.
+    // Of head size 256 more than 16 rows don't fit a wavefront's registers.)
+    const bool many = rows > (a.c.hd <= 128 ? 48 : 16);
+    const int nr = rows <= 8 ? 8 : (int)(rows + 15) / 16 * 16, qn = 128 / p.group;
+    const uint64_t wgs = p.c.nkv * (many ? (a.queries + (uint64_t)qn - 1) / qn : 1);
     if (wgs > 0x7FFFFFFFu) return hipErrorInvalidValue;
     // positions: of the query that sees the fewest
     const uint32_t seen = a.window && a.window <= a.position ? a.window : a.position + 1;
-    const uint64_t least = many ? 4 * 64 : 4 * kKv8Block;
+    // workgroups: as many as are resident at once of many rows; of few, one a CU (131071 positions: 32 splits of 8
+    // kv heads 52.1 us, 48 57.9, 64 52.5; 4113 positions: 16 splits 10.3, 32 9.5, 64 10.2)
+    const uint64_t least = many ? 4 * 64 : 4 * kKv8Block, per_cu = many && a.c.hd <= 128 ? 2 : 1;
     const uint64_t total = (uint64_t)a.queries * a.heads;
-    uint64_t splits = 2 * (uint64_t)cus / wgs;
+    uint64_t splits = per_cu * (uint64_t)cus / wgs;
     splits = splits < seen / least ? splits : seen / least;
     splits = splits < kMaxSplits ? splits : kMaxSplits;
     while (splits > 1 && splits * total * (a.c.hd + 2) > a.part_floats) splits--;
@@ -570,10 +641,14 @@ hipError_t launch_kv8_attention(const Kv8Attn &a, int cus, hipStream_t s) {
     p.part = a.part, p.part_ml = a.part + (size_t)p.splits * total * a.c.hd;
     const dim3 grid((unsigned)wgs, (unsigned)p.splits);
     auto go = [&](auto h) {
-        constexpr int HD = decltype(h)::value, PER_CU = HD == 256 ? 1 : 2;
+        constexpr int HD = decltype(h)::value;
         if (many) hipLaunchKernelGGL(kv8_many_kernel<HD>, grid, dim3(256), 0, s, p);
-        else if (nr == 8) hipLaunchKernelGGL((kv8_few_kernel<HD, 8, PER_CU>), grid, dim3(256), 0, s, p);
-        else hipLaunchKernelGGL((kv8_few_kernel<HD, 16, PER_CU>), grid, dim3(256), 0, s, p);
+        else if (nr == 8) hipLaunchKernelGGL((kv8_few_kernel<HD, 8>), grid, dim3(256), 0, s, p);
+        else if (nr == 16) hipLaunchKernelGGL((kv8_few_kernel<HD, 16>), grid, dim3(256), 0, s, p);
+        else if constexpr (HD <= 128) {
+            if (nr == 32) hipLaunchKernelGGL((kv8_few_kernel<HD, 32>), grid, dim3(256), 0, s, p);
+            else hipLaunchKernelGGL((kv8_few_kernel<HD, 48>), grid, dim3(256), 0, s, p);
+        }
         if (p.splits > 1)
             hipLaunchKernelGGL(kv8_join_kernel<HD>, dim3((unsigned)total), dim3(256), 0, s, p.part, (const float2 *)p.part_ml, p.out,
                                (size_t)total, p.splits);

@@ -363,7 +363,8 @@ size_t ziggy_hip_kv8_codes_length(uint32_t layers, uint32_t head_count_kv, uint3
 size_t ziggy_hip_kv8_scales_length(uint32_t layers, uint32_t head_count_kv, uint32_t head_dim,
                                    uint32_t context_length);
 /* Stores the rows k, v ([rows][head_count_kv * head_dim] f32, row_stride apart,
- * from k_offset_bytes and v_offset_bytes on) at positions position ..
+ * from k_offset_bytes and v_offset_bytes on; both may lie in the rows of a
+ * fused projection, the keys rotated in place) at positions position ..
  * position + rows - 1.  A block whose first position is among them starts
  * anew: its scale is max|x| / 127 over its new rows, a code the nearest
  * integer to x / scale (ties to even).  In a block that begins before
@@ -665,6 +666,16 @@ int ziggy_hip_sample_rows_f32(ZiggyHipContext *ctx, const ZiggyHipBuffer *logits
                               const ZiggyHipSamplingOptions *options, const ZiggyHipBuffer *uniforms,
                               ZiggyHipBuffer *out_tokens, uint32_t rows, uint32_t vocab, char *error_message,
                               size_t error_message_len);
+
+/* One decode step of `token` whose output is a token drawn on the device from
+ * the step's logits, as ziggy_hip_sample_rows_f32 draws it (its options, its
+ * refusals): step, sampling and a read-back of four bytes, where step_shortlist
+ * and the host sampler serve at most 64 candidates.  recent: the tokens so far,
+ * on the host; uniform in [0, 1).  The logits stay readable with
+ * session_read_logits; the position advances by one. */
+int ziggy_hip_session_step_sample(ZiggyHipSession *session, uint32_t token, const uint32_t *recent,
+                                  uint32_t recent_count, const ZiggyHipSamplingOptions *options, double uniform,
+                                  uint32_t *out_token, char *error_message, size_t error_message_len);
 
 /* Times one kernel of the decode step (no counterpart in the reference; its
  * Metal profiler times host-side encode, runtime/metal_profile.zig:80-315):

@@ -93,6 +93,19 @@ bool meets_cache(const ZiggyHipKv8Cache *c, const void *p, size_t n) {
 
 }  // namespace
 
+namespace zh {
+
+const char *sample_refusal(const ZiggyHipSamplingOptions &o, uint32_t vocab) {
+    if (vocab == 0 || vocab > 262144) return "sampling takes rows of 1 to 262144 logits";
+    if (o.top_k > 1024 && o.top_k < vocab) return "top_k is neither at most 1024 nor the whole vocabulary";
+    if (!isfinite(o.temperature) || !isfinite(o.repeat_penalty) || !(o.top_p >= 0.f && o.top_p <= 1.f) ||
+        !(o.min_p >= 0.f && o.min_p <= 1.f))
+        return "invalid sampling options";
+    return nullptr;
+}
+
+}  // namespace zh
+
 extern "C" {
 
 int ziggy_hip_wrap_buffer(ZiggyHipContext *ctx, void *device_memory, size_t length, ZiggyHipBuffer **out, char *err,
@@ -267,11 +280,9 @@ int ziggy_hip_sample_rows_f32(ZiggyHipContext *ctx, const ZiggyHipBuffer *logits
                               const ZiggyHipBuffer *uniforms, ZiggyHipBuffer *out, uint32_t rows, uint32_t vocab, char *err,
                               size_t err_len) {
     ZH_REFUSE(!ctx || !o, "null context or sampling options");
-    ZH_REFUSE(rows == 0 || vocab == 0 || vocab > 262144, "sampling takes rows of 1 to 262144 logits");
-    ZH_REFUSE(o->top_k > 1024 && o->top_k < vocab, "top_k %u is neither at most 1024 nor the whole vocabulary", o->top_k);
-    ZH_REFUSE(!isfinite(o->temperature) || !isfinite(o->repeat_penalty) || !(o->top_p >= 0.f && o->top_p <= 1.f) ||
-                  !(o->min_p >= 0.f && o->min_p <= 1.f),
-              "invalid sampling options");
+    ZH_REFUSE(rows == 0, "sampling needs rows");
+    const char *why = sample_refusal(*o, vocab);
+    ZH_REFUSE(why, "%s", why);
     if (stride == 0) stride = vocab;
     const bool penalty = o->repeat_penalty > 1.f && recent_count > 0 && o->temperature > 0;
     ZH_REFUSE(stride < vocab || !in_buffer(ctx, logits, rows_bytes(rows, vocab, stride)) ||

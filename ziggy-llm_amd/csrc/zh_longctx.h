@@ -64,6 +64,8 @@ struct SampleRows {
     void *work;  // sample_rows_bytes(vocab) a row
 };
 size_t sample_rows_bytes(uint32_t vocab);
+// why options or a vocabulary are not sampled on the device (null: they are)
+const char *sample_refusal(const ZiggyHipSamplingOptions &o, uint32_t vocab);
 hipError_t launch_sample_rows(const SampleRows &p, hipStream_t s);
 
 }  // namespace zh

@@ -22,6 +22,7 @@
 
 #include "zh_arena.h"
 #include "zh_internal.h"
+#include "zh_longctx.h"
 #include "zh_quant.h"
 #include "zh_step.h"
 
@@ -94,6 +95,10 @@ struct ZiggyHipSession {
     // output shortlist (allocated on first use): packed keys, entries
     unsigned long long *sl_keys = nullptr;
     uint32_t *sl_entries = nullptr;
+    // sampling on the device (allocated on first use): {random number, token}, the row's workspace, recent tokens
+    uint32_t *sp_io = nullptr, *sp_recent = nullptr;
+    void *sp_work = nullptr;
+    uint32_t sp_recent_cap = 0;
     uint32_t *b_tokens = nullptr;
     unsigned long long *b_argmax = nullptr;
     // multi-query attention of a verify pass: partials and arrival counters
@@ -939,6 +944,54 @@ int ziggy_hip_session_step_shortlist(ZiggyHipSession *s, uint32_t token, uint32_
     ZH_TRY(launch_copy_spans(CopySpans{{pin}, {s->sl_entries}, {(int)(2 * count)}}, sm), "shortlist readback");
     ZH_TRY(hipStreamSynchronize(sm), "shortlist");
     memcpy(out, pin, (size_t)count * 8);
+    s->logits_valid = true;
+    return ZIGGY_HIP_OK;
+}
+
+int ziggy_hip_session_step_sample(ZiggyHipSession *s, uint32_t token, const uint32_t *recent, uint32_t recent_count,
+                                  const ZiggyHipSamplingOptions *options, double uniform, uint32_t *out_token, char *err,
+                                  size_t err_len) {
+    if (!s || !options || !out_token || (recent_count && !recent))
+        return fail(err, err_len, ZIGGY_HIP_INVALID_ARGUMENT, "invalid step_sample arguments");
+    const uint32_t V = s->md.vocab_size;
+    if (const char *why = sample_refusal(*options, V)) return fail(err, err_len, ZIGGY_HIP_INVALID_ARGUMENT, why);
+    if (!(uniform >= 0.0 && uniform < 1.0))
+        return fail(err, err_len, ZIGGY_HIP_INVALID_ARGUMENT, "the random number lies outside [0, 1)");
+    const bool penalty = options->repeat_penalty > 1.f && options->temperature > 0.f && recent_count > 0;
+    if (!s->sp_io) {
+        ZH_TRY(hipMalloc((void **)&s->sp_io, 256), "sampling buffers");
+        s->allocs.push_back(s->sp_io);
+    }
+    if (!s->sp_work) {
+        ZH_TRY(hipMalloc(&s->sp_work, sample_rows_bytes(V)), "sampling buffers");
+        s->allocs.push_back(s->sp_work);
+    }
+    if (penalty && recent_count > s->sp_recent_cap) {
+        // (the stream is idle between calls; the outgrown list is freed with the session)
+        const uint32_t cap = recent_count < 4096 ? 4096 : 2 * std::min(recent_count, 0x7FFFFFFFu);
+        uint32_t *list = nullptr;
+        ZH_TRY(hipMalloc((void **)&list, (size_t)cap * 4), "sampling buffers");
+        s->allocs.push_back(list);
+        s->sp_recent = list, s->sp_recent_cap = cap;
+    }
+    const int st = host_step(s, token, false, nullptr, err, err_len);
+    if (st != ZIGGY_HIP_OK) return st;
+    hipStream_t sm = s->ctx->stream;
+    ZH_TRY(enqueue_output_logits(s, sm), "sampling output");
+    uint32_t *pin = s->ctx->pin + kPinHead;
+    const uint32_t pinned = penalty && recent_count <= kPinWords - kPinHead - 8 ? recent_count : 0;
+    memcpy(pin, &uniform, 8);
+    if (pinned) memcpy(pin + 8, recent, (size_t)pinned * 4);
+    else if (penalty) ZH_TRY(hipMemcpyAsync(s->sp_recent, recent, (size_t)recent_count * 4, hipMemcpyHostToDevice, sm), "sampling input");
+    ZH_TRY(launch_copy_spans(CopySpans{{s->sp_io, s->sp_recent}, {pin, pin + 8}, {2, (int)pinned}}, sm), "sampling input");
+    SampleRows p{};
+    p.x = s->logits, p.stride = V, p.rows = 1, p.vocab = V, p.o = *options, p.work = s->sp_work;
+    if (penalty) p.recent = s->sp_recent, p.recent_count = recent_count;
+    p.uniforms = (const double *)s->sp_io, p.out = s->sp_io + 2;
+    ZH_TRY(launch_sample_rows(p, sm), "sampling");
+    ZH_TRY(launch_copy_spans(CopySpans{{pin + 2}, {s->sp_io + 2}, {1}}, sm), "sampling readback");
+    ZH_TRY(hipStreamSynchronize(sm), "sampling");
+    *out_token = pin[2];
     s->logits_valid = true;
     return ZIGGY_HIP_OK;
 }

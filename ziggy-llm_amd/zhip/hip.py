@@ -245,6 +245,8 @@ def lib() -> ctypes.CDLL:
         "ziggy_hip_session_read_logits": [vp, vp] + E,
         "ziggy_hip_session_verify": [vp, u32, vp, u32, vp, ctypes.POINTER(u32)] + E,
         "ziggy_hip_session_step_shortlist": [vp, u32, u32, vp] + E,
+        "ziggy_hip_session_step_sample": [vp, u32, vp, u32, ctypes.POINTER(SamplingOptions), ctypes.c_double,
+                                          ctypes.POINTER(u32)] + E,
         "ziggy_hip_session_prefill_cached": [vp, vp, u32, ctypes.POINTER(u32), ctypes.POINTER(u32)] + E,
         "ziggy_hip_shortlist_len": [ctypes.POINTER(SamplingOptions), u32],
         "ziggy_hip_sample_shortlist": [vp, u32, vp, u32, ctypes.POINTER(SamplingOptions), ctypes.c_double,
@@ -359,7 +361,8 @@ class Context:
 
     def wrap(self, address: int, nbytes: int) -> Buffer:
         """A buffer over the caller's device memory (ziggy_hip_wrap_buffer), a torch tensor's data_ptr() for
-        instance; the caller keeps it alive and orders other streams' work on it."""
+        instance; the caller keeps it alive and orders other streams' work on it.  (torch brings a HIP runtime
+        of its own: a program with both initialises torch's GPU before it makes a Context.)"""
         h = ctypes.c_void_p()
         _call("ziggy_hip_wrap_buffer", self.h, address, nbytes, ctypes.byref(h))
         b = Buffer(self, h, nbytes)
@@ -628,6 +631,14 @@ class Session:
         out = (ShortlistEntry * count)()
         _call("ziggy_hip_session_step_shortlist", self.h, token, count, ctypes.cast(out, ctypes.c_void_p))
         return (np.array([e.token_id for e in out], np.uint32), np.array([e.logit for e in out], np.float32))
+
+    def step_sample(self, token: int, recent, options: SamplingOptions, uniform: float) -> int:
+        """One decode step of `token`; the next token drawn on the device (ziggy_hip_session_step_sample)."""
+        rec = np.ascontiguousarray(recent, np.uint32)
+        out = ctypes.c_uint32()
+        _call("ziggy_hip_session_step_sample", self.h, token, rec.ctypes.data if rec.size else None, rec.size,
+              ctypes.byref(options), uniform, ctypes.byref(out))
+        return out.value
 
     def verify(self, current: int, drafts):
         """(predicted tokens [len(drafts) + 1], emitted count) of one batched verify pass."""

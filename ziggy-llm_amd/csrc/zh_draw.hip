@@ -246,32 +246,43 @@ struct Finish {
     Key key[kThreads / 64];
 };
 
+// Inclusive prefix sum over the wavefront on the vector ALU: within rows of 16 by row shifts, then the
+// rows' ends broadcast to the rows behind.
+template <int CTRL, int ROWS> __device__ __forceinline__ u64 add_dpp(u64 v) {
+    const uint32_t lo = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)v, CTRL, ROWS, 0xF, false);
+    const uint32_t hi = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)(v >> 32), CTRL, ROWS, 0xF, false);
+    return v + ((u64)hi << 32 | lo);
+}
+__device__ __forceinline__ u64 wave_prefix(u64 v) {
+    v = add_dpp<0x111, 0xF>(v);  // row_shr:1, 2, 4, 8 (lanes before the row's start: 0)
+    v = add_dpp<0x112, 0xF>(v);
+    v = add_dpp<0x114, 0xF>(v);
+    v = add_dpp<0x118, 0xF>(v);
+    v = add_dpp<0x142, 0xA>(v);  // row_bcast:15 into rows 1 and 3
+    return add_dpp<0x143, 0xC>(v);  // row_bcast:31 into rows 2 and 3
+}
 // Inclusive prefix sum over the workgroup; *total: the whole.
 __device__ u64 prefix(Finish &f, u64 v, u64 *total) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    for (int d = 1; d < 64; d <<= 1) {
-        const u64 o = (u64)__shfl_up((long long)v, d);
-        if (lane >= d) v += o;
-    }
+    v = wave_prefix(v);
     __syncthreads();
     if (lane == 63) f.wave[wave] = v;
     __syncthreads();
     u64 before = 0, all = 0;
+#pragma unroll
     for (int i = 0; i < kThreads / 64; i++) {
-        if (i == wave) before = all;
-        all += f.wave[i];
+        const u64 w = f.wave[i];
+        before += i < wave ? w : 0;
+        all += w;
     }
     *total = all;
     return v + before;
 }
-// The lowest thread whose running sum `run` (of its own v) reaches target; *before: the sum ahead of it.
-// (None, which the callers' targets exclude: the last one with a weight.)
+// The thread whose running sum `run` (of its own v) reaches target, 1 .. the whole sum; *before: the sum
+// ahead of it.
 __device__ uint32_t first_reaching(Finish &f, u64 run, u64 v, u64 target, u64 *before) {
     __syncthreads();
-    if (threadIdx.x == 0) f.found = 0, f.value = 0;
-    __syncthreads();
-    const bool mine = v && run >= target && run - v < target;
-    if (mine) f.found = threadIdx.x, f.value = run - v;
+    if (v && run >= target && run - v < target) f.found = threadIdx.x, f.value = run - v;
     __syncthreads();
     *before = f.value;
     return f.found;
@@ -361,13 +372,27 @@ template <class K> __device__ Key largest(Finish &f, uint32_t n, K key) {
     return k;
 }
 
-// Calls take(logit, its id) for the row's logits of bins first .. last, 8 lanes a slice.
+// Calls take(logit, its id) for the row's logits of bins first .. last, 8 lanes a slice, 64 of a slice
+// under way at once.
 template <class T> __device__ __forceinline__ void of_bins(const RowWork &w, uint32_t slices, uint32_t first, uint32_t last, T take) {
+    constexpr int N = 8;
     const size_t slice = threadIdx.x / 8;
     if (slice >= slices) return;
     const uint32_t begin = w.run[slice * kBins + first] & 0xFFFFu, end = w.run[slice * kBins + last] >> 16;
-    for (uint32_t e = begin + threadIdx.x % 8; e < end; e += 8)
-        take(w.value[slice * kSliceLogits + e], (uint32_t)slice * kSliceLogits + w.from[slice * kSliceLogits + e]);
+    const float *value = w.value + slice * kSliceLogits;
+    const uint16_t *from = w.from + slice * kSliceLogits;
+    for (uint32_t e = begin + threadIdx.x % 8; e < end; e += 8 * N) {
+        float a[N];
+        uint32_t id[N];
+#pragma unroll
+        for (int k = 0; k < N; k++) {
+            const uint32_t at = min(e + 8 * k, end - 1);
+            a[k] = value[at], id[k] = from[at];
+        }
+#pragma unroll
+        for (int k = 0; k < N; k++)
+            if (e + 8 * k < end) take(a[k], (uint32_t)slice * kSliceLogits + id[k]);
+    }
 }
 static_assert(kThreads / 8 >= kMaxSlices, "8 lanes for every slice");
 
@@ -381,6 +406,13 @@ __global__ void __launch_bounds__(kThreads) draw_finish_kernel(SampleRows p) {
     if (p.o.temperature <= 0.f) return answer(~largest(f, n, [&](uint32_t i) { return Key{{ordered(x[i]), ~i, 0}}; }).w[1]);
     const Policy policy(p);
     const RowWork w = row_work(p, row);
+    // two bins' sums of every eighth slice, under way while the recent tokens are marked
+    constexpr int kAhead = 8, kLanes = kThreads / (kBins / 2);
+    const uint32_t slices = slices_of(n);
+    ulonglong2 ahead[kAhead];
+#pragma unroll
+    for (int k = 0; k < kAhead; k++)
+        ahead[k] = *reinterpret_cast<const ulonglong2 *>(w.sums + min(tid / (kBins / 2) + k * kLanes, slices - 1) * kBins + 2 * (tid % (kBins / 2)));
     // (the bins hold penalised logits, but for top-k's)
     if (p.recent) mark_recent(p, row, f.seen, (n + 31) / 32, 0);
     auto logit_of = [&](uint32_t i, float v) {
@@ -393,16 +425,26 @@ __global__ void __launch_bounds__(kThreads) draw_finish_kernel(SampleRows p) {
         return answer(~largest(f, n, [&](uint32_t i) { return Key{{ordered(x[i]), ~i, 0}}; }).w[1]);
 
     // the bins' sums over the slices, the largest logits' first
-    const uint32_t slices = slices_of(n);
     u64 total, before;
     auto sum_bins = [&]() {
+        for (uint32_t s = tid / (kBins / 2) + kAhead * kLanes; s < slices; s += kLanes) {
+            const ulonglong2 v = *reinterpret_cast<const ulonglong2 *>(w.sums + s * kBins + 2 * (tid % (kBins / 2)));
+            ahead[0].x += v.x, ahead[0].y += v.y;
+        }
+        u64 x = 0, y = 0;
+#pragma unroll
+        for (int k = 0; k < kAhead; k++) {
+            const bool in = tid / (kBins / 2) + k * kLanes < slices;
+            x += in ? ahead[k].x : 0, y += in ? ahead[k].y : 0;
+        }
+        __syncthreads();
+        f.list[2 * tid] = x, f.list[2 * tid + 1] = y;
+        __syncthreads();
         u64 v = 0;
-#pragma unroll 8
-        for (uint32_t s = tid / kBins; s < slices; s += kThreads / kBins) v += w.sums[s * kBins + tid % kBins];
-        __syncthreads();
-        f.sums[tid] = v;
-        __syncthreads();
-        return tid < kBins ? f.sums[tid] + f.sums[tid + kBins] + f.sums[tid + 2 * kBins] + f.sums[tid + 3 * kBins] : 0ull;
+        if (tid < kBins)
+#pragma unroll
+            for (int k = 0; k < kLanes; k++) v += f.list[k * kBins + tid];
+        return v;
     };
 
     if (policy.limited) {
@@ -435,9 +477,13 @@ __global__ void __launch_bounds__(kThreads) draw_finish_kernel(SampleRows p) {
         u64 mine = tid < k ? f.list[tid] : 0;
         const uint32_t id = ~(uint32_t)mine;
         const float a = tid < k ? logit_of(id, unordered((uint32_t)(mine >> 32))) : -INFINITY;
-        const Key best = largest(f, kThreads, [&](uint32_t) { return tid < k ? Key{{ordered(a), (uint32_t)(mine >> 32), ~id}} : Key{}; });
-        const float mx = unordered(best.w[0]);
-        if (!(fabsf(mx) < INFINITY)) return answer(~best.w[2]);
+        u64 best = wave_max_key(tid < k ? (u64)ordered(a) << 32 | (uint32_t)~tid : 0);  // of equal ones the first
+        __syncthreads();
+        if ((tid & 63) == 0) f.wave[tid >> 6] = best;
+        __syncthreads();
+        for (int j = 0; j < kThreads / 64; j++) best = f.wave[j] > best ? f.wave[j] : best;
+        const float mx = unordered((uint32_t)(best >> 32));
+        if (!(fabsf(mx) < INFINITY)) return answer(~(uint32_t)f.list[~(uint32_t)best]);
         float b = a;
         uint32_t token = id;
         if (policy.sorted && p.recent) {  // by weight: the penalised logits, ties as they stand

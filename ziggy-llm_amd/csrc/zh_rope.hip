@@ -29,12 +29,12 @@ template <bool ALIGNED> __global__ void __launch_bounds__(256) rope_rows_kernel(
     double f[kPairs];
     if (rotates)
         for (int j = 0; j < kPairs; j++) f[j] = turns_per_position(p, min(i0 + j, half - 1));
-    for (uint32_t r = blockIdx.x; r < p.rows; r += gridDim.x) {
-        const float *src = p.src + (size_t)r * p.src_stride;
-        float *dst = p.dst + (size_t)r * p.dst_stride;
+    for (size_t r = blockIdx.x; r < p.rows; r += gridDim.x) {
+        const float *src = p.src + r * p.src_stride;
+        float *dst = p.dst + r * p.dst_stride;
         float c[kPairs], s[kPairs];
         if (rotates) {
-            const double at = (double)(p.positions ? p.positions[r] : p.first + r);
+            const double at = (double)(p.positions ? p.positions[r] : p.first + (uint32_t)r);
             for (int j = 0; j < kPairs; j++) {
                 const double t = at * f[j];
                 sincospif((float)(2.0 * (t - rint(t))), &s[j], &c[j]);

@@ -109,14 +109,14 @@ template <int HD, int NR> struct Few {
     static constexpr int KB = HD % 64 ? 8 : 16;        // bytes of a lane's K load
     static constexpr int KL = HD / 4 / KB;             // K loads of a row
     static constexpr int KW = KB / 4;
-    static constexpr int PER_CU = NR <= 16 && HD <= 128 ? 2 : 1;  // workgroups whose registers a CU holds
+
 };
 template <int HD> struct Block8 {
     uint32_t k[2][HD / 16], v[HD / 16][2];
 };
 
 template <int HD, int NR>
-__global__ void __launch_bounds__(256, (Few<HD, NR>::PER_CU)) kv8_few_kernel(Kv8Params p) {
+__global__ void __launch_bounds__(256, 1) kv8_few_kernel(Kv8Params p) {
     using F = Few<HD, NR>;
     constexpr int CT = F::CT, P = F::P;
     __shared__ __align__(16) float os[4][NR][HD + 4];

@@ -11,6 +11,9 @@
 // positions, K and V straight from memory into operands.  Many (prompts): a workgroup's 128 rows share
 // tiles of 64 positions in LDS.  Both split the positions over workgroups where rows alone leave CUs
 // idle; a second launch joins the splits in their order, so results don't change from run to run.
+#include <algorithm>
+#include <cmath>
+
 #include "zh_longctx.h"
 
 namespace zh {
@@ -22,7 +25,7 @@ typedef _Float16 kh8 __attribute__((ext_vector_type(8)));
 typedef float kf4 __attribute__((ext_vector_type(4)));
 typedef float kf16 __attribute__((ext_vector_type(16)));
 
-constexpr int kMaxSplits = 64;  // one a lane when they are joined
+constexpr int kMaxSplits = 256;  // one a thread when they are joined
 constexpr float kWeight = 16384.f;  // of the largest weight: its pieces below binary16's 65504
 
 __device__ __forceinline__ uint32_t first_seen(uint32_t pos, uint32_t window) {
@@ -575,32 +578,43 @@ template <int HD> __global__ void __launch_bounds__(256, kManyPerCu<HD>) kv8_man
     if (p.splits > 1 && lh == 0) *reinterpret_cast<float2 *>(p.part_ml + 2 * at) = make_float2(m, l);
 }
 
-// The splits' partial results of a row joined in their order, a workgroup per row.  What a thread reads
-// goes out at once: the splits' maxima and sums a lane each, and its float4 of every N-th split.
+// The splits' partial results of a row joined in their order, a workgroup per row: the splits' maxima and
+// sums a thread each, and a float4 of every N-th split, eight of them under way at once.
 template <int HD> __global__ void __launch_bounds__(256) kv8_join_kernel(const float *__restrict__ part, const float2 *__restrict__ ml,
                                                                        float *__restrict__ out, size_t rows, int splits) {
-    constexpr int C = HD / 4, N = 256 / C, Z = (kMaxSplits + N - 1) / N;  // float4s of a row; splits side by side; of a thread
+    constexpr int C = HD / 4, N = 256 / C, Z = 8;  // float4s of a row; splits side by side
     __shared__ float4 acc[N][C];
-    __shared__ float weight[kMaxSplits];
+    __shared__ float weight[kMaxSplits], tops[4], sums[4];
     const size_t row = blockIdx.x;
-    const int c = threadIdx.x % C, n = threadIdx.x / C, lane = threadIdx.x & 63;
-    const float2 own = ml[(size_t)min(lane, splits - 1) * rows + row];
+    const int tid = threadIdx.x, c = tid % C, n = tid / C;
+    const float2 own = ml[(size_t)min(tid, splits - 1) * rows + row];
     float4 v[Z];
+    auto load = [&](int from) {
 #pragma unroll
-    for (int i = 0; i < Z; i++)
-        v[i] = *reinterpret_cast<const float4 *>(part + ((size_t)min(n + N * i, splits - 1) * rows + row) * HD + 4 * c);
-    const float m = finite(wave_max_f32(own.x));
-    float w = lane < splits ? __builtin_amdgcn_exp2f(own.x - m) * own.y : 0.f;
-    if (threadIdx.x < 64) weight[lane] = w;
-    for (int d = 1; d < 64; d <<= 1) w += __shfl_xor(w, d);
+        for (int i = 0; i < Z; i++)
+            v[i] = *reinterpret_cast<const float4 *>(part + ((size_t)min(from + n + N * i, splits - 1) * rows + row) * HD + 4 * c);
+    };
+    load(0);
+    float m = wave_max_f32(own.x);
+    if ((tid & 63) == 0) tops[tid >> 6] = m;
     __syncthreads();
+    m = finite(fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3])));
+    float w = tid < splits ? __builtin_amdgcn_exp2f(own.x - m) * own.y : 0.f;
+    weight[tid] = w;
+    for (int d = 1; d < 64; d <<= 1) w += __shfl_xor(w, d);
+    if ((tid & 63) == 0) sums[tid >> 6] = w;
+    __syncthreads();
+    w = (sums[0] + sums[1]) + (sums[2] + sums[3]);
     float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int from = 0; from < splits; from += N * Z) {
+        if (from) load(from);
 #pragma unroll
-    for (int i = 0; i < Z; i++)
-        if (n + N * i < splits) {
-            const float f = weight[n + N * i];
-            a.x = fmaf(f, v[i].x, a.x), a.y = fmaf(f, v[i].y, a.y), a.z = fmaf(f, v[i].z, a.z), a.w = fmaf(f, v[i].w, a.w);
-        }
+        for (int i = 0; i < Z; i++)
+            if (from + n + N * i < splits) {
+                const float f = weight[from + n + N * i];
+                a.x = fmaf(f, v[i].x, a.x), a.y = fmaf(f, v[i].y, a.y), a.z = fmaf(f, v[i].z, a.z), a.w = fmaf(f, v[i].w, a.w);
+            }
+    }
     if (n < N) acc[n][c] = a;
     __syncthreads();
     if (n) return;
@@ -627,15 +641,24 @@ hipError_t launch_kv8_attention(const Kv8Attn &a, int cus, hipStream_t s) {
     const int nr = rows <= 8 ? 8 : (int)(rows + 15) / 16 * 16, qn = 128 / p.group;
     const uint64_t wgs = p.c.nkv * (many ? (a.queries + (uint64_t)qn - 1) / qn : 1);
     if (wgs > 0x7FFFFFFFu) return hipErrorInvalidValue;
-    // positions: of the query that sees the fewest
-    const uint32_t seen = a.window && a.window <= a.position ? a.window : a.position + 1;
-    // workgroups: as many as are resident at once of many rows; of few, one a CU (131071 positions: 32 splits of 8
-    // kv heads 52.1 us, 48 57.9, 64 52.5; 4113 positions: 16 splits 10.3, 32 9.5, 64 10.2)
-    const uint64_t least = many ? 4 * 64 : 4 * kKv8Block, per_cu = many && a.c.hd <= 128 ? 2 : 1;
     const uint64_t total = (uint64_t)a.queries * a.heads;
-    uint64_t splits = per_cu * (uint64_t)cus / wgs;
-    splits = splits < seen / least ? splits : seen / least;
-    splits = splits < kMaxSplits ? splits : kMaxSplits;
+    uint64_t splits = 1;
+    if (!many) {
+        // one workgroup a CU, a block for each of its wavefronts at least (131071 positions, 8 kv heads: 32 splits
+        // 52.1 us, 48 57.9, 64 52.5; 4113 positions: 16 splits 10.3, 32 9.5, 64 10.2)
+        const uint32_t seen = a.window && a.window <= a.position ? a.window : a.position + 1;  // of the first query
+        splits = std::min({(uint64_t)cus / wgs, (uint64_t)seen / (4 * kKv8Block), (uint64_t)kMaxSplits});
+    } else {
+        // the split count whose estimated time is least, in us: the longest workgroup's tiles, in rounds of as many
+        // workgroups as are resident, and the join's launch and traffic
+        const uint64_t last = (uint64_t)a.position + a.queries, range = a.window ? std::min(last, (uint64_t)a.window + qn) : last;
+        const double tiles = (double)(range / 64 + 1), tile = 0.5 + 1.4 * a.c.hd / 128, resident = (a.c.hd <= 128 ? 2.0 : 1.0) * cus;
+        double best = 1e300;
+        for (uint64_t n = 1; n <= (uint64_t)kMaxSplits && 2 * n <= (uint64_t)tiles + 1; n++) {
+            const double t = std::ceil(wgs * n / resident) * std::ceil(tiles / n) * tile + (n > 1 ? 4.0 + n * (double)total * a.c.hd * 8 / 3e6 : 0.0);
+            if (t < best * 0.97) best = t, splits = n;
+        }
+    }
     while (splits > 1 && splits * total * (a.c.hd + 2) > a.part_floats) splits--;
     p.splits = splits > 1 ? (int)splits : 1;
     p.part = a.part, p.part_ml = a.part + (size_t)p.splits * total * a.c.hd;

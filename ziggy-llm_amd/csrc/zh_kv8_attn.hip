@@ -625,6 +625,40 @@ template <int HD> __global__ void __launch_bounds__(256) kv8_join_kernel(const f
     *reinterpret_cast<float4 *>(out + row * HD + 4 * c) = make_float4(a.x / w, a.y / w, a.z / w, a.w / w);
 }
 
+// The same for many rows: a thread takes four dims of a row through the splits, four of them under way.
+template <int HD> __global__ void __launch_bounds__(256) kv8_join_rows_kernel(const float *__restrict__ part, const float2 *__restrict__ ml,
+                                                                            float *__restrict__ out, size_t rows, int splits) {
+    constexpr int C = HD / 4, Z = 4;
+    const size_t u = (size_t)blockIdx.x * 256 + threadIdx.x, row = u / C;
+    const int d = 4 * (int)(u % C);
+    if (row >= rows) return;
+    float m = -INFINITY, l = 0.f;
+    float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int z = 0; z < splits; z += Z) {
+        float2 w[Z];
+        float4 v[Z];
+        float top = m;
+#pragma unroll
+        for (int i = 0; i < Z; i++) {
+            const size_t at = (size_t)min(z + i, splits - 1) * rows + row;
+            w[i] = ml[at];
+            v[i] = *reinterpret_cast<const float4 *>(part + at * HD + d);
+        }
+#pragma unroll
+        for (int i = 0; i < Z; i++) top = fmaxf(top, w[i].x);
+        const float mf = finite(top), al = __builtin_amdgcn_exp2f(m - mf);
+        m = top;
+        a.x *= al, a.y *= al, a.z *= al, a.w *= al, l *= al;
+#pragma unroll
+        for (int i = 0; i < Z; i++) {
+            const float f = z + i < splits ? __builtin_amdgcn_exp2f(w[i].x - mf) * w[i].y : 0.f;
+            if (z + i < splits) a.x = fmaf(f, v[i].x, a.x), a.y = fmaf(f, v[i].y, a.y), a.z = fmaf(f, v[i].z, a.z), a.w = fmaf(f, v[i].w, a.w);
+            l += f;
+        }
+    }
+    *reinterpret_cast<float4 *>(out + row * HD + d) = make_float4(a.x / l, a.y / l, a.z / l, a.w / l);
+}
+
 }  // namespace
 
 hipError_t launch_kv8_attention(const Kv8Attn &a, int cus, hipStream_t s) {
@@ -649,14 +683,19 @@ hipError_t launch_kv8_attention(const Kv8Attn &a, int cus, hipStream_t s) {
         const uint32_t seen = a.window && a.window <= a.position ? a.window : a.position + 1;  // of the first query
         splits = std::min({(uint64_t)cus / wgs, (uint64_t)seen / (4 * kKv8Block), (uint64_t)kMaxSplits});
     } else {
-        // the split count whose estimated time is least, in us: the longest workgroup's tiles, in rounds of as many
-        // workgroups as are resident, and the join's launch and traffic
+        // The split count whose estimated time is least, in us: the longest workgroup's tiles (2.2 of head size 128,
+        // 3.4 where two workgroups share a CU), in rounds of as many workgroups as are resident, and the join's launch
+        // and traffic.  (Longest range: the splits of a workgroup with a shorter one are shorter, or empty.  300 queries
+        // of 32 heads, 8 of them kv heads, after 4000: 1 split 158 us, 3 70.6, 6 62.9, 16 77.2; taken: 6.)
         const uint64_t last = (uint64_t)a.position + a.queries, range = a.window ? std::min(last, (uint64_t)a.window + qn) : last;
-        const double tiles = (double)(range / 64 + 1), tile = 0.5 + 1.4 * a.c.hd / 128, resident = (a.c.hd <= 128 ? 2.0 : 1.0) * cus;
+        const double tiles = (double)(range / 64 + 1), size = 0.25 + 0.75 * a.c.hd / 128;
+        const uint64_t per_cu = a.c.hd <= 128 ? 2 : 1;
         double best = 1e300;
-        for (uint64_t n = 1; n <= (uint64_t)kMaxSplits && 2 * n <= (uint64_t)tiles + 1; n++) {
-            const double t = std::ceil(wgs * n / resident) * std::ceil(tiles / n) * tile + (n > 1 ? 4.0 + n * (double)total * a.c.hd * 8 / 3e6 : 0.0);
-            if (t < best * 0.97) best = t, splits = n;
+        for (uint64_t n = 1; n <= (uint64_t)kMaxSplits && n <= (uint64_t)tiles; n++) {
+            const double tile = size * (wgs * n > (uint64_t)cus && per_cu == 2 ? 3.4 : 2.2);
+            const double t = (double)((wgs * n + per_cu * cus - 1) / (per_cu * cus)) * std::ceil(tiles / n) * tile +
+                             (n > 1 ? 2.5 + n * (double)total * a.c.hd * 8 / 4e6 : 0.0);
+            if (t < best * 0.98) best = t, splits = n;
         }
     }
     while (splits > 1 && splits * total * (a.c.hd + 2) > a.part_floats) splits--;
@@ -672,9 +711,13 @@ hipError_t launch_kv8_attention(const Kv8Attn &a, int cus, hipStream_t s) {
             if (nr == 32) hipLaunchKernelGGL((kv8_few_kernel<HD, 32>), grid, dim3(256), 0, s, p);
             else hipLaunchKernelGGL((kv8_few_kernel<HD, 48>), grid, dim3(256), 0, s, p);
         }
-        if (p.splits > 1)
-            hipLaunchKernelGGL(kv8_join_kernel<HD>, dim3((unsigned)total), dim3(256), 0, s, p.part, (const float2 *)p.part_ml, p.out,
-                               (size_t)total, p.splits);
+        if (p.splits == 1) return;
+        const float2 *ml = (const float2 *)p.part_ml;
+        if (total < 1024)  // (860 queries x 6 heads, 5 splits: 23.3 us a pass with a workgroup per row, 17.8 with a thread per four dims)
+            hipLaunchKernelGGL(kv8_join_kernel<HD>, dim3((unsigned)total), dim3(256), 0, s, p.part, ml, p.out, (size_t)total, p.splits);
+        else
+            hipLaunchKernelGGL(kv8_join_rows_kernel<HD>, dim3((unsigned)((total * (HD / 4) + 255) / 256)), dim3(256), 0, s, p.part, ml,
+                               p.out, (size_t)total, p.splits);
     };
     switch (a.c.hd) {
     case 64: go(std::integral_constant<int, 64>{}); break;

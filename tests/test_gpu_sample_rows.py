@@ -86,6 +86,23 @@ def test_ties(hip_ctx, kw):
     check(hip_ctx, x, np.array([0.013, 0.77, 0.35617, 0.6113]), kw)
 
 
+@pytest.mark.parametrize("kw", [k for k in POLICIES if k.get("temperature", 1) > 0], ids=str)
+def test_thousands_of_equal_or_near_logits(hip_ctx, kw):
+    """Rows whose finest bins hold more than a thousand logits: all equal; quarters; thousands of different values
+    within a billionth of the range; the same beside higher ones, with equal ones among them."""
+    rng = np.random.default_rng(53)
+    n = 60000
+    x = np.zeros((5, n), np.float32)
+    x[0] = 2.5
+    x[1] = np.rint(rng.normal(0, 2, n) * 4) / 4
+    x[2] = np.where(rng.random(n) < 0.5, 0.01 * (1 + 1e-4 * rng.random(n)), -10)
+    x[3] = np.where(rng.random(n) < 0.7, np.rint(rng.random(n) * 40) * 1e-7, -8)
+    x[3, rng.integers(0, n, 300)] = 3 + rng.random(300)
+    x[4] = np.where(rng.random(n) < 0.3, -1.0, np.where(rng.random(n) < 0.5, 1.0, 1.0 + 2.0 ** -23))
+    for u in ([0.02, 0.5, 0.31, 0.77, 0.64], [0.97, 0.11, 0.9, 0.4, 0.05]):
+        check(hip_ctx, x, np.array(u), kw)
+
+
 @pytest.mark.parametrize("kw", POLICIES, ids=str)
 def test_masked_logits(hip_ctx, kw):
     """-infinity where a grammar forbids a token: all but one, all but two, half of them."""

@@ -12,8 +12,9 @@
 //   finish  a workgroup per row: the bin in which a target lies, then 1024 finer bins of that bin's
 //           logits, then the few logits of the finer bin in order.  With top-k the bins above the k-th
 //           logit are sorted in LDS instead, and everything else is prefix sums of at most 1024.
-// A row whose fine bin (or whose bins above the k-th) hold more than LDS does -- thousands of equal
-// logits -- goes digit by digit of the key through the whole row instead.
+// Where a finer bin holds more logits than that -- a thousand equal ones, or nearly -- its logits' values
+// go digit by digit, and equal ones by the counts of their slices.  (128256 logits rounded to quarters,
+// nucleus of 0.9: 50 us; all equal: 0.52 ms.)
 #include "zh_longctx.h"
 
 namespace zh {
@@ -21,7 +22,7 @@ namespace zh {
 namespace {
 
 constexpr int kSliceLogits = 2048, kBins = 256, kFine = 1024, kThreads = 1024, kMaxSlices = 262144 / kSliceLogits;
-constexpr int kTopKMax = 1024, kList = 4096;  // candidates of a limited row, logits sorted in LDS
+constexpr int kList = 4096;  // logits sorted in LDS (top-k: at most 1024 of them are candidates)
 
 typedef unsigned long long u64;
 
@@ -242,7 +243,7 @@ struct Finish {
     u64 wave[kThreads / 64];
     uint32_t seen[262144 / 32];   // recent tokens
     u64 value;
-    uint32_t found, count;
+    uint32_t found, count, least, most;
     Key key[kThreads / 64];
 };
 
@@ -321,40 +322,9 @@ __device__ void sort_list(Finish &f, uint32_t n) {
         }
 }
 
-// The first element, in descending order of key(i), at which the sum of weight(i) reaches target (1 ..
-// the whole sum); *before: the sum of those ahead of it.  Digit by digit, whatever the row.
-template <class K, class W>
-__device__ Key reach(Finish &f, uint32_t n, u64 target, u64 *before, K key, W weight) {
-    Key b{};
-    u64 done = 0;
-    for (int d = 0; d < 12; d++) {
-        const int word = d / 4, shift = 24 - 8 * (d % 4);
-        __syncthreads();
-        if (threadIdx.x < 256) f.sums[threadIdx.x] = 0;
-        __syncthreads();
-        for (uint32_t i = threadIdx.x; i < n; i += kThreads) {
-            const Key k = key(i);
-            bool in = true;
-            for (int j = 0; j < 3; j++) {
-                const uint32_t mask = j < word ? 0xFFFFFFFFu : j > word || shift == 24 ? 0u : 0xFFFFFFFFu << (shift + 8);
-                in = in && ((k.w[j] ^ b.w[j]) & mask) == 0;
-            }
-            const u64 w = in ? weight(i) : 0;
-            if (w) atomicAdd(&f.sums[k.w[word] >> shift & 255u], w);
-        }
-        __syncthreads();
-        const u64 v = threadIdx.x < 256 ? f.sums[255 - threadIdx.x] : 0;
-        u64 total, ahead;
-        const u64 run = prefix(f, v, &total);
-        b.w[word] |= (255 - first_reaching(f, run, v, target - done, &ahead)) << shift;
-        done += ahead;
-    }
-    *before = done;
-    return b;
-}
-
 template <class K> __device__ Key largest(Finish &f, uint32_t n, K key) {
     Key k{};
+#pragma unroll 8
     for (uint32_t i = threadIdx.x; i < n; i += kThreads) {
         const Key c = key(i);
         if (at_least(c, k)) k = c;
@@ -447,8 +417,107 @@ __global__ void __launch_bounds__(kThreads) draw_finish_kernel(SampleRows p) {
         return v;
     };
 
+    // The logit at which the sum of weights reaches target, in descending order (equal logits: of ascending ids), as
+    // its key, value and complement of the id; *upto: the sum with it.  c: this thread's bin's sum, run: with those of
+    // the bins before.
+    auto find = [&](auto weight, u64 c, u64 run, u64 target, u64 *upto) {
+        u64 ahead, fine_ahead, all;
+        const int bin = (int)first_reaching(f, run, c, target, &ahead);
+        __syncthreads();
+        f.sums[tid] = 0;
+        __syncthreads();
+        of_bins(w, slices, bin, bin, [&](float a, uint32_t) {
+            float t;
+            bin_of(a, top, per_bin, t);
+            atomicAdd(&f.sums[fine_of(t, bin)], weight(a));
+        });
+        __syncthreads();
+        const u64 v = f.sums[tid], r = prefix(f, v, &all);
+        const int fine = (int)first_reaching(f, r, v, target - ahead, &fine_ahead);
+        __syncthreads();
+        if (tid == 0) f.count = 0, f.least = 0xFFFFFFFFu, f.most = 0;
+        __syncthreads();
+        // take(value, id) for the logits of the finer bin
+        auto of_fine = [&](auto take) {
+            of_bins(w, slices, bin, bin, [&](float a, uint32_t i) {
+                float t;
+                bin_of(a, top, per_bin, t);
+                if (fine_of(t, bin) == fine) take(ordered(a), i);
+            });
+        };
+        uint32_t lo = 0xFFFFFFFFu, hi = 0;
+        of_fine([&](uint32_t o, uint32_t i) {
+            lo = min(lo, o), hi = max(hi, o);
+            const uint32_t at = atomicAdd(&f.count, 1u);
+            if (at < kThreads) f.list[at] = (u64)o << 32 | (uint32_t)~i;
+        });
+        __syncthreads();
+        const uint32_t m = f.count;
+        u64 need = target - ahead - fine_ahead, last;
+        *upto = ahead + fine_ahead;
+        if (m <= kThreads) {
+            __syncthreads();
+            sort_list(f, m);
+            const u64 mine = tid < m ? f.list[tid] : 0;
+            const u64 wt = tid < m ? weight(unordered((uint32_t)(mine >> 32))) : 0;
+            const u64 rr = prefix(f, wt, &all);
+            const u64 key = f.list[first_reaching(f, rr, wt, need, &last)];
+            *upto += last + weight(unordered((uint32_t)(key >> 32)));
+            __syncthreads();
+            return key;
+        }
+        // the value: its digits, but for those that all of them share
+        atomicMin(&f.least, lo);
+        atomicMax(&f.most, hi);
+        __syncthreads();
+        uint32_t value = f.most;
+        const uint32_t differ = f.least ^ f.most;
+        for (int shift = 24; shift >= 0; shift -= 8) {
+            if (differ >> shift == 0) continue;  // (uniform)
+            value = value >> (shift + 8 < 32 ? shift + 8 : 31) >> (shift + 8 < 32 ? 0 : 1);  // the digits above
+            __syncthreads();
+            f.sums[tid] = 0;
+            __syncthreads();
+            of_fine([&](uint32_t o, uint32_t) {
+                const uint32_t above = shift == 24 ? 0 : o >> (shift + 8);
+                if (above == value) atomicAdd(&f.sums[255 - (o >> shift & 255u)], weight(unordered(o)));
+            });
+            __syncthreads();
+            const u64 s = f.sums[tid], q = prefix(f, s, &all);
+            value = (value << 8 | (255 - first_reaching(f, q, s, need, &last))) << shift;
+            need -= last, *upto += last;
+        }
+        // equal logits: the rank among them, by the slices' counts and then the ids of one slice
+        const u64 one = weight(unordered(value)), rank = (need + one - 1) / one;
+        __syncthreads();
+        f.sums[tid] = 0;
+        __syncthreads();
+        of_fine([&](uint32_t o, uint32_t i) {
+            if (o == value) atomicAdd(&f.sums[i / kSliceLogits], 1ull);
+        });
+        __syncthreads();
+        const u64 s = f.sums[tid], q = prefix(f, s, &all);
+        const uint32_t slice = first_reaching(f, q, s, rank, &last);
+        uint32_t *bits = reinterpret_cast<uint32_t *>(f.list);
+        __syncthreads();
+        if (tid < kSliceLogits / 32) bits[tid] = 0;
+        __syncthreads();
+        of_fine([&](uint32_t o, uint32_t i) {
+            if (o == value && i / kSliceLogits == slice) atomicOr(&bits[i % kSliceLogits / 32], 1u << (i % 32));
+        });
+        __syncthreads();
+        uint32_t word = tid < kSliceLogits / 32 ? bits[tid] : 0;
+        const u64 set = __popc(word), upto_word = prefix(f, set, &all);
+        u64 ahead_of_word;
+        const uint32_t at = first_reaching(f, upto_word, set, rank - last, &ahead_of_word);
+        word = bits[at];
+        for (u64 k = rank - last - ahead_of_word; k > 1; k--) word &= word - 1;
+        *upto += rank * one;
+        __syncthreads();
+        return (u64)value << 32 | (uint32_t)~(slice * kSliceLogits + 32 * at + (uint32_t)__ffs((int)word) - 1);
+    };
+
     if (policy.limited) {
-        auto by_raw = [&](uint32_t i) { return Key{{ordered(x[i]), ~i, 0}}; };
         const u64 c = sum_bins(), run = prefix(f, c, &total);
         const uint32_t k = (uint32_t)(total < policy.top_k ? total : policy.top_k);  // candidates above -infinity
         const uint32_t last = first_reaching(f, run, c, k, &before);
@@ -462,13 +531,16 @@ __global__ void __launch_bounds__(kThreads) draw_finish_kernel(SampleRows p) {
         __syncthreads();
         uint32_t m = f.count;
         __syncthreads();
-        if (m > kList) {  // thousands of logits about the k-th: the k-th by its digits, then those down to it
-            const Key end = reach(f, n, k, &before, by_raw, [&](uint32_t i) { return x[i] > -INFINITY ? 1ull : 0ull; });
+        if (m > kList) {  // thousands of logits about the k-th: those down to it alone
+            u64 upto;
+            const u64 end = find([](float) { return 1ull; }, c, run, k, &upto);
             __syncthreads();
             if (tid == 0) f.count = 0;
             __syncthreads();
-            for (uint32_t i = tid; i < n; i += kThreads)
-                if (x[i] > -INFINITY && at_least(by_raw(i), end)) f.list[atomicAdd(&f.count, 1u)] = (u64)ordered(x[i]) << 32 | (uint32_t)~i;
+            of_bins(w, slices, 0, last, [&](float v, uint32_t i) {
+                const u64 key = (u64)ordered(v) << 32 | (uint32_t)~i;
+                if (key >= end) f.list[atomicAdd(&f.count, 1u)] = key;
+            });
             __syncthreads();
             m = k;
         }
@@ -526,55 +598,10 @@ __global__ void __launch_bounds__(kThreads) draw_finish_kernel(SampleRows p) {
     }
 
     const u64 c = sum_bins(), run = prefix(f, c, &total);
-    auto by_logit = [&](uint32_t i) { return Key{{ordered(logit(i)), ~i, 0}}; };
-    // The logit at which the sum reaches target, as its key (value, then lowest id); *upto: the sum with it.
-    auto find = [&](u64 target, u64 *upto) {
-        u64 ahead, fine_ahead, all;
-        const int bin = (int)first_reaching(f, run, c, target, &ahead);
-        __syncthreads();
-        f.sums[tid] = 0;
-        __syncthreads();
-        of_bins(w, slices, bin, bin, [&](float a, uint32_t) {
-            float t;
-            bin_of(a, top, per_bin, t);
-            atomicAdd(&f.sums[fine_of(t, bin)], policy.weight(a, top));
-        });
-        __syncthreads();
-        const u64 v = f.sums[tid], r = prefix(f, v, &all);
-        const int fine = (int)first_reaching(f, r, v, target - ahead, &fine_ahead);
-        __syncthreads();
-        if (tid == 0) f.count = 0;
-        __syncthreads();
-        of_bins(w, slices, bin, bin, [&](float a, uint32_t i) {
-            float t;
-            bin_of(a, top, per_bin, t);
-            if (fine_of(t, bin) != fine) return;
-            const uint32_t at = atomicAdd(&f.count, 1u);
-            if (at < kThreads) f.list[at] = (u64)ordered(a) << 32 | (uint32_t)~i;
-        });
-        __syncthreads();
-        const uint32_t m = f.count;
-        __syncthreads();
-        if (m > kThreads) {
-            u64 b;
-            const Key k = reach(f, n, target, &b, by_logit, [&](uint32_t i) { return policy.weight(logit(i), top); });
-            *upto = b + policy.weight(unordered(k.w[0]), top);
-            return (u64)k.w[0] << 32 | k.w[1];
-        }
-        sort_list(f, m);
-        const u64 mine = tid < m ? f.list[tid] : 0;
-        const u64 wt = tid < m ? policy.weight(unordered((uint32_t)(mine >> 32)), top) : 0;
-        const u64 rr = prefix(f, wt, &all);
-        u64 last;
-        const uint32_t at = first_reaching(f, rr, wt, target - ahead - fine_ahead, &last);
-        const u64 key = f.list[at];
-        *upto = ahead + fine_ahead + last + policy.weight(unordered((uint32_t)(key >> 32)), top);
-        __syncthreads();
-        return key;
-    };
+    auto weight = [&](float a) { return policy.weight(a, top); };
     u64 upto;
-    find(target_of((double)p.o.top_p, total), &upto);
-    const u64 key = find(target_of(u, upto), &upto);
+    find(weight, c, run, target_of((double)p.o.top_p, total), &upto);
+    const u64 key = find(weight, c, run, target_of(u, upto), &upto);
     answer(~(uint32_t)key);
 }
 

@@ -64,6 +64,17 @@ __device__ __forceinline__ void load8(const float *q, int aligned, float (&v)[8]
     }
 }
 
+// the z-th of `parts` shares of 0 .. n - 1, the first n % parts of them one longer
+__device__ __forceinline__ void share(uint32_t n, uint32_t parts, uint32_t z, uint32_t &begin, uint32_t &end) {
+    if (parts == 1) {
+        begin = 0, end = n;
+        return;
+    }
+    const uint32_t each = n / parts, more = n - each * parts;
+    begin = each * z + min(z, more);
+    end = begin + each + (z < more ? 1u : 0u);
+}
+
 __device__ __forceinline__ float finite(float v) { return v == -INFINITY ? 0.f : v; }
 
 // two weights' pieces
@@ -132,8 +143,9 @@ __global__ void __launch_bounds__(256, 1) kv8_few_kernel(Kv8Params p) {
     const uint32_t pos_min = p.position + p.query_of(r0), pos_max = p.position + p.query_of(rlast);
     const uint32_t lo_min = first_seen(pos_min, p.window), lo_max = first_seen(pos_max, p.window);
     const uint32_t b_first = lo_min / kKv8Block, nb_all = pos_max / kKv8Block - b_first + 1;
-    const uint32_t b0 = b_first + (uint32_t)((uint64_t)nb_all * z / p.splits);
-    const uint32_t b1 = b_first + (uint32_t)((uint64_t)nb_all * (z + 1) / p.splits);
+    uint32_t b0, b1;
+    share(nb_all, (uint32_t)p.splits, (uint32_t)z, b0, b1);
+    b0 += b_first, b1 += b_first;
     const int nb = (int)(b1 - b0) > wave ? (int)((b1 - b0 - wave + 3) / 4) : 0;  // of this wavefront: b0 + wave + 4 t
 
     const size_t head0 = (size_t)kvh * p.c.blocks;
@@ -385,7 +397,9 @@ template <int HD> __global__ void __launch_bounds__(256, kManyPerCu<HD>) kv8_man
     const int q0 = qb * qn, qlast = min(q0 + qn, (int)p.queries) - 1;
     const uint32_t kv_last = p.position + qlast, kv_first = first_seen(p.position + q0, p.window);
     const int t_first = (int)(kv_first >> 6), nt_all = (int)(kv_last >> 6) + 1 - t_first;
-    const int t0 = t_first + (int)((int64_t)nt_all * z / p.splits), t1 = t_first + (int)((int64_t)nt_all * (z + 1) / p.splits);
+    uint32_t s0, s1;
+    share((uint32_t)nt_all, (uint32_t)p.splits, (uint32_t)z, s0, s1);
+    const int t0 = t_first + (int)s0, t1 = t_first + (int)s1;
     const int v = wave * 32 + l32, vq = (int)p.query_of(v), qi = q0 + vq, vh = v - vq * p.group, head = kvh * p.group + vh;
     const bool valid = v < qn * p.group && qi <= qlast;
     const int qc = min(qi, qlast);

@@ -132,3 +132,100 @@ def test_same_bits_each_time(hip_ctx, queries):
         hip_ctx.kv8_attention(cache, qb, out, 32, 0, 3000, queries)
     hip_ctx.commit()
     assert np.array_equal(out.read().view(np.uint32), first.view(np.uint32))
+
+
+def held(ctx, c, q, position, window=0):
+    queries, heads, hd = q.shape
+    cache = upload(ctx, [c], c.scales[0].shape[1] * 32)
+    out = ctx.empty(q.nbytes)
+    ctx.kv8_attention(cache, ctx.buffer(q), out, heads, 0, position, queries, window=window)
+    return out.read().reshape(q.shape)
+
+
+@pytest.mark.parametrize("garbage", [np.inf, -np.inf, 3e38, -3e38, -1.0, 0.0])
+@pytest.mark.parametrize("heads,kvh,hd", [(8, 2, 128), (4, 4, 64), (2, 1, 256)])
+def test_any_scale_out_of_the_window(hip_ctx, heads, kvh, hd, garbage):
+    """Scales that were never stored, ahead of the window and behind the queries."""
+    for position, queries, window in ((200, 1, 40), (200, 5, 40), (2048 + 97, 70, 65), (290, 140, 33)):
+        print("garbage", garbage, heads, hd, position, queries, window, flush=True)
+        rng = np.random.default_rng(position)
+        n = position + queries
+        c = oracle.Kv8(kvh, n + 70, hd, rng)
+        for w in range(2):
+            c.scales[w][:, :(position + 1 - window) // 32] = garbage
+            c.scales[w][:, (n - 1) // 32 + 1:] = garbage
+        q = rng.normal(0, 1, (queries, heads, hd)).astype(np.float32)
+        want, bound = oracle.kv8_attention(c, q, position, hd ** -0.5, window)
+        err = np.abs(held(hip_ctx, c, q, position, window) - want)
+        assert np.all(err <= bound), (err / bound).max()
+
+
+@pytest.mark.parametrize("heads,kvh,hd", [(8, 2, 128), (4, 4, 64), (6, 3, 96), (2, 1, 256)])
+@pytest.mark.parametrize("position,queries", [(60, 5), (70, 9), (3000, 9), (9, 200), (1500, 150)])
+@pytest.mark.parametrize("large", [2.0 ** 26, 2.0 ** 100])
+def test_values_of_later_positions_stay_out_of_earlier_rows(hip_ctx, heads, kvh, hd, position, queries, large):
+    """V of the last blocks, which the first queries don't see, is far larger than the others'.  (The bound is of
+    each row's own largest value; a factor of 2^-32 and more goes another way than 2^-26, whose log2 is held to 2^-19:
+    the rows without the large ones are off by another ln 2 times that.)"""
+    print("later values", heads, kvh, hd, position, queries, large, flush=True)
+    rng = np.random.default_rng(position + hd)
+    n = position + queries
+    c = oracle.Kv8(kvh, n, hd, rng)
+    first = (position + queries // 2) // 32 + 1
+    c.scales[1][:, first:] *= np.float32(large)
+    q = rng.normal(0, 1, (queries, heads, hd)).astype(np.float32)
+    want, bound = oracle.kv8_attention(c, q, position, hd ** -0.5)
+    bound = bound * (1 + 2.0 ** -19 / 2.0 ** -20)
+    err = np.abs(held(hip_ctx, c, q, position) - want)
+    assert np.all(err <= bound), (err / bound).max()
+
+
+@pytest.mark.parametrize("heads,kvh,hd", [(8, 2, 128), (4, 4, 64), (6, 3, 96), (2, 1, 256)])
+@pytest.mark.parametrize("position,queries", [(500, 1), (9000, 1), (500, 9), (2500, 12), (400, 150), (1500, 40)])
+def test_large_values_of_no_weight(hip_ctx, heads, kvh, hd, position, queries):
+    """A block of values 2^110 times the others', whose keys score hundreds below them, and one of values 2^-100
+    times theirs.  Bound: the weights' relative errors (longctx_oracle) times the sum of weight x |value|."""
+    print("weightless values", heads, kvh, hd, position, queries, flush=True)
+    rng = np.random.default_rng(position + hd)
+    n = position + queries
+    c = oracle.Kv8(kvh, n, hd, rng)
+    q = np.abs(rng.normal(0, 1, (queries, heads, hd))).astype(np.float32) + np.float32(0.5)
+    c.codes[0][:, 64:96] = -127
+    c.scales[0][:, 2] = 2.0
+    c.scales[1][:, 2] *= np.float32(2.0 ** 110)
+    c.scales[1][:, 4] *= np.float32(2.0 ** -100)
+    c.scales[1][:, 6] = 0
+    c.codes[1][:, 192:224] = 0
+    want, _ = oracle.kv8_attention(c, q, position, hd ** -0.5)
+    got = held(hip_ctx, c, q, position)
+    group = heads // kvh
+    scale = float(np.float32(hd ** -0.5))
+    for h in range(heads):
+        k = c.codes[0][h // group].astype(np.float64)[:n]
+        ks = np.repeat(c.scales[0][h // group].astype(np.float64), 32)[:n]
+        v = np.abs(c.codes[1][h // group].astype(np.float64)[:n] * np.repeat(c.scales[1][h // group].astype(np.float64), 32)[:n, None])
+        for i in range(queries):
+            p = position + i + 1
+            s = (k[:p] @ q[i, h].astype(np.float64)) * ks[:p] * scale
+            e = (hd + 8) * 2.0 ** -23 * ((np.abs(k[:p]) @ np.abs(q[i, h]).astype(np.float64)) * ks[:p] * scale)
+            # an error counts with the weight of its own position; the most of a weight below 2^-60 of the largest is 0
+            w = np.exp(s - s.max())
+            live = w > 2.0 ** -60
+            bound = (2 * e[live].max() + 2.0 ** -20 + p * 2.0 ** -22) * (w[live] @ v[:p][live]) / w.sum()
+            err = np.abs(got[i, h] - want[i, h])
+            assert np.all(err <= bound), (h, i, (err / bound).max())
+
+
+@pytest.mark.parametrize("queries", [1, 9, 80])
+@pytest.mark.parametrize("power", [-125, -110, 100])
+def test_values_near_the_ends_of_the_range(hip_ctx, queries, power):
+    """Scales of 2^power: outputs are scaled by it, to a step, but for what falls below 2^-126 (16 roundings of half
+    of 2^-149 at most: a sum and its share by each of four wavefronts, and of four splits)."""
+    rng = np.random.default_rng(power + 1000)
+    c = oracle.Kv8(2, 300, 64, rng)
+    q = rng.normal(0, 1, (queries, 4, 64)).astype(np.float32)
+    plain = held(hip_ctx, c, q, 200)
+    c.scales[1] *= np.float32(2.0 ** power * 64)
+    got = held(hip_ctx, c, q, 200)
+    want = plain.astype(np.float64) * 2.0 ** power * 64
+    assert np.all(np.abs(got - want) <= 2.0 ** -23 * np.abs(want) + 16 * 2.0 ** -150)

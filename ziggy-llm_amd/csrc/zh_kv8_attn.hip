@@ -11,6 +11,12 @@
 // positions, K and V straight from memory into operands.  Many (prompts): a workgroup's 128 rows share
 // tiles of 64 positions in LDS.  Both split the positions over workgroups where rows alone leave CUs
 // idle; a second launch joins the splits in their order, so results don't change from run to run.
+//
+// What bounds them (32 heads of 128 over 8 kv heads): one query of 131071 positions memory, 268 MB in 47.6
+// us, 5.6 TB/s, and 4.4 of the join; of 4113 positions the chain of loads, products and exchange (7.0 us,
+// of which 1.5 are its one block, and 2.2 of the join); 9 queries of 16398 positions vector issue and memory
+// about alike (22.3 and 3.9); 2048 queries of 14336 to 16384 positions the matrix cores, 936 us, 1.10 PFLOP/s
+// with both pieces counted.
 #include <algorithm>
 #include <cmath>
 
@@ -85,10 +91,10 @@ __device__ __forceinline__ void pieces(float a, float b, uint32_t &hi, uint32_t 
 }
 
 // A block's V scale as a share of the largest: its log2 goes into the weights' exponent, w = 2^(s +
-// log2 share - max), and the weights over the share add to the sum.  Shares below 2^-60, an all-zero
-// block's among them, count as 2^-60: their values are below what the largest one's rounding leaves,
-// and the sum keeps their weight.  (A multiplication of a block's outputs instead would be an FMA per
-// output and block.)
+// log2 share - max), and the weights over the share add to the sum.  (A multiplication of a block's
+// outputs instead would be an FMA per output and block.)  An all-zero block, whose codes are 0, counts as
+// a share of 2^-60: the sum keeps its weights.  Other shares are at least 2^-32 here (their log2 is held
+// to 2^-19): see plain_row.
 __device__ __forceinline__ void share_of(float scale, float big, float &log_share, float &inverse) {
     const float share = scale / big;
     log_share = big > 0.f ? __builtin_amdgcn_logf(share < 0x1p-60f ? 0x1p-60f : share) : 0.f * scale;
@@ -107,6 +113,57 @@ struct Kv8Params {
     float qscale;
 };
 
+// Scales of V, the largest and the smallest that is not 0, too far apart for weights that hold them in
+// their exponent: a row may see the small ones only, or give the large ones next to no weight.
+__device__ __forceinline__ bool far_apart(float largest, float smallest) { return !(smallest >= largest * 0x1p-32f); }
+constexpr float kNoScale = INFINITY;  // the smallest of none
+__device__ __forceinline__ float wave_min_scale(float scale) { return -wave_max_f32(scale > 0.f ? -scale : -kNoScale); }
+
+// One row by a wavefront in plain binary32, for such scales alone: blocks b, b + step, .. below `end`, a
+// position (half its dims) a lane for the scores, a dim a lane for the output.  acc[i]: the unnormalised
+// output of dim lane + 64 i.
+template <int HD>
+__device__ __forceinline__ void plain_row(const Kv8Params &p, int kvh, const float *q, uint32_t pos, uint32_t b, uint32_t end,
+                                          uint32_t step, float &m, float &l, float (&acc)[(HD + 63) / 64]) {
+    const int lane = threadIdx.x & 63, half = lane >> 5, at32 = lane & 31;
+    const size_t head0 = (size_t)kvh * p.c.blocks;
+    const uint32_t lo = first_seen(pos, p.window);
+    m = -INFINITY, l = 0.f;
+#pragma unroll
+    for (int i = 0; i < (HD + 63) / 64; i++) acc[i] = 0.f;
+#pragma unroll 1
+    for (; b < end; b += step) {
+        const uint32_t first = b * kKv8Block, at = first + at32;
+        if (first > pos || first + kKv8Block - 1 < lo) continue;
+        const float ks = p.c.ks[head0 + b], vs = p.c.vs[head0 + b];
+        const int8_t *kc = p.c.kc + (head0 + b) * (kKv8Block * HD) + at32 * HD + half * (HD / 2);
+        float s = 0.f;
+#pragma unroll 1
+        for (int d = 0; d < HD / 2; d += 4) {
+            const uint32_t c = *reinterpret_cast<const uint32_t *>(kc + d);
+#pragma unroll
+            for (int j = 0; j < 4; j++) s = fmaf(q[half * (HD / 2) + d + j] * p.qscale, (float)(int8_t)(c >> 8 * j), s);
+        }
+        const bool in = at >= lo && at <= pos;
+        s = in ? xsum<32>(s) * ks : -INFINITY;
+        const float mn = fmaxf(m, wave_max_f32(s)), al = __builtin_amdgcn_exp2f(m - finite(mn));
+        const float w = in ? __builtin_amdgcn_exp2f(s - finite(mn)) : 0.f;
+        m = mn, l *= al;
+#pragma unroll
+        for (int i = 0; i < (HD + 63) / 64; i++) acc[i] *= al;
+#pragma unroll 1
+        for (int j = 0; j < kKv8Block; j++) {
+            const float wj = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(w), j));
+            l += wj;
+#pragma unroll
+            for (int i = 0; i < (HD + 63) / 64; i++) {
+                const int d = min(lane + 64 * i, HD - 1);
+                acc[i] = fmaf(wj, (float)p.c.vc[(head0 + b) * (kKv8Block * HD) + d * kKv8Block + j] * vs, acc[i]);
+            }
+        }
+    }
+}
+
 // ---- few rows ----
 //
 // A wavefront takes blocks of 32 positions (4 wavefronts of a workgroup in turn).  Scores on
@@ -123,7 +180,6 @@ template <int HD, int NR> struct Few {
     static constexpr int KB = HD % 64 ? 8 : 16;        // bytes of a lane's K load
     static constexpr int KL = HD / 4 / KB;             // K loads of a row
     static constexpr int KW = KB / 4;
-
 };
 template <int HD> struct Block8 {
     uint32_t k[2][HD / 16], v[HD / 16][2];
@@ -164,7 +220,7 @@ __global__ void __launch_bounds__(256, 1) kv8_few_kernel(Kv8Params p) {
     };
     // of the wavefront's next 64 blocks, one a lane: the K scale, log2 of the V scale's share of `big` (the
     // largest V scale so far), and the share's inverse
-    float ksl = 0.f, vsl = 0.f, lvl = 0.f, inl = 0.f, big = 0.f;
+    float ksl = 0.f, vsl = 0.f, lvl = 0.f, inl = 0.f, big = 0.f, small = kNoScale;
     auto load_scales = [&](int t) {
         const uint32_t b = block_of(t + lane);
         ksl = p.c.ks[head0 + b], vsl = p.c.vs[head0 + b];
@@ -235,7 +291,9 @@ __global__ void __launch_bounds__(256, 1) kv8_few_kernel(Kv8Params p) {
             }
             big = next;
         }
+        small = fminf(small, wave_min_scale(vsl));
         share_of(vsl, big, lvl, inl);
+        return !far_apart(big, small);
     };
 
     auto compute = [&](const Block8<HD> &r, int t) {
@@ -324,10 +382,14 @@ __global__ void __launch_bounds__(256, 1) kv8_few_kernel(Kv8Params p) {
         }
     };
 
+    bool together = true;
     if (nb > 0) {
-        take_scales();
-        for (int t = 0; t < nb; t += 2) {
-            if (t && (t & 63) == 0) load_scales(t), take_scales();
+        together = take_scales();
+        for (int t = 0; t < nb && together; t += 2) {
+            if (t && (t & 63) == 0) {
+                load_scales(t);
+                together = take_scales();
+            }
             compute(x, t);
             load(x, t + 2);
             if (t + 1 < nb) compute(y, t + 1);
@@ -335,18 +397,31 @@ __global__ void __launch_bounds__(256, 1) kv8_few_kernel(Kv8Params p) {
         }
     }
     // the wavefront's rows: both pieces' outputs, the sum over its lanes
-    const float unit = big * (1.f / kWeight);
+    const uint32_t live = rlast - r0 + 1;
+    if (!together)
+#pragma unroll 1
+        for (uint32_t r = 0; r < live; r++) {
+            const uint32_t qi = p.query_of(r0 + r);
+            const float *q = p.q + (size_t)qi * p.q_stride + (size_t)(kvh * p.group + (int)(r0 + r - qi * p.group)) * HD;
+            float acc[(HD + 63) / 64], mr, lr;
+            plain_row<HD>(p, kvh, q, p.position + qi, b0 + wave, b1, 4, mr, lr, acc);
+#pragma unroll
+            for (int i = 0; i < (HD + 63) / 64; i++)
+                if (lane + 64 * i < HD) os[wave][r][lane + 64 * i] = acc[i];
+            if (lane == 0) ms[wave][r] = mr, ls[wave][r] = lr;
+        }
 #pragma unroll
     for (int c = 0; c < CT; c++) {
+        if (!together) break;
         const float sum = xsum<32>(xsum<16>(l[c]));
 #pragma unroll
         for (int d = 0; d < F::DT; d++)
 #pragma unroll
             for (int j = 0; j < 4; j++) {
                 if constexpr (F::PAIRED) {
-                    if (j % 2 == 0) os[wave][2 * g + j / 2][16 * d + i16] = (o[c][d][j] + o[c][d][j + 1]) * unit;
+                    if (j % 2 == 0) os[wave][2 * g + j / 2][16 * d + i16] = (o[c][d][j] + o[c][d][j + 1]) * (1.f / kWeight) * big;
                 } else
-                    os[wave][16 * c + 4 * g + j][16 * d + i16] = o[c][d][j] * unit;
+                    os[wave][16 * c + 4 * g + j][16 * d + i16] = o[c][d][j] * (1.f / kWeight) * big;
             }
         if (lane < 16 && (!F::PAIRED || lane % 2 == 0)) {
             const int r = F::PAIRED ? lane / 2 : 16 * c + lane;
@@ -354,7 +429,6 @@ __global__ void __launch_bounds__(256, 1) kv8_few_kernel(Kv8Params p) {
         }
     }
     __syncthreads();
-    const uint32_t live = rlast - r0 + 1;
     for (int u = tid; u < (int)live * (HD / 4); u += 256) {
         const int r = u / (HD / 4), d = 4 * (u % (HD / 4));
         const float mx = fmaxf(fmaxf(ms[0][r], ms[1][r]), fmaxf(ms[2][r], ms[3][r])), mf = finite(mx);
@@ -390,7 +464,7 @@ template <int HD> __global__ void __launch_bounds__(256, kManyPerCu<HD>) kv8_man
     constexpr int BUF = 64 * KST + HD * VST;
     constexpr int UN = 4 * HD, NU = (UN + 255) / 256;         // 16-byte pieces of a K or V tile, of a thread
     __shared__ __align__(16) char lds[2 * BUF];
-    __shared__ float top_scale[4];
+    __shared__ float top_scale[4], low_scale[4];
     const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, l32 = lane & 31, lh = lane >> 5;
     const int kvh = blockIdx.x % p.c.nkv, z = blockIdx.y;
     const int qn = 128 / p.group, nqb = ((int)p.queries + qn - 1) / qn, qb = nqb - 1 - (int)blockIdx.x / p.c.nkv;
@@ -408,7 +482,7 @@ template <int HD> __global__ void __launch_bounds__(256, kManyPerCu<HD>) kv8_man
     const uint32_t wave_first = p.position + min(q0 + wave * 32 / p.group, qlast);
     const uint32_t wave_lo = first_seen(p.position + min(q0 + (wave * 32 + 31) / p.group, qlast), p.window);
     const size_t head0 = (size_t)kvh * p.c.blocks;
-    const uint32_t last_block = kv_last / kKv8Block;
+    const uint32_t last_block = kv_last / kKv8Block, first_block = kv_first / kKv8Block;
 
     uint4 kr[NU], vr[NU];
     auto load = [&](int t) {
@@ -445,12 +519,16 @@ template <int HD> __global__ void __launch_bounds__(256, kManyPerCu<HD>) kv8_man
         }
     };
 
-    // the largest V scale in this workgroup's range
-    float big = 0.f;
+    // the largest V scale in this workgroup's range, and the smallest
+    float big = 0.f, small = kNoScale;
     for (int b = 2 * t0 + tid; b < 2 * t1; b += 256)
-        if ((uint32_t)b <= last_block) big = fmaxf(big, p.c.vs[head0 + b]);
-    big = wave_max_f32(big);
-    if (lane == 0) top_scale[wave] = big;
+        if ((uint32_t)b >= first_block && (uint32_t)b <= last_block) {
+            const float scale = p.c.vs[head0 + b];
+            big = fmaxf(big, scale);
+            if (scale > 0.f) small = fminf(small, scale);
+        }
+    big = wave_max_f32(big), small = wave_min_scale(small);
+    if (lane == 0) top_scale[wave] = big, low_scale[wave] = small;
     if (t0 < t1) load(t0);
 
     kh8 qh[KT], ql[KT];
@@ -485,11 +563,31 @@ template <int HD> __global__ void __launch_bounds__(256, kManyPerCu<HD>) kv8_man
     __syncthreads();
     const bool rows_here = wave * 32 < (qlast - q0 + 1) * p.group;  // else the wavefront only fills LDS
     big = fmaxf(fmaxf(top_scale[0], top_scale[1]), fmaxf(top_scale[2], top_scale[3]));
+    small = fminf(fminf(low_scale[0], low_scale[1]), fminf(low_scale[2], low_scale[3]));
+    if (far_apart(big, small)) {
+#pragma unroll 1
+        for (int r = 0; r < 32; r++) {
+            const int at = wave * 32 + r, i = q0 + at / p.group, h = kvh * p.group + at % p.group;
+            if (at >= qn * p.group || i > qlast) break;
+            float acc[(HD + 63) / 64], mr, lr;
+            plain_row<HD>(p, kvh, p.q + (size_t)i * p.q_stride + (size_t)h * HD, p.position + i, 2 * (uint32_t)t0,
+                          min(2 * (uint32_t)t1, last_block + 1), 1, mr, lr, acc);
+            const float n = p.splits > 1 && mr == -INFINITY && lr == 0.f ? 0.f : 1.f / lr;
+            const size_t row = (size_t)i * p.heads + h, to = (size_t)z * p.queries * p.heads + row;
+            float *dst = p.splits > 1 ? p.part + to * HD : p.out + row * HD;
+#pragma unroll
+            for (int k = 0; k < (HD + 63) / 64; k++)
+                if (lane + 64 * k < HD) dst[lane + 64 * k] = acc[k] * n;
+            if (p.splits > 1 && lane == 0) *reinterpret_cast<float2 *>(p.part_ml + 2 * to) = make_float2(mr, lr);
+        }
+        return;
+    }
     const int krow = (l32 & 0x13) | (l32 & 4) << 1 | (l32 & 8) >> 1;
 
     for (int t = t0; t < t1; t++) {
         const uint32_t ba = 2 * (uint32_t)t, bb = min(ba + 1, last_block);
-        const float kscale[2] = {p.c.ks[head0 + ba], p.c.ks[head0 + bb]}, vscale[2] = {p.c.vs[head0 + ba], p.c.vs[head0 + bb]};
+        // (a block ahead of every row's window holds any bytes: its scale counts as 0)
+        const float kscale[2] = {ba < first_block ? 0.f : p.c.ks[head0 + ba], p.c.ks[head0 + bb]}, vscale[2] = {p.c.vs[head0 + ba], p.c.vs[head0 + bb]};
         if (t + 1 < t1) load(t + 1);
         __builtin_amdgcn_sched_barrier(0);
         if (rows_here) {
@@ -580,7 +678,7 @@ template <int HD> __global__ void __launch_bounds__(256, kManyPerCu<HD>) kv8_man
     l = xsum<32>(l);
     if (!valid) return;
     // a split's outputs are those of its own positions (0 where it has none in sight)
-    const float inv = p.splits > 1 && m == -INFINITY && l == 0.f ? 0.f : big / (l * kWeight);
+    const float inv = p.splits > 1 && m == -INFINITY && l == 0.f ? 0.f : 1.f / (l * kWeight);
     const size_t row = (size_t)qi * p.heads + head, at = (size_t)z * p.queries * p.heads + row;
     float *dst = (p.splits > 1 ? p.part + at * HD : p.out + row * HD) + 4 * lh;
 #pragma unroll
@@ -588,7 +686,7 @@ template <int HD> __global__ void __launch_bounds__(256, kManyPerCu<HD>) kv8_man
 #pragma unroll
         for (int g = 0; g < 4; g++)
             *reinterpret_cast<float4 *>(dst + 32 * d + 8 * g) =
-                make_float4(o[d][4 * g] * inv, o[d][4 * g + 1] * inv, o[d][4 * g + 2] * inv, o[d][4 * g + 3] * inv);
+                make_float4(o[d][4 * g] * inv * big, o[d][4 * g + 1] * inv * big, o[d][4 * g + 2] * inv * big, o[d][4 * g + 3] * inv * big);
     if (p.splits > 1 && lh == 0) *reinterpret_cast<float2 *>(p.part_ml + 2 * at) = make_float2(m, l);
 }
 

@@ -177,3 +177,11 @@ def test_same_tokens_each_time(hip_ctx):
         hip_ctx.sample_rows(xb, out, ub, o, 16, 50000)
     hip_ctx.commit()
     assert np.array_equal(out.read(np.uint32), want)
+
+
+def test_a_penalty_that_leaves_no_finite_logit(hip_ctx):
+    """Logits that the penalty takes to -infinity, all of them: the first, as on the host."""
+    x = np.full((1, 40), -3e38, np.float32)
+    x[0, 7] = -2.9e38
+    for kw in (dict(), dict(top_p=0.9), dict(top_k=5), dict(top_k=5, top_p=0.5)):
+        check(hip_ctx, x, np.array([0.5]), dict(kw, penalty=2.0), np.arange(40, dtype=np.uint32)[None])

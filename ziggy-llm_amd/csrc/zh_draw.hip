@@ -15,6 +15,10 @@
 // Where a finer bin holds more logits than that -- a thousand equal ones, or nearly -- its logits' values
 // go digit by digit, and equal ones by the counts of their slices.  (128256 logits rounded to quarters,
 // nucleus of 0.9: 50 us; all equal: 0.52 ms.)
+//
+// What bounds it: three dependent launches, each a chain of a few memory round trips.  One row of 128256
+// logits, top-k 40: 2.2, 6.3 and 10.2 us; 16 rows of 151936, nucleus: 3.7, 9.4 and 16.0 (the logits'
+// 9.7 MB are 2.1 us of it).  A row whole in one workgroup, in one launch: 42 us at 32000 logits, these 19.
 #include "zh_longctx.h"
 
 namespace zh {
@@ -29,7 +33,6 @@ typedef unsigned long long u64;
 // a row's part of the workspace
 struct RowHead {
     float max, per_bin;  // of the binned logits; bins per unit
-    u64 pad;
 };
 struct SliceStats {
     float max, min, sum, count;  // of what is finite and no mask (above -1e30)
@@ -230,13 +233,6 @@ __global__ void __launch_bounds__(256) draw_bins_kernel(SampleRows p) {
 
 // ---- finish: a workgroup of 1024 per row ----
 
-struct Key {
-    uint32_t w[3];
-};
-__device__ __forceinline__ bool at_least(const Key &a, const Key &b) {
-    return a.w[0] != b.w[0] ? a.w[0] > b.w[0] : a.w[1] != b.w[1] ? a.w[1] > b.w[1] : a.w[2] >= b.w[2];
-}
-
 struct Finish {
     u64 list[kList];              // keys being sorted
     u64 sums[kFine];              // bins' sums; fine bins'
@@ -244,7 +240,6 @@ struct Finish {
     uint32_t seen[262144 / 32];   // recent tokens
     u64 value;
     uint32_t found, count, least, most;
-    Key key[kThreads / 64];
 };
 
 // Inclusive prefix sum over the wavefront on the vector ALU: within rows of 16 by row shifts, then the
@@ -322,24 +317,20 @@ __device__ void sort_list(Finish &f, uint32_t n) {
         }
 }
 
-template <class K> __device__ Key largest(Finish &f, uint32_t n, K key) {
-    Key k{};
+// The id of the first of the row's largest logits.
+template <class V> __device__ uint32_t first_of_largest(Finish &f, uint32_t n, V value) {
+    u64 k = 0;
 #pragma unroll 8
     for (uint32_t i = threadIdx.x; i < n; i += kThreads) {
-        const Key c = key(i);
-        if (at_least(c, k)) k = c;
+        const u64 c = (u64)ordered(value(i)) << 32 | (uint32_t)~i;
+        k = c > k ? c : k;
     }
-    for (int d = 32; d; d >>= 1) {
-        Key o;
-        for (int j = 0; j < 3; j++) o.w[j] = (uint32_t)__shfl_xor((int)k.w[j], d);
-        if (at_least(o, k)) k = o;
-    }
+    k = wave_max_key(k);
     __syncthreads();
-    if ((threadIdx.x & 63) == 0) f.key[threadIdx.x >> 6] = k;
+    if ((threadIdx.x & 63) == 0) f.wave[threadIdx.x >> 6] = k;
     __syncthreads();
-    for (int j = 0; j < kThreads / 64; j++)
-        if (at_least(f.key[j], k)) k = f.key[j];
-    return k;
+    for (int j = 0; j < kThreads / 64; j++) k = f.wave[j] > k ? f.wave[j] : k;
+    return ~(uint32_t)k;
 }
 
 // Calls take(logit, its id) for the row's logits of bins first .. last, 8 lanes a slice, 64 of a slice
@@ -373,7 +364,7 @@ __global__ void __launch_bounds__(kThreads) draw_finish_kernel(SampleRows p) {
     auto answer = [&](uint32_t id) {
         if (tid == 0) p.out[row] = id;
     };
-    if (p.o.temperature <= 0.f) return answer(~largest(f, n, [&](uint32_t i) { return Key{{ordered(x[i]), ~i, 0}}; }).w[1]);
+    if (p.o.temperature <= 0.f) return answer(first_of_largest(f, n, [&](uint32_t i) { return x[i]; }));
     const Policy policy(p);
     const RowWork w = row_work(p, row);
     // two bins' sums of every eighth slice, under way while the recent tokens are marked
@@ -391,8 +382,8 @@ __global__ void __launch_bounds__(kThreads) draw_finish_kernel(SampleRows p) {
     auto logit = [&](uint32_t i) { return logit_of(i, x[i]); };
     const double given = p.uniforms[row], u = given >= 0.0 ? fmin(given, 1.0) : 0.0;
     const float top = w.head->max, per_bin = w.head->per_bin;
-    if (!(fabsf(top) < INFINITY))  // no largest number: the first of the largest logits
-        return answer(~largest(f, n, [&](uint32_t i) { return Key{{ordered(x[i]), ~i, 0}}; }).w[1]);
+    if (!(fabsf(top) < INFINITY))  // no largest number: the first of the largest logits (of the binned ones)
+        return answer(first_of_largest(f, n, [&](uint32_t i) { return policy.limited ? x[i] : logit(i); }));
 
     // the bins' sums over the slices, the largest logits' first
     u64 total, before;

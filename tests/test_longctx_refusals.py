@@ -156,6 +156,13 @@ def test_attention(host):
     assert call(window=1) and call(window=0xFFFFFFFF) and call(position=0, queries=1, heads=4) and call(scale=-1.0)
 
 
+def test_attention_score_scale(host):
+    """A scale whose product with log2 e passes binary32 is refused, the largest below it taken."""
+    good, q, out = cache(host), host.buffer(4 * 8 * 64), host.buffer(4 * 8 * 64)
+    for scale, taken in ((3e38, False), (-2.4e38, False), (2.3e38, True), (-2.3e38, True), (float("-inf"), False)):
+        assert taken == host.call("ziggy_hip_kv8_attention_f32", host.ctx, ctypes.byref(good), q, Z(0), out, U(8), U(0), U(70), U(1), U(0), F(scale))
+
+
 def test_sampling(host):
     x, u, out, rec = host.buffer(4 * 1000 * 7), host.buffer(56), host.buffer(28), host.buffer(4 * 7 * 20)
 

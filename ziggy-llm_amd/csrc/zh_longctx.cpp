@@ -254,7 +254,8 @@ int ziggy_hip_kv8_attention_f32(ZiggyHipContext *ctx, const ZiggyHipKv8Cache *ca
               p.c.nkv);
     ZH_REFUSE(queries == 0 || position >= cache->context_length || queries > cache->context_length - position,
               "queries %u at position %u outside the context of %u", queries, position, cache->context_length);
-    ZH_REFUSE(!isfinite(scale), "invalid score scale");
+    const float qscale = scale * 1.44269504088896340736f;  // scores as powers of two
+    ZH_REFUSE(!isfinite(qscale), "invalid score scale");
     const size_t width = (size_t)heads * p.c.hd;
     if (q_stride == 0) q_stride = width;
     const size_t nq = rows_bytes(queries, width, q_stride), no = rows_bytes(queries, width, width);
@@ -267,7 +268,7 @@ int ziggy_hip_kv8_attention_f32(ZiggyHipContext *ctx, const ZiggyHipKv8Cache *ca
     p.out = (float *)out->ptr;
     p.heads = (int)heads;
     p.position = position, p.queries = queries, p.window = window;
-    p.qscale = scale * 1.44269504088896340736f;
+    p.qscale = qscale;
     p.part = (float *)ctx->scratch;
     p.part_floats = ctx->scratch_len / 4;
     OnDevice on(ctx->device);

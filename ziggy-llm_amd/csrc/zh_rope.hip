@@ -3,6 +3,9 @@
 // (x0, x1) -> m (x0 cos t - x1 sin t, x0 sin t + x1 cos t), t = position * f_i.  The angle is taken in
 // turns and in 64 bits, f_i / 2 pi = 2^(i exponent) / 2 pi, and reduced to half a turn either way
 // before it is rounded to 32 bits: at position 10^6 a 32-bit angle would be off by 0.06 rad.
+//
+// What bounds it: memory for a prompt (4096 rows of 40 heads of 128, 168 MB: 33.6 us, 5.0 TB/s; 59.4 with
+// 4-byte accesses, a head and a row's angles at a time), the launch for a step (40 heads of 128: 3.0 us).
 #include "zh_longctx.h"
 
 namespace zh {

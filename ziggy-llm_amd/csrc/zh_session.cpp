@@ -968,7 +968,7 @@ int ziggy_hip_session_step_sample(ZiggyHipSession *s, uint32_t token, const uint
     }
     if (penalty && recent_count > s->sp_recent_cap) {
         // (the stream is idle between calls; the outgrown list is freed with the session)
-        const uint32_t cap = recent_count < 4096 ? 4096 : 2 * std::min(recent_count, 0x7FFFFFFFu);
+        const uint32_t cap = std::max(std::max(4096u, recent_count), 2 * std::min(recent_count, 0x7FFFFFFFu));
         uint32_t *list = nullptr;
         ZH_TRY(hipMalloc((void **)&list, (size_t)cap * 4), "sampling buffers");
         s->allocs.push_back(list);

@@ -10,21 +10,6 @@ using namespace zh;
 
 namespace {
 
-// The context's device current for a call, the caller's again after it.
-struct OnDevice {
-    int before = -1;
-    explicit OnDevice(int device) {
-        int now = -1;
-        if (hipGetDevice(&now) == hipSuccess && now != device) {
-            before = now;
-            hipSetDevice(device);
-        }
-    }
-    ~OnDevice() {
-        if (before >= 0) hipSetDevice(before);
-    }
-};
-
 #define ZH_REFUSE(cond, ...)                      \
     if (cond) {                                   \
         set_err(err, err_len, __VA_ARGS__);       \

@@ -6,6 +6,21 @@
 
 namespace zh {
 
+// The context's device current for a call, the caller's again after it.
+struct OnDevice {
+    int before = -1;
+    explicit OnDevice(int device) {
+        int now = -1;
+        if (hipGetDevice(&now) == hipSuccess && now != device) {
+            before = now;
+            hipSetDevice(device);
+        }
+    }
+    ~OnDevice() {
+        if (before >= 0) hipSetDevice(before);
+    }
+};
+
 // Scaled rotary frequencies in turns a position (radians / 2 pi): 2^(i exponent) / 2 pi, blended.
 struct RopeFreq {
     double exponent;   // -2 log2(base) / rope_dim

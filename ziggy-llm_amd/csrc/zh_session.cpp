@@ -958,6 +958,12 @@ int ziggy_hip_session_step_sample(ZiggyHipSession *s, uint32_t token, const uint
     if (!(uniform >= 0.0 && uniform < 1.0))
         return fail(err, err_len, ZIGGY_HIP_INVALID_ARGUMENT, "the random number lies outside [0, 1)");
     const bool penalty = options->repeat_penalty > 1.f && options->temperature > 0.f && recent_count > 0;
+    OnDevice on(s->ctx->device);
+    try {
+        s->allocs.reserve(s->allocs.size() + 3);
+    } catch (const std::bad_alloc &) {
+        return fail(err, err_len, ZIGGY_HIP_BUFFER_FAILED, "out of host memory");
+    }
     if (!s->sp_io) {
         ZH_TRY(hipMalloc((void **)&s->sp_io, 256), "sampling buffers");
         s->allocs.push_back(s->sp_io);

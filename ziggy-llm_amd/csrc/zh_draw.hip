@@ -8,17 +8,20 @@
 // Three launches, none of which sorts the row:
 //   stats   slices of 2048 logits: maximum, minimum and mean, from which a linear scale of 256 bins
 //           is laid over the values, the largest in bin 0;
-//   bins    per slice the bins' sums of weights (top-k: counts), and its logits in the order of their bins;
+//   bins    per slice the bins' sums of weights, and its logits in the order of their bins;
 //   finish  a workgroup per row: the bin in which a target lies, then 1024 finer bins of that bin's
 //           logits, then the few logits of the finer bin in order.  With top-k the bins above the k-th
 //           logit are sorted in LDS instead, and everything else is prefix sums of at most 1024.
-// Where a finer bin holds more logits than that -- a thousand equal ones, or nearly -- its logits' values
-// go digit by digit, and equal ones by the counts of their slices.  (128256 logits rounded to quarters,
-// nucleus of 0.9: 50 us; all equal: 0.52 ms.)
+// What is left of a row at the end, up to 64 logits, is a wavefront's work without a barrier.  Where a
+// finer bin holds more than 1024 logits, equal ones or nearly, their values go digit by digit, and equal
+// ones by the counts of their slices.  (128256 logits rounded to quarters, nucleus of 0.9: 36 us; all
+// equal: 0.52 ms.)
 //
-// What bounds it: three dependent launches, each a chain of a few memory round trips.  One row of 128256
-// logits, top-k 40: 2.2, 6.3 and 10.2 us; 16 rows of 151936, nucleus: 3.7, 9.4 and 16.0 (the logits'
-// 9.7 MB are 2.1 us of it).  A row whole in one workgroup, in one launch: 42 us at 32000 logits, these 19.
+// What bounds it: three dependent launches, each a chain of memory round trips, barriers and LDS.  One row
+// of 128256 logits, top-k 40 of 0.9: 16.1 us (1.7, 4.8 and 5.3 of the launches); 16 rows of 151936, nucleus
+// of 0.95: 27.2 (2.9, 5.9 and 12.4; the logits' 9.7 MB are 2.1 us of it).  Of the finish, 3 us were barriers
+// of 16 wavefronts in the sums and sorts that a wavefront does now, 2 the tables of all bins where a top-k
+// lies in the first quarter.  A row whole in one workgroup, in one launch: 42 us at 32000 logits, these 19.
 #include "zh_longctx.h"
 
 namespace zh {
@@ -46,7 +49,7 @@ __host__ __device__ constexpr size_t row_bytes(uint32_t vocab) {
 struct RowWork {
     RowHead *head;
     SliceStats *stats;
-    u64 *sums;       // [slice][kBins]
+    u64 *sums;       // [slice][kBins] (without top-k)
     uint32_t *run;   // [slice][kBins]: where the bin's logits begin in the slice's order, and (high half) end
     float *value;    // [slice][kSliceLogits], in the order of their bins
     uint16_t *from;  // [slice][kSliceLogits]: of which logit of the slice
@@ -80,18 +83,21 @@ struct Policy {
     bool limited, sorted;
     uint32_t top_k;
     double per_t, least, unit;  // unit 2^s
+    float none;                 // exponents below it surely come to a weight of 0
     __device__ explicit Policy(const SampleRows &p) {
         top_k = p.o.top_k == 0 ? p.vocab : min(p.o.top_k, p.vocab);
         limited = top_k < p.vocab, sorted = p.o.top_p < 1.f;
         per_t = 1.0 / (double)p.o.temperature, least = (double)p.o.min_p;
         const int bits = top_k > 1 ? 32 - __clz((int)top_k - 1) : 0;
         unit = __longlong_as_double((long long)(1023 + 62 - bits) << 52);
+        none = fmaxf(logf(p.o.min_p), -0.6931472f * (float)(63 - bits)) - 0.01f;
     }
     // (the same operations wherever it is called: the sums of the bins and of their logits agree)
     __device__ __forceinline__ u64 weight(float a, float mx) const {
 #pragma clang fp contract(off)
-        if (!(a > -INFINITY)) return 0;
-        const double e = exp(((double)a - (double)mx) * per_t);
+        const double x = ((double)a - (double)mx) * per_t;
+        if (!(x > (double)none)) return 0;  // (-infinity, NaN too)
+        const double e = exp(x);
         return e >= least ? (u64)rint(e * unit) : 0;
     }
 };
@@ -138,6 +144,33 @@ struct Slice {
     }
 };
 
+// Inclusive prefix sum over the wavefront on the vector ALU: within rows of 16 by row shifts, then the
+// rows' ends broadcast to the rows behind.
+template <int CTRL, int ROWS> __device__ __forceinline__ u64 add_dpp(u64 v) {
+    const uint32_t lo = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)v, CTRL, ROWS, 0xF, false);
+    const uint32_t hi = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)(v >> 32), CTRL, ROWS, 0xF, false);
+    return v + ((u64)hi << 32 | lo);
+}
+__device__ __forceinline__ u64 wave_prefix(u64 v) {
+    v = add_dpp<0x111, 0xF>(v);  // row_shr:1, 2, 4, 8 (lanes before the row's start: 0)
+    v = add_dpp<0x112, 0xF>(v);
+    v = add_dpp<0x114, 0xF>(v);
+    v = add_dpp<0x118, 0xF>(v);
+    v = add_dpp<0x142, 0xA>(v);  // row_bcast:15 into rows 1 and 3
+    return add_dpp<0x143, 0xC>(v);  // row_bcast:31 into rows 2 and 3
+}
+// The sum over the wavefront, in every lane.
+__device__ __forceinline__ float wave_sum(float v) {
+    auto add = [&](auto ctrl) {
+        v += __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), decltype(ctrl)::value, 0xF, 0xF, false));
+    };
+    add(std::integral_constant<int, 0xB1>{});
+    add(std::integral_constant<int, 0x4E>{});
+    add(std::integral_constant<int, 0x141>{});
+    add(std::integral_constant<int, 0x140>{});
+    return xsum<32>(xsum<16>(v));
+}
+
 __global__ void __launch_bounds__(256) draw_stats_kernel(SampleRows p) {
     __shared__ uint32_t bits[kSliceLogits / 32];
     __shared__ float4 red[4];
@@ -149,10 +182,7 @@ __global__ void __launch_bounds__(256) draw_stats_kernel(SampleRows p) {
         mx = fmaxf(mx, s.a[i]);
         if (s.a[i] > -1e30f && s.a[i] < INFINITY) mn = fminf(mn, s.a[i]), sum += s.a[i], count += 1.f;
     }
-    for (int d = 32; d; d >>= 1) {
-        mx = fmaxf(mx, __shfl_xor(mx, d)), mn = fminf(mn, __shfl_xor(mn, d));
-        sum += __shfl_xor(sum, d), count += __shfl_xor(count, d);
-    }
+    mx = wave_max_f32(mx), mn = -wave_max_f32(-mn), sum = wave_sum(sum), count = wave_sum(count);
     if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = make_float4(mx, mn, sum, count);
     __syncthreads();
     if (threadIdx.x) return;
@@ -177,10 +207,7 @@ __global__ void __launch_bounds__(256) draw_bins_kernel(SampleRows p) {
     float mx = -INFINITY, mn = INFINITY, sum = 0.f, known = 0.f;
     for (uint32_t i = threadIdx.x & 63; i < slices; i += 64)
         mx = fmaxf(mx, all[i].x), mn = fminf(mn, all[i].y), sum += all[i].z, known += all[i].w;
-    for (int d = 32; d; d >>= 1) {
-        mx = fmaxf(mx, __shfl_xor(mx, d)), mn = fminf(mn, __shfl_xor(mn, d));
-        sum += __shfl_xor(sum, d), known += __shfl_xor(known, d);
-    }
+    mx = wave_max_f32(mx), mn = -wave_max_f32(-mn), sum = wave_sum(sum), known = wave_sum(known);
     // the scale: with top-k down to the mean; else to the lowest, or to where weights are 0, or, where
     // few lie far below the others, as far below the mean as half again the largest is above it
     const float above = mx - sum / known;
@@ -196,27 +223,23 @@ __global__ void __launch_bounds__(256) draw_bins_kernel(SampleRows p) {
         const u64 v = !(fabsf(mx) < INFINITY) ? 0ull : policy.limited ? (s.a[i] > -INFINITY ? 1ull : 0ull) : policy.weight(s.a[i], mx);
         at[i] = 0xFFFFFFFFu;  // no candidate: in no bin
         if (v) {
-            atomicAdd(&sums[b], v);
+            if (!policy.limited) atomicAdd(&sums[b], v);
             at[i] = (uint32_t)b << 16 | atomicAdd(&count[b], 1u);
         }
         whole += v;
     }
-    for (int d = 32; d; d >>= 1) whole += (u64)__shfl_xor((long long)whole, d);
-    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = whole;
+    whole = wave_prefix(whole);
+    if ((threadIdx.x & 63) == 63) red[threadIdx.x >> 6] = whole;
     __syncthreads();
     const uint32_t mine = count[threadIdx.x];
-    uint32_t upto = mine;
-    for (int d = 1; d < 64; d <<= 1) {
-        const uint32_t o = (uint32_t)__shfl_up((int)upto, d);
-        if ((int)(threadIdx.x & 63) >= d) upto += o;
-    }
+    uint32_t upto = (uint32_t)wave_prefix(mine);
     if ((threadIdx.x & 63) == 63) wave_count[threadIdx.x >> 6] = upto;
     __syncthreads();
     for (uint32_t k = 0; k < threadIdx.x >> 6; k++) upto += wave_count[k];
     begin[threadIdx.x] = upto - mine;
     const size_t slice = blockIdx.x;
     w.run[slice * kBins + threadIdx.x] = (upto - mine) | upto << 16;
-    w.sums[slice * kBins + threadIdx.x] = sums[threadIdx.x];
+    if (!policy.limited) w.sums[slice * kBins + threadIdx.x] = sums[threadIdx.x];
     if (threadIdx.x == 0) w.whole[slice] = red[0] + red[1] + red[2] + red[3];
     __syncthreads();
 #pragma unroll
@@ -235,28 +258,14 @@ __global__ void __launch_bounds__(256) draw_bins_kernel(SampleRows p) {
 
 struct Finish {
     u64 list[kList];              // keys being sorted
-    u64 sums[kFine];              // bins' sums; fine bins'
+    u64 sums[kFine];              // the fine bins' sums
+    u64 runs[kBins];              // the bins' running sums
     u64 wave[kThreads / 64];
     uint32_t seen[262144 / 32];   // recent tokens
-    u64 value;
+    u64 value, key;
     uint32_t found, count, least, most;
 };
 
-// Inclusive prefix sum over the wavefront on the vector ALU: within rows of 16 by row shifts, then the
-// rows' ends broadcast to the rows behind.
-template <int CTRL, int ROWS> __device__ __forceinline__ u64 add_dpp(u64 v) {
-    const uint32_t lo = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)v, CTRL, ROWS, 0xF, false);
-    const uint32_t hi = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)(v >> 32), CTRL, ROWS, 0xF, false);
-    return v + ((u64)hi << 32 | lo);
-}
-__device__ __forceinline__ u64 wave_prefix(u64 v) {
-    v = add_dpp<0x111, 0xF>(v);  // row_shr:1, 2, 4, 8 (lanes before the row's start: 0)
-    v = add_dpp<0x112, 0xF>(v);
-    v = add_dpp<0x114, 0xF>(v);
-    v = add_dpp<0x118, 0xF>(v);
-    v = add_dpp<0x142, 0xA>(v);  // row_bcast:15 into rows 1 and 3
-    return add_dpp<0x143, 0xC>(v);  // row_bcast:31 into rows 2 and 3
-}
 // Inclusive prefix sum over the workgroup; *total: the whole.
 __device__ u64 prefix(Finish &f, u64 v, u64 *total) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
@@ -284,37 +293,65 @@ __device__ uint32_t first_reaching(Finish &f, u64 run, u64 v, u64 target, u64 *b
     return f.found;
 }
 
+// The two in one: the thread at which the running sum of v reaches target.
+__device__ uint32_t reach(Finish &f, u64 v, u64 target, u64 *before) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    u64 run = wave_prefix(v);
+    if (lane == 63) f.wave[wave] = run;
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < kThreads / 64 - 1; i++) run += i < wave ? f.wave[i] : 0;
+    if (v && run >= target && run - v < target) f.found = threadIdx.x, f.value = run - v;
+    __syncthreads();
+    *before = f.value;
+    return f.found;
+}
+
 __device__ u64 target_of(double share, u64 total) {
     const double t = ceil(share * (double)total);
     const u64 c = t >= 1.0 ? (u64)t : 1ull;
     return c < total ? c : total;
 }
 
+// The keys of lanes 0 .. n - 1 of the first wavefront (they differ) in descending order, 0 in the lanes
+// behind: a key's place is the count of larger ones.  Takes f.list's first 64 places.
+__device__ __forceinline__ u64 wave_sorted(Finish &f, u64 key, uint32_t n) {
+    constexpr int N = 16;
+    const uint32_t lane = threadIdx.x;
+    f.list[lane] = lane < n ? key : 0;
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    uint32_t place = 0;
+    for (uint32_t i = 0; i < n; i += N) {
+        u64 other[N];
+#pragma unroll
+        for (int j = 0; j < N; j++) other[j] = f.list[i + j];
+#pragma unroll
+        for (int j = 0; j < N; j++) place += other[j] > key;
+    }
+    const int to = 4 * (int)(lane < n ? place : lane);
+    const u64 r = (u64)(uint32_t)__builtin_amdgcn_ds_permute(to, (int)(key >> 32)) << 32 | (uint32_t)__builtin_amdgcn_ds_permute(to, (int)key);
+    return lane < n ? r : 0;
+}
+
 // f.list[0 .. n) in descending order (n at most kList; the places up to a power of two are filled).
 __device__ void sort_list(Finish &f, uint32_t n) {
-    if (n <= 64) {  // a wavefront: each key's place is the count of larger ones (keys differ)
-        if (threadIdx.x < 64) {
-            const u64 k = threadIdx.x < n ? f.list[threadIdx.x] : 0;
-            uint32_t place = 0;
-            for (uint32_t i = 0; i < n; i++) place += f.list[i] > k;
-            if (threadIdx.x < n) f.list[place] = k;
-        }
-        __syncthreads();
-        return;
-    }
-    uint32_t size = 128;
+    uint32_t size = 64;
     while (size < n) size <<= 1;
     for (uint32_t i = n + threadIdx.x; i < size; i += kThreads) f.list[i] = 0;
     __syncthreads();
-    for (uint32_t run = 2; run <= size; run <<= 1)
-        for (uint32_t d = run >> 1; d; d >>= 1) {
+    // (a wavefront's 64 pairs lie in 128 places of its own while they are at most 64 apart: no barrier between such steps)
+    for (uint32_t r = 1; 1u << r <= size; r++)
+        for (int s = (int)r - 1; s >= 0; s--) {
+            const uint32_t d = 1u << s;
             for (uint32_t i = threadIdx.x; i < size / 2; i += kThreads) {
-                const uint32_t a = 2 * d * (i / d) + i % d, b = a + d;
+                const uint32_t a = (i >> s) << (s + 1) | (i & (d - 1)), b = a + d;
                 const u64 x = f.list[a], y = f.list[b];
-                if ((x < y) == ((a & run) == 0)) f.list[a] = y, f.list[b] = x;
+                if ((x < y) == ((a >> r & 1) == 0)) f.list[a] = y, f.list[b] = x;
             }
-            __syncthreads();
+            if (d >= 128 || (s == 0 && r >= 7)) __syncthreads();
+            else __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
         }
+    __syncthreads();
 }
 
 // The id of the first of the row's largest logits.
@@ -333,28 +370,39 @@ template <class V> __device__ uint32_t first_of_largest(Finish &f, uint32_t n, V
     return ~(uint32_t)k;
 }
 
-// Calls take(logit, its id) for the row's logits of bins first .. last, 8 lanes a slice, 64 of a slice
-// under way at once.
-template <class T> __device__ __forceinline__ void of_bins(const RowWork &w, uint32_t slices, uint32_t first, uint32_t last, T take) {
-    constexpr int N = 8;
-    const size_t slice = threadIdx.x / 8;
-    if (slice >= slices) return;
-    const uint32_t begin = w.run[slice * kBins + first] & 0xFFFFu, end = w.run[slice * kBins + last] >> 16;
-    const float *value = w.value + slice * kSliceLogits;
-    const uint16_t *from = w.from + slice * kSliceLogits;
-    for (uint32_t e = begin + threadIdx.x % 8; e < end; e += 8 * N) {
-        float a[N];
-        uint32_t id[N];
+// The row's logits of bins first .. last, 8 lanes a slice: the first 64 of a slice in registers, the
+// others read again each time.
+struct OfBins {
+    static constexpr int N = 8;
+    const float *value;
+    const uint16_t *from;
+    uint32_t base, begin, end;
+    float a[N];
+    uint32_t id[N];
+    __device__ __forceinline__ OfBins(const RowWork &w, uint32_t slices, uint32_t first, uint32_t last) {
+        const uint32_t slice = threadIdx.x / 8;
+        base = slice * kSliceLogits, begin = end = 0;
+        value = w.value + base, from = w.from + base;
+        if (slice < slices) begin = (w.run[slice * kBins + first] & 0xFFFFu) + threadIdx.x % 8, end = w.run[slice * kBins + last] >> 16;
+        if (begin < end) load(begin);
+    }
+    __device__ __forceinline__ void load(uint32_t e) {
 #pragma unroll
         for (int k = 0; k < N; k++) {
             const uint32_t at = min(e + 8 * k, end - 1);
             a[k] = value[at], id[k] = from[at];
         }
-#pragma unroll
-        for (int k = 0; k < N; k++)
-            if (e + 8 * k < end) take(a[k], (uint32_t)slice * kSliceLogits + id[k]);
     }
-}
+    // take(logit, its id) of each
+    template <class T> __device__ __forceinline__ void each(T take) {
+        for (uint32_t e = begin; e < end; e += 8 * N) {
+            if (end - begin > 8 * N) load(e);
+#pragma unroll
+            for (int k = 0; k < N; k++)
+                if (e + 8 * k < end) take(a[k], base + id[k]);
+        }
+    }
+};
 static_assert(kThreads / 8 >= kMaxSlices, "8 lanes for every slice");
 
 __global__ void __launch_bounds__(kThreads) draw_finish_kernel(SampleRows p) {
@@ -367,13 +415,33 @@ __global__ void __launch_bounds__(kThreads) draw_finish_kernel(SampleRows p) {
     if (p.o.temperature <= 0.f) return answer(first_of_largest(f, n, [&](uint32_t i) { return x[i]; }));
     const Policy policy(p);
     const RowWork w = row_work(p, row);
-    // two bins' sums of every eighth slice, under way while the recent tokens are marked
-    constexpr int kAhead = 8, kLanes = kThreads / (kBins / 2);
+    // the slices' tables of bins, 16 bytes of a slice a thread, under way while the recent tokens are marked: two bins'
+    // sums of every eighth slice; with top-k the runs of four of the first quarter's bins of every 64th
     const uint32_t slices = slices_of(n);
-    ulonglong2 ahead[kAhead];
+    constexpr int kAhead = 12;
+    ulonglong2 part[kAhead];
+    uint32_t quarters = 0;  // of the bins whose sums are known
+    auto load_counts = [&]() {
 #pragma unroll
-    for (int k = 0; k < kAhead; k++)
-        ahead[k] = *reinterpret_cast<const ulonglong2 *>(w.sums + min(tid / (kBins / 2) + k * kLanes, slices - 1) * kBins + 2 * (tid % (kBins / 2)));
+        for (uint32_t k = 0; k < 2; k++) {
+            const uint32_t slice = tid / 16 + 64 * k;
+            part[k] = make_ulonglong2(0, 0);
+            if (slice < slices) part[k] = reinterpret_cast<const ulonglong2 *>(w.run)[slice * 64 + quarters * 16 + tid % 16];
+        }
+    };
+    auto load_sums = [&](uint32_t from) {
+#pragma unroll
+        for (uint32_t k = 0; k < kAhead; k++) {
+            const uint32_t slice = from + tid / 128 + 8 * k;
+            part[k] = make_ulonglong2(0, 0);
+            if (slice < slices) part[k] = reinterpret_cast<const ulonglong2 *>(w.sums)[slice * 128 + tid % 128];
+        }
+    };
+    static_assert(kMaxSlices <= 128 && kThreads == 1024 && kBins == 256, "a thread's pieces of the tables");
+    if (policy.limited) load_counts();
+    else if (policy.sorted) load_sums(0);
+    const uint32_t lane = tid & 63;
+    const u64 mass = (lane < slices ? w.whole[lane] : 0) + (lane + 64 < slices ? w.whole[lane + 64] : 0);
     // (the bins hold penalised logits, but for top-k's)
     if (p.recent) mark_recent(p, row, f.seen, (n + 31) / 32, 0);
     auto logit_of = [&](uint32_t i, float v) {
@@ -385,52 +453,83 @@ __global__ void __launch_bounds__(kThreads) draw_finish_kernel(SampleRows p) {
     if (!(fabsf(top) < INFINITY))  // no largest number: the first of the largest logits (of the binned ones)
         return answer(first_of_largest(f, n, [&](uint32_t i) { return policy.limited ? x[i] : logit(i); }));
 
-    // the bins' sums over the slices, the largest logits' first
-    u64 total, before;
-    auto sum_bins = [&]() {
-        for (uint32_t s = tid / (kBins / 2) + kAhead * kLanes; s < slices; s += kLanes) {
-            const ulonglong2 v = *reinterpret_cast<const ulonglong2 *>(w.sums + s * kBins + 2 * (tid % (kBins / 2)));
-            ahead[0].x += v.x, ahead[0].y += v.y;
+    const u64 mass_upto = wave_prefix(mass);
+    u64 total = (u64)(uint32_t)__builtin_amdgcn_readlane((int)(mass_upto >> 32), 63) << 32 | (uint32_t)__builtin_amdgcn_readlane((int)mass_upto, 63), before;
+    // f.runs of the loaded bins: their running sums
+    auto run_counts = [&]() {
+        uint32_t c[4] = {};
+#pragma unroll
+        for (int k = 0; k < 2; k++) {
+            const uint32_t run[4] = {(uint32_t)part[k].x, (uint32_t)(part[k].x >> 32), (uint32_t)part[k].y, (uint32_t)(part[k].y >> 32)};
+            for (int j = 0; j < 4; j++) c[j] += (run[j] >> 16) - (run[j] & 0xFFFFu);
         }
+        uint32_t *counts = reinterpret_cast<uint32_t *>(f.list);  // [wavefront][64]
+        for (int j = 0; j < 4; j++) {
+            uint32_t a, b;
+            lane_pair<16>(c[j], a, b);
+            lane_pair<32>(a + b, a, b);
+            c[j] = a + b;
+        }
+        if (lane < 16) *reinterpret_cast<uint4 *>(counts + (tid & ~63u) + 4 * lane) = make_uint4(c[0], c[1], c[2], c[3]);
+        __syncthreads();
+        if (tid < 64) {
+            uint32_t v = 0;
+#pragma unroll
+            for (int k = 0; k < kThreads / 64; k++) v += counts[64 * k + tid];
+            f.runs[64 * quarters + tid] = wave_prefix(v) + (quarters ? f.runs[64 * quarters - 1] : 0);
+        }
+        quarters++;
+        __syncthreads();
+    };
+    auto run_sums = [&]() {
         u64 x = 0, y = 0;
+        for (uint32_t from = 0;;) {
 #pragma unroll
-        for (int k = 0; k < kAhead; k++) {
-            const bool in = tid / (kBins / 2) + k * kLanes < slices;
-            x += in ? ahead[k].x : 0, y += in ? ahead[k].y : 0;
+            for (int k = 0; k < kAhead; k++) x += part[k].x, y += part[k].y;
+            if ((from += 8 * kAhead) >= slices) break;
+            load_sums(from);
         }
+        f.list[2 * tid] = x, f.list[2 * tid + 1] = y;  // [8][kBins]
         __syncthreads();
-        f.list[2 * tid] = x, f.list[2 * tid + 1] = y;
-        __syncthreads();
-        u64 v = 0;
-        if (tid < kBins)
+        if (tid < 64) {
+            u64 v[4] = {};
 #pragma unroll
-            for (int k = 0; k < kLanes; k++) v += f.list[k * kBins + tid];
-        return v;
+            for (int k = 0; k < 8; k++)
+                for (int j = 0; j < 4; j++) v[j] += f.list[k * kBins + 4 * tid + j];
+            v[1] += v[0], v[2] += v[1], v[3] += v[2];
+            const u64 ahead = wave_prefix(v[3]) - v[3];
+            for (int j = 0; j < 4; j++) f.runs[4 * tid + j] = ahead + v[j];
+        }
+        quarters = 4;
+        __syncthreads();
+    };
+    // the bin in which the sum reaches target (every wavefront by itself); *ahead: the sum of the bins before
+    auto bin_reaching = [&](u64 target, u64 *ahead) {
+        uint32_t bin = 0;
+        for (uint32_t k = 0; k < quarters; k++) bin += (uint32_t)__popcll(__ballot(f.runs[64 * k + lane] < target));
+        *ahead = bin ? f.runs[bin - 1] : 0;
+        return (int)bin;
     };
 
     // The logit at which the sum of weights reaches target, in descending order (equal logits: of ascending ids), as
-    // its key, value and complement of the id; *upto: the sum with it.  c: this thread's bin's sum, run: with those of
-    // the bins before.
-    auto find = [&](auto weight, u64 c, u64 run, u64 target, u64 *upto) {
-        u64 ahead, fine_ahead, all;
-        const int bin = (int)first_reaching(f, run, c, target, &ahead);
+    // its key, value and complement of the id; *upto: the sum with it.  It lies in the given bin, ahead of which the sum
+    // is `ahead`.
+    auto find = [&](auto weight, int bin, u64 ahead, u64 target, u64 *upto) {
+        u64 fine_ahead;
+        f.sums[tid] = 0;  // (each thread's own, until here)
+        if (tid == 0) f.count = 0, f.least = 0xFFFFFFFFu, f.most = 0;
+        OfBins logits(w, slices, bin, bin);
         __syncthreads();
-        f.sums[tid] = 0;
-        __syncthreads();
-        of_bins(w, slices, bin, bin, [&](float a, uint32_t) {
+        logits.each([&](float a, uint32_t) {
             float t;
             bin_of(a, top, per_bin, t);
             atomicAdd(&f.sums[fine_of(t, bin)], weight(a));
         });
         __syncthreads();
-        const u64 v = f.sums[tid], r = prefix(f, v, &all);
-        const int fine = (int)first_reaching(f, r, v, target - ahead, &fine_ahead);
-        __syncthreads();
-        if (tid == 0) f.count = 0, f.least = 0xFFFFFFFFu, f.most = 0;
-        __syncthreads();
+        const int fine = (int)reach(f, f.sums[tid], target - ahead, &fine_ahead);
         // take(value, id) for the logits of the finer bin
         auto of_fine = [&](auto take) {
-            of_bins(w, slices, bin, bin, [&](float a, uint32_t i) {
+            logits.each([&](float a, uint32_t i) {
                 float t;
                 bin_of(a, top, per_bin, t);
                 if (fine_of(t, bin) == fine) take(ordered(a), i);
@@ -446,13 +545,22 @@ __global__ void __launch_bounds__(kThreads) draw_finish_kernel(SampleRows p) {
         const uint32_t m = f.count;
         u64 need = target - ahead - fine_ahead, last;
         *upto = ahead + fine_ahead;
+        if (m <= 64) {  // by a wavefront
+            if (tid < 64) {
+                const u64 key = wave_sorted(f, tid < m ? f.list[tid] : 0, m);
+                const u64 wt = tid < m ? weight(unordered((uint32_t)(key >> 32))) : 0, run = wave_prefix(wt);
+                if (wt && run >= need && run - wt < need) f.value = run, f.key = key;
+            }
+            __syncthreads();
+            *upto += f.value;
+            return f.key;
+        }
         if (m <= kThreads) {
             __syncthreads();
             sort_list(f, m);
             const u64 mine = tid < m ? f.list[tid] : 0;
             const u64 wt = tid < m ? weight(unordered((uint32_t)(mine >> 32))) : 0;
-            const u64 rr = prefix(f, wt, &all);
-            const u64 key = f.list[first_reaching(f, rr, wt, need, &last)];
+            const u64 key = f.list[reach(f, wt, need, &last)];
             *upto += last + weight(unordered((uint32_t)(key >> 32)));
             __syncthreads();
             return key;
@@ -474,8 +582,7 @@ __global__ void __launch_bounds__(kThreads) draw_finish_kernel(SampleRows p) {
                 if (above == value) atomicAdd(&f.sums[255 - (o >> shift & 255u)], weight(unordered(o)));
             });
             __syncthreads();
-            const u64 s = f.sums[tid], q = prefix(f, s, &all);
-            value = (value << 8 | (255 - first_reaching(f, q, s, need, &last))) << shift;
+            value = (value << 8 | (255 - reach(f, f.sums[tid], need, &last))) << shift;
             need -= last, *upto += last;
         }
         // equal logits: the rank among them, by the slices' counts and then the ids of one slice
@@ -487,8 +594,7 @@ __global__ void __launch_bounds__(kThreads) draw_finish_kernel(SampleRows p) {
             if (o == value) atomicAdd(&f.sums[i / kSliceLogits], 1ull);
         });
         __syncthreads();
-        const u64 s = f.sums[tid], q = prefix(f, s, &all);
-        const uint32_t slice = first_reaching(f, q, s, rank, &last);
+        const uint32_t slice = reach(f, f.sums[tid], rank, &last);
         uint32_t *bits = reinterpret_cast<uint32_t *>(f.list);
         __syncthreads();
         if (tid < kSliceLogits / 32) bits[tid] = 0;
@@ -498,9 +604,8 @@ __global__ void __launch_bounds__(kThreads) draw_finish_kernel(SampleRows p) {
         });
         __syncthreads();
         uint32_t word = tid < kSliceLogits / 32 ? bits[tid] : 0;
-        const u64 set = __popc(word), upto_word = prefix(f, set, &all);
         u64 ahead_of_word;
-        const uint32_t at = first_reaching(f, upto_word, set, rank - last, &ahead_of_word);
+        const uint32_t at = reach(f, __popc(word), rank - last, &ahead_of_word);
         word = bits[at];
         for (u64 k = rank - last - ahead_of_word; k > 1; k--) word &= word - 1;
         *upto += rank * one;
@@ -509,13 +614,12 @@ __global__ void __launch_bounds__(kThreads) draw_finish_kernel(SampleRows p) {
     };
 
     if (policy.limited) {
-        const u64 c = sum_bins(), run = prefix(f, c, &total);
         const uint32_t k = (uint32_t)(total < policy.top_k ? total : policy.top_k);  // candidates above -infinity
-        const uint32_t last = first_reaching(f, run, c, k, &before);
-        __syncthreads();
         if (tid == 0) f.count = 0;
-        __syncthreads();
-        of_bins(w, slices, 0, last, [&](float v, uint32_t i) {
+        for (run_counts(); f.runs[64 * quarters - 1] < k; run_counts()) load_counts();
+        const int last = bin_reaching(k, &before);
+        OfBins logits(w, slices, 0, last);
+        logits.each([&](float v, uint32_t i) {
             const uint32_t at = atomicAdd(&f.count, 1u);
             if (at < kList) f.list[at] = (u64)ordered(v) << 32 | (uint32_t)~i;
         });
@@ -524,16 +628,41 @@ __global__ void __launch_bounds__(kThreads) draw_finish_kernel(SampleRows p) {
         __syncthreads();
         if (m > kList) {  // thousands of logits about the k-th: those down to it alone
             u64 upto;
-            const u64 end = find([](float) { return 1ull; }, c, run, k, &upto);
+            const u64 end = find([](float) { return 1ull; }, last, before, k, &upto);
             __syncthreads();
             if (tid == 0) f.count = 0;
             __syncthreads();
-            of_bins(w, slices, 0, last, [&](float v, uint32_t i) {
+            logits.each([&](float v, uint32_t i) {
                 const u64 key = (u64)ordered(v) << 32 | (uint32_t)~i;
                 if (key >= end) f.list[atomicAdd(&f.count, 1u)] = key;
             });
             __syncthreads();
             m = k;
+        }
+        if (m <= 64) {  // as below, by a wavefront
+            if (tid >= 64) return;
+            const u64 mine = wave_sorted(f, tid < m ? f.list[tid] : 0, m);
+            const bool in = tid < k;
+            uint32_t token = ~(uint32_t)mine;
+            float b = in ? logit_of(token, unordered((uint32_t)(mine >> 32))) : -INFINITY;
+            const u64 key = in ? (u64)ordered(b) << 32 | (uint32_t)~tid : 0, best = wave_max_key(key);
+            const float mx = unordered((uint32_t)(best >> 32));
+            if (!(fabsf(mx) < INFINITY)) {
+                if (tid == ~(uint32_t)best) p.out[row] = token;
+                return;
+            }
+            if (policy.sorted && p.recent) {
+                const u64 next = wave_sorted(f, key, k);
+                b = in ? unordered((uint32_t)(next >> 32)) : -INFINITY;
+                token = (uint32_t)__shfl((int)token, (int)(~(uint32_t)next & 63));
+            }
+            const u64 v = policy.weight(b, mx), sum = wave_prefix(v);
+            auto sum_at = [&](int lane) { return (u64)__shfl((long long)sum, lane); };
+            auto reaching = [&](u64 target) { return __ffsll(__ballot(v && sum >= target && sum - v < target)) - 1; };
+            u64 all = sum_at(63);
+            if (policy.sorted) all = sum_at(reaching(target_of((double)p.o.top_p, all)));
+            if ((int)tid == reaching(target_of(u, all))) p.out[row] = token;
+            return;
         }
         sort_list(f, m);
         // this thread's candidate: rank tid in the order of the logits
@@ -588,11 +717,13 @@ __global__ void __launch_bounds__(kThreads) draw_finish_kernel(SampleRows p) {
         return;
     }
 
-    const u64 c = sum_bins(), run = prefix(f, c, &total);
-    auto weight = [&](float a) { return policy.weight(a, top); };
-    u64 upto;
-    find(weight, c, run, target_of((double)p.o.top_p, total), &upto);
-    const u64 key = find(weight, c, run, target_of(u, upto), &upto);
+    run_sums();
+    u64 upto, key = 0, target = target_of((double)p.o.top_p, total);
+    for (int i = 0; i < 2; i++) {  // where the nucleus ends, the draw in it
+        const int bin = bin_reaching(target, &before);
+        key = find([&](float a) { return policy.weight(a, top); }, bin, before, target, &upto);
+        target = target_of(u, upto);
+    }
     answer(~(uint32_t)key);
 }
 

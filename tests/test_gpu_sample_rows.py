@@ -185,3 +185,30 @@ def test_a_penalty_that_leaves_no_finite_logit(hip_ctx):
     x[0, 7] = -2.9e38
     for kw in (dict(), dict(top_p=0.9), dict(top_k=5), dict(top_k=5, top_p=0.5)):
         check(hip_ctx, x, np.array([0.5]), dict(kw, penalty=2.0), np.arange(40, dtype=np.uint32)[None])
+
+
+@pytest.mark.parametrize("top_k", [1, 2, 62, 63, 64, 65, 66, 127, 128, 129, 511, 513, 1023])
+@pytest.mark.parametrize("vocab", [1025, 1100, 3000, 50000])
+def test_counts_of_candidates_about_the_widths_of_sorts(hip_ctx, top_k, vocab):
+    rng = np.random.default_rng(top_k + vocab)
+    x = logits(rng, 4, vocab)
+    x[2] = np.round(x[2] * 8) / 8
+    x[3, : vocab // 2] = -np.inf
+    recent = np.argsort(-x, axis=1)[:, rng.integers(0, top_k + 3, 90)].astype(np.uint32)
+    for kw in (dict(), dict(top_p=0.9, temperature=2.0), dict(top_p=0.8, penalty=1.2), dict(penalty=1.5, temperature=0.6)):
+        check(hip_ctx, x, rng.random(4), dict(kw, top_k=top_k), recent)
+
+
+@pytest.mark.parametrize("equal", [63, 64, 65, 1023, 1024, 1025, 1026, 3000])
+def test_counts_of_equal_logits_about_the_widths_of_sorts(hip_ctx, equal):
+    """Logits that are equal, or apart by a step of 1, where the nucleus ends and the draw falls."""
+    rng = np.random.default_rng(equal)
+    vocab = 20000
+    x = logits(rng, 3, vocab)
+    for r in range(3):
+        at = rng.permutation(vocab)[:equal]
+        x[r, at] = 14.0
+        if r == 1:
+            x[r, at] = (np.float32(14).view(np.uint32) + np.arange(equal)).astype(np.uint32).view(np.float32)
+    for kw in (dict(top_p=0.5), dict(top_p=0.999), dict(top_p=0.9, min_p=0.3), dict(top_k=1000, top_p=0.7)):
+        check(hip_ctx, x, rng.random(3), kw)

@@ -29,7 +29,6 @@ namespace zh {
 namespace {
 
 constexpr int kSliceLogits = 2048, kBins = 256, kFine = 1024, kThreads = 1024, kMaxSlices = 262144 / kSliceLogits;
-constexpr int kList = 4096;  // logits sorted in LDS (top-k: at most 1024 of them are candidates)
 
 typedef unsigned long long u64;
 
@@ -257,7 +256,7 @@ __global__ void __launch_bounds__(256) draw_bins_kernel(SampleRows p) {
 // ---- finish: a workgroup of 1024 per row ----
 
 struct Finish {
-    u64 list[kList];              // keys being sorted
+    u64 list[2 * kThreads];       // logits' keys; the bins' sums of several slices; keys being sorted
     u64 sums[kFine];              // the fine bins' sums
     u64 runs[kBins];              // the bins' running sums
     u64 wave[kThreads / 64];
@@ -333,25 +332,50 @@ __device__ __forceinline__ u64 wave_sorted(Finish &f, u64 key, uint32_t n) {
     return lane < n ? r : 0;
 }
 
-// f.list[0 .. n) in descending order (n at most kList; the places up to a power of two are filled).
-__device__ void sort_list(Finish &f, uint32_t n) {
-    uint32_t size = 64;
-    while (size < n) size <<= 1;
-    for (uint32_t i = n + threadIdx.x; i < size; i += kThreads) f.list[i] = 0;
-    __syncthreads();
-    // (a wavefront's 64 pairs lie in 128 places of its own while they are at most 64 apart: no barrier between such steps)
-    for (uint32_t r = 1; 1u << r <= size; r++)
-        for (int s = (int)r - 1; s >= 0; s--) {
-            const uint32_t d = 1u << s;
-            for (uint32_t i = threadIdx.x; i < size / 2; i += kThreads) {
-                const uint32_t a = (i >> s) << (s + 1) | (i & (d - 1)), b = a + d;
-                const u64 x = f.list[a], y = f.list[b];
-                if ((x < y) == ((a >> r & 1) == 0)) f.list[a] = y, f.list[b] = x;
-            }
-            if (d >= 128 || (s == 0 && r >= 7)) __syncthreads();
-            else __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+// The larger or the smaller of a key and that of the lane whose number differs in bit S.
+template <int S> __device__ __forceinline__ u64 exchanged(u64 key, bool larger) {
+    u64 a = key, b;
+    if constexpr (S >= 4) {
+        uint32_t al, bl, ah, bh;
+        lane_pair<1 << S>((uint32_t)key, al, bl), lane_pair<1 << S>((uint32_t)(key >> 32), ah, bh);
+        a = (u64)ah << 32 | al, b = (u64)bh << 32 | bl;
+    } else if constexpr (S == 3) {
+        b = dpp_u64<0x128>(key);  // row_ror:8
+    } else if constexpr (S == 2) {
+        b = dpp_u64<0x1B>(dpp_u64<0x141>(key));  // lane ^ 7, then ^ 3
+    } else {
+        b = dpp_u64<S == 1 ? 0x4E : 0xB1>(key);
+    }
+    return (a > b) == larger ? a : b;
+}
+
+// The workgroup's keys in descending order, thread i the i-th: n keys that differ, of threads 0 .. n - 1, 0
+// behind.  A bitonic sort: in registers up to 32 lanes apart, through LDS beyond.
+__device__ u64 sorted(Finish &f, u64 key, uint32_t n) {
+    const uint32_t tid = threadIdx.x;
+    if (tid >= n) key = 0;
+    uint32_t steps = 6, half = 0;
+    while (1u << steps < n) steps++;
+    for (uint32_t r = 1; r <= steps; r++) {
+        const uint32_t down = tid >> r;  // bit 0: whether this block ascends
+        for (uint32_t s = r - 1; s >= 6 && s < r; s--) {
+            f.list[half + tid] = key;
+            __syncthreads();
+            const u64 o = f.list[half + (tid ^ 1u << s)];
+            half ^= kThreads;
+            key = (key > o) == (((tid >> s ^ down) & 1) == 0) ? key : o;
         }
-    __syncthreads();
+        auto larger = [&](int s) { return ((tid >> s ^ down) & 1) == 0; };
+        switch (r < 6 ? r : 6) {
+        case 6: key = exchanged<5>(key, larger(5)); [[fallthrough]];
+        case 5: key = exchanged<4>(key, larger(4)); [[fallthrough]];
+        case 4: key = exchanged<3>(key, larger(3)); [[fallthrough]];
+        case 3: key = exchanged<2>(key, larger(2)); [[fallthrough]];
+        case 2: key = exchanged<1>(key, larger(1)); [[fallthrough]];
+        default: key = exchanged<0>(key, larger(0));
+        }
+    }
+    return key;
 }
 
 // The id of the first of the row's largest logits.
@@ -556,14 +580,12 @@ __global__ void __launch_bounds__(kThreads) draw_finish_kernel(SampleRows p) {
             return f.key;
         }
         if (m <= kThreads) {
-            __syncthreads();
-            sort_list(f, m);
-            const u64 mine = tid < m ? f.list[tid] : 0;
+            const u64 mine = sorted(f, tid < m ? f.list[tid] : 0, m);
             const u64 wt = tid < m ? weight(unordered((uint32_t)(mine >> 32))) : 0;
-            const u64 key = f.list[reach(f, wt, need, &last)];
-            *upto += last + weight(unordered((uint32_t)(key >> 32)));
+            if (tid == reach(f, wt, need, &last)) f.key = mine;
             __syncthreads();
-            return key;
+            *upto += last + weight(unordered((uint32_t)(f.key >> 32)));
+            return f.key;
         }
         // the value: its digits, but for those that all of them share
         atomicMin(&f.least, lo);
@@ -621,12 +643,12 @@ __global__ void __launch_bounds__(kThreads) draw_finish_kernel(SampleRows p) {
         OfBins logits(w, slices, 0, last);
         logits.each([&](float v, uint32_t i) {
             const uint32_t at = atomicAdd(&f.count, 1u);
-            if (at < kList) f.list[at] = (u64)ordered(v) << 32 | (uint32_t)~i;
+            if (at < kThreads) f.list[at] = (u64)ordered(v) << 32 | (uint32_t)~i;
         });
         __syncthreads();
         uint32_t m = f.count;
         __syncthreads();
-        if (m > kList) {  // thousands of logits about the k-th: those down to it alone
+        if (m > kThreads) {  // many logits about the k-th: those down to it alone
             u64 upto;
             const u64 end = find([](float) { return 1ull; }, last, before, k, &upto);
             __syncthreads();
@@ -664,9 +686,8 @@ __global__ void __launch_bounds__(kThreads) draw_finish_kernel(SampleRows p) {
             if ((int)tid == reaching(target_of(u, all))) p.out[row] = token;
             return;
         }
-        sort_list(f, m);
         // this thread's candidate: rank tid in the order of the logits
-        u64 mine = tid < k ? f.list[tid] : 0;
+        u64 mine = sorted(f, tid < m ? f.list[tid] : 0, m);
         const uint32_t id = ~(uint32_t)mine;
         const float a = tid < k ? logit_of(id, unordered((uint32_t)(mine >> 32))) : -INFINITY;
         u64 best = wave_max_key(tid < k ? (u64)ordered(a) << 32 | (uint32_t)~tid : 0);  // of equal ones the first
@@ -675,16 +696,17 @@ __global__ void __launch_bounds__(kThreads) draw_finish_kernel(SampleRows p) {
         __syncthreads();
         for (int j = 0; j < kThreads / 64; j++) best = f.wave[j] > best ? f.wave[j] : best;
         const float mx = unordered((uint32_t)(best >> 32));
-        if (!(fabsf(mx) < INFINITY)) return answer(~(uint32_t)f.list[~(uint32_t)best]);
+        if (!(fabsf(mx) < INFINITY)) {
+            if (tid == ~(uint32_t)best) p.out[row] = id;
+            return;
+        }
         float b = a;
         uint32_t token = id;
         if (policy.sorted && p.recent) {  // by weight: the penalised logits, ties as they stand
-            __syncthreads();
             uint32_t *ids = reinterpret_cast<uint32_t *>(f.sums);
             ids[tid] = id;
-            f.list[tid] = tid < k ? (u64)ordered(a) << 32 | (uint32_t)~tid : 0;
-            sort_list(f, k);
-            mine = tid < k ? f.list[tid] : 0;
+            __syncthreads();
+            mine = sorted(f, (u64)ordered(a) << 32 | (uint32_t)~tid, k);
             b = tid < k ? unordered((uint32_t)(mine >> 32)) : -INFINITY;
             token = tid < k ? ids[~(uint32_t)mine] : 0;
         }

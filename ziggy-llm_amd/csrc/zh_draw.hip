@@ -378,11 +378,10 @@ __device__ u64 sorted(Finish &f, u64 key, uint32_t n) {
     return key;
 }
 
-// The id of the first of the row's largest logits.
-template <class V> __device__ uint32_t first_of_largest(Finish &f, uint32_t n, V value) {
+// The id of the first of the largest of logits begin .. end - 1.
+template <class V> __device__ uint32_t first_of_largest(Finish &f, uint32_t begin, uint32_t end, V value) {
     u64 k = 0;
-#pragma unroll 8
-    for (uint32_t i = threadIdx.x; i < n; i += kThreads) {
+    for (uint32_t i = begin + threadIdx.x; i < end; i += kThreads) {
         const u64 c = (u64)ordered(value(i)) << 32 | (uint32_t)~i;
         k = c > k ? c : k;
     }
@@ -436,9 +435,14 @@ __global__ void __launch_bounds__(kThreads) draw_finish_kernel(SampleRows p) {
     auto answer = [&](uint32_t id) {
         if (tid == 0) p.out[row] = id;
     };
-    if (p.o.temperature <= 0.f) return answer(first_of_largest(f, n, [&](uint32_t i) { return x[i]; }));
-    const Policy policy(p);
     const RowWork w = row_work(p, row);
+    if (p.o.temperature <= 0.f) {  // the first slice with the largest logit
+        auto key = [&](uint32_t slice) { return slice < slices_of(n) ? (u64)ordered(w.stats[slice].max) << 32 | (uint32_t)~slice : 0; };
+        const u64 a = key(tid & 63), b = key((tid & 63) + 64);
+        const uint32_t first = ~(uint32_t)wave_max_key(a > b ? a : b) * kSliceLogits;
+        return answer(first_of_largest(f, first, min(first + kSliceLogits, n), [&](uint32_t i) { return x[i]; }));
+    }
+    const Policy policy(p);
     // the slices' tables of bins, 16 bytes of a slice a thread, under way while the recent tokens are marked: two bins'
     // sums of every eighth slice; with top-k the runs of four of the first quarter's bins of every 64th
     const uint32_t slices = slices_of(n);
@@ -475,7 +479,7 @@ __global__ void __launch_bounds__(kThreads) draw_finish_kernel(SampleRows p) {
     const double given = p.uniforms[row], u = given >= 0.0 ? fmin(given, 1.0) : 0.0;
     const float top = w.head->max, per_bin = w.head->per_bin;
     if (!(fabsf(top) < INFINITY))  // no largest number: the first of the largest logits (of the binned ones)
-        return answer(first_of_largest(f, n, [&](uint32_t i) { return policy.limited ? x[i] : logit(i); }));
+        return answer(first_of_largest(f, 0, n, [&](uint32_t i) { return policy.limited ? x[i] : logit(i); }));
 
     const u64 mass_upto = wave_prefix(mass);
     u64 total = (u64)(uint32_t)__builtin_amdgcn_readlane((int)(mass_upto >> 32), 63) << 32 | (uint32_t)__builtin_amdgcn_readlane((int)mass_upto, 63), before;
@@ -754,11 +758,9 @@ __global__ void __launch_bounds__(kThreads) draw_finish_kernel(SampleRows p) {
 size_t sample_rows_bytes(uint32_t vocab) { return up256(row_bytes(vocab)); }
 
 hipError_t launch_sample_rows(const SampleRows &p, hipStream_t s) {
-    if (p.o.temperature > 0.f) {
-        const dim3 grid(slices_of(p.vocab), p.rows);
-        hipLaunchKernelGGL(draw_stats_kernel, grid, dim3(256), 0, s, p);
-        hipLaunchKernelGGL(draw_bins_kernel, grid, dim3(256), 0, s, p);
-    }
+    const dim3 grid(slices_of(p.vocab), p.rows);
+    hipLaunchKernelGGL(draw_stats_kernel, grid, dim3(256), 0, s, p);
+    if (p.o.temperature > 0.f) hipLaunchKernelGGL(draw_bins_kernel, grid, dim3(256), 0, s, p);
     hipLaunchKernelGGL(draw_finish_kernel, dim3(p.rows), dim3(kThreads), 0, s, p);
     return hipGetLastError();
 }

@@ -186,3 +186,46 @@ def test_wrapped_device_memory():
     repo = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
     r = subprocess.run([sys.executable, "-c", WRAP.format(repo=repo)], capture_output=True, text=True, timeout=100, cwd=repo)
     assert r.returncode == 0 and "wrapped ok" in r.stdout, r.stderr[-2000:]
+
+
+def test_two_contexts_at_once():
+    """Two threads, a context each, the same steps in sequences of their own: the outputs of either are those of a
+    context by itself (attention's splits and sampling share a context's workspace, not another's)."""
+    import threading
+    rng = np.random.default_rng(11)
+    heads, kvh, hd, n, vocab = 16, 4, 128, 6000, 40000
+    k, v = (rng.normal(0, 1, (n, kvh, hd)).astype(np.float32) for _ in range(2))
+    q, x = rng.normal(0, 1, (9, heads, hd)).astype(np.float32), rng.normal(0, 3, (3, vocab)).astype(np.float32)
+    u, o = rng.random(3), hip.SamplingOptions(temperature=0.9, top_p=0.9)
+
+    def steps(sign, results, start=None):
+        ctx = hip.Context(0)
+        c = ctx.kv8_cache(1, kvh, hd, n)
+        kb, vb, qb, xb, ub = ctx.buffer(k), ctx.buffer(v * np.float32(sign)), ctx.buffer(q), ctx.buffer(x * np.float32(sign)), ctx.buffer(u)
+        out, tokens = [ctx.empty(q.nbytes) for _ in range(2)], ctx.empty(12)
+        if start:
+            start.wait()
+        for _ in range(20):
+            ctx.begin()
+            ctx.kv8_store(c, kb, vb, 0, 0, n)
+            ctx.kv8_attention(c, qb, out[0], heads, 0, n - 1)
+            ctx.sample_rows(xb, tokens, ub, o, 3, vocab)
+            ctx.kv8_attention(c, qb, out[1], heads, 0, n - 9, 9)
+            ctx.commit()
+            results.append([out[0].read()[:heads * hd], out[1].read(), tokens.read(np.uint32)])
+        ctx.close()
+
+    alone, at_once = {1: [], -1: []}, {1: [], -1: []}
+    for sign in alone:
+        steps(sign, alone[sign])
+    start = threading.Barrier(2)
+    threads = [threading.Thread(target=steps, args=(sign, at_once[sign], start)) for sign in at_once]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    for sign in alone:
+        assert len(at_once[sign]) == 20
+        for got in at_once[sign] + alone[sign]:
+            for a, b in zip(got, alone[sign][0]):
+                assert np.array_equal(a, b)

@@ -366,13 +366,14 @@ size_t ziggy_hip_kv8_scales_length(uint32_t layers, uint32_t head_count_kv, uint
  * from k_offset_bytes and v_offset_bytes on; both may lie in the rows of a
  * fused projection, the keys rotated in place) at positions position ..
  * position + rows - 1.  A block whose first position is among them starts
- * anew: its scale is max|x| / 127 over its new rows, a code the nearest
- * integer to x / scale (ties to even).  In a block that begins before
- * `position` the earlier rows (which have to be stored by then) stay: its
- * scale grows to that of the new rows where that is larger (the earlier codes
- * are then rounded to the new scale), and never shrinks.  Rows behind the last
- * one keep their codes.  A row with an infinity or NaN makes its block's scale
- * NaN, and every row of the block reads as NaN until the block starts anew. */
+ * anew: its scale is max|x| over its new rows times 1/127 (a product in
+ * binary32), a code the nearest integer to x / scale (ties to even).  In a
+ * block that begins before `position` the earlier rows (which have to be stored
+ * by then) stay: its scale grows to that of the new rows where that is larger
+ * (the earlier codes are then rounded to the new scale), and never shrinks.
+ * Rows behind the last one keep their codes.  A row with an infinity or NaN
+ * makes its block's scale NaN, and every row of the block reads as NaN until
+ * the block starts anew. */
 int ziggy_hip_kv8_store(ZiggyHipContext *ctx, const ZiggyHipKv8Cache *cache, const ZiggyHipBuffer *k,
                         size_t k_offset_bytes, const ZiggyHipBuffer *v, size_t v_offset_bytes, size_t row_stride,
                         uint32_t layer, uint32_t position, uint32_t rows, char *error_message,

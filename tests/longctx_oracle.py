@@ -58,7 +58,7 @@ class Kv8:
                     new = x[lo - position:hi - position, h]
                     was = scales[h, b] if lo > b * BLOCK else np.float32(0)
                     top = np.abs(new).max() if np.isfinite(new).all() else np.float32(np.nan)
-                    now = np.maximum(was, np.float32(top) / np.float32(127))
+                    now = np.maximum(was, np.float32(top) * np.float32(1 / 127))
                     scales[h, b] = now
                     kept = codes[h, b * BLOCK:lo]
                     if np.isnan(now):

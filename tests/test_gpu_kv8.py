@@ -76,7 +76,7 @@ def test_ties_go_to_even(hip_ctx):
     heads, hd, context = 1, 128, 32
     scale = np.float32(0.0123)
     top = np.float32(scale * np.float32(127))
-    while np.float32(top / np.float32(127)) != scale:
+    while np.float32(top * np.float32(1 / 127)) != scale:
         top = np.nextafter(top, np.float32(np.inf))
     half = (np.arange(-126, 126) + 0.5) * float(scale)
     mid = half.astype(np.float32)

@@ -1,11 +1,12 @@
 // zh_kv8.hip -- K/V rows into and out of the cache held in 8 bits, a scale per block of 32 positions and
 // kv head.
 //
-// scale = max|x| / 127 of the block's rows, code = x / scale to the nearest integer (ties to even),
-// decided on the exact quotient.  The product with the reciprocal, rounded to an integer, is that unless
-// it lies next to a tie (within 3e-5; a wavefront in twenty has such a value): then every code of the
-// thread is decided by x - code * scale, which is exact there (the difference of near values), against
-// half the scale.  The maximum is taken of the bits of |x|, in which infinities and NaN are the largest.
+// scale = max|x| times 1/127, a product in binary32, of the block's rows; code = x / scale to the nearest
+// integer (ties to even), decided on the exact quotient.  The product with the reciprocal, rounded to an
+// integer, is that unless it lies next to a tie (within 3e-5; a wavefront in twenty has such a value):
+// then every code of the thread is decided by x - code * scale, which is exact there (the difference of
+// near values), against half the scale.  The maximum is taken of the bits of |x|, in which infinities and
+// NaN are the largest.
 //
 // What bounds it: memory for a prompt (4095 rows of 8 heads of 128, K and V, 42 MB: 11.7-13.9 us, 3.0-3.6
 // TB/s; the read-back of as many 6.3-7.5 us), the chain of load, maximum, scale and store for one row (3.6
@@ -100,7 +101,7 @@ __global__ void __launch_bounds__(256) kv8_store_kernel(Kv8Layer c, const float 
     if ((tid & 63) == 0) amax[tid >> 6] = top;
     __syncthreads();
     top = max(max(amax[0], amax[1]), max(amax[2], amax[3]));
-    float now = top < 0x7F800000u ? __uint_as_float(top) / 127.f : __uint_as_float(0x7FC00000u);
+    float now = top < 0x7F800000u ? __uint_as_float(top) * (1.f / 127.f) : __uint_as_float(0x7FC00000u);
     if (was > now || was != was) now = was;
     if (tid == 0) *scale = now;
 

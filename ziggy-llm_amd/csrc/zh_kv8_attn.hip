@@ -81,6 +81,7 @@ __device__ __forceinline__ void share(uint32_t n, uint32_t parts, uint32_t z, ui
     end = begin + each + (z < more ? 1u : 0u);
 }
 
+__device__ __forceinline__ float uniform(float v) { return __uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(v))); }
 __device__ __forceinline__ float finite(float v) { return v == -INFINITY ? 0.f : v; }
 
 // two weights' pieces
@@ -562,9 +563,9 @@ template <int HD> __global__ void __launch_bounds__(256, kManyPerCu<HD>) kv8_man
     if (t0 < t1) put(t0);
     __syncthreads();
     const bool rows_here = wave * 32 < (qlast - q0 + 1) * p.group;  // else the wavefront only fills LDS
-    big = fmaxf(fmaxf(top_scale[0], top_scale[1]), fmaxf(top_scale[2], top_scale[3]));
-    small = fminf(fminf(low_scale[0], low_scale[1]), fminf(low_scale[2], low_scale[3]));
-    if (far_apart(big, small)) {
+    big = uniform(fmaxf(fmaxf(top_scale[0], top_scale[1]), fmaxf(top_scale[2], top_scale[3])));
+    small = uniform(fminf(fminf(low_scale[0], low_scale[1]), fminf(low_scale[2], low_scale[3])));
+    if (__builtin_amdgcn_readfirstlane(far_apart(big, small))) {
 #pragma unroll 1
         for (int r = 0; r < 32; r++) {
             const int at = wave * 32 + r, i = q0 + at / p.group, h = kvh * p.group + at % p.group;

@@ -2,7 +2,8 @@
 //
 // (x0, x1) -> m (x0 cos t - x1 sin t, x0 sin t + x1 cos t), t = position * f_i.  The angle is taken in
 // turns and in 64 bits, f_i / 2 pi = 2^(i exponent) / 2 pi, and reduced to half a turn either way
-// before it is rounded to 32 bits: at position 10^6 a 32-bit angle would be off by 0.06 rad.
+// before it is rounded to 32 bits (at position 10^6 a 32-bit angle would be off by 0.06 rad); what the
+// rounding leaves off enters sine and cosine to first order.
 //
 // What bounds it: memory for a prompt (4096 rows of 40 heads of 128, 168 MB: 33.6 us, 5.0 TB/s; 59.4 with
 // 4-byte accesses, a head and a row's angles at a time), the launch for a step (40 heads of 128: 3.0 us).
@@ -39,9 +40,11 @@ template <bool ALIGNED> __global__ void __launch_bounds__(256) rope_rows_kernel(
         if (rotates) {
             const double at = (double)(p.positions ? p.positions[r] : p.first + (uint32_t)r);
             for (int j = 0; j < kPairs; j++) {
-                const double t = at * f[j];
-                sincospif((float)(2.0 * (t - rint(t))), &s[j], &c[j]);
-                c[j] *= p.magnitude, s[j] *= p.magnitude;
+                const double t = at * f[j], half_turns = 2.0 * (t - rint(t));
+                const float near = (float)half_turns, rest = (float)(half_turns - (double)near) * 3.14159265f;
+                float sn, cs;  // of the angle rounded, then of the angle
+                sincospif(near, &sn, &cs);
+                c[j] = fmaf(-rest, sn, cs) * p.magnitude, s[j] = fmaf(rest, cs, sn) * p.magnitude;
             }
         }
         if constexpr (ALIGNED) {

@@ -229,3 +229,34 @@ def test_values_near_the_ends_of_the_range(hip_ctx, queries, power):
     got = held(hip_ctx, c, q, 200)
     want = plain.astype(np.float64) * 2.0 ** power * 64
     assert np.all(np.abs(got - want) <= 2.0 ** -23 * np.abs(want) + 16 * 2.0 ** -150)
+
+
+@pytest.mark.parametrize("group", [3, 5, 7, 11, 17, 31, 33, 43, 63, 64])
+@pytest.mark.parametrize("queries", [1, 2, 3, 12, 41])
+def test_groups_of_any_size(hip_ctx, group, queries):
+    """Rows of a kv head that fill a workgroup's tile in part, queries that end inside one."""
+    for hd, position, window in ((64, 130, 0), (128, 2000, 77), (256, 40, 0)):
+        attend(hip_ctx, group, 1, hd, position, queries, window)
+
+
+@pytest.mark.parametrize("heads,kvh,hd", [(32, 8, 128), (5, 5, 64)])
+def test_a_session_of_steps_of_every_length(hip_ctx, heads, kvh, hd):
+    """A cache stored and read a few positions at a time, from the first, with the same buffers."""
+    rng = np.random.default_rng(1)
+    n = 170
+    k, v = (rng.normal(0, 1, (n, kvh, hd)).astype(np.float32) for _ in range(2))
+    q = rng.normal(0, 1, (n, heads, hd)).astype(np.float32)
+    near, cache = oracle.Kv8(kvh, n, hd), hip_ctx.kv8_cache(1, kvh, hd, n)
+    p = 0
+    for step in (1, 1, 2, 3, 5, 8, 13, 21, 34, 31, 32, 1, 17, 1):
+        near.store(k[p:p + step], v[p:p + step], p)
+        kb, vb, qb = (hip_ctx.buffer(a[p:p + step]) for a in (k, v, q))
+        out = hip_ctx.empty(qb.nbytes)
+        hip_ctx.begin()
+        hip_ctx.kv8_store(cache, kb, vb, 0, p, step)
+        hip_ctx.kv8_attention(cache, qb, out, heads, 0, p, step)
+        hip_ctx.commit()
+        want, bound = oracle.kv8_attention(near, q[p:p + step], p, hd ** -0.5)
+        assert np.all(np.abs(out.read().reshape(want.shape) - want) <= bound)
+        p += step
+    assert p == n

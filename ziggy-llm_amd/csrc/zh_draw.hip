@@ -111,11 +111,25 @@ __device__ __forceinline__ int fine_of(float t, int bin) {
 
 // The bits of the row's recent tokens with ids first .. first + 32 words - 1, into LDS.
 __device__ __forceinline__ void mark_recent(const SampleRows &p, uint32_t row, uint32_t *bits, uint32_t words, uint32_t first) {
+    constexpr int N = 4;  // of a thread under way at once
+    const uint32_t *recent = p.recent + (size_t)row * p.recent_count;
+    uint32_t id[N];
+    auto load = [&](size_t i) {
+#pragma unroll
+        for (int k = 0; k < N; k++) {
+            id[k] = 0xFFFFFFFFu;
+            if (i + k * blockDim.x < p.recent_count) id[k] = recent[i + k * blockDim.x];
+        }
+    };
+    load(threadIdx.x);
     for (uint32_t i = threadIdx.x; i < words; i += blockDim.x) bits[i] = 0;
     __syncthreads();
-    for (uint32_t i = threadIdx.x; i < p.recent_count; i += blockDim.x) {
-        const uint32_t id = p.recent[(size_t)row * p.recent_count + i];
-        if (id < p.vocab && id >= first && id - first < 32 * words) atomicOr(&bits[(id - first) / 32], 1u << (id % 32));
+    for (size_t i = threadIdx.x;;) {
+#pragma unroll
+        for (int k = 0; k < N; k++)
+            if (id[k] < p.vocab && id[k] >= first && id[k] - first < 32 * words) atomicOr(&bits[(id[k] - first) / 32], 1u << (id[k] % 32));
+        if ((i += N * blockDim.x) >= p.recent_count) break;
+        load(i);
     }
     __syncthreads();
 }

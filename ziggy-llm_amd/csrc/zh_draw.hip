@@ -227,6 +227,7 @@ __global__ void __launch_bounds__(256) draw_bins_kernel(SampleRows p) {
     float range = policy.limited ? above : fminf(fminf(43.7f * p.o.temperature, mx - mn), 2.5f * above);
     const float per_bin = range > 0.f && fabsf(mx) < INFINITY ? (float)kBins / range : 0.f;
     if (blockIdx.x == 0 && threadIdx.x == 0) w.head->max = mx, w.head->per_bin = per_bin;
+    const bool ordering = policy.limited || policy.sorted;  // else the draw goes by the ids: the slice's sum is all
     u64 whole = 0;
     uint32_t at[kSliceLogits / 256];  // bin, and the logit's place in it (in no order: their sums are exact)
 #pragma unroll
@@ -235,7 +236,7 @@ __global__ void __launch_bounds__(256) draw_bins_kernel(SampleRows p) {
         const int b = bin_of(s.a[i], mx, per_bin, t);
         const u64 v = !(fabsf(mx) < INFINITY) ? 0ull : policy.limited ? (s.a[i] > -INFINITY ? 1ull : 0ull) : policy.weight(s.a[i], mx);
         at[i] = 0xFFFFFFFFu;  // no candidate: in no bin
-        if (v) {
+        if (v && ordering) {
             if (!policy.limited) atomicAdd(&sums[b], v);
             at[i] = (uint32_t)b << 16 | atomicAdd(&count[b], 1u);
         }
@@ -244,6 +245,8 @@ __global__ void __launch_bounds__(256) draw_bins_kernel(SampleRows p) {
     whole = wave_prefix(whole);
     if ((threadIdx.x & 63) == 63) red[threadIdx.x >> 6] = whole;
     __syncthreads();
+    if (threadIdx.x == 0) w.whole[blockIdx.x] = red[0] + red[1] + red[2] + red[3];
+    if (!ordering) return;
     const uint32_t mine = count[threadIdx.x];
     uint32_t upto = (uint32_t)wave_prefix(mine);
     if ((threadIdx.x & 63) == 63) wave_count[threadIdx.x >> 6] = upto;
@@ -253,7 +256,6 @@ __global__ void __launch_bounds__(256) draw_bins_kernel(SampleRows p) {
     const size_t slice = blockIdx.x;
     w.run[slice * kBins + threadIdx.x] = (upto - mine) | upto << 16;
     if (!policy.limited) w.sums[slice * kBins + threadIdx.x] = sums[threadIdx.x];
-    if (threadIdx.x == 0) w.whole[slice] = red[0] + red[1] + red[2] + red[3];
     __syncthreads();
 #pragma unroll
     for (int i = 0; i < kSliceLogits / 256; i++)

@@ -14,12 +14,12 @@
 //           logit are sorted in LDS instead, and everything else is prefix sums of at most 1024.
 // What is left of a row at the end, up to 64 logits, is a wavefront's work without a barrier.  Where a
 // finer bin holds more than 1024 logits, equal ones or nearly, their values go digit by digit, and equal
-// ones by the counts of their slices.  (128256 logits rounded to quarters, nucleus of 0.9: 36 us; all
-// equal: 0.52 ms.)
+// ones by the counts of their slices.  (128256 logits rounded to quarters, nucleus of 0.9: 30-33 us; all
+// equal: 0.50 ms.)
 //
 // What bounds it: three dependent launches, each a chain of memory round trips, barriers and LDS.  One row
-// of 128256 logits, top-k 40 of 0.9: 16.1 us (1.7, 4.8 and 5.3 of the launches); 16 rows of 151936, nucleus
-// of 0.95: 27.2 (2.9, 5.9 and 12.4; the logits' 9.7 MB are 2.1 us of it).  Of the finish, 3 us were barriers
+// of 128256 logits, top-k 40 of 0.9: 15.4-16.4 us (1.7, 4.8 and 5.3 of the launches); 16 rows of 151936, nucleus
+// of 0.95: 24.0 (2.9, 5.9 and 12.4; the logits' 9.7 MB are 2.1 us of it).  Of the finish, 3 us were barriers
 // of 16 wavefronts in the sums and sorts that a wavefront does now, 2 the tables of all bins where a top-k
 // lies in the first quarter.  A row whole in one workgroup, in one launch: 42 us at 32000 logits, these 19.
 #include "zh_longctx.h"

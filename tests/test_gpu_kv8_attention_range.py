@@ -51,3 +51,22 @@ def test_one_small_weight(hip_ctx, hd, queries):
     err = np.abs(got - 100 * w / (1 + w))
     bound = 100 * (2.0 ** -37 + w * (2 * 2.0 ** -22 + 4 * 2.0 ** -24))
     assert np.all(err <= bound), (err / bound).max()
+
+
+@pytest.mark.parametrize("heads,kvh,hd", [(8, 2, 128), (4, 4, 64), (6, 3, 96), (2, 1, 256)])
+@pytest.mark.parametrize("queries", [1, 9, 80])
+def test_any_codes_behind_the_last_row(hip_ctx, heads, kvh, hd, queries):
+    """Codes that were never stored, -128 among them, behind the last query's row, in a block whose scale is near the
+    largest that a row gives (-128 of them lie past binary32), and beside blocks of far smaller scales."""
+    print("codes behind the last row", heads, kvh, hd, queries, flush=True)
+    rng = np.random.default_rng(hd + queries)
+    n = 101
+    c = oracle.Kv8(kvh, n, hd, rng)
+    c.scales[1][:, -1] = np.float32(3.4e38) / np.float32(127)
+    c.codes[1][:, 96:n] = rng.integers(-9, 10, c.codes[1][:, 96:n].shape)
+    c.codes[1][:, n:] = -128
+    c.codes[0][:, n:] = -128
+    q = rng.normal(0, 1, (queries, heads, hd)).astype(np.float32)
+    want, bound = oracle.kv8_attention(c, q, n - queries, hd ** -0.5)
+    err = np.abs(attend(hip_ctx, c, q, n - queries, hd ** -0.5) - want)
+    assert np.all(err <= bound), (err / bound).max()

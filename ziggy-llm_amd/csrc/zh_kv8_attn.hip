@@ -162,7 +162,8 @@ __device__ __forceinline__ void plain_row(const Kv8Params &p, int kvh, const flo
 #pragma unroll
             for (int i = 0; i < (HD + 63) / 64; i++) {
                 const int d = min(lane + 64 * i, HD - 1);
-                acc[i] = fmaf(wj, (float)p.c.vc[(head0 + b) * (kKv8Block * HD) + d * kKv8Block + j] * vs, acc[i]);
+                // (a code out of sight may be -128, its value past binary32: the weight of 0 takes the scale first)
+                acc[i] = fmaf(wj * vs, (float)p.c.vc[(head0 + b) * (kKv8Block * HD) + d * kKv8Block + j], acc[i]);
             }
         }
     }

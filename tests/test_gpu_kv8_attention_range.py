@@ -1,4 +1,6 @@
 """Attention over the 8-bit cache where weights and values span many orders of magnitude."""
+import time
+
 import numpy as np
 import pytest
 
@@ -70,3 +72,69 @@ def test_any_codes_behind_the_last_row(hip_ctx, heads, kvh, hd, queries):
     want, bound = oracle.kv8_attention(c, q, n - queries, hd ** -0.5)
     err = np.abs(attend(hip_ctx, c, q, n - queries, hd ** -0.5) - want)
     assert np.all(err <= bound), (err / bound).max()
+
+
+@pytest.mark.parametrize("heads,kvh,hd,position,queries", [(32, 8, 128, 4000, 1), (32, 8, 128, 8000, 9), (8, 2, 128, 3000, 300), (8, 8, 64, 2000, 200),
+                                                           (4, 2, 256, 1500, 100)])
+def test_one_block_of_tiny_values_costs_little(hip_ctx, heads, kvh, hd, position, queries):
+    """The first block's values are 2^-40 times the others': within four times the time without it (a row at a time
+    would be 6 to 300 times).  Least of several runs of a few passes each."""
+    print("tiny first block", heads, kvh, hd, position, queries, flush=True)
+    rng = np.random.default_rng(1)
+    q = hip_ctx.buffer(rng.normal(0, 1, (queries, heads, hd)).astype(np.float32))
+    out = hip_ctx.empty(4 * queries * heads * hd)
+    c = oracle.Kv8(kvh, position + queries, hd, rng)
+    caches = [upload(hip_ctx, [c], position + queries)]
+    c.scales[1][:, 0] *= np.float32(2.0 ** -40)
+    caches.append(upload(hip_ctx, [c], position + queries))
+    least = [np.inf, np.inf]
+    for _ in range(10):
+        for i, cache in enumerate(caches):
+            t = time.perf_counter()
+            hip_ctx.begin()
+            for _ in range(5):
+                hip_ctx.kv8_attention(cache, q, out, heads, 0, position, queries)
+            hip_ctx.commit()
+            least[i] = min(least[i], time.perf_counter() - t)
+    assert least[1] <= 4 * least[0], least
+
+
+@pytest.mark.parametrize("heads,kvh,hd", [(8, 2, 128), (4, 4, 64), (6, 3, 96), (34, 2, 256), (64, 1, 128)])
+@pytest.mark.parametrize("position,queries,window", [(150, 1, 0), (150, 9, 0), (3000, 7, 0), (3000, 12, 700), (64, 150, 0), (1500, 90, 77), (10, 300, 33)])
+def test_scales_far_apart_everywhere(hip_ctx, heads, kvh, hd, position, queries, window):
+    """Every block's V scale at random between 2^-100 and 2^100 and its keys' scores tens apart, blocks of zeros
+    among them; the blocks out of every row's sight hold NaN scales and codes of -128.  Bound: the weights' relative
+    errors (longctx_oracle) times the sum of weight x |value|, weights below 2^-60 of a row's largest left out."""
+    print("far apart", heads, kvh, hd, position, queries, window, flush=True)
+    rng = np.random.default_rng(position + hd + queries)
+    n = position + queries
+    c = oracle.Kv8(kvh, n, hd, rng)
+    c.scales[1][:] = 2.0 ** rng.uniform(-100, 100, c.scales[1].shape)
+    c.scales[0][:] *= 3
+    for b in range(2, c.nb, 5):
+        c.codes[1][:, 32 * b:32 * b + 32] = 0
+        c.scales[1][:, b] = 0
+    first = max(0, position + 1 - window) if window else 0
+    for w in range(2):
+        c.scales[w][:, :first // 32] = np.nan
+        c.scales[w][:, (n - 1) // 32 + 1:] = np.nan
+        c.codes[w][:, n:] = -128
+    q = rng.normal(0, 1, (queries, heads, hd)).astype(np.float32)
+    want, _ = oracle.kv8_attention(c, q, position, hd ** -0.5, window)
+    got = attend(hip_ctx, c, q, position, hd ** -0.5, window)
+    scale = float(np.float32(hd ** -0.5))
+    for h in range(0, heads, max(1, heads // 6)):
+        kv = h // (heads // kvh)
+        k, ks = c.codes[0][kv].astype(np.float64), np.repeat(c.scales[0][kv].astype(np.float64), 32)
+        v = np.abs(c.codes[1][kv].astype(np.float64) * np.repeat(c.scales[1][kv].astype(np.float64), 32)[:, None])
+        for i in range(0, queries, max(1, queries // 25)):
+            p = position + i + 1
+            at = slice(max(0, p - window) if window else 0, p)
+            s = (k[at] @ q[i, h].astype(np.float64)) * ks[at] * scale
+            e = (hd + 8) * 2.0 ** -23 * ((np.abs(k[at]) @ np.abs(q[i, h]).astype(np.float64)) * ks[at] * scale)
+            w = np.exp(s - s.max())
+            live = w > 2.0 ** -60
+            some = (w[~live] @ v[at][~live]) / w.sum()
+            bound = (2 * e.max() + 2.0 ** -20 + p * 2.0 ** -22) * (w[live] @ v[at][live]) / w.sum() + some
+            err = np.abs(got[i, h] - want[i, h])
+            assert np.all(err <= bound), (h, i, (err / bound).max())

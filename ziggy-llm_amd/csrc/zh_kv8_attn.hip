@@ -98,7 +98,7 @@ __device__ __forceinline__ void pieces(float a, float b, uint32_t &hi, uint32_t 
 // log2 share - max), and the weights over the share add to the sum.  (A multiplication of a block's
 // outputs instead would be an FMA per output and block.)  An all-zero block, whose codes are 0, counts as
 // a share of 2^-60: the sum keeps its weights.  Other shares are at least 2^-32 here (their log2 is held
-// to 2^-19): see plain_row.
+// to 2^-19): see far_apart.
 __device__ __forceinline__ void share_of(float scale, float big, float &log_share, float &inverse) {
     const float share = scale / big;
     log_share = big > 0.f ? __builtin_amdgcn_logf(share < 0x1p-60f ? 0x1p-60f : share) : 0.f * scale;
@@ -123,50 +123,21 @@ __device__ __forceinline__ bool far_apart(float largest, float smallest) { retur
 constexpr float kNoScale = INFINITY;  // the smallest of none
 __device__ __forceinline__ float wave_min_scale(float scale) { return -wave_max_f32(scale > 0.f ? -scale : -kNoScale); }
 
-// One row by a wavefront in plain binary32, for such scales alone: blocks b, b + step, .. below `end`, a
-// position (half its dims) a lane for the scores, a dim a lane for the output.  acc[i]: the unnormalised
-// output of dim lane + 64 i.
-template <int HD>
-__device__ __forceinline__ void plain_row(const Kv8Params &p, int kvh, const float *q, uint32_t pos, uint32_t b, uint32_t end,
-                                          uint32_t step, float &m, float &l, float (&acc)[(HD + 63) / 64]) {
-    const int lane = threadIdx.x & 63, half = lane >> 5, at32 = lane & 31;
-    const size_t head0 = (size_t)kvh * p.c.blocks;
-    const uint32_t lo = first_seen(pos, p.window);
-    m = -INFINITY, l = 0.f;
-#pragma unroll
-    for (int i = 0; i < (HD + 63) / 64; i++) acc[i] = 0.f;
-#pragma unroll 1
-    for (; b < end; b += step) {
-        const uint32_t first = b * kKv8Block, at = first + at32;
-        if (first > pos || first + kKv8Block - 1 < lo) continue;
-        const float ks = p.c.ks[head0 + b], vs = p.c.vs[head0 + b];
-        const int8_t *kc = p.c.kc + (head0 + b) * (kKv8Block * HD) + at32 * HD + half * (HD / 2);
-        float s = 0.f;
-#pragma unroll 1
-        for (int d = 0; d < HD / 2; d += 4) {
-            const uint32_t c = *reinterpret_cast<const uint32_t *>(kc + d);
-#pragma unroll
-            for (int j = 0; j < 4; j++) s = fmaf(q[half * (HD / 2) + d + j] * p.qscale, (float)(int8_t)(c >> 8 * j), s);
-        }
-        const bool in = at >= lo && at <= pos;
-        s = in ? xsum<32>(s) * ks : -INFINITY;
-        const float mn = fmaxf(m, wave_max_f32(s)), al = __builtin_amdgcn_exp2f(m - finite(mn));
-        const float w = in ? __builtin_amdgcn_exp2f(s - finite(mn)) : 0.f;
-        m = mn, l *= al;
-#pragma unroll
-        for (int i = 0; i < (HD + 63) / 64; i++) acc[i] *= al;
-#pragma unroll 1
-        for (int j = 0; j < kKv8Block; j++) {
-            const float wj = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(w), j));
-            l += wj;
-#pragma unroll
-            for (int i = 0; i < (HD + 63) / 64; i++) {
-                const int d = min(lane + 64 * i, HD - 1);
-                // (a code out of sight may be -128, its value past binary32: the weight of 0 takes the scale first)
-                acc[i] = fmaf(wj * vs, (float)p.c.vc[(head0 + b) * (kKv8Block * HD) + d * kKv8Block + j], acc[i]);
-            }
-        }
-    }
+// For such scales alone (the first block's 2^-40 of the others': 2048 queries after 14336 positions 1754 us against
+// 993, 9 queries after 16389 35.5 against 26.3, one after 4112 11.1 against 10.4): a block's weights are of its own largest, w = 2^(s - block max), their outputs a
+// product by themselves, which the scale and 2^(block max - max) multiply on their way into the row's:
+// o = o 2^(was - max) + (t 2^(block max - max)) scale.  The pieces then hold what counts of each block.
+//
+// One block of a row: its largest score `top` (-infinity: none in sight) in scores' unit f, the row's running
+// maximum m (updated); `was`: what the row's sums shrink by, the result: what the block's do, -1 of a block out of
+// sight, which gives nothing whatever its scale.
+__device__ __forceinline__ float take_block(float top, float f, float &block_max, float &m, float &was) {
+    const bool seen = top > -INFINITY;
+    block_max = seen ? top * f : 0.f;
+    const float mn = seen ? fmaxf(m, block_max) : m;
+    was = __builtin_amdgcn_exp2f(m - finite(mn));
+    m = mn;
+    return seen ? __builtin_amdgcn_exp2f(block_max - mn) : -1.f;
 }
 
 // ---- few rows ----
@@ -301,12 +272,8 @@ __global__ void __launch_bounds__(256, 1) kv8_few_kernel(Kv8Params p) {
         return !far_apart(big, small);
     };
 
-    auto compute = [&](const Block8<HD> &r, int t) {
-        const uint32_t first = block_of(t) * kKv8Block;
-        auto of_block = [&](float v) { return __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(v), t & 63)); };
-        const float ks = of_block(ksl), lv = of_block(lvl), inv = of_block(inl);
-        const bool edge = first < lo_max || first + kKv8Block - 1 > pos_min;
-        kf4 s[CT][2];
+    // a block's scores, in units of ks down[c]
+    auto scores = [&](const Block8<HD> &r, kf4 (&s)[CT][2]) {
 #pragma unroll
         for (int pt = 0; pt < 2; pt++) {
 #pragma unroll
@@ -320,29 +287,56 @@ __global__ void __launch_bounds__(256, 1) kv8_few_kernel(Kv8Params p) {
                     for (int j = 0; j < P; j++) s[c][pt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, qb[c][j][k], s[c][pt], 0, 0, 0);
             }
         }
+    };
+    // this lane's 8 scores of tile c, those out of sight -infinity; which are in sight
+    auto column = [&](const kf4 (&s)[CT][2], int c, bool edge, uint32_t first, float (&w)[8]) {
+#pragma unroll
+        for (int e = 0; e < 8; e++) {
+            w[e] = s[c][e >> 2][e & 3];
+            if constexpr (F::PAIRED)  // the other piece's column
+                w[e] += __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(w[e]), 0xB1, 0xF, 0xF, false));
+        }
+        uint32_t keep = 255;
+        if (edge) {
+            const uint32_t pos = p.position + p.query_of(row_of(c, i16)), lo = first_seen(pos, p.window);
+            keep = 0;
+#pragma unroll
+            for (int e = 0; e < 8; e++) {
+                const uint32_t at = first + 8 * g + e;
+                const bool in = at >= lo && at <= pos;
+                keep |= (uint32_t)in << e;
+                if (!in) w[e] = -INFINITY;
+            }
+        }
+        return keep;
+    };
+    // the column's weights' pieces, and their sum
+    auto weigh = [&](const float (&w)[8], kh8 (&ph)[P]) {
+        float sum = 0.f;
+        uint32_t hi[4], lo[4];
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+            sum += w[2 * e] + w[2 * e + 1];
+            pieces(w[2 * e], w[2 * e + 1], hi[e], lo[e]);
+            if constexpr (F::PAIRED) hi[e] = i16 & 1 ? lo[e] : hi[e];
+        }
+        ph[0] = __builtin_bit_cast(kh8, uint4{hi[0], hi[1], hi[2], hi[3]});
+        if constexpr (!F::PAIRED) ph[1] = __builtin_bit_cast(kh8, uint4{lo[0], lo[1], lo[2], lo[3]});
+        return sum;
+    };
+    auto compute = [&](const Block8<HD> &r, int t) {
+        const uint32_t first = block_of(t) * kKv8Block;
+        auto of_block = [&](float v) { return __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(v), t & 63)); };
+        const float ks = of_block(ksl), lv = of_block(lvl), inv = of_block(inl);
+        const bool edge = first < lo_max || first + kKv8Block - 1 > pos_min;
+        kf4 s[CT][2];
+        scores(r, s);
         kh8 ph[CT][P];
 #pragma unroll
         for (int c = 0; c < CT; c++) {
             float w[8], mx = -INFINITY;
             const float f = ks * down[c];
-#pragma unroll
-            for (int e = 0; e < 8; e++) {
-                w[e] = s[c][e >> 2][e & 3];
-                if constexpr (F::PAIRED)  // the other piece's column
-                    w[e] += __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(w[e]), 0xB1, 0xF, 0xF, false));
-            }
-            uint32_t keep = 255;
-            if (edge) {
-                const uint32_t pos = p.position + p.query_of(row_of(c, i16)), lo = first_seen(pos, p.window);
-                keep = 0;
-#pragma unroll
-                for (int e = 0; e < 8; e++) {
-                    const uint32_t at = first + 8 * g + e;
-                    const bool in = at >= lo && at <= pos;
-                    keep |= (uint32_t)in << e;
-                    if (!in) w[e] = -INFINITY;
-                }
-            }
+            const uint32_t keep = column(s, c, edge, first, w);
 #pragma unroll
             for (int e = 0; e < 8; e++) mx = fmaxf(mx, w[e]);
             mx = fmaf(xmax<32>(xmax<16>(mx)), f, lv);
@@ -358,22 +352,13 @@ __global__ void __launch_bounds__(256, 1) kv8_few_kernel(Kv8Params p) {
                 }
             }
             const float to = lv - finite(m[c]);
-            float sum = 0.f;
 #pragma unroll
             for (int e = 0; e < 8; e++) w[e] = __builtin_amdgcn_exp2f(fmaf(w[e], f, to));
             if (edge)
 #pragma unroll
                 for (int e = 0; e < 8; e++)
                     if (!(keep >> e & 1u)) w[e] = 0.f;
-            uint32_t hi[4], lo[4];
-#pragma unroll
-            for (int e = 0; e < 4; e++) {
-                sum += w[2 * e] + w[2 * e + 1];
-                pieces(w[2 * e], w[2 * e + 1], hi[e], lo[e]);
-                if constexpr (F::PAIRED) hi[e] = i16 & 1 ? lo[e] : hi[e];
-            }
-            ph[c][0] = __builtin_bit_cast(kh8, uint4{hi[0], hi[1], hi[2], hi[3]});
-            if constexpr (!F::PAIRED) ph[c][1] = __builtin_bit_cast(kh8, uint4{lo[0], lo[1], lo[2], lo[3]});
+            const float sum = weigh(w, ph[c]);
             // (a row with none of the block in sight takes nothing from it, whatever its scale)
             l[c] += sum == 0.f ? 0.f : sum * inv;
         }
@@ -387,7 +372,50 @@ __global__ void __launch_bounds__(256, 1) kv8_few_kernel(Kv8Params p) {
         }
     };
 
+    // the same where scales are far apart
+    auto compute_far = [&](const Block8<HD> &r, int t) {
+        const uint32_t first = block_of(t) * kKv8Block;
+        auto of_block = [&](float v) { return __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(v), t & 63)); };
+        const float ks = of_block(ksl), vs = of_block(vsl);
+        kf4 s[CT][2];
+        scores(r, s);
+        kh8 ph[CT][P];
+        float was[CT][4], now[CT][4];  // of the rows that this lane holds outputs of
+#pragma unroll
+        for (int c = 0; c < CT; c++) {
+            float w[8], top = -INFINITY, block_max, shrink;
+            const float f = ks * down[c];
+            const uint32_t keep = column(s, c, true, first, w);
+#pragma unroll
+            for (int e = 0; e < 8; e++) top = fmaxf(top, w[e]);
+            const float share = take_block(xmax<32>(xmax<16>(top)), f, block_max, m[c], shrink);
+#pragma unroll
+            for (int e = 0; e < 8; e++) {
+                w[e] = __builtin_amdgcn_exp2f(fmaf(w[e], f, -block_max));
+                if (!(keep >> e & 1u)) w[e] = 0.f;
+            }
+            const float sum = weigh(w, ph[c]);
+            l[c] = fmaf(l[c], shrink, sum == 0.f ? 0.f : sum * fmaxf(share, 0.f));
+#pragma unroll
+            for (int j = 0; j < 4; j++) was[c][j] = __shfl(shrink, 4 * g + j), now[c][j] = __shfl(share * (1.f / kWeight), 4 * g + j);
+        }
+#pragma unroll
+        for (int d = 0; d < F::DT; d++) {
+            const kh8 v = widen8(r.v[d][0], r.v[d][1]);
+#pragma unroll
+            for (int c = 0; c < CT; c++) {
+                kf4 b = kf4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int j = 0; j < P; j++) b = __builtin_amdgcn_mfma_f32_16x16x32_f16(ph[c][j], v, b, 0, 0, 0);
+#pragma unroll
+                for (int j = 0; j < 4; j++)
+                    o[c][d][j] = now[c][j] < 0.f ? o[c][d][j] * was[c][j] : fmaf(b[j] * now[c][j], vs, o[c][d][j] * was[c][j]);
+            }
+        }
+    };
+
     bool together = true;
+    float weight_unit = 1.f / kWeight;  // of the outputs' weights
     if (nb > 0) {
         together = take_scales();
         for (int t = 0; t < nb && together; t += 2) {
@@ -401,32 +429,34 @@ __global__ void __launch_bounds__(256, 1) kv8_few_kernel(Kv8Params p) {
             load(y, t + 3);
         }
     }
+    if (!together) {  // from the first block again
+#pragma unroll
+        for (int c = 0; c < CT; c++) {
+            m[c] = -INFINITY, l[c] = 0.f;
+#pragma unroll
+            for (int d = 0; d < F::DT; d++) o[c][d] = kf4{0.f, 0.f, 0.f, 0.f};
+        }
+#pragma unroll 1
+        for (int t = 0; t < nb; t++) {
+            if ((t & 63) == 0) load_scales(t);
+            load(x, t);
+            compute_far(x, t);
+        }
+        big = 1.f, weight_unit = 1.f;
+    }
     // the wavefront's rows: both pieces' outputs, the sum over its lanes
     const uint32_t live = rlast - r0 + 1;
-    if (!together)
-#pragma unroll 1
-        for (uint32_t r = 0; r < live; r++) {
-            const uint32_t qi = p.query_of(r0 + r);
-            const float *q = p.q + (size_t)qi * p.q_stride + (size_t)(kvh * p.group + (int)(r0 + r - qi * p.group)) * HD;
-            float acc[(HD + 63) / 64], mr, lr;
-            plain_row<HD>(p, kvh, q, p.position + qi, b0 + wave, b1, 4, mr, lr, acc);
-#pragma unroll
-            for (int i = 0; i < (HD + 63) / 64; i++)
-                if (lane + 64 * i < HD) os[wave][r][lane + 64 * i] = acc[i];
-            if (lane == 0) ms[wave][r] = mr, ls[wave][r] = lr;
-        }
 #pragma unroll
     for (int c = 0; c < CT; c++) {
-        if (!together) break;
         const float sum = xsum<32>(xsum<16>(l[c]));
 #pragma unroll
         for (int d = 0; d < F::DT; d++)
 #pragma unroll
             for (int j = 0; j < 4; j++) {
                 if constexpr (F::PAIRED) {
-                    if (j % 2 == 0) os[wave][2 * g + j / 2][16 * d + i16] = (o[c][d][j] + o[c][d][j + 1]) * (1.f / kWeight) * big;
+                    if (j % 2 == 0) os[wave][2 * g + j / 2][16 * d + i16] = (o[c][d][j] + o[c][d][j + 1]) * weight_unit * big;
                 } else
-                    os[wave][16 * c + 4 * g + j][16 * d + i16] = o[c][d][j] * (1.f / kWeight) * big;
+                    os[wave][16 * c + 4 * g + j][16 * d + i16] = o[c][d][j] * weight_unit * big;
             }
         if (lane < 16 && (!F::PAIRED || lane % 2 == 0)) {
             const int r = F::PAIRED ? lane / 2 : 16 * c + lane;
@@ -569,60 +599,115 @@ template <int HD> __global__ void __launch_bounds__(256, kManyPerCu<HD>) kv8_man
     const bool rows_here = wave * 32 < (qlast - q0 + 1) * p.group;  // else the wavefront only fills LDS
     big = uniform(fmaxf(fmaxf(top_scale[0], top_scale[1]), fmaxf(top_scale[2], top_scale[3])));
     small = uniform(fminf(fminf(low_scale[0], low_scale[1]), fminf(low_scale[2], low_scale[3])));
-    if (__builtin_amdgcn_readfirstlane(far_apart(big, small))) {
-#pragma unroll 1
-        for (int r = 0; r < 32; r++) {
-            const int at = wave * 32 + r, i = q0 + at / p.group, h = kvh * p.group + at % p.group;
-            if (at >= qn * p.group || i > qlast) break;
-            float acc[(HD + 63) / 64], mr, lr;
-            plain_row<HD>(p, kvh, p.q + (size_t)i * p.q_stride + (size_t)h * HD, p.position + i, 2 * (uint32_t)t0,
-                          min(2 * (uint32_t)t1, last_block + 1), 1, mr, lr, acc);
-            const float n = p.splits > 1 && mr == -INFINITY && lr == 0.f ? 0.f : 1.f / lr;
-            const size_t row = (size_t)i * p.heads + h, to = (size_t)z * p.queries * p.heads + row;
-            float *dst = p.splits > 1 ? p.part + to * HD : p.out + row * HD;
-#pragma unroll
-            for (int k = 0; k < (HD + 63) / 64; k++)
-                if (lane + 64 * k < HD) dst[lane + 64 * k] = acc[k] * n;
-            if (p.splits > 1 && lane == 0) *reinterpret_cast<float2 *>(p.part_ml + 2 * to) = make_float2(mr, lr);
-        }
-        return;
-    }
     const int krow = (l32 & 0x13) | (l32 & 4) << 1 | (l32 & 8) >> 1;
 
-    for (int t = t0; t < t1; t++) {
+    // a tile's scores, in units of its blocks' K scales times down
+    auto scores = [&](int t, kf16 (&s)[2]) {
+        const char *ks = lds + (t & 1) * BUF + krow * KST + 16 * lh;
+#pragma unroll
+        for (int pt = 0; pt < 2; pt++) {
+#pragma unroll
+            for (int r = 0; r < 16; r++) s[pt][r] = 0.f;
+#pragma unroll
+            for (int k = 0; k < KT; k++) {
+                const kh8 a = *reinterpret_cast<const kh8 *>(ks + pt * 32 * KST + 32 * k);
+                s[pt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, qh[k], s[pt], 0, 0, 0);
+                s[pt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, ql[k], s[pt], 0, 0, 0);
+            }
+        }
+    };
+    // those out of this row's sight -infinity; which are in sight
+    auto mask = [&](int t, kf16 (&s)[2]) {
+        uint32_t keep = 0;
+#pragma unroll
+        for (int pt = 0; pt < 2; pt++)
+#pragma unroll
+            for (int r = 0; r < 16; r++) {
+                const uint32_t at = 64 * (uint32_t)t + 32 * pt + 16 * (r >> 3) + 8 * lh + (r & 7);
+                const bool in = at >= qlo && at <= qpos;
+                keep |= (uint32_t)in << (16 * pt + r);
+                if (!in) s[pt][r] = -INFINITY;
+            }
+        return keep;
+    };
+    // a block's weights' pieces, and their sum
+    auto weigh = [&](const kf16 &w, kh8 (&ph)[2], kh8 (&pl)[2]) {
+        float sum = 0.f;
+        uint32_t hi[8], lo[8];
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+            const float a = w[2 * i], b = w[2 * i + 1];
+            sum += a + b;
+            pieces(a, b, hi[i], lo[i]);
+        }
+#pragma unroll
+        for (int k = 0; k < 2; k++) {
+            ph[k] = __builtin_bit_cast(kh8, uint4{hi[4 * k], hi[4 * k + 1], hi[4 * k + 2], hi[4 * k + 3]});
+            pl[k] = __builtin_bit_cast(kh8, uint4{lo[4 * k], lo[4 * k + 1], lo[4 * k + 2], lo[4 * k + 3]});
+        }
+        return sum;
+    };
+    const bool apart = __builtin_amdgcn_readfirstlane(far_apart(big, small));
+    const float weight_unit = apart ? 1.f : kWeight;  // of the outputs' weights
+    if (apart) {
+        big = 1.f;
+#pragma unroll 1
+        for (int t = t0; t < t1; t++) {
+            const uint32_t ba = 2 * (uint32_t)t, bb = min(ba + 1, last_block);
+            if (t + 1 < t1) load(t + 1);
+            if (rows_here) {
+                const char *vs = lds + (t & 1) * BUF + 64 * KST + l32 * VST + 16 * lh;
+                kf16 s[2];
+                scores(t, s);
+                const uint32_t keep = mask(t, s);
+#pragma unroll
+                for (int pt = 0; pt < 2; pt++) {
+                    const float f = p.c.ks[head0 + (pt ? bb : ba)] * down, vscale = p.c.vs[head0 + (pt ? bb : ba)];
+                    float top = s[pt][0], block_max, was;
+#pragma unroll
+                    for (int r = 1; r < 16; r++) top = fmaxf(top, s[pt][r]);
+                    const float share = take_block(xmax<32>(top), f, block_max, m, was), out_share = share * (1.f / kWeight);
+#pragma unroll
+                    for (int r = 0; r < 16; r++) {
+                        s[pt][r] = __builtin_amdgcn_exp2f(fmaf(s[pt][r], f, -block_max));
+                        if (!(keep >> (16 * pt + r) & 1u)) s[pt][r] = 0.f;
+                    }
+                    kh8 ph[2], pl[2];
+                    const float sum = weigh(s[pt], ph, pl);
+                    l = fmaf(l, was, sum == 0.f ? 0.f : sum * fmaxf(share, 0.f));
+#pragma unroll
+                    for (int d = 0; d < DT; d++) {
+                        kf16 b;
+#pragma unroll
+                        for (int r = 0; r < 16; r++) b[r] = 0.f;
+#pragma unroll
+                        for (int k = 0; k < 2; k++) {
+                            const kh8 a = *reinterpret_cast<const kh8 *>(vs + d * 32 * VST + pt * 64 + 32 * k);
+                            b = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, ph[k], b, 0, 0, 0);
+                            b = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, pl[k], b, 0, 0, 0);
+                        }
+#pragma unroll
+                        for (int r = 0; r < 16; r++) o[d][r] = share < 0.f ? o[d][r] * was : fmaf(b[r] * out_share, vscale, o[d][r] * was);
+                    }
+                }
+            }
+            if (t + 1 < t1) put(t + 1);
+            __syncthreads();
+        }
+    }
+    for (int t = apart ? t1 : t0; t < t1; t++) {
         const uint32_t ba = 2 * (uint32_t)t, bb = min(ba + 1, last_block);
         // (a block ahead of every row's window holds any bytes: its scale counts as 0)
         const float kscale[2] = {ba < first_block ? 0.f : p.c.ks[head0 + ba], p.c.ks[head0 + bb]}, vscale[2] = {p.c.vs[head0 + ba], p.c.vs[head0 + bb]};
         if (t + 1 < t1) load(t + 1);
         __builtin_amdgcn_sched_barrier(0);
         if (rows_here) {
-            const char *ks = lds + (t & 1) * BUF + krow * KST + 16 * lh, *vs = lds + (t & 1) * BUF + 64 * KST + l32 * VST + 16 * lh;
+            const char *vs = lds + (t & 1) * BUF + 64 * KST + l32 * VST + 16 * lh;
             kf16 s[2];
-#pragma unroll
-            for (int pt = 0; pt < 2; pt++) {
-#pragma unroll
-                for (int r = 0; r < 16; r++) s[pt][r] = 0.f;
-#pragma unroll
-                for (int k = 0; k < KT; k++) {
-                    const kh8 a = *reinterpret_cast<const kh8 *>(ks + pt * 32 * KST + 32 * k);
-                    s[pt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, qh[k], s[pt], 0, 0, 0);
-                    s[pt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, ql[k], s[pt], 0, 0, 0);
-                }
-            }
+            scores(t, s);
             const bool edge = 64 * (uint32_t)t + 63 > wave_first || 64 * (uint32_t)t < wave_lo;
             uint32_t keep = 0xFFFFFFFFu;
-            if (edge) {
-                keep = 0;
-#pragma unroll
-                for (int pt = 0; pt < 2; pt++)
-#pragma unroll
-                    for (int r = 0; r < 16; r++) {
-                        const uint32_t at = 64 * (uint32_t)t + 32 * pt + 16 * (r >> 3) + 8 * lh + (r & 7);
-                        const bool in = at >= qlo && at <= qpos;
-                        keep |= (uint32_t)in << (16 * pt + r);
-                        if (!in) s[pt][r] = -INFINITY;
-                    }
-            }
+            if (edge) keep = mask(t, s);
             float f[2], lv[2], inv[2], mx = -INFINITY;
 #pragma unroll
             for (int pt = 0; pt < 2; pt++) {
@@ -647,33 +732,24 @@ template <int HD> __global__ void __launch_bounds__(256, kManyPerCu<HD>) kv8_man
 #pragma unroll
             for (int pt = 0; pt < 2; pt++) {
                 const float c = lv[pt] - mf;
-                float sum = 0.f;
 #pragma unroll
                 for (int r = 0; r < 16; r++) s[pt][r] = __builtin_amdgcn_exp2f(fmaf(s[pt][r], f[pt], c));
                 if (edge)
 #pragma unroll
                     for (int r = 0; r < 16; r++)
                         if (!(keep >> (16 * pt + r) & 1u)) s[pt][r] = 0.f;
-                uint32_t hi[8], lo[8];
-#pragma unroll
-                for (int i = 0; i < 8; i++) {
-                    const float a = s[pt][2 * i], b = s[pt][2 * i + 1];
-                    sum += a + b;
-                    pieces(a, b, hi[i], lo[i]);
-                }
+                kh8 ph[2], pl[2];
+                const float sum = weigh(s[pt], ph, pl);
                 // (a row with none of the block in sight takes nothing from it, whatever its scale)
                 l += sum == 0.f ? 0.f : sum * inv[pt];
 #pragma unroll
-                for (int k = 0; k < 2; k++) {
-                    const kh8 ph = __builtin_bit_cast(kh8, uint4{hi[4 * k], hi[4 * k + 1], hi[4 * k + 2], hi[4 * k + 3]}),
-                              pl = __builtin_bit_cast(kh8, uint4{lo[4 * k], lo[4 * k + 1], lo[4 * k + 2], lo[4 * k + 3]});
+                for (int k = 0; k < 2; k++)
 #pragma unroll
                     for (int d = 0; d < DT; d++) {
                         const kh8 a = *reinterpret_cast<const kh8 *>(vs + d * 32 * VST + pt * 64 + 32 * k);
-                        o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, ph, o[d], 0, 0, 0);
-                        o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, pl, o[d], 0, 0, 0);
+                        o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, ph[k], o[d], 0, 0, 0);
+                        o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, pl[k], o[d], 0, 0, 0);
                     }
-                }
                 __builtin_amdgcn_sched_barrier(0);
             }
         }
@@ -683,7 +759,7 @@ template <int HD> __global__ void __launch_bounds__(256, kManyPerCu<HD>) kv8_man
     l = xsum<32>(l);
     if (!valid) return;
     // a split's outputs are those of its own positions (0 where it has none in sight)
-    const float inv = p.splits > 1 && m == -INFINITY && l == 0.f ? 0.f : 1.f / (l * kWeight);
+    const float inv = p.splits > 1 && m == -INFINITY && l == 0.f ? 0.f : 1.f / (l * weight_unit);
     const size_t row = (size_t)qi * p.heads + head, at = (size_t)z * p.queries * p.heads + row;
     float *dst = (p.splits > 1 ? p.part + at * HD : p.out + row * HD) + 4 * lh;
 #pragma unroll

@@ -138,3 +138,23 @@ def test_scales_far_apart_everywhere(hip_ctx, heads, kvh, hd, position, queries,
             bound = (2 * e.max() + 2.0 ** -20 + p * 2.0 ** -22) * (w[live] @ v[at][live]) / w.sum() + some
             err = np.abs(got[i, h] - want[i, h])
             assert np.all(err <= bound), (h, i, (err / bound).max())
+
+
+@pytest.mark.parametrize("heads,kvh,hd", [(8, 2, 128), (4, 4, 64), (6, 3, 96), (2, 1, 256)])
+@pytest.mark.parametrize("position,queries", [(60, 1), (60, 9), (5000, 1), (3000, 9), (60, 70), (3000, 70), (2500, 600)])
+@pytest.mark.parametrize("far", [False, True])
+def test_values_whose_sum_passes_binary32(hip_ctx, heads, kvh, hd, position, queries, far):
+    """Values near binary32's end under weights about alike: their mean is a number, their sum is none.  far: with
+    blocks of values 2^-60 times theirs among them."""
+    print("large values", heads, kvh, hd, position, queries, far, flush=True)
+    rng = np.random.default_rng(position + hd)
+    n = position + queries
+    c = oracle.Kv8(kvh, n, hd, rng)
+    c.scales[1][:] = (np.float32(3.39e38) / np.float32(127)) * rng.uniform(0.9, 1, c.scales[1].shape).astype(np.float32)
+    c.codes[1][:] = rng.integers(100, 128, c.codes[1].shape)
+    if far:
+        c.scales[1][:, 1::3] *= np.float32(2.0 ** -60)
+    q = rng.normal(0, 0.1, (queries, heads, hd)).astype(np.float32)
+    want, bound = oracle.kv8_attention(c, q, position, hd ** -0.5)
+    err = np.abs(attend(hip_ctx, c, q, position, hd ** -0.5) - want)
+    assert np.all(err <= bound), (err / bound).max()

@@ -105,6 +105,17 @@ __device__ __forceinline__ void share_of(float scale, float big, float &log_shar
     inverse = __builtin_amdgcn_exp2f(-log_share);
 }
 
+// Four dims' sums of weighted outputs, in 64 bits: the mean of values lies within binary32, their sum may not, nor
+// the products with weights below 1.
+struct Wide4 {
+    double x, y, z, w;
+    __device__ __forceinline__ void add(double f, const float4 &v) {
+        x = fma(f, (double)v.x, x), y = fma(f, (double)v.y, y), z = fma(f, (double)v.z, z), w = fma(f, (double)v.w, w);
+    }
+    __device__ __forceinline__ void shrink(double f) { x *= f, y *= f, z *= f, w *= f; }
+    __device__ __forceinline__ float4 over(double n) const { return make_float4((float)(x * n), (float)(y * n), (float)(z * n), (float)(w * n)); }
+};
+
 struct Kv8Params {
     Kv8Layer c;
     const float *q;
@@ -126,8 +137,10 @@ __device__ __forceinline__ float wave_min_scale(float scale) { return -wave_max_
 // For such scales alone (the first block's 2^-40 of the others': 2048 queries after 14336 positions 1754 us against
 // 993, 9 queries after 16389 35.5 against 26.3, one after 4112 11.1 against 10.4): a block's weights are of its own largest, w = 2^(s - block max), their outputs a
 // product by themselves, which the scale and 2^(block max - max) multiply on their way into the row's:
-// o = o 2^(was - max) + (t 2^(block max - max)) scale.  The pieces then hold what counts of each block.
-//
+// o = o 2^(was - max) + (t 2^(block max - max)) scale.  The pieces then hold what counts of each block.  Sums of
+// 2^31 values past 2^87 would leave binary32: they are taken in units of 2^32, which costs values below 2^-94 bits.
+__device__ __forceinline__ float far_unit(float largest) { return largest >= 0x1p80f ? 0x1p32f : 1.f; }
+
 // One block of a row: its largest score `top` (-infinity: none in sight) in scores' unit f, the row's running
 // maximum m (updated); `was`: what the row's sums shrink by, the result: what the block's do, -1 of a block out of
 // sight, which gives nothing whatever its scale.
@@ -166,7 +179,7 @@ __global__ void __launch_bounds__(256, 1) kv8_few_kernel(Kv8Params p) {
     using F = Few<HD, NR>;
     constexpr int CT = F::CT, P = F::P;
     __shared__ __align__(16) float os[4][NR][HD + 4];
-    __shared__ float ms[4][NR], ls[4][NR];
+    __shared__ float ms[4][NR], ls[4][NR], unit[4];  // unit: of a wavefront's outputs
     const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, i16 = lane & 15, g = lane >> 4;
     const int kvh = blockIdx.x % p.c.nkv, z = blockIdx.y;
     const uint32_t rows = p.queries * (uint32_t)p.group, r0 = blockIdx.x / p.c.nkv * NR;
@@ -376,7 +389,7 @@ __global__ void __launch_bounds__(256, 1) kv8_few_kernel(Kv8Params p) {
     auto compute_far = [&](const Block8<HD> &r, int t) {
         const uint32_t first = block_of(t) * kKv8Block;
         auto of_block = [&](float v) { return __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(v), t & 63)); };
-        const float ks = of_block(ksl), vs = of_block(vsl);
+        const float ks = of_block(ksl), vs = of_block(vsl) / big;
         kf4 s[CT][2];
         scores(r, s);
         kh8 ph[CT][P];
@@ -437,12 +450,17 @@ __global__ void __launch_bounds__(256, 1) kv8_few_kernel(Kv8Params p) {
             for (int d = 0; d < F::DT; d++) o[c][d] = kf4{0.f, 0.f, 0.f, 0.f};
         }
 #pragma unroll 1
+        for (int t = 0; t < nb; t += 64) {
+            load_scales(t);
+            big = fmaxf(big, wave_max_f32(vsl));
+        }
+        big = far_unit(big), weight_unit = 1.f;
+#pragma unroll 1
         for (int t = 0; t < nb; t++) {
             if ((t & 63) == 0) load_scales(t);
             load(x, t);
             compute_far(x, t);
         }
-        big = 1.f, weight_unit = 1.f;
     }
     // the wavefront's rows: both pieces' outputs, the sum over its lanes
     const uint32_t live = rlast - r0 + 1;
@@ -454,33 +472,33 @@ __global__ void __launch_bounds__(256, 1) kv8_few_kernel(Kv8Params p) {
 #pragma unroll
             for (int j = 0; j < 4; j++) {
                 if constexpr (F::PAIRED) {
-                    if (j % 2 == 0) os[wave][2 * g + j / 2][16 * d + i16] = (o[c][d][j] + o[c][d][j + 1]) * weight_unit * big;
+                    if (j % 2 == 0) os[wave][2 * g + j / 2][16 * d + i16] = (o[c][d][j] + o[c][d][j + 1]) * weight_unit;
                 } else
-                    os[wave][16 * c + 4 * g + j][16 * d + i16] = o[c][d][j] * weight_unit * big;
+                    os[wave][16 * c + 4 * g + j][16 * d + i16] = o[c][d][j] * weight_unit;
             }
         if (lane < 16 && (!F::PAIRED || lane % 2 == 0)) {
             const int r = F::PAIRED ? lane / 2 : 16 * c + lane;
             ms[wave][r] = m[c], ls[wave][r] = sum;
         }
     }
+    if (lane == 0) unit[wave] = big;
     __syncthreads();
     for (int u = tid; u < (int)live * (HD / 4); u += 256) {
         const int r = u / (HD / 4), d = 4 * (u % (HD / 4));
         const float mx = fmaxf(fmaxf(ms[0][r], ms[1][r]), fmaxf(ms[2][r], ms[3][r])), mf = finite(mx);
         float sum = 0.f;
-        float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
+        Wide4 a = {};
 #pragma unroll
         for (int w = 0; w < 4; w++) {
             const float al = __builtin_amdgcn_exp2f(ms[w][r] - mf);
-            const float4 v = *reinterpret_cast<const float4 *>(&os[w][r][d]);
             sum = fmaf(al, ls[w][r], sum);
-            a.x = fmaf(al, v.x, a.x), a.y = fmaf(al, v.y, a.y), a.z = fmaf(al, v.z, a.z), a.w = fmaf(al, v.w, a.w);
+            a.add((double)al * unit[w], *reinterpret_cast<const float4 *>(&os[w][r][d]));
         }
         const uint32_t gr = r0 + r, qi = p.query_of(gr);
         const size_t to = (size_t)qi * p.heads + kvh * p.group + (gr - qi * p.group), at = (size_t)z * p.queries * p.heads + to;
         // a split's outputs are those of its own positions (0 where it has none in sight)
         const float n = p.splits > 1 && mx == -INFINITY && sum == 0.f ? 0.f : 1.f / sum;
-        *reinterpret_cast<float4 *>(p.splits > 1 ? p.part + at * HD + d : p.out + to * HD + d) = make_float4(a.x * n, a.y * n, a.z * n, a.w * n);
+        *reinterpret_cast<float4 *>(p.splits > 1 ? p.part + at * HD + d : p.out + to * HD + d) = a.over(n);
         if (p.splits > 1 && d == 0) *reinterpret_cast<float2 *>(p.part_ml + 2 * at) = make_float2(mx, sum);
     }
 }
@@ -650,7 +668,7 @@ template <int HD> __global__ void __launch_bounds__(256, kManyPerCu<HD>) kv8_man
     const bool apart = __builtin_amdgcn_readfirstlane(far_apart(big, small));
     const float weight_unit = apart ? 1.f : kWeight;  // of the outputs' weights
     if (apart) {
-        big = 1.f;
+        big = far_unit(big);
 #pragma unroll 1
         for (int t = t0; t < t1; t++) {
             const uint32_t ba = 2 * (uint32_t)t, bb = min(ba + 1, last_block);
@@ -662,7 +680,7 @@ template <int HD> __global__ void __launch_bounds__(256, kManyPerCu<HD>) kv8_man
                 const uint32_t keep = mask(t, s);
 #pragma unroll
                 for (int pt = 0; pt < 2; pt++) {
-                    const float f = p.c.ks[head0 + (pt ? bb : ba)] * down, vscale = p.c.vs[head0 + (pt ? bb : ba)];
+                    const float f = p.c.ks[head0 + (pt ? bb : ba)] * down, vscale = p.c.vs[head0 + (pt ? bb : ba)] / big;
                     float top = s[pt][0], block_max, was;
 #pragma unroll
                     for (int r = 1; r < 16; r++) top = fmaxf(top, s[pt][r]);
@@ -776,7 +794,7 @@ template <int HD> __global__ void __launch_bounds__(256, kManyPerCu<HD>) kv8_man
 template <int HD> __global__ void __launch_bounds__(256) kv8_join_kernel(const float *__restrict__ part, const float2 *__restrict__ ml,
                                                                        float *__restrict__ out, size_t rows, int splits) {
     constexpr int C = HD / 4, N = 256 / C, Z = 8;  // float4s of a row; splits side by side
-    __shared__ float4 acc[N][C];
+    __shared__ Wide4 acc[N][C];
     __shared__ float weight[kMaxSplits], tops[4], sums[4];
     const size_t row = blockIdx.x;
     const int tid = threadIdx.x, c = tid % C, n = tid / C;
@@ -798,24 +816,21 @@ template <int HD> __global__ void __launch_bounds__(256) kv8_join_kernel(const f
     if ((tid & 63) == 0) sums[tid >> 6] = w;
     __syncthreads();
     w = (sums[0] + sums[1]) + (sums[2] + sums[3]);
-    float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
+    Wide4 a = {};
     for (int from = 0; from < splits; from += N * Z) {
         if (from) load(from);
 #pragma unroll
         for (int i = 0; i < Z; i++)
-            if (from + n + N * i < splits) {
-                const float f = weight[from + n + N * i];
-                a.x = fmaf(f, v[i].x, a.x), a.y = fmaf(f, v[i].y, a.y), a.z = fmaf(f, v[i].z, a.z), a.w = fmaf(f, v[i].w, a.w);
-            }
+            if (from + n + N * i < splits) a.add(weight[from + n + N * i], v[i]);
     }
     if (n < N) acc[n][c] = a;
     __syncthreads();
     if (n) return;
     for (int k = 1; k < N; k++) {
-        const float4 o = acc[k][c];
+        const Wide4 o = acc[k][c];
         a.x += o.x, a.y += o.y, a.z += o.z, a.w += o.w;
     }
-    *reinterpret_cast<float4 *>(out + row * HD + 4 * c) = make_float4(a.x / w, a.y / w, a.z / w, a.w / w);
+    *reinterpret_cast<float4 *>(out + row * HD + 4 * c) = a.over(1.f / w);
 }
 
 // The same for many rows: a thread takes four dims of a row through the splits, four of them under way.
@@ -826,7 +841,7 @@ template <int HD> __global__ void __launch_bounds__(256) kv8_join_rows_kernel(co
     const int d = 4 * (int)(u % C);
     if (row >= rows) return;
     float m = -INFINITY, l = 0.f;
-    float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
+    Wide4 a = {};
     for (int z = 0; z < splits; z += Z) {
         float2 w[Z];
         float4 v[Z];
@@ -841,15 +856,15 @@ template <int HD> __global__ void __launch_bounds__(256) kv8_join_rows_kernel(co
         for (int i = 0; i < Z; i++) top = fmaxf(top, w[i].x);
         const float mf = finite(top), al = __builtin_amdgcn_exp2f(m - mf);
         m = top;
-        a.x *= al, a.y *= al, a.z *= al, a.w *= al, l *= al;
+        a.shrink(al), l *= al;
 #pragma unroll
         for (int i = 0; i < Z; i++) {
             const float f = z + i < splits ? __builtin_amdgcn_exp2f(w[i].x - mf) * w[i].y : 0.f;
-            if (z + i < splits) a.x = fmaf(f, v[i].x, a.x), a.y = fmaf(f, v[i].y, a.y), a.z = fmaf(f, v[i].z, a.z), a.w = fmaf(f, v[i].w, a.w);
+            if (z + i < splits) a.add(f, v[i]);
             l += f;
         }
     }
-    *reinterpret_cast<float4 *>(out + row * HD + d) = make_float4(a.x / l, a.y / l, a.z / l, a.w / l);
+    *reinterpret_cast<float4 *>(out + row * HD + d) = a.over(1.f / l);
 }
 
 }  // namespace

@@ -8,7 +8,8 @@
 // Three launches, none of which sorts the row:
 //   stats   slices of 2048 logits: maximum, minimum and mean, from which a linear scale of 256 bins
 //           is laid over the values, the largest in bin 0;
-//   bins    per slice the bins' sums of weights, and its logits in the order of their bins;
+//   bins    per slice the bins' sums of weights (with top-k, which comes first: counts of the logits that may
+//           have a weight), and its logits in the order of their bins;
 //   finish  a workgroup per row: the bin in which a target lies, then 1024 finer bins of that bin's
 //           logits, then the few logits of the finer bin in order.  With top-k the bins above the k-th
 //           logit are sorted in LDS instead, and everything else is prefix sums of at most 1024.
@@ -90,6 +91,12 @@ struct Policy {
         const int bits = top_k > 1 ? 32 - __clz((int)top_k - 1) : 0;
         unit = __longlong_as_double((long long)(1023 + 62 - bits) << 52);
         none = fmaxf(logf(p.o.min_p), -0.6931472f * (float)(63 - bits)) - 0.01f;
+    }
+    // With top-k: logits below it have a weight of 0, penalised or not, and are no candidates.  (The largest weight's
+    // logit is at least the largest logit penalised; a penalty raises none.)
+    __device__ float least_logit(const SampleRows &p, float largest) const {
+        const float base = p.recent ? penalised(largest, p.o.repeat_penalty) : largest;
+        return base + 1.001f * none * p.o.temperature - 1e-6f * fabsf(base);
     }
     // (the same operations wherever it is called: the sums of the bins and of their logits agree)
     __device__ __forceinline__ u64 weight(float a, float mx) const {
@@ -221,10 +228,11 @@ __global__ void __launch_bounds__(256) draw_bins_kernel(SampleRows p) {
     for (uint32_t i = threadIdx.x & 63; i < slices; i += 64)
         mx = fmaxf(mx, all[i].x), mn = fminf(mn, all[i].y), sum += all[i].z, known += all[i].w;
     mx = wave_max_f32(mx), mn = -wave_max_f32(-mn), sum = wave_sum(sum), known = wave_sum(known);
-    // the scale: with top-k down to the mean; else to the lowest, or to where weights are 0, or, where
-    // few lie far below the others, as far below the mean as half again the largest is above it
-    const float above = mx - sum / known;
-    float range = policy.limited ? above : fminf(fminf(43.7f * p.o.temperature, mx - mn), 2.5f * above);
+    // the scale: with top-k down to the mean, or to where weights are surely 0 (which a logit of -10000 or one far
+    // above the others would take the mean past); else to the lowest, or to where weights are 0, or, where few lie
+    // far below the others, as far below the mean as half again the largest is above it
+    const float above = mx - sum / known, least = policy.limited ? policy.least_logit(p, mx) : -INFINITY;
+    float range = policy.limited ? fminf(above, mx - least) : fminf(fminf(43.7f * p.o.temperature, mx - mn), 2.5f * above);
     const float per_bin = range > 0.f && fabsf(mx) < INFINITY ? (float)kBins / range : 0.f;
     if (blockIdx.x == 0 && threadIdx.x == 0) w.head->max = mx, w.head->per_bin = per_bin;
     const bool ordering = policy.limited || policy.sorted;  // else the draw goes by the ids: the slice's sum is all
@@ -234,7 +242,7 @@ __global__ void __launch_bounds__(256) draw_bins_kernel(SampleRows p) {
     for (int i = 0; i < kSliceLogits / 256; i++) {
         float t;
         const int b = bin_of(s.a[i], mx, per_bin, t);
-        const u64 v = !(fabsf(mx) < INFINITY) ? 0ull : policy.limited ? (s.a[i] > -INFINITY ? 1ull : 0ull) : policy.weight(s.a[i], mx);
+        const u64 v = !(fabsf(mx) < INFINITY) ? 0ull : policy.limited ? (s.a[i] > -INFINITY && s.a[i] >= least ? 1ull : 0ull) : policy.weight(s.a[i], mx);
         at[i] = 0xFFFFFFFFu;  // no candidate: in no bin
         if (v && ordering) {
             if (!policy.limited) atomicAdd(&sums[b], v);
@@ -656,7 +664,7 @@ __global__ void __launch_bounds__(kThreads) draw_finish_kernel(SampleRows p) {
     };
 
     if (policy.limited) {
-        const uint32_t k = (uint32_t)(total < policy.top_k ? total : policy.top_k);  // candidates above -infinity
+        const uint32_t k = (uint32_t)(total < policy.top_k ? total : policy.top_k);  // (the binned ones)
         if (tid == 0) f.count = 0;
         for (run_counts(); f.runs[64 * quarters - 1] < k; run_counts()) load_counts();
         const int last = bin_reaching(k, &before);

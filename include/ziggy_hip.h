@@ -373,7 +373,17 @@ size_t ziggy_hip_kv8_scales_length(uint32_t layers, uint32_t head_count_kv, uint
  * (the earlier codes are then rounded to the new scale), and never shrinks.
  * Rows behind the last one keep their codes.  A row with an infinity or NaN
  * makes its block's scale NaN, and every row of the block reads as NaN until
- * the block starts anew. */
+ * the block starts anew.
+ * A value of a block stored at once is off by at most half the scale; every
+ * later store that makes the scale grow rounds the block's codes once more, so
+ * after g of them it is off by at most (1 + g) / 2 of the scale.
+ * Rows that are taken back (rejected drafts, a rewind) are overwritten by the
+ * next store at an earlier position, but what they made of the block stays: its
+ * scale, the rounding of the rows before them, a NaN.  A caller that takes rows
+ * back, or wants every row rounded once, keeps the f32 rows of the open block
+ * and stores from the block's first position each time (position / 32 * 32, its
+ * rows so far ahead of the new ones): the block starts anew, and the cache is
+ * that of the rows that were kept, bit for bit. */
 int ziggy_hip_kv8_store(ZiggyHipContext *ctx, const ZiggyHipKv8Cache *cache, const ZiggyHipBuffer *k,
                         size_t k_offset_bytes, const ZiggyHipBuffer *v, size_t v_offset_bytes, size_t row_stride,
                         uint32_t layer, uint32_t position, uint32_t rows, char *error_message,

@@ -158,3 +158,26 @@ def test_values_whose_sum_passes_binary32(hip_ctx, heads, kvh, hd, position, que
     want, bound = oracle.kv8_attention(c, q, position, hd ** -0.5)
     err = np.abs(attend(hip_ctx, c, q, position, hd ** -0.5) - want)
     assert np.all(err <= bound), (err / bound).max()
+
+
+@pytest.mark.parametrize("which", [0, 1])
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("position,queries", [(100, 1), (92, 9), (60, 80), (2000, 1), (1990, 100)])
+def test_a_marked_block_beside_scales_far_apart(hip_ctx, which, hd, position, queries):
+    """A NaN scale of K or V in the block of positions 96 .. 127 of one kv head: NaN in every row that sees it, in no
+    other; other rows as without it."""
+    print("marked beside far", which, hd, position, queries, flush=True)
+    rng = np.random.default_rng(position + hd)
+    n = position + queries
+    c = oracle.Kv8(2, n, hd, rng)
+    c.scales[1][:, ::2] *= np.float32(2.0 ** -50)
+    q = rng.normal(0, 1, (queries, 4, hd)).astype(np.float32)
+    plain = attend(hip_ctx, c, q, position, hd ** -0.5)
+    assert np.isfinite(plain).all()
+    c.scales[which][1, 3] = np.nan
+    got = attend(hip_ctx, c, q, position, hd ** -0.5)
+    seen = np.arange(position, n) >= 96
+    marked = np.broadcast_to((seen[:, None] & (np.arange(4) >= 2))[..., None], got.shape)
+    assert np.array_equal(np.isnan(got), marked)
+    want, bound = oracle.kv8_attention(c, q, position, hd ** -0.5)
+    assert np.all(np.abs(got - want)[~marked] <= bound[~marked])

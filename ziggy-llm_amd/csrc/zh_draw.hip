@@ -12,17 +12,18 @@
 //           have a weight), and its logits in the order of their bins;
 //   finish  a workgroup per row: the bin in which a target lies, then 1024 finer bins of that bin's
 //           logits, then the few logits of the finer bin in order.  With top-k the bins above the k-th
-//           logit are sorted in LDS instead, and everything else is prefix sums of at most 1024.
+//           logit are sorted instead (in registers; through LDS what lies in different wavefronts), and
+//           everything else is prefix sums of at most 1024.
 // What is left of a row at the end, up to 64 logits, is a wavefront's work without a barrier.  Where a
 // finer bin holds more than 1024 logits, equal ones or nearly, their values go digit by digit, and equal
-// ones by the counts of their slices.  (128256 logits rounded to quarters, nucleus of 0.9: 30-33 us; all
-// equal: 0.50 ms.)
+// ones by the counts of their slices.  (128256 logits rounded to quarters, nucleus of 0.9: 29 us; all
+// equal: 0.51 ms, top-k 0.31.)
 //
 // What bounds it: three dependent launches, each a chain of memory round trips, barriers and LDS.  One row
-// of 128256 logits, top-k 40 of 0.9: 15.4-16.4 us (1.7, 4.8 and 5.3 of the launches); 16 rows of 151936, nucleus
-// of 0.95: 24.0 (2.9, 5.9 and 12.4; the logits' 9.7 MB are 2.1 us of it).  Of the finish, 3 us were barriers
+// of 128256 logits, top-k 40 of 0.9: 16.2 us a pass (the launches' least of 60: 1.8, 5.4 and 6.1); 16 rows of 151936,
+// nucleus of 0.95: 23.7 (3.0, 6.2 and 12.9; the logits' 9.7 MB are 2.1 us of it).  Of the finish, 3 us were barriers
 // of 16 wavefronts in the sums and sorts that a wavefront does now, 2 the tables of all bins where a top-k
-// lies in the first quarter.  A row whole in one workgroup, in one launch: 42 us at 32000 logits, these 19.
+// lies in the first quarter.  A row whole in one workgroup, in one launch: 42 us at 32000 logits, these 21.
 #include "zh_longctx.h"
 
 namespace zh {

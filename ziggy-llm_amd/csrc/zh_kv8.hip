@@ -8,9 +8,9 @@
 // near values), against half the scale.  The maximum is taken of the bits of |x|, in which infinities and
 // NaN are the largest.
 //
-// What bounds it: memory for a prompt (4095 rows of 8 heads of 128, K and V, 42 MB: 11.7-13.9 us, 3.0-3.6
-// TB/s; the read-back of as many 6.3-7.5 us), the chain of load, maximum, scale and store for one row (3.6
-// us; 5.7 with the exact decision and the rescaling unrolled in line, 2000 instructions more to fetch).
+// What bounds it: memory for a prompt (4095 rows of 8 heads of 128, K and V, 42 MB: mean 13.8 us, least 12.4, 3.0-3.4
+// TB/s; the read-back of as many 7.4 and 6.5), the chain of load, maximum, scale and store for one row (3.5
+// us, least 3.1; 5.7 with the exact decision and the rescaling unrolled in line, 2000 instructions more to fetch).
 // Tried and slower: two blocks a workgroup (17.7 us), V's words from four rows per thread without LDS
 // (17.0), workgroups ordered heads first (15.4; all against 14.7 then).
 #include "zh_longctx.h"

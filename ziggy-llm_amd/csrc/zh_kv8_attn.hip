@@ -12,11 +12,11 @@
 // tiles of 64 positions in LDS.  Both split the positions over workgroups where rows alone leave CUs
 // idle; a second launch joins the splits in their order, so results don't change from run to run.
 //
-// What bounds them (32 heads of 128 over 8 kv heads): one query of 131071 positions memory, 268 MB in 47.6
-// us, 5.6 TB/s, and 4.4 of the join; of 4113 positions the chain of loads, products and exchange (7.0 us,
-// of which 1.5 are its one block, and 2.2 of the join); 9 queries of 16398 positions vector issue and memory
-// about alike (22.3 and 3.9); 2048 queries of 14336 to 16384 positions the matrix cores, 936 us, 1.10 PFLOP/s
-// with both pieces counted.
+// What bounds them (32 heads of 128 over 8 kv heads; mean and least of 60 launches): one query of 131071
+// positions memory, 268 MB in 49.9 (47.9) us, 5.4 TB/s, and 4.8 (4.3) of the join; of 4113 positions the chain
+// of loads, products and exchange, 7.4 (7.0), of which 1.5 are its one block, and 3.1 (2.4) of the join; 9 queries
+// of 16398 positions vector issue and memory about alike, 22.7 (22.0) and 4.5 (3.8); 2048 queries of 14336 to 16384
+// positions the matrix cores, 992 (958), 1.04 PFLOP/s with both pieces counted.
 #include <algorithm>
 #include <cmath>
 
@@ -134,11 +134,13 @@ __device__ __forceinline__ bool far_apart(float largest, float smallest) { retur
 constexpr float kNoScale = INFINITY;  // the smallest of none
 __device__ __forceinline__ float wave_min_scale(float scale) { return -wave_max_f32(scale > 0.f ? -scale : -kNoScale); }
 
-// For such scales alone (the first block's 2^-40 of the others': 2048 queries after 14336 positions 1754 us against
-// 993, 9 queries after 16389 35.5 against 26.3, one after 4112 11.1 against 10.4): a block's weights are of its own largest, w = 2^(s - block max), their outputs a
-// product by themselves, which the scale and 2^(block max - max) multiply on their way into the row's:
+// For such scales alone: a block's weights are of its own largest, w = 2^(s - block max), their outputs t a
+// product by themselves, which 2^(block max - max) and the scale multiply on their way into the row's:
 // o = o 2^(was - max) + (t 2^(block max - max)) scale.  The pieces then hold what counts of each block.  Sums of
 // 2^31 values past 2^87 would leave binary32: they are taken in units of 2^32, which costs values below 2^-94 bits.
+// (A pass where the first block's values are 2^-40 of the others': 2048 queries after 14336 positions 1779 us against
+// 994, 9 queries after 16389 36.3 against 26.4, one after 4112 11.3 against 10.3.  A row at a time without matrix
+// cores: 288 ms, 1106 and 57 us.)
 __device__ __forceinline__ float far_unit(float largest) { return largest >= 0x1p80f ? 0x1p32f : 1.f; }
 
 // One block of a row: its largest score `top` (-infinity: none in sight) in scores' unit f, the row's running

@@ -5,8 +5,8 @@
 // before it is rounded to 32 bits (at position 10^6 a 32-bit angle would be off by 0.06 rad); what the
 // rounding leaves off enters sine and cosine to first order.
 //
-// What bounds it: memory for a prompt (4096 rows of 40 heads of 128, 168 MB: 33.6 us, 5.0 TB/s; 59.4 with
-// 4-byte accesses, a head and a row's angles at a time), the launch for a step (40 heads of 128: 3.0 us).
+// What bounds it: memory for a prompt (4096 rows of 40 heads of 128, 168 MB: 34.0 us, 4.9 TB/s; 59.4 with
+// 4-byte accesses, a head and a row's angles at a time), the launch for a step (40 heads of 128: 3.1-3.5 us).
 #include "zh_longctx.h"
 
 namespace zh {

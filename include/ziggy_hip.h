@@ -670,6 +670,9 @@ int ziggy_hip_sample_logits(const float *logits, uint32_t count, const uint32_t 
  * exact integers of 2^-s (s = 62 less the bits of the candidates' count: at
  * least 44), so a row's token depends on nothing but its inputs; a weight below
  * 2^-(s+1) of the largest counts as 0, and a token of weight 0 is not drawn.
+ * Where the limits go by weight, the order is the logits': candidates whose
+ * logits differ by less than 64-bit weights tell (1e-16 of the temperature)
+ * stand in it, where the host sampler leaves them as they come.
  * Logits of NaN count as -infinity.  A row without a finite largest logit
  * gives its first candidate of the largest value, as the host sampler. */
 int ziggy_hip_sample_rows_f32(ZiggyHipContext *ctx, const ZiggyHipBuffer *logits, size_t row_stride,

@@ -51,6 +51,14 @@ def test_the_largest_logit_penalised_below_all_others(hip_ctx):
             check(hip_ctx, x, np.array([u]), dict(kw, penalty=3.0), recent, host=u > 0)
 
 
+@pytest.mark.parametrize("kw", [dict(top_p=0.5), dict(top_k=40, top_p=0.6), dict(top_k=900, top_p=0.8, min_p=0.5), dict(top_p=0.9, temperature=3.0)], ids=str)
+def test_logits_whose_weights_are_equal(hip_ctx, kw):
+    """Logits of 1e-30: every weight is 1 in 64 bits, the nucleus and the draw go by the logits (the host sampler's by
+    the ids)."""
+    rng = np.random.default_rng(9)
+    check(hip_ctx, (rng.normal(0, 1, (5, 5000)) * 1e-30).astype(np.float32), rng.random(5), kw, host=False)
+
+
 @pytest.mark.parametrize("top_k", [40, 500])
 @pytest.mark.parametrize("name", list(ROWS))
 def test_time(hip_ctx, name, top_k):

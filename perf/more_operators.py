@@ -15,7 +15,8 @@ The cache's layout, bytes of one layer, G = head dim / 32:
   V codes  [page][kv head][half 2][g 4][d 16][j 8][t G]: dims 32 t + d (lower half) and 32 t + 16 + d of position
            32 half + 8 g + j
   scales   [page][kv head][position 64][t G]: 2^(byte - 127)
-A code is a sign and one of 0, .5, 1, 1.5, 2, 3, 4, 6.
+A code is a sign and one of 0, .5, 1, 1.5, 2, 3, 4, 6; a scale the least power of two, from 2^-96 to 2^92, that is at
+least a seventh of the largest of its 32 values.
 """
 import math
 import os
@@ -304,8 +305,8 @@ def _in_four_bits(x):
     """(codes, scale bytes) of float32 rows, 32 values a scale."""
     x = x.reshape(*x.shape[:-1], -1, 32)
     part, power = torch.frexp(x.abs().amax(dim=-1, keepdim=True))  # largest = part * 2^power, part in [.5, 1)
-    power = torch.where(part <= 0.875, power - 3, power - 2).clamp(-120, 125)
-    power = torch.where(part > 0, power, torch.full_like(power, -120))
+    power = torch.where(part <= 0.875, power - 3, power - 2).clamp(-96, 92)
+    power = torch.where(part > 0, power, torch.full_like(power, -96))
     a = torch.ldexp(x.double().abs(), -power)
     step = torch.where(a < 2, 0.5, torch.where(a < 4, 1.0, 2.0))
     a = (torch.round(a / step) * step).clamp(max=6)
@@ -471,7 +472,7 @@ def _exact_heads(c, x, at, weights):
 def _exact_four_bits(x):
     """Each value of 32 that share a scale as the nearest one that 4 bits hold."""
     x = x.float().double().reshape(*x.shape[:-1], -1, 32)
-    scale = torch.exp2(torch.ceil(torch.log2(x.abs().amax(dim=-1, keepdim=True).clamp(min=2.0 ** -126) / 7)).clamp(-120, 125))
+    scale = torch.exp2(torch.ceil(torch.log2(x.abs().amax(dim=-1, keepdim=True).clamp(min=2.0 ** -126) / 7)).clamp(-96, 92))
     near, best = torch.full_like(x, math.inf), torch.zeros_like(x)
     for code in (0, 2, 4, 6, 1, 3, 5, 7):  # even ones first: they win ties
         off = (x.abs() - VALUES[code] * scale).abs()

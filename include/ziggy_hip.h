@@ -404,6 +404,106 @@ int ziggy_hip_kv8_attention_f32(ZiggyHipContext *ctx, const ZiggyHipKv8Cache *ca
                                 uint32_t position, uint32_t queries, uint32_t window, float scale,
                                 char *error_message, size_t error_message_len);
 
+/* ---- operators of a step that serves several sequences (no counterpart in the reference) ----
+ * The caller's sequences share one pool of pages of ZIGGY_HIP_KV_PAGE_POSITIONS
+ * (64) positions.  A batch says which rows of the step's inputs are whose; its
+ * tables are device memory, so that a captured step is replayed with other
+ * ones.  What they hold can't be checked on the host: the kernels take no index
+ * from them that lies outside the buffers (see below), and nothing else of
+ * them is refused. */
+
+/* Sequence s has rows row_starts[s] .. row_starts[s + 1] - 1 (none, one or
+ * many; sequences' rows follow each other from row 0 on), which are the last of
+ * its lengths[s] positions: row row_starts[s] + i is at position
+ * lengths[s] - (row_starts[s + 1] - row_starts[s]) + i.  Position t lies in
+ * pool page page_table[s * pages_per_sequence + t / 64].  Rows behind the last
+ * sequence's are no one's: what a call would write of them stays as it was.
+ * max_rows and max_length: what no sequence has more rows and positions than
+ * (0: `rows`, and all that its pages hold); the kernels' grids follow them, so
+ * tight ones are faster.  Rows and positions past them, rows ahead of position
+ * 0, and positions whose page is not one of the pool's are passed over: not
+ * stored, and not attended to.  A sequence's pages are its own while its rows
+ * are appended; sequences may share pages that are only read. */
+typedef struct {
+    const ZiggyHipBuffer *page_table; /* u32 [sequences][pages_per_sequence]; entries past a sequence's length are not read */
+    const ZiggyHipBuffer *row_starts; /* u32 [sequences + 1], ascending */
+    const ZiggyHipBuffer *lengths;    /* u32 [sequences] */
+    uint32_t sequences, pages_per_sequence; /* at most 65536, and 2^24 pages */
+    uint32_t rows;                    /* rows of the step's inputs and outputs */
+    uint32_t max_rows, max_length;
+} ZiggyHipBatch;
+
+/* What a model does to its query and key heads ahead of the attention:
+ *   x -> x (w + weight_offset) / sqrt(mean(x^2) + eps)   (w: q_norm or k_norm, head_dim floats; NULL: x)
+ * over the head's head_dim values, then the rotation (NULL: none). */
+typedef struct {
+    const ZiggyHipRopeDesc *rope;
+    const ZiggyHipBuffer *freq_factors; /* as for ziggy_hip_rope_rows_f32, or NULL */
+    const ZiggyHipBuffer *q_norm, *k_norm;
+    float eps, weight_offset;
+} ZiggyHipHeadsDesc;
+
+/* Norms and rotates `rows` rows in one pass: the first q_heads heads of a row
+ * with q_norm, the k_heads behind them with k_norm, as
+ * ziggy_hip_rms_norm_per_head_f32 and ziggy_hip_rope_rows_f32 one after the
+ * other (positions, strides, offsets and in-place rows as there).  heads->rope
+ * is not NULL. */
+int ziggy_hip_norm_rope_rows_f32(ZiggyHipContext *ctx, const ZiggyHipHeadsDesc *heads, const ZiggyHipBuffer *src,
+                                 size_t src_offset_bytes, size_t src_row_stride, ZiggyHipBuffer *dst,
+                                 size_t dst_offset_bytes, size_t dst_row_stride, const ZiggyHipBuffer *positions,
+                                 uint32_t first_position, uint32_t rows, uint32_t q_heads, uint32_t k_heads,
+                                 char *error_message, size_t error_message_len);
+
+/* K/V cache in 4 bits, in pages.  Of each position and kv head, 32 consecutive
+ * dims share a scale 2^x, x the least integer of -96 .. 92 with max|v| <= 7 2^x
+ * (92 where that is not enough); a value is a sign and one of 0, 0.5, 1, 1.5,
+ * 2, 3, 4, 6 times the scale, the nearest (ties to the even of these eight;
+ * past 6: 6).  A position depends on no other: rows may be taken back and
+ * stored again.  A position of a kv head whose key or value holds an infinity
+ * or a NaN is marked: all of its key and value read as NaN, and so does every
+ * output that attends to it.  With G = head_dim / 32, for each layer:
+ *   k_codes  [page][kv head][position 64][g 4][t G][4]: dims 32 t + 8 g .. + 7, the lower half of a byte first
+ *   v_codes  [page][kv head][half 2][g 4][d 16][j 8][t G]: dims 32 t + d (lower half of the byte) and 32 t + 16 + d
+ *            of position 32 half + 8 g + j
+ *   k_scales, v_scales [page][kv head][position 64][t G]: x + 127 (a marked position: 255 in k_scales)
+ * codes: bit 3 the sign, bits 2 .. 0 which of the eight.  A cache starts as any
+ * bytes at all: what was never stored is not read into a result. */
+typedef struct {
+    ZiggyHipBuffer *k_codes, *k_scales, *v_codes, *v_scales;
+    uint32_t layers, head_count_kv, head_dim, pages; /* head_dim 64, 96, 128 or 256; at most 2^24 pages */
+} ZiggyHipKv4Cache;
+/* Bytes of each codes and of each scales buffer of such a cache (0: a shape that is not served). */
+size_t ziggy_hip_kv4_codes_length(uint32_t layers, uint32_t head_count_kv, uint32_t head_dim, uint32_t pages);
+size_t ziggy_hip_kv4_scales_length(uint32_t layers, uint32_t head_count_kv, uint32_t head_dim, uint32_t pages);
+/* Appends the batch's rows to a layer: keys normalised and rotated as `heads`
+ * says (NULL: as they are), values as they are.  The rows lie in `src`,
+ * row_stride apart, head_count_kv * head_dim floats from k_offset_bytes and
+ * from v_offset_bytes on.  With q_heads > 0 the query heads of the same rows,
+ * from q_offset_bytes on, are normalised and rotated on the way, into q_out
+ * (q_out_row_stride apart from q_out_offset_bytes on; src itself, at the same
+ * offset and stride, turns them in place).  Keys are computed in 64 bits and
+ * rounded to binary32 before they are rounded to 4 bits. */
+int ziggy_hip_kv4_append(ZiggyHipContext *ctx, const ZiggyHipKv4Cache *cache, uint32_t layer, const ZiggyHipBatch *batch,
+                         const ZiggyHipHeadsDesc *heads, const ZiggyHipBuffer *src, size_t k_offset_bytes,
+                         size_t v_offset_bytes, size_t row_stride, uint32_t q_heads, size_t q_offset_bytes,
+                         ZiggyHipBuffer *q_out, size_t q_out_offset_bytes, size_t q_out_row_stride,
+                         char *error_message, size_t error_message_len);
+/* Reads the batch's rows back as f32 ([rows][head_count_kv * head_dim]); a
+ * batch of one sequence with as many rows as positions reads all of it. */
+int ziggy_hip_kv4_load_f32(ZiggyHipContext *ctx, const ZiggyHipKv4Cache *cache, uint32_t layer,
+                           const ZiggyHipBatch *batch, ZiggyHipBuffer *k_out, ZiggyHipBuffer *v_out,
+                           char *error_message, size_t error_message_len);
+/* Attention of the batch's rows (head_count heads each, q_row_stride apart from
+ * q_offset_bytes on, already rotated, their K/V appended).  The row at position
+ * p attends to its sequence's positions up to p, or, with window > 0, to the
+ * last `window` of them; a row that none is left for gets zeros.  output:
+ * [rows][head_count * head_dim].  head_count is a multiple of the cache's
+ * head_count_kv (at most 64 times as many). */
+int ziggy_hip_kv4_attention_f32(ZiggyHipContext *ctx, const ZiggyHipKv4Cache *cache, uint32_t layer,
+                                const ZiggyHipBatch *batch, const ZiggyHipBuffer *q, size_t q_offset_bytes,
+                                size_t q_row_stride, ZiggyHipBuffer *output, uint32_t head_count, uint32_t window,
+                                float scale, char *error_message, size_t error_message_len);
+
 /* ---- decode session (replaces the Zig gpu.Session, runtime/gpu/session.zig:27-651,
  * which drives the entry points above one dispatch at a time).  The session
  * uploads the weights once (DenseTensorStore.prewarm,
@@ -680,6 +780,22 @@ int ziggy_hip_sample_rows_f32(ZiggyHipContext *ctx, const ZiggyHipBuffer *logits
                               const ZiggyHipSamplingOptions *options, const ZiggyHipBuffer *uniforms,
                               ZiggyHipBuffer *out_tokens, uint32_t rows, uint32_t vocab, char *error_message,
                               size_t error_message_len);
+
+/* What the sampler's logits say of given tokens: out_logprobs[r] = x_t - ln sum
+ * exp(x) for t = tokens[r] (u32) of logits row r ([rows][vocab], row_stride
+ * floats apart; vocab at most 262144), NaN where t is no token of the vocabulary.
+ * out_entropy (or NULL): -sum p ln p of the row in nats.  With top_count > 0
+ * (at most 64, and vocab) out_top_tokens and out_top_logprobs [rows][top_count]:
+ * the best tokens, highest first, ties to the lower id, and their log
+ * probabilities.  Logits of NaN count as -infinity, as for the sampler.  A row whose
+ * largest logit is infinite either way has log probabilities and entropy of NaN
+ * (its top tokens are in order all the same).  Exponentials are binary32, sums
+ * and logarithms 64 bits. */
+#define ZIGGY_HIP_MAX_TOP_LOGPROBS 64
+int ziggy_hip_token_logprobs_f32(ZiggyHipContext *ctx, const ZiggyHipBuffer *logits, size_t row_stride,
+                                 const ZiggyHipBuffer *tokens, ZiggyHipBuffer *out_logprobs, ZiggyHipBuffer *out_entropy,
+                                 uint32_t top_count, ZiggyHipBuffer *out_top_tokens, ZiggyHipBuffer *out_top_logprobs,
+                                 uint32_t rows, uint32_t vocab, char *error_message, size_t error_message_len);
 
 /* One decode step of `token` whose output is a token drawn on the device from
  * the step's logits, as ziggy_hip_sample_rows_f32 draws it (its options, its

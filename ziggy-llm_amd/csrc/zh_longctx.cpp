@@ -4,39 +4,12 @@
 
 #include <new>
 
+#include "zh_args.h"
 #include "zh_longctx.h"
 
 using namespace zh;
 
 namespace {
-
-#define ZH_REFUSE(cond, ...)                      \
-    if (cond) {                                   \
-        set_err(err, err_len, __VA_ARGS__);       \
-        return ZIGGY_HIP_INVALID_ARGUMENT;        \
-    }
-
-// a * b + c, or SIZE_MAX where it does not fit
-size_t span(size_t a, size_t b, size_t c = 0) {
-    size_t r;
-    return __builtin_mul_overflow(a, b, &r) || __builtin_add_overflow(r, c, &r) ? SIZE_MAX : r;
-}
-
-// `need` bytes of b from `off` on, on the context's device
-bool in_buffer(const ZiggyHipContext *ctx, const ZiggyHipBuffer *b, size_t need, size_t off = 0) {
-    return b && b->ptr && b->device == ctx->device && off <= b->len && need <= b->len - off;
-}
-
-// the bytes of `rows` rows of `width` floats, `stride` floats apart
-size_t rows_bytes(size_t rows, size_t width, size_t stride) {
-    const size_t floats = span(rows - 1, stride, width);
-    return span(floats, 4);
-}
-
-bool overlap(const void *a, size_t na, const void *b, size_t nb) {
-    const uintptr_t x = (uintptr_t)a, y = (uintptr_t)b;
-    return x < y ? y - x < na : x - y < nb;
-}
 
 bool kv8_shape(uint32_t layers, uint32_t nkv, uint32_t hd, uint32_t context) {
     return layers && nkv && nkv <= 1024 && context && context <= 0x7FFFFFE0u && (hd == 64 || hd == 96 || hd == 128 || hd == 256);
@@ -79,6 +52,36 @@ bool meets_cache(const ZiggyHipKv8Cache *c, const void *p, size_t n) {
 }  // namespace
 
 namespace zh {
+
+const char *rope_refusal(const ZiggyHipRopeDesc &d) {
+    if (d.head_dim == 0 || d.head_dim % 2 || d.head_dim > 512 || d.rope_dim < 2 || d.rope_dim % 2 || d.rope_dim > d.head_dim ||
+        d.rope_style > 1 || d.scaling > ZIGGY_HIP_ROPE_BANDS)
+        return "unsupported rope shape";
+    if (!(d.freq_base > 0) || !isfinite(d.freq_base) || !isfinite(d.magnitude)) return "invalid rope frequencies";
+    if (d.scaling != ZIGGY_HIP_ROPE_NONE && (!(d.factor > 0) || !isfinite(d.factor))) return "invalid rope factor";
+    if (d.scaling >= ZIGGY_HIP_ROPE_YARN && (d.original_context == 0 || !(d.low > 0) || !(d.high > d.low) || !isfinite(d.high)))
+        return "invalid rope blend";
+    if (d.scaling == ZIGGY_HIP_ROPE_YARN && !(d.freq_base > 1)) return "the YaRN blend needs a base above 1";
+    return nullptr;
+}
+
+RopeFreq rope_freq(const ZiggyHipRopeDesc &d) {
+    RopeFreq f{};
+    const double base = d.freq_base, dim = d.rope_dim, turns = 6.283185307179586476925;
+    f.exponent = -2.0 * log2(base) / dim;
+    f.inv_factor = d.scaling == ZIGGY_HIP_ROPE_NONE ? 1.0 : 1.0 / (double)d.factor;
+    if (d.scaling == ZIGGY_HIP_ROPE_YARN) {
+        auto pair_of = [&](double t) { return dim * log(d.original_context / (turns * t)) / (2.0 * log(base)); };
+        const double lo = fmax(0.0, floor(pair_of(d.high))), hi = fmin(dim - 1.0, ceil(pair_of(d.low)));
+        const double run = fmax(0.001, hi - lo);
+        f.a = 1.0 + lo / run, f.b = -1.0 / run;
+    } else if (d.scaling == ZIGGY_HIP_ROPE_BANDS) {
+        const double run = (double)d.high - (double)d.low;
+        f.a = -(double)d.low / run, f.b = (double)d.original_context / run;
+        f.by_turns = 1;
+    }
+    return f;
+}
 
 const char *sample_refusal(const ZiggyHipSamplingOptions &o, uint32_t vocab) {
     if (vocab == 0 || vocab > 262144) return "sampling takes rows of 1 to 262144 logits";
@@ -128,15 +131,8 @@ int ziggy_hip_rope_rows_f32(ZiggyHipContext *ctx, const ZiggyHipRopeDesc *d, con
                             const ZiggyHipBuffer *positions, uint32_t first, const ZiggyHipBuffer *factors, uint32_t rows,
                             uint32_t heads, char *err, size_t err_len) {
     ZH_REFUSE(!ctx || !d, "null context or rope description");
-    ZH_REFUSE(d->head_dim == 0 || d->head_dim % 2 || d->head_dim > 512 || d->rope_dim < 2 || d->rope_dim % 2 ||
-                  d->rope_dim > d->head_dim || d->rope_style > 1 || d->scaling > ZIGGY_HIP_ROPE_BANDS,
-              "unsupported rope shape");
-    ZH_REFUSE(!(d->freq_base > 0) || !isfinite(d->freq_base) || !isfinite(d->magnitude), "invalid rope frequencies");
-    ZH_REFUSE(d->scaling != ZIGGY_HIP_ROPE_NONE && (!(d->factor > 0) || !isfinite(d->factor)), "invalid rope factor");
-    ZH_REFUSE(d->scaling >= ZIGGY_HIP_ROPE_YARN &&
-                  (d->original_context == 0 || !(d->low > 0) || !(d->high > d->low) || !isfinite(d->high)),
-              "invalid rope blend");
-    ZH_REFUSE(d->scaling == ZIGGY_HIP_ROPE_YARN && !(d->freq_base > 1), "the YaRN blend needs a base above 1");
+    const char *why = rope_refusal(*d);
+    ZH_REFUSE(why, "%s", why);
     ZH_REFUSE(rows == 0 || heads == 0 || heads > 65536, "rope needs rows and heads (at most 65536)");
     const size_t width = (size_t)heads * d->head_dim;
     if (sstride == 0) sstride = width;
@@ -161,20 +157,7 @@ int ziggy_hip_rope_rows_f32(ZiggyHipContext *ctx, const ZiggyHipRopeDesc *d, con
     p.heads = (int)heads, p.hd = (int)d->head_dim, p.rd = (int)d->rope_dim, p.style = (int)d->rope_style;
     p.magnitude = d->magnitude;
     p.aligned = !(((uintptr_t)p.src | (uintptr_t)p.dst) % 16) && sstride % 4 == 0 && dstride % 4 == 0;
-    RopeFreq &f = p.freq;
-    const double base = d->freq_base, dim = d->rope_dim, turns = 6.283185307179586476925;
-    f.exponent = -2.0 * log2(base) / dim;
-    f.inv_factor = d->scaling == ZIGGY_HIP_ROPE_NONE ? 1.0 : 1.0 / (double)d->factor;
-    if (d->scaling == ZIGGY_HIP_ROPE_YARN) {
-        auto pair_of = [&](double t) { return dim * log(d->original_context / (turns * t)) / (2.0 * log(base)); };
-        const double lo = fmax(0.0, floor(pair_of(d->high))), hi = fmin(dim - 1.0, ceil(pair_of(d->low)));
-        const double run = fmax(0.001, hi - lo);
-        f.a = 1.0 + lo / run, f.b = -1.0 / run;
-    } else if (d->scaling == ZIGGY_HIP_ROPE_BANDS) {
-        const double run = (double)d->high - (double)d->low;
-        f.a = -(double)d->low / run, f.b = (double)d->original_context / run;
-        f.by_turns = 1;
-    }
+    p.freq = rope_freq(*d);
     OnDevice on(ctx->device);
     ZH_TRY(launch_rope_rows(p, (int)ctx->info.compute_units, ctx->stream), "rope_rows");
     return finish_op(ctx, "rope_rows", err, err_len);

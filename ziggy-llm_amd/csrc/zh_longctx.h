@@ -2,24 +2,9 @@
 // attention, sampling on the device); their arguments are checked in zh_longctx.cpp.
 #pragma once
 
-#include "zh_internal.h"
+#include "zh_args.h"
 
 namespace zh {
-
-// The context's device current for a call, the caller's again after it.
-struct OnDevice {
-    int before = -1;
-    explicit OnDevice(int device) {
-        int now = -1;
-        if (hipGetDevice(&now) == hipSuccess && now != device) {
-            before = now;
-            hipSetDevice(device);
-        }
-    }
-    ~OnDevice() {
-        if (before >= 0) hipSetDevice(before);
-    }
-};
 
 // Scaled rotary frequencies in turns a position (radians / 2 pi): 2^(i exponent) / 2 pi, blended.
 struct RopeFreq {
@@ -28,6 +13,9 @@ struct RopeFreq {
     double a, b;       // g_i = clamp(a + b x, 0, 1), x the pair (YARN) or the turns a position (BANDS); LINEAR: 0, 0
     int by_turns;
 };
+// why a rope description is not served (null: it is), and its frequencies
+const char *rope_refusal(const ZiggyHipRopeDesc &d);
+RopeFreq rope_freq(const ZiggyHipRopeDesc &d);
 struct RopeRows {
     RopeFreq freq;
     const float *src;

@@ -1,0 +1,98 @@
+// zh_serving.h -- launchers of the operators that serve several sequences (norms with the rotation, the paged
+// 4-bit cache and its attention, log probabilities); their arguments are checked in zh_serving.cpp.
+#pragma once
+
+#include "zh_longctx.h"
+
+namespace zh {
+
+constexpr int kPage = ZIGGY_HIP_KV_PAGE_POSITIONS;
+
+// A batch whose tables the host can't see: what a kernel takes from them goes through the members below, which stay
+// in bounds whatever they hold.
+struct Batch {
+    const uint32_t *pages, *starts, *lengths;
+    uint32_t sequences, per_seq, rows, max_rows;
+    uint32_t cap;   // positions that a sequence may have
+    uint32_t pool;  // pages of the cache
+};
+// One sequence's share of a batch.
+struct Sequence {
+    uint32_t index, row0, rows;
+    int first;  // position of row0 (below 0 where there are more rows than positions)
+};
+__device__ __forceinline__ Sequence sequence_of(const Batch &b, uint32_t s) {
+    Sequence q;
+    const uint32_t a = b.starts[s], z = b.starts[s + 1], n = b.lengths[s];
+    q.index = s;
+    q.row0 = a < b.rows ? a : b.rows;
+    const uint32_t end = z < b.rows ? z : b.rows, all = end > q.row0 ? end - q.row0 : 0u;
+    q.rows = all < b.max_rows ? all : b.max_rows;
+    q.first = (int)(n < 0x7FFFFFFFu ? n : 0x7FFFFFFFu) - (int)all;
+    return q;
+}
+// the pool's page that position t < cap lies in; `pool` or above: none
+__device__ __forceinline__ uint32_t page_of(const Batch &b, uint32_t s, uint32_t t) {
+    return b.pages[(size_t)s * b.per_seq + t / kPage];
+}
+
+// One layer of a 4-bit cache.
+struct Kv4Layer {
+    uint8_t *kc, *vc, *ks, *vs;
+    int nkv, hd;
+    // a page's and kv head's first code byte, and scale byte
+    __device__ __forceinline__ size_t codes(uint32_t page, int head) const { return ((size_t)page * nkv + head) * (kPage / 2 * hd); }
+    __device__ __forceinline__ size_t scales(uint32_t page, int head) const { return ((size_t)page * nkv + head) * (kPage / 32 * hd); }
+};
+
+struct HeadRows {
+    RopeFreq freq;
+    int rotates, hd, rd, style;
+    float magnitude;
+    const float *factors, *q_norm, *k_norm;
+    float eps, weight_offset;
+    // f32 rows: q_heads heads, then k_heads
+    const float *src;
+    float *dst;
+    size_t src_stride, dst_stride;
+    int q_heads, k_heads;
+    const uint32_t *positions;  // without a cache: null: first + row
+    uint32_t first, rows;
+    // rows that go into a cache (c.kc not null): heads c.nkv, the rows and positions of the batch
+    Kv4Layer c;
+    Batch b;
+    const float *k, *v;
+    int aligned;  // every row and head starts on 16 bytes
+};
+hipError_t launch_head_rows(const HeadRows &p, int cus, hipStream_t s);
+hipError_t launch_kv4_load(const Kv4Layer &c, const Batch &b, float *k, float *v, hipStream_t s);
+
+struct Kv4Attn {
+    Kv4Layer c;
+    Batch b;
+    const float *q;
+    size_t q_stride;
+    float *out;  // [rows][heads * hd]
+    int heads;
+    uint32_t window;      // 0: none
+    float qscale, qsign;  // score scale x log2 e, above 0; -1, 0 or 1: what the queries are multiplied by ahead
+    int q_aligned;
+    float *part;          // workspace
+    size_t part_floats;
+};
+hipError_t launch_kv4_attention(const Kv4Attn &p, int cus, hipStream_t s);
+
+struct TokenLogprobs {
+    const float *x;
+    size_t stride;
+    const uint32_t *tokens;
+    float *out, *entropy, *top;
+    uint32_t *top_tokens;
+    uint32_t rows, vocab;
+    int k;
+    void *work;
+    size_t work_bytes;
+};
+hipError_t launch_token_logprobs(const TokenLogprobs &p, int cus, hipStream_t s);
+
+}  // namespace zh

@@ -138,6 +138,69 @@ class Kv8Cache:
         return self._desc
 
 
+KV_PAGE = 64  # ZIGGY_HIP_KV_PAGE_POSITIONS
+MAX_TOP_LOGPROBS = 64  # ZIGGY_HIP_MAX_TOP_LOGPROBS
+
+
+class BatchDesc(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_void_p) for n in ("page_table", "row_starts", "lengths")] + [
+        (n, ctypes.c_uint32) for n in ("sequences", "pages_per_sequence", "rows", "max_rows", "max_length")]
+
+
+class HeadsDesc(ctypes.Structure):
+    _fields_ = [("rope", ctypes.POINTER(RopeDesc))] + [(n, ctypes.c_void_p) for n in ("freq_factors", "q_norm", "k_norm")] + [
+        ("eps", ctypes.c_float), ("weight_offset", ctypes.c_float)]
+
+
+class Kv4CacheDesc(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_void_p) for n in ("k_codes", "k_scales", "v_codes", "v_scales")] + [
+        (n, ctypes.c_uint32) for n in ("layers", "head_count_kv", "head_dim", "pages")]
+
+
+class _OverBuffers:
+    """A description that refers to buffers, which it keeps alive."""
+
+    def __init__(self, desc, *buffers):
+        self.buffers, self._desc = buffers, desc
+
+    @property
+    def desc(self):
+        if not all(b is None or b.h for b in self.buffers):
+            raise HipError(6, "a buffer was freed")
+        return self._desc
+
+
+def _handle(b: "Buffer | None"):
+    return b.h if b else None
+
+
+class Batch(_OverBuffers):
+    """Which rows of a step are whose, and where the sequences' pages lie (ZiggyHipBatch)."""
+
+    def __init__(self, page_table: "Buffer", row_starts: "Buffer", lengths: "Buffer", sequences: int,
+                 pages_per_sequence: int, rows: int, max_rows: int = 0, max_length: int = 0):
+        super().__init__(BatchDesc(page_table.h, row_starts.h, lengths.h, sequences, pages_per_sequence, rows, max_rows,
+                                   max_length), page_table, row_starts, lengths)
+
+
+class Heads(_OverBuffers):
+    """Norms and rotation of query and key heads (ZiggyHipHeadsDesc)."""
+
+    def __init__(self, rope: RopeDesc | None, q_norm: "Buffer | None" = None, k_norm: "Buffer | None" = None,
+                 eps: float = 1e-6, weight_offset: float = 0.0, freq_factors: "Buffer | None" = None):
+        super().__init__(HeadsDesc(ctypes.pointer(rope) if rope else None, _handle(freq_factors), _handle(q_norm),
+                                   _handle(k_norm), eps, weight_offset), freq_factors, q_norm, k_norm)
+
+
+class Kv4Cache(_OverBuffers):
+    """A paged K/V cache in 4 bits over four buffers (ZiggyHipKv4Cache has their layout); Context.kv4_cache makes one."""
+
+    def __init__(self, k_codes: "Buffer", k_scales: "Buffer", v_codes: "Buffer", v_scales: "Buffer", layers: int,
+                 heads_kv: int, head_dim: int, pages: int):
+        super().__init__(Kv4CacheDesc(k_codes.h, k_scales.h, v_codes.h, v_scales.h, layers, heads_kv, head_dim, pages),
+                         k_codes, k_scales, v_codes, v_scales)
+
+
 class MoeLayerDesc(ctypes.Structure):
     _fields_ = [(n, TensorDesc) for n in MOE_LAYER_FIELDS]
 
@@ -220,6 +283,15 @@ def lib() -> ctypes.CDLL:
         "ziggy_hip_kv8_store": [vp, ctypes.POINTER(Kv8CacheDesc), vp, sz, vp, sz, sz, u32, u32, u32] + E,
         "ziggy_hip_kv8_load_f32": [vp, ctypes.POINTER(Kv8CacheDesc), vp, vp, u32, u32, u32] + E,
         "ziggy_hip_kv8_attention_f32": [vp, ctypes.POINTER(Kv8CacheDesc), vp, sz, vp, u32, u32, u32, u32, u32, f] + E,
+        "ziggy_hip_norm_rope_rows_f32": [vp, ctypes.POINTER(HeadsDesc), vp, sz, sz, vp, sz, sz, vp, u32, u32, u32, u32] + E,
+        "ziggy_hip_kv4_codes_length": [u32, u32, u32, u32],
+        "ziggy_hip_kv4_scales_length": [u32, u32, u32, u32],
+        "ziggy_hip_kv4_append": [vp, ctypes.POINTER(Kv4CacheDesc), u32, ctypes.POINTER(BatchDesc), ctypes.POINTER(HeadsDesc),
+                                 vp, sz, sz, sz, u32, sz, vp, sz, sz] + E,
+        "ziggy_hip_kv4_load_f32": [vp, ctypes.POINTER(Kv4CacheDesc), u32, ctypes.POINTER(BatchDesc), vp, vp] + E,
+        "ziggy_hip_kv4_attention_f32": [vp, ctypes.POINTER(Kv4CacheDesc), u32, ctypes.POINTER(BatchDesc), vp, sz, sz, vp, u32,
+                                        u32, f] + E,
+        "ziggy_hip_token_logprobs_f32": [vp, vp, sz, vp, vp, vp, u32, vp, vp, u32, u32] + E,
         "ziggy_hip_sample_rows_f32": [vp, vp, sz, vp, u32, ctypes.POINTER(SamplingOptions), vp, vp, u32, u32] + E,
         "ziggy_hip_session_create": [vp, ctypes.POINTER(ModelDesc), ctypes.POINTER(TensorDesc),
                                      ctypes.POINTER(TensorDesc), ctypes.POINTER(TensorDesc),
@@ -271,6 +343,7 @@ def lib() -> ctypes.CDLL:
                 "ziggy_hip_session_position": u32, "ziggy_hip_version": ctypes.c_char_p,
                 "ziggy_hip_session_kv_pages": u32,
                 "ziggy_hip_kv8_codes_length": sz, "ziggy_hip_kv8_scales_length": sz,
+                "ziggy_hip_kv4_codes_length": sz, "ziggy_hip_kv4_scales_length": sz,
                 "ziggy_hip_shortlist_len": u32}
     for name, args in sigs.items():
         fn = getattr(L, name)
@@ -375,6 +448,13 @@ class Context:
         scales = lib().ziggy_hip_kv8_scales_length(layers, heads_kv, head_dim, context)
         return Kv8Cache(self.empty(codes), self.empty(scales), self.empty(codes), self.empty(scales), layers, heads_kv,
                         head_dim, context)
+
+    def kv4_cache(self, layers: int, heads_kv: int, head_dim: int, pages: int) -> Kv4Cache:
+        """An empty paged K/V cache in 4 bits."""
+        codes = lib().ziggy_hip_kv4_codes_length(layers, heads_kv, head_dim, pages)
+        scales = lib().ziggy_hip_kv4_scales_length(layers, heads_kv, head_dim, pages)
+        return Kv4Cache(self.empty(codes), self.empty(scales), self.empty(codes), self.empty(scales), layers, heads_kv,
+                        head_dim, pages)
 
     # ---- primitive ops ----
     def matvec(self, ttype, m: Buffer, x: Buffer, y: Buffer, rows, cols, add=False, m_off=0, y_off=0):
@@ -505,6 +585,34 @@ class Context:
                     recent: Buffer | None = None, recent_count: int = 0, row_stride: int = 0):
         _call("ziggy_hip_sample_rows_f32", self.h, logits.h, row_stride, recent.h if recent else None, recent_count,
               ctypes.byref(options), uniforms.h, out.h, rows, vocab)
+
+    # ---- operators of a step that serves several sequences ----
+    def norm_rope_rows(self, heads: Heads, src: Buffer, dst: Buffer, rows: int, q_heads: int, k_heads: int = 0,
+                       positions: Buffer | None = None, first_position: int = 0, src_stride: int = 0, dst_stride: int = 0,
+                       src_off: int = 0, dst_off: int = 0):
+        _call("ziggy_hip_norm_rope_rows_f32", self.h, ctypes.byref(heads.desc), src.h, src_off, src_stride, dst.h, dst_off,
+              dst_stride, _handle(positions), first_position, rows, q_heads, k_heads)
+
+    def kv4_append(self, cache: Kv4Cache, layer: int, batch: Batch, heads: Heads | None, src: Buffer, k_off: int, v_off: int,
+                   row_stride: int = 0, q_heads: int = 0, q_off: int = 0, q_out: Buffer | None = None, q_out_off: int = 0,
+                   q_out_stride: int = 0):
+        _call("ziggy_hip_kv4_append", self.h, ctypes.byref(cache.desc), layer, ctypes.byref(batch.desc),
+              ctypes.byref(heads.desc) if heads else None, src.h, k_off, v_off, row_stride, q_heads, q_off, _handle(q_out),
+              q_out_off, q_out_stride)
+
+    def kv4_load(self, cache: Kv4Cache, layer: int, batch: Batch, k_out: Buffer, v_out: Buffer):
+        _call("ziggy_hip_kv4_load_f32", self.h, ctypes.byref(cache.desc), layer, ctypes.byref(batch.desc), k_out.h, v_out.h)
+
+    def kv4_attention(self, cache: Kv4Cache, layer: int, batch: Batch, q: Buffer, out: Buffer, heads: int, window: int = 0,
+                      scale: float | None = None, q_off: int = 0, q_stride: int = 0):
+        scale = 1.0 / np.sqrt(cache.desc.head_dim) if scale is None else scale
+        _call("ziggy_hip_kv4_attention_f32", self.h, ctypes.byref(cache.desc), layer, ctypes.byref(batch.desc), q.h, q_off,
+              q_stride, out.h, heads, window, float(scale))
+
+    def token_logprobs(self, logits: Buffer, tokens: Buffer, out: Buffer, rows: int, vocab: int, entropy: Buffer | None = None,
+                       top: int = 0, top_tokens: Buffer | None = None, top_logprobs: Buffer | None = None, row_stride: int = 0):
+        _call("ziggy_hip_token_logprobs_f32", self.h, logits.h, row_stride, tokens.h, out.h, _handle(entropy), top,
+              _handle(top_tokens), _handle(top_logprobs), rows, vocab)
 
     def begin(self):
         _call("ziggy_hip_begin_sequence", self.h)

@@ -15,21 +15,6 @@ __device__ __forceinline__ double turns_per_position(const HeadRows &p, int i) {
     return p.factors ? f / (double)p.factors[i] : f;
 }
 
-// The sequence that row r belongs to; rows 0: none.  Every lane of a wavefront takes part.
-__device__ __forceinline__ Sequence sequence_of_row(const Batch &b, uint32_t r) {
-    uint32_t s = 0;  // starts at or below r behind the first
-    for (uint32_t from = 0; from < b.sequences; from += 64) {
-        const uint32_t i = from + (threadIdx.x & 63);
-        const u64 below = __ballot(i < b.sequences && b.starts[min(i, b.sequences - 1) + 1] <= r);
-        s += (uint32_t)__popcll(below);
-        if (~below) break;
-    }
-    Sequence q{};
-    if (s < b.sequences) q = sequence_of(b, s);
-    if (r < q.row0 || r - q.row0 >= q.rows) q.rows = 0;
-    return q;
-}
-
 // LDS of a wavefront's own lanes: what they wrote is what they read behind this
 __device__ __forceinline__ void wave_fence() {
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");

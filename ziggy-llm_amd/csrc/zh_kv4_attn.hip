@@ -5,6 +5,8 @@
 // and V enter the matrix cores exactly and no scale is left over to weigh scores or outputs by.  A query and a
 // weight enter as three bf16 pieces, cut off by truncation, whose sum they are to the bit.  Products accumulate in
 // binary32, maximum and sum are binary32.
+#include <algorithm>
+
 #include "zh_serving.h"
 
 namespace zh {
@@ -27,36 +29,122 @@ struct Kv4Params {
     int heads, group, q_aligned;
     uint32_t window;
     float qscale, qsign;
+    uint32_t few;       // columns up to which a sequence is the few-column kernel's (0: none is)
+    uint32_t wgs;       // few: workgroups to spread the blocks over
+    int splits;         // many: of each tile's positions
+    float *part;        // partial outputs, and {maximum, sum} of each
+    float2 *part_ml;
 };
 
-// A sequence's tile of columns (its rows' heads of one kv head, row by row) by the tile's number in the batch;
-// count 0: none.  Every lane of a wavefront takes part.
+// The positions that columns first .. last of a sequence see: some of them (first .. last) and all (full_first ..
+// full_last), and the blocks of 32 that hold the former.
+struct Range {
+    int first, last, full_first, full_last;
+    int begin, end;
+};
+__device__ __forceinline__ int first_seen(int pos, uint32_t window) {
+    return window && (int64_t)pos >= (int64_t)window ? pos + 1 - (int)window : 0;
+}
+__device__ __forceinline__ Range range_of(const Kv4Params &p, const Sequence &q, uint32_t first_row, uint32_t last_row) {
+    Range r;
+    const int a = q.first + (int)first_row, z = q.first + (int)last_row, top = (int)p.b.cap - 1;
+    r.first = first_seen(a, p.window), r.full_first = first_seen(z, p.window);
+    r.last = min(z, top), r.full_last = min(a, top);
+    r.begin = r.first / kBlock;
+    r.end = r.last < r.first ? r.begin : r.last / kBlock + 1;
+    return r;
+}
+
+// the z-th of `parts` shares of begin .. end - 1, the first of them one longer where they are not alike
+__device__ __forceinline__ void share(int &begin, int &end, uint32_t parts, uint32_t z) {
+    const uint32_t n = (uint32_t)(end - begin), each = n / parts, more = n - each * parts;
+    begin += (int)(each * z + min(z, more));
+    end = begin + (int)(each + (z < more ? 1u : 0u));
+}
+
+// inclusive sum over a wavefront's lanes
+__device__ __forceinline__ uint32_t running_sum(uint32_t n) {
+    const int lane = threadIdx.x & 63;
+    for (int d = 1; d < 64; d <<= 1) {
+        const uint32_t o = (uint32_t)__shfl_up((int)n, d);
+        if (lane >= d) n += o;
+    }
+    return n;
+}
+
+// A tile of columns (a sequence's rows' heads of one kv head, row by row), by its number among those of the sequences
+// with more than `few` columns; count 0: none.  Every lane of a wavefront takes part.
 struct Tile {
     Sequence q;
     uint32_t first, count;  // columns
 };
-template <int COLUMNS> __device__ __forceinline__ Tile tile_of(const Batch &b, uint32_t group, uint32_t number) {
+template <int COLUMNS> __device__ __forceinline__ Tile tile_of(const Kv4Params &p, uint32_t number) {
     Tile t{};
-    const uint32_t lane = threadIdx.x & 63;
+    const uint32_t lane = threadIdx.x & 63, group = (uint32_t)p.group;
     uint32_t before = 0;
-    for (uint32_t from = 0; from < b.sequences; from += 64) {
+    for (uint32_t from = 0; from < p.b.sequences; from += 64) {
         uint32_t n = 0;
-        if (from + lane < b.sequences) n = (sequence_of(b, from + lane).rows * group + COLUMNS - 1) / COLUMNS;
-        uint32_t sum = n;  // of this lane and those before it
-        for (int d = 1; d < 64; d <<= 1) {
-            const uint32_t o = (uint32_t)__shfl_up((int)sum, d);
-            if ((int)lane >= d) sum += o;
-        }
+        if (from + lane < p.b.sequences) n = sequence_of(p.b, from + lane).rows * group;
+        n = n > p.few ? (n + COLUMNS - 1) / COLUMNS : 0u;
+        const uint32_t sum = running_sum(n);
         const u64 past = __ballot(before + sum > number);
         if (past) {
             const int at = __ffsll(past) - 1;
-            t.q = sequence_of(b, from + at);
+            t.q = sequence_of(p.b, from + at);
             t.first = (number - before - (uint32_t)__shfl((int)(sum - n), at)) * COLUMNS;
             const uint32_t all = t.q.rows * group;  // (tables that don't ascend may pass 32 bits in the sums)
             t.count = t.first < all ? min((uint32_t)COLUMNS, all - t.first) : 0u;
             return t;
         }
         before += (uint32_t)__shfl((int)sum, 63);
+    }
+    return t;
+}
+
+// How the few-column kernel spreads a batch: each sequence's blocks of 32 positions, times the kv heads, over p.wgs
+// workgroups, `quota` blocks each at most.  A sequence's blocks are split evenly; its items follow each other, the kv
+// heads side by side.  Splits that are to be joined have slots in the workspace, at most 2 p.wgs of them: a sequence has
+// two splits only where it has more than a quota.
+struct Share {
+    Sequence q;
+    Range r;            // of the whole sequence
+    uint32_t splits;    // 0: none
+    uint32_t index;     // item: within the sequence's
+    uint32_t slot;      // of the sequence's first split
+};
+constexpr uint32_t kLeastBlocks = 4;  // one for each wavefront
+
+// The item with this number, or (by_sequence) the sequence.  Every lane of a wavefront takes part.
+template <bool BY_SEQUENCE> __device__ __forceinline__ Share share_of(const Kv4Params &p, uint32_t number) {
+    const uint32_t lane = threadIdx.x & 63, nkv = (uint32_t)p.c.nkv;
+    auto blocks = [&](uint32_t s) -> uint32_t {
+        if (s >= p.b.sequences) return 0u;
+        const Sequence q = sequence_of(p.b, s);
+        if (q.rows == 0 || q.rows * p.group > p.few) return 0u;
+        const Range r = range_of(p, q, 0, q.rows - 1);
+        return max((uint32_t)(r.end - r.begin), 1u);  // rows that see nothing have an item, which writes zeros
+    };
+    uint32_t own = blocks(lane);
+    u64 total = own;
+    for (uint32_t from = 64; from < p.b.sequences; from += 64) total += blocks(from + lane);
+    for (int d = 1; d < 64; d <<= 1) total += __shfl_xor(total, d);
+    const uint32_t quota = max(kLeastBlocks, (uint32_t)ceil((double)total * nkv / p.wgs));
+    Share t{};
+    uint32_t items = 0, slots = 0;
+    for (uint32_t from = 0; from < p.b.sequences; from += 64) {
+        const uint32_t n = from ? blocks(from + lane) : own, splits = (n + quota - 1) / quota;
+        const uint32_t sum = running_sum(splits * nkv), slot_sum = running_sum(splits > 1 ? splits * nkv : 0u);
+        const u64 past = __ballot(BY_SEQUENCE ? from + lane == number : items + sum > number);
+        if (past) {
+            const int at = __ffsll(past) - 1;
+            t.q = sequence_of(p.b, from + at);
+            t.splits = (uint32_t)__shfl((int)splits, at);
+            if (t.splits) t.r = range_of(p, t.q, 0, t.q.rows - 1);
+            t.index = number - items - (uint32_t)__shfl((int)(sum - splits * nkv), at);
+            t.slot = slots + (uint32_t)__shfl((int)slot_sum, at) - (t.splits > 1 ? t.splits * nkv : 0u);
+            return t;
+        }
+        items += (uint32_t)__shfl((int)sum, 63), slots += (uint32_t)__shfl((int)slot_sum, 63);
     }
     return t;
 }
@@ -94,40 +182,61 @@ __device__ __forceinline__ float finite(float v) { return v == -INFINITY ? 0.f :
 template <int HD> struct Lane4 {
     static constexpr int G = HD / 32;
     uint32_t k[2][G], v[2 * G];
-    uint8_t ks[2][G];
-    uint32_t vs[2 * G];
-    __device__ __forceinline__ void load(const Kv4Layer &c, uint32_t page, int head, int half) {
+    uint32_t ks[2][(G + 3) / 4], vs[2 * G];
+    __device__ __forceinline__ void load_k(const Kv4Layer &c, uint32_t page, int head, int half) {
         const int i = threadIdx.x & 15, g = threadIdx.x >> 4 & 3;
         const size_t codes = c.codes(page, head), scales = c.scales(page, head);
 #pragma unroll
         for (int pt = 0; pt < 2; pt++) {
             const int pos = kBlock * half + 8 * (i >> 2) + 4 * pt + (i & 3);
             __builtin_memcpy(k[pt], c.kc + codes + (size_t)pos * (HD / 2) + g * 4 * G, 4 * G);
+            if constexpr (G % 4) ks[pt][0] = 0;
             __builtin_memcpy(ks[pt], c.ks + scales + (size_t)pos * G, G);
         }
+    }
+    __device__ __forceinline__ void load_v(const Kv4Layer &c, uint32_t page, int head, int half) {
+        const int i = threadIdx.x & 15, g = threadIdx.x >> 4 & 3;
+        const size_t codes = c.codes(page, head), scales = c.scales(page, head);
         __builtin_memcpy(v, c.vc + codes + (size_t)half * (16 * HD) + (g * 16 + i) * 8 * G, 8 * G);
         __builtin_memcpy(vs, c.vs + scales + (size_t)(kBlock * half + 8 * g) * G, 8 * G);
+    }
+    // V's positions outside first .. last of the block as zeros: what was never stored may read as NaN
+    __device__ __forceinline__ void clear_v(int first, int last) {
+        const int g = threadIdx.x >> 4 & 3;
+#pragma unroll
+        for (int w = 0; w < 2 * G; w++) {
+            uint32_t keep = 0;
+#pragma unroll
+            for (int b = 0; b < 4; b++) {
+                const int pos = 8 * g + (4 * w + b) / G;
+                if (pos >= first && pos <= last) keep |= 255u << 8 * b;
+            }
+            v[w] &= keep, vs[w] &= keep;
+        }
     }
 };
 
 // One wavefront's columns: their queries, running maxima and sums, and outputs.  Scores S^T[position][column] = K Q^T on
 // 16x16x32 products, outputs O^T[dim][column] = V^T P^T: what a lane gets of S^T, positions 8 g .. 8 g + 7 of column i,
 // is what it gives of P^T.
-template <int HD, int CT> struct Columns {
-    static constexpr int G = HD / 32, DT = HD / 16;
-    fb8 q[CT][G][3];
+template <int HD, int CT, int AWAY> struct Columns {
+    static constexpr int G = HD / 32, DT = HD / 16, NEAR = 3 - AWAY;
+    fb8 q[CT][G][NEAR];
+    const fb8 *away;  // the queries' other pieces, [CT][G][AWAY][64] in LDS
     ff4 o[CT][DT];
     float m[CT], l[CT];
     int lo[CT], hi[CT];  // the positions that a column sees, both included
 
-    __device__ __forceinline__ void begin(const Kv4Params &p, const Tile &t, uint32_t first, int head) {
+    // columns first .. first + count - 1 of a sequence
+    __device__ __forceinline__ void begin(const Kv4Params &p, const Sequence &t, uint32_t first, uint32_t count, int head, fb8 *lds) {
+        away = lds;
         const int i = threadIdx.x & 15, g = threadIdx.x >> 4 & 3;
 #pragma unroll
         for (int c = 0; c < CT; c++) {
-            const uint32_t column = min(first + 16 * c + i, t.first + t.count - 1), row = column / p.group;
-            const float *src = p.q + (size_t)(t.q.row0 + row) * p.q_stride + (size_t)(head * p.group + (int)(column - row * p.group)) * HD;
-            hi[c] = t.q.first + (int)row;
-            lo[c] = p.window && (int64_t)hi[c] - p.window >= 0 ? hi[c] + 1 - (int)p.window : 0;
+            const uint32_t column = first + min((uint32_t)(16 * c + i), count - 1), row = column / p.group;
+            const float *src = p.q + (size_t)(t.row0 + row) * p.q_stride + (size_t)(head * p.group + (int)(column - row * p.group)) * HD;
+            hi[c] = t.first + (int)row;
+            lo[c] = first_seen(hi[c], p.window);
             hi[c] = min(hi[c], (int)p.b.cap - 1);
 #pragma unroll
             for (int k = 0; k < G; k++) {
@@ -142,7 +251,13 @@ template <int HD, int CT> struct Columns {
                 }
 #pragma unroll
                 for (int e = 0; e < 8; e++) v[e] *= p.qsign;
-                pieces(v, q[c][k]);
+                fb8 all[3];
+                pieces(v, all);
+#pragma unroll
+                for (int e = 0; e < 3; e++) {
+                    if (e < NEAR) q[c][k][e] = all[e];
+                    else lds[((c * G + k) * AWAY + e - NEAR) * 64 + (threadIdx.x & 63)] = all[e];
+                }
             }
             m[c] = -INFINITY, l[c] = 0.f;
 #pragma unroll
@@ -150,48 +265,75 @@ template <int HD, int CT> struct Columns {
         }
     }
 
-    // 32 positions from `at` on; of these only first .. last are any column's to see
-    __device__ __forceinline__ void take(const Kv4Params &p, const Lane4<HD> &x, int at, int first, int last) {
+    // 32 positions from `at` on; hidden: their page is none.  after_k, after_v: K's and V's registers are free.
+    template <class K, class V>
+    __device__ __forceinline__ void take(float qscale, const Range &r, Lane4<HD> &x, int at, bool hidden, K after_k, V after_v) {
         const int g = threadIdx.x >> 4 & 3;
-        const bool edge = at < first || at + kBlock - 1 > last;
+        int lane = threadIdx.x & 63;
+        if constexpr (AWAY > 0) __asm__ volatile("" : "+v"(lane));  // (the pieces in LDS are read where they are used, not ahead of the loop)
         ff4 s[CT][2];
 #pragma unroll
-        for (int pt = 0; pt < 2; pt++) {
+        for (int c = 0; c < CT; c++) s[c][0] = s[c][1] = ff4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-            for (int c = 0; c < CT; c++) s[c][pt] = ff4{0.f, 0.f, 0.f, 0.f};
+        for (int t = 0; t < G; t++) {
+            fb8 a[2], far[CT][AWAY ? AWAY : 1];
 #pragma unroll
-            for (int t = 0; t < G; t++) {
-                const float scale = __uint_as_float((uint32_t)x.ks[pt][t] << 23);
-                uint32_t w[4] = {widen<0>(x.k[pt][t], scale), widen<1>(x.k[pt][t], scale), widen<2>(x.k[pt][t], scale), widen<3>(x.k[pt][t], scale)};
-                fb8 a;
-                __builtin_memcpy(&a, w, 16);
+            for (int c = 0; c < CT; c++)
+#pragma unroll
+                for (int k = 0; k < AWAY; k++) far[c][k] = away[((c * G + t) * AWAY + k) * 64 + lane];
+#pragma unroll
+            for (int pt = 0; pt < 2; pt++) {
+                const float scale = scale_of(x.ks[pt][t / 4], t % 4);
+                const uint32_t w[4] = {widen<0>(x.k[pt][t], scale), widen<1>(x.k[pt][t], scale), widen<2>(x.k[pt][t], scale), widen<3>(x.k[pt][t], scale)};
+                __builtin_memcpy(&a[pt], w, 16);
+            }
+#pragma unroll
+            for (int k = 0; k < 3; k++)
 #pragma unroll
                 for (int c = 0; c < CT; c++)
 #pragma unroll
-                    for (int k = 0; k < 3; k++) s[c][pt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, q[c][t][k], s[c][pt], 0, 0, 0);
-            }
+                    for (int pt = 0; pt < 2; pt++) s[c][pt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a[pt], k < NEAR ? q[c][t][k < NEAR ? k : 0] : far[c][k < NEAR ? 0 : k - NEAR], s[c][pt], 0, 0, 0);
+            if constexpr (HD * CT > 128) __builtin_amdgcn_sched_barrier(0);
         }
+        after_k();
         fb8 w[CT][3];
+        float next[CT];
+        bool grows = false;
+        if (hidden || at < r.full_first || at + kBlock - 1 > r.full_last) {
+#pragma unroll
+            for (int c = 0; c < CT; c++)
+#pragma unroll
+                for (int e = 0; e < 8; e++) {
+                    const int pos = at + 8 * g + e;
+                    if (hidden || pos < lo[c] || pos > hi[c]) s[c][e >> 2][e & 3] = -INFINITY;
+                }
+            x.clear_v(r.first - at, hidden ? -1 : r.last - at);
+        }
 #pragma unroll
         for (int c = 0; c < CT; c++) {
-            float v[8];
+            float top = s[c][0][0];
 #pragma unroll
-            for (int e = 0; e < 8; e++) {
-                const int pos = at + 8 * g + e;
-                v[e] = pos >= lo[c] && pos <= hi[c] && pos >= first && pos <= last ? s[c][e >> 2][e & 3] : -INFINITY;
+            for (int e = 1; e < 8; e++) top = fmaxf(top, s[c][e >> 2][e & 3]);
+            next[c] = fmaxf(m[c], xmax<32>(xmax<16>(top)) * qscale);
+            grows = grows || next[c] > m[c];
+        }
+        if (__any(grows)) {
+#pragma unroll
+            for (int c = 0; c < CT; c++) {
+                const float was = __builtin_amdgcn_exp2f(m[c] - finite(next[c]));
+                m[c] = next[c];
+                l[c] *= was;
+#pragma unroll
+                for (int d = 0; d < DT; d++) o[c][d] *= was;
             }
-            float top = v[0];
+        }
 #pragma unroll
-            for (int e = 1; e < 8; e++) top = fmaxf(top, v[e]);
-            top = xmax<32>(xmax<16>(top)) * p.qscale;
-            const float next = fmaxf(m[c], top), nf = finite(next), was = __builtin_amdgcn_exp2f(m[c] - nf);
-            m[c] = next;
-            float sum = 0.f;
+        for (int c = 0; c < CT; c++) {
+            const float mf = finite(m[c]);
+            float v[8], sum = 0.f;
 #pragma unroll
-            for (int e = 0; e < 8; e++) v[e] = __builtin_amdgcn_exp2f(fmaf(v[e], p.qscale, -nf)), sum += v[e];
-            l[c] = fmaf(l[c], was, sum);
-#pragma unroll
-            for (int d = 0; d < DT; d++) o[c][d] *= was;
+            for (int e = 0; e < 8; e++) v[e] = __builtin_amdgcn_exp2f(fmaf(s[c][e >> 2][e & 3], qscale, -mf)), sum += v[e];
+            l[c] += sum;
             pieces(v, w[c]);
         }
 #pragma unroll
@@ -203,52 +345,224 @@ template <int HD, int CT> struct Columns {
 #pragma unroll
                 for (int e = 0; e < 2; e++) {
                     const int n = (j + e) * G + t;  // byte of this position's dims
-                    const bool out = edge && (at + 8 * g + j + e < first || at + 8 * g + j + e > last);
                     const float scale = scale_of(x.vs[n >> 2], n & 3);
                     const uint32_t word = x.v[n >> 2];
-                    const uint32_t u = (n & 3) == 0 ? widen<0>(word, scale) : (n & 3) == 1 ? widen<1>(word, scale) : (n & 3) == 2 ? widen<2>(word, scale) : widen<3>(word, scale);
-                    y[e] = out ? 0u : u;  // (what was never stored may read as NaN)
+                    y[e] = (n & 3) == 0 ? widen<0>(word, scale) : (n & 3) == 1 ? widen<1>(word, scale) : (n & 3) == 2 ? widen<2>(word, scale) : widen<3>(word, scale);
                 }
                 a[0][j / 2] = __builtin_amdgcn_perm(y[1], y[0], 0x05040100u);
                 a[1][j / 2] = __builtin_amdgcn_perm(y[1], y[0], 0x07060302u);
             }
+            fb8 b[2];
+            __builtin_memcpy(b, a, 32);
 #pragma unroll
-            for (int h = 0; h < 2; h++) {
-                fb8 b;
-                __builtin_memcpy(&b, a[h], 16);
+            for (int k = 0; k < 3; k++)
 #pragma unroll
                 for (int c = 0; c < CT; c++)
 #pragma unroll
-                    for (int k = 0; k < 3; k++) o[c][2 * t + h] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(b, w[c][k], o[c][2 * t + h], 0, 0, 0);
+                    for (int h = 0; h < 2; h++) o[c][2 * t + h] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(b[h], w[c][k], o[c][2 * t + h], 0, 0, 0);
+            if constexpr (HD * CT > 128) __builtin_amdgcn_sched_barrier(0);
+        }
+        after_v();
+    }
+
+    // The blocks begin, begin + step .. below end.  DEEP: the next block's loads go out ahead of the work on this one, into
+    // registers of their own; otherwise K's and V's follow each other into the same ones as they come free.
+    template <bool DEEP> __device__ __forceinline__ void run(const Kv4Params &p, const Range &r, uint32_t sequence, int head, int begin, int end, int step) {
+        if (begin >= end) return;
+        const int lane = threadIdx.x & 63;
+        uint32_t pages = 0;  // of the next 64 blocks, one a lane; those that the pool doesn't have: 0, not seen
+        u64 missing = 0;
+        auto look = [&](int b) {
+            const int at = b + step * lane;
+            pages = 0xFFFFFFFFu;
+            if (at < end) pages = page_of(p.b, sequence, (uint32_t)at * kBlock);
+            const bool none = pages >= p.b.pool;
+            if (none) pages = 0;
+            missing = __ballot(none);
+        };
+        look(begin);
+        const int n = (end - begin + step - 1) / step;
+        auto page = [&](int i) { return (uint32_t)__builtin_amdgcn_readlane((int)pages, i & 63); };
+        auto half = [&](int i) { return (begin + step * i) & 1; };
+        if constexpr (DEEP) {
+            Lane4<HD> x[2];
+            auto work = [&](int i, Lane4<HD> &now, Lane4<HD> &after) {
+                const bool hidden = missing >> (i & 63) & 1;
+                if ((i & 63) == 63) look(begin + step * (i + 1));
+                const int j = min(i + 1, n - 1);  // (the last one's again, unused)
+                after.load_k(p.c, page(j), head, half(j)), after.load_v(p.c, page(j), head, half(j));
+                take(p.qscale, r, now, (begin + step * i) * kBlock, hidden, [] {}, [] {});
+            };
+            x[0].load_k(p.c, page(0), head, half(0)), x[0].load_v(p.c, page(0), head, half(0));
+            for (int i = 0; i < n; i += 2) {
+                work(i, x[0], x[1]);
+                if (i + 1 < n) work(i + 1, x[1], x[0]);
+            }
+        } else {
+            Lane4<HD> x;
+            x.load_k(p.c, page(0), head, half(0)), x.load_v(p.c, page(0), head, half(0));
+            for (int i = 0; i < n; i++) {
+                const bool hidden = missing >> (i & 63) & 1;
+                if ((i & 63) == 63) look(begin + step * (i + 1));
+                const int j = min(i + 1, n - 1);
+                const uint32_t next = page(j);
+                take(p.qscale, r, x, (begin + step * i) * kBlock, hidden, [&] { x.load_k(p.c, next, head, half(j)); },
+                     [&] { x.load_v(p.c, next, head, half(j)); });
             }
         }
     }
 };
 
-// A wavefront takes 16 columns through all of their positions.
-template <int HD> __global__ void __launch_bounds__(64) kv4_simple_kernel(Kv4Params p) {
-    const int head = blockIdx.x % p.c.nkv, i = threadIdx.x & 15, g = threadIdx.x >> 4;
-    const Tile t = tile_of<16>(p.b, (uint32_t)p.group, blockIdx.x / p.c.nkv);
-    if (t.count == 0) return;
-    Columns<HD, 1> x;
-    x.begin(p, t, t.first, head);
-    const int row0 = (int)(t.first / p.group), row1 = (int)((t.first + t.count - 1) / p.group);
-    const int last = min(t.q.first + row1, (int)p.b.cap - 1);
-    const int first = p.window && (int64_t)t.q.first + row0 - p.window >= 0 ? t.q.first + row0 + 1 - (int)p.window : 0;
-    for (int at = first / kBlock * kBlock; at <= last; at += kBlock) {
-        const uint32_t page = page_of(p.b, t.q.index, (uint32_t)at);
-        if (page >= p.b.pool) continue;
-        Lane4<HD> y;
-        y.load(p.c, page, head, at / kBlock & 1);
-        x.take(p, y, at, first, last);
-    }
-    const float l = xsum<32>(xsum<16>(x.l[0])), inv = l == 0.f ? 0.f : 1.f / l;
-    if ((uint32_t)i >= t.count) return;
-    const uint32_t column = t.first + i, row = column / p.group;
-    float *to = p.out + ((size_t)(t.q.row0 + row) * p.heads + head * p.group + (column - row * p.group)) * HD + 4 * g;
+__device__ __forceinline__ float *column_of(float *out, const Kv4Params &p, const Sequence &q, int head, uint32_t column, int hd) {
+    const uint32_t row = column / p.group;
+    return out + ((size_t)(q.row0 + row) * p.heads + head * p.group + (column - row * p.group)) * hd;
+}
+
+// Few columns (decoding): a workgroup takes an item, its wavefronts blocks in turn, joined in LDS.
+template <int HD, int CT> __global__ void __launch_bounds__(256, 2) kv4_few_kernel(Kv4Params p) {
+    constexpr int N = 16 * CT, C = HD / 4, AWAY = HD * CT > 128 ? 2 : 0, PIECES = 4 * CT * (HD / 32) * AWAY * 64;  // (their 16 bytes)
+    // the queries' pieces, then the wavefronts' outputs
+    __shared__ __align__(16) float lds[4 * N * (HD + 4) > 4 * PIECES ? 4 * N * (HD + 4) : 4 * PIECES];
+    __shared__ float ms[4][N], ls[4][N];
+    float(*os)[N][HD + 4] = reinterpret_cast<float(*)[N][HD + 4]>(lds);
+    const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), i = tid & 15, g = tid >> 4 & 3;
+    const Share t = share_of<false>(p, blockIdx.x);
+    if (t.splits == 0) return;
+    const int head = (int)(t.index % p.c.nkv);
+    const uint32_t z = t.index / p.c.nkv, count = t.q.rows * p.group;
+    int begin = t.r.begin, end = t.r.end;
+    share(begin, end, t.splits, z);
+    Columns<HD, CT, AWAY> x;
+    x.begin(p, t.q, 0, count, head, reinterpret_cast<fb8 *>(lds) + wave * (PIECES / 4));
+    x.template run<HD * CT <= 128>(p, t.r, t.q.index, head, begin + wave, end, 4);
+    if (AWAY) __syncthreads();
 #pragma unroll
-    for (int d = 0; d < HD / 16; d++)
-        *reinterpret_cast<float4 *>(to + 16 * d) = make_float4(x.o[0][d][0] * inv, x.o[0][d][1] * inv, x.o[0][d][2] * inv, x.o[0][d][3] * inv);
+    for (int c = 0; c < CT; c++) {
+        if ((uint32_t)(16 * c) >= count) break;
+        const float l = xsum<32>(xsum<16>(x.l[c]));
+        if (g == 0) ms[wave][16 * c + i] = x.m[c], ls[wave][16 * c + i] = l;
+#pragma unroll
+        for (int d = 0; d < HD / 16; d++)
+            *reinterpret_cast<float4 *>(&os[wave][16 * c + i][16 * d + 4 * g]) = make_float4(x.o[c][d][0], x.o[c][d][1], x.o[c][d][2], x.o[c][d][3]);
+    }
+    __syncthreads();
+    for (uint32_t u = tid; u < count * C; u += 256) {
+        const uint32_t column = u / C;
+        const int d = 4 * (int)(u % C);
+        const float m = fmaxf(fmaxf(ms[0][column], ms[1][column]), fmaxf(ms[2][column], ms[3][column])), mf = finite(m);
+        float l = 0.f;
+        float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+        for (int w = 0; w < 4; w++) {
+            const float f = __builtin_amdgcn_exp2f(ms[w][column] - mf);
+            const float4 v = *reinterpret_cast<const float4 *>(&os[w][column][d]);
+            l = fmaf(f, ls[w][column], l);
+            o.x = fmaf(f, v.x, o.x), o.y = fmaf(f, v.y, o.y), o.z = fmaf(f, v.z, o.z), o.w = fmaf(f, v.w, o.w);
+        }
+        if (t.splits > 1) {
+            const size_t at = ((size_t)t.slot + z * p.c.nkv + head) * N + column;
+            *reinterpret_cast<float4 *>(p.part + at * HD + d) = o;
+            if (d == 0) p.part_ml[at] = make_float2(m, l);
+        } else {
+            const float inv = l == 0.f ? 0.f : 1.f / l;  // (rows that see nothing: zeros)
+            *reinterpret_cast<float4 *>(column_of(p.out, p, t.q, head, column, HD) + d) = make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv);
+        }
+    }
+}
+
+// Joins the splits of a sequence's kv head, a column at a time: a float4 of every N-th split a thread.
+template <int HD, int CT> __global__ void __launch_bounds__(256) kv4_few_join_kernel(Kv4Params p) {
+    constexpr int C = HD / 4, N = 256 / C;
+    __shared__ float4 os[N][C];
+    __shared__ float ls[N], ms[4];
+    const Share t = share_of<true>(p, blockIdx.x / p.c.nkv);
+    if (t.splits < 2) return;
+    const int head = (int)(blockIdx.x % p.c.nkv), tid = threadIdx.x, c = tid % C, n = tid / C;
+    const uint32_t count = t.q.rows * p.group;
+    for (uint32_t column = blockIdx.y; column < count; column += gridDim.y) {
+        auto at = [&](uint32_t z) { return ((size_t)t.slot + z * p.c.nkv + head) * (16 * CT) + column; };
+        float m = -INFINITY;
+        for (uint32_t z = tid; z < t.splits; z += 256) m = fmaxf(m, p.part_ml[at(z)].x);
+        m = wave_max_f32(m);
+        if ((tid & 63) == 0) ms[tid >> 6] = m;
+        __syncthreads();
+        m = finite(fmaxf(fmaxf(ms[0], ms[1]), fmaxf(ms[2], ms[3])));
+        float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+        float l = 0.f;
+        if (n < N)
+            for (uint32_t z = n; z < t.splits; z += N) {
+                const float2 ml = p.part_ml[at(z)];
+                const float4 v = *reinterpret_cast<const float4 *>(p.part + at(z) * HD + 4 * c);
+                const float f = __builtin_amdgcn_exp2f(ml.x - m);
+                l = fmaf(f, ml.y, l);
+                o.x = fmaf(f, v.x, o.x), o.y = fmaf(f, v.y, o.y), o.z = fmaf(f, v.z, o.z), o.w = fmaf(f, v.w, o.w);
+            }
+        if (n < N) {
+            os[n][c] = o;
+            if (c == 0) ls[n] = l;
+        }
+        __syncthreads();
+        if (n == 0) {
+            for (int k = 1; k < N; k++) {
+                const float4 v = os[k][c];
+                o.x += v.x, o.y += v.y, o.z += v.z, o.w += v.w, l += ls[k];
+            }
+            const float inv = l == 0.f ? 0.f : 1.f / l;
+            *reinterpret_cast<float4 *>(column_of(p.out, p, t.q, head, column, HD) + 4 * c) = make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv);
+        }
+        __syncthreads();
+    }
+}
+
+// Many columns (prompts): a wavefront takes a tile, through a split of its positions.
+template <int HD, int CT, int AWAY> __global__ void __launch_bounds__(256, 2) kv4_many_kernel(Kv4Params p) {
+    __shared__ fb8 held[4][CT * (HD / 32) * AWAY * 64];
+    const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), i = threadIdx.x & 15, g = threadIdx.x >> 4 & 3;
+    const int head = (int)(blockIdx.x % p.c.nkv);
+    // the longest (last) first
+    const uint32_t number = (gridDim.x - 1 - blockIdx.x) / p.c.nkv * 4 + wave;
+    const Tile t = tile_of<16 * CT>(p, number);
+    if (t.count == 0) return;
+    const Range r = range_of(p, t.q, t.first / p.group, (t.first + t.count - 1) / p.group);
+    int begin = r.begin, end = r.end;
+    share(begin, end, (uint32_t)p.splits, blockIdx.y);
+    Columns<HD, CT, AWAY> x;
+    x.begin(p, t.q, t.first, t.count, head, held[wave]);
+    x.template run<false>(p, r, t.q.index, head, begin, end, 1);
+#pragma unroll
+    for (int c = 0; c < CT; c++) {
+        const float l = xsum<32>(xsum<16>(x.l[c])), inv = l == 0.f ? 0.f : 1.f / l;
+        if ((uint32_t)(16 * c + i) >= t.count) continue;
+        float *out = p.splits > 1 ? p.part + (size_t)blockIdx.y * p.b.rows * p.heads * HD : p.out;
+        float *to = column_of(out, p, t.q, head, t.first + 16 * c + i, HD);
+#pragma unroll
+        for (int d = 0; d < HD / 16; d++)
+            *reinterpret_cast<float4 *>(to + 16 * d + 4 * g) = make_float4(x.o[c][d][0] * inv, x.o[c][d][1] * inv, x.o[c][d][2] * inv, x.o[c][d][3] * inv);
+        if (p.splits > 1 && g == 0) p.part_ml[(to - p.part) / HD] = make_float2(x.m[c], l);
+    }
+}
+
+// The splits of a row's heads joined, a thread four dims.
+template <int HD> __global__ void __launch_bounds__(256) kv4_many_join_kernel(Kv4Params p) {
+    const Sequence q = sequence_of_row(p.b, blockIdx.x);
+    if (q.rows * p.group <= p.few) return;  // (none's, or the other kernel's)
+    for (uint32_t u = threadIdx.x; u < (uint32_t)p.heads * (HD / 4); u += 256) {
+        const size_t at = (size_t)blockIdx.x * p.heads + u / (HD / 4), each = (size_t)p.b.rows * p.heads;
+        const int d = 4 * (int)(u % (HD / 4));
+        float m = -INFINITY, l = 0.f;
+        for (int z = 0; z < p.splits; z++) m = fmaxf(m, p.part_ml[z * each + at].x);
+        m = finite(m);
+        float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+        for (int z = 0; z < p.splits; z++) {
+            const float2 ml = p.part_ml[z * each + at];
+            const float4 v = *reinterpret_cast<const float4 *>(p.part + (z * each + at) * HD + d);
+            const float f = __builtin_amdgcn_exp2f(ml.x - m) * ml.y;
+            l += f;
+            o.x = fmaf(f, v.x, o.x), o.y = fmaf(f, v.y, o.y), o.z = fmaf(f, v.z, o.z), o.w = fmaf(f, v.w, o.w);
+        }
+        const float inv = l == 0.f ? 0.f : 1.f / l;
+        *reinterpret_cast<float4 *>(p.out + at * HD + d) = make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv);
+    }
 }
 
 }  // namespace
@@ -258,14 +572,47 @@ hipError_t launch_kv4_attention(const Kv4Attn &a, int cus, hipStream_t s) {
     p.c = a.c, p.b = a.b, p.q = a.q, p.q_stride = a.q_stride, p.out = a.out;
     p.heads = a.heads, p.group = a.heads / a.c.nkv, p.q_aligned = a.q_aligned;
     p.window = a.window, p.qscale = a.qscale, p.qsign = a.qsign;
-    const uint64_t wgs = a.c.nkv * ((uint64_t)a.b.rows * p.group / 16 + a.b.sequences);  // at most
-    if (wgs > 0x7FFFFFFFu) return hipErrorInvalidValue;
-    const dim3 grid((unsigned)wgs);
+    p.part = a.part;
+    const uint64_t nkv = a.c.nkv, most = (uint64_t)a.b.max_rows * p.group, all = (uint64_t)a.b.rows * p.group;
+    const int ct = a.c.hd <= 128 ? 2 : 1;                     // column tiles that a wavefront's registers hold
+    const uint32_t limit = 16u * ct;
+    const uint64_t blocks = (a.b.cap + kBlock - 1) / kBlock;  // of a sequence, at most
+    // a batch of one sequence is one kernel's; others may hold sequences of both kinds
+    p.few = a.b.sequences == 1 && most > limit ? 0 : limit;
+    auto go = [&](auto h, auto tiles) {
+        constexpr int HD = decltype(h)::value, CT = decltype(tiles)::value;
+        if (p.few) {
+            p.wgs = 2 * cus;
+            const size_t slot = (size_t)limit * (HD + 2);  // floats
+            while (p.wgs > 1 && 2 * p.wgs * slot > a.part_floats) p.wgs /= 2;
+            p.part_ml = (float2 *)(p.part + (size_t)2 * p.wgs * limit * HD);
+            const uint64_t per = (blocks + kLeastBlocks - 1) / kLeastBlocks;  // splits of a sequence, at most
+            const uint64_t items = std::min(p.wgs + a.b.sequences * nkv, a.b.sequences * nkv * per);
+            const bool split = per > 1;
+            const dim3 join((unsigned)(a.b.sequences * nkv), (unsigned)std::min<uint64_t>(std::min<uint64_t>(most, limit), std::max<uint64_t>(1, 1024 / (a.b.sequences * nkv))));
+            if (most <= 16) {
+                hipLaunchKernelGGL((kv4_few_kernel<HD, 1>), dim3((unsigned)items), dim3(256), 0, s, p);
+                if (split) hipLaunchKernelGGL((kv4_few_join_kernel<HD, 1>), join, dim3(256), 0, s, p);
+            } else {
+                hipLaunchKernelGGL((kv4_few_kernel<HD, CT>), dim3((unsigned)items), dim3(256), 0, s, p);
+                if (split) hipLaunchKernelGGL((kv4_few_join_kernel<HD, CT>), join, dim3(256), 0, s, p);
+            }
+        }
+        if (most > p.few) {
+            const uint64_t n = std::min<uint64_t>(all / (16 * CT) + a.b.sequences, all), wgs = (n + 3) / 4 * nkv;
+            const uint64_t each = (uint64_t)a.b.rows * a.heads * (HD + 2);
+            p.splits = (int)std::max<uint64_t>(1, std::min<uint64_t>({2 * (uint64_t)cus / wgs, blocks / 4, a.part_floats / each}));
+            p.part_ml = (float2 *)(p.part + (size_t)p.splits * a.b.rows * a.heads * HD);
+            hipLaunchKernelGGL((kv4_many_kernel<HD, CT, 2>), dim3((unsigned)wgs, (unsigned)p.splits), dim3(256), 0, s, p);
+            if (p.splits > 1) hipLaunchKernelGGL((kv4_many_join_kernel<HD>), dim3(a.b.rows), dim3(256), 0, s, p);
+        }
+    };
+    if (a.b.sequences * nkv * 2 > 0x7FFFFFFFu || (all / 16 + a.b.sequences + 4) * nkv > 0x7FFFFFFFu) return hipErrorInvalidValue;
     switch (a.c.hd) {
-    case 64: hipLaunchKernelGGL(kv4_simple_kernel<64>, grid, dim3(64), 0, s, p); break;
-    case 96: hipLaunchKernelGGL(kv4_simple_kernel<96>, grid, dim3(64), 0, s, p); break;
-    case 128: hipLaunchKernelGGL(kv4_simple_kernel<128>, grid, dim3(64), 0, s, p); break;
-    case 256: hipLaunchKernelGGL(kv4_simple_kernel<256>, grid, dim3(64), 0, s, p); break;
+    case 64: go(std::integral_constant<int, 64>{}, std::integral_constant<int, 2>{}); break;
+    case 96: go(std::integral_constant<int, 96>{}, std::integral_constant<int, 2>{}); break;
+    case 128: go(std::integral_constant<int, 128>{}, std::integral_constant<int, 2>{}); break;
+    case 256: go(std::integral_constant<int, 256>{}, std::integral_constant<int, 1>{}); break;
     default: return hipErrorInvalidValue;
     }
     return hipGetLastError();

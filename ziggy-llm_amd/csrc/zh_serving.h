@@ -31,6 +31,20 @@ __device__ __forceinline__ Sequence sequence_of(const Batch &b, uint32_t s) {
     q.first = (int)(n < 0x7FFFFFFFu ? n : 0x7FFFFFFFu) - (int)all;
     return q;
 }
+// The sequence that row r belongs to; rows 0: none.  Every lane of a wavefront takes part.
+__device__ __forceinline__ Sequence sequence_of_row(const Batch &b, uint32_t r) {
+    uint32_t s = 0;  // starts at or below r behind the first
+    for (uint32_t from = 0; from < b.sequences; from += 64) {
+        const uint32_t i = from + (threadIdx.x & 63);
+        const unsigned long long below = __ballot(i < b.sequences && b.starts[min(i, b.sequences - 1) + 1] <= r);
+        s += (uint32_t)__popcll(below);
+        if (~below) break;
+    }
+    Sequence q{};
+    if (s < b.sequences) q = sequence_of(b, s);
+    if (r < q.row0 || r - q.row0 >= q.rows) q.rows = 0;
+    return q;
+}
 // the pool's page that position t < cap lies in; `pool` or above: none
 __device__ __forceinline__ uint32_t page_of(const Batch &b, uint32_t s, uint32_t t) {
     return b.pages[(size_t)s * b.per_seq + t / kPage];

@@ -1,4 +1,17 @@
 // zh_logprobs.hip -- log probabilities of given tokens, the rows' entropy and their best tokens.
+//
+// ln p_t = (x_t - m) - ln S, S = sum e^(x - m), m the largest logit; the entropy is ln S - T / S, T = sum e^d d of
+// d = x - m.  The largest's own weight, 1, stays out of the sums, so that ln S = log1p(S') keeps its digits where one
+// token takes nearly everything.
+//
+// Two launches, one pass over the logits:
+//   slices  a workgroup per 2048 logits (8192 where rows alone fill the device), held in registers: the largest, the
+//           sums relative to it, and its k best in order;
+//   rows    a workgroup per row joins its slices.
+// The k best: a value that at least k others of the slice reach (the k-th of 64 columns' largest) leaves few
+// candidates, and a candidate's place is the count of those above it: no sort, no dependence on the order of arrival.
+#include <algorithm>
+
 #include "zh_serving.h"
 
 namespace zh {
@@ -7,7 +20,19 @@ namespace {
 
 typedef unsigned long long u64;
 
-// orders by value, the highest first, then by index, the lowest first; NaN as -infinity, the zeros equal
+constexpr int kThreads = 256, kCandidates = 1024, kMaxSlices = 128, kTop = ZIGGY_HIP_MAX_TOP_LOGPROBS;
+
+struct SliceSums {
+    u64 best;     // the largest
+    double s, t;  // of the others' weights relative to it, and of those times their logits less its own
+};
+struct LogprobsWork {
+    SliceSums *sums;  // [row][slice]
+    u64 *top;         // [row][slice][k]
+    uint32_t slices;
+};
+
+// orders by value, the highest first, then by index, the lowest first; NaN as -infinity, the zeros equal; above 0
 __device__ __forceinline__ u64 key_of(float v, uint32_t i) {
     const uint32_t b = __float_as_uint(v != v ? -INFINITY : v + 0.f);
     return (u64)(b & 0x80000000u ? ~b : b | 0x80000000u) << 32 | (0xFFFFFFFFu - i);
@@ -16,66 +41,233 @@ __device__ __forceinline__ float value_of_key(u64 k) {
     const uint32_t o = (uint32_t)(k >> 32);
     return __uint_as_float(o & 0x80000000u ? o & 0x7FFFFFFFu : ~o);
 }
+__device__ __forceinline__ uint32_t index_of_key(u64 k) { return 0xFFFFFFFFu - (uint32_t)k; }
 
-// A workgroup per row.
-__global__ void __launch_bounds__(1024) logprobs_kernel(TokenLogprobs p) {
-    __shared__ u64 best[16];
-    __shared__ double sums[2][16];
-    const uint32_t r = blockIdx.x, tid = threadIdx.x, wave = tid >> 6;
-    const float *x = p.x + (size_t)r * p.stride;
-    auto top_below = [&](u64 limit) {
+// e^d for d <= 0 to about a step and a half of binary32: the exponent's own rounding comes back to first order
+__device__ __forceinline__ float exp_of(float d) {
+    const float t = d * 1.44269504f, r = fmaf(d, 1.44269504f, -t) + d * 1.92596299e-8f, e = __builtin_amdgcn_exp2f(t);
+    return fmaf(e, r * 0.693147181f, e);
+}
+
+__device__ __forceinline__ double wave_sum(double v) {
+    auto add = [](double x, u64 y) { return x + __longlong_as_double((long long)y); };
+    v = add(v, dpp_u64<0xB1>((u64)__double_as_longlong(v)));
+    v = add(v, dpp_u64<0x4E>((u64)__double_as_longlong(v)));
+    v = add(v, dpp_u64<0x141>((u64)__double_as_longlong(v)));
+    v = add(v, dpp_u64<0x140>((u64)__double_as_longlong(v)));
+    auto far = [](double x, auto d) {
+        const u64 u = (u64)__double_as_longlong(x);
+        uint32_t a0, b0, a1, b1;
+        lane_pair<decltype(d)::value>((uint32_t)u, a0, b0);
+        lane_pair<decltype(d)::value>((uint32_t)(u >> 32), a1, b1);
+        return __longlong_as_double((long long)((u64)a1 << 32 | a0)) + __longlong_as_double((long long)((u64)b1 << 32 | b0));
+    };
+    v = far(v, std::integral_constant<int, 16>{});
+    return far(v, std::integral_constant<int, 32>{});
+}
+
+// candidates' places by counting: those of rank below k go to `to`
+__device__ __forceinline__ void place(const u64 *candidates, int n, int k, u64 *to) {
+    for (int i = threadIdx.x; i < n; i += blockDim.x) {
+        const u64 own = candidates[i];
+        int rank = 0;
+        for (int j = 0; j < n; j++) rank += candidates[j] > own;
+        if (rank < k) to[rank] = own;
+    }
+}
+
+// A workgroup per slice of 256 V logits.
+template <int V> __global__ void __launch_bounds__(kThreads) logprobs_slice_kernel(TokenLogprobs p, LogprobsWork w) {
+    __shared__ u64 best[4], columns[4][64], candidates[kCandidates], limit;
+    __shared__ double sums[2][4];
+    __shared__ int found;
+    const uint32_t row = blockIdx.x / w.slices, slice = blockIdx.x % w.slices, first = slice * (kThreads * V);
+    const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
+    const float *x = p.x + (size_t)row * p.stride + first;
+    const uint32_t n = min((uint32_t)(kThreads * V), p.vocab - first);
+    float v[V];
+    auto at = [&](int j) { return (uint32_t)((j / 4 * kThreads + tid) * 4 + j % 4); };
+#pragma unroll
+    for (int j = 0; j < V; j += 4) {
+        if (at(j) + 4 <= n) {
+            __builtin_memcpy(&v[j], x + at(j), 16);
+        } else {
+#pragma unroll
+            for (int e = 0; e < 4; e++) v[j + e] = at(j) + e < n ? x[at(j) + e] : -INFINITY;
+        }
+    }
+    u64 own = 0;
+#pragma unroll
+    for (int j = 0; j < V; j++) {
+        if (v[j] != v[j]) v[j] = -INFINITY;
+        const u64 k = key_of(v[j], first + at(j));
+        if (at(j) < n && k > own) own = k;
+    }
+    u64 m = wave_max_key(own);
+    if (lane == 0) best[wave] = m;
+    if (p.k) columns[wave][lane] = own;
+    if (tid == 0) found = 0, limit = 1;
+    __syncthreads();
+    m = max(max(best[0], best[1]), max(best[2], best[3]));
+    const float top = value_of_key(m);
+    const uint32_t skip = index_of_key(m) - first;
+    double s = 0.0, t = 0.0;
+#pragma unroll
+    for (int j = 0; j < V; j += 4) {  // four at a time in binary32
+        float e[4], d[4];
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            d[i] = fmaxf(v[j + i] - top, -1000.f);  // (a weight of 0 all the same)
+            e[i] = at(j + i) == skip ? 0.f : exp_of(d[i]);
+        }
+        s += (double)((e[0] + e[1]) + (e[2] + e[3]));
+        t += (double)(fmaf(e[0], d[0], e[1] * d[1]) + fmaf(e[2], d[2], e[3] * d[3]));
+    }
+    s = wave_sum(s), t = wave_sum(t);
+    if (lane == 0) sums[0][wave] = s, sums[1][wave] = t;
+    if (p.k && wave == 0) {
+        // the k-th of the columns' largest
+        const u64 column = max(max(columns[0][lane], columns[1][lane]), max(columns[2][lane], columns[3][lane]));
+        int rank = 0;
+#pragma unroll 16
+        for (int i = 0; i < 64; i++) {
+            const u64 other = (u64)(uint32_t)__builtin_amdgcn_readlane((int)(column >> 32), i) << 32 | (uint32_t)__builtin_amdgcn_readlane((int)column, i);
+            rank += other > column;
+        }
+        if (rank == p.k - 1 && column) limit = column;
+    }
+    __syncthreads();
+    const size_t out = (size_t)row * w.slices + slice;
+    if (tid == 0) w.sums[out] = {m, (sums[0][0] + sums[0][1]) + (sums[0][2] + sums[0][3]), (sums[1][0] + sums[1][1]) + (sums[1][2] + sums[1][3])};
+    if (p.k == 0) return;
+    const u64 least = limit;
+    if (own >= least) {
+#pragma unroll
+        for (int j = 0; j < V; j++) {
+            const u64 k = key_of(v[j], first + at(j));
+            if (at(j) < n && k >= least) {
+                const int i = atomicAdd(&found, 1);
+                if (i < kCandidates) candidates[i] = k;
+            }
+        }
+    }
+    __syncthreads();
+    u64 *to = w.top + out * p.k;
+    const int c = found;
+    if (c <= kCandidates) {
+        for (int i = c + tid; i < p.k; i += kThreads) to[i] = 0;  // (fewer logits than that)
+        place(candidates, c, p.k, to);
+        return;
+    }
+    // the best crowd a few columns (their places in the slice alike to a multiple of 256): one after the other
+    for (int i = 0; i < p.k; i++) {
         u64 k = 0;
-        for (uint32_t i = tid; i < p.vocab; i += 1024) {
-            const u64 n = key_of(x[i], i);
-            if (n < limit && n > k) k = n;
+#pragma unroll
+        for (int j = 0; j < V; j++) {
+            const u64 o = key_of(v[j], first + at(j));
+            if (at(j) < n && o > k && (i == 0 || o < m)) k = o;
         }
         k = wave_max_key(k);
-        if ((tid & 63) == 0) best[wave] = k;
         __syncthreads();
-        k = 0;
-        for (int w = 0; w < 16; w++) k = best[w] > k ? best[w] : k;
+        if (lane == 0) best[wave] = k;
         __syncthreads();
-        return k;
-    };
-    u64 k = top_below(~0ull);
-    const float m = value_of_key(k);
-    const uint32_t at = 0xFFFFFFFFu - (uint32_t)k;  // its own weight, 1, stays out of the sum, which may be next to nothing
-    double s = 0, t = 0;
-    for (uint32_t i = tid; i < p.vocab; i += 1024) {
-        if (i == at) continue;
-        const float v = x[i], d = v != v ? -INFINITY : v - m, e = expf(d);
-        s += (double)e;
-        if (e > 0.f) t += (double)e * (double)d;
+        m = max(max(best[0], best[1]), max(best[2], best[3]));
+        if (tid == 0) to[i] = m;
     }
-    for (int d = 1; d < 64; d <<= 1) s += __shfl_xor(s, d), t += __shfl_xor(t, d);
-    if ((tid & 63) == 0) sums[0][wave] = s, sums[1][wave] = t;
+}
+
+// A workgroup per row.
+__global__ void __launch_bounds__(1024) logprobs_row_kernel(TokenLogprobs p, LogprobsWork w) {
+    __shared__ u64 best[2], heads[8][kMaxSlices], candidates[kTop * kMaxSlices], placed[kTop], limits[8];
+    __shared__ double sums[2][2];
+    __shared__ int found;
+    const uint32_t row = blockIdx.x, n = w.slices;
+    const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
+    const SliceSums *from = w.sums + (size_t)row * n;
+    const u64 *top = w.top + (size_t)row * n * p.k;
+    SliceSums own{};
+    if ((uint32_t)tid < n) own = from[tid];
+    const uint32_t token = p.tokens[row];
+    const float given = token < p.vocab ? p.x[(size_t)row * p.stride + token] : 0.f;
+    // For each j of 1, 2, 4 .. k: of the slices' j-th best the ceil(k / j)-th largest is a value that k logits reach.
+    const int group = tid >> 7, j = 1 << group, i = tid & 127;
+    if (p.k) {
+        heads[group][i] = (uint32_t)i < n && j <= p.k ? top[(size_t)i * p.k + j - 1] : 0ull;
+        if (i == 0) limits[group] = 1;
+    }
+    if (tid == 0) found = 0;
+    if (tid < 64 * 2) {
+        const u64 m = wave_max_key(own.best);
+        if (lane == 0) best[wave] = m;
+    }
     __syncthreads();
-    s = t = 0;
-    for (int w = 0; w < 16; w++) s += sums[0][w], t += sums[1][w];
-    const double nan = (double)__uint_as_float(0x7FC00000u), log_s = isfinite(m) ? log1p(s) : nan;
-    if (tid == 0) {
-        const uint32_t token = p.tokens[r];
-        double y = nan;
-        if (token < p.vocab) {
-            const float v = x[token];
-            y = ((double)(v != v ? -INFINITY : v) - (double)m) - log_s;
+    const u64 m = max(best[0], best[1]);
+    const float largest = value_of_key(m);
+    if (tid < 64 * 2) {
+        double s = 0.0, t = 0.0;
+        if (own.best == m) s = own.s, t = own.t;
+        else if (own.best && value_of_key(own.best) > -INFINITY) {
+            const double d = (double)value_of_key(own.best) - (double)largest, f = exp(d);
+            s = f * (1.0 + own.s), t = f > 0.0 ? f * (own.t + d * (1.0 + own.s)) : 0.0;
         }
-        p.out[r] = (float)y;
-        if (p.entropy) p.entropy[r] = (float)(log_s - t / (1.0 + s));
+        s = wave_sum(s), t = wave_sum(t);
+        if (lane == 0) sums[0][wave] = s, sums[1][wave] = t;
     }
-    for (int i = 0; i < p.k; i++) {
-        if (tid == 0) {
-            p.top_tokens[(size_t)r * p.k + i] = 0xFFFFFFFFu - (uint32_t)k;
-            p.top[(size_t)r * p.k + i] = (float)(((double)value_of_key(k) - (double)m) - log_s);
+    if (p.k) {
+        const u64 mine = heads[group][i];
+        int rank = 0;
+        for (uint32_t o = 0; o < n; o++) rank += heads[group][o] > mine;
+        if (mine && rank == (p.k + j - 1) / j - 1) limits[group] = mine;
+    }
+    __syncthreads();
+    const double s = sums[0][0] + sums[0][1], t = sums[1][0] + sums[1][1], nan = (double)__uint_as_float(0x7FC00000u);
+    const double log_s = isfinite(largest) ? log1p(s) : nan;
+    auto logprob = [&](float v) { return (float)(((double)(v != v ? -INFINITY : v) - (double)largest) - log_s); };
+    if (tid == 0) {
+        p.out[row] = token < p.vocab ? logprob(given) : (float)nan;
+        if (p.entropy) p.entropy[row] = (float)(log_s - t / (1.0 + s));
+    }
+    if (p.k == 0) return;
+    u64 least = 1;
+#pragma unroll
+    for (int g = 0; g < 8; g++) least = max(least, limits[g]);
+    // a slice's are in order: an eighth of a wavefront takes a slice until one falls below
+    for (uint32_t a = (uint32_t)tid / 8; a < n; a += 128)
+        for (int b = tid & 7; b < p.k; b += 8) {
+            const u64 k = top[(size_t)a * p.k + b];
+            if (k < least) break;
+            candidates[atomicAdd(&found, 1)] = k;
         }
-        if (i + 1 < p.k) k = top_below(k);
+    __syncthreads();
+    place(candidates, found, p.k, placed);
+    __syncthreads();
+    if (tid < p.k) {
+        p.top_tokens[(size_t)row * p.k + tid] = index_of_key(placed[tid]);
+        p.top[(size_t)row * p.k + tid] = logprob(value_of_key(placed[tid]));
     }
 }
 
 }  // namespace
 
-hipError_t launch_token_logprobs(const TokenLogprobs &p, int cus, hipStream_t s) {
-    hipLaunchKernelGGL(logprobs_kernel, dim3(p.rows), dim3(1024), 0, s, p);
+hipError_t launch_token_logprobs(const TokenLogprobs &a, int cus, hipStream_t s) {
+    // slices of 2048 logits fill the device while there are up to 16 workgroups a CU of them
+    const bool wide = (uint64_t)a.rows * ((a.vocab + 2047) / 2048) > 16ull * cus;
+    LogprobsWork w{};
+    w.slices = wide ? (a.vocab + 8191) / 8192 : (a.vocab + 2047) / 2048;
+    const size_t each = w.slices * (sizeof(SliceSums) + 8 * (size_t)a.k);
+    const uint32_t most = (uint32_t)std::min<size_t>(a.work_bytes / each, 0x7FFFFFFFu / w.slices);
+    TokenLogprobs p = a;
+    for (uint32_t r = 0; r < a.rows; r += p.rows) {  // as many rows at a time as the workspace holds
+        p.rows = std::min(a.rows - r, most);
+        p.x = a.x + (size_t)r * a.stride, p.tokens = a.tokens + r, p.out = a.out + r;
+        p.entropy = a.entropy ? a.entropy + r : nullptr;
+        if (a.k) p.top = a.top + (size_t)r * a.k, p.top_tokens = a.top_tokens + (size_t)r * a.k;
+        w.sums = (SliceSums *)a.work, w.top = (u64 *)(w.sums + (size_t)p.rows * w.slices);
+        const dim3 grid(p.rows * w.slices);
+        if (wide) hipLaunchKernelGGL(logprobs_slice_kernel<32>, grid, dim3(kThreads), 0, s, p, w);
+        else hipLaunchKernelGGL(logprobs_slice_kernel<8>, grid, dim3(kThreads), 0, s, p, w);
+        hipLaunchKernelGGL(logprobs_row_kernel, dim3(p.rows), dim3(1024), 0, s, p, w);
+    }
     return hipGetLastError();
 }
 

@@ -1,8 +1,8 @@
 // zh_logprobs.hip -- log probabilities of given tokens, the rows' entropy and their best tokens.
 //
 // ln p_t = (x_t - m) - ln S, S = sum e^(x - m), m the largest logit; the entropy is ln S - T / S, T = sum e^d d of
-// d = x - m.  The largest's own weight, 1, stays out of the sums, so that ln S = log1p(S') keeps its digits where one
-// token takes nearly everything.
+// d = x - m.  The largest's own weight, 1, stays out of the sums (others as large are counted), so that ln S = log1p(S')
+// keeps its digits where one token takes nearly everything.
 //
 // Two launches, one pass over the logits:
 //   slices  a workgroup per 2048 logits (8192 where rows alone fill the device), held in registers: the largest, the
@@ -23,8 +23,9 @@ typedef unsigned long long u64;
 constexpr int kThreads = 256, kCandidates = 1024, kMaxSlices = 128, kTop = ZIGGY_HIP_MAX_TOP_LOGPROBS;
 
 struct SliceSums {
-    u64 best;     // the largest
-    double s, t;  // of the others' weights relative to it, and of those times their logits less its own
+    float top;       // the largest
+    uint32_t count;  // logits that are
+    double s, t;     // of the others' weights relative to it, and of those times their logits less its own
 };
 struct LogprobsWork {
     SliceSums *sums;  // [row][slice]
@@ -43,10 +44,11 @@ __device__ __forceinline__ float value_of_key(u64 k) {
 }
 __device__ __forceinline__ uint32_t index_of_key(u64 k) { return 0xFFFFFFFFu - (uint32_t)k; }
 
-// e^d for d <= 0 to about a step and a half of binary32: the exponent's own rounding comes back to first order
+// e^d for d <= 0 to about a step and a half of binary32: what the exponent's rounding leaves off comes back to first
+// order.  -infinity (and NaN) as -150: 0 all the same.
 __device__ __forceinline__ float exp_of(float d) {
-    const float t = d * 1.44269504f, r = fmaf(d, 1.44269504f, -t) + d * 1.92596299e-8f, e = __builtin_amdgcn_exp2f(t);
-    return fmaf(e, r * 0.693147181f, e);
+    const float t = d * 1.44269504f, r = fmaf(t, 1.90465421e-9f, fmaf(t, -0.693147182f, d)), e = __builtin_amdgcn_exp2f(t);
+    return fmaf(e, r, e);
 }
 
 __device__ __forceinline__ double wave_sum(double v) {
@@ -78,11 +80,13 @@ __device__ __forceinline__ void place(const u64 *candidates, int n, int k, u64 *
 
 // A workgroup per slice of 256 V logits.
 template <int V> __global__ void __launch_bounds__(kThreads) logprobs_slice_kernel(TokenLogprobs p, LogprobsWork w) {
-    __shared__ u64 best[4], columns[4][64], candidates[kCandidates], limit;
+    __shared__ u64 columns[4][64], candidates[kCandidates];
     __shared__ double sums[2][4];
-    __shared__ int found;
+    __shared__ float tops[4];
+    __shared__ uint32_t counts[4];
+    __shared__ int ranks[64], found;
     const uint32_t row = blockIdx.x / w.slices, slice = blockIdx.x % w.slices, first = slice * (kThreads * V);
-    const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
+    const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
     const float *x = p.x + (size_t)row * p.stride + first;
     const uint32_t n = min((uint32_t)(kThreads * V), p.vocab - first);
     float v[V];
@@ -96,51 +100,70 @@ template <int V> __global__ void __launch_bounds__(kThreads) logprobs_slice_kern
             for (int e = 0; e < 4; e++) v[j + e] = at(j) + e < n ? x[at(j) + e] : -INFINITY;
         }
     }
-    u64 own = 0;
+    float top = -INFINITY;  // (fmaxf passes over NaN)
 #pragma unroll
-    for (int j = 0; j < V; j++) {
-        if (v[j] != v[j]) v[j] = -INFINITY;
-        const u64 k = key_of(v[j], first + at(j));
-        if (at(j) < n && k > own) own = k;
-    }
-    u64 m = wave_max_key(own);
-    if (lane == 0) best[wave] = m;
-    if (p.k) columns[wave][lane] = own;
-    if (tid == 0) found = 0, limit = 1;
-    __syncthreads();
-    m = max(max(best[0], best[1]), max(best[2], best[3]));
-    const float top = value_of_key(m);
-    const uint32_t skip = index_of_key(m) - first;
-    double s = 0.0, t = 0.0;
+    for (int j = 0; j < V; j++) top = fmaxf(top, v[j]);
+    u64 own = 0;  // this thread's best, while the best are asked for
+    if (p.k) {
+        uint32_t best = 0;
 #pragma unroll
-    for (int j = 0; j < V; j += 4) {  // four at a time in binary32
-        float e[4], d[4];
-#pragma unroll
-        for (int i = 0; i < 4; i++) {
-            d[i] = fmaxf(v[j + i] - top, -1000.f);  // (a weight of 0 all the same)
-            e[i] = at(j + i) == skip ? 0.f : exp_of(d[i]);
+        for (int j = V - 1; j >= 0; j--) {
+            if (v[j] != v[j]) v[j] = -INFINITY;
+            if (v[j] == top) best = at(j);
         }
-        s += (double)((e[0] + e[1]) + (e[2] + e[3]));
-        t += (double)(fmaf(e[0], d[0], e[1] * d[1]) + fmaf(e[2], d[2], e[3] * d[3]));
+        if (best < n) own = key_of(top, first + best);  // (-infinity: the first of its own or none's)
+        columns[wave][lane] = own;
+        if (wave == 0) ranks[lane] = 0;
+    }
+    top = wave_max_f32(top);
+    if (lane == 0) tops[wave] = top;
+    if (tid == 0) found = 0;
+    __syncthreads();
+    top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
+    double s = 0.0, t = 0.0;
+    uint32_t count = 0;
+#pragma unroll
+    for (int j = 0; j < V; j += 8) {  // eight at a time in binary32
+        float e[8], d[8];
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+            d[i] = fmaxf(v[j + i] - top, -150.f);
+            const bool largest = v[j + i] == top;
+            count += largest;
+            e[i] = largest ? 0.f : exp_of(d[i]);
+        }
+        s += (double)(((e[0] + e[1]) + (e[2] + e[3])) + ((e[4] + e[5]) + (e[6] + e[7])));
+        t += (double)((fmaf(e[0], d[0], e[1] * d[1]) + fmaf(e[2], d[2], e[3] * d[3])) + (fmaf(e[4], d[4], e[5] * d[5]) + fmaf(e[6], d[6], e[7] * d[7])));
     }
     s = wave_sum(s), t = wave_sum(t);
-    if (lane == 0) sums[0][wave] = s, sums[1][wave] = t;
-    if (p.k && wave == 0) {
-        // the k-th of the columns' largest
-        const u64 column = max(max(columns[0][lane], columns[1][lane]), max(columns[2][lane], columns[3][lane]));
+    for (int d = 1; d < 64; d <<= 1) count += (uint32_t)__shfl_xor((int)count, d);
+    if (lane == 0) sums[0][wave] = s, sums[1][wave] = t, counts[wave] = count;
+    u64 column = 0;
+    if (p.k) {
+        // ranks of the columns' largest, each wavefront against sixteen of them
+        column = max(max(columns[0][lane], columns[1][lane]), max(columns[2][lane], columns[3][lane]));
         int rank = 0;
-#pragma unroll 16
-        for (int i = 0; i < 64; i++) {
-            const u64 other = (u64)(uint32_t)__builtin_amdgcn_readlane((int)(column >> 32), i) << 32 | (uint32_t)__builtin_amdgcn_readlane((int)column, i);
+#pragma unroll
+        for (int i = 0; i < 16; i++) {
+            const u64 other = (u64)(uint32_t)__builtin_amdgcn_readlane((int)(column >> 32), 16 * wave + i) << 32 |
+                              (uint32_t)__builtin_amdgcn_readlane((int)column, 16 * wave + i);
             rank += other > column;
         }
-        if (rank == p.k - 1 && column) limit = column;
+        atomicAdd(&ranks[lane], rank);
     }
     __syncthreads();
     const size_t out = (size_t)row * w.slices + slice;
-    if (tid == 0) w.sums[out] = {m, (sums[0][0] + sums[0][1]) + (sums[0][2] + sums[0][3]), (sums[1][0] + sums[1][1]) + (sums[1][2] + sums[1][3])};
+    if (tid == 0)
+        w.sums[out] = {top, counts[0] + counts[1] + counts[2] + counts[3], (sums[0][0] + sums[0][1]) + (sums[0][2] + sums[0][3]),
+                       (sums[1][0] + sums[1][1]) + (sums[1][2] + sums[1][3])};
     if (p.k == 0) return;
-    const u64 least = limit;
+    // the k-th of the columns' largest, which k logits reach
+    const u64 here = __ballot(ranks[lane] == p.k - 1 && column);
+    u64 least = 1;
+    if (here) {
+        const int i = __ffsll(here) - 1;
+        least = (u64)(uint32_t)__builtin_amdgcn_readlane((int)(column >> 32), i) << 32 | (uint32_t)__builtin_amdgcn_readlane((int)column, i);
+    }
     if (own >= least) {
 #pragma unroll
         for (int j = 0; j < V; j++) {
@@ -160,32 +183,34 @@ template <int V> __global__ void __launch_bounds__(kThreads) logprobs_slice_kern
         return;
     }
     // the best crowd a few columns (their places in the slice alike to a multiple of 256): one after the other
+    u64 last = ~0ull;
     for (int i = 0; i < p.k; i++) {
         u64 k = 0;
 #pragma unroll
         for (int j = 0; j < V; j++) {
             const u64 o = key_of(v[j], first + at(j));
-            if (at(j) < n && o > k && (i == 0 || o < m)) k = o;
+            if (at(j) < n && o > k && o < last) k = o;
         }
         k = wave_max_key(k);
         __syncthreads();
-        if (lane == 0) best[wave] = k;
+        if (lane == 0) columns[0][wave] = k;
         __syncthreads();
-        m = max(max(best[0], best[1]), max(best[2], best[3]));
-        if (tid == 0) to[i] = m;
+        last = max(max(columns[0][0], columns[0][1]), max(columns[0][2], columns[0][3]));
+        if (tid == 0) to[i] = last;
     }
 }
 
 // A workgroup per row.
 __global__ void __launch_bounds__(1024) logprobs_row_kernel(TokenLogprobs p, LogprobsWork w) {
-    __shared__ u64 best[2], heads[8][kMaxSlices], candidates[kTop * kMaxSlices], placed[kTop], limits[8];
-    __shared__ double sums[2][2];
+    __shared__ __align__(16) u64 heads[8][kMaxSlices], candidates[kTop * kMaxSlices], placed[kTop], limits[8];
+    __shared__ double sums[3][2];
+    __shared__ float tops[2];
     __shared__ int found;
     const uint32_t row = blockIdx.x, n = w.slices;
     const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
     const SliceSums *from = w.sums + (size_t)row * n;
     const u64 *top = w.top + (size_t)row * n * p.k;
-    SliceSums own{};
+    SliceSums own{-INFINITY, 0, 0.0, 0.0};
     if ((uint32_t)tid < n) own = from[tid];
     const uint32_t token = p.tokens[row];
     const float given = token < p.vocab ? p.x[(size_t)row * p.stride + token] : 0.f;
@@ -197,30 +222,32 @@ __global__ void __launch_bounds__(1024) logprobs_row_kernel(TokenLogprobs p, Log
     }
     if (tid == 0) found = 0;
     if (tid < 64 * 2) {
-        const u64 m = wave_max_key(own.best);
-        if (lane == 0) best[wave] = m;
+        const float m = wave_max_f32(own.top);
+        if (lane == 0) tops[wave] = m;
     }
     __syncthreads();
-    const u64 m = max(best[0], best[1]);
-    const float largest = value_of_key(m);
+    const float largest = fmaxf(tops[0], tops[1]);
     if (tid < 64 * 2) {
-        double s = 0.0, t = 0.0;
-        if (own.best == m) s = own.s, t = own.t;
-        else if (own.best && value_of_key(own.best) > -INFINITY) {
-            const double d = (double)value_of_key(own.best) - (double)largest, f = exp(d);
-            s = f * (1.0 + own.s), t = f > 0.0 ? f * (own.t + d * (1.0 + own.s)) : 0.0;
+        // slices that have the largest give its count, the others their weights
+        double s = own.s, t = own.t, count = own.top == largest ? (double)own.count : 0.0;
+        if (own.top != largest) {
+            const double d = fmax((double)own.top - (double)largest, -1000.0), f = exp(d), all = own.count + own.s;
+            s = f * all, t = f * (own.t + d * all);
         }
-        s = wave_sum(s), t = wave_sum(t);
-        if (lane == 0) sums[0][wave] = s, sums[1][wave] = t;
+        s = wave_sum(s), t = wave_sum(t), count = wave_sum(count);
+        if (lane == 0) sums[0][wave] = s, sums[1][wave] = t, sums[2][wave] = count;
     }
-    if (p.k) {
+    if (j <= p.k) {
         const u64 mine = heads[group][i];
         int rank = 0;
-        for (uint32_t o = 0; o < n; o++) rank += heads[group][o] > mine;
+        for (uint32_t o = 0; o < n; o += 2) {  // (those behind the last are 0)
+            const ulonglong2 other = *reinterpret_cast<const ulonglong2 *>(&heads[group][o]);
+            rank += (other.x > mine) + (other.y > mine);
+        }
         if (mine && rank == (p.k + j - 1) / j - 1) limits[group] = mine;
     }
     __syncthreads();
-    const double s = sums[0][0] + sums[0][1], t = sums[1][0] + sums[1][1], nan = (double)__uint_as_float(0x7FC00000u);
+    const double s = (sums[0][0] + sums[0][1]) + (sums[2][0] + sums[2][1] - 1.0), t = sums[1][0] + sums[1][1], nan = (double)__uint_as_float(0x7FC00000u);
     const double log_s = isfinite(largest) ? log1p(s) : nan;
     auto logprob = [&](float v) { return (float)(((double)(v != v ? -INFINITY : v) - (double)largest) - log_s); };
     if (tid == 0) {

@@ -19,6 +19,10 @@ typedef __bf16 fb8 __attribute__((ext_vector_type(8)));
 typedef float ff4 __attribute__((ext_vector_type(4)));
 
 constexpr int kBlock = 32;  // positions of a product
+// The running maximum stays where it is while scores pass it by no more than this many powers of two: the outputs are
+// scaled again only where one does (with every new maximum of 32 columns, 200 of 480 blocks of a prompt).  Sums of 2^30
+// weights of 2^3 and values of 6 2^92 end below 2^128.
+constexpr float kSlack = 3.f;
 
 struct Kv4Params {
     Kv4Layer c;
@@ -62,6 +66,12 @@ __device__ __forceinline__ void share(int &begin, int &end, uint32_t parts, uint
     end = begin + (int)(each + (z < more ? 1u : 0u));
 }
 
+// What every lane has alike, in scalar registers.
+__device__ __forceinline__ uint32_t uniform(uint32_t v) { return (uint32_t)__builtin_amdgcn_readfirstlane((int)v); }
+__device__ __forceinline__ Sequence uniform(const Sequence &q) {
+    return {uniform(q.index), uniform(q.row0), uniform(q.rows), (int)uniform((uint32_t)q.first)};
+}
+
 // inclusive sum over a wavefront's lanes
 __device__ __forceinline__ uint32_t running_sum(uint32_t n) {
     const int lane = threadIdx.x & 63;
@@ -90,13 +100,13 @@ template <int COLUMNS> __device__ __forceinline__ Tile tile_of(const Kv4Params &
         const u64 past = __ballot(before + sum > number);
         if (past) {
             const int at = __ffsll(past) - 1;
-            t.q = sequence_of(p.b, from + at);
-            t.first = (number - before - (uint32_t)__shfl((int)(sum - n), at)) * COLUMNS;
+            t.q = uniform(sequence_of(p.b, from + at));
+            t.first = (number - before - (uint32_t)__builtin_amdgcn_readlane((int)(sum - n), at)) * COLUMNS;
             const uint32_t all = t.q.rows * group;  // (tables that don't ascend may pass 32 bits in the sums)
             t.count = t.first < all ? min((uint32_t)COLUMNS, all - t.first) : 0u;
             return t;
         }
-        before += (uint32_t)__shfl((int)sum, 63);
+        before += (uint32_t)__builtin_amdgcn_readlane((int)sum, 63);
     }
     return t;
 }
@@ -128,7 +138,7 @@ template <bool BY_SEQUENCE> __device__ __forceinline__ Share share_of(const Kv4P
     u64 total = own;
     for (uint32_t from = 64; from < p.b.sequences; from += 64) total += blocks(from + lane);
     for (int d = 1; d < 64; d <<= 1) total += __shfl_xor(total, d);
-    const uint32_t quota = max(kLeastBlocks, (uint32_t)ceil((double)total * nkv / p.wgs));
+    const uint32_t quota = uniform(max(kLeastBlocks, (uint32_t)ceil((double)total * nkv / p.wgs)));
     Share t{};
     uint32_t items = 0, slots = 0;
     for (uint32_t from = 0; from < p.b.sequences; from += 64) {
@@ -137,14 +147,14 @@ template <bool BY_SEQUENCE> __device__ __forceinline__ Share share_of(const Kv4P
         const u64 past = __ballot(BY_SEQUENCE ? from + lane == number : items + sum > number);
         if (past) {
             const int at = __ffsll(past) - 1;
-            t.q = sequence_of(p.b, from + at);
-            t.splits = (uint32_t)__shfl((int)splits, at);
+            t.q = uniform(sequence_of(p.b, from + at));
+            t.splits = (uint32_t)__builtin_amdgcn_readlane((int)splits, at);
             if (t.splits) t.r = range_of(p, t.q, 0, t.q.rows - 1);
-            t.index = number - items - (uint32_t)__shfl((int)(sum - splits * nkv), at);
-            t.slot = slots + (uint32_t)__shfl((int)slot_sum, at) - (t.splits > 1 ? t.splits * nkv : 0u);
+            t.index = number - items - (uint32_t)__builtin_amdgcn_readlane((int)(sum - splits * nkv), at);
+            t.slot = slots + (uint32_t)__builtin_amdgcn_readlane((int)slot_sum, at) - (t.splits > 1 ? t.splits * nkv : 0u);
             return t;
         }
-        items += (uint32_t)__shfl((int)sum, 63), slots += (uint32_t)__shfl((int)slot_sum, 63);
+        items += (uint32_t)__builtin_amdgcn_readlane((int)sum, 63), slots += (uint32_t)__builtin_amdgcn_readlane((int)slot_sum, 63);
     }
     return t;
 }
@@ -181,24 +191,22 @@ __device__ __forceinline__ float finite(float v) { return v == -INFINITY ? 0.f :
 // every 32 dims), and V's dims 32 t + i and 32 t + 16 + i of positions 8 g .. 8 g + 7.
 template <int HD> struct Lane4 {
     static constexpr int G = HD / 32;
-    uint32_t k[2][G], v[2 * G];
-    uint32_t ks[2][(G + 3) / 4], vs[2 * G];
+    uint32_t k[2][G], v[2 * G], ks[2][(G + 3) / 4], vs[2 * G];
     __device__ __forceinline__ void load_k(const Kv4Layer &c, uint32_t page, int head, int half) {
-        const int i = threadIdx.x & 15, g = threadIdx.x >> 4 & 3;
-        const size_t codes = c.codes(page, head), scales = c.scales(page, head);
+        const uint32_t i = threadIdx.x & 15, g = threadIdx.x >> 4 & 3, row = 8 * (i >> 2) + (i & 3);
+        const uint8_t *codes = c.kc + c.codes(page, head) + half * (kBlock / 2 * HD), *scales = c.ks + c.scales(page, head) + half * (kBlock * G);
 #pragma unroll
         for (int pt = 0; pt < 2; pt++) {
-            const int pos = kBlock * half + 8 * (i >> 2) + 4 * pt + (i & 3);
-            __builtin_memcpy(k[pt], c.kc + codes + (size_t)pos * (HD / 2) + g * 4 * G, 4 * G);
+            __builtin_memcpy(k[pt], codes + (row * (HD / 2) + g * 4 * G) + pt * (2 * HD), 4 * G);
             if constexpr (G % 4) ks[pt][0] = 0;
-            __builtin_memcpy(ks[pt], c.ks + scales + (size_t)pos * G, G);
+            __builtin_memcpy(ks[pt], scales + row * G + pt * (4 * G), G);
         }
     }
     __device__ __forceinline__ void load_v(const Kv4Layer &c, uint32_t page, int head, int half) {
-        const int i = threadIdx.x & 15, g = threadIdx.x >> 4 & 3;
-        const size_t codes = c.codes(page, head), scales = c.scales(page, head);
-        __builtin_memcpy(v, c.vc + codes + (size_t)half * (16 * HD) + (g * 16 + i) * 8 * G, 8 * G);
-        __builtin_memcpy(vs, c.vs + scales + (size_t)(kBlock * half + 8 * g) * G, 8 * G);
+        const uint32_t i = threadIdx.x & 15, g = threadIdx.x >> 4 & 3;
+        const uint8_t *codes = c.vc + c.codes(page, head) + half * (kBlock / 2 * HD), *scales = c.vs + c.scales(page, head) + half * (kBlock * G);
+        __builtin_memcpy(v, codes + (g * 16 + i) * (8 * G), 8 * G);
+        __builtin_memcpy(vs, scales + g * (8 * G), 8 * G);
     }
     // V's positions outside first .. last of the block as zeros: what was never stored may read as NaN
     __device__ __forceinline__ void clear_v(int first, int last) {
@@ -213,6 +221,32 @@ template <int HD> struct Lane4 {
             }
             v[w] &= keep, vs[w] &= keep;
         }
+    }
+    // K's 16 rows of half pt, dims 32 t ..: the left operand of scores
+    __device__ __forceinline__ fb8 key(int t, int pt) const {
+        const float scale = scale_of(ks[pt][t / 4], t % 4);
+        const uint32_t w[4] = {widen<0>(k[pt][t], scale), widen<1>(k[pt][t], scale), widen<2>(k[pt][t], scale), widen<3>(k[pt][t], scale)};
+        fb8 a;
+        __builtin_memcpy(&a, w, 16);
+        return a;
+    }
+    // V's dims 32 t + i and 32 t + 16 + i: the left operands of two tiles of outputs
+    __device__ __forceinline__ void values(int t, fb8 (&b)[2]) const {
+        uint32_t a[2][4];
+#pragma unroll
+        for (int j = 0; j < 8; j += 2) {
+            uint32_t y[2];
+#pragma unroll
+            for (int e = 0; e < 2; e++) {
+                const int n = (j + e) * G + t;  // byte of this position's dims
+                const float scale = scale_of(vs[n >> 2], n & 3);
+                const uint32_t word = v[n >> 2];
+                y[e] = (n & 3) == 0 ? widen<0>(word, scale) : (n & 3) == 1 ? widen<1>(word, scale) : (n & 3) == 2 ? widen<2>(word, scale) : widen<3>(word, scale);
+            }
+            a[0][j / 2] = __builtin_amdgcn_perm(y[1], y[0], 0x05040100u);
+            a[1][j / 2] = __builtin_amdgcn_perm(y[1], y[0], 0x07060302u);
+        }
+        __builtin_memcpy(b, a, 32);
     }
 };
 
@@ -265,9 +299,10 @@ template <int HD, int CT, int AWAY> struct Columns {
         }
     }
 
-    // 32 positions from `at` on; hidden: their page is none.  after_k, after_v: K's and V's registers are free.
-    template <class K, class V>
-    __device__ __forceinline__ void take(float qscale, const Range &r, Lane4<HD> &x, int at, bool hidden, K after_k, V after_v) {
+    // 32 positions from `at` on, key(t, pt) and values(t, b) their operands.  edge: some columns may not see all of them
+    // (hidden: their page is none).  after_k: the keys are through.
+    template <bool HOLD, class K, class V, class A>
+    __device__ __forceinline__ void take(float qscale, int at, bool edge, bool hidden, K key, V values, A after_k) {
         const int g = threadIdx.x >> 4 & 3;
         int lane = threadIdx.x & 63;
         if constexpr (AWAY > 0) __asm__ volatile("" : "+v"(lane));  // (the pieces in LDS are read where they are used, not ahead of the loop)
@@ -281,25 +316,17 @@ template <int HD, int CT, int AWAY> struct Columns {
             for (int c = 0; c < CT; c++)
 #pragma unroll
                 for (int k = 0; k < AWAY; k++) far[c][k] = away[((c * G + t) * AWAY + k) * 64 + lane];
-#pragma unroll
-            for (int pt = 0; pt < 2; pt++) {
-                const float scale = scale_of(x.ks[pt][t / 4], t % 4);
-                const uint32_t w[4] = {widen<0>(x.k[pt][t], scale), widen<1>(x.k[pt][t], scale), widen<2>(x.k[pt][t], scale), widen<3>(x.k[pt][t], scale)};
-                __builtin_memcpy(&a[pt], w, 16);
-            }
+            a[0] = key(t, 0), a[1] = key(t, 1);
 #pragma unroll
             for (int k = 0; k < 3; k++)
 #pragma unroll
                 for (int c = 0; c < CT; c++)
 #pragma unroll
                     for (int pt = 0; pt < 2; pt++) s[c][pt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a[pt], k < NEAR ? q[c][t][k < NEAR ? k : 0] : far[c][k < NEAR ? 0 : k - NEAR], s[c][pt], 0, 0, 0);
-            if constexpr (HD * CT > 128) __builtin_amdgcn_sched_barrier(0);
+            if constexpr (HOLD) __builtin_amdgcn_sched_barrier(0);  // (or the operands of all steps take registers at once)
         }
         after_k();
-        fb8 w[CT][3];
-        float next[CT];
-        bool grows = false;
-        if (hidden || at < r.full_first || at + kBlock - 1 > r.full_last) {
+        if (edge) {
 #pragma unroll
             for (int c = 0; c < CT; c++)
 #pragma unroll
@@ -307,15 +334,16 @@ template <int HD, int CT, int AWAY> struct Columns {
                     const int pos = at + 8 * g + e;
                     if (hidden || pos < lo[c] || pos > hi[c]) s[c][e >> 2][e & 3] = -INFINITY;
                 }
-            x.clear_v(r.first - at, hidden ? -1 : r.last - at);
         }
+        float next[CT];
+        bool grows = false;
 #pragma unroll
         for (int c = 0; c < CT; c++) {
             float top = s[c][0][0];
 #pragma unroll
             for (int e = 1; e < 8; e++) top = fmaxf(top, s[c][e >> 2][e & 3]);
             next[c] = fmaxf(m[c], xmax<32>(xmax<16>(top)) * qscale);
-            grows = grows || next[c] > m[c];
+            grows = grows || next[c] > m[c] + kSlack;  // (-infinity: the first)
         }
         if (__any(grows)) {
 #pragma unroll
@@ -327,6 +355,7 @@ template <int HD, int CT, int AWAY> struct Columns {
                 for (int d = 0; d < DT; d++) o[c][d] *= was;
             }
         }
+        fb8 w[CT][3];
 #pragma unroll
         for (int c = 0; c < CT; c++) {
             const float mf = finite(m[c]);
@@ -338,36 +367,21 @@ template <int HD, int CT, int AWAY> struct Columns {
         }
 #pragma unroll
         for (int t = 0; t < G; t++) {
-            uint32_t a[2][4];
-#pragma unroll
-            for (int j = 0; j < 8; j += 2) {
-                uint32_t y[2];
-#pragma unroll
-                for (int e = 0; e < 2; e++) {
-                    const int n = (j + e) * G + t;  // byte of this position's dims
-                    const float scale = scale_of(x.vs[n >> 2], n & 3);
-                    const uint32_t word = x.v[n >> 2];
-                    y[e] = (n & 3) == 0 ? widen<0>(word, scale) : (n & 3) == 1 ? widen<1>(word, scale) : (n & 3) == 2 ? widen<2>(word, scale) : widen<3>(word, scale);
-                }
-                a[0][j / 2] = __builtin_amdgcn_perm(y[1], y[0], 0x05040100u);
-                a[1][j / 2] = __builtin_amdgcn_perm(y[1], y[0], 0x07060302u);
-            }
             fb8 b[2];
-            __builtin_memcpy(b, a, 32);
+            values(t, b);
 #pragma unroll
             for (int k = 0; k < 3; k++)
 #pragma unroll
                 for (int c = 0; c < CT; c++)
 #pragma unroll
                     for (int h = 0; h < 2; h++) o[c][2 * t + h] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(b[h], w[c][k], o[c][2 * t + h], 0, 0, 0);
-            if constexpr (HD * CT > 128) __builtin_amdgcn_sched_barrier(0);
+            if constexpr (HOLD) __builtin_amdgcn_sched_barrier(0);
         }
-        after_v();
     }
 
     // The blocks begin, begin + step .. below end.  DEEP: the next block's loads go out ahead of the work on this one, into
     // registers of their own; otherwise K's and V's follow each other into the same ones as they come free.
-    template <bool DEEP> __device__ __forceinline__ void run(const Kv4Params &p, const Range &r, uint32_t sequence, int head, int begin, int end, int step) {
+    template <bool DEEP, bool HOLD> __device__ __forceinline__ void run(const Kv4Params &p, const Range &r, uint32_t sequence, int head, int begin, int end, int step) {
         if (begin >= end) return;
         const int lane = threadIdx.x & 63;
         uint32_t pages = 0;  // of the next 64 blocks, one a lane; those that the pool doesn't have: 0, not seen
@@ -384,31 +398,41 @@ template <int HD, int CT, int AWAY> struct Columns {
         const int n = (end - begin + step - 1) / step;
         auto page = [&](int i) { return (uint32_t)__builtin_amdgcn_readlane((int)pages, i & 63); };
         auto half = [&](int i) { return (begin + step * i) & 1; };
-        if constexpr (DEEP) {
-            Lane4<HD> x[2];
-            auto work = [&](int i, Lane4<HD> &now, Lane4<HD> &after) {
-                const bool hidden = missing >> (i & 63) & 1;
-                if ((i & 63) == 63) look(begin + step * (i + 1));
-                const int j = min(i + 1, n - 1);  // (the last one's again, unused)
-                after.load_k(p.c, page(j), head, half(j)), after.load_v(p.c, page(j), head, half(j));
-                take(p.qscale, r, now, (begin + step * i) * kBlock, hidden, [] {}, [] {});
-            };
-            x[0].load_k(p.c, page(0), head, half(0)), x[0].load_v(p.c, page(0), head, half(0));
-            for (int i = 0; i < n; i += 2) {
-                work(i, x[0], x[1]);
-                if (i + 1 < n) work(i + 1, x[1], x[0]);
+        // Inner blocks and those at an edge in loops of their own: where the two meet within one, the compiler copies the
+        // outputs' registers in every iteration (104 of 480 instructions).  Twice unrolled for the same reason.
+        int i = 0;
+        auto at = [&](int j) { return (begin + step * j) * kBlock; };
+        auto inner = [&](int j) { return at(j) >= r.full_first && at(j) + kBlock - 1 <= r.full_last && !(missing >> (j & 63) & 1); };
+        Lane4<HD> x, y;
+        x.load_k(p.c, page(0), head, half(0)), x.load_v(p.c, page(0), head, half(0));
+        auto edge_block = [&] {
+            const bool hidden = missing >> (i & 63) & 1;
+            if ((i & 63) == 63) look(begin + step * (i + 1));
+            const int j = min(i + 1, n - 1);  // (the last one's again, unused)
+            const uint32_t next = page(j);
+            x.clear_v(r.first - at(i), hidden ? -1 : r.last - at(i));
+            take<HOLD>(p.qscale, at(i), true, hidden, [&](int t, int pt) { return x.key(t, pt); }, [&](int t, fb8(&b)[2]) { x.values(t, b); },
+                             [&] { x.load_k(p.c, next, head, half(j)); });
+            x.load_v(p.c, next, head, half(j));
+            i++;
+        };
+        auto inner_block = [&](Lane4<HD> &now, Lane4<HD> &after) {
+            if ((i & 63) == 63) look(begin + step * (i + 1));
+            const int j = min(i + 1, n - 1);
+            const uint32_t next = page(j);
+            if constexpr (DEEP) after.load_k(p.c, next, head, half(j)), after.load_v(p.c, next, head, half(j));
+            take<HOLD>(p.qscale, at(i), false, false, [&](int t, int pt) { return now.key(t, pt); }, [&](int t, fb8(&b)[2]) { now.values(t, b); },
+                              [&] { if constexpr (!DEEP) after.load_k(p.c, next, head, half(j)); });
+            if constexpr (!DEEP) after.load_v(p.c, next, head, half(j));
+            i++;
+        };
+        while (i < n) {
+            while (i < n && !inner(i)) edge_block();
+            while (i + 1 < n && inner(i) && (((i & 63) != 63) && inner(i + 1))) {
+                if constexpr (DEEP) inner_block(x, y), inner_block(y, x);
+                else inner_block(x, x), inner_block(x, x);
             }
-        } else {
-            Lane4<HD> x;
-            x.load_k(p.c, page(0), head, half(0)), x.load_v(p.c, page(0), head, half(0));
-            for (int i = 0; i < n; i++) {
-                const bool hidden = missing >> (i & 63) & 1;
-                if ((i & 63) == 63) look(begin + step * (i + 1));
-                const int j = min(i + 1, n - 1);
-                const uint32_t next = page(j);
-                take(p.qscale, r, x, (begin + step * i) * kBlock, hidden, [&] { x.load_k(p.c, next, head, half(j)); },
-                     [&] { x.load_v(p.c, next, head, half(j)); });
-            }
+            if (i < n && inner(i)) edge_block();  // (one left of a pair: nothing is hidden of it)
         }
     }
 };
@@ -434,7 +458,7 @@ template <int HD, int CT> __global__ void __launch_bounds__(256, 2) kv4_few_kern
     share(begin, end, t.splits, z);
     Columns<HD, CT, AWAY> x;
     x.begin(p, t.q, 0, count, head, reinterpret_cast<fb8 *>(lds) + wave * (PIECES / 4));
-    x.template run<HD * CT <= 128>(p, t.r, t.q.index, head, begin + wave, end, 4);
+    x.template run<HD * CT <= 128, (HD * CT > 128)>(p, t.r, t.q.index, head, begin + wave, end, 4);
     if (AWAY) __syncthreads();
 #pragma unroll
     for (int c = 0; c < CT; c++) {
@@ -514,27 +538,100 @@ template <int HD, int CT> __global__ void __launch_bounds__(256) kv4_few_join_ke
     }
 }
 
-// Many columns (prompts): a wavefront takes a tile, through a split of its positions.
+// Many columns (prompts): a workgroup takes a tile of 64 CT columns, a wavefront 16 CT of them, through a split of its
+// pages.  A page's operands are widened once, a quarter by each wavefront, into LDS, in the order in which the
+// products take them; two pages' room, so that one barrier a page is enough.
+template <int HD> struct Quarter {  // wavefront (half h, pt): K rows of half h, its 16 of pt; V of half h, every second t from pt on
+    static constexpr int G = HD / 32, T = (G + 1) / 2;
+    Lane4<HD> x;
+    __device__ __forceinline__ void load(const Kv4Layer &c, uint32_t page, int head, int wave) {
+        const uint32_t i = threadIdx.x & 15, g = threadIdx.x >> 4 & 3, row = 8 * (i >> 2) + (i & 3);
+        const int half = wave >> 1, pt = wave & 1;
+        const uint8_t *codes = c.kc + c.codes(page, head) + half * (kBlock / 2 * HD) + pt * (2 * HD);
+        const uint8_t *scales = c.ks + c.scales(page, head) + half * (kBlock * G) + pt * (4 * G);
+        __builtin_memcpy(x.k[0], codes + (row * (HD / 2) + g * 4 * G), 4 * G);
+        if constexpr (G % 4) x.ks[0][0] = 0;
+        __builtin_memcpy(x.ks[0], scales + row * G, G);
+        x.load_v(c, page, head, half);
+    }
+    // to: K's chunks [half][pt][t], V's [half][dim tile], of 64 lanes each
+    __device__ __forceinline__ void store(fb8 *to, int wave) const {
+        const int lane = threadIdx.x & 63;
+#pragma unroll
+        for (int t = 0; t < G; t++) to[(wave * G + t) * 64 + lane] = x.key(t, 0);
+        fb8 *v = to + 4 * G * 64 + (wave >> 1) * (2 * G * 64) + lane;
+        auto put = [&](int t) {
+            fb8 b[2];
+            x.values(t, b);
+            v[2 * t * 64] = b[0], v[(2 * t + 1) * 64] = b[1];
+        };
+        if (wave & 1) {
+#pragma unroll
+            for (int t = 1; t < G; t += 2) put(t);
+        } else {
+#pragma unroll
+            for (int t = 0; t < G; t += 2) put(t);
+        }
+    }
+};
+
 template <int HD, int CT, int AWAY> __global__ void __launch_bounds__(256, 2) kv4_many_kernel(Kv4Params p) {
-    __shared__ fb8 held[4][CT * (HD / 32) * AWAY * 64];
-    const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), i = threadIdx.x & 15, g = threadIdx.x >> 4 & 3;
+    constexpr int G = HD / 32, PAGE = 8 * G * 64;  // a page's operands
+    __shared__ fb8 pages[2][PAGE];
+    __shared__ fb8 held[AWAY ? 4 : 1][AWAY ? CT * G * AWAY * 64 : 1];
+    const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), i = threadIdx.x & 15, g = threadIdx.x >> 4 & 3, lane = threadIdx.x & 63;
     const int head = (int)(blockIdx.x % p.c.nkv);
-    // the longest (last) first
-    const uint32_t number = (gridDim.x - 1 - blockIdx.x) / p.c.nkv * 4 + wave;
-    const Tile t = tile_of<16 * CT>(p, number);
+    const Tile t = tile_of<64 * CT>(p, (gridDim.x - 1 - blockIdx.x) / p.c.nkv);  // the longest (last) first
     if (t.count == 0) return;
     const Range r = range_of(p, t.q, t.first / p.group, (t.first + t.count - 1) / p.group);
-    int begin = r.begin, end = r.end;
+    int begin = r.begin / 2, end = r.end > r.begin ? (r.end + 1) / 2 : r.begin / 2;
     share(begin, end, (uint32_t)p.splits, blockIdx.y);
     Columns<HD, CT, AWAY> x;
-    x.begin(p, t.q, t.first, t.count, head, held[wave]);
-    x.template run<false>(p, r, t.q.index, head, begin, end, 1);
+    const uint32_t first = t.first + 16 * CT * wave;
+    x.begin(p, t.q, min(first, t.first + t.count - 1), first < t.first + t.count ? t.first + t.count - first : 1, head, held[AWAY ? wave : 0]);
+    uint32_t ids = 0;  // of the next 64 pages, one a lane; those that the pool doesn't have: 0, not seen
+    u64 missing = 0;
+    auto look = [&](int b) {
+        ids = 0xFFFFFFFFu;
+        if (b + lane < end) ids = page_of(p.b, t.q.index, (uint32_t)(b + lane) * kPage);
+        const bool none = ids >= p.b.pool;
+        if (none) ids = 0;
+        missing = __ballot(none);
+    };
+    auto id = [&](int n) { return (uint32_t)__builtin_amdgcn_readlane((int)ids, (n - begin) & 63); };
+    Quarter<HD> y;
+    if (begin < end) {
+        look(begin);
+        y.load(p.c, id(begin), head, wave);
+    }
+    for (int n = begin; n < end; n++) {
+        const int at = n * kPage;
+        const bool hidden = missing >> ((n - begin) & 63) & 1, edge = hidden || at < r.full_first || at + kPage - 1 > r.full_last;
+        fb8 *page = pages[n & 1];
+        if (edge) {
+            const int from = at + kBlock * (wave >> 1);
+            y.x.clear_v(r.first - from, hidden ? -1 : r.last - from);
+        }
+        y.store(page, wave);
+        if (n + 1 < end) {
+            if (((n - begin) & 63) == 63) look(n + 1);
+            y.load(p.c, id(n + 1), head, wave);
+        }
+        __syncthreads();
+#pragma unroll
+        for (int h = 0; h < 2; h++) {
+            auto key = [&](int t, int pt) { return page[((2 * h + pt) * G + t) * 64 + lane]; };
+            auto values = [&](int t, fb8(&b)[2]) { b[0] = page[(4 * G + 2 * G * h + 2 * t) * 64 + lane], b[1] = page[(4 * G + 2 * G * h + 2 * t + 1) * 64 + lane]; };
+            x.template take<false>(p.qscale, at + kBlock * h, edge, hidden, key, values, [] {});
+        }
+    }
 #pragma unroll
     for (int c = 0; c < CT; c++) {
         const float l = xsum<32>(xsum<16>(x.l[c])), inv = l == 0.f ? 0.f : 1.f / l;
-        if ((uint32_t)(16 * c + i) >= t.count) continue;
+        const uint32_t column = first + 16 * c + i;
+        if (column >= t.first + t.count) continue;
         float *out = p.splits > 1 ? p.part + (size_t)blockIdx.y * p.b.rows * p.heads * HD : p.out;
-        float *to = column_of(out, p, t.q, head, t.first + 16 * c + i, HD);
+        float *to = column_of(out, p, t.q, head, column, HD);
 #pragma unroll
         for (int d = 0; d < HD / 16; d++)
             *reinterpret_cast<float4 *>(to + 16 * d + 4 * g) = make_float4(x.o[c][d][0] * inv, x.o[c][d][1] * inv, x.o[c][d][2] * inv, x.o[c][d][3] * inv);
@@ -599,11 +696,11 @@ hipError_t launch_kv4_attention(const Kv4Attn &a, int cus, hipStream_t s) {
             }
         }
         if (most > p.few) {
-            const uint64_t n = std::min<uint64_t>(all / (16 * CT) + a.b.sequences, all), wgs = (n + 3) / 4 * nkv;
+            const uint64_t n = std::min<uint64_t>(all / (64 * CT) + a.b.sequences, all), wgs = n * nkv;
             const uint64_t each = (uint64_t)a.b.rows * a.heads * (HD + 2);
-            p.splits = (int)std::max<uint64_t>(1, std::min<uint64_t>({2 * (uint64_t)cus / wgs, blocks / 4, a.part_floats / each}));
+            p.splits = (int)std::max<uint64_t>(1, std::min<uint64_t>({2 * (uint64_t)cus / wgs, blocks / 8, a.part_floats / each}));
             p.part_ml = (float2 *)(p.part + (size_t)p.splits * a.b.rows * a.heads * HD);
-            hipLaunchKernelGGL((kv4_many_kernel<HD, CT, 2>), dim3((unsigned)wgs, (unsigned)p.splits), dim3(256), 0, s, p);
+            hipLaunchKernelGGL((kv4_many_kernel<HD, CT, 0>), dim3((unsigned)wgs, (unsigned)p.splits), dim3(256), 0, s, p);
             if (p.splits > 1) hipLaunchKernelGGL((kv4_many_join_kernel<HD>), dim3(a.b.rows), dim3(256), 0, s, p);
         }
     };

@@ -299,49 +299,55 @@ template <int HD, int CT, int AWAY> struct Columns {
         }
     }
 
-    // 32 positions from `at` on, key(t, pt) and values(t, b) their operands.  edge: some columns may not see all of them
-    // (hidden: their page is none).  after_k: the keys are through.
-    template <bool HOLD, class K, class V, class A>
-    __device__ __forceinline__ void take(float qscale, int at, bool edge, bool hidden, K key, V values, A after_k) {
+    // 32 H positions from `at` on, key(h, t, pt) and values(h, t, b) their operands.  edge: some columns may not see all of
+    // them (hidden: their page is none).  after_k, after_w: the keys are through, the scores are.
+    template <int H, bool HOLD, class K, class V, class A, class B>
+    __device__ __forceinline__ void take(float qscale, int at, bool edge, bool hidden, K key, V values, A after_k, B after_w) {
         const int g = threadIdx.x >> 4 & 3;
         int lane = threadIdx.x & 63;
         if constexpr (AWAY > 0) __asm__ volatile("" : "+v"(lane));  // (the pieces in LDS are read where they are used, not ahead of the loop)
-        ff4 s[CT][2];
+        ff4 s[H][CT][2];
 #pragma unroll
-        for (int c = 0; c < CT; c++) s[c][0] = s[c][1] = ff4{0.f, 0.f, 0.f, 0.f};
+        for (int h = 0; h < H; h++) {
 #pragma unroll
-        for (int t = 0; t < G; t++) {
-            fb8 a[2], far[CT][AWAY ? AWAY : 1];
+            for (int c = 0; c < CT; c++) s[h][c][0] = s[h][c][1] = ff4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-            for (int c = 0; c < CT; c++)
-#pragma unroll
-                for (int k = 0; k < AWAY; k++) far[c][k] = away[((c * G + t) * AWAY + k) * 64 + lane];
-            a[0] = key(t, 0), a[1] = key(t, 1);
-#pragma unroll
-            for (int k = 0; k < 3; k++)
+            for (int t = 0; t < G; t++) {
+                fb8 a[2], far[CT][AWAY ? AWAY : 1];
 #pragma unroll
                 for (int c = 0; c < CT; c++)
 #pragma unroll
-                    for (int pt = 0; pt < 2; pt++) s[c][pt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a[pt], k < NEAR ? q[c][t][k < NEAR ? k : 0] : far[c][k < NEAR ? 0 : k - NEAR], s[c][pt], 0, 0, 0);
-            if constexpr (HOLD) __builtin_amdgcn_sched_barrier(0);  // (or the operands of all steps take registers at once)
+                    for (int k = 0; k < AWAY; k++) far[c][k] = away[((c * G + t) * AWAY + k) * 64 + lane];
+                a[0] = key(h, t, 0), a[1] = key(h, t, 1);
+#pragma unroll
+                for (int k = 0; k < 3; k++)
+#pragma unroll
+                    for (int c = 0; c < CT; c++)
+#pragma unroll
+                        for (int pt = 0; pt < 2; pt++)
+                            s[h][c][pt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a[pt], k < NEAR ? q[c][t][k < NEAR ? k : 0] : far[c][k < NEAR ? 0 : k - NEAR], s[h][c][pt], 0, 0, 0);
+                if constexpr (HOLD) __builtin_amdgcn_sched_barrier(0);  // (or the operands of all steps take registers at once)
+            }
         }
         after_k();
         if (edge) {
 #pragma unroll
-            for (int c = 0; c < CT; c++)
+            for (int h = 0; h < H; h++)
 #pragma unroll
-                for (int e = 0; e < 8; e++) {
-                    const int pos = at + 8 * g + e;
-                    if (hidden || pos < lo[c] || pos > hi[c]) s[c][e >> 2][e & 3] = -INFINITY;
-                }
+                for (int c = 0; c < CT; c++)
+#pragma unroll
+                    for (int e = 0; e < 8; e++) {
+                        const int pos = at + kBlock * h + 8 * g + e;
+                        if (hidden || pos < lo[c] || pos > hi[c]) s[h][c][e >> 2][e & 3] = -INFINITY;
+                    }
         }
         float next[CT];
         bool grows = false;
 #pragma unroll
         for (int c = 0; c < CT; c++) {
-            float top = s[c][0][0];
+            float top = s[0][c][0][0];
 #pragma unroll
-            for (int e = 1; e < 8; e++) top = fmaxf(top, s[c][e >> 2][e & 3]);
+            for (int e = 1; e < 8 * H; e++) top = fmaxf(top, s[e >> 3][c][e >> 2 & 1][e & 3]);
             next[c] = fmaxf(m[c], xmax<32>(xmax<16>(top)) * qscale);
             grows = grows || next[c] > m[c] + kSlack;  // (-infinity: the first)
         }
@@ -355,27 +361,31 @@ template <int HD, int CT, int AWAY> struct Columns {
                 for (int d = 0; d < DT; d++) o[c][d] *= was;
             }
         }
-        fb8 w[CT][3];
 #pragma unroll
-        for (int c = 0; c < CT; c++) {
-            const float mf = finite(m[c]);
-            float v[8], sum = 0.f;
+        for (int h = 0; h < H; h++) {
+            fb8 w[CT][3];
 #pragma unroll
-            for (int e = 0; e < 8; e++) v[e] = __builtin_amdgcn_exp2f(fmaf(s[c][e >> 2][e & 3], qscale, -mf)), sum += v[e];
-            l[c] += sum;
-            pieces(v, w[c]);
-        }
+            for (int c = 0; c < CT; c++) {
+                const float mf = finite(m[c]);
+                float v[8], sum = 0.f;
 #pragma unroll
-        for (int t = 0; t < G; t++) {
-            fb8 b[2];
-            values(t, b);
+                for (int e = 0; e < 8; e++) v[e] = __builtin_amdgcn_exp2f(fmaf(s[h][c][e >> 2][e & 3], qscale, -mf)), sum += v[e];
+                l[c] += sum;
+                pieces(v, w[c]);
+            }
+            if (h == H - 1) after_w();
 #pragma unroll
-            for (int k = 0; k < 3; k++)
+            for (int t = 0; t < G; t++) {
+                fb8 b[2];
+                values(h, t, b);
 #pragma unroll
-                for (int c = 0; c < CT; c++)
+                for (int k = 0; k < 3; k++)
 #pragma unroll
-                    for (int h = 0; h < 2; h++) o[c][2 * t + h] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(b[h], w[c][k], o[c][2 * t + h], 0, 0, 0);
-            if constexpr (HOLD) __builtin_amdgcn_sched_barrier(0);
+                    for (int c = 0; c < CT; c++)
+#pragma unroll
+                        for (int d = 0; d < 2; d++) o[c][2 * t + d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(b[d], w[c][k], o[c][2 * t + d], 0, 0, 0);
+                if constexpr (HOLD) __builtin_amdgcn_sched_barrier(0);
+            }
         }
     }
 
@@ -411,8 +421,8 @@ template <int HD, int CT, int AWAY> struct Columns {
             const int j = min(i + 1, n - 1);  // (the last one's again, unused)
             const uint32_t next = page(j);
             x.clear_v(r.first - at(i), hidden ? -1 : r.last - at(i));
-            take<HOLD>(p.qscale, at(i), true, hidden, [&](int t, int pt) { return x.key(t, pt); }, [&](int t, fb8(&b)[2]) { x.values(t, b); },
-                             [&] { x.load_k(p.c, next, head, half(j)); });
+            take<1, HOLD>(p.qscale, at(i), true, hidden, [&](int, int t, int pt) { return x.key(t, pt); }, [&](int, int t, fb8(&b)[2]) { x.values(t, b); },
+                          [&] { x.load_k(p.c, next, head, half(j)); }, [] {});
             x.load_v(p.c, next, head, half(j));
             i++;
         };
@@ -421,8 +431,8 @@ template <int HD, int CT, int AWAY> struct Columns {
             const int j = min(i + 1, n - 1);
             const uint32_t next = page(j);
             if constexpr (DEEP) after.load_k(p.c, next, head, half(j)), after.load_v(p.c, next, head, half(j));
-            take<HOLD>(p.qscale, at(i), false, false, [&](int t, int pt) { return now.key(t, pt); }, [&](int t, fb8(&b)[2]) { now.values(t, b); },
-                              [&] { if constexpr (!DEEP) after.load_k(p.c, next, head, half(j)); });
+            take<1, HOLD>(p.qscale, at(i), false, false, [&](int, int t, int pt) { return now.key(t, pt); }, [&](int, int t, fb8(&b)[2]) { now.values(t, b); },
+                          [&] { if constexpr (!DEEP) after.load_k(p.c, next, head, half(j)); }, [] {});
             if constexpr (!DEEP) after.load_v(p.c, next, head, half(j));
             i++;
         };
@@ -613,17 +623,14 @@ template <int HD, int CT, int AWAY> __global__ void __launch_bounds__(256, 2) kv
             y.x.clear_v(r.first - from, hidden ? -1 : r.last - from);
         }
         y.store(page, wave);
-        if (n + 1 < end) {
-            if (((n - begin) & 63) == 63) look(n + 1);
-            y.load(p.c, id(n + 1), head, wave);
-        }
+        if (n + 1 < end && ((n - begin) & 63) == 63) look(n + 1);
         __syncthreads();
-#pragma unroll
-        for (int h = 0; h < 2; h++) {
-            auto key = [&](int t, int pt) { return page[((2 * h + pt) * G + t) * 64 + lane]; };
-            auto values = [&](int t, fb8(&b)[2]) { b[0] = page[(4 * G + 2 * G * h + 2 * t) * 64 + lane], b[1] = page[(4 * G + 2 * G * h + 2 * t + 1) * 64 + lane]; };
-            x.template take<false>(p.qscale, at + kBlock * h, edge, hidden, key, values, [] {});
-        }
+        x.template take<2, false>(p.qscale, at, edge, hidden, [&](int h, int t, int pt) { return page[((2 * h + pt) * G + t) * 64 + lane]; },
+                                  [&](int h, int t, fb8(&b)[2]) {
+                                      const fb8 *v = page + (4 * G + 2 * G * h + 2 * t) * 64 + lane;
+                                      b[0] = v[0], b[1] = v[64];
+                                  },
+                                  [] {}, [&] { y.load(p.c, id(min(n + 1, end - 1)), head, wave); });
     }
 #pragma unroll
     for (int c = 0; c < CT; c++) {

@@ -111,50 +111,57 @@ template <int COLUMNS> __device__ __forceinline__ Tile tile_of(const Kv4Params &
     return t;
 }
 
-// How the few-column kernel spreads a batch: each sequence's blocks of 32 positions, times the kv heads, over p.wgs
-// workgroups, `quota` blocks each at most.  A sequence's blocks are split evenly; its items follow each other, the kv
-// heads side by side.  Splits that are to be joined have slots in the workspace, at most 2 p.wgs of them: a sequence has
-// two splits only where it has more than a quota.
+// How the few-column kernel spreads a batch: each sequence's tiles of columns, times the kv heads, go through the
+// sequence's blocks of 32 positions; together they are spread over p.wgs workgroups, `quota` blocks each at most.  A
+// tile's blocks are split evenly; its items follow each other, the kv heads side by side.  Splits that are to be joined
+// have slots in the workspace, at most 2 p.wgs of them: a tile has two splits only where it has more than a quota.
 struct Share {
     Sequence q;
-    Range r;            // of the whole sequence
-    uint32_t splits;    // 0: none
-    uint32_t index;     // item: within the sequence's
-    uint32_t slot;      // of the sequence's first split
+    uint32_t splits, tiles; // 0: none
+    uint32_t index;         // item: within the sequence's
+    uint32_t slot;          // of the sequence's first split
 };
-constexpr uint32_t kLeastBlocks = 4;  // one for each wavefront
+constexpr uint32_t kFewWaves = 4, kLeastBlocks = kFewWaves;  // of a workgroup: one for each wavefront
 
 // The item with this number, or (by_sequence) the sequence.  Every lane of a wavefront takes part.
-template <bool BY_SEQUENCE> __device__ __forceinline__ Share share_of(const Kv4Params &p, uint32_t number) {
+template <bool BY_SEQUENCE, int COLUMNS> __device__ __forceinline__ Share share_of(const Kv4Params &p, uint32_t number) {
     const uint32_t lane = threadIdx.x & 63, nkv = (uint32_t)p.c.nkv;
-    auto blocks = [&](uint32_t s) -> uint32_t {
-        if (s >= p.b.sequences) return 0u;
-        const Sequence q = sequence_of(p.b, s);
-        if (q.rows == 0 || q.rows * p.group > p.few) return 0u;
+    // this lane's sequence, its tiles and blocks (of all columns: a tile's own are no more)
+    Sequence q{};
+    uint32_t tiles = 0, blocks = 0;
+    auto look = [&](uint32_t s) {
+        q.rows = tiles = blocks = 0;
+        if (s >= p.b.sequences) return;
+        q = sequence_of(p.b, s);
+        const uint32_t columns = q.rows * p.group;
+        if (columns == 0 || columns > p.few) return;
         const Range r = range_of(p, q, 0, q.rows - 1);
-        return max((uint32_t)(r.end - r.begin), 1u);  // rows that see nothing have an item, which writes zeros
+        tiles = (columns + COLUMNS - 1) / COLUMNS;
+        blocks = max((uint32_t)(r.end - r.begin), 1u);  // rows that see nothing have an item, which writes zeros
     };
-    uint32_t own = blocks(lane);
-    u64 total = own;
-    for (uint32_t from = 64; from < p.b.sequences; from += 64) total += blocks(from + lane);
+    look(lane);
+    u64 total = (u64)blocks * tiles;
+    for (uint32_t from = 64; from < p.b.sequences; from += 64) look(from + lane), total += (u64)blocks * tiles;
+    if (p.b.sequences > 64) look(lane);
     for (int d = 1; d < 64; d <<= 1) total += __shfl_xor(total, d);
     const uint32_t quota = uniform(max(kLeastBlocks, (uint32_t)ceil((double)total * nkv / p.wgs)));
     Share t{};
     uint32_t items = 0, slots = 0;
     for (uint32_t from = 0; from < p.b.sequences; from += 64) {
-        const uint32_t n = from ? blocks(from + lane) : own, splits = (n + quota - 1) / quota;
-        const uint32_t sum = running_sum(splits * nkv), slot_sum = running_sum(splits > 1 ? splits * nkv : 0u);
+        if (from) look(from + lane);
+        const uint32_t splits = (blocks + quota - 1) / quota, n = splits * tiles * nkv;
+        const uint32_t sum = running_sum(n), slot_sum = running_sum(splits > 1 ? n : 0u);
         const u64 past = __ballot(BY_SEQUENCE ? from + lane == number : items + sum > number);
+        auto of = [&](uint32_t v, int at) { return (uint32_t)__builtin_amdgcn_readlane((int)v, at); };
         if (past) {
             const int at = __ffsll(past) - 1;
-            t.q = uniform(sequence_of(p.b, from + at));
-            t.splits = (uint32_t)__builtin_amdgcn_readlane((int)splits, at);
-            if (t.splits) t.r = range_of(p, t.q, 0, t.q.rows - 1);
-            t.index = number - items - (uint32_t)__builtin_amdgcn_readlane((int)(sum - splits * nkv), at);
-            t.slot = slots + (uint32_t)__builtin_amdgcn_readlane((int)slot_sum, at) - (t.splits > 1 ? t.splits * nkv : 0u);
+            t.q = {of(q.index, at), of(q.row0, at), of(q.rows, at), (int)of((uint32_t)q.first, at)};
+            t.splits = of(splits, at), t.tiles = of(tiles, at);
+            t.index = number - items - of(sum - n, at);
+            t.slot = slots + of(slot_sum, at) - (t.splits > 1 ? t.splits * t.tiles * nkv : 0u);
             return t;
         }
-        items += (uint32_t)__builtin_amdgcn_readlane((int)sum, 63), slots += (uint32_t)__builtin_amdgcn_readlane((int)slot_sum, 63);
+        items += of(sum, 63), slots += of(slot_sum, 63);
     }
     return t;
 }
@@ -436,13 +443,19 @@ template <int HD, int CT, int AWAY> struct Columns {
             if constexpr (!DEEP) after.load_v(p.c, next, head, half(j));
             i++;
         };
+        auto both = [&](Lane4<HD> &now, Lane4<HD> &after) {
+            const bool hidden = missing >> (i & 63) & 1, edge = !inner(i);
+            if ((i & 63) == 63) look(begin + step * (i + 1));
+            const int j = min(i + 1, n - 1);
+            const uint32_t next = page(j);
+            after.load_k(p.c, next, head, half(j)), after.load_v(p.c, next, head, half(j));
+            if (edge) now.clear_v(r.first - at(i), hidden ? -1 : r.last - at(i));
+            take<1, HOLD>(p.qscale, at(i), edge, hidden, [&](int, int t, int pt) { return now.key(t, pt); }, [&](int, int t, fb8(&b)[2]) { now.values(t, b); }, [] {}, [] {});
+            i++;
+        };
         while (i < n) {
-            while (i < n && !inner(i)) edge_block();
-            while (i + 1 < n && inner(i) && (((i & 63) != 63) && inner(i + 1))) {
-                if constexpr (DEEP) inner_block(x, y), inner_block(y, x);
-                else inner_block(x, x), inner_block(x, x);
-            }
-            if (i < n && inner(i)) edge_block();  // (one left of a pair: nothing is hidden of it)
+            both(x, y);
+            if (i < n) both(y, x);
         }
     }
 };
@@ -453,22 +466,24 @@ __device__ __forceinline__ float *column_of(float *out, const Kv4Params &p, cons
 }
 
 // Few columns (decoding): a workgroup takes an item, its wavefronts blocks in turn, joined in LDS.
-template <int HD, int CT> __global__ void __launch_bounds__(256, 2) kv4_few_kernel(Kv4Params p) {
-    constexpr int N = 16 * CT, C = HD / 4, AWAY = HD * CT > 128 ? 2 : 0, PIECES = 4 * CT * (HD / 32) * AWAY * 64;  // (their 16 bytes)
+template <int HD, int CT> __global__ void __launch_bounds__(64 * kFewWaves, 2) kv4_few_kernel(Kv4Params p) {
+    constexpr int N = 16 * CT, C = HD / 4, AWAY = HD * CT > 128 ? 2 : 0, PIECES = CT * (HD / 32) * AWAY * 64;  // of a wavefront (16 bytes each)
+    constexpr int OUTPUTS = kFewWaves * N * (HD + 4), HELD = kFewWaves * PIECES * 4;
     // the queries' pieces, then the wavefronts' outputs
-    __shared__ __align__(16) float lds[4 * N * (HD + 4) > 4 * PIECES ? 4 * N * (HD + 4) : 4 * PIECES];
-    __shared__ float ms[4][N], ls[4][N];
+    __shared__ __align__(16) float lds[OUTPUTS > HELD ? OUTPUTS : HELD];
+    __shared__ float ms[kFewWaves][N], ls[kFewWaves][N];
     float(*os)[N][HD + 4] = reinterpret_cast<float(*)[N][HD + 4]>(lds);
     const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), i = tid & 15, g = tid >> 4 & 3;
-    const Share t = share_of<false>(p, blockIdx.x);
+    const Share t = share_of<false, N>(p, blockIdx.x);
     if (t.splits == 0) return;
     const int head = (int)(t.index % p.c.nkv);
-    const uint32_t z = t.index / p.c.nkv, count = t.q.rows * p.group;
-    int begin = t.r.begin, end = t.r.end;
+    const uint32_t z = t.index / p.c.nkv % t.splits, first = t.index / p.c.nkv / t.splits * N, count = min(t.q.rows * p.group - first, (uint32_t)N);
+    const Range r = range_of(p, t.q, first / p.group, (first + count - 1) / p.group);
+    int begin = r.begin, end = r.end;
     share(begin, end, t.splits, z);
     Columns<HD, CT, AWAY> x;
-    x.begin(p, t.q, 0, count, head, reinterpret_cast<fb8 *>(lds) + wave * (PIECES / 4));
-    x.template run<HD * CT <= 128, (HD * CT > 128)>(p, t.r, t.q.index, head, begin + wave, end, 4);
+    x.begin(p, t.q, first, count, head, reinterpret_cast<fb8 *>(lds) + wave * PIECES);
+    x.template run<HD * CT <= 128, (HD * CT > 128)>(p, r, t.q.index, head, begin + wave, end, kFewWaves);
     if (AWAY) __syncthreads();
 #pragma unroll
     for (int c = 0; c < CT; c++) {
@@ -480,66 +495,83 @@ template <int HD, int CT> __global__ void __launch_bounds__(256, 2) kv4_few_kern
             *reinterpret_cast<float4 *>(&os[wave][16 * c + i][16 * d + 4 * g]) = make_float4(x.o[c][d][0], x.o[c][d][1], x.o[c][d][2], x.o[c][d][3]);
     }
     __syncthreads();
-    for (uint32_t u = tid; u < count * C; u += 256) {
+    for (uint32_t u = tid; u < count * C; u += 64 * kFewWaves) {
         const uint32_t column = u / C;
         const int d = 4 * (int)(u % C);
-        const float m = fmaxf(fmaxf(ms[0][column], ms[1][column]), fmaxf(ms[2][column], ms[3][column])), mf = finite(m);
+        float m = ms[0][column];
+#pragma unroll
+        for (int w = 1; w < (int)kFewWaves; w++) m = fmaxf(m, ms[w][column]);
+        const float mf = finite(m);
         float l = 0.f;
         float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-        for (int w = 0; w < 4; w++) {
+        for (int w = 0; w < (int)kFewWaves; w++) {
             const float f = __builtin_amdgcn_exp2f(ms[w][column] - mf);
             const float4 v = *reinterpret_cast<const float4 *>(&os[w][column][d]);
             l = fmaf(f, ls[w][column], l);
             o.x = fmaf(f, v.x, o.x), o.y = fmaf(f, v.y, o.y), o.z = fmaf(f, v.z, o.z), o.w = fmaf(f, v.w, o.w);
         }
         if (t.splits > 1) {
-            const size_t at = ((size_t)t.slot + z * p.c.nkv + head) * N + column;
+            const size_t at = ((size_t)t.slot + t.index) * N + column;
             *reinterpret_cast<float4 *>(p.part + at * HD + d) = o;
             if (d == 0) p.part_ml[at] = make_float2(m, l);
         } else {
             const float inv = l == 0.f ? 0.f : 1.f / l;  // (rows that see nothing: zeros)
-            *reinterpret_cast<float4 *>(column_of(p.out, p, t.q, head, column, HD) + d) = make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv);
+            *reinterpret_cast<float4 *>(column_of(p.out, p, t.q, head, first + column, HD) + d) = make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv);
         }
     }
 }
 
-// Joins the splits of a sequence's kv head, a column at a time: a float4 of every N-th split a thread.
+// Joins the splits of a sequence's kv head, a column at a time: a float4 of every N-th split a thread, four under way.
 template <int HD, int CT> __global__ void __launch_bounds__(256) kv4_few_join_kernel(Kv4Params p) {
-    constexpr int C = HD / 4, N = 256 / C;
+    constexpr int C = HD / 4, N = 256 / C, Z = 4;
     __shared__ float4 os[N][C];
-    __shared__ float ls[N], ms[4];
-    const Share t = share_of<true>(p, blockIdx.x / p.c.nkv);
+    __shared__ float ls[N], ms[N];
+    const Share t = share_of<true, 16 * CT>(p, blockIdx.x / p.c.nkv);
     if (t.splits < 2) return;
     const int head = (int)(blockIdx.x % p.c.nkv), tid = threadIdx.x, c = tid % C, n = tid / C;
     const uint32_t count = t.q.rows * p.group;
     for (uint32_t column = blockIdx.y; column < count; column += gridDim.y) {
-        auto at = [&](uint32_t z) { return ((size_t)t.slot + z * p.c.nkv + head) * (16 * CT) + column; };
-        float m = -INFINITY;
-        for (uint32_t z = tid; z < t.splits; z += 256) m = fmaxf(m, p.part_ml[at(z)].x);
-        m = wave_max_f32(m);
-        if ((tid & 63) == 0) ms[tid >> 6] = m;
-        __syncthreads();
-        m = finite(fmaxf(fmaxf(ms[0], ms[1]), fmaxf(ms[2], ms[3])));
+        const uint32_t tile = column / (16 * CT), within = column - tile * (16 * CT);
+        auto at = [&](uint32_t z) { return ((size_t)t.slot + (tile * t.splits + min(z, t.splits - 1)) * p.c.nkv + head) * (16 * CT) + within; };
         float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-        float l = 0.f;
+        float m = -INFINITY, l = 0.f;
         if (n < N)
-            for (uint32_t z = n; z < t.splits; z += N) {
-                const float2 ml = p.part_ml[at(z)];
-                const float4 v = *reinterpret_cast<const float4 *>(p.part + at(z) * HD + 4 * c);
-                const float f = __builtin_amdgcn_exp2f(ml.x - m);
-                l = fmaf(f, ml.y, l);
-                o.x = fmaf(f, v.x, o.x), o.y = fmaf(f, v.y, o.y), o.z = fmaf(f, v.z, o.z), o.w = fmaf(f, v.w, o.w);
+            for (uint32_t z = n; z < t.splits; z += N * Z) {
+                float2 ml[Z];
+                float4 v[Z];
+                float top = m;
+#pragma unroll
+                for (int e = 0; e < Z; e++) {
+                    ml[e] = p.part_ml[at(z + e * N)];
+                    v[e] = *reinterpret_cast<const float4 *>(p.part + at(z + e * N) * HD + 4 * c);
+                }
+#pragma unroll
+                for (int e = 0; e < Z; e++) top = fmaxf(top, ml[e].x);
+                const float mf = finite(top), was = __builtin_amdgcn_exp2f(m - mf);
+                m = top;
+                l *= was, o.x *= was, o.y *= was, o.z *= was, o.w *= was;
+#pragma unroll
+                for (int e = 0; e < Z; e++) {
+                    const float f = z + e * N < t.splits ? __builtin_amdgcn_exp2f(ml[e].x - mf) : 0.f;
+                    l = fmaf(f, ml[e].y, l);
+                    o.x = fmaf(f, v[e].x, o.x), o.y = fmaf(f, v[e].y, o.y), o.z = fmaf(f, v[e].z, o.z), o.w = fmaf(f, v[e].w, o.w);
+                }
             }
         if (n < N) {
             os[n][c] = o;
-            if (c == 0) ls[n] = l;
+            if (c == 0) ls[n] = l, ms[n] = m;
         }
         __syncthreads();
         if (n == 0) {
-            for (int k = 1; k < N; k++) {
+            for (int k = 1; k < N; k++) m = fmaxf(m, ms[k]);
+            const float mf = finite(m);
+            o = make_float4(0.f, 0.f, 0.f, 0.f), l = 0.f;
+            for (int k = 0; k < N; k++) {
+                const float f = __builtin_amdgcn_exp2f(ms[k] - mf);
                 const float4 v = os[k][c];
-                o.x += v.x, o.y += v.y, o.z += v.z, o.w += v.w, l += ls[k];
+                l = fmaf(f, ls[k], l);
+                o.x = fmaf(f, v.x, o.x), o.y = fmaf(f, v.y, o.y), o.z = fmaf(f, v.z, o.z), o.w = fmaf(f, v.w, o.w);
             }
             const float inv = l == 0.f ? 0.f : 1.f / l;
             *reinterpret_cast<float4 *>(column_of(p.out, p, t.q, head, column, HD) + 4 * c) = make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv);
@@ -650,7 +682,8 @@ template <int HD, int CT, int AWAY> __global__ void __launch_bounds__(256, 2) kv
 template <int HD> __global__ void __launch_bounds__(256) kv4_many_join_kernel(Kv4Params p) {
     const Sequence q = sequence_of_row(p.b, blockIdx.x);
     if (q.rows * p.group <= p.few) return;  // (none's, or the other kernel's)
-    for (uint32_t u = threadIdx.x; u < (uint32_t)p.heads * (HD / 4); u += 256) {
+    const uint32_t u = blockIdx.y * 256 + threadIdx.x;
+    if (u < (uint32_t)p.heads * (HD / 4)) {
         const size_t at = (size_t)blockIdx.x * p.heads + u / (HD / 4), each = (size_t)p.b.rows * p.heads;
         const int d = 4 * (int)(u % (HD / 4));
         float m = -INFINITY, l = 0.f;
@@ -678,45 +711,45 @@ hipError_t launch_kv4_attention(const Kv4Attn &a, int cus, hipStream_t s) {
     p.window = a.window, p.qscale = a.qscale, p.qsign = a.qsign;
     p.part = a.part;
     const uint64_t nkv = a.c.nkv, most = (uint64_t)a.b.max_rows * p.group, all = (uint64_t)a.b.rows * p.group;
-    const int ct = a.c.hd <= 128 ? 2 : 1;                     // column tiles that a wavefront's registers hold
-    const uint32_t limit = 16u * ct;
     const uint64_t blocks = (a.b.cap + kBlock - 1) / kBlock;  // of a sequence, at most
+    const uint32_t limit = a.c.hd <= 128 ? 64 : 32;
     // a batch of one sequence is one kernel's; others may hold sequences of both kinds
     p.few = a.b.sequences == 1 && most > limit ? 0 : limit;
-    auto go = [&](auto h, auto tiles) {
+    auto few = [&](auto h, auto tiles) {
         constexpr int HD = decltype(h)::value, CT = decltype(tiles)::value;
-        if (p.few) {
-            p.wgs = 2 * cus;
-            const size_t slot = (size_t)limit * (HD + 2);  // floats
-            while (p.wgs > 1 && 2 * p.wgs * slot > a.part_floats) p.wgs /= 2;
-            p.part_ml = (float2 *)(p.part + (size_t)2 * p.wgs * limit * HD);
-            const uint64_t per = (blocks + kLeastBlocks - 1) / kLeastBlocks;  // splits of a sequence, at most
-            const uint64_t items = std::min(p.wgs + a.b.sequences * nkv, a.b.sequences * nkv * per);
-            const bool split = per > 1;
-            const dim3 join((unsigned)(a.b.sequences * nkv), (unsigned)std::min<uint64_t>(std::min<uint64_t>(most, limit), std::max<uint64_t>(1, 1024 / (a.b.sequences * nkv))));
-            if (most <= 16) {
-                hipLaunchKernelGGL((kv4_few_kernel<HD, 1>), dim3((unsigned)items), dim3(256), 0, s, p);
-                if (split) hipLaunchKernelGGL((kv4_few_join_kernel<HD, 1>), join, dim3(256), 0, s, p);
-            } else {
-                hipLaunchKernelGGL((kv4_few_kernel<HD, CT>), dim3((unsigned)items), dim3(256), 0, s, p);
-                if (split) hipLaunchKernelGGL((kv4_few_join_kernel<HD, CT>), join, dim3(256), 0, s, p);
-            }
-        }
-        if (most > p.few) {
-            const uint64_t n = std::min<uint64_t>(all / (64 * CT) + a.b.sequences, all), wgs = n * nkv;
-            const uint64_t each = (uint64_t)a.b.rows * a.heads * (HD + 2);
-            p.splits = (int)std::max<uint64_t>(1, std::min<uint64_t>({2 * (uint64_t)cus / wgs, blocks / 8, a.part_floats / each}));
-            p.part_ml = (float2 *)(p.part + (size_t)p.splits * a.b.rows * a.heads * HD);
-            hipLaunchKernelGGL((kv4_many_kernel<HD, CT, 0>), dim3((unsigned)wgs, (unsigned)p.splits), dim3(256), 0, s, p);
-            if (p.splits > 1) hipLaunchKernelGGL((kv4_many_join_kernel<HD>), dim3(a.b.rows), dim3(256), 0, s, p);
-        }
+        constexpr uint64_t N = 16 * CT;
+        p.wgs = 2 * cus;
+        while (p.wgs > 1 && 2 * p.wgs * N * (HD + 2) > a.part_floats) p.wgs /= 2;
+        p.part_ml = (float2 *)(p.part + (size_t)2 * p.wgs * N * HD);
+        const uint64_t columns = std::min<uint64_t>(most, limit), tiles_of = (columns + N - 1) / N;
+        const uint64_t per = (blocks + kLeastBlocks - 1) / kLeastBlocks, all_tiles = a.b.sequences * nkv * tiles_of;  // splits of a tile, and tiles, at most
+        const uint64_t items = std::min(p.wgs + all_tiles, all_tiles * per);
+        hipLaunchKernelGGL((kv4_few_kernel<HD, CT>), dim3((unsigned)items), dim3(64 * kFewWaves), 0, s, p);
+        if (per == 1) return;
+        const dim3 join((unsigned)(a.b.sequences * nkv), (unsigned)std::min<uint64_t>(columns, std::max<uint64_t>(1, 1024 / (a.b.sequences * nkv))));
+        hipLaunchKernelGGL((kv4_few_join_kernel<HD, CT>), join, dim3(256), 0, s, p);
     };
-    if (a.b.sequences * nkv * 2 > 0x7FFFFFFFu || (all / 16 + a.b.sequences + 4) * nkv > 0x7FFFFFFFu) return hipErrorInvalidValue;
+    auto many = [&](auto h, auto tiles) {
+        constexpr int HD = decltype(h)::value, CT = decltype(tiles)::value;
+        const uint64_t n = std::min<uint64_t>(all / (64 * CT) + a.b.sequences, all), wgs = n * nkv;
+        const uint64_t each = (uint64_t)a.b.rows * a.heads * (HD + 2);
+        p.splits = (int)std::max<uint64_t>(1, std::min<uint64_t>({2 * (uint64_t)cus / wgs, blocks / 8, a.part_floats / each}));
+        p.part_ml = (float2 *)(p.part + (size_t)p.splits * a.b.rows * a.heads * HD);
+        hipLaunchKernelGGL((kv4_many_kernel<HD, CT, 0>), dim3((unsigned)wgs, (unsigned)p.splits), dim3(256), 0, s, p);
+        if (p.splits > 1)
+            hipLaunchKernelGGL((kv4_many_join_kernel<HD>), dim3(a.b.rows, (a.heads * (HD / 4) + 255) / 256), dim3(256), 0, s, p);
+    };
+    auto go = [&](auto h, auto one, auto more, auto prompt) {
+        if (p.few && most <= 16 * decltype(one)::value) few(h, one);
+        else if (p.few) few(h, more);
+        if (most > p.few) many(h, prompt);
+    };
+    if (a.b.sequences * nkv * 8 > 0x7FFFFFFFu || (all / 16 + a.b.sequences + 4) * nkv > 0x7FFFFFFFu) return hipErrorInvalidValue;
     switch (a.c.hd) {
-    case 64: go(std::integral_constant<int, 64>{}, std::integral_constant<int, 2>{}); break;
-    case 96: go(std::integral_constant<int, 96>{}, std::integral_constant<int, 2>{}); break;
-    case 128: go(std::integral_constant<int, 128>{}, std::integral_constant<int, 2>{}); break;
-    case 256: go(std::integral_constant<int, 256>{}, std::integral_constant<int, 1>{}); break;
+    case 64: go(std::integral_constant<int, 64>{}, std::integral_constant<int, 1>{}, std::integral_constant<int, 4>{}, std::integral_constant<int, 2>{}); break;
+    case 96: go(std::integral_constant<int, 96>{}, std::integral_constant<int, 1>{}, std::integral_constant<int, 2>{}, std::integral_constant<int, 2>{}); break;
+    case 128: go(std::integral_constant<int, 128>{}, std::integral_constant<int, 1>{}, std::integral_constant<int, 2>{}, std::integral_constant<int, 2>{}); break;
+    case 256: go(std::integral_constant<int, 256>{}, std::integral_constant<int, 1>{}, std::integral_constant<int, 1>{}, std::integral_constant<int, 1>{}); break;
     default: return hipErrorInvalidValue;
     }
     return hipGetLastError();

@@ -72,16 +72,6 @@ __device__ __forceinline__ Sequence uniform(const Sequence &q) {
     return {uniform(q.index), uniform(q.row0), uniform(q.rows), (int)uniform((uint32_t)q.first)};
 }
 
-// inclusive sum over a wavefront's lanes
-__device__ __forceinline__ uint32_t running_sum(uint32_t n) {
-    const int lane = threadIdx.x & 63;
-    for (int d = 1; d < 64; d <<= 1) {
-        const uint32_t o = (uint32_t)__shfl_up((int)n, d);
-        if (lane >= d) n += o;
-    }
-    return n;
-}
-
 // A tile of columns (a sequence's rows' heads of one kv head, row by row), by its number among those of the sequences
 // with more than `few` columns; count 0: none.  Every lane of a wavefront takes part.
 struct Tile {
@@ -126,6 +116,7 @@ constexpr uint32_t kFewWaves = 4, kLeastBlocks = kFewWaves;  // of a workgroup: 
 // The item with this number, or (by_sequence) the sequence.  Every lane of a wavefront takes part.
 template <bool BY_SEQUENCE, int COLUMNS> __device__ __forceinline__ Share share_of(const Kv4Params &p, uint32_t number) {
     const uint32_t lane = threadIdx.x & 63, nkv = (uint32_t)p.c.nkv;
+    auto of = [](uint32_t v, int at) { return (uint32_t)__builtin_amdgcn_readlane((int)v, at); };
     // this lane's sequence, its tiles and blocks (of all columns: a tile's own are no more)
     Sequence q{};
     uint32_t tiles = 0, blocks = 0;
@@ -143,7 +134,8 @@ template <bool BY_SEQUENCE, int COLUMNS> __device__ __forceinline__ Share share_
     u64 total = (u64)blocks * tiles;
     for (uint32_t from = 64; from < p.b.sequences; from += 64) look(from + lane), total += (u64)blocks * tiles;
     if (p.b.sequences > 64) look(lane);
-    for (int d = 1; d < 64; d <<= 1) total += __shfl_xor(total, d);
+    total = running_sum(total);
+    total = (u64)of((uint32_t)(total >> 32), 63) << 32 | of((uint32_t)total, 63);
     const uint32_t quota = uniform(max(kLeastBlocks, (uint32_t)ceil((double)total * nkv / p.wgs)));
     Share t{};
     uint32_t items = 0, slots = 0;
@@ -152,7 +144,6 @@ template <bool BY_SEQUENCE, int COLUMNS> __device__ __forceinline__ Share share_
         const uint32_t splits = (blocks + quota - 1) / quota, n = splits * tiles * nkv;
         const uint32_t sum = running_sum(n), slot_sum = running_sum(splits > 1 ? n : 0u);
         const u64 past = __ballot(BY_SEQUENCE ? from + lane == number : items + sum > number);
-        auto of = [&](uint32_t v, int at) { return (uint32_t)__builtin_amdgcn_readlane((int)v, at); };
         if (past) {
             const int at = __ffsll(past) - 1;
             t.q = {of(q.index, at), of(q.row0, at), of(q.rows, at), (int)of((uint32_t)q.first, at)};
@@ -190,9 +181,16 @@ __device__ __forceinline__ void pieces(const float (&v)[8], fb8 (&to)[3]) {
 template <int SEL> __device__ __forceinline__ uint32_t widen(uint32_t w, float scale) {
     return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, scale, SEL));
 }
-__device__ __forceinline__ float scale_of(uint32_t w, int byte) { return __uint_as_float((w >> (8 * byte) & 255u) << 23); }
+// 2^(byte - 127) as far as the conversion looks: it takes the scale's exponent alone, whatever sign and fraction are
+// (every byte with 256 of them: the same), so a shift brings the byte there and nothing is masked.
+__device__ __forceinline__ float scale_of(uint32_t w, int byte) { return __uint_as_float(byte < 3 ? w << (23 - 8 * byte) : w >> 1); }
 
 __device__ __forceinline__ float finite(float v) { return v == -INFINITY ? 0.f : v; }
+// the sum over four lanes side by side
+__device__ __forceinline__ float four(float v) {
+    v += __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), 0xB1, 0xF, 0xF, false));
+    return v + __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), 0x4E, 0xF, 0xF, false));
+}
 
 // A lane's part of 32 positions: lane (i, g) holds K rows 8 (i / 4) + 4 pt + i % 4 of both halves pt (its words g of
 // every 32 dims), and V's dims 32 t + i and 32 t + 16 + i of positions 8 g .. 8 g + 7.
@@ -260,8 +258,11 @@ template <int HD> struct Lane4 {
 // One wavefront's columns: their queries, running maxima and sums, and outputs.  Scores S^T[position][column] = K Q^T on
 // 16x16x32 products, outputs O^T[dim][column] = V^T P^T: what a lane gets of S^T, positions 8 g .. 8 g + 7 of column i,
 // is what it gives of P^T.
-template <int HD, int CT, int AWAY> struct Columns {
-    static constexpr int G = HD / 32, DT = HD / 16, NEAR = 3 - AWAY;
+// PACKED (CT 1): four columns at most, whose three pieces, and a fourth of zeros, are sixteen: lane i holds piece i % 4 of
+// column i / 4, so that a product of all pieces is one instead of three.  Scores of the pieces add up across four lanes,
+// outputs once at the end.
+template <int HD, int CT, int AWAY, bool PACKED = false> struct Columns {
+    static constexpr int G = HD / 32, DT = HD / 16, P = PACKED ? 1 : 3, NEAR = P - AWAY;
     fb8 q[CT][G][NEAR];
     const fb8 *away;  // the queries' other pieces, [CT][G][AWAY][64] in LDS
     ff4 o[CT][DT];
@@ -274,7 +275,7 @@ template <int HD, int CT, int AWAY> struct Columns {
         const int i = threadIdx.x & 15, g = threadIdx.x >> 4 & 3;
 #pragma unroll
         for (int c = 0; c < CT; c++) {
-            const uint32_t column = first + min((uint32_t)(16 * c + i), count - 1), row = column / p.group;
+            const uint32_t column = first + min((uint32_t)(PACKED ? i >> 2 : 16 * c + i), count - 1), row = column / p.group;
             const float *src = p.q + (size_t)(t.row0 + row) * p.q_stride + (size_t)(head * p.group + (int)(column - row * p.group)) * HD;
             hi[c] = t.first + (int)row;
             lo[c] = first_seen(hi[c], p.window);
@@ -294,8 +295,12 @@ template <int HD, int CT, int AWAY> struct Columns {
                 for (int e = 0; e < 8; e++) v[e] *= p.qsign;
                 fb8 all[3];
                 pieces(v, all);
+                if constexpr (PACKED) {
+                    const fb8 none = {};
+                    all[0] = i & 2 ? (i & 1 ? none : all[2]) : i & 1 ? all[1] : all[0];
+                }
 #pragma unroll
-                for (int e = 0; e < 3; e++) {
+                for (int e = 0; e < P; e++) {
                     if (e < NEAR) q[c][k][e] = all[e];
                     else lds[((c * G + k) * AWAY + e - NEAR) * 64 + (threadIdx.x & 63)] = all[e];
                 }
@@ -311,6 +316,8 @@ template <int HD, int CT, int AWAY> struct Columns {
     template <int H, bool HOLD, class K, class V, class A, class B>
     __device__ __forceinline__ void take(float qscale, int at, bool edge, bool hidden, K key, V values, A after_k, B after_w) {
         const int g = threadIdx.x >> 4 & 3;
+        // of a weight, lane i % 4 = 1 takes off the first piece, 2 the second too; 3 (whose weights nothing reads) as 2
+        const float second = PACKED && (threadIdx.x & 3) > 0 ? -1.f : 0.f, third = PACKED && (threadIdx.x & 3) > 1 ? -1.f : 0.f;
         int lane = threadIdx.x & 63;
         if constexpr (AWAY > 0) __asm__ volatile("" : "+v"(lane));  // (the pieces in LDS are read where they are used, not ahead of the loop)
         ff4 s[H][CT][2];
@@ -327,7 +334,7 @@ template <int HD, int CT, int AWAY> struct Columns {
                     for (int k = 0; k < AWAY; k++) far[c][k] = away[((c * G + t) * AWAY + k) * 64 + lane];
                 a[0] = key(h, t, 0), a[1] = key(h, t, 1);
 #pragma unroll
-                for (int k = 0; k < 3; k++)
+                for (int k = 0; k < P; k++)
 #pragma unroll
                     for (int c = 0; c < CT; c++)
 #pragma unroll
@@ -337,6 +344,12 @@ template <int HD, int CT, int AWAY> struct Columns {
             }
         }
         after_k();
+        if constexpr (PACKED) {
+#pragma unroll
+            for (int h = 0; h < H; h++)
+#pragma unroll
+                for (int e = 0; e < 8; e++) s[h][0][e >> 2][e & 3] = four(s[h][0][e >> 2][e & 3]);
+        }
         if (edge) {
 #pragma unroll
             for (int h = 0; h < H; h++)
@@ -370,7 +383,7 @@ template <int HD, int CT, int AWAY> struct Columns {
         }
 #pragma unroll
         for (int h = 0; h < H; h++) {
-            fb8 w[CT][3];
+            fb8 w[CT][P];
 #pragma unroll
             for (int c = 0; c < CT; c++) {
                 const float mf = finite(m[c]);
@@ -378,7 +391,19 @@ template <int HD, int CT, int AWAY> struct Columns {
 #pragma unroll
                 for (int e = 0; e < 8; e++) v[e] = __builtin_amdgcn_exp2f(fmaf(s[h][c][e >> 2][e & 3], qscale, -mf)), sum += v[e];
                 l[c] += sum;
-                pieces(v, w[c]);
+                if constexpr (PACKED) {
+                    uint32_t own[4];
+#pragma unroll
+                    for (int e = 0; e < 8; e++) {
+                        v[e] = fmaf(second, __uint_as_float(cut(v[e])), v[e]);
+                        v[e] = fmaf(third, __uint_as_float(cut(v[e])), v[e]);
+                    }
+#pragma unroll
+                    for (int e = 0; e < 4; e++) own[e] = upper(v[2 * e], v[2 * e + 1]);
+                    __builtin_memcpy(&w[c][0], own, 16);
+                } else {
+                    pieces(v, w[c]);
+                }
             }
             if (h == H - 1) after_w();
 #pragma unroll
@@ -386,7 +411,7 @@ template <int HD, int CT, int AWAY> struct Columns {
                 fb8 b[2];
                 values(h, t, b);
 #pragma unroll
-                for (int k = 0; k < 3; k++)
+                for (int k = 0; k < P; k++)
 #pragma unroll
                     for (int c = 0; c < CT; c++)
 #pragma unroll
@@ -396,9 +421,8 @@ template <int HD, int CT, int AWAY> struct Columns {
         }
     }
 
-    // The blocks begin, begin + step .. below end.  DEEP: the next block's loads go out ahead of the work on this one, into
-    // registers of their own; otherwise K's and V's follow each other into the same ones as they come free.
-    template <bool DEEP, bool HOLD> __device__ __forceinline__ void run(const Kv4Params &p, const Range &r, uint32_t sequence, int head, int begin, int end, int step) {
+    // The blocks begin, begin + step .. below end, the next one's loads under way during the work on one.
+    template <bool HOLD> __device__ __forceinline__ void run(const Kv4Params &p, const Range &r, uint32_t sequence, int head, int begin, int end, int step) {
         if (begin >= end) return;
         const int lane = threadIdx.x & 63;
         uint32_t pages = 0;  // of the next 64 blocks, one a lane; those that the pool doesn't have: 0, not seen
@@ -415,34 +439,11 @@ template <int HD, int CT, int AWAY> struct Columns {
         const int n = (end - begin + step - 1) / step;
         auto page = [&](int i) { return (uint32_t)__builtin_amdgcn_readlane((int)pages, i & 63); };
         auto half = [&](int i) { return (begin + step * i) & 1; };
-        // Inner blocks and those at an edge in loops of their own: where the two meet within one, the compiler copies the
-        // outputs' registers in every iteration (104 of 480 instructions).  Twice unrolled for the same reason.
         int i = 0;
         auto at = [&](int j) { return (begin + step * j) * kBlock; };
         auto inner = [&](int j) { return at(j) >= r.full_first && at(j) + kBlock - 1 <= r.full_last && !(missing >> (j & 63) & 1); };
         Lane4<HD> x, y;
         x.load_k(p.c, page(0), head, half(0)), x.load_v(p.c, page(0), head, half(0));
-        auto edge_block = [&] {
-            const bool hidden = missing >> (i & 63) & 1;
-            if ((i & 63) == 63) look(begin + step * (i + 1));
-            const int j = min(i + 1, n - 1);  // (the last one's again, unused)
-            const uint32_t next = page(j);
-            x.clear_v(r.first - at(i), hidden ? -1 : r.last - at(i));
-            take<1, HOLD>(p.qscale, at(i), true, hidden, [&](int, int t, int pt) { return x.key(t, pt); }, [&](int, int t, fb8(&b)[2]) { x.values(t, b); },
-                          [&] { x.load_k(p.c, next, head, half(j)); }, [] {});
-            x.load_v(p.c, next, head, half(j));
-            i++;
-        };
-        auto inner_block = [&](Lane4<HD> &now, Lane4<HD> &after) {
-            if ((i & 63) == 63) look(begin + step * (i + 1));
-            const int j = min(i + 1, n - 1);
-            const uint32_t next = page(j);
-            if constexpr (DEEP) after.load_k(p.c, next, head, half(j)), after.load_v(p.c, next, head, half(j));
-            take<1, HOLD>(p.qscale, at(i), false, false, [&](int, int t, int pt) { return now.key(t, pt); }, [&](int, int t, fb8(&b)[2]) { now.values(t, b); },
-                          [&] { if constexpr (!DEEP) after.load_k(p.c, next, head, half(j)); }, [] {});
-            if constexpr (!DEEP) after.load_v(p.c, next, head, half(j));
-            i++;
-        };
         auto both = [&](Lane4<HD> &now, Lane4<HD> &after) {
             const bool hidden = missing >> (i & 63) & 1, edge = !inner(i);
             if ((i & 63) == 63) look(begin + step * (i + 1));
@@ -466,8 +467,8 @@ __device__ __forceinline__ float *column_of(float *out, const Kv4Params &p, cons
 }
 
 // Few columns (decoding): a workgroup takes an item, its wavefronts blocks in turn, joined in LDS.
-template <int HD, int CT> __global__ void __launch_bounds__(64 * kFewWaves, 2) kv4_few_kernel(Kv4Params p) {
-    constexpr int N = 16 * CT, C = HD / 4, AWAY = HD * CT > 128 ? 2 : 0, PIECES = CT * (HD / 32) * AWAY * 64;  // of a wavefront (16 bytes each)
+template <int HD, int CT, bool PACKED> __global__ void __launch_bounds__(64 * kFewWaves, 2) kv4_few_kernel(Kv4Params p) {
+    constexpr int N = PACKED ? 4 : 16 * CT, C = HD / 4, AWAY = !PACKED && HD * CT > 128 ? 2 : 0, PIECES = CT * (HD / 32) * AWAY * 64;  // of a wavefront (16 bytes each)
     constexpr int OUTPUTS = kFewWaves * N * (HD + 4), HELD = kFewWaves * PIECES * 4;
     // the queries' pieces, then the wavefronts' outputs
     __shared__ __align__(16) float lds[OUTPUTS > HELD ? OUTPUTS : HELD];
@@ -481,18 +482,22 @@ template <int HD, int CT> __global__ void __launch_bounds__(64 * kFewWaves, 2) k
     const Range r = range_of(p, t.q, first / p.group, (first + count - 1) / p.group);
     int begin = r.begin, end = r.end;
     share(begin, end, t.splits, z);
-    Columns<HD, CT, AWAY> x;
+    Columns<HD, CT, AWAY, PACKED> x;
     x.begin(p, t.q, first, count, head, reinterpret_cast<fb8 *>(lds) + wave * PIECES);
-    x.template run<HD * CT <= 128, (HD * CT > 128)>(p, r, t.q.index, head, begin + wave, end, kFewWaves);
+    x.template run<(HD * CT > 128)>(p, r, t.q.index, head, begin + wave, end, kFewWaves);
     if (AWAY) __syncthreads();
 #pragma unroll
     for (int c = 0; c < CT; c++) {
         if ((uint32_t)(16 * c) >= count) break;
         const float l = xsum<32>(xsum<16>(x.l[c]));
-        if (g == 0) ms[wave][16 * c + i] = x.m[c], ls[wave][16 * c + i] = l;
+        const int column = PACKED ? i >> 2 : 16 * c + i;
+        if (g == 0 && !(PACKED && (i & 3))) ms[wave][column] = x.m[c], ls[wave][column] = l;
 #pragma unroll
-        for (int d = 0; d < HD / 16; d++)
-            *reinterpret_cast<float4 *>(&os[wave][16 * c + i][16 * d + 4 * g]) = make_float4(x.o[c][d][0], x.o[c][d][1], x.o[c][d][2], x.o[c][d][3]);
+        for (int d = 0; d < HD / 16; d++) {
+            float4 v = make_float4(x.o[c][d][0], x.o[c][d][1], x.o[c][d][2], x.o[c][d][3]);
+            if (PACKED) v = make_float4(four(v.x), four(v.y), four(v.z), four(v.w));
+            if (!(PACKED && (i & 3))) *reinterpret_cast<float4 *>(&os[wave][column][16 * d + 4 * g]) = v;
+        }
     }
     __syncthreads();
     for (uint32_t u = tid; u < count * C; u += 64 * kFewWaves) {
@@ -523,17 +528,17 @@ template <int HD, int CT> __global__ void __launch_bounds__(64 * kFewWaves, 2) k
 }
 
 // Joins the splits of a sequence's kv head, a column at a time: a float4 of every N-th split a thread, four under way.
-template <int HD, int CT> __global__ void __launch_bounds__(256) kv4_few_join_kernel(Kv4Params p) {
+template <int HD, int COLUMNS> __global__ void __launch_bounds__(256) kv4_few_join_kernel(Kv4Params p) {
     constexpr int C = HD / 4, N = 256 / C, Z = 4;
     __shared__ float4 os[N][C];
     __shared__ float ls[N], ms[N];
-    const Share t = share_of<true, 16 * CT>(p, blockIdx.x / p.c.nkv);
+    const Share t = share_of<true, COLUMNS>(p, blockIdx.x / p.c.nkv);
     if (t.splits < 2) return;
     const int head = (int)(blockIdx.x % p.c.nkv), tid = threadIdx.x, c = tid % C, n = tid / C;
     const uint32_t count = t.q.rows * p.group;
     for (uint32_t column = blockIdx.y; column < count; column += gridDim.y) {
-        const uint32_t tile = column / (16 * CT), within = column - tile * (16 * CT);
-        auto at = [&](uint32_t z) { return ((size_t)t.slot + (tile * t.splits + min(z, t.splits - 1)) * p.c.nkv + head) * (16 * CT) + within; };
+        const uint32_t tile = column / COLUMNS, within = column - tile * COLUMNS;
+        auto at = [&](uint32_t z) { return ((size_t)t.slot + (tile * t.splits + min(z, t.splits - 1)) * p.c.nkv + head) * COLUMNS + within; };
         float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
         float m = -INFINITY, l = 0.f;
         if (n < N)
@@ -715,19 +720,20 @@ hipError_t launch_kv4_attention(const Kv4Attn &a, int cus, hipStream_t s) {
     const uint32_t limit = a.c.hd <= 128 ? 64 : 32;
     // a batch of one sequence is one kernel's; others may hold sequences of both kinds
     p.few = a.b.sequences == 1 && most > limit ? 0 : limit;
-    auto few = [&](auto h, auto tiles) {
+    auto few = [&](auto h, auto tiles, auto packed) {
         constexpr int HD = decltype(h)::value, CT = decltype(tiles)::value;
-        constexpr uint64_t N = 16 * CT;
+        constexpr bool PACKED = decltype(packed)::value;
+        constexpr uint64_t N = PACKED ? 4 : 16 * CT;
         p.wgs = 2 * cus;
         while (p.wgs > 1 && 2 * p.wgs * N * (HD + 2) > a.part_floats) p.wgs /= 2;
         p.part_ml = (float2 *)(p.part + (size_t)2 * p.wgs * N * HD);
         const uint64_t columns = std::min<uint64_t>(most, limit), tiles_of = (columns + N - 1) / N;
         const uint64_t per = (blocks + kLeastBlocks - 1) / kLeastBlocks, all_tiles = a.b.sequences * nkv * tiles_of;  // splits of a tile, and tiles, at most
         const uint64_t items = std::min(p.wgs + all_tiles, all_tiles * per);
-        hipLaunchKernelGGL((kv4_few_kernel<HD, CT>), dim3((unsigned)items), dim3(64 * kFewWaves), 0, s, p);
+        hipLaunchKernelGGL((kv4_few_kernel<HD, CT, PACKED>), dim3((unsigned)items), dim3(64 * kFewWaves), 0, s, p);
         if (per == 1) return;
         const dim3 join((unsigned)(a.b.sequences * nkv), (unsigned)std::min<uint64_t>(columns, std::max<uint64_t>(1, 1024 / (a.b.sequences * nkv))));
-        hipLaunchKernelGGL((kv4_few_join_kernel<HD, CT>), join, dim3(256), 0, s, p);
+        hipLaunchKernelGGL((kv4_few_join_kernel<HD, (int)N>), join, dim3(256), 0, s, p);
     };
     auto many = [&](auto h, auto tiles) {
         constexpr int HD = decltype(h)::value, CT = decltype(tiles)::value;
@@ -740,8 +746,9 @@ hipError_t launch_kv4_attention(const Kv4Attn &a, int cus, hipStream_t s) {
             hipLaunchKernelGGL((kv4_many_join_kernel<HD>), dim3(a.b.rows, (a.heads * (HD / 4) + 255) / 256), dim3(256), 0, s, p);
     };
     auto go = [&](auto h, auto one, auto more, auto prompt) {
-        if (p.few && most <= 16 * decltype(one)::value) few(h, one);
-        else if (p.few) few(h, more);
+        if (p.few && most <= 4) few(h, one, std::true_type{});
+        else if (p.few && most <= 16) few(h, one, std::false_type{});
+        else if (p.few) few(h, more, std::false_type{});
         if (most > p.few) many(h, prompt);
     };
     if (a.b.sequences * nkv * 8 > 0x7FFFFFFFu || (all / 16 + a.b.sequences + 4) * nkv > 0x7FFFFFFFu) return hipErrorInvalidValue;

@@ -50,6 +50,24 @@ __device__ __forceinline__ uint32_t page_of(const Batch &b, uint32_t s, uint32_t
     return b.pages[(size_t)s * b.per_seq + t / kPage];
 }
 
+// Inclusive sums over a wavefront on the vector ALU: within rows of 16 by row shifts, then the rows' ends broadcast to
+// the rows behind.  Every lane takes part.
+template <int CTRL, int ROWS> __device__ __forceinline__ uint32_t moved(uint32_t v) {
+    return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, ROWS, 0xF, false);
+}
+template <int CTRL, int ROWS, class T> __device__ __forceinline__ T add_moved(T v) {
+    if constexpr (sizeof(T) == 4) return v + (T)moved<CTRL, ROWS>((uint32_t)v);
+    else return v + ((T)moved<CTRL, ROWS>((uint32_t)((unsigned long long)v >> 32)) << 32 | (T)moved<CTRL, ROWS>((uint32_t)v));
+}
+template <class T> __device__ __forceinline__ T running_sum(T v) {
+    v = add_moved<0x111, 0xF>(v);  // row_shr:1, 2, 4, 8 (lanes before the row's start: 0)
+    v = add_moved<0x112, 0xF>(v);
+    v = add_moved<0x114, 0xF>(v);
+    v = add_moved<0x118, 0xF>(v);
+    v = add_moved<0x142, 0xA>(v);  // row_bcast:15 into rows 1 and 3
+    return add_moved<0x143, 0xC>(v);  // row_bcast:31 into rows 2 and 3
+}
+
 // One layer of a 4-bit cache.
 struct Kv4Layer {
     uint8_t *kc, *vc, *ks, *vs;

@@ -27,21 +27,99 @@ __device__ __forceinline__ uint32_t scale_byte(uint32_t bits) {
     return min(max(e, 33u) - 2u, 219u);
 }
 
-// A team of lanes takes a head, a lane four pairs of it.
-template <bool ALIGNED, bool CACHE> __global__ void __launch_bounds__(256) head_rows_kernel(HeadRows p, int units, int team) {
-    __shared__ double2 table[256];
-    __shared__ __align__(16) float held[CACHE ? 2 : 1][CACHE ? 2048 : 1];  // of each team: a key, and a value
-    __shared__ float held_scale[CACHE ? 256 : 1];
-    const int tid = threadIdx.x, u = tid % team, slot = tid / team, hp = 256 / team;
-    const int half = p.rotates ? p.rd / 2 : 0, i0 = 4 * u;
+// The sum over a team of 8 .. 64 lanes, in each of them.
+__device__ __forceinline__ double team_sum(double v, int team) {
+    auto add = [&](u64 o) { v += __longlong_as_double((long long)o); };
+    add(dpp_u64<0xB1>((u64)__double_as_longlong(v)));
+    add(dpp_u64<0x4E>((u64)__double_as_longlong(v)));
+    add(dpp_u64<0x141>((u64)__double_as_longlong(v)));
+    if (team > 8) add(dpp_u64<0x140>((u64)__double_as_longlong(v)));
+    auto far = [&](auto d) {
+        const u64 u = (u64)__double_as_longlong(v);
+        uint32_t a0, b0, a1, b1;
+        lane_pair<decltype(d)::value>((uint32_t)u, a0, b0);
+        lane_pair<decltype(d)::value>((uint32_t)(u >> 32), a1, b1);
+        v = __longlong_as_double((long long)((u64)a1 << 32 | a0)) + __longlong_as_double((long long)((u64)b1 << 32 | b0));
+    };
+    if (team > 16) far(std::integral_constant<int, 16>{});
+    if (team > 32) far(std::integral_constant<int, 32>{});
+    return v;
+}
+// 1 / sqrt(x) to a step or two of 64 bits: the hardware's estimate, and two steps of Newton's
+__device__ __forceinline__ double inverse_root(double x) {
+    double y = __builtin_amdgcn_rsq(x);
+    if (!(x > 0.0 && x < INFINITY)) return y;  // (0: infinity, an infinity: 0)
+    y = fma(0.5 * y, fma(-x * y, y, 1.0), y);
+    return fma(0.5 * y, fma(-x * y, y, 1.0), y);
+}
+
+// A lane's eight values of a head, two vectors: which of them turn with which.
+//   SPLIT   a[j] with b[j] (halves, all of the head turning), 16-byte loads
+//   PAIRS   neighbours, 16-byte loads
+//   MIXED   halves of part of the head, neighbours behind, 16-byte loads
+//   LOOSE   any of these, value by value
+enum Layout { SPLIT, PAIRS, MIXED, LOOSE };
+
+struct HeadPlan {
+    int units, team;        // lanes of a head: those with values, rounded up to a power of two
+    int chunks;             // wavefronts that share a row's heads
+    uint32_t spread, each;  // rows that follow each other lie on one XCD: `each` of them on every one of `spread`
+    int wave_bytes;         // of LDS
+};
+
+// A wavefront takes a row's heads (or every chunks-th team of them): its sines and cosines once, a pair a lane, then
+// a head a team of lanes.
+template <int LAYOUT, bool CACHE> __global__ void __launch_bounds__(256) head_rows_kernel(HeadRows p, HeadPlan plan) {
+    extern __shared__ __align__(16) char lds[];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), team = plan.team, u = lane % team, slot = lane / team;
+    const uint32_t unit = blockIdx.x * 4 + wave, at_row = unit / plan.chunks, chunk = unit - at_row * plan.chunks;
+    const uint32_t r = at_row % plan.spread * plan.each + at_row / plan.spread;
+    if (at_row / plan.spread >= plan.each || r >= p.rows) return;
+    const int half = p.rotates ? p.rd / 2 : 0, i0 = 4 * u, hp = 64 / team;
+    double2 *table = reinterpret_cast<double2 *>(lds + wave * plan.wave_bytes);
     // pair i: halves (i, i + half), neighbours (2 i, 2 i + 1) of interleaved ones and of what does not turn
     auto turns = [&](int j) { return i0 + j < half; };
-    auto split = [&](int j) { return p.style && turns(j); };
+    auto split = [&](int j) { return LAYOUT == SPLIT || (LAYOUT != PAIRS && p.style && turns(j)); };
     auto first_of = [&](int j) { return split(j) ? i0 + j : 2 * (i0 + j); };
     auto second_of = [&](int j) { return split(j) ? i0 + j + half : 2 * (i0 + j) + 1; };
-    auto in = [&](int j) { return u < units && 2 * (i0 + j) < p.hd; };
-    // ALIGNED: a unit's pairs are alike, and lie in two float4
+    auto in = [&](int j) { return u < plan.units && 2 * (i0 + j) < p.hd; };
     const int d0 = split(0) ? i0 : 2 * i0, d1 = split(0) ? i0 + half : 2 * i0 + 4;
+    const bool some = u < plan.units, whole = some && d1 < p.hd;
+    // x[0][j], x[1][j]: pair j
+    auto load = [&](const float *src, float (&x)[2][4]) {
+        if constexpr (LAYOUT == LOOSE) {
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                x[0][j] = in(j) ? src[first_of(j)] : 0.f;
+                x[1][j] = in(j) ? src[second_of(j)] : 0.f;
+            }
+        } else {
+            float4 a = make_float4(0.f, 0.f, 0.f, 0.f), b = a;
+            if (some) a = *reinterpret_cast<const float4 *>(src + d0);
+            if (whole) b = *reinterpret_cast<const float4 *>(src + d1);
+            const bool halves = split(0);
+            x[0][0] = a.x, x[1][3] = b.w;
+            x[0][1] = halves ? a.y : a.z, x[0][2] = halves ? a.z : b.x, x[0][3] = halves ? a.w : b.z;
+            x[1][0] = halves ? b.x : a.y, x[1][1] = halves ? b.y : a.w, x[1][2] = halves ? b.z : b.y;
+        }
+    };
+    auto store = [&](float *dst, const float (&y)[2][4]) {
+        if constexpr (LAYOUT == LOOSE) {
+#pragma unroll
+            for (int j = 0; j < 4; j++)
+                if (in(j)) dst[first_of(j)] = y[0][j], dst[second_of(j)] = y[1][j];
+        } else {
+            const bool halves = split(0);
+            const float4 a = make_float4(y[0][0], halves ? y[0][1] : y[1][0], halves ? y[0][2] : y[0][1], halves ? y[0][3] : y[1][1]);
+            const float4 b = make_float4(halves ? y[1][0] : y[0][2], halves ? y[1][1] : y[1][2], halves ? y[1][2] : y[0][3], y[1][3]);
+            if (some) *reinterpret_cast<float4 *>(dst + d0) = a;
+            if (whole) *reinterpret_cast<float4 *>(dst + d1) = b;
+        }
+    };
+    const int f32_heads = p.q_heads + p.k_heads, step = plan.chunks * hp, h0 = (int)chunk * hp + slot;
+    const float *row = p.src + r * p.src_stride;
+    float x[2][2][4];  // of this head and the next
+    if (h0 < f32_heads) load(row + (size_t)h0 * p.hd, x[0]);
     float wq[2][4], wk[2][4];
 #pragma unroll
     for (int j = 0; j < 4; j++) {
@@ -52,170 +130,152 @@ template <bool ALIGNED, bool CACHE> __global__ void __launch_bounds__(256) head_
             wk[e][j] = p.k_norm && in(j) ? p.k_norm[d[e]] : 0.f;
         }
     }
-    const double f = tid < half ? turns_per_position(p, tid) : 0.0;
-    const int f32_heads = p.q_heads + p.k_heads, heads = f32_heads + (CACHE ? p.c.nkv : 0);
-    for (uint32_t r = blockIdx.x; r < p.rows; r += gridDim.x) {
-        int pos = 0;
-        double at;
-        uint32_t page = 0;
-        bool stored = false;
-        if constexpr (CACHE) {
-            const Sequence q = sequence_of_row(p.b, r);
-            pos = q.first + (int)(r - q.row0);
-            if (q.rows == 0 || pos < 0) continue;  // (the workgroup's wavefronts alike)
-            stored = (uint32_t)pos < p.b.cap;
-            if (stored) page = page_of(p.b, q.index, (uint32_t)pos);
-            stored = stored && page < p.b.pool;
-            at = (double)pos;
-        } else {
-            at = (double)(p.positions ? p.positions[r] : p.first + r);
-        }
-        __syncthreads();  // the row before is done with the table
-        if (tid < half) {
-            const double t = at * f;
-            double sn, cs;
-            sincospi(2.0 * (t - rint(t)), &sn, &cs);
-            table[tid] = make_double2(cs * (double)p.magnitude, sn * (double)p.magnitude);
-        }
-        __syncthreads();
-        for (int h = blockIdx.y * hp + slot; h < heads; h += gridDim.y * hp) {
-            const bool cached = CACHE && h >= f32_heads, key = cached || h >= p.q_heads;
-            const float *src = cached ? p.k + r * p.src_stride + (size_t)(h - f32_heads) * p.hd : p.src + r * p.src_stride + (size_t)h * p.hd;
-            float x[2][4] = {};
-            if (ALIGNED) {
-                if (u < units) {
-                    const float4 a = *reinterpret_cast<const float4 *>(src + d0);
-                    const float4 b = d1 < p.hd ? *reinterpret_cast<const float4 *>(src + d1) : make_float4(0.f, 0.f, 0.f, 0.f);
-                    if (split(0)) {
-                        x[0][0] = a.x, x[0][1] = a.y, x[0][2] = a.z, x[0][3] = a.w;
-                        x[1][0] = b.x, x[1][1] = b.y, x[1][2] = b.z, x[1][3] = b.w;
-                    } else {
-                        x[0][0] = a.x, x[1][0] = a.y, x[0][1] = a.z, x[1][1] = a.w;
-                        x[0][2] = b.x, x[1][2] = b.y, x[0][3] = b.z, x[1][3] = b.w;
-                    }
-                }
-            } else {
+    double at;
+    int pos = 0;
+    uint32_t page = 0;
+    bool stored = false;
+    if constexpr (CACHE) {
+        const Sequence q = sequence_of_row(p.b, r);
+        pos = q.first + (int)(r - q.row0);
+        if (q.rows == 0 || pos < 0) return;
+        stored = (uint32_t)pos < p.b.cap;
+        if (stored) page = page_of(p.b, q.index, (uint32_t)pos);
+        stored = stored && page < p.b.pool;
+        at = (double)pos;
+    } else {
+        at = (double)(p.positions ? p.positions[r] : p.first + r);
+    }
+    for (int i = lane; i < half; i += 64) {
+        const double t = at * turns_per_position(p, i);
+        double s, c;
+        sincospi(2.0 * (t - rint(t)), &s, &c);
+        table[i] = make_double2(c * (double)p.magnitude, s * (double)p.magnitude);
+    }
+    wave_fence();
+    double cs[4], sn[4];
 #pragma unroll
-                for (int j = 0; j < 4; j++) {
-                    if (in(j)) x[0][j] = src[first_of(j)];
-                    if (in(j)) x[1][j] = src[second_of(j)];
-                }
-            }
-            const bool normed = key ? p.k_norm : p.q_norm;
-            double inv = 1.0;
+    for (int j = 0; j < 4; j++) {
+        const double2 v = turns(j) ? table[i0 + j] : make_double2(1.0, 0.0);
+        cs[j] = v.x, sn[j] = v.y;
+    }
+    auto norm_of = [&](const float (&v)[2][4]) {
+        double ss = 0.0;
+#pragma unroll
+        for (int j = 0; j < 4; j++) ss = fma((double)v[0][j], (double)v[0][j], fma((double)v[1][j], (double)v[1][j], ss));
+        return inverse_root(team_sum(ss, team) / p.hd + (double)p.eps);
+    };
+    auto turn = [&](int h, const float (&v)[2][4]) {
+        const bool key = h >= p.q_heads, normed = key ? p.k_norm : p.q_norm;
+        const float inv = normed ? (float)norm_of(v) : 1.f;
+        float y[2][4];
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            float a = v[0][j], c = v[1][j];
             if (normed) {
-                double ss = 0.0;
-#pragma unroll
-                for (int j = 0; j < 4; j++) ss = fma((double)x[0][j], (double)x[0][j], fma((double)x[1][j], (double)x[1][j], ss));
-                for (int m = 1; m < team; m <<= 1) ss += __shfl_xor(ss, m);
-                inv = 1.0 / sqrt(ss / p.hd + (double)p.eps);
+                a *= (key ? wk[0][j] + p.weight_offset : wq[0][j]) * inv;
+                c *= (key ? wk[1][j] + p.weight_offset : wq[1][j]) * inv;
             }
-            if (!cached) {
-                float *dst = p.dst + r * p.dst_stride + (size_t)h * p.hd, y[2][4];
-                const float fi = (float)inv;
-#pragma unroll
-                for (int j = 0; j < 4; j++) {
-                    float a = x[0][j], b = x[1][j];
-                    if (normed) {
-                        a *= (key ? wk[0][j] + p.weight_offset : wq[0][j]) * fi;
-                        b *= (key ? wk[1][j] + p.weight_offset : wq[1][j]) * fi;
-                    }
-                    y[0][j] = a, y[1][j] = b;
-                    if (turns(j)) {
-                        const double2 cs = table[i0 + j];
-                        const float c = (float)cs.x, s = (float)cs.y;
-                        y[0][j] = a * c - b * s, y[1][j] = a * s + b * c;
-                    }
-                }
-                if (ALIGNED) {
-                    if (u < units) {
-                        *reinterpret_cast<float4 *>(dst + d0) = split(0) ? make_float4(y[0][0], y[0][1], y[0][2], y[0][3]) : make_float4(y[0][0], y[1][0], y[0][1], y[1][1]);
-                        if (d1 < p.hd)
-                            *reinterpret_cast<float4 *>(dst + d1) = split(0) ? make_float4(y[1][0], y[1][1], y[1][2], y[1][3]) : make_float4(y[0][2], y[1][2], y[0][3], y[1][3]);
-                    }
+            const float fc = (float)cs[j], fs = (float)sn[j];
+            const bool t = LAYOUT == SPLIT || turns(j);
+            y[0][j] = t ? a * fc - c * fs : a, y[1][j] = t ? a * fs + c * fc : c;
+        }
+        store(p.dst + r * p.dst_stride + (size_t)h * p.hd, y);
+    };
+    for (int h = h0; h < f32_heads; h += 2 * step) {  // the next head's load goes out ahead of the work on one
+        if (h + step < f32_heads) load(row + (size_t)(h + step) * p.hd, x[1]);
+        turn(h, x[0]);
+        if (h + 2 * step < f32_heads) load(row + (size_t)(h + 2 * step) * p.hd, x[0]);
+        if (h + step < f32_heads) turn(h + step, x[1]);
+    }
+    if constexpr (CACHE) {
+        if (!stored) return;
+        const int g_n = p.hd / 32, c = u, g = c & 3, t = c >> 2, at64 = pos % kPage;
+        const bool holds = c < 4 * g_n;
+        float *key_at = reinterpret_cast<float *>(table + half) + lane / team * 8 * team, *value_at = key_at + 512;
+        float *scale_at = key_at - lane / team * 8 * team + 1024 + lane / team * team;
+        // keys and values behind the other heads, so that few rows' are spread over wavefronts too
+        for (int h = (h0 + step - f32_heads % step) % step; h < p.c.nkv; h += step) {
+            load(p.k + r * p.src_stride + (size_t)h * p.hd, x[0]);
+            const float *vs = p.v + r * p.src_stride + (size_t)h * p.hd;
+            float k8[8] = {}, v8[8] = {};
+            if (holds) {
+                if constexpr (LAYOUT != LOOSE) {
+                    *reinterpret_cast<float4 *>(v8) = *reinterpret_cast<const float4 *>(vs + 8 * c);
+                    *reinterpret_cast<float4 *>(v8 + 4) = *reinterpret_cast<const float4 *>(vs + 8 * c + 4);
                 } else {
 #pragma unroll
-                    for (int j = 0; j < 4; j++) {
-                        if (in(j)) dst[first_of(j)] = y[0][j];
-                        if (in(j)) dst[second_of(j)] = y[1][j];
-                    }
+                    for (int e = 0; e < 8; e++) v8[e] = vs[8 * c + e];
                 }
             }
-            if constexpr (CACHE) {
-                if (!cached || !stored) continue;
-                const int kvh = h - f32_heads, g_n = p.hd / 32, c = u, g = c & 3, t = c >> 2;
-                float *key_at = held[0] + slot * 8 * team, *value_at = held[1] + slot * 8 * team, *scale_at = held_scale + slot * team;
+            const double inv = p.k_norm ? norm_of(x[0]) : 1.0;
 #pragma unroll
-                for (int j = 0; j < 4; j++) {
-                    double a = (double)x[0][j], b = (double)x[1][j];
-                    if (normed) {
-                        a *= ((double)wk[0][j] + (double)p.weight_offset) * inv;
-                        b *= ((double)wk[1][j] + (double)p.weight_offset) * inv;
-                    }
-                    if (turns(j)) {
-                        const double2 cs = table[i0 + j];
-                        const double y = a * cs.x - b * cs.y;
-                        b = a * cs.y + b * cs.x, a = y;
-                    }
-                    if (in(j)) key_at[first_of(j)] = (float)a;
-                    if (in(j)) key_at[second_of(j)] = (float)b;
+            for (int j = 0; j < 4; j++) {
+                double a = (double)x[0][0][j], b = (double)x[0][1][j];
+                if (p.k_norm) {
+                    a *= ((double)wk[0][j] + (double)p.weight_offset) * inv;
+                    b *= ((double)wk[1][j] + (double)p.weight_offset) * inv;
                 }
-                const float *vs = p.v + r * p.src_stride + (size_t)kvh * p.hd;
-                const bool holds = c < 4 * g_n;
-                float k8[8] = {}, v8[8] = {};
-                if (holds) {
-                    if (ALIGNED) {
-                        *reinterpret_cast<float4 *>(v8) = *reinterpret_cast<const float4 *>(vs + 8 * c);
-                        *reinterpret_cast<float4 *>(v8 + 4) = *reinterpret_cast<const float4 *>(vs + 8 * c + 4);
-                    } else {
+                if (turns(j)) {
+                    const double y = a * cs[j] - b * sn[j];
+                    b = a * sn[j] + b * cs[j], a = y;
+                }
+                if (in(j)) key_at[first_of(j)] = (float)a, key_at[second_of(j)] = (float)b;
+            }
+            if (holds) {
+                *reinterpret_cast<float4 *>(value_at + 8 * c) = make_float4(v8[0], v8[1], v8[2], v8[3]);
+                *reinterpret_cast<float4 *>(value_at + 8 * c + 4) = make_float4(v8[4], v8[5], v8[6], v8[7]);
+            }
+            wave_fence();
+            uint32_t kmax = 0, vmax = 0;
+            if (holds) {
+                *reinterpret_cast<float4 *>(k8) = *reinterpret_cast<const float4 *>(key_at + 8 * c);
+                *reinterpret_cast<float4 *>(k8 + 4) = *reinterpret_cast<const float4 *>(key_at + 8 * c + 4);
 #pragma unroll
-                        for (int e = 0; e < 8; e++) v8[e] = vs[8 * c + e];
-                    }
+                for (int e = 0; e < 8; e++)
+                    kmax = max(kmax, __float_as_uint(k8[e]) & 0x7FFFFFFFu), vmax = max(vmax, __float_as_uint(v8[e]) & 0x7FFFFFFFu);
+            }
+            kmax = max(kmax, moved<0xB1, 0xF>(kmax)), vmax = max(vmax, moved<0xB1, 0xF>(vmax));
+            kmax = max(kmax, moved<0x4E, 0xF>(kmax)), vmax = max(vmax, moved<0x4E, 0xF>(vmax));
+            const u64 lanes = team == 64 ? ~0ull : ((1ull << team) - 1) << (slot * team);
+            const bool marked = __ballot(max(kmax, vmax) >= 0x7F800000u) & lanes;
+            const uint32_t kb = scale_byte(kmax), vb = marked ? 127u : scale_byte(vmax);
+            const float ks = __uint_as_float(kb << 23);
+            uint32_t w = 0;
+            w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, k8[0], k8[1], ks, 0);
+            w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, k8[2], k8[3], ks, 1);
+            w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, k8[4], k8[5], ks, 2);
+            w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, k8[6], k8[7], ks, 3);
+            const size_t codes = p.c.codes(page, h), scales = p.c.scales(page, h) + (size_t)at64 * g_n;
+            if (holds) {
+                *reinterpret_cast<uint32_t *>(p.c.kc + codes + (size_t)at64 * (p.hd / 2) + (g * g_n + t) * 4) = marked ? 0u : w;
+                if (g == 0) {
+                    p.c.ks[scales + t] = (uint8_t)(marked ? 255u : kb);
+                    p.c.vs[scales + t] = (uint8_t)vb;
+                    scale_at[t] = __uint_as_float(vb << 23);
+                }
+            }
+            wave_fence();
+            if (holds) {
+                // four bytes of the position's, dim by dim: of one dim where it has that many
+                uint8_t *to = p.c.vc + codes + (size_t)(at64 / 8) * (128 * g_n) + at64 % 8 * g_n;
+                uint32_t bytes[4];
 #pragma unroll
-                    for (int e = 0; e < 8; e++) value_at[8 * c + e] = v8[e];
+                for (int e = 0; e < 4; e++) {
+                    const int n4 = 4 * c + e, d = n4 / g_n, tt = n4 % g_n;
+                    bytes[e] = marked ? 0u : __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(0u, value_at[32 * tt + d], value_at[32 * tt + 16 + d], scale_at[tt], 0) & 255u;
                 }
-                wave_fence();
-                uint32_t kmax = 0, vmax = 0;
-                if (holds) {
-#pragma unroll
-                    for (int e = 0; e < 8; e++) {
-                        k8[e] = key_at[8 * c + e];
-                        kmax = max(kmax, __float_as_uint(k8[e]) & 0x7FFFFFFFu), vmax = max(vmax, __float_as_uint(v8[e]) & 0x7FFFFFFFu);
-                    }
-                }
-                for (int m = 1; m < 4; m <<= 1) kmax = max(kmax, (uint32_t)__shfl_xor((int)kmax, m)), vmax = max(vmax, (uint32_t)__shfl_xor((int)vmax, m));
-                const u64 lanes = team == 64 ? ~0ull : ((1ull << team) - 1) << ((tid & 63) / team * team);
-                const bool marked = __ballot(max(kmax, vmax) >= 0x7F800000u) & lanes;
-                const uint32_t kb = scale_byte(kmax), vb = marked ? 127u : scale_byte(vmax);
-                const float ks = __uint_as_float(kb << 23);
-                uint32_t w = 0;
-                w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, k8[0], k8[1], ks, 0);
-                w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, k8[2], k8[3], ks, 1);
-                w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, k8[4], k8[5], ks, 2);
-                w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, k8[6], k8[7], ks, 3);
-                const int at64 = pos % kPage;
-                const size_t codes = p.c.codes(page, kvh), scales = p.c.scales(page, kvh) + (size_t)at64 * g_n;
-                if (holds) {
-                    *reinterpret_cast<uint32_t *>(p.c.kc + codes + (size_t)at64 * (p.hd / 2) + (g * g_n + t) * 4) = marked ? 0u : w;
-                    if (g == 0) {
-                        p.c.ks[scales + t] = (uint8_t)(marked ? 255u : kb);
-                        p.c.vs[scales + t] = (uint8_t)vb;
-                        scale_at[t] = __uint_as_float(vb << 23);
-                    }
-                }
-                wave_fence();
-                if (holds) {
-                    uint8_t *to = p.c.vc + codes + (size_t)(at64 / 8) * (128 * g_n) + at64 % 8 * g_n;
+                if (g_n % 4 == 0) {
+                    const int d = 4 * c / g_n, tt = 4 * c % g_n;
+                    *reinterpret_cast<uint32_t *>(to + d * 8 * g_n + tt) = bytes[0] | bytes[1] << 8 | bytes[2] << 16 | bytes[3] << 24;
+                } else {
 #pragma unroll
                     for (int e = 0; e < 4; e++) {
-                        const int n = 4 * c + e, d = n / g_n, tt = n % g_n;
-                        const float a = value_at[32 * tt + d], b = value_at[32 * tt + 16 + d];
-                        const uint32_t byte = marked ? 0u : __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(0u, a, b, scale_at[tt], 0);
-                        to[d * 8 * g_n + tt] = (uint8_t)byte;
+                        const int n4 = 4 * c + e;
+                        to[n4 / g_n * 8 * g_n + n4 % g_n] = (uint8_t)bytes[e];
                     }
                 }
-                wave_fence();
             }
+            wave_fence();
         }
     }
 }
@@ -226,50 +286,79 @@ __device__ __forceinline__ float value_of(uint32_t code) {
     return code & 8u ? -v : v;
 }
 
-// A workgroup reads a row back, a thread eight dims of a key and of a value at a time.
+// A workgroup reads a row back: a thread eight dims of a key, then the dims 32 t + d and 32 t + 16 + d of a value, which
+// go through LDS to be written in order.
 __global__ void __launch_bounds__(256) kv4_load_kernel(Kv4Layer c, Batch b, float *k, float *v) {
+    __shared__ __align__(16) float held[4096];
     const uint32_t r = blockIdx.x;
     const Sequence q = sequence_of_row(b, r);
     const int pos = q.first + (int)(r - q.row0), gn = c.hd / 32;
     if (q.rows == 0 || pos < 0 || (uint32_t)pos >= b.cap) return;
     const uint32_t page = page_of(b, q.index, (uint32_t)pos);
     if (page >= b.pool) return;
-    const int at64 = pos % kPage, each = c.hd / 8;
-    for (int i = threadIdx.x; i < c.nkv * each; i += 256) {
-        const int head = i / each, n = i % each, t = n / 4, g = n % 4;
-        const size_t codes = c.codes(page, head), scales = c.scales(page, head) + (size_t)at64 * gn + t;
-        const uint32_t w = *reinterpret_cast<const uint32_t *>(c.kc + codes + (size_t)at64 * (c.hd / 2) + (g * gn + t) * 4);
-        const uint32_t kb = c.ks[scales], vb = c.vs[scales];
-        const float ks = kb == 255u ? __uint_as_float(0x7FC00000u) : __uint_as_float(kb << 23);
-        const float vs = kb == 255u ? ks : __uint_as_float(vb << 23);
-        const uint8_t *from = c.vc + codes + (size_t)(at64 / 8) * (128 * gn) + at64 % 8 * gn + t;
-        const size_t to = (size_t)r * c.nkv * c.hd + (size_t)head * c.hd + 8 * n;
-#pragma unroll
-        for (int e = 0; e < 8; e++) {
-            k[to + e] = value_of(w >> 4 * e) * ks;
-            const int d = (8 * n + e) % 32;
-            v[to + e] = value_of((uint32_t)from[d % 16 * 8 * gn] >> (d < 16 ? 0 : 4)) * vs;
+    const int at64 = pos % kPage, each = c.hd / 8, some = 4096 / c.hd;  // heads that LDS holds
+    const float nan = __uint_as_float(0x7FC00000u);
+    for (int from = 0; from < c.nkv; from += some) {
+        const int heads = min(some, c.nkv - from);
+        const size_t to = (size_t)r * c.nkv * c.hd + (size_t)from * c.hd;
+        for (int i = threadIdx.x; i < heads * 16; i += 256) {
+            const int head = from + i / 16, d = i % 16;
+            const uint8_t *bytes = c.vc + c.codes(page, head) + (size_t)(at64 / 8) * (128 * gn) + d * 8 * gn + at64 % 8 * gn;
+            const uint8_t *ks = c.ks + c.scales(page, head) + (size_t)at64 * gn, *vs = c.vs + c.scales(page, head) + (size_t)at64 * gn;
+            for (int t = 0; t < gn; t++) {
+                const float scale = ks[t] == 255u ? nan : __uint_as_float((uint32_t)vs[t] << 23);
+                held[i / 16 * c.hd + 32 * t + d] = value_of(bytes[t]) * scale;
+                held[i / 16 * c.hd + 32 * t + 16 + d] = value_of(bytes[t] >> 4) * scale;
+            }
         }
+        for (int i = threadIdx.x; i < heads * each; i += 256) {
+            const int head = from + i / each, n = i % each, t = n / 4, g = n % 4;
+            const uint32_t w = *reinterpret_cast<const uint32_t *>(c.kc + c.codes(page, head) + (size_t)at64 * (c.hd / 2) + (g * gn + t) * 4);
+            const uint32_t byte = c.ks[c.scales(page, head) + (size_t)at64 * gn + t];
+            const float scale = byte == 255u ? nan : __uint_as_float(byte << 23);
+            float x[8];
+#pragma unroll
+            for (int e = 0; e < 8; e++) x[e] = value_of(w >> 4 * e) * scale;
+            *reinterpret_cast<float4 *>(k + to + 8 * i) = make_float4(x[0], x[1], x[2], x[3]);
+            *reinterpret_cast<float4 *>(k + to + 8 * i + 4) = make_float4(x[4], x[5], x[6], x[7]);
+        }
+        __syncthreads();
+        for (int i = threadIdx.x; i < heads * c.hd / 4; i += 256) *reinterpret_cast<float4 *>(v + to + 4 * i) = *reinterpret_cast<const float4 *>(held + 4 * i);
+        __syncthreads();
     }
 }
 
 }  // namespace
 
 hipError_t launch_head_rows(const HeadRows &p, int cus, hipStream_t s) {
-    const int units = (p.hd + 7) / 8;
-    int team = 8;
-    while (team < units) team *= 2;  // at most 64: hd is at most 512
+    HeadPlan plan{};
+    plan.units = (p.hd + 7) / 8;
+    plan.team = 8;
+    while (plan.team < plan.units) plan.team *= 2;  // at most 64: hd is at most 512
     const bool cache = p.c.kc != nullptr;
-    const int hp = 256 / team, heads = p.q_heads + p.k_heads + (cache ? p.c.nkv : 0);
-    // few rows: their heads over workgroups; many: a workgroup takes every head of several rows
-    const uint32_t passes = (uint32_t)(heads + hp - 1) / hp, want = 8u * (uint32_t)cus;
-    const uint32_t spread = want / p.rows < 1 ? 1 : want / p.rows, gy = passes < spread ? passes : spread;
-    const dim3 grid(p.rows < want / gy ? p.rows : want / gy, gy);
+    const int hp = 64 / plan.team, heads = p.q_heads + p.k_heads + (cache ? p.c.nkv : 0), passes = (heads + hp - 1) / hp;
+    // few rows: their heads over wavefronts, up to 16 a CU
+    const uint32_t want = 16u * (uint32_t)cus / p.rows;
+    plan.chunks = want < 1 ? 1 : want < (uint32_t)passes ? (int)want : passes;
+    plan.spread = cache ? 8 : 1, plan.each = (p.rows + plan.spread - 1) / plan.spread;
+    const int half = p.rotates ? p.rd / 2 : 0;
+    plan.wave_bytes = half * 16 + (cache ? 2 * 512 * 4 + 64 * 4 : 0);
+    const uint64_t units = (uint64_t)plan.spread * plan.each * plan.chunks;
+    if (units > 0x7FFFFFF0ull) return hipErrorInvalidValue;
+    const dim3 grid((unsigned)((units + 3) / 4));
     const bool aligned = p.aligned && p.hd % 4 == 0 && (!p.rotates || p.rd % 8 == 0);
-    if (cache && aligned) hipLaunchKernelGGL((head_rows_kernel<true, true>), grid, dim3(256), 0, s, p, units, team);
-    else if (cache) hipLaunchKernelGGL((head_rows_kernel<false, true>), grid, dim3(256), 0, s, p, units, team);
-    else if (aligned) hipLaunchKernelGGL((head_rows_kernel<true, false>), grid, dim3(256), 0, s, p, units, team);
-    else hipLaunchKernelGGL((head_rows_kernel<false, false>), grid, dim3(256), 0, s, p, units, team);
+    const Layout layout = !aligned ? LOOSE : !p.rotates || !p.style ? PAIRS : p.rd == p.hd ? SPLIT : MIXED;
+    auto go = [&](auto l) {
+        constexpr int L = decltype(l)::value;
+        if (cache) hipLaunchKernelGGL((head_rows_kernel<L, true>), grid, dim3(256), 4 * plan.wave_bytes, s, p, plan);
+        else hipLaunchKernelGGL((head_rows_kernel<L, false>), grid, dim3(256), 4 * plan.wave_bytes, s, p, plan);
+    };
+    switch (layout) {
+    case SPLIT: go(std::integral_constant<int, SPLIT>{}); break;
+    case PAIRS: go(std::integral_constant<int, PAIRS>{}); break;
+    case MIXED: go(std::integral_constant<int, MIXED>{}); break;
+    default: go(std::integral_constant<int, LOOSE>{});
+    }
     return hipGetLastError();
 }
 

@@ -33,15 +33,19 @@ __device__ __forceinline__ Sequence sequence_of(const Batch &b, uint32_t s) {
 }
 // The sequence that row r belongs to; rows 0: none.  Every lane of a wavefront takes part.
 __device__ __forceinline__ Sequence sequence_of_row(const Batch &b, uint32_t r) {
-    uint32_t s = 0;  // starts at or below r behind the first
-    for (uint32_t from = 0; from < b.sequences; from += 64) {
-        const uint32_t i = from + (threadIdx.x & 63);
-        const unsigned long long below = __ballot(i < b.sequences && b.starts[min(i, b.sequences - 1) + 1] <= r);
-        s += (uint32_t)__popcll(below);
-        if (~below) break;
-    }
     Sequence q{};
-    if (s < b.sequences) q = sequence_of(b, s);
+    const int lane = threadIdx.x & 63;
+    for (uint32_t from = 0; from < b.sequences; from += 64) {
+        Sequence own{};  // this lane's sequence
+        uint32_t end = 0xFFFFFFFFu;
+        if (from + lane < b.sequences) own = sequence_of(b, from + lane), end = b.starts[from + lane + 1];
+        const unsigned long long below = __ballot(end <= r);  // sequences that end ahead of r: the first ones
+        if (!~below) continue;
+        const int at = __popcll(below);
+        auto of = [&](uint32_t v) { return (uint32_t)__builtin_amdgcn_readlane((int)v, at); };
+        q = {of(own.index), of(own.row0), of(own.rows), (int)of((uint32_t)own.first)};
+        break;
+    }
     if (r < q.row0 || r - q.row0 >= q.rows) q.rows = 0;
     return q;
 }

@@ -54,18 +54,28 @@ __device__ __forceinline__ double inverse_root(double x) {
 }
 
 // A lane's eight values of a head, two vectors: which of them turn with which.
-//   SPLIT   a[j] with b[j] (halves, all of the head turning), 16-byte loads
-//   PAIRS   neighbours, 16-byte loads
-//   MIXED   halves of part of the head, neighbours behind, 16-byte loads
+//   SPLIT   a[j] with b[j] (halves, all of the head turning): values 4 u and hd / 2 + 4 u on
+//   PAIRS   neighbours, of the same values
+//   MIXED   halves of part of the head, neighbours behind: 16-byte loads, but not of whole lines
 //   LOOSE   any of these, value by value
 enum Layout { SPLIT, PAIRS, MIXED, LOOSE };
+
+constexpr int kAhead = 2;  // heads of a team whose loads are under way ahead of the one at work
 
 struct HeadPlan {
     int units, team;        // lanes of a head: those with values, rounded up to a power of two
     int chunks;             // wavefronts that share a row's heads
     uint32_t spread, each;  // rows that follow each other lie on one XCD: `each` of them on every one of `spread`
     int wave_bytes;         // of LDS
+    int streams;            // the output is more than the caches hold
 };
+
+// streams: past the caches (4095 rows of 40 heads of 128: 41 us without, 34 with; of parts of lines it costs time)
+__device__ __forceinline__ void put(float *to, float4 v, int streams) {
+    typedef float f4 __attribute__((ext_vector_type(4)));
+    if (streams) __builtin_nontemporal_store(f4{v.x, v.y, v.z, v.w}, reinterpret_cast<f4 *>(to));
+    else *reinterpret_cast<float4 *>(to) = v;
+}
 
 // A wavefront takes a row's heads (or every chunks-th team of them): its sines and cosines once, a pair a lane, then
 // a head a team of lanes.
@@ -78,12 +88,13 @@ template <int LAYOUT, bool CACHE> __global__ void __launch_bounds__(256) head_ro
     const int half = p.rotates ? p.rd / 2 : 0, i0 = 4 * u, hp = 64 / team;
     double2 *table = reinterpret_cast<double2 *>(lds + wave * plan.wave_bytes);
     // pair i: halves (i, i + half), neighbours (2 i, 2 i + 1) of interleaved ones and of what does not turn
-    auto turns = [&](int j) { return i0 + j < half; };
+    auto pair = [&](int j) { return LAYOUT == PAIRS ? 2 * u + (j & 1) + (j >> 1) * (p.hd / 4) : i0 + j; };
+    auto turns = [&](int j) { return pair(j) < half; };
     auto split = [&](int j) { return LAYOUT == SPLIT || (LAYOUT != PAIRS && p.style && turns(j)); };
-    auto first_of = [&](int j) { return split(j) ? i0 + j : 2 * (i0 + j); };
-    auto second_of = [&](int j) { return split(j) ? i0 + j + half : 2 * (i0 + j) + 1; };
-    auto in = [&](int j) { return u < plan.units && 2 * (i0 + j) < p.hd; };
-    const int d0 = split(0) ? i0 : 2 * i0, d1 = split(0) ? i0 + half : 2 * i0 + 4;
+    auto first_of = [&](int j) { return split(j) ? pair(j) : 2 * pair(j); };
+    auto second_of = [&](int j) { return split(j) ? pair(j) + half : 2 * pair(j) + 1; };
+    auto in = [&](int j) { return u < plan.units && 2 * pair(j) < p.hd; };
+    const int d0 = split(0) ? i0 : LAYOUT == PAIRS ? 4 * u : 2 * i0, d1 = split(0) ? i0 + half : LAYOUT == PAIRS ? p.hd / 2 + 4 * u : 2 * i0 + 4;
     const bool some = u < plan.units, whole = some && d1 < p.hd;
     // x[0][j], x[1][j]: pair j
     auto load = [&](const float *src, float (&x)[2][4]) {
@@ -112,14 +123,16 @@ template <int LAYOUT, bool CACHE> __global__ void __launch_bounds__(256) head_ro
             const bool halves = split(0);
             const float4 a = make_float4(y[0][0], halves ? y[0][1] : y[1][0], halves ? y[0][2] : y[0][1], halves ? y[0][3] : y[1][1]);
             const float4 b = make_float4(halves ? y[1][0] : y[0][2], halves ? y[1][1] : y[1][2], halves ? y[1][2] : y[0][3], y[1][3]);
-            if (some) *reinterpret_cast<float4 *>(dst + d0) = a;
-            if (whole) *reinterpret_cast<float4 *>(dst + d1) = b;
+            if (some) put(dst + d0, a, plan.streams);
+            if (whole) put(dst + d1, b, plan.streams);
         }
     };
     const int f32_heads = p.q_heads + p.k_heads, step = plan.chunks * hp, h0 = (int)chunk * hp + slot;
     const float *row = p.src + r * p.src_stride;
-    float x[2][2][4];  // of this head and the next
-    if (h0 < f32_heads) load(row + (size_t)h0 * p.hd, x[0]);
+    float x[kAhead + 1][2][4];  // of this head and the next ones
+#pragma unroll
+    for (int b = 0; b < kAhead; b++)
+        if (h0 + b * step < f32_heads) load(row + (size_t)(h0 + b * step) * p.hd, x[b]);
     float wq[2][4], wk[2][4];
 #pragma unroll
     for (int j = 0; j < 4; j++) {
@@ -155,7 +168,7 @@ template <int LAYOUT, bool CACHE> __global__ void __launch_bounds__(256) head_ro
     double cs[4], sn[4];
 #pragma unroll
     for (int j = 0; j < 4; j++) {
-        const double2 v = turns(j) ? table[i0 + j] : make_double2(1.0, 0.0);
+        const double2 v = turns(j) ? table[pair(j)] : make_double2(1.0, 0.0);
         cs[j] = v.x, sn[j] = v.y;
     }
     auto norm_of = [&](const float (&v)[2][4]) {
@@ -181,11 +194,13 @@ template <int LAYOUT, bool CACHE> __global__ void __launch_bounds__(256) head_ro
         }
         store(p.dst + r * p.dst_stride + (size_t)h * p.hd, y);
     };
-    for (int h = h0; h < f32_heads; h += 2 * step) {  // the next head's load goes out ahead of the work on one
-        if (h + step < f32_heads) load(row + (size_t)(h + step) * p.hd, x[1]);
-        turn(h, x[0]);
-        if (h + 2 * step < f32_heads) load(row + (size_t)(h + 2 * step) * p.hd, x[0]);
-        if (h + step < f32_heads) turn(h + step, x[1]);
+    for (int h = h0; h < f32_heads; h += (kAhead + 1) * step) {
+#pragma unroll
+        for (int b = 0; b <= kAhead; b++) {
+            const int now = h + b * step, next = now + kAhead * step;
+            if (next < f32_heads) load(row + (size_t)next * p.hd, x[(b + kAhead) % (kAhead + 1)]);
+            if (now < f32_heads) turn(now, x[b]);
+        }
     }
     if constexpr (CACHE) {
         if (!stored) return;
@@ -280,51 +295,64 @@ template <int LAYOUT, bool CACHE> __global__ void __launch_bounds__(256) head_ro
     }
 }
 
+// what a code (bits 3 .. 0) stands for
 __device__ __forceinline__ float value_of(uint32_t code) {
-    const uint32_t m = code & 7u;
-    const float v = m < 4 ? 0.5f * (float)m : m < 6 ? (float)m - 2.f : 2.f * (float)m - 8.f;
-    return code & 8u ? -v : v;
+    typedef float f2 __attribute__((ext_vector_type(2)));
+    const f2 v = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(code, 1.f, 0);
+    return v[0];
 }
 
-// A workgroup reads a row back: a thread eight dims of a key, then the dims 32 t + d and 32 t + 16 + d of a value, which
-// go through LDS to be written in order.
-__global__ void __launch_bounds__(256) kv4_load_kernel(Kv4Layer c, Batch b, float *k, float *v) {
-    __shared__ __align__(16) float held[4096];
-    const uint32_t r = blockIdx.x;
+// A wavefront reads a row back, 1024 / HD heads at a time: a lane eight dims of a key, then the dims 32 t + d and
+// 32 t + 16 + d of a value, which go through LDS to be written in order.
+template <int HD> __global__ void __launch_bounds__(256) kv4_load_kernel(Kv4Layer c, Batch b, float *k, float *v) {
+    constexpr int G = HD / 32, EACH = HD / 8, SOME = 1024 / HD, HELD = HD + 4;
+    __shared__ __align__(16) float lds[4][SOME * HELD];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+    const uint32_t r = blockIdx.x * 4 + wave;
+    if (r >= b.rows) return;
     const Sequence q = sequence_of_row(b, r);
-    const int pos = q.first + (int)(r - q.row0), gn = c.hd / 32;
+    const int pos = q.first + (int)(r - q.row0);
     if (q.rows == 0 || pos < 0 || (uint32_t)pos >= b.cap) return;
     const uint32_t page = page_of(b, q.index, (uint32_t)pos);
     if (page >= b.pool) return;
-    const int at64 = pos % kPage, each = c.hd / 8, some = 4096 / c.hd;  // heads that LDS holds
+    const int at64 = pos % kPage;
     const float nan = __uint_as_float(0x7FC00000u);
-    for (int from = 0; from < c.nkv; from += some) {
-        const int heads = min(some, c.nkv - from);
-        const size_t to = (size_t)r * c.nkv * c.hd + (size_t)from * c.hd;
-        for (int i = threadIdx.x; i < heads * 16; i += 256) {
-            const int head = from + i / 16, d = i % 16;
-            const uint8_t *bytes = c.vc + c.codes(page, head) + (size_t)(at64 / 8) * (128 * gn) + d * 8 * gn + at64 % 8 * gn;
-            const uint8_t *ks = c.ks + c.scales(page, head) + (size_t)at64 * gn, *vs = c.vs + c.scales(page, head) + (size_t)at64 * gn;
-            for (int t = 0; t < gn; t++) {
+    float *held = lds[wave];
+    for (int from = 0; from < c.nkv; from += SOME) {
+        const int heads = min(SOME, c.nkv - from);
+        const size_t to = ((size_t)r * c.nkv + from) * HD;
+#pragma unroll
+        for (int e = 0; e < SOME * 16; e += 64) {
+            const int i = e + lane, head = i / 16, d = i % 16;
+            if (i >= heads * 16) break;
+            uint8_t bytes[G], ks[G], vs[G];
+            __builtin_memcpy(bytes, c.vc + c.codes(page, from + head) + (size_t)(at64 / 8) * (128 * G) + d * 8 * G + at64 % 8 * G, G);
+            __builtin_memcpy(ks, c.ks + c.scales(page, from + head) + (size_t)at64 * G, G);
+            __builtin_memcpy(vs, c.vs + c.scales(page, from + head) + (size_t)at64 * G, G);
+#pragma unroll
+            for (int t = 0; t < G; t++) {
                 const float scale = ks[t] == 255u ? nan : __uint_as_float((uint32_t)vs[t] << 23);
-                held[i / 16 * c.hd + 32 * t + d] = value_of(bytes[t]) * scale;
-                held[i / 16 * c.hd + 32 * t + 16 + d] = value_of(bytes[t] >> 4) * scale;
+                held[head * HELD + 32 * t + d] = value_of(bytes[t]) * scale;
+                held[head * HELD + 32 * t + 16 + d] = value_of(bytes[t] >> 4) * scale;
             }
         }
-        for (int i = threadIdx.x; i < heads * each; i += 256) {
-            const int head = from + i / each, n = i % each, t = n / 4, g = n % 4;
-            const uint32_t w = *reinterpret_cast<const uint32_t *>(c.kc + c.codes(page, head) + (size_t)at64 * (c.hd / 2) + (g * gn + t) * 4);
-            const uint32_t byte = c.ks[c.scales(page, head) + (size_t)at64 * gn + t];
+#pragma unroll
+        for (int e = 0; e < SOME * EACH; e += 64) {
+            const int i = e + lane, head = from + i / EACH, n = i % EACH, t = n / 4, g = n % 4;
+            if (i >= heads * EACH) break;
+            const uint32_t w = *reinterpret_cast<const uint32_t *>(c.kc + c.codes(page, head) + (size_t)at64 * (HD / 2) + (g * G + t) * 4);
+            const uint32_t byte = c.ks[c.scales(page, head) + (size_t)at64 * G + t];
             const float scale = byte == 255u ? nan : __uint_as_float(byte << 23);
             float x[8];
 #pragma unroll
-            for (int e = 0; e < 8; e++) x[e] = value_of(w >> 4 * e) * scale;
+            for (int j = 0; j < 8; j++) x[j] = value_of(w >> 4 * j) * scale;
             *reinterpret_cast<float4 *>(k + to + 8 * i) = make_float4(x[0], x[1], x[2], x[3]);
             *reinterpret_cast<float4 *>(k + to + 8 * i + 4) = make_float4(x[4], x[5], x[6], x[7]);
         }
-        __syncthreads();
-        for (int i = threadIdx.x; i < heads * c.hd / 4; i += 256) *reinterpret_cast<float4 *>(v + to + 4 * i) = *reinterpret_cast<const float4 *>(held + 4 * i);
-        __syncthreads();
+        wave_fence();
+        for (int i = lane; i < heads * (HD / 4); i += 64)
+            *reinterpret_cast<float4 *>(v + to + 4 * i) = *reinterpret_cast<const float4 *>(held + i / (HD / 4) * HELD + 4 * (i % (HD / 4)));
+        wave_fence();
     }
 }
 
@@ -346,8 +374,9 @@ hipError_t launch_head_rows(const HeadRows &p, int cus, hipStream_t s) {
     const uint64_t units = (uint64_t)plan.spread * plan.each * plan.chunks;
     if (units > 0x7FFFFFF0ull) return hipErrorInvalidValue;
     const dim3 grid((unsigned)((units + 3) / 4));
-    const bool aligned = p.aligned && p.hd % 4 == 0 && (!p.rotates || p.rd % 8 == 0);
-    const Layout layout = !aligned ? LOOSE : !p.rotates || !p.style ? PAIRS : p.rd == p.hd ? SPLIT : MIXED;
+    const bool aligned = p.aligned && p.hd % 8 == 0, pairs = !p.rotates || !p.style;
+    const Layout layout = !aligned ? LOOSE : pairs ? PAIRS : p.rd == p.hd ? SPLIT : p.rd % 8 == 0 ? MIXED : LOOSE;
+    plan.streams = layout <= PAIRS && (uint64_t)p.rows * (p.q_heads + p.k_heads) * p.hd * 4 > (16u << 20);
     auto go = [&](auto l) {
         constexpr int L = decltype(l)::value;
         if (cache) hipLaunchKernelGGL((head_rows_kernel<L, true>), grid, dim3(256), 4 * plan.wave_bytes, s, p, plan);
@@ -363,7 +392,13 @@ hipError_t launch_head_rows(const HeadRows &p, int cus, hipStream_t s) {
 }
 
 hipError_t launch_kv4_load(const Kv4Layer &c, const Batch &b, float *k, float *v, hipStream_t s) {
-    hipLaunchKernelGGL(kv4_load_kernel, dim3(b.rows), dim3(256), 0, s, c, b, k, v);
+    const dim3 grid((b.rows + 3) / 4);
+    switch (c.hd) {
+    case 64: hipLaunchKernelGGL(kv4_load_kernel<64>, grid, dim3(256), 0, s, c, b, k, v); break;
+    case 96: hipLaunchKernelGGL(kv4_load_kernel<96>, grid, dim3(256), 0, s, c, b, k, v); break;
+    case 128: hipLaunchKernelGGL(kv4_load_kernel<128>, grid, dim3(256), 0, s, c, b, k, v); break;
+    default: hipLaunchKernelGGL(kv4_load_kernel<256>, grid, dim3(256), 0, s, c, b, k, v);
+    }
     return hipGetLastError();
 }
 

@@ -269,9 +269,11 @@ template <int HD, int CT, int AWAY, bool PACKED = false> struct Columns {
     float m[CT], l[CT];
     int lo[CT], hi[CT];  // the positions that a column sees, both included
 
-    // columns first .. first + count - 1 of a sequence
-    __device__ __forceinline__ void begin(const Kv4Params &p, const Sequence &t, uint32_t first, uint32_t count, int head, fb8 *lds) {
-        away = lds;
+    // Columns first .. first + count - 1 of a sequence: their queries on the way, then in pieces.
+    struct Raw {
+        float v[CT][G][8];
+    };
+    __device__ __forceinline__ void fetch(const Kv4Params &p, const Sequence &t, uint32_t first, uint32_t count, int head, Raw &raw) {
         const int i = threadIdx.x & 15, g = threadIdx.x >> 4 & 3;
 #pragma unroll
         for (int c = 0; c < CT; c++) {
@@ -282,18 +284,28 @@ template <int HD, int CT, int AWAY, bool PACKED = false> struct Columns {
             hi[c] = min(hi[c], (int)p.b.cap - 1);
 #pragma unroll
             for (int k = 0; k < G; k++) {
-                float v[8];
                 const float *from = src + 32 * k + 8 * g;
                 if (p.q_aligned) {
-                    *reinterpret_cast<float4 *>(v) = *reinterpret_cast<const float4 *>(from);
-                    *reinterpret_cast<float4 *>(v + 4) = *reinterpret_cast<const float4 *>(from + 4);
+                    *reinterpret_cast<float4 *>(raw.v[c][k]) = *reinterpret_cast<const float4 *>(from);
+                    *reinterpret_cast<float4 *>(raw.v[c][k] + 4) = *reinterpret_cast<const float4 *>(from + 4);
                 } else {
 #pragma unroll
-                    for (int e = 0; e < 8; e++) v[e] = from[e];
+                    for (int e = 0; e < 8; e++) raw.v[c][k][e] = from[e];
                 }
+            }
+        }
+    }
+    __device__ __forceinline__ void begin(const Kv4Params &p, const Raw &raw, fb8 *lds) {
+        const int i = threadIdx.x & 15;
+        away = lds;
 #pragma unroll
-                for (int e = 0; e < 8; e++) v[e] *= p.qsign;
+        for (int c = 0; c < CT; c++) {
+#pragma unroll
+            for (int k = 0; k < G; k++) {
+                float v[8];
                 fb8 all[3];
+#pragma unroll
+                for (int e = 0; e < 8; e++) v[e] = raw.v[c][k][e] * p.qsign;
                 pieces(v, all);
                 if constexpr (PACKED) {
                     const fb8 none = {};
@@ -422,8 +434,13 @@ template <int HD, int CT, int AWAY, bool PACKED = false> struct Columns {
     }
 
     // The blocks begin, begin + step .. below end, the next one's loads under way during the work on one.
-    template <bool HOLD> __device__ __forceinline__ void run(const Kv4Params &p, const Range &r, uint32_t sequence, int head, int begin, int end, int step) {
-        if (begin >= end) return;
+    // ready: what else has to be done before, behind the first loads.
+    template <bool HOLD, class F>
+    __device__ __forceinline__ void run(const Kv4Params &p, const Range &r, uint32_t sequence, int head, int begin, int end, int step, F ready) {
+        if (begin >= end) {
+            ready();
+            return;
+        }
         const int lane = threadIdx.x & 63;
         uint32_t pages = 0;  // of the next 64 blocks, one a lane; those that the pool doesn't have: 0, not seen
         u64 missing = 0;
@@ -444,6 +461,8 @@ template <int HD, int CT, int AWAY, bool PACKED = false> struct Columns {
         auto inner = [&](int j) { return at(j) >= r.full_first && at(j) + kBlock - 1 <= r.full_last && !(missing >> (j & 63) & 1); };
         Lane4<HD> x, y;
         x.load_k(p.c, page(0), head, half(0)), x.load_v(p.c, page(0), head, half(0));
+        __builtin_amdgcn_sched_barrier(0);
+        ready();
         auto both = [&](Lane4<HD> &now, Lane4<HD> &after) {
             const bool hidden = missing >> (i & 63) & 1, edge = !inner(i);
             if ((i & 63) == 63) look(begin + step * (i + 1));
@@ -483,8 +502,9 @@ template <int HD, int CT, bool PACKED> __global__ void __launch_bounds__(64 * kF
     int begin = r.begin, end = r.end;
     share(begin, end, t.splits, z);
     Columns<HD, CT, AWAY, PACKED> x;
-    x.begin(p, t.q, first, count, head, reinterpret_cast<fb8 *>(lds) + wave * PIECES);
-    x.template run<(HD * CT > 128)>(p, r, t.q.index, head, begin + wave, end, kFewWaves);
+    typename Columns<HD, CT, AWAY, PACKED>::Raw raw;
+    x.fetch(p, t.q, first, count, head, raw);
+    x.template run<(HD * CT > 128)>(p, r, t.q.index, head, begin + wave, end, kFewWaves, [&] { x.begin(p, raw, reinterpret_cast<fb8 *>(lds) + wave * PIECES); });
     if (AWAY) __syncthreads();
 #pragma unroll
     for (int c = 0; c < CT; c++) {
@@ -635,7 +655,8 @@ template <int HD, int CT, int AWAY> __global__ void __launch_bounds__(256, 2) kv
     share(begin, end, (uint32_t)p.splits, blockIdx.y);
     Columns<HD, CT, AWAY> x;
     const uint32_t first = t.first + 16 * CT * wave;
-    x.begin(p, t.q, min(first, t.first + t.count - 1), first < t.first + t.count ? t.first + t.count - first : 1, head, held[AWAY ? wave : 0]);
+    typename Columns<HD, CT, AWAY>::Raw raw;
+    x.fetch(p, t.q, min(first, t.first + t.count - 1), first < t.first + t.count ? t.first + t.count - first : 1, head, raw);
     uint32_t ids = 0;  // of the next 64 pages, one a lane; those that the pool doesn't have: 0, not seen
     u64 missing = 0;
     auto look = [&](int b) {
@@ -651,6 +672,7 @@ template <int HD, int CT, int AWAY> __global__ void __launch_bounds__(256, 2) kv
         look(begin);
         y.load(p.c, id(begin), head, wave);
     }
+    x.begin(p, raw, held[AWAY ? wave : 0]);
     for (int n = begin; n < end; n++) {
         const int at = n * kPage;
         const bool hidden = missing >> ((n - begin) & 63) & 1, edge = hidden || at < r.full_first || at + kPage - 1 > r.full_last;

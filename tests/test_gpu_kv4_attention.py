@@ -159,6 +159,56 @@ def test_small_weights_beside_a_dominant_key(hip_ctx):
     assert np.all(np.abs(got - want) <= (2 * 60 * 2.0 ** -23 + 2.0 ** -20) * 18)
 
 
+@pytest.mark.parametrize("rows,length", [(1, 2), (1, 70), (3, 130), (1, 5000), (9, 200), (80, 100)])
+@pytest.mark.parametrize("hd", [64, 96, 128, 256])
+def test_every_bit_of_a_weight_counts(hip_ctx, hd, rows, length):
+    """One value of 1 among zeros, and one key that sees the query's first value: the output is w / (w + n - 1),
+    w = exp(q k scale).  Tolerance: the score is one exact product, rounded with the scale to 2^-22 of itself; the
+    exponential and its pieces 2^-21; the sums of n - 1 ones are exact, the others' 2^-22: a piece lost, or taken
+    twice, would be 2^-16 or 2^-8."""
+    for group in (1, 4, 16):
+        rng = np.random.default_rng(hd + rows + group)
+        batch = oracle.Batch([rows], [length], rng)
+        cache = oracle.Kv4(1, batch.pool, 1, hd)
+        for t in range(length):
+            page, slot = batch.place(0, t)
+            cache.scales[0][0, page, slot] = cache.scales[1][0, page, slot] = 127
+            cache.codes[0][0, page, slot, 0] = 2 if t == 1 else 0  # 1 and 0
+            cache.codes[1][0, page, slot] = 2 if t == 1 else 0
+        q = np.zeros((rows, group, hd), np.float32)
+        q[..., 0] = rng.uniform(-6, 6, (rows, group))
+        got, _, _ = attend(hip_ctx, [], [], group, 1, hd, batch=batch, cache=cache, q=q, rng=rng, scale=0.7)
+        score = q[..., :1].astype(np.float64) * float(np.float32(0.7))
+        others = np.arange(length - rows, length)[:, None, None]  # positions in sight but the one
+        want = np.where(others >= 1, np.exp(score) / (np.exp(score) + others), 0.0)
+        off = np.abs(got - want)
+        assert np.all(off <= (np.abs(score) * 2.0 ** -21 + 2.0 ** -20) * want), (off / np.maximum(want, 1e-300)).max()
+
+
+@pytest.mark.parametrize("rows,lengths", [([1], [300]), ([1] * 5, [64, 900, 20, 300, 3000]), ([4], [500]), ([40], [200]), ([200], [300])])
+def test_errors_over_all_outputs(hip_ctx, rows, lengths):
+    """The worst case of the bound above is far from what happens: roundings go both ways.  A score's 3 hd products add up
+    with as many roundings, each of at most 2^-24 of the sum so far (2^-24 / sqrt(3) of it in the mean), which in the
+    mean over scores is at most R = sqrt(sum (q k scale)^2): sqrt(hd) 2^-24 R together.  The scale's roundings and the
+    maximum's add 2^-22 R.  That is a weight's error relative to itself; the exponential's is 2^-22, the sums' and the
+    outputs' less.  An output's error is the sum of w error (v - output), in the mean of squares as large beside the
+    output, a sum of w v of values of either sign, as the weights' errors are beside 1; 1.5 times that for what the mean
+    over few rows leaves open.  (Products of 128: 6 10^-6 here; a weight's third piece taken twice is 9 10^-6.)"""
+    for heads, kvh, hd in ((4, 4, 128), (8, 2, 128), (16, 1, 64), (2, 1, 256)):
+        rng = np.random.default_rng(heads + hd)
+        batch = oracle.Batch(rows, lengths, rng)
+        cache = oracle.Kv4(1, batch.pool, kvh, hd, rng)
+        q = rng.normal(0, 0.7, (batch.n, heads, hd)).astype(np.float32)
+        got, want, _ = attend(hip_ctx, rows, lengths, heads, kvh, hd, batch=batch, cache=cache, q=q, rng=rng)
+        squares = []
+        for r, s, p in batch.positions():
+            at = np.arange(p + 1)
+            k, _ = cache.rows(0, batch.table[s, at // 64].astype(int), at % 64)
+            squares.append((np.repeat(k ** 2, heads // kvh, axis=1) * q[r].astype(np.float64) ** 2).sum(axis=2).mean() / hd)
+        size = np.sqrt(np.mean(squares))
+        assert np.linalg.norm(got - want) <= 1.5 * ((np.sqrt(hd) + 4) * 2.0 ** -24 * size + 2.0 ** -21) * np.linalg.norm(want), (heads, kvh, hd, size)
+
+
 def test_marked_positions(hip_ctx):
     """A position with a NaN: rows that see it are NaN throughout (its kv head's), the others as without it."""
     rng = np.random.default_rng(7)

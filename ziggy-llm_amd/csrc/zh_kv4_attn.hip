@@ -328,7 +328,7 @@ template <int HD, int CT, int AWAY, bool PACKED = false> struct Columns {
     template <int H, bool HOLD, class K, class V, class A, class B>
     __device__ __forceinline__ void take(float qscale, int at, bool edge, bool hidden, K key, V values, A after_k, B after_w) {
         const int g = threadIdx.x >> 4 & 3;
-        // of a weight, lane i % 4 = 1 takes off the first piece, 2 the second too; 3 (whose weights nothing reads) as 2
+        // of a weight, lane i % 4 = 1 takes off the first piece, 2 the second too (3 as well: its outputs are left out)
         const float second = PACKED && (threadIdx.x & 3) > 0 ? -1.f : 0.f, third = PACKED && (threadIdx.x & 3) > 1 ? -1.f : 0.f;
         int lane = threadIdx.x & 63;
         if constexpr (AWAY > 0) __asm__ volatile("" : "+v"(lane));  // (the pieces in LDS are read where they are used, not ahead of the loop)
@@ -515,7 +515,10 @@ template <int HD, int CT, bool PACKED> __global__ void __launch_bounds__(64 * kF
 #pragma unroll
         for (int d = 0; d < HD / 16; d++) {
             float4 v = make_float4(x.o[c][d][0], x.o[c][d][1], x.o[c][d][2], x.o[c][d][3]);
-            if (PACKED) v = make_float4(four(v.x), four(v.y), four(v.z), four(v.w));
+            if (PACKED) {
+                if ((i & 3) == 3) v = make_float4(0.f, 0.f, 0.f, 0.f);  // (the third piece's once more)
+                v = make_float4(four(v.x), four(v.y), four(v.z), four(v.w));
+            }
             if (!(PACKED && (i & 3))) *reinterpret_cast<float4 *>(&os[wave][column][16 * d + 4 * g]) = v;
         }
     }

@@ -8,8 +8,8 @@
 //   slices  a workgroup per 2048 logits (8192 where rows alone fill the device), held in registers: the largest, the
 //           sums relative to it, and its k best in order;
 //   rows    a workgroup per row joins its slices.
-// The k best: a value that at least k others of the slice reach (the k-th of 64 columns' largest) leaves few
-// candidates, and a candidate's place is the count of those above it: no sort, no dependence on the order of arrival.
+// The k best of a slice: a value that k logits reach (see limit_of) leaves few candidates, and a candidate's place is
+// the count of those above it: no sort, no dependence on the order of arrival.
 #include <algorithm>
 
 #include "zh_serving.h"
@@ -30,7 +30,7 @@ struct SliceSums {
 struct LogprobsWork {
     SliceSums *sums;  // [row][slice]
     u64 *top;         // [row][slice][k]
-    uint32_t slices;
+    uint32_t slices, logits;  // of a row, and (all but the last) of a slice: a multiple of 4
 };
 
 // orders by value, the highest first, then by index, the lowest first; NaN as -infinity, the zeros equal; above 0
@@ -68,27 +68,56 @@ __device__ __forceinline__ double wave_sum(double v) {
     return far(v, std::integral_constant<int, 32>{});
 }
 
-// candidates' places by counting: those of rank below k go to `to`
-__device__ __forceinline__ void place(const u64 *candidates, int n, int k, u64 *to) {
+// candidates' places by counting: to(rank, candidate) for those of rank below k
+template <class F> __device__ __forceinline__ void place(const u64 *candidates, int n, int k, F to) {
     for (int i = threadIdx.x; i < n; i += blockDim.x) {
         const u64 own = candidates[i];
-        int rank = 0;
-        for (int j = 0; j < n; j++) rank += candidates[j] > own;
-        if (rank < k) to[rank] = own;
+        int rank = 0, j = 0;
+        for (; j + 8 <= n; j += 8) {
+            ulonglong2 o[4];
+#pragma unroll
+            for (int e = 0; e < 4; e++) o[e] = *reinterpret_cast<const ulonglong2 *>(candidates + j + 2 * e);
+#pragma unroll
+            for (int e = 0; e < 4; e++) rank += (o[e].x > own) + (o[e].y > own);
+        }
+        for (; j < n; j++) rank += candidates[j] > own;
+        if (rank < k) to(rank, own);
     }
 }
 
-// A workgroup per slice of 256 V logits.
+// lanes of this one's row of 16 with a larger value
+__device__ __forceinline__ int above_in_row(float v) {
+    int above = 0;
+    auto turn = [&](auto by) {  // the lane so many on within the row
+        const float other = __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), 0x120 + decltype(by)::value, 0xF, 0xF, false));
+        above += other > v;
+    };
+    turn(std::integral_constant<int, 1>{}), turn(std::integral_constant<int, 2>{}), turn(std::integral_constant<int, 3>{});
+    turn(std::integral_constant<int, 4>{}), turn(std::integral_constant<int, 5>{}), turn(std::integral_constant<int, 6>{});
+    turn(std::integral_constant<int, 7>{}), turn(std::integral_constant<int, 8>{}), turn(std::integral_constant<int, 9>{});
+    turn(std::integral_constant<int, 10>{}), turn(std::integral_constant<int, 11>{}), turn(std::integral_constant<int, 12>{});
+    turn(std::integral_constant<int, 13>{}), turn(std::integral_constant<int, 14>{}), turn(std::integral_constant<int, 15>{});
+    return above;
+}
+// the largest of four lanes, and of a row of 16
+template <int CTRL> __device__ __forceinline__ float max_moved(float v) {
+    return fmaxf(v, __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), CTRL, 0xF, 0xF, false)));
+}
+__device__ __forceinline__ float quad_max(float v) { return max_moved<0x4E>(max_moved<0xB1>(v)); }
+__device__ __forceinline__ float row_max(float v) { return max_moved<0x140>(max_moved<0x141>(quad_max(v))); }
+
+// A workgroup per slice of 256 V logits.  Its k best are of the finite ones alone.
 template <int V> __global__ void __launch_bounds__(kThreads) logprobs_slice_kernel(TokenLogprobs p, LogprobsWork w) {
-    __shared__ u64 columns[4][64], candidates[kCandidates];
+    __shared__ __align__(16) u64 candidates[kCandidates];
+    __shared__ u64 best[4];
     __shared__ double sums[2][4];
-    __shared__ float tops[4];
+    __shared__ float rows[16], quads[64];
     __shared__ uint32_t counts[4];
-    __shared__ int ranks[64], found;
-    const uint32_t row = blockIdx.x / w.slices, slice = blockIdx.x % w.slices, first = slice * (kThreads * V);
+    __shared__ int found[4], ranks[64];
+    const uint32_t row = blockIdx.x / w.slices, slice = blockIdx.x % w.slices, first = slice * w.logits;
     const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
     const float *x = p.x + (size_t)row * p.stride + first;
-    const uint32_t n = min((uint32_t)(kThreads * V), p.vocab - first);
+    const uint32_t n = min(w.logits, p.vocab - first);
     float v[V];
     auto at = [&](int j) { return (uint32_t)((j / 4 * kThreads + tid) * 4 + j % 4); };
 #pragma unroll
@@ -100,26 +129,52 @@ template <int V> __global__ void __launch_bounds__(kThreads) logprobs_slice_kern
             for (int e = 0; e < 4; e++) v[j + e] = at(j) + e < n ? x[at(j) + e] : -INFINITY;
         }
     }
-    float top = -INFINITY;  // (fmaxf passes over NaN)
+    float own = -INFINITY;  // (fmaxf passes over NaN)
 #pragma unroll
-    for (int j = 0; j < V; j++) top = fmaxf(top, v[j]);
-    u64 own = 0;  // this thread's best, while the best are asked for
-    if (p.k) {
-        uint32_t best = 0;
-#pragma unroll
-        for (int j = V - 1; j >= 0; j--) {
-            if (v[j] != v[j]) v[j] = -INFINITY;
-            if (v[j] == top) best = at(j);
-        }
-        if (best < n) own = key_of(top, first + best);  // (-infinity: the first of its own or none's)
-        columns[wave][lane] = own;
-        if (wave == 0) ranks[lane] = 0;
+    for (int j = 0; j < V; j++) own = fmaxf(own, v[j]);
+    // A value that k logits reach: up to 16 the k-th largest of the 16 rows' (of 16 lanes) largest, up to 48 that of the
+    // 64 quads' largest, past that the least of the rows' ceil(k / 16)-th.  (That alone leaves 50 candidates a slice for k
+    // up to 16 and 70 up to 32, the others k and a few more: 33 x 128256 logits, 5 tokens 13.3 us and 9.5, 20 tokens 14.5
+    // and 12.)
+    const float row_top = row_max(own);
+    const bool by_quads = p.k > 16 && p.k <= 48;
+    if (lane % 16 == 0) rows[wave * 4 + lane / 16] = row_top;
+    if (by_quads) {
+        const float quad = quad_max(own);
+        if (lane % 4 == 0) quads[wave * 16 + lane / 4] = quad;
+    } else if (p.k > 48) {
+        const float low = -row_max(above_in_row(own) < (p.k + 15) / 16 ? -own : -INFINITY);
+        if (lane % 16 == 0) quads[wave * 4 + lane / 16] = low;
     }
-    top = wave_max_f32(top);
-    if (lane == 0) tops[wave] = top;
-    if (tid == 0) found = 0;
+    if (tid < 64) ranks[tid] = 0;
     __syncthreads();
-    top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
+    const float of_row = rows[lane % 16], top = row_max(of_row);
+    float least = -INFINITY;
+    if (by_quads) {
+        const float quad = quads[lane];
+        int above = 0;
+#pragma unroll
+        for (int i = 0; i < 64; i++) above += __uint_as_float((uint32_t)__builtin_amdgcn_readlane((int)__float_as_uint(quad), i)) > quad;
+        least = -wave_max_f32(above < p.k ? -quad : -INFINITY);
+    } else if (p.k > 48) {
+        least = -row_max(-quads[lane % 16]);
+    } else if (p.k) {
+        least = -row_max(above_in_row(of_row) < p.k ? -of_row : -INFINITY);
+    }
+    least = fmaxf(least, -3.402823466e38f);  // finite ones (all of them where a row has none)
+    constexpr int EACH = kCandidates / 4;
+    int have = 0;  // of this wavefront
+    if (p.k && __any(own >= least)) {
+#pragma unroll
+        for (int j = 0; j < V; j++) {
+            const u64 which = __ballot(v[j] >= least);
+            if (!which) continue;
+            const int to = have + __popcll(which & ((1ull << lane) - 1));
+            if (v[j] >= least && to < EACH) candidates[wave * EACH + to] = key_of(v[j], first + at(j));
+            have += __popcll(which);
+        }
+    }
+    if (lane == 0) found[wave] = have;
     double s = 0.0, t = 0.0;
     uint32_t count = 0;
 #pragma unroll
@@ -136,84 +191,88 @@ template <int V> __global__ void __launch_bounds__(kThreads) logprobs_slice_kern
         t += (double)((fmaf(e[0], d[0], e[1] * d[1]) + fmaf(e[2], d[2], e[3] * d[3])) + (fmaf(e[4], d[4], e[5] * d[5]) + fmaf(e[6], d[6], e[7] * d[7])));
     }
     s = wave_sum(s), t = wave_sum(t);
-    for (int d = 1; d < 64; d <<= 1) count += (uint32_t)__shfl_xor((int)count, d);
-    if (lane == 0) sums[0][wave] = s, sums[1][wave] = t, counts[wave] = count;
-    u64 column = 0;
-    if (p.k) {
-        // ranks of the columns' largest, each wavefront against sixteen of them
-        column = max(max(columns[0][lane], columns[1][lane]), max(columns[2][lane], columns[3][lane]));
-        int rank = 0;
-#pragma unroll
-        for (int i = 0; i < 16; i++) {
-            const u64 other = (u64)(uint32_t)__builtin_amdgcn_readlane((int)(column >> 32), 16 * wave + i) << 32 |
-                              (uint32_t)__builtin_amdgcn_readlane((int)column, 16 * wave + i);
-            rank += other > column;
-        }
-        atomicAdd(&ranks[lane], rank);
-    }
+    count = running_sum(count);
+    if (lane == 63) sums[0][wave] = s, sums[1][wave] = t, counts[wave] = count;
     __syncthreads();
     const size_t out = (size_t)row * w.slices + slice;
     if (tid == 0)
         w.sums[out] = {top, counts[0] + counts[1] + counts[2] + counts[3], (sums[0][0] + sums[0][1]) + (sums[0][2] + sums[0][3]),
                        (sums[1][0] + sums[1][1]) + (sums[1][2] + sums[1][3])};
     if (p.k == 0) return;
-    // the k-th of the columns' largest, which k logits reach
-    const u64 here = __ballot(ranks[lane] == p.k - 1 && column);
-    u64 least = 1;
-    if (here) {
-        const int i = __ffsll(here) - 1;
-        least = (u64)(uint32_t)__builtin_amdgcn_readlane((int)(column >> 32), i) << 32 | (uint32_t)__builtin_amdgcn_readlane((int)column, i);
-    }
-    if (own >= least) {
-#pragma unroll
-        for (int j = 0; j < V; j++) {
-            const u64 k = key_of(v[j], first + at(j));
-            if (at(j) < n && k >= least) {
-                const int i = atomicAdd(&found, 1);
-                if (i < kCandidates) candidates[i] = k;
-            }
-        }
-    }
-    __syncthreads();
     u64 *to = w.top + out * p.k;
-    const int c = found;
-    if (c <= kCandidates) {
-        for (int i = c + tid; i < p.k; i += kThreads) to[i] = 0;  // (fewer logits than that)
-        place(candidates, c, p.k, to);
+    const int c0 = found[0], c1 = c0 + found[1], c2 = c1 + found[2], c = c2 + found[3];
+    // the i-th of the wavefronts' candidates
+    auto candidate = [&](int i) { return candidates[i < c0 ? i : i < c1 ? EACH + i - c0 : i < c2 ? 2 * EACH + i - c1 : 3 * EACH + i - c2]; };
+    if (max(max(found[0], found[1]), max(found[2], found[3])) <= EACH) {
+        for (int i = c + tid; i < p.k; i += kThreads) to[i] = 0;  // (fewer than that)
+        if (c <= 64) {  // a lane each, every wavefront against its own
+            const u64 mine = lane < c ? candidate(lane) : 0ull;
+            int rank = 0;
+            for (int j = 0; j < found[wave]; j += 4) {
+                u64 o[4];
+#pragma unroll
+                for (int e = 0; e < 4; e++) o[e] = candidates[wave * EACH + min(j + e, EACH - 1)];
+#pragma unroll
+                for (int e = 0; e < 4; e++) rank += j + e < found[wave] && o[e] > mine;
+            }
+            atomicAdd(&ranks[lane], rank);
+            __syncthreads();
+            if (wave == 0 && lane < c && ranks[lane] < p.k) to[ranks[lane]] = mine;
+            return;
+        }
+        for (int i = tid; i < c; i += kThreads) {
+            const u64 mine = candidate(i);
+            int rank = 0;
+            for (int q = 0; q < 4; q++)
+                for (int j = 0; j < found[q]; j += 8) {
+                    ulonglong2 o[4];
+#pragma unroll
+                    for (int e = 0; e < 4; e++) o[e] = *reinterpret_cast<const ulonglong2 *>(candidates + q * EACH + j + 2 * e);
+#pragma unroll
+                    for (int e = 0; e < 4; e++) rank += (j + 2 * e < found[q] && o[e].x > mine) + (j + 2 * e + 1 < found[q] && o[e].y > mine);
+                }
+            if (rank < p.k) to[rank] = mine;
+        }
         return;
     }
-    // the best crowd a few columns (their places in the slice alike to a multiple of 256): one after the other
+    // many are equal, or the best crowd a few rows of lanes: one after the other
     u64 last = ~0ull;
     for (int i = 0; i < p.k; i++) {
         u64 k = 0;
 #pragma unroll
         for (int j = 0; j < V; j++) {
             const u64 o = key_of(v[j], first + at(j));
-            if (at(j) < n && o > k && o < last) k = o;
+            if (v[j] >= least && o > k && o < last) k = o;
         }
         k = wave_max_key(k);
         __syncthreads();
-        if (lane == 0) columns[0][wave] = k;
+        if (lane == 0) best[wave] = k;
         __syncthreads();
-        last = max(max(columns[0][0], columns[0][1]), max(columns[0][2], columns[0][3]));
+        last = max(max(best[0], best[1]), max(best[2], best[3]));
         if (tid == 0) to[i] = last;
     }
 }
 
 // A workgroup per row.
 __global__ void __launch_bounds__(1024) logprobs_row_kernel(TokenLogprobs p, LogprobsWork w) {
-    __shared__ __align__(16) u64 heads[8][kMaxSlices], candidates[kTop * kMaxSlices], placed[kTop], limits[8];
-    __shared__ double sums[3][2];
+    __shared__ __align__(16) u64 heads[8][kMaxSlices], candidates[kTop * kMaxSlices];
+    __shared__ uint32_t taken[16];
+    __shared__ u64 limits[8];
+    __shared__ double sums[3][2], shared_log;
     __shared__ float tops[2];
     __shared__ int found;
     const uint32_t row = blockIdx.x, n = w.slices;
-    const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
+    const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
     const SliceSums *from = w.sums + (size_t)row * n;
     const u64 *top = w.top + (size_t)row * n * p.k;
     SliceSums own{-INFINITY, 0, 0.0, 0.0};
     if ((uint32_t)tid < n) own = from[tid];
-    const uint32_t token = p.tokens[row];
-    const float given = token < p.vocab ? p.x[(size_t)row * p.stride + token] : 0.f;
+    float given = 0.f;
+    uint32_t token = 0;
+    if (tid == 0) {
+        token = p.tokens[row];
+        if (token < p.vocab) given = p.x[(size_t)row * p.stride + token];
+    }
     // For each j of 1, 2, 4 .. k: of the slices' j-th best the ceil(k / j)-th largest is a value that k logits reach.
     const int group = tid >> 7, j = 1 << group, i = tid & 127;
     if (p.k) {
@@ -221,13 +280,38 @@ __global__ void __launch_bounds__(1024) logprobs_row_kernel(TokenLogprobs p, Log
         if (i == 0) limits[group] = 1;
     }
     if (tid == 0) found = 0;
-    if (tid < 64 * 2) {
+    if (wave < 2) {
         const float m = wave_max_f32(own.top);
         if (lane == 0) tops[wave] = m;
     }
     __syncthreads();
     const float largest = fmaxf(tops[0], tops[1]);
-    if (tid < 64 * 2) {
+    if (j <= p.k) {
+        const u64 mine = heads[group][i];
+        int rank = 0;
+        for (uint32_t o = 0; o < n; o += 8) {  // (those behind the last are 0)
+            ulonglong2 other[4];
+#pragma unroll
+            for (int e = 0; e < 4; e++) other[e] = *reinterpret_cast<const ulonglong2 *>(&heads[group][o + 2 * e]);
+#pragma unroll
+            for (int e = 0; e < 4; e++) rank += (other[e].x > mine) + (other[e].y > mine);
+        }
+        if (mine && rank == (p.k + j - 1) / j - 1) limits[group] = mine;
+    }
+    __syncthreads();
+    if (wave >= 2 && p.k) {
+        u64 least = 1;
+#pragma unroll
+        for (int g = 0; g < 8; g++) least = max(least, limits[g]);
+        // a slice's are in order: eight lanes take a slice until one falls below
+        for (uint32_t a = (uint32_t)(tid - 128) / 8; a < n; a += 112)
+            for (int b = tid & 7; b < p.k; b += 8) {
+                const u64 k = top[(size_t)a * p.k + b];
+                if (k < least) break;
+                candidates[atomicAdd(&found, 1)] = k;
+            }
+    }
+    if (wave < 2) {  // meanwhile the sums
         // slices that have the largest give its count, the others their weights
         double s = own.s, t = own.t, count = own.top == largest ? (double)own.count : 0.0;
         if (own.top != largest) {
@@ -237,50 +321,53 @@ __global__ void __launch_bounds__(1024) logprobs_row_kernel(TokenLogprobs p, Log
         s = wave_sum(s), t = wave_sum(t), count = wave_sum(count);
         if (lane == 0) sums[0][wave] = s, sums[1][wave] = t, sums[2][wave] = count;
     }
-    if (j <= p.k) {
-        const u64 mine = heads[group][i];
-        int rank = 0;
-        for (uint32_t o = 0; o < n; o += 2) {  // (those behind the last are 0)
-            const ulonglong2 other = *reinterpret_cast<const ulonglong2 *>(&heads[group][o]);
-            rank += (other.x > mine) + (other.y > mine);
-        }
-        if (mine && rank == (p.k + j - 1) / j - 1) limits[group] = mine;
-    }
     __syncthreads();
-    const double s = (sums[0][0] + sums[0][1]) + (sums[2][0] + sums[2][1] - 1.0), t = sums[1][0] + sums[1][1], nan = (double)__uint_as_float(0x7FC00000u);
-    const double log_s = isfinite(largest) ? log1p(s) : nan;
-    auto logprob = [&](float v) { return (float)(((double)(v != v ? -INFINITY : v) - (double)largest) - log_s); };
-    if (tid == 0) {
-        p.out[row] = token < p.vocab ? logprob(given) : (float)nan;
-        if (p.entropy) p.entropy[row] = (float)(log_s - t / (1.0 + s));
+    auto logprob = [&](float v, double log_s) { return (float)(((double)(v != v ? -INFINITY : v) - (double)largest) - log_s); };
+    if (wave == 0) {
+        const double s = (sums[0][0] + sums[0][1]) + (sums[2][0] + sums[2][1] - 1.0), t = sums[1][0] + sums[1][1], nan = (double)__uint_as_float(0x7FC00000u);
+        const double log_s = isfinite(largest) ? log1p(s) : nan;
+        if (lane == 0) {
+            shared_log = log_s;
+            p.out[row] = token < p.vocab ? logprob(given, log_s) : (float)nan;
+            if (p.entropy) p.entropy[row] = (float)(log_s - t / (1.0 + s));
+        }
     }
     if (p.k == 0) return;
-    u64 least = 1;
-#pragma unroll
-    for (int g = 0; g < 8; g++) least = max(least, limits[g]);
-    // a slice's are in order: an eighth of a wavefront takes a slice until one falls below
-    for (uint32_t a = (uint32_t)tid / 8; a < n; a += 128)
-        for (int b = tid & 7; b < p.k; b += 8) {
-            const u64 k = top[(size_t)a * p.k + b];
-            if (k < least) break;
-            candidates[atomicAdd(&found, 1)] = k;
+    __syncthreads();
+    const double log_s = shared_log;
+    place(candidates, found, p.k, [&](int rank, u64 k) {
+        p.top_tokens[(size_t)row * p.k + rank] = index_of_key(k);
+        p.top[(size_t)row * p.k + rank] = logprob(value_of_key(k), log_s);
+    });
+    // fewer finite logits than k: all of them are placed, +infinities too; the first of the others follow
+    uint32_t have = (uint32_t)found;
+    for (uint32_t at = 0; have < (uint32_t)p.k && at < p.vocab; at += 1024) {
+        const float v = at + tid < p.vocab ? p.x[(size_t)row * p.stride + at + tid] : 0.f;
+        const bool none = at + tid < p.vocab && (v != v || v == -INFINITY);
+        const u64 which = __ballot(none);
+        __syncthreads();
+        if (lane == 0) taken[wave] = (uint32_t)__popcll(which);
+        __syncthreads();
+        uint32_t rank = have + (uint32_t)__popcll(which & ((1ull << lane) - 1)), all = 0;
+        for (int i = 0; i < 16; i++) rank += i < wave ? taken[i] : 0u, all += taken[i];
+        if (none && rank < (uint32_t)p.k) {
+            p.top_tokens[(size_t)row * p.k + rank] = at + tid;
+            p.top[(size_t)row * p.k + rank] = logprob(-INFINITY, log_s);
         }
-    __syncthreads();
-    place(candidates, found, p.k, placed);
-    __syncthreads();
-    if (tid < p.k) {
-        p.top_tokens[(size_t)row * p.k + tid] = index_of_key(placed[tid]);
-        p.top[(size_t)row * p.k + tid] = logprob(value_of_key(placed[tid]));
+        have += all;
     }
 }
 
 }  // namespace
 
 hipError_t launch_token_logprobs(const TokenLogprobs &a, int cus, hipStream_t s) {
-    // slices of 2048 logits fill the device while there are up to 16 workgroups a CU of them
-    const bool wide = (uint64_t)a.rows * ((a.vocab + 2047) / 2048) > 16ull * cus;
+    // The fewer workgroups the rows make, the smaller their slices: 2048 logits up to 4 workgroups a CU, 4096 up to 16.
+    auto wgs = [&](uint32_t slice) { return (uint64_t)a.rows * ((a.vocab + slice - 1) / slice); };
+    const uint32_t slice = wgs(2048) <= 4ull * cus ? 2048 : wgs(4096) <= 16ull * cus ? 4096 : 8192;
     LogprobsWork w{};
-    w.slices = wide ? (a.vocab + 8191) / 8192 : (a.vocab + 2047) / 2048;
+    w.slices = (a.vocab + slice - 1) / slice;
+    w.logits = ((a.vocab + w.slices - 1) / w.slices + 3) / 4 * 4;  // alike, so that the last one's lanes aren't mostly empty
+    w.slices = (a.vocab + w.logits - 1) / w.logits;
     const size_t each = w.slices * (sizeof(SliceSums) + 8 * (size_t)a.k);
     const uint32_t most = (uint32_t)std::min<size_t>(a.work_bytes / each, 0x7FFFFFFFu / w.slices);
     TokenLogprobs p = a;
@@ -291,7 +378,8 @@ hipError_t launch_token_logprobs(const TokenLogprobs &a, int cus, hipStream_t s)
         if (a.k) p.top = a.top + (size_t)r * a.k, p.top_tokens = a.top_tokens + (size_t)r * a.k;
         w.sums = (SliceSums *)a.work, w.top = (u64 *)(w.sums + (size_t)p.rows * w.slices);
         const dim3 grid(p.rows * w.slices);
-        if (wide) hipLaunchKernelGGL(logprobs_slice_kernel<32>, grid, dim3(kThreads), 0, s, p, w);
+        if (slice == 8192) hipLaunchKernelGGL(logprobs_slice_kernel<32>, grid, dim3(kThreads), 0, s, p, w);
+        else if (slice == 4096) hipLaunchKernelGGL(logprobs_slice_kernel<16>, grid, dim3(kThreads), 0, s, p, w);
         else hipLaunchKernelGGL(logprobs_slice_kernel<8>, grid, dim3(kThreads), 0, s, p, w);
         hipLaunchKernelGGL(logprobs_row_kernel, dim3(p.rows), dim3(1024), 0, s, p, w);
     }

@@ -36,6 +36,7 @@ struct Kv4Params {
     uint32_t few;       // columns up to which a sequence is the few-column kernel's (0: none is)
     uint32_t wgs;       // few: workgroups to spread the blocks over
     int splits;         // many: of each tile's positions
+    uint32_t *plan;     // of more than 64 sequences: see Plan
     float *part;        // partial outputs, and {maximum, sum} of each
     float2 *part_ml;
 };
@@ -72,32 +73,50 @@ __device__ __forceinline__ Sequence uniform(const Sequence &q) {
     return {uniform(q.index), uniform(q.row0), uniform(q.rows), (int)uniform((uint32_t)q.first)};
 }
 
+// Of more than 64 sequences a kernel of its own makes a table, which the others search: for each sequence the end of its
+// items among the few-column kernel's and of its tiles among the other's, and the slot of its first split.  (Up to 64 every
+// wavefront has a sequence a lane, and a table would cost a launch.)
+struct Plan {
+    const uint32_t *quota, *items, *tiles, *slots;
+    __host__ __device__ static size_t words(uint32_t sequences) { return 4 + 3 * (size_t)sequences; }
+    __device__ __forceinline__ explicit Plan(const Kv4Params &p)
+        : quota(p.plan), items(p.plan + 4), tiles(items + p.b.sequences), slots(tiles + p.b.sequences) {}
+};
+constexpr uint32_t kLanes = 64;
+
 // A tile of columns (a sequence's rows' heads of one kv head, row by row), by its number among those of the sequences
 // with more than `few` columns; count 0: none.  Every lane of a wavefront takes part.
 struct Tile {
     Sequence q;
     uint32_t first, count;  // columns
 };
+template <int COLUMNS> __device__ __forceinline__ uint32_t tiles_of(const Kv4Params &p, uint32_t columns) {
+    return columns > p.few ? (columns + COLUMNS - 1) / COLUMNS : 0u;
+}
 template <int COLUMNS> __device__ __forceinline__ Tile tile_of(const Kv4Params &p, uint32_t number) {
     Tile t{};
     const uint32_t lane = threadIdx.x & 63, group = (uint32_t)p.group;
-    uint32_t before = 0;
-    for (uint32_t from = 0; from < p.b.sequences; from += 64) {
-        uint32_t n = 0;
-        if (from + lane < p.b.sequences) n = sequence_of(p.b, from + lane).rows * group;
-        n = n > p.few ? (n + COLUMNS - 1) / COLUMNS : 0u;
-        const uint32_t sum = running_sum(n);
-        const u64 past = __ballot(before + sum > number);
-        if (past) {
-            const int at = __ffsll(past) - 1;
-            t.q = uniform(sequence_of(p.b, from + at));
-            t.first = (number - before - (uint32_t)__builtin_amdgcn_readlane((int)(sum - n), at)) * COLUMNS;
-            const uint32_t all = t.q.rows * group;  // (tables that don't ascend may pass 32 bits in the sums)
-            t.count = t.first < all ? min((uint32_t)COLUMNS, all - t.first) : 0u;
-            return t;
-        }
-        before += (uint32_t)__builtin_amdgcn_readlane((int)sum, 63);
+    uint32_t before;
+    if (p.b.sequences > kLanes) {
+        const Plan plan(p);
+        const uint32_t s = count_up_to(plan.tiles, p.b.sequences, number);
+        if (s >= p.b.sequences) return t;
+        t.q = uniform(sequence_of(p.b, s));
+        before = s ? uniform(plan.tiles[s - 1]) : 0u;
+    } else {
+        Sequence q{};
+        if (lane < p.b.sequences) q = sequence_of(p.b, lane);
+        const uint32_t n = tiles_of<COLUMNS>(p, q.rows * group), sum = running_sum(n);
+        const u64 past = __ballot(sum > number);
+        if (!past) return t;
+        const int at = __ffsll(past) - 1;
+        auto of = [&](uint32_t v) { return (uint32_t)__builtin_amdgcn_readlane((int)v, at); };
+        t.q = {of(q.index), of(q.row0), of(q.rows), (int)of((uint32_t)q.first)};
+        before = of(sum - n);
     }
+    t.first = (number - before) * COLUMNS;
+    const uint32_t all = t.q.rows * group;  // (tables that don't ascend may pass 32 bits in the sums)
+    t.count = number >= before && t.first < all ? min((uint32_t)COLUMNS, all - t.first) : 0u;
     return t;
 }
 
@@ -113,48 +132,105 @@ struct Share {
 };
 constexpr uint32_t kFewWaves = 4, kLeastBlocks = kFewWaves;  // of a workgroup: one for each wavefront
 
-// The item with this number, or (by_sequence) the sequence.  Every lane of a wavefront takes part.
+// A sequence's tiles, and its blocks (of all columns: a tile's own are no more).
+template <int COLUMNS> __device__ __forceinline__ void load_of(const Kv4Params &p, const Sequence &q, uint32_t &tiles, uint32_t &blocks) {
+    const uint32_t columns = q.rows * p.group;
+    tiles = blocks = 0;
+    if (columns == 0 || columns > p.few) return;
+    const Range r = range_of(p, q, 0, q.rows - 1);
+    tiles = (columns + COLUMNS - 1) / COLUMNS;
+    blocks = max((uint32_t)(r.end - r.begin), 1u);  // rows that see nothing have an item, which writes zeros
+}
+__device__ __forceinline__ uint32_t quota_of(const Kv4Params &p, u64 total) {
+    return max(kLeastBlocks, (uint32_t)ceil((double)total * p.c.nkv / p.wgs));
+}
+
+// The item with this number, or (BY_SEQUENCE) the sequence.  Every lane of a wavefront takes part.
 template <bool BY_SEQUENCE, int COLUMNS> __device__ __forceinline__ Share share_of(const Kv4Params &p, uint32_t number) {
     const uint32_t lane = threadIdx.x & 63, nkv = (uint32_t)p.c.nkv;
-    auto of = [](uint32_t v, int at) { return (uint32_t)__builtin_amdgcn_readlane((int)v, at); };
-    // this lane's sequence, its tiles and blocks (of all columns: a tile's own are no more)
-    Sequence q{};
-    uint32_t tiles = 0, blocks = 0;
-    auto look = [&](uint32_t s) {
-        q.rows = tiles = blocks = 0;
-        if (s >= p.b.sequences) return;
-        q = sequence_of(p.b, s);
-        const uint32_t columns = q.rows * p.group;
-        if (columns == 0 || columns > p.few) return;
-        const Range r = range_of(p, q, 0, q.rows - 1);
-        tiles = (columns + COLUMNS - 1) / COLUMNS;
-        blocks = max((uint32_t)(r.end - r.begin), 1u);  // rows that see nothing have an item, which writes zeros
-    };
-    look(lane);
-    u64 total = (u64)blocks * tiles;
-    for (uint32_t from = 64; from < p.b.sequences; from += 64) look(from + lane), total += (u64)blocks * tiles;
-    if (p.b.sequences > 64) look(lane);
-    total = running_sum(total);
-    total = (u64)of((uint32_t)(total >> 32), 63) << 32 | of((uint32_t)total, 63);
-    const uint32_t quota = uniform(max(kLeastBlocks, (uint32_t)ceil((double)total * nkv / p.wgs)));
     Share t{};
-    uint32_t items = 0, slots = 0;
-    for (uint32_t from = 0; from < p.b.sequences; from += 64) {
-        if (from) look(from + lane);
-        const uint32_t splits = (blocks + quota - 1) / quota, n = splits * tiles * nkv;
-        const uint32_t sum = running_sum(n), slot_sum = running_sum(splits > 1 ? n : 0u);
-        const u64 past = __ballot(BY_SEQUENCE ? from + lane == number : items + sum > number);
-        if (past) {
-            const int at = __ffsll(past) - 1;
-            t.q = {of(q.index, at), of(q.row0, at), of(q.rows, at), (int)of((uint32_t)q.first, at)};
-            t.splits = of(splits, at), t.tiles = of(tiles, at);
-            t.index = number - items - of(sum - n, at);
-            t.slot = slots + of(slot_sum, at) - (t.splits > 1 ? t.splits * t.tiles * nkv : 0u);
-            return t;
-        }
-        items += of(sum, 63), slots += of(slot_sum, 63);
+    if (p.b.sequences > kLanes) {
+        const Plan plan(p);
+        const uint32_t s = BY_SEQUENCE ? number : count_up_to(plan.items, p.b.sequences, number);
+        if (s >= p.b.sequences) return t;
+        t.q = uniform(sequence_of(p.b, s));
+        uint32_t blocks;
+        load_of<COLUMNS>(p, t.q, t.tiles, blocks);
+        const uint32_t quota = uniform(plan.quota[0]);
+        t.splits = (blocks + quota - 1) / quota;
+        t.index = number - (s ? uniform(plan.items[s - 1]) : 0u);
+        if (!BY_SEQUENCE && t.index >= t.splits * t.tiles * nkv) t.splits = 0;  // (tables that changed on the way)
+        t.slot = uniform(plan.slots[s]);
+        return t;
     }
+    auto of = [](uint32_t v, int at) { return (uint32_t)__builtin_amdgcn_readlane((int)v, at); };
+    Sequence q{};  // a lane's
+    uint32_t tiles = 0, blocks = 0;
+    if (lane < p.b.sequences) q = sequence_of(p.b, lane), load_of<COLUMNS>(p, q, tiles, blocks);
+    u64 total = running_sum((u64)blocks * tiles);
+    total = (u64)of((uint32_t)(total >> 32), 63) << 32 | of((uint32_t)total, 63);
+    const uint32_t quota = uniform(quota_of(p, total)), splits = (blocks + quota - 1) / quota, n = splits * tiles * nkv;
+    const uint32_t sum = running_sum(n), slot_sum = running_sum(splits > 1 ? n : 0u);
+    const u64 past = __ballot(BY_SEQUENCE ? lane == number : sum > number);
+    if (!past) return t;
+    const int at = __ffsll(past) - 1;
+    t.q = {of(q.index, at), of(q.row0, at), of(q.rows, at), (int)of((uint32_t)q.first, at)};
+    t.splits = of(splits, at), t.tiles = of(tiles, at);
+    t.index = number - of(sum - n, at);
+    t.slot = of(slot_sum, at) - (t.splits > 1 ? t.splits * t.tiles * nkv : 0u);
     return t;
+}
+
+// The table of more than 64 sequences: one workgroup, 1024 sequences at a time.
+template <int FEW, int MANY> __global__ void __launch_bounds__(1024) kv4_plan_kernel(Kv4Params p) {
+    __shared__ u64 totals[16];
+    __shared__ uint32_t sums[3][16];
+    const Plan plan(p);
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    uint32_t tiles, blocks;
+    auto look = [&](uint32_t s, Sequence &q) {
+        q.rows = tiles = blocks = 0;
+        if (s < p.b.sequences) q = sequence_of(p.b, s), load_of<FEW>(p, q, tiles, blocks);
+    };
+    u64 total = 0;
+    for (uint32_t s = threadIdx.x; s < p.b.sequences; s += 1024) {
+        Sequence q;
+        look(s, q);
+        total += (u64)blocks * tiles;
+    }
+    total = running_sum(total);
+    if (lane == 63) totals[wave] = total;
+    __syncthreads();
+    total = 0;
+    for (int i = 0; i < 16; i++) total += totals[i];
+    const uint32_t quota = quota_of(p, total);
+    if (threadIdx.x == 0) p.plan[0] = quota;
+    uint32_t before[3] = {};
+    for (uint32_t from = 0; from < p.b.sequences; from += 1024) {
+        const uint32_t s = from + threadIdx.x;
+        Sequence q;
+        look(s, q);
+        const uint32_t splits = (blocks + quota - 1) / quota, n = splits * tiles * p.c.nkv;
+        const uint32_t own[3] = {n, tiles_of<MANY>(p, q.rows * p.group), splits > 1 ? n : 0u};
+        uint32_t sum[3];
+        for (int k = 0; k < 3; k++) {
+            sum[k] = running_sum(own[k]);
+            if (lane == 63) sums[k][wave] = sum[k];
+        }
+        __syncthreads();
+        for (int k = 0; k < 3; k++) {
+            uint32_t all = 0, ahead = 0;
+            for (int i = 0; i < 16; i++) ahead += i < wave ? sums[k][i] : 0u, all += sums[k][i];
+            sum[k] += before[k] + ahead;
+            before[k] += all;
+        }
+        if (s < p.b.sequences) {
+            const_cast<uint32_t *>(plan.items)[s] = sum[0];
+            const_cast<uint32_t *>(plan.tiles)[s] = sum[1];
+            const_cast<uint32_t *>(plan.slots)[s] = sum[2] - own[2];
+        }
+        __syncthreads();
+    }
 }
 
 __device__ __forceinline__ uint32_t cut(float v) { return __float_as_uint(v) & 0xFFFF0000u; }
@@ -324,9 +400,9 @@ template <int HD, int CT, int AWAY, bool PACKED = false> struct Columns {
     }
 
     // 32 H positions from `at` on, key(h, t, pt) and values(h, t, b) their operands.  edge: some columns may not see all of
-    // them (hidden: their page is none).  after_k, after_w: the keys are through, the scores are.
-    template <int H, bool HOLD, class K, class V, class A, class B>
-    __device__ __forceinline__ void take(float qscale, int at, bool edge, bool hidden, K key, V values, A after_k, B after_w) {
+    // them (hidden: their page is none).  after_w: runs when the scores are through.
+    template <int H, bool HOLD, class K, class V, class B>
+    __device__ __forceinline__ void take(float qscale, int at, bool edge, bool hidden, K key, V values, B after_w) {
         const int g = threadIdx.x >> 4 & 3;
         // of a weight, lane i % 4 = 1 takes off the first piece, 2 the second too (3 as well: its outputs are left out)
         const float second = PACKED && (threadIdx.x & 3) > 0 ? -1.f : 0.f, third = PACKED && (threadIdx.x & 3) > 1 ? -1.f : 0.f;
@@ -355,7 +431,6 @@ template <int HD, int CT, int AWAY, bool PACKED = false> struct Columns {
                 if constexpr (HOLD) __builtin_amdgcn_sched_barrier(0);  // (or the operands of all steps take registers at once)
             }
         }
-        after_k();
         if constexpr (PACKED) {
 #pragma unroll
             for (int h = 0; h < H; h++)
@@ -470,7 +545,7 @@ template <int HD, int CT, int AWAY, bool PACKED = false> struct Columns {
             const uint32_t next = page(j);
             after.load_k(p.c, next, head, half(j)), after.load_v(p.c, next, head, half(j));
             if (edge) now.clear_v(r.first - at(i), hidden ? -1 : r.last - at(i));
-            take<1, HOLD>(p.qscale, at(i), edge, hidden, [&](int, int t, int pt) { return now.key(t, pt); }, [&](int, int t, fb8(&b)[2]) { now.values(t, b); }, [] {}, [] {});
+            take<1, HOLD>(p.qscale, at(i), edge, hidden, [&](int, int t, int pt) { return now.key(t, pt); }, [&](int, int t, fb8(&b)[2]) { now.values(t, b); }, [] {});
             i++;
         };
         while (i < n) {
@@ -645,10 +720,9 @@ template <int HD> struct Quarter {  // wavefront (half h, pt): K rows of half h,
     }
 };
 
-template <int HD, int CT, int AWAY> __global__ void __launch_bounds__(256, 2) kv4_many_kernel(Kv4Params p) {
+template <int HD, int CT> __global__ void __launch_bounds__(256, 2) kv4_many_kernel(Kv4Params p) {
     constexpr int G = HD / 32, PAGE = 8 * G * 64;  // a page's operands
     __shared__ fb8 pages[2][PAGE];
-    __shared__ fb8 held[AWAY ? 4 : 1][AWAY ? CT * G * AWAY * 64 : 1];
     const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), i = threadIdx.x & 15, g = threadIdx.x >> 4 & 3, lane = threadIdx.x & 63;
     const int head = (int)(blockIdx.x % p.c.nkv);
     const Tile t = tile_of<64 * CT>(p, (gridDim.x - 1 - blockIdx.x) / p.c.nkv);  // the longest (last) first
@@ -656,9 +730,9 @@ template <int HD, int CT, int AWAY> __global__ void __launch_bounds__(256, 2) kv
     const Range r = range_of(p, t.q, t.first / p.group, (t.first + t.count - 1) / p.group);
     int begin = r.begin / 2, end = r.end > r.begin ? (r.end + 1) / 2 : r.begin / 2;
     share(begin, end, (uint32_t)p.splits, blockIdx.y);
-    Columns<HD, CT, AWAY> x;
+    Columns<HD, CT, 0> x;
     const uint32_t first = t.first + 16 * CT * wave;
-    typename Columns<HD, CT, AWAY>::Raw raw;
+    typename Columns<HD, CT, 0>::Raw raw;
     x.fetch(p, t.q, min(first, t.first + t.count - 1), first < t.first + t.count ? t.first + t.count - first : 1, head, raw);
     uint32_t ids = 0;  // of the next 64 pages, one a lane; those that the pool doesn't have: 0, not seen
     u64 missing = 0;
@@ -675,7 +749,7 @@ template <int HD, int CT, int AWAY> __global__ void __launch_bounds__(256, 2) kv
         look(begin);
         y.load(p.c, id(begin), head, wave);
     }
-    x.begin(p, raw, held[AWAY ? wave : 0]);
+    x.begin(p, raw, nullptr);
     for (int n = begin; n < end; n++) {
         const int at = n * kPage;
         const bool hidden = missing >> ((n - begin) & 63) & 1, edge = hidden || at < r.full_first || at + kPage - 1 > r.full_last;
@@ -692,7 +766,7 @@ template <int HD, int CT, int AWAY> __global__ void __launch_bounds__(256, 2) kv
                                       const fb8 *v = page + (4 * G + 2 * G * h + 2 * t) * 64 + lane;
                                       b[0] = v[0], b[1] = v[64];
                                   },
-                                  [] {}, [&] { y.load(p.c, id(min(n + 1, end - 1)), head, wave); });
+                                  [&] { y.load(p.c, id(min(n + 1, end - 1)), head, wave); });
     }
 #pragma unroll
     for (int c = 0; c < CT; c++) {
@@ -739,22 +813,31 @@ hipError_t launch_kv4_attention(const Kv4Attn &a, int cus, hipStream_t s) {
     p.c = a.c, p.b = a.b, p.q = a.q, p.q_stride = a.q_stride, p.out = a.out;
     p.heads = a.heads, p.group = a.heads / a.c.nkv, p.q_aligned = a.q_aligned;
     p.window = a.window, p.qscale = a.qscale, p.qsign = a.qsign;
-    p.part = a.part;
     const uint64_t nkv = a.c.nkv, most = (uint64_t)a.b.max_rows * p.group, all = (uint64_t)a.b.rows * p.group;
     const uint64_t blocks = (a.b.cap + kBlock - 1) / kBlock;  // of a sequence, at most
     const uint32_t limit = a.c.hd <= 128 ? 64 : 32;
     // a batch of one sequence is one kernel's; others may hold sequences of both kinds
     p.few = a.b.sequences == 1 && most > limit ? 0 : limit;
-    auto few = [&](auto h, auto tiles, auto packed) {
+    const bool planned = a.b.sequences > kLanes;
+    p.plan = (uint32_t *)a.part;
+    const size_t plan_floats = planned ? (Plan::words(a.b.sequences) + 3) / 4 * 4 : 0;
+    if (a.part_floats < plan_floats + 4 * 64 * 260) return hipErrorInvalidValue;
+    p.part = a.part + plan_floats;
+    const size_t part_floats = a.part_floats - plan_floats;
+    auto plan = [&](auto f, auto m) {
+        if (planned) hipLaunchKernelGGL((kv4_plan_kernel<decltype(f)::value, decltype(m)::value>), dim3(1), dim3(1024), 0, s, p);
+    };
+    auto few = [&](auto h, auto tiles, auto packed, auto prompt) {
         constexpr int HD = decltype(h)::value, CT = decltype(tiles)::value;
         constexpr bool PACKED = decltype(packed)::value;
         constexpr uint64_t N = PACKED ? 4 : 16 * CT;
         p.wgs = 2 * cus;
-        while (p.wgs > 1 && 2 * p.wgs * N * (HD + 2) > a.part_floats) p.wgs /= 2;
+        while (p.wgs > 1 && 2 * p.wgs * N * (HD + 2) > part_floats) p.wgs /= 2;
         p.part_ml = (float2 *)(p.part + (size_t)2 * p.wgs * N * HD);
         const uint64_t columns = std::min<uint64_t>(most, limit), tiles_of = (columns + N - 1) / N;
         const uint64_t per = (blocks + kLeastBlocks - 1) / kLeastBlocks, all_tiles = a.b.sequences * nkv * tiles_of;  // splits of a tile, and tiles, at most
         const uint64_t items = std::min(p.wgs + all_tiles, all_tiles * per);
+        plan(std::integral_constant<int, (int)N>{}, std::integral_constant<int, 64 * decltype(prompt)::value>{});
         hipLaunchKernelGGL((kv4_few_kernel<HD, CT, PACKED>), dim3((unsigned)items), dim3(64 * kFewWaves), 0, s, p);
         if (per == 1) return;
         const dim3 join((unsigned)(a.b.sequences * nkv), (unsigned)std::min<uint64_t>(columns, std::max<uint64_t>(1, 1024 / (a.b.sequences * nkv))));
@@ -764,16 +847,16 @@ hipError_t launch_kv4_attention(const Kv4Attn &a, int cus, hipStream_t s) {
         constexpr int HD = decltype(h)::value, CT = decltype(tiles)::value;
         const uint64_t n = std::min<uint64_t>(all / (64 * CT) + a.b.sequences, all), wgs = n * nkv;
         const uint64_t each = (uint64_t)a.b.rows * a.heads * (HD + 2);
-        p.splits = (int)std::max<uint64_t>(1, std::min<uint64_t>({2 * (uint64_t)cus / wgs, blocks / 8, a.part_floats / each}));
+        p.splits = (int)std::max<uint64_t>(1, std::min<uint64_t>({2 * (uint64_t)cus / wgs, blocks / 8, part_floats / each}));
         p.part_ml = (float2 *)(p.part + (size_t)p.splits * a.b.rows * a.heads * HD);
-        hipLaunchKernelGGL((kv4_many_kernel<HD, CT, 0>), dim3((unsigned)wgs, (unsigned)p.splits), dim3(256), 0, s, p);
+        hipLaunchKernelGGL((kv4_many_kernel<HD, CT>), dim3((unsigned)wgs, (unsigned)p.splits), dim3(256), 0, s, p);
         if (p.splits > 1)
             hipLaunchKernelGGL((kv4_many_join_kernel<HD>), dim3(a.b.rows, (a.heads * (HD / 4) + 255) / 256), dim3(256), 0, s, p);
     };
     auto go = [&](auto h, auto one, auto more, auto prompt) {
-        if (p.few && most <= 4) few(h, one, std::true_type{});
-        else if (p.few && most <= 16) few(h, one, std::false_type{});
-        else if (p.few) few(h, more, std::false_type{});
+        if (p.few && most <= 4) few(h, one, std::true_type{}, prompt);
+        else if (p.few && most <= 16) few(h, one, std::false_type{}, prompt);
+        else if (p.few) few(h, more, std::false_type{}, prompt);
         if (most > p.few) many(h, prompt);
     };
     if (a.b.sequences * nkv * 8 > 0x7FFFFFFFu || (all / 16 + a.b.sequences + 4) * nkv > 0x7FFFFFFFu) return hipErrorInvalidValue;

@@ -31,20 +31,38 @@ __device__ __forceinline__ Sequence sequence_of(const Batch &b, uint32_t s) {
     q.first = (int)(n < 0x7FFFFFFFu ? n : 0x7FFFFFFFu) - (int)all;
     return q;
 }
+// How many of the ascending values at ends[0 .. n - 1] are at most r, 64 probes at a time.  Every lane takes part; what
+// does not ascend gives some number from 0 to n.
+__device__ __forceinline__ uint32_t count_up_to(const uint32_t *ends, uint32_t n, uint32_t r) {
+    const uint32_t lane = threadIdx.x & 63;
+    uint32_t base = 0;
+    while (n > 0) {
+        const uint32_t step = (n + 63) / 64, at = (lane + 1) * step;  // the lane's probe is the last of its step
+        const uint32_t c = (uint32_t)__popcll(__ballot(at <= n && ends[base + min(at, n) - 1] <= r));
+        if (step == 1) return base + c;
+        base += c * step;
+        n = min(step, n - c * step);
+    }
+    return base;
+}
+
 // The sequence that row r belongs to; rows 0: none.  Every lane of a wavefront takes part.
 __device__ __forceinline__ Sequence sequence_of_row(const Batch &b, uint32_t r) {
     Sequence q{};
     const int lane = threadIdx.x & 63;
-    for (uint32_t from = 0; from < b.sequences; from += 64) {
-        Sequence own{};  // this lane's sequence
+    auto of = [&](uint32_t v, int at) { return (uint32_t)__builtin_amdgcn_readlane((int)v, at); };
+    if (b.sequences <= 64) {  // every lane a sequence, one round of loads
+        Sequence own{};
         uint32_t end = 0xFFFFFFFFu;
-        if (from + lane < b.sequences) own = sequence_of(b, from + lane), end = b.starts[from + lane + 1];
+        if ((uint32_t)lane < b.sequences) own = sequence_of(b, lane), end = b.starts[lane + 1];
         const unsigned long long below = __ballot(end <= r);  // sequences that end ahead of r: the first ones
-        if (!~below) continue;
+        if (!~below) return q;
         const int at = __popcll(below);
-        auto of = [&](uint32_t v) { return (uint32_t)__builtin_amdgcn_readlane((int)v, at); };
-        q = {of(own.index), of(own.row0), of(own.rows), (int)of((uint32_t)own.first)};
-        break;
+        if (at < 64) q = {of(own.index, at), of(own.row0, at), of(own.rows, at), (int)of((uint32_t)own.first, at)};
+    } else {
+        const uint32_t s = count_up_to(b.starts + 1, b.sequences, r);
+        if (s < b.sequences) q = sequence_of(b, s);
+        q = {of(q.index, 0), of(q.row0, 0), of(q.rows, 0), (int)of((uint32_t)q.first, 0)};
     }
     if (r < q.row0 || r - q.row0 >= q.rows) q.rows = 0;
     return q;

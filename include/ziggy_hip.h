@@ -420,16 +420,19 @@ int ziggy_hip_kv8_attention_f32(ZiggyHipContext *ctx, const ZiggyHipKv8Cache *ca
  * sequence's are no one's: what a call would write of them stays as it was.
  * max_rows and max_length: what no sequence has more rows and positions than
  * (0: `rows`, and all that its pages hold); the kernels' grids follow them, so
- * tight ones are faster.  Rows and positions past them, rows ahead of position
- * 0, and positions whose page is not one of the pool's are passed over: not
- * stored, and not attended to.  A sequence's pages are its own while its rows
- * are appended; sequences may share pages that are only read. */
+ * tight ones are faster.  Positions past max_length, and positions whose page
+ * is not one of the pool's, are passed over: not stored, not read back, and
+ * not attended to.  Rows past max_rows are no one's, as those behind the last
+ * sequence; so are rows ahead of position 0 (more rows than positions), but
+ * that the attention gives them zeros.  The tables stay as they are while a
+ * call runs.  A sequence's pages are its own while its rows are appended;
+ * sequences may share pages that are only read. */
 typedef struct {
     const ZiggyHipBuffer *page_table; /* u32 [sequences][pages_per_sequence]; entries past a sequence's length are not read */
     const ZiggyHipBuffer *row_starts; /* u32 [sequences + 1], ascending */
     const ZiggyHipBuffer *lengths;    /* u32 [sequences] */
     uint32_t sequences, pages_per_sequence; /* at most 65536, and 2^24 pages */
-    uint32_t rows;                    /* rows of the step's inputs and outputs */
+    uint32_t rows;                    /* rows of the step's inputs and outputs, at most 2^25 */
     uint32_t max_rows, max_length;
 } ZiggyHipBatch;
 
@@ -447,7 +450,7 @@ typedef struct {
  * with q_norm, the k_heads behind them with k_norm, as
  * ziggy_hip_rms_norm_per_head_f32 and ziggy_hip_rope_rows_f32 one after the
  * other (positions, strides, offsets and in-place rows as there).  heads->rope
- * is not NULL. */
+ * is not NULL; at most 2^25 rows. */
 int ziggy_hip_norm_rope_rows_f32(ZiggyHipContext *ctx, const ZiggyHipHeadsDesc *heads, const ZiggyHipBuffer *src,
                                  size_t src_offset_bytes, size_t src_row_stride, ZiggyHipBuffer *dst,
                                  size_t dst_offset_bytes, size_t dst_row_stride, const ZiggyHipBuffer *positions,
@@ -481,15 +484,17 @@ size_t ziggy_hip_kv4_scales_length(uint32_t layers, uint32_t head_count_kv, uint
  * from v_offset_bytes on.  With q_heads > 0 the query heads of the same rows,
  * from q_offset_bytes on, are normalised and rotated on the way, into q_out
  * (q_out_row_stride apart from q_out_offset_bytes on; src itself, at the same
- * offset and stride, turns them in place).  Keys are computed in 64 bits and
- * rounded to binary32 before they are rounded to 4 bits. */
+ * offset and stride, turns them in place); those of positions that are passed
+ * over too.  Keys are computed in 64 bits and rounded to binary32 before they
+ * are rounded to 4 bits. */
 int ziggy_hip_kv4_append(ZiggyHipContext *ctx, const ZiggyHipKv4Cache *cache, uint32_t layer, const ZiggyHipBatch *batch,
                          const ZiggyHipHeadsDesc *heads, const ZiggyHipBuffer *src, size_t k_offset_bytes,
                          size_t v_offset_bytes, size_t row_stride, uint32_t q_heads, size_t q_offset_bytes,
                          ZiggyHipBuffer *q_out, size_t q_out_offset_bytes, size_t q_out_row_stride,
                          char *error_message, size_t error_message_len);
 /* Reads the batch's rows back as f32 ([rows][head_count_kv * head_dim]); a
- * batch of one sequence with as many rows as positions reads all of it. */
+ * batch of one sequence with as many rows as positions reads all of it.  Rows
+ * of positions that are passed over stay as they were. */
 int ziggy_hip_kv4_load_f32(ZiggyHipContext *ctx, const ZiggyHipKv4Cache *cache, uint32_t layer,
                            const ZiggyHipBatch *batch, ZiggyHipBuffer *k_out, ZiggyHipBuffer *v_out,
                            char *error_message, size_t error_message_len);
@@ -498,7 +503,8 @@ int ziggy_hip_kv4_load_f32(ZiggyHipContext *ctx, const ZiggyHipKv4Cache *cache, 
  * p attends to its sequence's positions up to p, or, with window > 0, to the
  * last `window` of them; a row that none is left for gets zeros.  output:
  * [rows][head_count * head_dim].  head_count is a multiple of the cache's
- * head_count_kv (at most 64 times as many). */
+ * head_count_kv (at most 64 times as many).  At most 2^21 sequences x
+ * head_count_kv, and 2^29 rows x head_count. */
 int ziggy_hip_kv4_attention_f32(ZiggyHipContext *ctx, const ZiggyHipKv4Cache *cache, uint32_t layer,
                                 const ZiggyHipBatch *batch, const ZiggyHipBuffer *q, size_t q_offset_bytes,
                                 size_t q_row_stride, ZiggyHipBuffer *output, uint32_t head_count, uint32_t window,

@@ -214,3 +214,28 @@ def test_freed_buffers_and_null_contexts_in_the_binding():
     with pytest.raises(hip.HipError) as e:
         hip._call("ziggy_hip_kv4_load_f32", None, None, 0, None, None, None)
     assert e.value.status == 6
+
+
+def test_more_rows_and_sequences_than_a_launch_has(host):
+    x, y = host.buffer(1 << 40), host.buffer(1 << 40)
+    for rows, taken in ((1 << 25, True), ((1 << 25) + 1, False)):
+        args = [host.ctx, ref(heads(host, head_dim=2, rope_dim=2)), x, Z(0), Z(0), y, Z(0), Z(0), None, U(0), U(rows), U(1), U(0)]
+        assert host.call("ziggy_hip_norm_rope_rows_f32", *args) == taken
+        b = batch(host, rows=rows)
+        assert host.call("ziggy_hip_kv4_load_f32", host.ctx, ref(cache(host)), U(0), ref(b), x, y) == taken
+        assert host.call("ziggy_hip_kv4_append", host.ctx, ref(cache(host)), U(0), ref(b), None, x, Z(0), Z(1024), Z(512), U(0), Z(0), None, Z(0), Z(0)) == taken
+    for kvh, heads_, sequences, rows, taken in ((64, 64, 1 << 15, 8, True), (64, 64, (1 << 15) + 1, 8, False), (4, 16, 2, 1 << 25, True), (4, 20, 2, 1 << 25, False)):
+        c, b = cache(host, kvh=kvh), batch(host, sequences=sequences, rows=rows, page_table=x, row_starts=host.buffer(1 << 20), lengths=host.buffer(1 << 20))
+        q, out = host.buffer(1 << 42), host.buffer(1 << 42)
+        assert host.call("ziggy_hip_kv4_attention_f32", host.ctx, ref(c), U(0), ref(b), q, Z(0), Z(0), out, U(heads_), U(0), F(0.1)) == taken
+
+
+def test_outputs_behind_a_cache_in_its_buffers(host):
+    """What counts is where the arrays end, not the buffers that they lie in."""
+    at, codes = 1 << 41, 2 * 4 * 10 * 32 * 64
+    arena = host.buffer(1 << 24, at=at)
+    c, b = cache(host, k_codes=arena), batch(host)
+    q = host.buffer(4 * 8 * 64 * 20)
+    for off, taken in ((codes, True), (codes - 4, False)):
+        out = host.buffer(4 * 8 * 64 * 20, at=at + off)
+        assert host.call("ziggy_hip_kv4_attention_f32", host.ctx, ref(c), U(0), ref(b), q, Z(0), Z(0), out, U(8), U(0), F(0.1)) == taken

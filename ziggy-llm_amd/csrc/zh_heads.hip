@@ -372,7 +372,6 @@ hipError_t launch_head_rows(const HeadRows &p, int cus, hipStream_t s) {
     const int half = p.rotates ? p.rd / 2 : 0;
     plan.wave_bytes = half * 16 + (cache ? 2 * 512 * 4 + 64 * 4 : 0);
     const uint64_t units = (uint64_t)plan.spread * plan.each * plan.chunks;
-    if (units > 0x7FFFFFF0ull) return hipErrorInvalidValue;
     const dim3 grid((unsigned)((units + 3) / 4));
     const bool aligned = p.aligned && p.hd % 8 == 0, pairs = !p.rotates || !p.style;
     const Layout layout = !aligned ? LOOSE : pairs ? PAIRS : p.rd == p.hd ? SPLIT : p.rd % 8 == 0 ? MIXED : LOOSE;

@@ -859,7 +859,6 @@ hipError_t launch_kv4_attention(const Kv4Attn &a, int cus, hipStream_t s) {
         else if (p.few) few(h, more, std::false_type{}, prompt);
         if (most > p.few) many(h, prompt);
     };
-    if (a.b.sequences * nkv * 8 > 0x7FFFFFFFu || (all / 16 + a.b.sequences + 4) * nkv > 0x7FFFFFFFu) return hipErrorInvalidValue;
     switch (a.c.hd) {
     case 64: go(std::integral_constant<int, 64>{}, std::integral_constant<int, 1>{}, std::integral_constant<int, 4>{}, std::integral_constant<int, 2>{}); break;
     case 96: go(std::integral_constant<int, 96>{}, std::integral_constant<int, 1>{}, std::integral_constant<int, 2>{}, std::integral_constant<int, 2>{}); break;

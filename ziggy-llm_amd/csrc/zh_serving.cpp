@@ -34,17 +34,20 @@ const char *kv4_layer(const ZiggyHipContext *ctx, const ZiggyHipKv4Cache *c, uin
     return nullptr;
 }
 
-// whether [p, p + n) meets one of the cache's buffers
+// whether [p, p + n) meets one of the cache's arrays
 bool meets_cache(const ZiggyHipKv4Cache *c, const void *p, size_t n) {
-    for (const ZiggyHipBuffer *b : {c->k_codes, c->v_codes, c->k_scales, c->v_scales})
-        if (overlap(b->ptr, b->len, p, n)) return true;
-    return false;
+    const size_t nc = ziggy_hip_kv4_codes_length(c->layers, c->head_count_kv, c->head_dim, c->pages), ns = nc / 16;
+    return overlap(c->k_codes->ptr, nc, p, n) || overlap(c->v_codes->ptr, nc, p, n) || overlap(c->k_scales->ptr, ns, p, n) ||
+           overlap(c->v_scales->ptr, ns, p, n);
 }
+
+// Rows of one call: a wavefront has one, and a launch less than 2^32 threads.
+constexpr uint32_t kMostRows = 1u << 25;
 
 // a batch whose tables lie in their buffers; null: why not
 const char *batch_of(const ZiggyHipContext *ctx, const ZiggyHipBatch *d, const ZiggyHipKv4Cache *c, Batch *out) {
     if (!d || d->sequences == 0 || d->sequences > 65536 || d->pages_per_sequence == 0 || d->pages_per_sequence > (1u << 24) ||
-        d->rows == 0 || d->rows > 0x7FFFFFFFu)
+        d->rows == 0 || d->rows > kMostRows)
         return "unsupported batch";
     const size_t np = (size_t)d->sequences * d->pages_per_sequence * 4, n = (size_t)d->sequences * 4;
     if (!in_buffer(ctx, d->page_table, np) || !in_buffer(ctx, d->row_starts, n + 4) || !in_buffer(ctx, d->lengths, n))
@@ -108,7 +111,8 @@ int ziggy_hip_norm_rope_rows_f32(ZiggyHipContext *ctx, const ZiggyHipHeadsDesc *
     p.hd = (int)d->rope->head_dim;
     const char *why = heads_of(ctx, d, d->rope->head_dim, &p);
     ZH_REFUSE(why, "%s", why);
-    ZH_REFUSE(rows == 0 || q_heads > 65536 || k_heads > 65536 || q_heads + k_heads == 0, "rows and heads (at most 65536) are needed");
+    ZH_REFUSE(rows == 0 || rows > kMostRows || q_heads > 65536 || k_heads > 65536 || q_heads + k_heads == 0,
+              "1 to 33554432 rows of 1 to 65536 heads are served");
     const size_t width = (size_t)(q_heads + k_heads) * p.hd;
     if (sstride == 0) sstride = width;
     if (dstride == 0) dstride = width;
@@ -222,6 +226,7 @@ int ziggy_hip_kv4_attention_f32(ZiggyHipContext *ctx, const ZiggyHipKv4Cache *ca
     if (!why) why = batch_of(ctx, batch, cache, &p.b);
     ZH_REFUSE(why, "%s", why);
     ZH_REFUSE(heads == 0 || heads % p.c.nkv || heads / p.c.nkv > 64, "unsupported query heads %u over %d kv heads", heads, p.c.nkv);
+    ZH_REFUSE((uint64_t)p.b.sequences * p.c.nkv > (1u << 21) || (uint64_t)p.b.rows * heads > (1u << 29), "too many sequences or rows for one call");
     // scores as powers of two; the scale's sign goes to the queries
     p.qscale = fabsf(scale) * 1.44269504088896340736f, p.qsign = scale > 0 ? 1.f : scale < 0 ? -1.f : 0.f;
     ZH_REFUSE(!isfinite(p.qscale), "invalid score scale");

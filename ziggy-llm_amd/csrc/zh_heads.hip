@@ -15,12 +15,6 @@ __device__ __forceinline__ double turns_per_position(const HeadRows &p, int i) {
     return p.factors ? f / (double)p.factors[i] : f;
 }
 
-// LDS of a wavefront's own lanes: what they wrote is what they read behind this
-__device__ __forceinline__ void wave_fence() {
-    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-    __builtin_amdgcn_wave_barrier();
-}
-
 // the scale byte (its exponent + 127) of 32 values whose largest magnitude has these bits
 __device__ __forceinline__ uint32_t scale_byte(uint32_t bits) {
     const uint32_t e = (bits >> 23) + ((bits & 0x7FFFFFu) > 0x600000u ? 1u : 0u);  // 7 2^x is 1.75 2^(x + 2)
@@ -65,7 +59,6 @@ constexpr int kAhead = 2;  // heads of a team whose loads are under way ahead of
 struct HeadPlan {
     int units, team;        // lanes of a head: those with values, rounded up to a power of two
     int chunks;             // wavefronts that share a row's heads
-    uint32_t spread, each;  // rows that follow each other lie on one XCD: `each` of them on every one of `spread`
     int wave_bytes;         // of LDS
     int streams;            // the output is more than the caches hold
 };
@@ -82,9 +75,8 @@ __device__ __forceinline__ void put(float *to, float4 v, int streams) {
 template <int LAYOUT, bool CACHE> __global__ void __launch_bounds__(256) head_rows_kernel(HeadRows p, HeadPlan plan) {
     extern __shared__ __align__(16) char lds[];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), team = plan.team, u = lane % team, slot = lane / team;
-    const uint32_t unit = blockIdx.x * 4 + wave, at_row = unit / plan.chunks, chunk = unit - at_row * plan.chunks;
-    const uint32_t r = at_row % plan.spread * plan.each + at_row / plan.spread;
-    if (at_row / plan.spread >= plan.each || r >= p.rows) return;
+    const uint32_t unit = blockIdx.x * 4 + wave, r = unit / plan.chunks, chunk = unit - r * plan.chunks;
+    if (r >= p.rows) return;
     const int half = p.rotates ? p.rd / 2 : 0, i0 = 4 * u, hp = 64 / team;
     double2 *table = reinterpret_cast<double2 *>(lds + wave * plan.wave_bytes);
     // pair i: halves (i, i + half), neighbours (2 i, 2 i + 1) of interleaved ones and of what does not turn
@@ -365,14 +357,13 @@ hipError_t launch_head_rows(const HeadRows &p, int cus, hipStream_t s) {
     while (plan.team < plan.units) plan.team *= 2;  // at most 64: hd is at most 512
     const bool cache = p.c.kc != nullptr;
     const int hp = 64 / plan.team, heads = p.q_heads + p.k_heads + (cache ? p.c.nkv : 0), passes = (heads + hp - 1) / hp;
-    // few rows: their heads over wavefronts, up to 16 a CU
+    // Few rows: their heads over wavefronts, up to 16 a CU.  (A row of 40 heads by one wavefront is ten passes in a row; 4 and
+    // 64 a CU are within 0.5 us of this at 1 to 200 rows.)
     const uint32_t want = 16u * (uint32_t)cus / p.rows;
     plan.chunks = want < 1 ? 1 : want < (uint32_t)passes ? (int)want : passes;
-    plan.spread = cache ? 8 : 1, plan.each = (p.rows + plan.spread - 1) / plan.spread;
     const int half = p.rotates ? p.rd / 2 : 0;
     plan.wave_bytes = half * 16 + (cache ? 2 * 512 * 4 + 64 * 4 : 0);
-    const uint64_t units = (uint64_t)plan.spread * plan.each * plan.chunks;
-    const dim3 grid((unsigned)((units + 3) / 4));
+    const dim3 grid((unsigned)(((uint64_t)p.rows * plan.chunks + 3) / 4));
     const bool aligned = p.aligned && p.hd % 8 == 0, pairs = !p.rotates || !p.style;
     const Layout layout = !aligned ? LOOSE : pairs ? PAIRS : p.rd == p.hd ? SPLIT : p.rd % 8 == 0 ? MIXED : LOOSE;
     plan.streams = layout <= PAIRS && (uint64_t)p.rows * (p.q_heads + p.k_heads) * p.hd * 4 > (16u << 20);

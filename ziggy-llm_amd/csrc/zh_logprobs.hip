@@ -5,10 +5,10 @@
 // keeps its digits where one token takes nearly everything.
 //
 // Two launches, one pass over the logits:
-//   slices  a workgroup per 2048 logits (8192 where rows alone fill the device), held in registers: the largest, the
+//   slices  a workgroup per 4096 logits (8192 where those fill the device), held in registers: the largest, the
 //           sums relative to it, and its k best in order;
 //   rows    a workgroup per row joins its slices.
-// The k best of a slice: a value that k logits reach (see limit_of) leaves few candidates, and a candidate's place is
+// The k best of a slice: a value that k logits reach leaves few candidates, and a candidate's place is
 // the count of those above it: no sort, no dependence on the order of arrival.
 #include <algorithm>
 
@@ -20,7 +20,7 @@ namespace {
 
 typedef unsigned long long u64;
 
-constexpr int kThreads = 256, kCandidates = 1024, kMaxSlices = 128, kTop = ZIGGY_HIP_MAX_TOP_LOGPROBS;
+constexpr int kThreads = 256, kCandidates = 1024, kMaxSlices = 64, kTop = ZIGGY_HIP_MAX_TOP_LOGPROBS;
 
 struct SliceSums {
     float top;       // the largest
@@ -253,95 +253,85 @@ template <int V> __global__ void __launch_bounds__(kThreads) logprobs_slice_kern
     }
 }
 
-// A workgroup per row.
-__global__ void __launch_bounds__(1024) logprobs_row_kernel(TokenLogprobs p, LogprobsWork w) {
-    __shared__ __align__(16) u64 heads[8][kMaxSlices], candidates[kTop * kMaxSlices];
-    __shared__ uint32_t taken[16];
-    __shared__ u64 limits[8];
-    __shared__ double sums[3][2], shared_log;
-    __shared__ float tops[2];
+// A workgroup per row: the last wavefront joins the slices' sums, a lane each, while the others find the best.
+constexpr int kRowThreads = 512, kLists = 7;
+__global__ void __launch_bounds__(kRowThreads) logprobs_row_kernel(TokenLogprobs p, LogprobsWork w) {
+    __shared__ __align__(16) u64 heads[kLists][kMaxSlices], candidates[kTop * kMaxSlices];
+    __shared__ uint32_t taken[kRowThreads / 64];
+    __shared__ u64 limits[kLists];
+    __shared__ double shared_log;
+    __shared__ float shared_largest;
     __shared__ int found;
     const uint32_t row = blockIdx.x, n = w.slices;
     const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
-    const SliceSums *from = w.sums + (size_t)row * n;
     const u64 *top = w.top + (size_t)row * n * p.k;
-    SliceSums own{-INFINITY, 0, 0.0, 0.0};
-    if ((uint32_t)tid < n) own = from[tid];
-    float given = 0.f;
-    uint32_t token = 0;
-    if (tid == 0) {
-        token = p.tokens[row];
-        if (token < p.vocab) given = p.x[(size_t)row * p.stride + token];
-    }
-    // For each j of 1, 2, 4 .. k: of the slices' j-th best the ceil(k / j)-th largest is a value that k logits reach.
-    const int group = tid >> 7, j = 1 << group, i = tid & 127;
-    if (p.k) {
-        heads[group][i] = (uint32_t)i < n && j <= p.k ? top[(size_t)i * p.k + j - 1] : 0ull;
-        if (i == 0) limits[group] = 1;
-    }
     if (tid == 0) found = 0;
-    if (wave < 2) {
-        const float m = wave_max_f32(own.top);
-        if (lane == 0) tops[wave] = m;
-    }
-    __syncthreads();
-    const float largest = fmaxf(tops[0], tops[1]);
-    if (j <= p.k) {
-        const u64 mine = heads[group][i];
+    // For each j of 1, 2, 4 .. k: of the slices' j-th best the ceil(k / j)-th largest is a value that k logits reach.
+    const int j = 1 << wave;
+    if (wave < kLists && p.k) {
+        const u64 mine = (uint32_t)lane < n && j <= p.k ? top[(size_t)lane * p.k + j - 1] : 0ull;
+        if (lane == 0) limits[wave] = 1;
+        heads[wave][lane] = mine;
+        wave_fence();
         int rank = 0;
         for (uint32_t o = 0; o < n; o += 8) {  // (those behind the last are 0)
             ulonglong2 other[4];
 #pragma unroll
-            for (int e = 0; e < 4; e++) other[e] = *reinterpret_cast<const ulonglong2 *>(&heads[group][o + 2 * e]);
+            for (int e = 0; e < 4; e++) other[e] = *reinterpret_cast<const ulonglong2 *>(&heads[wave][o + 2 * e]);
 #pragma unroll
             for (int e = 0; e < 4; e++) rank += (other[e].x > mine) + (other[e].y > mine);
         }
-        if (mine && rank == (p.k + j - 1) / j - 1) limits[group] = mine;
+        if (mine && rank == (p.k + j - 1) / j - 1) limits[wave] = mine;
+    }
+    SliceSums own{-INFINITY, 0, 0.0, 0.0};
+    float given = 0.f;
+    uint32_t token = 0;
+    if (wave == kLists) {
+        token = p.tokens[row];
+        if ((uint32_t)lane < n) own = w.sums[(size_t)row * n + lane];
+        if (token < p.vocab) given = p.x[(size_t)row * p.stride + token];
     }
     __syncthreads();
-    if (wave >= 2 && p.k) {
+    if (wave < kLists && p.k) {
         u64 least = 1;
 #pragma unroll
-        for (int g = 0; g < 8; g++) least = max(least, limits[g]);
+        for (int g = 0; g < kLists; g++) least = max(least, limits[g]);
         // a slice's are in order: eight lanes take a slice until one falls below
-        for (uint32_t a = (uint32_t)(tid - 128) / 8; a < n; a += 112)
+        for (uint32_t a = (uint32_t)tid / 8; a < n; a += 64 * kLists / 8)
             for (int b = tid & 7; b < p.k; b += 8) {
                 const u64 k = top[(size_t)a * p.k + b];
                 if (k < least) break;
                 candidates[atomicAdd(&found, 1)] = k;
             }
     }
-    if (wave < 2) {  // meanwhile the sums
+    auto logprob = [&](float v, float largest, double log_s) { return (float)(((double)(v != v ? -INFINITY : v) - (double)largest) - log_s); };
+    if (wave == kLists) {  // meanwhile the sums
+        const float largest = wave_max_f32(own.top);
         // slices that have the largest give its count, the others their weights
         double s = own.s, t = own.t, count = own.top == largest ? (double)own.count : 0.0;
         if (own.top != largest) {
             const double d = fmax((double)own.top - (double)largest, -1000.0), f = exp(d), all = own.count + own.s;
             s = f * all, t = f * (own.t + d * all);
         }
-        s = wave_sum(s), t = wave_sum(t), count = wave_sum(count);
-        if (lane == 0) sums[0][wave] = s, sums[1][wave] = t, sums[2][wave] = count;
-    }
-    __syncthreads();
-    auto logprob = [&](float v, double log_s) { return (float)(((double)(v != v ? -INFINITY : v) - (double)largest) - log_s); };
-    if (wave == 0) {
-        const double s = (sums[0][0] + sums[0][1]) + (sums[2][0] + sums[2][1] - 1.0), t = sums[1][0] + sums[1][1], nan = (double)__uint_as_float(0x7FC00000u);
-        const double log_s = isfinite(largest) ? log1p(s) : nan;
+        s = wave_sum(s) + (wave_sum(count) - 1.0), t = wave_sum(t);
+        const double nan = (double)__uint_as_float(0x7FC00000u), log_s = isfinite(largest) ? log1p(s) : nan;
         if (lane == 0) {
-            shared_log = log_s;
-            p.out[row] = token < p.vocab ? logprob(given, log_s) : (float)nan;
+            shared_log = log_s, shared_largest = largest;
+            p.out[row] = token < p.vocab ? logprob(given, largest, log_s) : (float)nan;
             if (p.entropy) p.entropy[row] = (float)(log_s - t / (1.0 + s));
         }
     }
     if (p.k == 0) return;
     __syncthreads();
     const double log_s = shared_log;
+    const float largest = shared_largest;
     place(candidates, found, p.k, [&](int rank, u64 k) {
         p.top_tokens[(size_t)row * p.k + rank] = index_of_key(k);
-        p.top[(size_t)row * p.k + rank] = logprob(value_of_key(k), log_s);
+        p.top[(size_t)row * p.k + rank] = logprob(value_of_key(k), largest, log_s);
     });
     // fewer finite logits than k: all of them are placed, +infinities too; the first of the others follow
     uint32_t have = (uint32_t)found;
-    for (uint32_t at = 0; have < (uint32_t)p.k && at < p.vocab; at += 1024) {
+    for (uint32_t at = 0; have < (uint32_t)p.k && at < p.vocab; at += kRowThreads) {
         const float v = at + tid < p.vocab ? p.x[(size_t)row * p.stride + at + tid] : 0.f;
         const bool none = at + tid < p.vocab && (v != v || v == -INFINITY);
         const u64 which = __ballot(none);
@@ -349,10 +339,10 @@ __global__ void __launch_bounds__(1024) logprobs_row_kernel(TokenLogprobs p, Log
         if (lane == 0) taken[wave] = (uint32_t)__popcll(which);
         __syncthreads();
         uint32_t rank = have + (uint32_t)__popcll(which & ((1ull << lane) - 1)), all = 0;
-        for (int i = 0; i < 16; i++) rank += i < wave ? taken[i] : 0u, all += taken[i];
+        for (int i = 0; i < kRowThreads / 64; i++) rank += i < wave ? taken[i] : 0u, all += taken[i];
         if (none && rank < (uint32_t)p.k) {
             p.top_tokens[(size_t)row * p.k + rank] = at + tid;
-            p.top[(size_t)row * p.k + rank] = logprob(-INFINITY, log_s);
+            p.top[(size_t)row * p.k + rank] = logprob(-INFINITY, largest, log_s);
         }
         have += all;
     }
@@ -361,9 +351,9 @@ __global__ void __launch_bounds__(1024) logprobs_row_kernel(TokenLogprobs p, Log
 }  // namespace
 
 hipError_t launch_token_logprobs(const TokenLogprobs &a, int cus, hipStream_t s) {
-    // The fewer workgroups the rows make, the smaller their slices: 2048 logits up to 4 workgroups a CU, 4096 up to 16.
-    auto wgs = [&](uint32_t slice) { return (uint64_t)a.rows * ((a.vocab + slice - 1) / slice); };
-    const uint32_t slice = wgs(2048) <= 4ull * cus ? 2048 : wgs(4096) <= 16ull * cus ? 4096 : 8192;
+    // The fewer workgroups the rows make, the smaller their slices.  (Of 4096 logits and of 8192: a row of 151936 4.7 us and
+    // 5.5, 8 rows 6.3 and 6.8, 33 of 128256 12.0 and 10.8, 511 of 151936 67 and 57.)
+    const uint32_t slice = (uint64_t)a.rows * ((a.vocab + 4095) / 4096) <= 2ull * cus ? 4096 : 8192;
     LogprobsWork w{};
     w.slices = (a.vocab + slice - 1) / slice;
     w.logits = ((a.vocab + w.slices - 1) / w.slices + 3) / 4 * 4;  // alike, so that the last one's lanes aren't mostly empty
@@ -379,9 +369,8 @@ hipError_t launch_token_logprobs(const TokenLogprobs &a, int cus, hipStream_t s)
         w.sums = (SliceSums *)a.work, w.top = (u64 *)(w.sums + (size_t)p.rows * w.slices);
         const dim3 grid(p.rows * w.slices);
         if (slice == 8192) hipLaunchKernelGGL(logprobs_slice_kernel<32>, grid, dim3(kThreads), 0, s, p, w);
-        else if (slice == 4096) hipLaunchKernelGGL(logprobs_slice_kernel<16>, grid, dim3(kThreads), 0, s, p, w);
-        else hipLaunchKernelGGL(logprobs_slice_kernel<8>, grid, dim3(kThreads), 0, s, p, w);
-        hipLaunchKernelGGL(logprobs_row_kernel, dim3(p.rows), dim3(1024), 0, s, p, w);
+        else hipLaunchKernelGGL(logprobs_slice_kernel<16>, grid, dim3(kThreads), 0, s, p, w);
+        hipLaunchKernelGGL(logprobs_row_kernel, dim3(p.rows), dim3(kRowThreads), 0, s, p, w);
     }
     return hipGetLastError();
 }

@@ -90,6 +90,12 @@ template <class T> __device__ __forceinline__ T running_sum(T v) {
     return add_moved<0x143, 0xC>(v);  // row_bcast:31 into rows 2 and 3
 }
 
+// LDS of a wavefront's own lanes: what they wrote is what they read behind this
+__device__ __forceinline__ void wave_fence() {
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+}
+
 // One layer of a 4-bit cache.
 struct Kv4Layer {
     uint8_t *kc, *vc, *ks, *vs;

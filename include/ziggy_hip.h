@@ -795,8 +795,8 @@ int ziggy_hip_sample_rows_f32(ZiggyHipContext *ctx, const ZiggyHipBuffer *logits
  * the best tokens, highest first, ties to the lower id, and their log
  * probabilities.  Logits of NaN count as -infinity, as for the sampler.  A row whose
  * largest logit is infinite either way has log probabilities and entropy of NaN
- * (its top tokens are in order all the same).  Exponentials are binary32, sums
- * and logarithms 64 bits. */
+ * (its top tokens are in order all the same).  Exponentials are binary32 and
+ * add up eight at a time; sums of those and logarithms are 64 bits. */
 #define ZIGGY_HIP_MAX_TOP_LOGPROBS 64
 int ziggy_hip_token_logprobs_f32(ZiggyHipContext *ctx, const ZiggyHipBuffer *logits, size_t row_stride,
                                  const ZiggyHipBuffer *tokens, ZiggyHipBuffer *out_logprobs, ZiggyHipBuffer *out_entropy,

@@ -5,6 +5,17 @@
 // and V enter the matrix cores exactly and no scale is left over to weigh scores or outputs by.  A query and a
 // weight enter as three bf16 pieces, cut off by truncation, whose sum they are to the bit.  Products accumulate in
 // binary32, maximum and sum are binary32.
+//
+// Two kernels.  Few columns (a sequence's rows times the query heads of a kv head, up to 64; 32 of head size 256): every
+// wavefront streams blocks of 32 positions from memory straight into the products' operands, and the batch's blocks are
+// spread over the card, so that long contexts are split and joined.  Many: four wavefronts share pages widened into LDS.
+// (48 columns, 7 sequences of 2000 positions, 8 kv heads of 128: 28.2 us by the first, 33.8 by the second; 64 columns, one
+// of 9000, heads of 64: 17.0 and 19.3.)
+//
+// What bounds it (32 heads over 8 kv heads of 128).  A query at 131071 positions: memory, 30.4 us for 143 MB, and the join
+// 4.7.  At 4113: the chain launch, lengths, page, codes, products, exchange 6.7, and the join's 3.6.  48 sequences of up to
+// 16384 positions: memory and the last workgroups of uneven sequences, 75 us for 311 MB, and 5.8.  2048 queries at 16384:
+// the matrix cores, 1.04 ms for three pieces of both products, 1.49 PFLOP/s (library products of bf16 reach 1.34).
 #include <algorithm>
 
 #include "zh_serving.h"
@@ -34,7 +45,7 @@ struct Kv4Params {
     uint32_t window;
     float qscale, qsign;
     uint32_t few;       // columns up to which a sequence is the few-column kernel's (0: none is)
-    uint32_t wgs;       // few: workgroups to spread the blocks over
+    uint32_t wgs;       // few: workgroups to spread the blocks over, at most
     int splits;         // many: of each tile's positions
     uint32_t *plan;     // of more than 64 sequences: see Plan
     float *part;        // partial outputs, and {maximum, sum} of each
@@ -74,8 +85,9 @@ __device__ __forceinline__ Sequence uniform(const Sequence &q) {
 }
 
 // Of more than 64 sequences a kernel of its own makes a table, which the others search: for each sequence the end of its
-// items among the few-column kernel's and of its tiles among the other's, and the slot of its first split.  (Up to 64 every
-// wavefront has a sequence a lane, and a table would cost a launch.)
+// items among the few-column kernel's and of its tiles among the other's, and the slot of its first split.  Up to 64 every
+// wavefront has a sequence a lane, and a table would cost a launch, 4.4 us.  (Every wavefront going through all sequences,
+// 64 at a time, and the table: 2048 sequences of 512 positions 828 us and 302, 512 of 512 127 and 88, 128 of 1024 40 and 43.)
 struct Plan {
     const uint32_t *quota, *items, *tiles, *slots;
     __host__ __device__ static size_t words(uint32_t sequences) { return 4 + 3 * (size_t)sequences; }
@@ -130,7 +142,7 @@ struct Share {
     uint32_t index;         // item: within the sequence's
     uint32_t slot;          // of the sequence's first split
 };
-constexpr uint32_t kFewWaves = 4, kLeastBlocks = kFewWaves;  // of a workgroup: one for each wavefront
+constexpr uint32_t kFewWaves = 4, kLeastBlocks = kFewWaves;  // of a workgroup: one for each wavefront (16: 4113 positions 9.2 us, not 7.8)
 
 // A sequence's tiles, and its blocks (of all columns: a tile's own are no more).
 template <int COLUMNS> __device__ __forceinline__ void load_of(const Kv4Params &p, const Sequence &q, uint32_t &tiles, uint32_t &blocks) {
@@ -141,8 +153,13 @@ template <int COLUMNS> __device__ __forceinline__ void load_of(const Kv4Params &
     tiles = (columns + COLUMNS - 1) / COLUMNS;
     blocks = max((uint32_t)(r.end - r.begin), 1u);  // rows that see nothing have an item, which writes zeros
 }
-__device__ __forceinline__ uint32_t quota_of(const Kv4Params &p, u64 total) {
-    return max(kLeastBlocks, (uint32_t)ceil((double)total * p.c.nkv / p.wgs));
+// One workgroup a CU while that leaves it up to 8 blocks a wavefront, two past that.  (One and two, 8 kv heads of 128: a
+// query at 4113 positions 6.65 us and 7.35, 16000 8.9 and 10.1, 32000 12.8 and 13.1, 131071 34.8 and 30.2; 48 sequences 85
+// and 76, with three 76.)  Where it is one, half a workgroup is kept for every tile, as its blocks rarely are whole quotas:
+// a few items more than CUs take another round (three sequences of 3000 positions, 264 items: 9.4 us).
+__device__ __forceinline__ uint32_t quota_of(const Kv4Params &p, u64 total, uint32_t tiles) {
+    const double blocks = (double)total * p.c.nkv, cus = 0.5 * p.wgs, one = ceil(blocks / (cus - 0.5 * fmin((double)tiles * p.c.nkv, cus)));
+    return max(kLeastBlocks, (uint32_t)(one <= 8 * kFewWaves ? one : ceil(blocks / p.wgs)));
 }
 
 // The item with this number, or (BY_SEQUENCE) the sequence.  Every lane of a wavefront takes part.
@@ -169,7 +186,7 @@ template <bool BY_SEQUENCE, int COLUMNS> __device__ __forceinline__ Share share_
     if (lane < p.b.sequences) q = sequence_of(p.b, lane), load_of<COLUMNS>(p, q, tiles, blocks);
     u64 total = running_sum((u64)blocks * tiles);
     total = (u64)of((uint32_t)(total >> 32), 63) << 32 | of((uint32_t)total, 63);
-    const uint32_t quota = uniform(quota_of(p, total)), splits = (blocks + quota - 1) / quota, n = splits * tiles * nkv;
+    const uint32_t quota = uniform(quota_of(p, total, of(running_sum(tiles), 63))), splits = (blocks + quota - 1) / quota, n = splits * tiles * nkv;
     const uint32_t sum = running_sum(n), slot_sum = running_sum(splits > 1 ? n : 0u);
     const u64 past = __ballot(BY_SEQUENCE ? lane == number : sum > number);
     if (!past) return t;
@@ -184,7 +201,7 @@ template <bool BY_SEQUENCE, int COLUMNS> __device__ __forceinline__ Share share_
 // The table of more than 64 sequences: one workgroup, 1024 sequences at a time.
 template <int FEW, int MANY> __global__ void __launch_bounds__(1024) kv4_plan_kernel(Kv4Params p) {
     __shared__ u64 totals[16];
-    __shared__ uint32_t sums[3][16];
+    __shared__ uint32_t all_tiles[16], sums[3][16];
     const Plan plan(p);
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     uint32_t tiles, blocks;
@@ -193,17 +210,19 @@ template <int FEW, int MANY> __global__ void __launch_bounds__(1024) kv4_plan_ke
         if (s < p.b.sequences) q = sequence_of(p.b, s), load_of<FEW>(p, q, tiles, blocks);
     };
     u64 total = 0;
+    uint32_t count = 0;
     for (uint32_t s = threadIdx.x; s < p.b.sequences; s += 1024) {
         Sequence q;
         look(s, q);
         total += (u64)blocks * tiles;
+        count += tiles;
     }
-    total = running_sum(total);
-    if (lane == 63) totals[wave] = total;
+    total = running_sum(total), count = running_sum(count);
+    if (lane == 63) totals[wave] = total, all_tiles[wave] = count;
     __syncthreads();
-    total = 0;
-    for (int i = 0; i < 16; i++) total += totals[i];
-    const uint32_t quota = quota_of(p, total);
+    total = count = 0;
+    for (int i = 0; i < 16; i++) total += totals[i], count += all_tiles[i];
+    const uint32_t quota = quota_of(p, total, count);
     if (threadIdx.x == 0) p.plan[0] = quota;
     uint32_t before[3] = {};
     for (uint32_t from = 0; from < p.b.sequences; from += 1024) {
@@ -336,7 +355,7 @@ template <int HD> struct Lane4 {
 // is what it gives of P^T.
 // PACKED (CT 1): four columns at most, whose three pieces, and a fourth of zeros, are sixteen: lane i holds piece i % 4 of
 // column i / 4, so that a product of all pieces is one instead of three.  Scores of the pieces add up across four lanes,
-// outputs once at the end.
+// outputs once at the end.  (A query at 131071 positions 30.7 us, without 38.6; 48 sequences 75 and 95.)
 template <int HD, int CT, int AWAY, bool PACKED = false> struct Columns {
     static constexpr int G = HD / 32, DT = HD / 16, P = PACKED ? 1 : 3, NEAR = P - AWAY;
     fb8 q[CT][G][NEAR];
@@ -560,7 +579,9 @@ __device__ __forceinline__ float *column_of(float *out, const Kv4Params &p, cons
     return out + ((size_t)(q.row0 + row) * p.heads + head * p.group + (column - row * p.group)) * hd;
 }
 
-// Few columns (decoding): a workgroup takes an item, its wavefronts blocks in turn, joined in LDS.
+// Few columns (decoding): a workgroup takes an item, its wavefronts blocks in turn, joined in LDS.  (Eight wavefronts: a
+// batch of 48 103 us instead of 84.  One workgroup a share of exactly as many blocks, sequences cut wherever it ends: 79
+// instead of 75, 4113 positions 10.1 instead of 7.5, for the registers and the chain of loads of every unit in a row.)
 template <int HD, int CT, bool PACKED> __global__ void __launch_bounds__(64 * kFewWaves, 2) kv4_few_kernel(Kv4Params p) {
     constexpr int N = PACKED ? 4 : 16 * CT, C = HD / 4, AWAY = !PACKED && HD * CT > 128 ? 2 : 0, PIECES = CT * (HD / 32) * AWAY * 64;  // of a wavefront (16 bytes each)
     constexpr int OUTPUTS = kFewWaves * N * (HD + 4), HELD = kFewWaves * PIECES * 4;
@@ -685,7 +706,8 @@ template <int HD, int COLUMNS> __global__ void __launch_bounds__(256) kv4_few_jo
 
 // Many columns (prompts): a workgroup takes a tile of 64 CT columns, a wavefront 16 CT of them, through a split of its
 // pages.  A page's operands are widened once, a quarter by each wavefront, into LDS, in the order in which the
-// products take them; two pages' room, so that one barrier a page is enough.
+// products take them; two pages' room, so that one barrier a page is enough.  (2048 queries at 16384: CT 2 1.04 ms, CT 1
+// 1.28; every wavefront widening all for itself 1.62.)
 template <int HD> struct Quarter {  // wavefront (half h, pt): K rows of half h, its 16 of pt; V of half h, every second t from pt on
     static constexpr int G = HD / 32, T = (G + 1) / 2;
     Lane4<HD> x;

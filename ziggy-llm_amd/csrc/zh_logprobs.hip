@@ -8,8 +8,12 @@
 //   slices  a workgroup per 4096 logits (8192 where those fill the device), held in registers: the largest, the
 //           sums relative to it, and its k best in order;
 //   rows    a workgroup per row joins its slices.
-// The k best of a slice: a value that k logits reach leaves few candidates, and a candidate's place is
-// the count of those above it: no sort, no dependence on the order of arrival.
+// The k best of a slice: a value that k logits reach leaves few candidates, and a candidate's place is the count of those
+// above it: no sort, no dependence on the order of arrival.
+//
+// What bounds it: 511 rows of 151936 memory (56 us for 311 MB, 5.5 TB/s); 33 of 128256 the loads and the sums 7.6 us, 20
+// alternatives of each slice 4, the rows 3.9 (17 MB are 3.3 us of memory); one row the chain of two launches, load,
+// exchange and join (4.7 + 3.7).
 #include <algorithm>
 
 #include "zh_serving.h"
@@ -132,12 +136,12 @@ template <int V> __global__ void __launch_bounds__(kThreads) logprobs_slice_kern
     float own = -INFINITY;  // (fmaxf passes over NaN)
 #pragma unroll
     for (int j = 0; j < V; j++) own = fmaxf(own, v[j]);
-    // A value that k logits reach: up to 16 the k-th largest of the 16 rows' (of 16 lanes) largest, up to 48 that of the
-    // 64 quads' largest, past that the least of the rows' ceil(k / 16)-th.  (That alone leaves 50 candidates a slice for k
-    // up to 16 and 70 up to 32, the others k and a few more: 33 x 128256 logits, 5 tokens 13.3 us and 9.5, 20 tokens 14.5
-    // and 12.)
+    // A value that k logits reach: up to 12 the k-th largest of the 16 rows' (of 16 lanes) largest, up to 48 that of the
+    // 64 quads' largest, past that the least of the rows' ceil(k / 16)-th.  (The finer, the fewer candidates and the more to
+    // compare.  33 x 128256 logits, by rows and by quads: 12 tokens 10.3 and 11.3 us, 16 tokens 12.0 and 11.4; the last
+    // leaves 50 to 140 candidates: 20 tokens 14.5 us, 50 tokens 22.)
     const float row_top = row_max(own);
-    const bool by_quads = p.k > 16 && p.k <= 48;
+    const bool by_quads = p.k > 12 && p.k <= 48;
     if (lane % 16 == 0) rows[wave * 4 + lane / 16] = row_top;
     if (by_quads) {
         const float quad = quad_max(own);

@@ -111,6 +111,30 @@ def test_thousands_of_sequences(hip_ctx, sequences):
     assert np.all(y[-1] == 7) and np.all(np.abs(y[:-1] - want) <= bound)
 
 
+@pytest.mark.parametrize("hd", [64, 96, 128, 256])
+@pytest.mark.parametrize("heads,kvh,rows", [(2, 2, 1), (4, 2, 2), (12, 2, 2), (5, 1, 3), (8, 2, 8), (6, 1, 9), (3, 1, 60)])
+@pytest.mark.parametrize("sequences", [64, 65, 100])
+def test_every_width_of_a_batch(hip_ctx, sequences, heads, kvh, rows, hd):
+    """Up to 1, 4, 16, 32 columns and more, some sequences long enough to be split, with the table of many sequences and
+    without; the widths that the batch names, and no word of them."""
+    print("width", sequences, heads, kvh, rows, hd, flush=True)
+    rng = np.random.default_rng(sequences + rows)
+    n = rng.integers(0, rows + 1, sequences)
+    n[7] = rows
+    lengths = np.maximum(n, rng.integers(1, 70, sequences))
+    lengths[7], lengths[-3] = 2100, 700
+    batch = oracle.Batch(n, lengths, rng)
+    cache = oracle.Kv4(1, batch.pool, kvh, hd, rng)
+    got = oracle.upload(hip_ctx, cache)
+    q = rng.normal(0, 0.7, (batch.n, heads, hd)).astype(np.float32)
+    src, want, bound = hip_ctx.buffer(q), *oracle.attention(cache, 0, batch, q, hd ** -0.5, 1500)
+    for limits in (dict(max_rows=rows, max_length=2100), dict()):
+        out = hip_ctx.buffer(np.full(q.shape, 7, np.float32))
+        hip_ctx.kv4_attention(got, 0, batch.on(hip_ctx, **limits), src, out, heads, 1500)
+        off = np.abs(out.read().reshape(q.shape) - want)
+        assert np.all(off <= bound), (limits, np.argwhere(~(off <= bound))[:4])
+
+
 def test_thousands_of_long_sequences_share_pages(hip_ctx):
     """3000 sequences of a row over the same 2000 positions: splits and workspace at their most; all rows alike."""
     rng = np.random.default_rng(4)

@@ -159,7 +159,7 @@ template <int COLUMNS> __device__ __forceinline__ void load_of(const Kv4Params &
 // a few items more than CUs take another round (three sequences of 3000 positions, 264 items: 9.4 us).
 __device__ __forceinline__ uint32_t quota_of(const Kv4Params &p, u64 total, uint32_t tiles) {
     const double blocks = (double)total * p.c.nkv, cus = 0.5 * p.wgs, one = ceil(blocks / (cus - 0.5 * fmin((double)tiles * p.c.nkv, cus)));
-    return max(kLeastBlocks, (uint32_t)(one <= 8 * kFewWaves ? one : ceil(blocks / p.wgs)));
+    return max(kLeastBlocks, (uint32_t)fmin(one <= 8 * kFewWaves ? one : ceil(blocks / p.wgs), 0x1p31));
 }
 
 // The item with this number, or (BY_SEQUENCE) the sequence.  Every lane of a wavefront takes part.

@@ -582,21 +582,19 @@ __device__ __forceinline__ float *column_of(float *out, const Kv4Params &p, cons
 // Few columns (decoding): a workgroup takes an item, its wavefronts blocks in turn, joined in LDS.  (Eight wavefronts: a
 // batch of 48 103 us instead of 84.  One workgroup a share of exactly as many blocks, sequences cut wherever it ends: 79
 // instead of 75, 4113 positions 10.1 instead of 7.5, for the registers and the chain of loads of every unit in a row.)
-template <int HD, int CT, bool PACKED> __global__ void __launch_bounds__(64 * kFewWaves, 2) kv4_few_kernel(Kv4Params p) {
-    constexpr int N = PACKED ? 4 : 16 * CT, C = HD / 4, AWAY = !PACKED && HD * CT > 128 ? 2 : 0, PIECES = CT * (HD / 32) * AWAY * 64;  // of a wavefront (16 bytes each)
-    constexpr int OUTPUTS = kFewWaves * N * (HD + 4), HELD = kFewWaves * PIECES * 4;
-    // the queries' pieces, then the wavefronts' outputs
-    __shared__ __align__(16) float lds[OUTPUTS > HELD ? OUTPUTS : HELD];
-    __shared__ float ms[kFewWaves][N], ls[kFewWaves][N];
+template <int HD, int CT, bool PACKED> struct FewItem {
+    static constexpr int N = PACKED ? 4 : 16 * CT, AWAY = !PACKED && HD * CT > 128 ? 2 : 0, PIECES = CT * (HD / 32) * AWAY * 64;  // of a wavefront (16 bytes each)
+    static constexpr int OUTPUTS = kFewWaves * N * (HD + 4), HELD = kFewWaves * PIECES * 4;
+    static constexpr int LDS = (OUTPUTS > HELD ? OUTPUTS : HELD) + 2 * kFewWaves * N;
+};
+// lds: the queries' pieces, then the wavefronts' outputs, and their maxima and sums.  SLOT: columns of a slot.
+template <int HD, int CT, bool PACKED, int SLOT>
+__device__ __forceinline__ void few_item(const Kv4Params &p, const Share &t, int head, const Range &r, int begin, int end, uint32_t first, uint32_t count, float *lds) {
+    typedef FewItem<HD, CT, PACKED> I;
+    constexpr int N = I::N, C = HD / 4, AWAY = I::AWAY, PIECES = I::PIECES;
     float(*os)[N][HD + 4] = reinterpret_cast<float(*)[N][HD + 4]>(lds);
+    float(*ms)[N] = reinterpret_cast<float(*)[N]>(lds + (I::LDS - 2 * kFewWaves * N)), (*ls)[N] = ms + kFewWaves;
     const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), i = tid & 15, g = tid >> 4 & 3;
-    const Share t = share_of<false, N>(p, blockIdx.x);
-    if (t.splits == 0) return;
-    const int head = (int)(t.index % p.c.nkv);
-    const uint32_t z = t.index / p.c.nkv % t.splits, first = t.index / p.c.nkv / t.splits * N, count = min(t.q.rows * p.group - first, (uint32_t)N);
-    const Range r = range_of(p, t.q, first / p.group, (first + count - 1) / p.group);
-    int begin = r.begin, end = r.end;
-    share(begin, end, t.splits, z);
     Columns<HD, CT, AWAY, PACKED> x;
     typename Columns<HD, CT, AWAY, PACKED>::Raw raw;
     x.fetch(p, t.q, first, count, head, raw);
@@ -636,13 +634,37 @@ template <int HD, int CT, bool PACKED> __global__ void __launch_bounds__(64 * kF
             o.x = fmaf(f, v.x, o.x), o.y = fmaf(f, v.y, o.y), o.z = fmaf(f, v.z, o.z), o.w = fmaf(f, v.w, o.w);
         }
         if (t.splits > 1) {
-            const size_t at = ((size_t)t.slot + t.index) * N + column;
+            const size_t at = ((size_t)t.slot + t.index) * SLOT + column;
             *reinterpret_cast<float4 *>(p.part + at * HD + d) = o;
             if (d == 0) p.part_ml[at] = make_float2(m, l);
         } else {
             const float inv = l == 0.f ? 0.f : 1.f / l;  // (rows that see nothing: zeros)
             *reinterpret_cast<float4 *>(column_of(p.out, p, t.q, head, first + column, HD) + d) = make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv);
         }
+    }
+}
+
+// Items of up to 16 CT columns (4: PACKED), each at its own width: beside a prompt's chunk or drafts to verify most
+// sequences of a batch have one row.
+template <int HD, int CT, bool PACKED> __global__ void __launch_bounds__(64 * kFewWaves, 2) kv4_few_kernel(Kv4Params p) {
+    constexpr int N = FewItem<HD, CT, PACKED>::N;
+    __shared__ __align__(16) float lds[FewItem<HD, CT, PACKED>::LDS];
+    const Share t = share_of<false, N>(p, blockIdx.x);
+    if (t.splits == 0) return;
+    const int head = (int)(t.index % p.c.nkv);
+    const uint32_t z = t.index / p.c.nkv % t.splits, first = t.index / p.c.nkv / t.splits * N, count = min(t.q.rows * p.group - first, (uint32_t)N);
+    const Range r = range_of(p, t.q, first / p.group, (first + count - 1) / p.group);
+    int begin = r.begin, end = r.end;
+    share(begin, end, t.splits, z);
+    if (PACKED || count <= 4) few_item<HD, 1, true, N>(p, t, head, r, begin, end, first, count, lds);
+    if constexpr (!PACKED) {
+        if (count > 4 && (CT == 1 || count <= 16)) few_item<HD, 1, false, N>(p, t, head, r, begin, end, first, count, lds);
+        if constexpr (CT > 1)
+            if (count > 16 && (CT == 2 || count <= 32)) few_item<HD, 2, false, N>(p, t, head, r, begin, end, first, count, lds);
+        if constexpr (CT > 2)
+            if (count > 32 && (CT == 3 || count <= 48)) few_item<HD, 3, false, N>(p, t, head, r, begin, end, first, count, lds);
+        if constexpr (CT > 3)
+            if (count > 48) few_item<HD, 4, false, N>(p, t, head, r, begin, end, first, count, lds);
     }
 }
 

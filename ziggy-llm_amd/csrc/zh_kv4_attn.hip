@@ -46,7 +46,8 @@ struct Kv4Params {
     float qscale, qsign;
     uint32_t few;       // columns up to which a sequence is the few-column kernel's (0: none is)
     uint32_t wgs;       // few: workgroups to spread the blocks over, at most
-    int splits;         // many: of each tile's positions
+    uint32_t cus;       // many: workgroups to spread the tiles over, two for each
+    uint32_t splits;    // of each tile's positions, at most
     uint32_t *plan;     // of more than 64 sequences: see Plan
     float *part;        // partial outputs, and {maximum, sum} of each
     float2 *part_ml;
@@ -96,21 +97,42 @@ struct Plan {
 };
 constexpr uint32_t kLanes = 64;
 
-// A tile of columns (a sequence's rows' heads of one kv head, row by row), by its number among those of the sequences
-// with more than `few` columns; count 0: none.  Every lane of a wavefront takes part.
-struct Tile {
-    Sequence q;
-    uint32_t first, count;  // columns
-};
+// The work of the many-column kernel: tiles of columns (a sequence's rows' heads of one kv head, row by row) of the
+// sequences with more than `few` columns, times the kv heads, times the splits of their positions that fill the card.
 template <int COLUMNS> __device__ __forceinline__ uint32_t tiles_of(const Kv4Params &p, uint32_t columns) {
     return columns > p.few ? (columns + COLUMNS - 1) / COLUMNS : 0u;
 }
-template <int COLUMNS> __device__ __forceinline__ Tile tile_of(const Kv4Params &p, uint32_t number) {
+// How many splits, from the number of tiles that the batch turns out to have.  (A chunk of 400 rows beside 47 sequences of
+// one: 133 us without.)
+__device__ __forceinline__ uint32_t splits_of(const Kv4Params &p, uint32_t tiles) {
+    return max(1u, min(p.splits, 2 * p.cus / max(tiles * p.c.nkv, 1u)));
+}
+template <int COLUMNS> __device__ __forceinline__ uint32_t all_tiles(const Kv4Params &p) {
+    if (p.b.sequences > kLanes) return uniform(Plan(p).tiles[p.b.sequences - 1]);
+    const uint32_t lane = threadIdx.x & 63;
+    const uint32_t n = lane < p.b.sequences ? tiles_of<COLUMNS>(p, sequence_of(p.b, lane).rows * p.group) : 0u;
+    return (uint32_t)__builtin_amdgcn_readlane((int)running_sum(n), 63);
+}
+// A workgroup's item, the last tiles, which see most, first; count 0: none.  Every lane of a wavefront takes part.
+struct Tile {
+    Sequence q;
+    uint32_t first, count;  // columns
+    uint32_t split, splits;
+    int head;
+};
+template <int COLUMNS> __device__ __forceinline__ Tile tile_of(const Kv4Params &p, uint32_t block) {
     Tile t{};
-    const uint32_t lane = threadIdx.x & 63, group = (uint32_t)p.group;
-    uint32_t before;
+    const uint32_t lane = threadIdx.x & 63, group = (uint32_t)p.group, nkv = (uint32_t)p.c.nkv;
+    uint32_t before, number;
+    auto item = [&](uint32_t tiles) {
+        t.splits = splits_of(p, tiles);
+        const uint32_t items = tiles * nkv * t.splits, i = items - 1 - block;
+        t.head = (int)(i % nkv), t.split = i / nkv % t.splits, number = i / nkv / t.splits;
+        return block < items;
+    };
     if (p.b.sequences > kLanes) {
         const Plan plan(p);
+        if (!item(uniform(plan.tiles[p.b.sequences - 1]))) return t;
         const uint32_t s = count_up_to(plan.tiles, p.b.sequences, number);
         if (s >= p.b.sequences) return t;
         t.q = uniform(sequence_of(p.b, s));
@@ -119,6 +141,7 @@ template <int COLUMNS> __device__ __forceinline__ Tile tile_of(const Kv4Params &
         Sequence q{};
         if (lane < p.b.sequences) q = sequence_of(p.b, lane);
         const uint32_t n = tiles_of<COLUMNS>(p, q.rows * group), sum = running_sum(n);
+        if (!item((uint32_t)__builtin_amdgcn_readlane((int)sum, 63))) return t;
         const u64 past = __ballot(sum > number);
         if (!past) return t;
         const int at = __ffsll(past) - 1;
@@ -768,12 +791,12 @@ template <int HD, int CT> __global__ void __launch_bounds__(256, 2) kv4_many_ker
     constexpr int G = HD / 32, PAGE = 8 * G * 64;  // a page's operands
     __shared__ fb8 pages[2][PAGE];
     const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), i = threadIdx.x & 15, g = threadIdx.x >> 4 & 3, lane = threadIdx.x & 63;
-    const int head = (int)(blockIdx.x % p.c.nkv);
-    const Tile t = tile_of<64 * CT>(p, (gridDim.x - 1 - blockIdx.x) / p.c.nkv);  // the longest (last) first
+    const Tile t = tile_of<64 * CT>(p, blockIdx.x);
     if (t.count == 0) return;
+    const int head = t.head;
     const Range r = range_of(p, t.q, t.first / p.group, (t.first + t.count - 1) / p.group);
     int begin = r.begin / 2, end = r.end > r.begin ? (r.end + 1) / 2 : r.begin / 2;
-    share(begin, end, (uint32_t)p.splits, blockIdx.y);
+    share(begin, end, t.splits, t.split);
     Columns<HD, CT, 0> x;
     const uint32_t first = t.first + 16 * CT * wave;
     typename Columns<HD, CT, 0>::Raw raw;
@@ -817,17 +840,19 @@ template <int HD, int CT> __global__ void __launch_bounds__(256, 2) kv4_many_ker
         const float l = xsum<32>(xsum<16>(x.l[c])), inv = l == 0.f ? 0.f : 1.f / l;
         const uint32_t column = first + 16 * c + i;
         if (column >= t.first + t.count) continue;
-        float *out = p.splits > 1 ? p.part + (size_t)blockIdx.y * p.b.rows * p.heads * HD : p.out;
+        float *out = t.splits > 1 ? p.part + (size_t)t.split * p.b.rows * p.heads * HD : p.out;
         float *to = column_of(out, p, t.q, head, column, HD);
 #pragma unroll
         for (int d = 0; d < HD / 16; d++)
             *reinterpret_cast<float4 *>(to + 16 * d + 4 * g) = make_float4(x.o[c][d][0] * inv, x.o[c][d][1] * inv, x.o[c][d][2] * inv, x.o[c][d][3] * inv);
-        if (p.splits > 1 && g == 0) p.part_ml[(to - p.part) / HD] = make_float2(x.m[c], l);
+        if (t.splits > 1 && g == 0) p.part_ml[(to - p.part) / HD] = make_float2(x.m[c], l);
     }
 }
 
 // The splits of a row's heads joined, a thread four dims.
-template <int HD> __global__ void __launch_bounds__(256) kv4_many_join_kernel(Kv4Params p) {
+template <int HD, int COLUMNS> __global__ void __launch_bounds__(256) kv4_many_join_kernel(Kv4Params p) {
+    const int splits = (int)splits_of(p, all_tiles<COLUMNS>(p));
+    if (splits == 1) return;
     const Sequence q = sequence_of_row(p.b, blockIdx.x);
     if (q.rows * p.group <= p.few) return;  // (none's, or the other kernel's)
     const uint32_t u = blockIdx.y * 256 + threadIdx.x;
@@ -835,10 +860,10 @@ template <int HD> __global__ void __launch_bounds__(256) kv4_many_join_kernel(Kv
         const size_t at = (size_t)blockIdx.x * p.heads + u / (HD / 4), each = (size_t)p.b.rows * p.heads;
         const int d = 4 * (int)(u % (HD / 4));
         float m = -INFINITY, l = 0.f;
-        for (int z = 0; z < p.splits; z++) m = fmaxf(m, p.part_ml[z * each + at].x);
+        for (int z = 0; z < splits; z++) m = fmaxf(m, p.part_ml[z * each + at].x);
         m = finite(m);
         float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-        for (int z = 0; z < p.splits; z++) {
+        for (int z = 0; z < splits; z++) {
             const float2 ml = p.part_ml[z * each + at];
             const float4 v = *reinterpret_cast<const float4 *>(p.part + (z * each + at) * HD + d);
             const float f = __builtin_amdgcn_exp2f(ml.x - m) * ml.y;
@@ -889,13 +914,20 @@ hipError_t launch_kv4_attention(const Kv4Attn &a, int cus, hipStream_t s) {
     };
     auto many = [&](auto h, auto tiles) {
         constexpr int HD = decltype(h)::value, CT = decltype(tiles)::value;
-        const uint64_t n = std::min<uint64_t>(all / (64 * CT) + a.b.sequences, all), wgs = n * nkv;
+        constexpr uint64_t N = 64 * CT;
+        // tiles of a sequence alone; of several, at most and at least as many, however the rows are theirs
+        const bool one = a.b.sequences == 1;
+        const uint64_t few_columns = (uint64_t)p.few * a.b.sequences;
+        const uint64_t most_tiles = one ? (most + N - 1) / N : all / N + std::min<uint64_t>(a.b.sequences, all / (p.few + 1));
+        const uint64_t least_tiles = one ? most_tiles : std::max<uint64_t>(1, all > few_columns ? (all - few_columns) / N : 1);
         const uint64_t each = (uint64_t)a.b.rows * a.heads * (HD + 2);
-        p.splits = (int)std::max<uint64_t>(1, std::min<uint64_t>({2 * (uint64_t)cus / wgs, blocks / 8, part_floats / each}));
+        p.cus = (uint32_t)cus;
+        p.splits = (uint32_t)std::max<uint64_t>(1, std::min<uint64_t>({2 * (uint64_t)cus / (least_tiles * nkv), blocks / 8, part_floats / each}));
         p.part_ml = (float2 *)(p.part + (size_t)p.splits * a.b.rows * a.heads * HD);
-        hipLaunchKernelGGL((kv4_many_kernel<HD, CT>), dim3((unsigned)wgs, (unsigned)p.splits), dim3(256), 0, s, p);
+        const uint64_t items = p.splits > 1 ? std::max<uint64_t>(most_tiles * nkv, 2 * (uint64_t)cus) : most_tiles * nkv;
+        hipLaunchKernelGGL((kv4_many_kernel<HD, CT>), dim3((unsigned)items), dim3(256), 0, s, p);
         if (p.splits > 1)
-            hipLaunchKernelGGL((kv4_many_join_kernel<HD>), dim3(a.b.rows, (a.heads * (HD / 4) + 255) / 256), dim3(256), 0, s, p);
+            hipLaunchKernelGGL((kv4_many_join_kernel<HD, (int)N>), dim3(a.b.rows, (a.heads * (HD / 4) + 255) / 256), dim3(256), 0, s, p);
     };
     auto go = [&](auto h, auto one, auto more, auto prompt) {
         if (p.few && most <= 4) few(h, one, std::true_type{}, prompt);

@@ -103,7 +103,7 @@ template <int COLUMNS> __device__ __forceinline__ uint32_t tiles_of(const Kv4Par
     return columns > p.few ? (columns + COLUMNS - 1) / COLUMNS : 0u;
 }
 // How many splits, from the number of tiles that the batch turns out to have.  (A chunk of 400 rows beside 47 sequences of
-// one: 133 us without.)
+// one: 57 us and the join 8, from as many as it may have 133.)
 __device__ __forceinline__ uint32_t splits_of(const Kv4Params &p, uint32_t tiles) {
     return max(1u, min(p.splits, 2 * p.cus / max(tiles * p.c.nkv, 1u)));
 }
@@ -668,7 +668,7 @@ __device__ __forceinline__ void few_item(const Kv4Params &p, const Share &t, int
 }
 
 // Items of up to 16 CT columns (4: PACKED), each at its own width: beside a prompt's chunk or drafts to verify most
-// sequences of a batch have one row.
+// sequences of a batch have one row.  (47 of a row beside one of 6: 60 us, all at that one's width 111.)
 template <int HD, int CT, bool PACKED> __global__ void __launch_bounds__(64 * kFewWaves, 2) kv4_few_kernel(Kv4Params p) {
     constexpr int N = FewItem<HD, CT, PACKED>::N;
     __shared__ __align__(16) float lds[FewItem<HD, CT, PACKED>::LDS];
@@ -909,7 +909,8 @@ hipError_t launch_kv4_attention(const Kv4Attn &a, int cus, hipStream_t s) {
         plan(std::integral_constant<int, (int)N>{}, std::integral_constant<int, 64 * decltype(prompt)::value>{});
         hipLaunchKernelGGL((kv4_few_kernel<HD, CT, PACKED>), dim3((unsigned)items), dim3(64 * kFewWaves), 0, s, p);
         if (per == 1) return;
-        const dim3 join((unsigned)(a.b.sequences * nkv), (unsigned)std::min<uint64_t>(columns, std::max<uint64_t>(1, 1024 / (a.b.sequences * nkv))));
+        // what is resident at once, 8 workgroups a CU (40 sequences of up to 4 rows: 7.0 us, of half as many 9.1, of twice 8.5)
+        const dim3 join((unsigned)(a.b.sequences * nkv), (unsigned)std::min<uint64_t>(columns, std::max<uint64_t>(1, 8 * (uint64_t)cus / (a.b.sequences * nkv))));
         hipLaunchKernelGGL((kv4_few_join_kernel<HD, (int)N>), join, dim3(256), 0, s, p);
     };
     auto many = [&](auto h, auto tiles) {

@@ -49,8 +49,10 @@ struct Kv4Params {
     uint32_t cus;       // many: workgroups to spread the tiles over, two for each
     uint32_t splits;    // of each tile's positions, at most
     uint32_t *plan;     // of more than 64 sequences: see Plan
-    float *part;        // partial outputs, and {maximum, sum} of each
+    float *part;        // few: partial outputs, and {maximum, sum} of each
     float2 *part_ml;
+    float *many_part;   // many: theirs
+    float2 *many_part_ml;
 };
 
 // The positions that columns first .. last of a sequence see: some of them (first .. last) and all (full_first ..
@@ -692,15 +694,15 @@ template <int HD, int CT, bool PACKED> __global__ void __launch_bounds__(64 * kF
 }
 
 // Joins the splits of a sequence's kv head, a column at a time: a float4 of every N-th split a thread, four under way.
-template <int HD, int COLUMNS> __global__ void __launch_bounds__(256) kv4_few_join_kernel(Kv4Params p) {
+template <int HD, int COLUMNS> __device__ __forceinline__ void join_few(const Kv4Params &p, uint32_t unit, uint32_t from, uint32_t step) {
     constexpr int C = HD / 4, N = 256 / C, Z = 4;
     __shared__ float4 os[N][C];
     __shared__ float ls[N], ms[N];
-    const Share t = share_of<true, COLUMNS>(p, blockIdx.x / p.c.nkv);
+    const Share t = share_of<true, COLUMNS>(p, unit / p.c.nkv);
     if (t.splits < 2) return;
-    const int head = (int)(blockIdx.x % p.c.nkv), tid = threadIdx.x, c = tid % C, n = tid / C;
+    const int head = (int)(unit % p.c.nkv), tid = threadIdx.x, c = tid % C, n = tid / C;
     const uint32_t count = t.q.rows * p.group;
-    for (uint32_t column = blockIdx.y; column < count; column += gridDim.y) {
+    for (uint32_t column = from; column < count; column += step) {
         const uint32_t tile = column / COLUMNS, within = column - tile * COLUMNS;
         auto at = [&](uint32_t z) { return ((size_t)t.slot + (tile * t.splits + min(z, t.splits - 1)) * p.c.nkv + head) * COLUMNS + within; };
         float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
@@ -747,6 +749,9 @@ template <int HD, int COLUMNS> __global__ void __launch_bounds__(256) kv4_few_jo
         }
         __syncthreads();
     }
+}
+template <int HD, int COLUMNS> __global__ void __launch_bounds__(256) kv4_few_join_kernel(Kv4Params p) {
+    join_few<HD, COLUMNS>(p, blockIdx.x, blockIdx.y, gridDim.y);
 }
 
 // Many columns (prompts): a workgroup takes a tile of 64 CT columns, a wavefront 16 CT of them, through a split of its
@@ -840,38 +845,49 @@ template <int HD, int CT> __global__ void __launch_bounds__(256, 2) kv4_many_ker
         const float l = xsum<32>(xsum<16>(x.l[c])), inv = l == 0.f ? 0.f : 1.f / l;
         const uint32_t column = first + 16 * c + i;
         if (column >= t.first + t.count) continue;
-        float *out = t.splits > 1 ? p.part + (size_t)t.split * p.b.rows * p.heads * HD : p.out;
+        float *out = t.splits > 1 ? p.many_part + (size_t)t.split * p.b.rows * p.heads * HD : p.out;
         float *to = column_of(out, p, t.q, head, column, HD);
 #pragma unroll
         for (int d = 0; d < HD / 16; d++)
             *reinterpret_cast<float4 *>(to + 16 * d + 4 * g) = make_float4(x.o[c][d][0] * inv, x.o[c][d][1] * inv, x.o[c][d][2] * inv, x.o[c][d][3] * inv);
-        if (t.splits > 1 && g == 0) p.part_ml[(to - p.part) / HD] = make_float2(x.m[c], l);
+        if (t.splits > 1 && g == 0) p.many_part_ml[(to - p.many_part) / HD] = make_float2(x.m[c], l);
     }
 }
-
 // The splits of a row's heads joined, a thread four dims.
-template <int HD, int COLUMNS> __global__ void __launch_bounds__(256) kv4_many_join_kernel(Kv4Params p) {
+template <int HD, int COLUMNS> __device__ __forceinline__ void join_many(const Kv4Params &p, uint32_t row, uint32_t block) {
     const int splits = (int)splits_of(p, all_tiles<COLUMNS>(p));
     if (splits == 1) return;
-    const Sequence q = sequence_of_row(p.b, blockIdx.x);
+    const Sequence q = sequence_of_row(p.b, row);
     if (q.rows * p.group <= p.few) return;  // (none's, or the other kernel's)
-    const uint32_t u = blockIdx.y * 256 + threadIdx.x;
+    const uint32_t u = block * 256 + threadIdx.x;
     if (u < (uint32_t)p.heads * (HD / 4)) {
-        const size_t at = (size_t)blockIdx.x * p.heads + u / (HD / 4), each = (size_t)p.b.rows * p.heads;
+        const size_t at = (size_t)row * p.heads + u / (HD / 4), each = (size_t)p.b.rows * p.heads;
         const int d = 4 * (int)(u % (HD / 4));
         float m = -INFINITY, l = 0.f;
-        for (int z = 0; z < splits; z++) m = fmaxf(m, p.part_ml[z * each + at].x);
+        for (int z = 0; z < splits; z++) m = fmaxf(m, p.many_part_ml[z * each + at].x);
         m = finite(m);
         float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
         for (int z = 0; z < splits; z++) {
-            const float2 ml = p.part_ml[z * each + at];
-            const float4 v = *reinterpret_cast<const float4 *>(p.part + (z * each + at) * HD + d);
+            const float2 ml = p.many_part_ml[z * each + at];
+            const float4 v = *reinterpret_cast<const float4 *>(p.many_part + (z * each + at) * HD + d);
             const float f = __builtin_amdgcn_exp2f(ml.x - m) * ml.y;
             l += f;
             o.x = fmaf(f, v.x, o.x), o.y = fmaf(f, v.y, o.y), o.z = fmaf(f, v.z, o.z), o.w = fmaf(f, v.w, o.w);
         }
         const float inv = l == 0.f ? 0.f : 1.f / l;
         *reinterpret_cast<float4 *>(p.out + at * HD + d) = make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv);
+    }
+}
+template <int HD, int COLUMNS> __global__ void __launch_bounds__(256) kv4_many_join_kernel(Kv4Params p) {
+    join_many<HD, COLUMNS>(p, blockIdx.x, blockIdx.y);
+}
+// Both joins in one launch (a small batch's time is its launches').  x: `units` of the one, then the rows of the other; y:
+// few_y and many_y of them.
+template <int HD, int FEW, int MANY> __global__ void __launch_bounds__(256) kv4_both_join_kernel(Kv4Params p, uint32_t units, uint32_t few_y, uint32_t many_y) {
+    if (blockIdx.x < units) {
+        if (blockIdx.y < few_y) join_few<HD, FEW>(p, blockIdx.x, blockIdx.y, few_y);
+    } else if (blockIdx.y < many_y) {
+        join_many<HD, MANY>(p, blockIdx.x - units, blockIdx.y);
     }
 }
 
@@ -891,56 +907,70 @@ hipError_t launch_kv4_attention(const Kv4Attn &a, int cus, hipStream_t s) {
     p.plan = (uint32_t *)a.part;
     const size_t plan_floats = planned ? (Plan::words(a.b.sequences) + 3) / 4 * 4 : 0;
     if (a.part_floats < plan_floats + 4 * 64 * 260) return hipErrorInvalidValue;
-    p.part = a.part + plan_floats;
-    const size_t part_floats = a.part_floats - plan_floats;
-    auto plan = [&](auto f, auto m) {
-        if (planned) hipLaunchKernelGGL((kv4_plan_kernel<decltype(f)::value, decltype(m)::value>), dim3(1), dim3(1024), 0, s, p);
-    };
-    auto few = [&](auto h, auto tiles, auto packed, auto prompt) {
-        constexpr int HD = decltype(h)::value, CT = decltype(tiles)::value;
-        constexpr bool PACKED = decltype(packed)::value;
-        constexpr uint64_t N = PACKED ? 4 : 16 * CT;
-        p.wgs = 2 * cus;
-        while (p.wgs > 1 && 2 * p.wgs * N * (HD + 2) > part_floats) p.wgs /= 2;
-        p.part_ml = (float2 *)(p.part + (size_t)2 * p.wgs * N * HD);
-        const uint64_t columns = std::min<uint64_t>(most, limit), tiles_of = (columns + N - 1) / N;
-        const uint64_t per = (blocks + kLeastBlocks - 1) / kLeastBlocks, all_tiles = a.b.sequences * nkv * tiles_of;  // splits of a tile, and tiles, at most
-        const uint64_t items = std::min(p.wgs + all_tiles, all_tiles * per);
-        plan(std::integral_constant<int, (int)N>{}, std::integral_constant<int, 64 * decltype(prompt)::value>{});
-        hipLaunchKernelGGL((kv4_few_kernel<HD, CT, PACKED>), dim3((unsigned)items), dim3(64 * kFewWaves), 0, s, p);
-        if (per == 1) return;
+    auto go = [&](auto h, auto ct_few, auto ct_many) {
+        constexpr int HD = decltype(h)::value, FEW = decltype(ct_few)::value, MANY = decltype(ct_many)::value;
+        constexpr uint64_t M = 64 * MANY;
+        const bool several = a.b.sequences > 1, many = most > p.few;
+        const uint64_t units = a.b.sequences * nkv, columns = std::min<uint64_t>(most, limit);
+        const uint64_t n = many || most > 16 ? 16 * FEW : most > 4 ? 16 : 4;  // columns of a few-column item
+        const uint64_t per = (blocks + kLeastBlocks - 1) / kLeastBlocks;      // its splits, at most
+        uint64_t few_items = 0, many_items = 0;
+        float *part = a.part + plan_floats;
+        size_t part_floats = a.part_floats - plan_floats;
+        if (p.few) {
+            p.wgs = 2 * cus;
+            while (p.wgs > 1 && 2 * p.wgs * n * (HD + 2) > part_floats / 2) p.wgs /= 2;
+            const uint64_t tiles = units * ((columns + n - 1) / n), slots = 2 * (uint64_t)p.wgs * n;
+            few_items = std::min(p.wgs + tiles, tiles * per);
+            p.part = part, p.part_ml = (float2 *)(part + slots * HD);
+            part += slots * (HD + 2), part_floats -= slots * (HD + 2);
+        }
+        if (many) {
+            // tiles of a sequence alone; of several, at most and at least as many, however the rows are theirs
+            const uint64_t few_columns = (uint64_t)p.few * a.b.sequences;
+            const uint64_t most_tiles = several ? all / M + std::min<uint64_t>(a.b.sequences, all / (p.few + 1)) : (most + M - 1) / M;
+            const uint64_t least_tiles = several ? std::max<uint64_t>(1, all > few_columns ? (all - few_columns) / M : 1) : most_tiles;
+            const uint64_t each = (uint64_t)a.b.rows * a.heads * (HD + 2);
+            p.cus = (uint32_t)cus;
+            p.splits = (uint32_t)std::max<uint64_t>(1, std::min<uint64_t>({2 * (uint64_t)cus / (least_tiles * nkv), blocks / 8, part_floats / each}));
+            p.many_part = part, p.many_part_ml = (float2 *)(part + (size_t)p.splits * a.b.rows * a.heads * HD);
+            many_items = p.splits > 1 ? std::max<uint64_t>(most_tiles * nkv, 2 * (uint64_t)cus) : most_tiles * nkv;
+        }
         // what is resident at once, 8 workgroups a CU (40 sequences of up to 4 rows: 7.0 us, of half as many 9.1, of twice 8.5)
-        const dim3 join((unsigned)(a.b.sequences * nkv), (unsigned)std::min<uint64_t>(columns, std::max<uint64_t>(1, 8 * (uint64_t)cus / (a.b.sequences * nkv))));
-        hipLaunchKernelGGL((kv4_few_join_kernel<HD, (int)N>), join, dim3(256), 0, s, p);
-    };
-    auto many = [&](auto h, auto tiles) {
-        constexpr int HD = decltype(h)::value, CT = decltype(tiles)::value;
-        constexpr uint64_t N = 64 * CT;
-        // tiles of a sequence alone; of several, at most and at least as many, however the rows are theirs
-        const bool one = a.b.sequences == 1;
-        const uint64_t few_columns = (uint64_t)p.few * a.b.sequences;
-        const uint64_t most_tiles = one ? (most + N - 1) / N : all / N + std::min<uint64_t>(a.b.sequences, all / (p.few + 1));
-        const uint64_t least_tiles = one ? most_tiles : std::max<uint64_t>(1, all > few_columns ? (all - few_columns) / N : 1);
-        const uint64_t each = (uint64_t)a.b.rows * a.heads * (HD + 2);
-        p.cus = (uint32_t)cus;
-        p.splits = (uint32_t)std::max<uint64_t>(1, std::min<uint64_t>({2 * (uint64_t)cus / (least_tiles * nkv), blocks / 8, part_floats / each}));
-        p.part_ml = (float2 *)(p.part + (size_t)p.splits * a.b.rows * a.heads * HD);
-        const uint64_t items = p.splits > 1 ? std::max<uint64_t>(most_tiles * nkv, 2 * (uint64_t)cus) : most_tiles * nkv;
-        hipLaunchKernelGGL((kv4_many_kernel<HD, CT>), dim3((unsigned)items), dim3(256), 0, s, p);
-        if (p.splits > 1)
-            hipLaunchKernelGGL((kv4_many_join_kernel<HD, (int)N>), dim3(a.b.rows, (a.heads * (HD / 4) + 255) / 256), dim3(256), 0, s, p);
-    };
-    auto go = [&](auto h, auto one, auto more, auto prompt) {
-        if (p.few && most <= 4) few(h, one, std::true_type{}, prompt);
-        else if (p.few && most <= 16) few(h, one, std::false_type{}, prompt);
-        else if (p.few) few(h, more, std::false_type{}, prompt);
-        if (most > p.few) many(h, prompt);
+        const unsigned few_y = (unsigned)std::min<uint64_t>(columns, std::max<uint64_t>(1, 8 * (uint64_t)cus / units));
+        const unsigned many_y = (unsigned)((a.heads * (HD / 4) + 255) / 256);
+        auto plan = [&](auto f) {
+            if (planned) hipLaunchKernelGGL((kv4_plan_kernel<decltype(f)::value, (int)M>), dim3(1), dim3(1024), 0, s, p);
+        };
+        auto few = [&](auto ct, auto packed) {
+            constexpr int CT = decltype(ct)::value, N = FewItem<HD, CT, decltype(packed)::value>::N;
+            plan(std::integral_constant<int, N>{});
+            hipLaunchKernelGGL((kv4_few_kernel<HD, CT, decltype(packed)::value>), dim3((unsigned)few_items), dim3(64 * kFewWaves), 0, s, p);
+            if (per > 1 && !many) hipLaunchKernelGGL((kv4_few_join_kernel<HD, N>), dim3((unsigned)units, few_y), dim3(256), 0, s, p);
+        };
+        if (!p.few) {
+            hipLaunchKernelGGL((kv4_many_kernel<HD, MANY>), dim3((unsigned)many_items), dim3(256), 0, s, p);
+            if (p.splits > 1) hipLaunchKernelGGL((kv4_many_join_kernel<HD, (int)M>), dim3(a.b.rows, many_y), dim3(256), 0, s, p);
+        } else if (many) {
+            few(ct_few, std::false_type{});
+            hipLaunchKernelGGL((kv4_many_kernel<HD, MANY>), dim3((unsigned)many_items), dim3(256), 0, s, p);
+            const unsigned rows = p.splits > 1 ? a.b.rows : 0;
+            if (per > 1)
+                hipLaunchKernelGGL((kv4_both_join_kernel<HD, 16 * FEW, (int)M>), dim3((unsigned)units + rows, rows ? std::max(few_y, many_y) : few_y), dim3(256), 0, s, p,
+                                   (uint32_t)units, few_y, many_y);
+        } else if (most <= 4) {
+            few(std::integral_constant<int, 1>{}, std::true_type{});
+        } else if (most <= 16) {
+            few(std::integral_constant<int, 1>{}, std::false_type{});
+        } else {
+            few(ct_few, std::false_type{});
+        }
     };
     switch (a.c.hd) {
-    case 64: go(std::integral_constant<int, 64>{}, std::integral_constant<int, 1>{}, std::integral_constant<int, 4>{}, std::integral_constant<int, 2>{}); break;
-    case 96: go(std::integral_constant<int, 96>{}, std::integral_constant<int, 1>{}, std::integral_constant<int, 2>{}, std::integral_constant<int, 2>{}); break;
-    case 128: go(std::integral_constant<int, 128>{}, std::integral_constant<int, 1>{}, std::integral_constant<int, 2>{}, std::integral_constant<int, 2>{}); break;
-    case 256: go(std::integral_constant<int, 256>{}, std::integral_constant<int, 1>{}, std::integral_constant<int, 1>{}, std::integral_constant<int, 1>{}); break;
+    case 64: go(std::integral_constant<int, 64>{}, std::integral_constant<int, 4>{}, std::integral_constant<int, 2>{}); break;
+    case 96: go(std::integral_constant<int, 96>{}, std::integral_constant<int, 2>{}, std::integral_constant<int, 2>{}); break;
+    case 128: go(std::integral_constant<int, 128>{}, std::integral_constant<int, 2>{}, std::integral_constant<int, 2>{}); break;
+    case 256: go(std::integral_constant<int, 256>{}, std::integral_constant<int, 1>{}, std::integral_constant<int, 1>{}); break;
     default: return hipErrorInvalidValue;
     }
     return hipGetLastError();

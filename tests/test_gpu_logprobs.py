@@ -140,3 +140,22 @@ def test_beside_the_sampler(hip_ctx):
     hip_ctx.token_logprobs(lb, out, y, 5, 32000, top=2, top_tokens=ids, top_logprobs=best)
     hip_ctx.commit()
     assert np.array_equal(out.read(np.uint32), ids.read(np.uint32)[::2]) and np.array_equal(y.read(), best.read()[::2])
+
+
+@pytest.mark.parametrize("vocab", [200, 1024, 4096, 4097, 8191, 8192, 8193])
+@pytest.mark.parametrize("top", [0, 1, 13, 48, 64])
+def test_rows_about_the_size_of_a_slice(hip_ctx, vocab, top):
+    """Rows that one workgroup answers, and those that two do: ordinary ones, ties by the hundred, few finite logits, none,
+    infinities and NaN among them."""
+    rng = np.random.default_rng(vocab * 3 + top)
+    x = logits(rng, 10, vocab)
+    x[1] = np.round(x[1])
+    x[2, :] = -2.5
+    x[3, rng.permutation(vocab)[:vocab - 20]] = -np.inf
+    x[4, rng.permutation(vocab)[:vocab // 2]] = np.nan
+    x[5, :] = -np.inf
+    x[6, vocab // 3] = np.inf
+    x[7, :] = np.nan
+    x[8, :vocab // 2] = 3.0  # (a wavefront's list overflows)
+    x[9] = np.sort(x[9])
+    check(hip_ctx, x, list(rng.integers(0, vocab, 9)) + [vocab], top, stride=vocab + 3)

@@ -7,7 +7,7 @@
 // Two launches, one pass over the logits:
 //   slices  a workgroup per 4096 logits (8192 where those fill the device), held in registers: the largest, the
 //           sums relative to it, and its k best in order;
-//   rows    a workgroup per row joins its slices.
+//   rows    a workgroup per row joins its slices (rows of up to 8192 logits: one slice, which is the answer).
 // The k best of a slice: a value that k logits reach leaves few candidates, and a candidate's place is the count of those
 // above it: no sort, no dependence on the order of arrival.
 //
@@ -110,8 +110,41 @@ template <int CTRL> __device__ __forceinline__ float max_moved(float v) {
 __device__ __forceinline__ float quad_max(float v) { return max_moved<0x4E>(max_moved<0xB1>(v)); }
 __device__ __forceinline__ float row_max(float v) { return max_moved<0x140>(max_moved<0x141>(quad_max(v))); }
 
-// A workgroup per slice of 256 V logits.  Its k best are of the finite ones alone.
-template <int V> __global__ void __launch_bounds__(kThreads) logprobs_slice_kernel(TokenLogprobs p, LogprobsWork w) {
+__device__ __forceinline__ float logprob_of(float v, float largest, double log_s) {
+    return (float)(((double)(v != v ? -INFINITY : v) - (double)largest) - log_s);
+}
+// A row's log probability and entropy, by the first lane: s the weights beside one of the largest, t = sum e^d d.
+__device__ __forceinline__ double finish_row(const TokenLogprobs &p, uint32_t row, float largest, double s, double t, uint32_t token, float given, bool first) {
+    const double nan = (double)__uint_as_float(0x7FC00000u), log_s = isfinite(largest) ? log1p(s) : nan;
+    if (first) {
+        p.out[row] = token < p.vocab ? logprob_of(given, largest, log_s) : (float)nan;
+        if (p.entropy) p.entropy[row] = (float)(log_s - t / (1.0 + s));
+    }
+    return log_s;
+}
+__device__ __forceinline__ void put_best(const TokenLogprobs &p, uint32_t row, int rank, uint32_t token, float v, float largest, double log_s) {
+    p.top_tokens[(size_t)row * p.k + rank] = token;
+    p.top[(size_t)row * p.k + rank] = logprob_of(v, largest, log_s);
+}
+// Fewer finite logits than k: `have` are placed, all of them, +infinities too; the first of the others follow.
+template <int THREADS> __device__ __forceinline__ void put_others(const TokenLogprobs &p, uint32_t row, uint32_t have, float largest, double log_s, uint32_t *taken) {
+    const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
+    for (uint32_t at = 0; have < (uint32_t)p.k && at < p.vocab; at += THREADS) {
+        const float v = at + tid < p.vocab ? p.x[(size_t)row * p.stride + at + tid] : 0.f;
+        const bool none = at + tid < p.vocab && (v != v || v == -INFINITY);
+        const u64 which = __ballot(none);
+        __syncthreads();
+        if (lane == 0) taken[wave] = (uint32_t)__popcll(which);
+        __syncthreads();
+        uint32_t rank = have + (uint32_t)__popcll(which & ((1ull << lane) - 1)), all = 0;
+        for (int i = 0; i < THREADS / 64; i++) rank += i < wave ? taken[i] : 0u, all += taken[i];
+        if (none && rank < (uint32_t)p.k) put_best(p, row, (int)rank, at + tid, -INFINITY, largest, log_s);
+        have += all;
+    }
+}
+
+// A workgroup per slice of 256 V logits.  Its k best are of the finite ones alone.  WHOLE: the slice is the row.
+template <int V, bool WHOLE> __global__ void __launch_bounds__(kThreads) logprobs_slice_kernel(TokenLogprobs p, LogprobsWork w) {
     __shared__ __align__(16) u64 candidates[kCandidates];
     __shared__ u64 best[4];
     __shared__ double sums[2][4];
@@ -122,6 +155,12 @@ template <int V> __global__ void __launch_bounds__(kThreads) logprobs_slice_kern
     const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
     const float *x = p.x + (size_t)row * p.stride + first;
     const uint32_t n = min(w.logits, p.vocab - first);
+    uint32_t token = 0;
+    float given = 0.f;
+    if (WHOLE && wave == 0) {
+        token = p.tokens[row];
+        if (token < p.vocab) given = x[token];
+    }
     float v[V];
     auto at = [&](int j) { return (uint32_t)((j / 4 * kThreads + tid) * 4 + j % 4); };
 #pragma unroll
@@ -199,16 +238,22 @@ template <int V> __global__ void __launch_bounds__(kThreads) logprobs_slice_kern
     if (lane == 63) sums[0][wave] = s, sums[1][wave] = t, counts[wave] = count;
     __syncthreads();
     const size_t out = (size_t)row * w.slices + slice;
-    if (tid == 0)
-        w.sums[out] = {top, counts[0] + counts[1] + counts[2] + counts[3], (sums[0][0] + sums[0][1]) + (sums[0][2] + sums[0][3]),
-                       (sums[1][0] + sums[1][1]) + (sums[1][2] + sums[1][3])};
+    const SliceSums all = {top, counts[0] + counts[1] + counts[2] + counts[3], (sums[0][0] + sums[0][1]) + (sums[0][2] + sums[0][3]),
+                           (sums[1][0] + sums[1][1]) + (sums[1][2] + sums[1][3])};
+    double log_s = 0.0;
+    if constexpr (WHOLE) log_s = finish_row(p, row, top, all.s + ((double)all.count - 1.0), all.t, token, given, tid == 0);
+    else if (tid == 0) w.sums[out] = all;
     if (p.k == 0) return;
-    u64 *to = w.top + out * p.k;
+    auto put = [&](int rank, u64 key) {
+        if constexpr (WHOLE) put_best(p, row, rank, index_of_key(key), value_of_key(key), top, log_s);
+        else w.top[out * p.k + rank] = key;
+    };
     const int c0 = found[0], c1 = c0 + found[1], c2 = c1 + found[2], c = c2 + found[3];
     // the i-th of the wavefronts' candidates
     auto candidate = [&](int i) { return candidates[i < c0 ? i : i < c1 ? EACH + i - c0 : i < c2 ? 2 * EACH + i - c1 : 3 * EACH + i - c2]; };
     if (max(max(found[0], found[1]), max(found[2], found[3])) <= EACH) {
-        for (int i = c + tid; i < p.k; i += kThreads) to[i] = 0;  // (fewer than that)
+        if constexpr (WHOLE) put_others<kThreads>(p, row, (uint32_t)c, top, log_s, counts);
+        else for (int i = c + tid; i < p.k; i += kThreads) put(i, 0);  // (fewer than that)
         if (c <= 64) {  // a lane each, every wavefront against its own
             const u64 mine = lane < c ? candidate(lane) : 0ull;
             int rank = 0;
@@ -221,7 +266,7 @@ template <int V> __global__ void __launch_bounds__(kThreads) logprobs_slice_kern
             }
             atomicAdd(&ranks[lane], rank);
             __syncthreads();
-            if (wave == 0 && lane < c && ranks[lane] < p.k) to[ranks[lane]] = mine;
+            if (wave == 0 && lane < c && ranks[lane] < p.k) put(ranks[lane], mine);
             return;
         }
         for (int i = tid; i < c; i += kThreads) {
@@ -235,13 +280,14 @@ template <int V> __global__ void __launch_bounds__(kThreads) logprobs_slice_kern
 #pragma unroll
                     for (int e = 0; e < 4; e++) rank += (j + 2 * e < found[q] && o[e].x > mine) + (j + 2 * e + 1 < found[q] && o[e].y > mine);
                 }
-            if (rank < p.k) to[rank] = mine;
+            if (rank < p.k) put(rank, mine);
         }
         return;
     }
     // many are equal, or the best crowd a few rows of lanes: one after the other
     u64 last = ~0ull;
-    for (int i = 0; i < p.k; i++) {
+    int i = 0;
+    for (; i < p.k; i++) {
         u64 k = 0;
 #pragma unroll
         for (int j = 0; j < V; j++) {
@@ -253,8 +299,10 @@ template <int V> __global__ void __launch_bounds__(kThreads) logprobs_slice_kern
         if (lane == 0) best[wave] = k;
         __syncthreads();
         last = max(max(best[0], best[1]), max(best[2], best[3]));
-        if (tid == 0) to[i] = last;
+        if (WHOLE && last == 0) break;
+        if (tid == 0) put(i, last);
     }
+    if constexpr (WHOLE) put_others<kThreads>(p, row, (uint32_t)i, top, log_s, counts);
 }
 
 // A workgroup per row: the last wavefront joins the slices' sums, a lane each, while the others find the best.
@@ -308,7 +356,6 @@ __global__ void __launch_bounds__(kRowThreads) logprobs_row_kernel(TokenLogprobs
                 candidates[atomicAdd(&found, 1)] = k;
             }
     }
-    auto logprob = [&](float v, float largest, double log_s) { return (float)(((double)(v != v ? -INFINITY : v) - (double)largest) - log_s); };
     if (wave == kLists) {  // meanwhile the sums
         const float largest = wave_max_f32(own.top);
         // slices that have the largest give its count, the others their weights
@@ -318,38 +365,15 @@ __global__ void __launch_bounds__(kRowThreads) logprobs_row_kernel(TokenLogprobs
             s = f * all, t = f * (own.t + d * all);
         }
         s = wave_sum(s) + (wave_sum(count) - 1.0), t = wave_sum(t);
-        const double nan = (double)__uint_as_float(0x7FC00000u), log_s = isfinite(largest) ? log1p(s) : nan;
-        if (lane == 0) {
-            shared_log = log_s, shared_largest = largest;
-            p.out[row] = token < p.vocab ? logprob(given, largest, log_s) : (float)nan;
-            if (p.entropy) p.entropy[row] = (float)(log_s - t / (1.0 + s));
-        }
+        const double log_s = finish_row(p, row, largest, s, t, token, given, lane == 0);
+        if (lane == 0) shared_log = log_s, shared_largest = largest;
     }
     if (p.k == 0) return;
     __syncthreads();
     const double log_s = shared_log;
     const float largest = shared_largest;
-    place(candidates, found, p.k, [&](int rank, u64 k) {
-        p.top_tokens[(size_t)row * p.k + rank] = index_of_key(k);
-        p.top[(size_t)row * p.k + rank] = logprob(value_of_key(k), largest, log_s);
-    });
-    // fewer finite logits than k: all of them are placed, +infinities too; the first of the others follow
-    uint32_t have = (uint32_t)found;
-    for (uint32_t at = 0; have < (uint32_t)p.k && at < p.vocab; at += kRowThreads) {
-        const float v = at + tid < p.vocab ? p.x[(size_t)row * p.stride + at + tid] : 0.f;
-        const bool none = at + tid < p.vocab && (v != v || v == -INFINITY);
-        const u64 which = __ballot(none);
-        __syncthreads();
-        if (lane == 0) taken[wave] = (uint32_t)__popcll(which);
-        __syncthreads();
-        uint32_t rank = have + (uint32_t)__popcll(which & ((1ull << lane) - 1)), all = 0;
-        for (int i = 0; i < kRowThreads / 64; i++) rank += i < wave ? taken[i] : 0u, all += taken[i];
-        if (none && rank < (uint32_t)p.k) {
-            p.top_tokens[(size_t)row * p.k + rank] = at + tid;
-            p.top[(size_t)row * p.k + rank] = logprob(-INFINITY, largest, log_s);
-        }
-        have += all;
-    }
+    place(candidates, found, p.k, [&](int rank, u64 k) { put_best(p, row, rank, index_of_key(k), value_of_key(k), largest, log_s); });
+    put_others<kRowThreads>(p, row, (uint32_t)found, largest, log_s, taken);
 }
 
 }  // namespace
@@ -357,7 +381,9 @@ __global__ void __launch_bounds__(kRowThreads) logprobs_row_kernel(TokenLogprobs
 hipError_t launch_token_logprobs(const TokenLogprobs &a, int cus, hipStream_t s) {
     // The fewer workgroups the rows make, the smaller their slices.  (Of 4096 logits and of 8192: a row of 151936 4.7 us and
     // 5.5, 8 rows 6.3 and 6.8, 33 of 128256 12.0 and 10.8, 511 of 151936 67 and 57.)
-    const uint32_t slice = (uint64_t)a.rows * ((a.vocab + 4095) / 4096) <= 2ull * cus ? 4096 : 8192;
+    // A row that is one slice needs no second launch (200 rows of 1500 logits, 20 tokens: 6.3 us, with it 5.9 and 4.1).
+    const bool whole = a.vocab <= 8192;
+    const uint32_t slice = a.vocab <= 4096 || (!whole && (uint64_t)a.rows * ((a.vocab + 4095) / 4096) <= 2ull * cus) ? 4096 : 8192;
     LogprobsWork w{};
     w.slices = (a.vocab + slice - 1) / slice;
     w.logits = ((a.vocab + w.slices - 1) / w.slices + 3) / 4 * 4;  // alike, so that the last one's lanes aren't mostly empty
@@ -372,8 +398,13 @@ hipError_t launch_token_logprobs(const TokenLogprobs &a, int cus, hipStream_t s)
         if (a.k) p.top = a.top + (size_t)r * a.k, p.top_tokens = a.top_tokens + (size_t)r * a.k;
         w.sums = (SliceSums *)a.work, w.top = (u64 *)(w.sums + (size_t)p.rows * w.slices);
         const dim3 grid(p.rows * w.slices);
-        if (slice == 8192) hipLaunchKernelGGL(logprobs_slice_kernel<32>, grid, dim3(kThreads), 0, s, p, w);
-        else hipLaunchKernelGGL(logprobs_slice_kernel<16>, grid, dim3(kThreads), 0, s, p, w);
+        if (whole) {
+            if (slice == 8192) hipLaunchKernelGGL((logprobs_slice_kernel<32, true>), grid, dim3(kThreads), 0, s, p, w);
+            else hipLaunchKernelGGL((logprobs_slice_kernel<16, true>), grid, dim3(kThreads), 0, s, p, w);
+            continue;
+        }
+        if (slice == 8192) hipLaunchKernelGGL((logprobs_slice_kernel<32, false>), grid, dim3(kThreads), 0, s, p, w);
+        else hipLaunchKernelGGL((logprobs_slice_kernel<16, false>), grid, dim3(kThreads), 0, s, p, w);
         hipLaunchKernelGGL(logprobs_row_kernel, dim3(p.rows), dim3(kRowThreads), 0, s, p, w);
     }
     return hipGetLastError();

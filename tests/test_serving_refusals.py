@@ -124,7 +124,7 @@ def test_append(host):
     tables = batch(host)
     w = host.buffer(256)
 
-    def call(c=good, layer=1, b=tables, d=heads(host, q_norm=w, k_norm=w), src=src, k=2048, v=3072, stride=1100, q=8, qo=0, out=q_out, oo=0, os=0, ctx=host.ctx):
+    def call(c=good, layer=1, b=tables, d=heads(host, q_norm=w, k_norm=w), src=src, k=2048, v=4 * 768, stride=1100, q=8, qo=0, out=q_out, oo=0, os=0, ctx=host.ctx):
         return host.call("ziggy_hip_kv4_append", ctx, ref(c), U(layer), ref(b), ref(d), src, Z(k), Z(v), Z(stride), U(q), Z(qo), out, Z(oo), Z(os))
 
     try_all(host, call, {}, bad_caches_and_batches(host, good) + bad_heads(host) + [

@@ -84,7 +84,8 @@ __device__ __forceinline__ void put(float *to, float4 v, int streams) {
 // a head a team of lanes.
 template <int LAYOUT, bool CACHE> __global__ void __launch_bounds__(256) head_rows_kernel(HeadRows p, HeadPlan plan) {
     extern __shared__ __align__(16) char lds[];
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), team = plan.team, u = lane % team, slot = lane / team;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+    const int team = plan.team, u = lane % team, slot = lane / team;
     const uint32_t unit = blockIdx.x * 4 + wave, r = unit / plan.chunks, chunk = unit - r * plan.chunks;
     if (r >= p.rows) return;
     const int half = p.rotates ? p.rd / 2 : 0, i0 = 4 * u, hp = 64 / team;
@@ -279,7 +280,8 @@ template <int LAYOUT, bool CACHE> __global__ void __launch_bounds__(256) head_ro
 #pragma unroll
                 for (int e = 0; e < 4; e++) {
                     const int n4 = 4 * c + e, d = n4 / g_n, tt = n4 % g_n;
-                    bytes[e] = marked ? 0u : __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(0u, value_at[32 * tt + d], value_at[32 * tt + 16 + d], scale_at[tt], 0) & 255u;
+                    const uint32_t two = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(0u, value_at[32 * tt + d], value_at[32 * tt + 16 + d], scale_at[tt], 0);
+                    bytes[e] = marked ? 0u : two & 255u;
                 }
                 if (g_n % 4 == 0) {
                     const int d = 4 * c / g_n, tt = 4 * c % g_n;

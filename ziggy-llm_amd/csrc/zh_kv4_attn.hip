@@ -366,7 +366,10 @@ template <int HD> struct Lane4 {
                 const int n = (j + e) * G + t;  // byte of this position's dims
                 const float scale = scale_of(vs[n >> 2], n & 3);
                 const uint32_t word = v[n >> 2];
-                y[e] = (n & 3) == 0 ? widen<0>(word, scale) : (n & 3) == 1 ? widen<1>(word, scale) : (n & 3) == 2 ? widen<2>(word, scale) : widen<3>(word, scale);
+                y[e] = (n & 3) == 0   ? widen<0>(word, scale)
+                       : (n & 3) == 1 ? widen<1>(word, scale)
+                       : (n & 3) == 2 ? widen<2>(word, scale)
+                                      : widen<3>(word, scale);
             }
             a[0][j / 2] = __builtin_amdgcn_perm(y[1], y[0], 0x05040100u);
             a[1][j / 2] = __builtin_amdgcn_perm(y[1], y[0], 0x07060302u);
@@ -471,7 +474,8 @@ template <int HD, int CT, int AWAY, bool PACKED = false> struct Columns {
                     for (int c = 0; c < CT; c++)
 #pragma unroll
                         for (int pt = 0; pt < 2; pt++)
-                            s[h][c][pt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a[pt], k < NEAR ? q[c][t][k < NEAR ? k : 0] : far[c][k < NEAR ? 0 : k - NEAR], s[h][c][pt], 0, 0, 0);
+                            s[h][c][pt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
+                                a[pt], k < NEAR ? q[c][t][k < NEAR ? k : 0] : far[c][k < NEAR ? 0 : k - NEAR], s[h][c][pt], 0, 0, 0);
                 if constexpr (HOLD) __builtin_amdgcn_sched_barrier(0);  // (or the operands of all steps take registers at once)
             }
         }
@@ -546,7 +550,8 @@ template <int HD, int CT, int AWAY, bool PACKED = false> struct Columns {
 #pragma unroll
                     for (int c = 0; c < CT; c++)
 #pragma unroll
-                        for (int d = 0; d < 2; d++) o[c][2 * t + d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(b[d], w[c][k], o[c][2 * t + d], 0, 0, 0);
+                        for (int d = 0; d < 2; d++)
+                            o[c][2 * t + d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(b[d], w[c][k], o[c][2 * t + d], 0, 0, 0);
                 if constexpr (HOLD) __builtin_amdgcn_sched_barrier(0);
             }
         }
@@ -589,7 +594,8 @@ template <int HD, int CT, int AWAY, bool PACKED = false> struct Columns {
             const uint32_t next = page(j);
             after.load_k(p.c, next, head, half(j)), after.load_v(p.c, next, head, half(j));
             if (edge) now.clear_v(r.first - at(i), hidden ? -1 : r.last - at(i));
-            take<1, HOLD>(p.qscale, at(i), edge, hidden, [&](int, int t, int pt) { return now.key(t, pt); }, [&](int, int t, fb8(&b)[2]) { now.values(t, b); }, [] {});
+            take<1, HOLD>(p.qscale, at(i), edge, hidden, [&](int, int t, int pt) { return now.key(t, pt); },
+                          [&](int, int t, fb8(&b)[2]) { now.values(t, b); }, [] {});
             i++;
         };
         while (i < n) {
@@ -608,13 +614,15 @@ __device__ __forceinline__ float *column_of(float *out, const Kv4Params &p, cons
 // batch of 48 103 us instead of 84.  One workgroup a share of exactly as many blocks, sequences cut wherever it ends: 79
 // instead of 75, 4113 positions 10.1 instead of 7.5, for the registers and the chain of loads of every unit in a row.)
 template <int HD, int CT, bool PACKED> struct FewItem {
-    static constexpr int N = PACKED ? 4 : 16 * CT, AWAY = !PACKED && HD * CT > 128 ? 2 : 0, PIECES = CT * (HD / 32) * AWAY * 64;  // of a wavefront (16 bytes each)
+    static constexpr int N = PACKED ? 4 : 16 * CT, AWAY = !PACKED && HD * CT > 128 ? 2 : 0;
+    static constexpr int PIECES = CT * (HD / 32) * AWAY * 64;  // of a wavefront (16 bytes each)
     static constexpr int OUTPUTS = kFewWaves * N * (HD + 4), HELD = kFewWaves * PIECES * 4;
     static constexpr int LDS = (OUTPUTS > HELD ? OUTPUTS : HELD) + 2 * kFewWaves * N;
 };
 // lds: the queries' pieces, then the wavefronts' outputs, and their maxima and sums.  SLOT: columns of a slot.
 template <int HD, int CT, bool PACKED, int SLOT>
-__device__ __forceinline__ void few_item(const Kv4Params &p, const Share &t, int head, const Range &r, int begin, int end, uint32_t first, uint32_t count, float *lds) {
+__device__ __forceinline__ void few_item(const Kv4Params &p, const Share &t, int head, const Range &r, int begin, int end, uint32_t first,
+                                         uint32_t count, float *lds) {
     typedef FewItem<HD, CT, PACKED> I;
     constexpr int N = I::N, C = HD / 4, AWAY = I::AWAY, PIECES = I::PIECES;
     float(*os)[N][HD + 4] = reinterpret_cast<float(*)[N][HD + 4]>(lds);
@@ -623,7 +631,8 @@ __device__ __forceinline__ void few_item(const Kv4Params &p, const Share &t, int
     Columns<HD, CT, AWAY, PACKED> x;
     typename Columns<HD, CT, AWAY, PACKED>::Raw raw;
     x.fetch(p, t.q, first, count, head, raw);
-    x.template run<(HD * CT > 128)>(p, r, t.q.index, head, begin + wave, end, kFewWaves, [&] { x.begin(p, raw, reinterpret_cast<fb8 *>(lds) + wave * PIECES); });
+    x.template run<(HD * CT > 128)>(p, r, t.q.index, head, begin + wave, end, kFewWaves,
+                                    [&] { x.begin(p, raw, reinterpret_cast<fb8 *>(lds) + wave * PIECES); });
     if (AWAY) __syncthreads();
 #pragma unroll
     for (int c = 0; c < CT; c++) {
@@ -897,7 +906,8 @@ template <int HD, int COLUMNS> __global__ void __launch_bounds__(256) kv4_many_j
 }
 // Both joins in one launch (a small batch's time is its launches').  x: `units` of the one, then the rows of the other; y:
 // few_y and many_y of them.
-template <int HD, int FEW, int MANY> __global__ void __launch_bounds__(256) kv4_both_join_kernel(Kv4Params p, uint32_t units, uint32_t few_y, uint32_t many_y) {
+template <int HD, int FEW, int MANY>
+__global__ void __launch_bounds__(256) kv4_both_join_kernel(Kv4Params p, uint32_t units, uint32_t few_y, uint32_t many_y) {
     if (blockIdx.x < units) {
         if (blockIdx.y < few_y) join_few<HD, FEW>(p, blockIdx.x, blockIdx.y, few_y);
     } else if (blockIdx.y < many_y) {
@@ -948,7 +958,8 @@ hipError_t launch_kv4_attention(const Kv4Attn &a, int cus, hipStream_t s) {
             p.cus = (uint32_t)cus;
             // Two pages a split at least, and 32 splits at most.  (180 rows at 1000 positions, 4 heads over 2 kv heads of 128, with
             // the join: 18.8 us, of four pages at least 23.8; at 8000 31.3, with 62 splits 34.2.)
-            p.splits = (uint32_t)std::max<uint64_t>(1, std::min<uint64_t>({2 * (uint64_t)cus / (least_tiles * nkv), blocks / 4, 32, part_floats / each}));
+            p.splits = (uint32_t)std::max<uint64_t>(1, std::min<uint64_t>({2 * (uint64_t)cus / (least_tiles * nkv), blocks / 4, 32,
+                                                                           part_floats / each}));
             p.many_part = part, p.many_part_ml = (float2 *)(part + (size_t)p.splits * a.b.rows * a.heads * HD);
             many_items = p.splits > 1 ? std::max<uint64_t>(most_tiles * nkv, 2 * (uint64_t)cus) : most_tiles * nkv;
         }
@@ -972,8 +983,9 @@ hipError_t launch_kv4_attention(const Kv4Attn &a, int cus, hipStream_t s) {
             hipLaunchKernelGGL((kv4_many_kernel<HD, MANY>), dim3((unsigned)many_items), dim3(256), 0, s, p);
             const unsigned rows = p.splits > 1 ? a.b.rows : 0;
             if (per > 1)
-                hipLaunchKernelGGL((kv4_both_join_kernel<HD, 16 * FEW, (int)M>), dim3((unsigned)units + rows, rows ? std::max(few_y, many_y) : few_y), dim3(256), 0, s, p,
-                                   (uint32_t)units, few_y, many_y);
+                hipLaunchKernelGGL((kv4_both_join_kernel<HD, 16 * FEW, (int)M>),
+                                   dim3((unsigned)units + rows, rows ? std::max(few_y, many_y) : few_y), dim3(256), 0, s, p, (uint32_t)units,
+                                   few_y, many_y);
         } else if (most <= 4) {
             few(std::integral_constant<int, 1>{}, std::true_type{});
         } else if (most <= 16) {

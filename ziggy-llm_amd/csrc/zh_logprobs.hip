@@ -114,7 +114,8 @@ __device__ __forceinline__ float logprob_of(float v, float largest, double log_s
     return (float)(((double)(v != v ? -INFINITY : v) - (double)largest) - log_s);
 }
 // A row's log probability and entropy, by the first lane: s the weights beside one of the largest, t = sum e^d d.
-__device__ __forceinline__ double finish_row(const TokenLogprobs &p, uint32_t row, float largest, double s, double t, uint32_t token, float given, bool first) {
+__device__ __forceinline__ double finish_row(const TokenLogprobs &p, uint32_t row, float largest, double s, double t, uint32_t token,
+                                             float given, bool first) {
     const double nan = (double)__uint_as_float(0x7FC00000u), log_s = isfinite(largest) ? log1p(s) : nan;
     if (first) {
         p.out[row] = token < p.vocab ? logprob_of(given, largest, log_s) : (float)nan;
@@ -127,7 +128,8 @@ __device__ __forceinline__ void put_best(const TokenLogprobs &p, uint32_t row, i
     p.top[(size_t)row * p.k + rank] = logprob_of(v, largest, log_s);
 }
 // Fewer finite logits than k: `have` are placed, all of them, +infinities too; the first of the others follow.
-template <int THREADS> __device__ __forceinline__ void put_others(const TokenLogprobs &p, uint32_t row, uint32_t have, float largest, double log_s, uint32_t *taken) {
+template <int THREADS>
+__device__ __forceinline__ void put_others(const TokenLogprobs &p, uint32_t row, uint32_t have, float largest, double log_s, uint32_t *taken) {
     const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
     for (uint32_t at = 0; have < (uint32_t)p.k && at < p.vocab; at += THREADS) {
         const float v = at + tid < p.vocab ? p.x[(size_t)row * p.stride + at + tid] : 0.f;
@@ -231,7 +233,8 @@ template <int V, bool WHOLE> __global__ void __launch_bounds__(kThreads) logprob
             e[i] = largest ? 0.f : exp_of(d[i]);
         }
         s += (double)(((e[0] + e[1]) + (e[2] + e[3])) + ((e[4] + e[5]) + (e[6] + e[7])));
-        t += (double)((fmaf(e[0], d[0], e[1] * d[1]) + fmaf(e[2], d[2], e[3] * d[3])) + (fmaf(e[4], d[4], e[5] * d[5]) + fmaf(e[6], d[6], e[7] * d[7])));
+        t += (double)((fmaf(e[0], d[0], e[1] * d[1]) + fmaf(e[2], d[2], e[3] * d[3])) +
+                      (fmaf(e[4], d[4], e[5] * d[5]) + fmaf(e[6], d[6], e[7] * d[7])));
     }
     s = wave_sum(s), t = wave_sum(t);
     count = running_sum(count);

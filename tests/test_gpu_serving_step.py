@@ -1,5 +1,8 @@
 """The operators that serve several sequences together, as a serving loop uses them: heads normalised and rotated, K/V
 appended to pages, attention, the output head, a draw, its log probabilities, each step's calls in one open sequence."""
+import os
+import subprocess
+import sys
 import threading
 
 import numpy as np
@@ -231,3 +234,59 @@ def test_tables_that_change_between_calls(hip_ctx):
     for i, out in enumerate(outs):
         want, bound = oracle.attention(cache, 0, b[i % 2], q, hd ** -0.5)
         assert np.all(np.abs(out.read().reshape(want.shape) - want) <= bound)
+
+WRAPPED = r"""
+import sys
+import torch
+g = torch.Generator(device="cuda").manual_seed(3)
+heads, kvh, hd, rows, vocab, pages = 4, 2, 64, 70, 3000, 4
+x = torch.randn(rows, (heads + 2 * kvh) * hd, generator=g, device="cuda")
+kc, vc = (torch.zeros(kvh * pages * 32 * hd, dtype=torch.uint8, device="cuda") for _ in range(2))
+ks, vs = (torch.zeros(kvh * pages * 2 * hd, dtype=torch.uint8, device="cuda") for _ in range(2))
+table = torch.tensor([[3, 1], [0, -1]], dtype=torch.int32, device="cuda")
+starts = torch.tensor([0, 66, 70], dtype=torch.int32, device="cuda")
+lengths = torch.tensor([66, 4], dtype=torch.int32, device="cuda")
+out = torch.full((rows, heads * hd), 7.0, device="cuda")
+logits = torch.randn(2, vocab, generator=g, device="cuda")
+tokens = torch.tensor([5, vocab - 1], dtype=torch.int32, device="cuda")
+lp = torch.zeros(2, device="cuda")
+other = torch.cuda.Stream()
+with torch.cuda.stream(other):  # made on a stream of torch's, which is waited for before the calls
+    logits = logits * 2
+torch.cuda.synchronize()
+sys.path[:0] = sys.argv[1:]
+from zhip import hip
+ctx = hip.Context(0)
+w = lambda t: ctx.wrap(t.data_ptr(), t.numel() * t.element_size())
+cache = hip.Kv4Cache(w(kc), w(ks), w(vc), w(vs), 1, kvh, hd, pages)
+batch = hip.Batch(w(table), w(starts), w(lengths), 2, 2, rows)
+src, width = w(x), (heads + 2 * kvh) * hd
+ctx.begin()
+ctx.kv4_append(cache, 0, batch, None, src, 4 * heads * hd, 4 * (heads + kvh) * hd, width)
+ctx.kv4_attention(cache, 0, batch, src, w(out), heads, q_stride=width)
+ctx.token_logprobs(w(logits), w(tokens), w(lp), 2, vocab)
+ctx.commit()
+want = torch.log_softmax(logits.double(), 1)[torch.arange(2, device="cuda"), tokens.long()]
+assert bool(((lp.double() - want).abs() <= 2.0 ** -21 + 2.0 ** -24 * want.abs()).all())
+# the same calls on buffers of the context's own
+own = hip.Kv4Cache(*(ctx.buffer(t.cpu().numpy() * 0) for t in (kc, ks, vc, vs)), 1, kvh, hd, pages)
+y = ctx.empty(4 * out.numel())
+b = hip.Batch(*(ctx.buffer(t.cpu().numpy()) for t in (table, starts, lengths)), 2, 2, rows)
+s = ctx.buffer(x.cpu().numpy())
+ctx.kv4_append(own, 0, b, None, s, 4 * heads * hd, 4 * (heads + kvh) * hd, width)
+ctx.kv4_attention(own, 0, b, s, y, heads, q_stride=width)
+assert (out.cpu().numpy().reshape(-1) == y.read()).all()
+for t, o in zip((kc, ks, vc, vs), own.buffers):
+    assert (t.cpu().numpy() == o.read("u1")).all()
+ctx.close()
+print("wrapped: fine")
+"""
+
+
+def test_torch_memory():
+    """The operators on torch's tensors, tables among them.  In a process of its own: torch brings its HIP runtime, which
+    has to be the first one loaded."""
+    pytest.importorskip("torch")
+    repo = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    r = subprocess.run([sys.executable, "-c", WRAPPED, os.path.join(repo, "ziggy-llm_amd")], capture_output=True, text=True, timeout=100)
+    assert r.returncode == 0 and "wrapped: fine" in r.stdout, r.stdout[-2000:] + r.stderr[-2000:]

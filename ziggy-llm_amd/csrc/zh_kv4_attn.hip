@@ -34,6 +34,11 @@ constexpr int kBlock = 32;  // positions of a product
 // scaled again only where one does (with every new maximum of 32 columns, 200 of 480 blocks of a prompt).  Sums of 2^30
 // weights of 2^3 and values of 6 2^92 end below 2^128.
 constexpr float kSlack = 3.f;
+// Scores in powers of two from which on the maximum, rounded, is off by more than an eighth.  Below it s qscale - max is one
+// fused step, whose exact result holds the maximum's rounding too, alike in all weights of a column.  From 2^31 on that
+// would pass the exponents there are (a lone key at a score of 10^10 had a weight of 0, or an infinite one), so past this
+// one the score is rounded as the maximum was: the largest comes to 0 whatever it is.
+constexpr float kFar = 0x1p22f;
 
 struct Kv4Params {
     Kv4Layer c;
@@ -305,6 +310,13 @@ template <int SEL> __device__ __forceinline__ uint32_t widen(uint32_t w, float s
 // (every byte with 256 of them: the same), so a shift brings the byte there and nothing is masked.
 __device__ __forceinline__ float scale_of(uint32_t w, int byte) { return __uint_as_float(byte < 3 ? w << (23 - 8 * byte) : w >> 1); }
 
+// v f - m, the product rounded
+__device__ __forceinline__ float product_less(float v, float f, float m) {
+#pragma clang fp contract(off)
+    const float z = v * f;
+    return z - m;
+}
+
 __device__ __forceinline__ float finite(float v) { return v == -INFINITY ? 0.f : v; }
 // the sum over four lanes side by side
 __device__ __forceinline__ float four(float v) {
@@ -390,6 +402,8 @@ template <int HD, int CT, int AWAY, bool PACKED = false> struct Columns {
     const fb8 *away;  // the queries' other pieces, [CT][G][AWAY][64] in LDS
     ff4 o[CT][DT];
     float m[CT], l[CT];
+    float base[CT];  // what comes off the scores: the maximum (none yet: 0), or 0 where it already is (see kFar)
+    bool far;        // some column's maximum is kFar or more either way
     int lo[CT], hi[CT];  // the positions that a column sees, both included
 
     // Columns first .. first + count - 1 of a sequence: their queries on the way, then in pieces.
@@ -420,7 +434,7 @@ template <int HD, int CT, int AWAY, bool PACKED = false> struct Columns {
     }
     __device__ __forceinline__ void begin(const Kv4Params &p, const Raw &raw, fb8 *lds) {
         const int i = threadIdx.x & 15;
-        away = lds;
+        away = lds, far = false;
 #pragma unroll
         for (int c = 0; c < CT; c++) {
 #pragma unroll
@@ -440,7 +454,7 @@ template <int HD, int CT, int AWAY, bool PACKED = false> struct Columns {
                     else lds[((c * G + k) * AWAY + e - NEAR) * 64 + (threadIdx.x & 63)] = all[e];
                 }
             }
-            m[c] = -INFINITY, l[c] = 0.f;
+            m[c] = -INFINITY, l[c] = base[c] = 0.f;
 #pragma unroll
             for (int d = 0; d < DT; d++) o[c][d] = ff4{0.f, 0.f, 0.f, 0.f};
         }
@@ -515,16 +529,34 @@ template <int HD, int CT, int AWAY, bool PACKED = false> struct Columns {
 #pragma unroll
                 for (int d = 0; d < DT; d++) o[c][d] *= was;
             }
+            bool some = false;
+#pragma unroll
+            for (int c = 0; c < CT; c++) {
+                const bool is = fabsf(finite(m[c])) >= kFar;
+                base[c] = is ? 0.f : finite(m[c]);
+                some = some || is;
+            }
+            far = __any(some);
+        }
+        if (far) {
+            const float inverse = 1.f / qscale;  // (scores are below 2^128: qscale is above 2^-106)
+#pragma unroll
+            for (int c = 0; c < CT; c++) {
+                if (fabsf(finite(m[c])) < kFar) continue;
+#pragma unroll
+                for (int h = 0; h < H; h++)
+#pragma unroll
+                    for (int e = 0; e < 8; e++) s[h][c][e >> 2][e & 3] = product_less(s[h][c][e >> 2][e & 3], qscale, m[c]) * inverse;
+            }
         }
 #pragma unroll
         for (int h = 0; h < H; h++) {
             fb8 w[CT][P];
 #pragma unroll
             for (int c = 0; c < CT; c++) {
-                const float mf = finite(m[c]);
                 float v[8], sum = 0.f;
 #pragma unroll
-                for (int e = 0; e < 8; e++) v[e] = __builtin_amdgcn_exp2f(fmaf(s[h][c][e >> 2][e & 3], qscale, -mf)), sum += v[e];
+                for (int e = 0; e < 8; e++) v[e] = __builtin_amdgcn_exp2f(fmaf(s[h][c][e >> 2][e & 3], qscale, -base[c])), sum += v[e];
                 l[c] += sum;
                 if constexpr (PACKED) {
                     uint32_t own[4];

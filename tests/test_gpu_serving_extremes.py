@@ -4,6 +4,7 @@ import pytest
 
 from tests import serving_oracle as oracle
 from tests.test_gpu_kv4_attention import attend
+from zhip import hip
 
 pytestmark = pytest.mark.gpu
 
@@ -40,3 +41,28 @@ def test_scores_of_any_size(hip_ctx, hd, rows, lengths, size):
             v = v[best == best.max(), 0]
             off = np.abs(got[r] - v.mean(axis=0))[~ordinary[r]]
             assert np.all(off <= (2.0 ** -20 + (p + 1) * 2.0 ** -21) * np.abs(v).max()), (group, r, off.max())
+
+
+@pytest.mark.parametrize("style", [0, 1])
+@pytest.mark.parametrize("size,weight,eps", [(1e-40, 1, 0.0), (1e-42, 1, 0.0), (3e-39, 1, 0.0), (1e37, 1, 1e-6), (1e30, 1e-20, 1e-6),
+                                             (1e-30, 1e20, 0.0), (1e-42, 1e-30, 0.0), (1e37, 1e30, 0.0)])
+def test_norms_of_any_size(hip_ctx, style, size, weight, eps):
+    """Heads and weights from denormal to the largest: the factor 1 / sqrt(mean x^2) alone, or times a weight, may be
+    no binary32 number where the normalised value is.
+    Tolerance: as for ordinary heads (the factor's rounding, the normalised value's, the weight's sum with the offset, its product,
+    and the rotation's three: 8 2^-24 of the pair)."""
+    rng = np.random.default_rng(17)
+    heads, rows = 5, 3
+    for hd, rd, extra in ((128, 128, 0), (96, 48, 0), (64, 64, 1), (512, 6, 0)):
+        x = (size * rng.normal(0, 1, (rows, heads, hd))).astype(np.float32)
+        w = [(weight * rng.normal(1, 0.2, hd)).astype(np.float32) for _ in range(2)]
+        held = np.concatenate([x.reshape(rows, -1), np.zeros((rows, extra), np.float32)], axis=1)
+        src = hip_ctx.buffer(held)
+        d = hip.Heads(hip.RopeDesc(hd, rd, style), *(hip_ctx.buffer(v) for v in w), eps=eps)
+        hip_ctx.norm_rope_rows(d, src, src, rows, 3, 2, first_position=5, src_stride=held.shape[1], dst_stride=held.shape[1])
+        got = src.read().reshape(held.shape)[:, :heads * hd].reshape(x.shape)
+        y = np.concatenate([oracle.norm(x[:, :3], w[0], eps), oracle.norm(x[:, 3:], w[1], eps)], axis=1)
+        want, pair = oracle.rope(y, np.arange(5, 5 + rows), oracle.rope_frequencies(rd, 10000.0), rd, style)
+        pair = np.maximum(pair, np.abs(want))
+        off = np.abs(got - want)
+        assert np.all(off <= 8 * 2.0 ** -24 * pair + 2.0 ** -149), (hd, rd, (off / pair).max())

@@ -182,14 +182,18 @@ template <int LAYOUT, bool CACHE> __global__ void __launch_bounds__(256) head_ro
     };
     auto turn = [&](int h, const float (&v)[2][4]) {
         const bool key = h >= p.q_heads, normed = key ? p.k_norm : p.q_norm;
-        const float inv = normed ? (float)norm_of(v) : 1.f;
+        // The factor 1 / rms as a power of two and a binary32 number of .5 to 1: where all values are denormal, or next to the
+        // largest, it is itself no binary32 number, nor is its product with a weight.  What it makes of a value is.
+        const double inv = normed ? norm_of(v) : 1.0;
+        const int power = __builtin_amdgcn_frexp_exp(inv);
+        const float part = (float)__builtin_amdgcn_frexp_mant(inv);
         float y[2][4];
 #pragma unroll
         for (int j = 0; j < 4; j++) {
             float a = v[0][j], c = v[1][j];
             if (normed) {
-                a *= (key ? wk[0][j] + p.weight_offset : wq[0][j]) * inv;
-                c *= (key ? wk[1][j] + p.weight_offset : wq[1][j]) * inv;
+                a = ldexpf(a, power) * part * (key ? wk[0][j] + p.weight_offset : wq[0][j]);
+                c = ldexpf(c, power) * part * (key ? wk[1][j] + p.weight_offset : wq[1][j]);
             }
             const float fc = (float)cs[j], fs = (float)sn[j];
             const bool t = LAYOUT == SPLIT || turns(j);

@@ -66,3 +66,26 @@ def test_norms_of_any_size(hip_ctx, style, size, weight, eps):
         pair = np.maximum(pair, np.abs(want))
         off = np.abs(got - want)
         assert np.all(off <= 8 * 2.0 ** -24 * pair + 2.0 ** -149), (hd, rd, (off / pair).max())
+
+
+@pytest.mark.parametrize("hd", [64, 128, 256])
+@pytest.mark.parametrize("rows,lengths,window", [([100], [100], 0), ([70], [700], 0), ([100], [20000], 1024), ([90], [90], 33), ([300], [9000], 100),
+                                                 ([90, 65, 1], [100, 1500, 70], 0), ([120, 1, 80], [6000, 90, 80], 500)])
+def test_room_that_a_batch_does_not_use(hip_ctx, hd, rows, lengths, window):
+    """Prompts whose pages could hold far more positions than they have: right, and to the bit as with the limit that
+    fits, as the parts of a sum follow what the rows see and not what they might.  A window far into a context too."""
+    heads, kvh = 8, 2
+    rng = np.random.default_rng(hd + sum(lengths))
+    batch = oracle.Batch(rows, lengths, rng, extra_pages=1500)
+    cache = oracle.Kv4(1, batch.pool, kvh, hd, rng)
+    got = oracle.upload(hip_ctx, cache)
+    q = rng.normal(0, 0.7, (batch.n, heads, hd)).astype(np.float32)
+    src, y = hip_ctx.buffer(q), []
+    for limit in (max(lengths), 0, 2 * max(lengths)):
+        print("room", rows, lengths, window, hd, limit, flush=True)
+        out = hip_ctx.buffer(np.full(q.shape, 7, np.float32))
+        hip_ctx.kv4_attention(got, 0, batch.on(hip_ctx, max_rows=max(rows), max_length=limit), src, out, heads, window)
+        y.append(out.read().reshape(q.shape))
+    want, bound = oracle.attention(cache, 0, batch, q, hd ** -0.5, window)
+    assert np.all(np.abs(y[0] - want) <= bound)
+    assert np.array_equal(y[0], y[1]) and np.array_equal(y[0], y[2])

@@ -114,6 +114,14 @@ template <int COLUMNS> __device__ __forceinline__ uint32_t tiles_of(const Kv4Par
 __device__ __forceinline__ uint32_t splits_of(const Kv4Params &p, uint32_t tiles) {
     return max(1u, min(p.splits, 2 * p.cus / max(tiles * p.c.nkv, 1u)));
 }
+// Of these a sequence has as many as leave each two pages of what its rows see, whatever room it has besides: the parts that
+// its sums are taken in follow from its tables.  (8 heads over 2 kv heads of 128, with the join: 64 rows of a fresh prompt
+// with room for 131072 positions 15.2 us, of all splits that might be 18.8; 180 rows at 1000 positions 19.0 and 21.3; 100 rows
+// at 100000 with a window of 1024 20.1 and 22.3.  Of four pages each, 180 rows at 1000: 23.8.)
+__device__ __forceinline__ uint32_t splits_of(const Kv4Params &p, const Sequence &q, uint32_t splits) {
+    const Range r = range_of(p, q, 0, q.rows - 1);
+    return max(1u, min(splits, (uint32_t)((r.end + 1) / 2 - r.begin / 2) / 2));
+}
 template <int COLUMNS> __device__ __forceinline__ uint32_t all_tiles(const Kv4Params &p) {
     if (p.b.sequences > kLanes) return uniform(Plan(p).tiles[p.b.sequences - 1]);
     const uint32_t lane = threadIdx.x & 63;
@@ -159,6 +167,8 @@ template <int COLUMNS> __device__ __forceinline__ Tile tile_of(const Kv4Params &
     t.first = (number - before) * COLUMNS;
     const uint32_t all = t.q.rows * group;  // (tables that don't ascend may pass 32 bits in the sums)
     t.count = number >= before && t.first < all ? min((uint32_t)COLUMNS, all - t.first) : 0u;
+    if (t.count) t.splits = splits_of(p, t.q, t.splits);
+    if (t.split >= t.splits) t.count = 0;
     return t;
 }
 
@@ -896,10 +906,12 @@ template <int HD, int CT> __global__ void __launch_bounds__(256, 2) kv4_many_ker
 }
 // The splits of a row's heads joined, a thread four dims.
 template <int HD, int COLUMNS> __device__ __forceinline__ void join_many(const Kv4Params &p, uint32_t row, uint32_t block) {
-    const int splits = (int)splits_of(p, all_tiles<COLUMNS>(p));
-    if (splits == 1) return;
+    const uint32_t most = splits_of(p, all_tiles<COLUMNS>(p));
+    if (most == 1) return;
     const Sequence q = sequence_of_row(p.b, row);
     if (q.rows * p.group <= p.few) return;  // (none's, or the other kernel's)
+    const int splits = (int)splits_of(p, q, most);
+    if (splits == 1) return;
     const uint32_t u = block * 256 + threadIdx.x;
     if (u < (uint32_t)p.heads * (HD / 4)) {
         const size_t at = (size_t)row * p.heads + u / (HD / 4), each = (size_t)p.b.rows * p.heads;
@@ -988,9 +1000,10 @@ hipError_t launch_kv4_attention(const Kv4Attn &a, int cus, hipStream_t s) {
             const uint64_t least_tiles = several ? std::max<uint64_t>(1, all > few_columns ? (all - few_columns) / M : 1) : most_tiles;
             const uint64_t each = (uint64_t)a.b.rows * a.heads * (HD + 2);
             p.cus = (uint32_t)cus;
-            // Two pages a split at least, and 32 splits at most.  (180 rows at 1000 positions, 4 heads over 2 kv heads of 128, with
-            // the join: 18.8 us, of four pages at least 23.8; at 8000 31.3, with 62 splits 34.2.)
-            p.splits = (uint32_t)std::max<uint64_t>(1, std::min<uint64_t>({2 * (uint64_t)cus / (least_tiles * nkv), blocks / 4, 32,
+            // of the positions that a tile's rows see, two pages a split at least, and 32 splits at most
+            const uint64_t tile_rows = std::min<uint64_t>(a.b.max_rows, (M - 1) / p.group + 2), pages = (a.b.cap + kPage - 1) / kPage;
+            const uint64_t seen = a.window ? std::min(pages, (a.window + tile_rows - 2) / kPage + 2) : pages;
+            p.splits = (uint32_t)std::max<uint64_t>(1, std::min<uint64_t>({2 * (uint64_t)cus / (least_tiles * nkv), seen / 2, 32,
                                                                            part_floats / each}));
             p.many_part = part, p.many_part_ml = (float2 *)(part + (size_t)p.splits * a.b.rows * a.heads * HD);
             many_items = p.splits > 1 ? std::max<uint64_t>(most_tiles * nkv, 2 * (uint64_t)cus) : most_tiles * nkv;

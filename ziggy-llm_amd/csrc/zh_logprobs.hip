@@ -392,9 +392,10 @@ hipError_t launch_token_logprobs(const TokenLogprobs &a, int cus, hipStream_t s)
     w.logits = ((a.vocab + w.slices - 1) / w.slices + 3) / 4 * 4;  // alike, so that the last one's lanes aren't mostly empty
     w.slices = (a.vocab + w.logits - 1) / w.logits;
     const size_t each = w.slices * (sizeof(SliceSums) + 8 * (size_t)a.k);
-    const uint32_t most = (uint32_t)std::min<size_t>(a.work_bytes / each, 0x7FFFFFFFu / w.slices);
+    // as many rows at a time as the workspace holds; rows that are one slice need none of it, but a launch has less than 2^32 threads
+    const uint32_t most = whole ? 0xFFFFFFFFu / kThreads : (uint32_t)std::min<size_t>(a.work_bytes / each, 0x7FFFFFFFu / w.slices);
     TokenLogprobs p = a;
-    for (uint32_t r = 0; r < a.rows; r += p.rows) {  // as many rows at a time as the workspace holds
+    for (uint32_t r = 0; r < a.rows; r += p.rows) {
         p.rows = std::min(a.rows - r, most);
         p.x = a.x + (size_t)r * a.stride, p.tokens = a.tokens + r, p.out = a.out + r;
         p.entropy = a.entropy ? a.entropy + r : nullptr;

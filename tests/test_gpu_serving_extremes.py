@@ -89,3 +89,90 @@ def test_room_that_a_batch_does_not_use(hip_ctx, hd, rows, lengths, window):
     want, bound = oracle.attention(cache, 0, batch, q, hd ** -0.5, window)
     assert np.all(np.abs(y[0] - want) <= bound)
     assert np.array_equal(y[0], y[1]) and np.array_equal(y[0], y[2])
+
+
+def pool_of(cache, kvh, hd):
+    """K and V of every position of the pool [kv head][page x position][hd], in 64 bits."""
+    k, v = (oracle.of_four_bits(cache.codes[w][0], cache.scales[w][0]).transpose(2, 0, 1, 3).reshape(kvh, -1, hd) for w in range(2))
+    return k, v
+
+
+def near(got, x, k, v, seen, scale):
+    """Outputs [columns][hd] of one kv head for queries x [columns][hd], seen [columns][positions].
+    Tolerance: weights are off by 2 e of themselves for scores off by e (the score's own and the maximum's, as
+    serving_oracle.attention has them) and by 2^-20, the sums of n terms, three pieces each, by 3 n 2^-24 of the sum of
+    their magnitudes; the quotient of two such sums by twice that.  Of sum w |v|, not of the largest value: a few keys in
+    tens of thousands have nearly all the weight."""
+    z = x.astype(np.float64) @ k.T * float(np.float32(scale))
+    e = (3 * k.shape[1] + 8) * 2.0 ** -23 * (np.abs(x.astype(np.float64)) @ np.abs(k).T).max(axis=1) * scale
+    z[~seen] = -np.inf
+    w = np.exp(z - z.max(axis=1, keepdims=True))
+    w /= w.sum(axis=1, keepdims=True)
+    bound = 2 * (2 * e + 2.0 ** -20 + 3 * 2.0 ** -24 * seen.sum(axis=1))[:, None] * (w @ np.abs(v))
+    off = np.abs(got - w @ v)
+    assert np.all(off <= bound), ((off / bound).max(), np.argwhere(~(off <= bound))[:4])
+
+
+def with_loud_first_page(pages, kvh, hd, rng):
+    """A pool whose page 0, which no sequence has, would take all the weight if it were seen in place of a missing one."""
+    cache = oracle.Kv4(1, pages, kvh, hd, rng)
+    cache.scales[0][0, 0] = 140
+    return cache
+
+
+@pytest.mark.parametrize("sequences,group,hd", [(64, 1, 64), (64, 8, 64), (100, 1, 128), (64, 24, 64)])
+def test_long_lists_of_pages_of_single_rows(hip_ctx, sequences, group, hd):
+    """Sequences so long, and so many, that a wavefront goes through its list of 64 blocks' pages several times (300 blocks
+    of 39990 positions): every page from the list of its own time, and pages that the pool lacks on both sides of the
+    lists' ends.  The sequences read the same pages, each in an order of its own."""
+    rng = np.random.default_rng(sequences + group)
+    kvh, length, scale = 8, 39990, hd ** -0.5
+    pages = -(-length // 64)
+    cache = with_loud_first_page(pages + 1, kvh, hd, rng)
+    table = np.stack([rng.permutation(pages) + 1 for _ in range(sequences)]).astype(np.uint32)
+    seen = np.ones((sequences, pages + 1, 64), bool)
+    seen[:, 0] = False
+    for s in range(sequences):
+        seen[s, table[s, -1], length % 64:] = False
+        for p in np.concatenate([rng.permutation(pages - 1)[:20], [126, 127, 128, 129, 130, 255, 256, 257, 384, 512, 513]]):
+            seen[s, table[s, p] if table[s, p] <= pages else 0] = False
+            table[s, p] = pages + 1 + rng.integers(0, 1 << 31)
+    q = rng.normal(0, 0.7, (sequences, kvh * group, hd)).astype(np.float32)
+    print("lists", sequences, group, hd, flush=True)
+    on = hip.Batch(hip_ctx.buffer(table), hip_ctx.buffer(np.arange(sequences + 1, dtype=np.uint32)),
+                   hip_ctx.buffer(np.full(sequences, length, np.uint32)), sequences, pages, sequences, 1, length)
+    out = hip_ctx.empty(q.nbytes)
+    hip_ctx.kv4_attention(oracle.upload(hip_ctx, cache), 0, on, hip_ctx.buffer(q), out, kvh * group)
+    got = out.read().reshape(sequences, kvh, group, hd)
+    k, v = pool_of(cache, kvh, hd)
+    some = range(0, sequences, 1 if group == 1 else 7)
+    for h in range(kvh):
+        near(np.concatenate([got[s, h] for s in some]), np.concatenate([q[s, h * group:(h + 1) * group] for s in some]), k[h], v[h],
+             np.repeat(seen.reshape(sequences, -1)[list(some)], group, axis=0), scale)
+
+
+@pytest.mark.parametrize("rows,length,heads,kvh,hd", [(1024, 9390, 64, 8, 64), (70, 140000, 2, 1, 64), (70, 143000, 2, 1, 256)])
+def test_long_lists_of_pages_of_prompts(hip_ctx, rows, length, heads, kvh, hd):
+    """The same for a prompt's tiles: so many that each goes through all 147 pages, and splits of more than 64 pages."""
+    rng = np.random.default_rng(rows + hd)
+    group, scale, pages = heads // kvh, hd ** -0.5, -(-length // 64)
+    cache = with_loud_first_page(pages + 1, kvh, hd, rng)
+    order = (rng.permutation(pages) + 1).astype(np.uint32)
+    table, here = order.copy(), np.ones(length, bool)
+    for p in np.concatenate([rng.permutation(pages - rows // 64 - 2)[:pages // 30], [63, 64, 65, 66, 127, 128, 129]]):
+        table[p] = pages + 1 + rng.integers(0, 1 << 31)
+        here[64 * p:64 * p + 64] = False
+    q = rng.normal(0, 0.7, (rows, heads, hd)).astype(np.float32)
+    print("prompt lists", rows, length, hd, flush=True)
+    on = hip.Batch(hip_ctx.buffer(table), hip_ctx.buffer(np.array([0, rows], np.uint32)), hip_ctx.buffer(np.array([length], np.uint32)),
+                   1, pages, rows, rows, length)
+    out = hip_ctx.empty(q.nbytes)
+    hip_ctx.kv4_attention(oracle.upload(hip_ctx, cache), 0, on, hip_ctx.buffer(q), out, heads)
+    got = out.read().reshape(q.shape)
+    k, v = pool_of(cache, kvh, hd)
+    at = (order[np.arange(length) // 64].astype(int) * 64 + np.arange(length) % 64)
+    some = np.unique(np.concatenate([[0, 1, rows - 1], rng.integers(0, rows, 12)]))
+    seen = (np.arange(length) <= (length - rows + some)[:, None]) & here
+    for h in range(kvh):
+        mine = slice(h * group, (h + 1) * group)
+        near(got[some, mine].reshape(-1, hd), q[some, mine].reshape(-1, hd), k[h][at], v[h][at], np.repeat(seen, group, axis=0), scale)

@@ -18,37 +18,12 @@ namespace {
 
 typedef unsigned long long u64;
 
-__device__ __forceinline__ double turns_per_position(const HeadRows &p, int i) {
-    double f = exp2((double)i * p.freq.exponent) * 0.15915494309189533577;
-    const double g = fmin(fmax(p.freq.a + p.freq.b * (p.freq.by_turns ? f : (double)i), 0.0), 1.0);
-    f *= g + (1.0 - g) * p.freq.inv_factor;
-    return p.factors ? f / (double)p.factors[i] : f;
-}
-
 // the scale byte (its exponent + 127) of 32 values whose largest magnitude has these bits
 __device__ __forceinline__ uint32_t scale_byte(uint32_t bits) {
     const uint32_t e = (bits >> 23) + ((bits & 0x7FFFFFu) > 0x600000u ? 1u : 0u);  // 7 2^x is 1.75 2^(x + 2)
     return min(max(e, 33u) - 2u, 219u);
 }
 
-// The sum over a team of 8 .. 64 lanes, in each of them.
-__device__ __forceinline__ double team_sum(double v, int team) {
-    auto add = [&](u64 o) { v += __longlong_as_double((long long)o); };
-    add(dpp_u64<0xB1>((u64)__double_as_longlong(v)));
-    add(dpp_u64<0x4E>((u64)__double_as_longlong(v)));
-    add(dpp_u64<0x141>((u64)__double_as_longlong(v)));
-    if (team > 8) add(dpp_u64<0x140>((u64)__double_as_longlong(v)));
-    auto far = [&](auto d) {
-        const u64 u = (u64)__double_as_longlong(v);
-        uint32_t a0, b0, a1, b1;
-        lane_pair<decltype(d)::value>((uint32_t)u, a0, b0);
-        lane_pair<decltype(d)::value>((uint32_t)(u >> 32), a1, b1);
-        v = __longlong_as_double((long long)((u64)a1 << 32 | a0)) + __longlong_as_double((long long)((u64)b1 << 32 | b0));
-    };
-    if (team > 16) far(std::integral_constant<int, 16>{});
-    if (team > 32) far(std::integral_constant<int, 32>{});
-    return v;
-}
 // 1 / sqrt(x) to a step or two of 64 bits: the hardware's estimate, and two steps of Newton's
 __device__ __forceinline__ double inverse_root(double x) {
     double y = __builtin_amdgcn_rsq(x);
@@ -162,7 +137,7 @@ template <int LAYOUT, bool CACHE> __global__ void __launch_bounds__(256) head_ro
         at = (double)(p.positions ? p.positions[r] : p.first + r);
     }
     for (int i = lane; i < half; i += 64) {
-        const double t = at * turns_per_position(p, i);
+        const double t = at * p.freq.turns_per_position(i, p.factors);
         double s, c;
         sincospi(2.0 * (t - rint(t)), &s, &c);
         table[i] = make_double2(c * (double)p.magnitude, s * (double)p.magnitude);

@@ -55,23 +55,6 @@ __device__ __forceinline__ float exp_of(float d) {
     return fmaf(e, r, e);
 }
 
-__device__ __forceinline__ double wave_sum(double v) {
-    auto add = [](double x, u64 y) { return x + __longlong_as_double((long long)y); };
-    v = add(v, dpp_u64<0xB1>((u64)__double_as_longlong(v)));
-    v = add(v, dpp_u64<0x4E>((u64)__double_as_longlong(v)));
-    v = add(v, dpp_u64<0x141>((u64)__double_as_longlong(v)));
-    v = add(v, dpp_u64<0x140>((u64)__double_as_longlong(v)));
-    auto far = [](double x, auto d) {
-        const u64 u = (u64)__double_as_longlong(x);
-        uint32_t a0, b0, a1, b1;
-        lane_pair<decltype(d)::value>((uint32_t)u, a0, b0);
-        lane_pair<decltype(d)::value>((uint32_t)(u >> 32), a1, b1);
-        return __longlong_as_double((long long)((u64)a1 << 32 | a0)) + __longlong_as_double((long long)((u64)b1 << 32 | b0));
-    };
-    v = far(v, std::integral_constant<int, 16>{});
-    return far(v, std::integral_constant<int, 32>{});
-}
-
 // candidates' places by counting: to(rank, candidate) for those of rank below k
 template <class F> __device__ __forceinline__ void place(const u64 *candidates, int n, int k, F to) {
     for (int i = threadIdx.x; i < n; i += blockDim.x) {
@@ -236,7 +219,7 @@ template <int V, bool WHOLE> __global__ void __launch_bounds__(kThreads) logprob
         t += (double)((fmaf(e[0], d[0], e[1] * d[1]) + fmaf(e[2], d[2], e[3] * d[3])) +
                       (fmaf(e[4], d[4], e[5] * d[5]) + fmaf(e[6], d[6], e[7] * d[7])));
     }
-    s = wave_sum(s), t = wave_sum(t);
+    s = team_sum(s, 64), t = team_sum(t, 64);
     count = running_sum(count);
     if (lane == 63) sums[0][wave] = s, sums[1][wave] = t, counts[wave] = count;
     __syncthreads();
@@ -367,7 +350,7 @@ __global__ void __launch_bounds__(kRowThreads) logprobs_row_kernel(TokenLogprobs
             const double d = fmax((double)own.top - (double)largest, -1000.0), f = exp(d), all = own.count + own.s;
             s = f * all, t = f * (own.t + d * all);
         }
-        s = wave_sum(s) + (wave_sum(count) - 1.0), t = wave_sum(t);
+        s = team_sum(s, 64) + (team_sum(count, 64) - 1.0), t = team_sum(t, 64);
         const double log_s = finish_row(p, row, largest, s, t, token, given, lane == 0);
         if (lane == 0) shared_log = log_s, shared_largest = largest;
     }

@@ -12,6 +12,13 @@ struct RopeFreq {
     double inv_factor; // 1 / factor (1: no scaling)
     double a, b;       // g_i = clamp(a + b x, 0, 1), x the pair (YARN) or the turns a position (BANDS); LINEAR: 0, 0
     int by_turns;
+    // of pair i; factors (or null) divide the frequencies
+    __device__ __forceinline__ double turns_per_position(int i, const float *factors) const {
+        double f = exp2((double)i * exponent) * 0.15915494309189533577;
+        const double g = fmin(fmax(a + b * (by_turns ? f : (double)i), 0.0), 1.0);
+        f *= g + (1.0 - g) * inv_factor;
+        return factors ? f / (double)factors[i] : f;
+    }
 };
 // why a rope description is not served (null: it is), and its frequencies
 const char *rope_refusal(const ZiggyHipRopeDesc &d);

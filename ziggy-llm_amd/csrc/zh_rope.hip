@@ -16,13 +16,6 @@ namespace {
 constexpr int kPairs = 4;  // pairs of a thread: two float4 of every head it takes
 constexpr int kBatch = 3;  // heads whose loads go out together
 
-__device__ __forceinline__ double turns_per_position(const RopeRows &p, int i) {
-    double f = exp2((double)i * p.freq.exponent) * 0.15915494309189533577;
-    const double g = fmin(fmax(p.freq.a + p.freq.b * (p.freq.by_turns ? f : (double)i), 0.0), 1.0);
-    f *= g + (1.0 - g) * p.freq.inv_factor;
-    return p.factors ? f / (double)p.factors[i] : f;
-}
-
 // A thread takes four pairs (or eight values behind the rotated ones) of every hp-th head of its rows.
 template <bool ALIGNED> __global__ void __launch_bounds__(256) rope_rows_kernel(RopeRows p, int units, int hp) {
     const int u = threadIdx.x % units, h0 = threadIdx.x / units, half = p.rd / 2, turning = (half + kPairs - 1) / kPairs;
@@ -32,7 +25,7 @@ template <bool ALIGNED> __global__ void __launch_bounds__(256) rope_rows_kernel(
     const int n = rotates ? min(kPairs, half - i0) : min(8, p.hd - i0);
     double f[kPairs];
     if (rotates)
-        for (int j = 0; j < kPairs; j++) f[j] = turns_per_position(p, min(i0 + j, half - 1));
+        for (int j = 0; j < kPairs; j++) f[j] = p.freq.turns_per_position(min(i0 + j, half - 1), p.factors);
     for (size_t r = blockIdx.x; r < p.rows; r += gridDim.x) {
         const float *src = p.src + r * p.src_stride;
         float *dst = p.dst + r * p.dst_stride;

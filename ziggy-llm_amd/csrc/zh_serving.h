@@ -90,6 +90,25 @@ template <class T> __device__ __forceinline__ T running_sum(T v) {
     return add_moved<0x143, 0xC>(v);  // row_bcast:31 into rows 2 and 3
 }
 
+// The sum over a team of 8 .. 64 lanes, in each of them.
+__device__ __forceinline__ double team_sum(double v, int team) {
+    auto add = [&](unsigned long long o) { v += __longlong_as_double((long long)o); };
+    add(dpp_u64<0xB1>((unsigned long long)__double_as_longlong(v)));
+    add(dpp_u64<0x4E>((unsigned long long)__double_as_longlong(v)));
+    add(dpp_u64<0x141>((unsigned long long)__double_as_longlong(v)));
+    if (team > 8) add(dpp_u64<0x140>((unsigned long long)__double_as_longlong(v)));
+    auto far = [&](auto d) {
+        const unsigned long long u = (unsigned long long)__double_as_longlong(v);
+        uint32_t a0, b0, a1, b1;
+        lane_pair<decltype(d)::value>((uint32_t)u, a0, b0);
+        lane_pair<decltype(d)::value>((uint32_t)(u >> 32), a1, b1);
+        v = __longlong_as_double((long long)((unsigned long long)a1 << 32 | a0)) + __longlong_as_double((long long)((unsigned long long)b1 << 32 | b0));
+    };
+    if (team > 16) far(std::integral_constant<int, 16>{});
+    if (team > 32) far(std::integral_constant<int, 32>{});
+    return v;
+}
+
 // LDS of a wavefront's own lanes: what they wrote is what they read behind this
 __device__ __forceinline__ void wave_fence() {
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");

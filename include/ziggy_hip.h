@@ -398,7 +398,10 @@ int ziggy_hip_kv8_load_f32(ZiggyHipContext *ctx, const ZiggyHipKv8Cache *cache, 
  * or, with window > 0, to the last `window` of them; what lies at other
  * positions is not read into the result, whatever it is.  output:
  * [queries][head_count * head_dim].  head_count is a multiple of the cache's
- * head_count_kv (at most 64 times as many). */
+ * head_count_kv (at most 64 times as many).  Blocks' V scales go into the
+ * weights' exponents, beside the scores: an output may be off by 2^-24 of the
+ * row's largest score (scale q . k), relative to itself; where that one passes
+ * 2^24 either way, rows may be wrong altogether, or NaN. */
 int ziggy_hip_kv8_attention_f32(ZiggyHipContext *ctx, const ZiggyHipKv8Cache *cache, const ZiggyHipBuffer *q,
                                 size_t q_row_stride, ZiggyHipBuffer *output, uint32_t head_count, uint32_t layer,
                                 uint32_t position, uint32_t queries, uint32_t window, float scale,
@@ -407,10 +410,10 @@ int ziggy_hip_kv8_attention_f32(ZiggyHipContext *ctx, const ZiggyHipKv8Cache *ca
 /* ---- operators of a step that serves several sequences (no counterpart in the reference) ----
  * The caller's sequences share one pool of pages of ZIGGY_HIP_KV_PAGE_POSITIONS
  * (64) positions.  A batch says which rows of the step's inputs are whose; its
- * tables are device memory, so that a captured step is replayed with other
- * ones.  What they hold can't be checked on the host: the kernels take no index
- * from them that lies outside the buffers (see below), and nothing else of
- * them is refused. */
+ * tables are device memory, read when a call runs: within one open sequence they
+ * may hold others from call to call (ziggy_hip_copy_buffer_region).  What they
+ * hold can't be checked on the host: the kernels take no index from them that
+ * lies outside the buffers (see below), and nothing else of them is refused. */
 
 /* Sequence s has rows row_starts[s] .. row_starts[s + 1] - 1 (none, one or
  * many; sequences' rows follow each other from row 0 on), which are the last of
@@ -419,8 +422,10 @@ int ziggy_hip_kv8_attention_f32(ZiggyHipContext *ctx, const ZiggyHipKv8Cache *ca
  * pool page page_table[s * pages_per_sequence + t / 64].  Rows behind the last
  * sequence's are no one's: what a call would write of them stays as it was.
  * max_rows and max_length: what no sequence has more rows and positions than
- * (0: `rows`, and all that its pages hold); the kernels' grids follow them, so
- * tight ones are faster.  Positions past max_length, and positions whose page
+ * (0: `rows`, and all that its pages hold); the kernels' grids follow them, and
+ * max_rows the attention's kernels (of one sequence the one for that many rows,
+ * of several also the one for prompts where that many would need it), so tight
+ * ones are faster.  Positions past max_length, and positions whose page
  * is not one of the pool's, are passed over: not stored, not read back, and
  * not attended to.  Rows past max_rows are no one's, as those behind the last
  * sequence; so are rows ahead of position 0 (more rows than positions), but
@@ -504,7 +509,9 @@ int ziggy_hip_kv4_load_f32(ZiggyHipContext *ctx, const ZiggyHipKv4Cache *cache, 
  * last `window` of them; a row that none is left for gets zeros.  output:
  * [rows][head_count * head_dim].  head_count is a multiple of the cache's
  * head_count_kv (at most 64 times as many).  At most 2^21 sequences x
- * head_count_kv, and 2^29 rows x head_count. */
+ * head_count_kv, and 2^29 rows x head_count.  Scores are binary32 of any size
+ * that it holds; one past its end is an infinity: above, its row's output is
+ * NaN, below, its position has no weight (a row that sees only such: zeros). */
 int ziggy_hip_kv4_attention_f32(ZiggyHipContext *ctx, const ZiggyHipKv4Cache *cache, uint32_t layer,
                                 const ZiggyHipBatch *batch, const ZiggyHipBuffer *q, size_t q_offset_bytes,
                                 size_t q_row_stride, ZiggyHipBuffer *output, uint32_t head_count, uint32_t window,

@@ -176,3 +176,29 @@ def test_long_lists_of_pages_of_prompts(hip_ctx, rows, length, heads, kvh, hd):
     for h in range(kvh):
         mine = slice(h * group, (h + 1) * group)
         near(got[some, mine].reshape(-1, hd), q[some, mine].reshape(-1, hd), k[h][at], v[h][at], np.repeat(seen, group, axis=0), scale)
+
+
+@pytest.mark.parametrize("rows,length", [(1, 2), (3, 50), (12, 200), (80, 90)])
+def test_scores_past_the_range(hip_ctx, rows, length):
+    """One key whose score is above binary32's largest, or below its least, beside keys of 0, and rows that see it alone.
+    Below: without weight, so the mean of the other values in sight (to n 2^-23 and n 2^-24 of the largest), zeros where
+    there are none.  Above: NaN."""
+    rng = np.random.default_rng(rows)
+    hd = 64
+    batch = oracle.Batch([rows], [length], rng)
+    cache = oracle.Kv4(1, batch.pool, 1, hd, rng)
+    cache.codes[0][:] = 0
+    first = length - rows  # what the first row sees last
+    page, slot = batch.place(0, first)
+    cache.codes[0][0, page, slot, 0, 3] = 7
+    cache.scales[0][0, page, slot] = 219
+    q = np.zeros((rows, 2, hd), np.float32)
+    q[:, 0, 3], q[:, 1, 3] = -3e38, 3e38
+    for window in (0, 1):
+        got = attend(hip_ctx, [], [], 2, 1, hd, batch=batch, cache=cache, q=q, rng=rng, scale=0.5, window=window)[0]
+        for r in range(rows):
+            at = np.arange(max(0, first + r + 1 - window) if window else 0, first + r + 1)
+            v = cache.rows(0, batch.table[0, at // 64].astype(int), at % 64)[1][at != first, 0]
+            want = v.mean(axis=0) if len(v) else np.zeros(hd)
+            assert np.all(np.abs(got[r, 0] - want) <= (2.0 ** -20 + at.size * 2.0 ** -21) * np.abs(v).max(initial=0))
+            assert np.isnan(got[r, 1]).all() == (first in at)

@@ -3,13 +3,15 @@
 //
 // y = R(p) (x (w + o) / sqrt(mean x^2 + eps)), R(p) turning pair i by p base^(-2 i / rd).  Sums of squares, angles, sines
 // and a key's whole way are 64 bits, so that its codes do not hang on binary32's roundings; a query's or an f32 key's
-// factors are rounded once and applied in binary32.
+// factors are rounded once and applied in binary32, the normalised value ahead of its weight.
 //
-// What bounds it: memory where there are many rows (4095 rows of 40 heads of 128: 33.3 us, 5.0 TB/s read and written;
-// 4.9 thousand rows of four prompts appended, 32 query and 8 kv heads: 32.2 us for 151 MB, read back 9.4), the chain
-// launch, tables, page, sines, norm where there are few (one row 4.2 us, 32 rows appended 6.5, read back 4.4).  A wavefront
-// a row: its sines are shared by all its heads, and there is nothing to wait for but its own loads (a workgroup a row, with
-// barriers: 43 to 50 us).
+// What bounds it: memory where there are many rows (4095 rows of 40 heads of 128: 33.3 us, 5.0 TB/s read and written), the
+// chain launch, tables, page, sines, norm where there are few (one row 4.3 us, 32 rows appended 6.4, read back 4.9).  Between
+// the two lie prompts' chunks on their way into the cache and back, 3012 rows of four with 32 query and 8 kv heads: appended
+// in 32 us for 129 MB by the counters (126.6 have to move), 4.0 TB/s, as every row's bytes wait for its sequence, page and
+// sines; read back in 9.3 us for 32 MB, 3.4 TB/s, of which 28.0 have to move: a position's V codes are four bytes of every
+// 32, so a row fetches 2.3 times its codes.  A wavefront a row: its sines are shared by all its heads, and there is nothing to
+// wait for but its own loads (a workgroup a row, with barriers: 43 to 50 us).
 #include "zh_serving.h"
 
 namespace zh {

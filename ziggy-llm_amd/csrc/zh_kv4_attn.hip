@@ -12,10 +12,11 @@
 // (48 columns, 7 sequences of 2000 positions, 8 kv heads of 128: 28.2 us by the first, 33.8 by the second; 64 columns, one
 // of 9000, heads of 64: 17.0 and 19.3.)
 //
-// What bounds it (32 heads over 8 kv heads of 128).  A query at 131071 positions: memory, 30.4 us for 143 MB, and the join
-// 4.7.  At 4113: the chain launch, lengths, page, codes, products, exchange 6.7, and the join's 3.6.  48 sequences of up to
-// 16384 positions: memory and the last workgroups of uneven sequences, 75 us for 311 MB, and 5.8.  2048 queries at 16384:
-// the matrix cores, 1.04 ms for three pieces of both products, 1.49 PFLOP/s (library products of bf16 reach 1.34).
+// What bounds it (32 heads over 8 kv heads of 128; kernel times under the profiler).  A query at 131071 positions: memory,
+// 30.7 us for 143 MB, and the join 4.8.  At 4113: the chain launch, lengths, page, codes, products, exchange 7.0, and the
+// join's 3.6.  48 sequences of up to 16384 positions: memory and the last workgroups of uneven sequences, 76 us for 311 MB,
+// and 6.4.  2048 queries at 16384: the matrix cores, 1.03 to 1.09 ms by card for three pieces of both products, 1.42 to 1.51
+// PFLOP/s (library products of bf16 reach 1.34).
 #include <algorithm>
 
 #include "zh_serving.h"
@@ -94,8 +95,10 @@ __device__ __forceinline__ Sequence uniform(const Sequence &q) {
 
 // Of more than 64 sequences a kernel of its own makes a table, which the others search: for each sequence the end of its
 // items among the few-column kernel's and of its tiles among the other's, and the slot of its first split.  Up to 64 every
-// wavefront has a sequence a lane, and a table would cost a launch, 4.4 us.  (Every wavefront going through all sequences,
-// 64 at a time, and the table: 2048 sequences of 512 positions 828 us and 302, 512 of 512 127 and 88, 128 of 1024 40 and 43.)
+// wavefront has a sequence a lane, and a table would cost a launch, 4.6 us.  The border is where the lanes end, not where
+// the table begins to pay: with every wavefront going through all sequences, 64 at a time, and with the table 2048 sequences
+// of 512 positions took 828 us and 302, 512 of 512 127 and 88, but 128 of 1024 40 and 43, 65 of 2048 45 and 49.  A third form
+// for those in between would have to take two sequences a lane; without it they pay up to 4 us.
 struct Plan {
     const uint32_t *quota, *items, *tiles, *slots;
     __host__ __device__ static size_t words(uint32_t sequences) { return 4 + 3 * (size_t)sequences; }
